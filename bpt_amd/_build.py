@@ -1,9 +1,11 @@
-"""Compiles the four native libraries in-tree:
+"""Compiles the native libraries in-tree:
 
   bpt_amd/csrc/libbptgraph.so  host C++ (g++)            <- bptgraph.cpp
-  bpt_amd/csrc/libbptattn.so   gfx950 HIP (hipcc)        <- bptattn.hip
+  bpt_amd/csrc/libbptattn.so   gfx950 HIP (hipcc)        <- bptattn.hip, bpttiles.h
+  bpt_amd/csrc/libbptscore.so  gfx950 HIP (hipcc)        <- bptscore.hip, bpttiles.h  (attention with capped scores and distance)
+  bpt_amd/csrc/libbptblock.so  gfx950 HIP (hipcc)        <- bptblock.hip, bpttiles.h  (layer norm of a sum, relu kept in 8 bits)
   bpt_amd/csrc/libbptplan.so   gfx950 HIP (hipcc)        <- bptplan.hip  (plans built on the GPU; rocPRIM headers)
-  bpt_amd/csrc/bptop.so        host C++ (g++, torch)     <- bptop.cpp    (host side of the ops and their autograd; links both)
+  bpt_amd/csrc/bptop.so        host C++ (g++, torch)     <- bptop.cpp, bptblockop.cpp  (host side of the ops and their autograd; links them)
 
 hipcc cross-compiles for gfx950 without a GPU.  Run `python -m bpt_amd._build`.
 """
@@ -15,6 +17,8 @@ CSRC = os.path.join(os.path.dirname(os.path.abspath(__file__)), "csrc")
 GRAPH_SO = os.path.join(CSRC, "libbptgraph.so")
 ATTN_SO = os.path.join(CSRC, "libbptattn.so")
 PLAN_SO = os.path.join(CSRC, "libbptplan.so")
+SCORE_SO = os.path.join(CSRC, "libbptscore.so")
+BLOCK_SO = os.path.join(CSRC, "libbptblock.so")
 OP_SO = os.path.join(CSRC, "bptop.so")
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
@@ -58,8 +62,13 @@ def build_plan(verbose=True):
     return PLAN_SO
 
 
+def build_block(verbose=True):
+    _run([HIPCC] + HIP_FLAGS + [os.path.join(CSRC, "bptblock.hip"), "-o", BLOCK_SO], verbose)
+    return BLOCK_SO
+
+
 def build_op(verbose=True):
-    """After build_attn and build_plan, whose libraries it links (found beside it at run time)."""
+    """After the HIP libraries, which it links (found beside it at run time)."""
     import sysconfig
     import torch
     from torch.utils import cpp_extension
@@ -68,8 +77,8 @@ def build_op(verbose=True):
     libs = os.path.join(os.path.dirname(torch.__file__), "lib")
     _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-DTORCH_EXTENSION_NAME=bptop",
           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM"]
-         + [f"-I{p}" for p in include] + [os.path.join(CSRC, "bptop.cpp"), "-o", OP_SO, f"-L{libs}", f"-L{CSRC}",
-                                          "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python", "-ltorch", "-l:libbptattn.so", "-l:libbptplan.so", "-Wl,-rpath,$ORIGIN"], verbose)
+         + [f"-I{p}" for p in include] + [os.path.join(CSRC, "bptop.cpp"), os.path.join(CSRC, "bptblockop.cpp"), "-o", OP_SO, f"-L{libs}", f"-L{CSRC}",
+                                          "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python", "-ltorch", "-l:libbptattn.so", "-l:libbptplan.so", "-l:libbptblock.so", "-Wl,-rpath,$ORIGIN"], verbose)
     return OP_SO
 
 
@@ -77,9 +86,9 @@ def build_all(verbose=True):
     """The HIP compilations take most of the time and run side by side."""
     from concurrent.futures import ThreadPoolExecutor
     with ThreadPoolExecutor(2) as pool:
-        plan = pool.submit(build_plan, verbose)
+        others = pool.map(lambda build: build(verbose), (build_plan, build_block))
         graph, attn = build_graph(verbose), build_attn(verbose)
-        return graph, attn, plan.result(), build_op(verbose)
+        return (graph, attn, *others, build_op(verbose))
 
 
 if __name__ == "__main__":

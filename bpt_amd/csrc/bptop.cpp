@@ -1003,7 +1003,10 @@ std::vector<py::object> take_used() {
 
 }  // namespace
 
+void bind_block(py::module_ &m);        // bptblockop.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+    bind_block(m);
     m.attr("ATTN_FWD") = (int)ATTN_FWD;
     m.attr("ATTN_BWD") = (int)ATTN_BWD;
     m.attr("ATTN_FWD_NARROW") = (int)ATTN_FWD_NARROW;

@@ -1236,3 +1236,20 @@ _FORCE_GENERIC = False
 def force_generic_enabled():
     """What set_force_generic last set."""
     return _FORCE_GENERIC
+
+
+# ---- relu kept in 8 bits (bpt_amd/csrc/bptblock.hip; no counterpart in the reference) ---------------------------------------------
+def relu8_forward(a, dropout_p=0.0, seed=0):
+    """(y, codes, exps) of activations a of any shape, float32 or bfloat16: y = relu(a), with dropout_p > 0 zeroed where a hash of
+    (seed, index) says so and divided by 1 - dropout_p elsewhere; codes (uint8, a's shape) and exps (int8, one for every 64 neighbouring
+    elements in memory order) are y in 8 bits, y ~ codes * 2 ** exps: exps the smallest exponent (-126 at least) with which 255 steps
+    reach the 64 elements' largest, codes rounded to the nearest and 1 at least where y > 0, so an element is off by half a step, 2 ** -8
+    of that largest, or by less than a step where it is smaller than half of one.  exps 127: an element is infinite or NaN, and the codes
+    stand for NaN."""
+    return _native.relu8_forward(a, float(dropout_p), int(seed) & (2 ** 64 - 1))
+
+
+def relu8_backward(dy, codes, exps, dropout_p=0.0):
+    """(da, y8): the gradient of relu8_forward's a, dy / (1 - dropout_p) where the code is not 0 and 0 elsewhere, and what the codes stand
+    for (exact in either type), in dy's type."""
+    return _native.relu8_backward(dy, codes, exps, float(dropout_p))

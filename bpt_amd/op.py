@@ -13,7 +13,8 @@ from .graphop import (maskedmm_csr_backward, maskedmm_csr_forward, node_mul_edge
                       sparse_softmax_backward, sparse_softmax_forward, vector_spmm_backward, vector_spmm_forward)
 
 __all__ = ["SparseSoftmax", "MaskedMMCSR", "NodeMulEdge", "VectorSPMM", "BPTAttention", "EdgeTypeEmbedding",
-           "sparse_softmax", "masked_mm", "node_mul_edge", "vec_spmm", "bpt_attention", "edge_type_embedding"]
+           "sparse_softmax", "masked_mm", "node_mul_edge", "vec_spmm", "bpt_attention", "edge_type_embedding",
+           "add_layer_norm", "relu_linear8"]
 
 
 class SparseSoftmax(Function):
@@ -424,3 +425,28 @@ def bpt_attention(row, indptr_r, eid_r, indices_r, col, indptr_c, eid_c, indices
     a = torch.nn.functional.dropout(sparse_softmax(col, indptr_c, eid_c, e * scale), p=float(dropout_p), training=dropout_p > 0)
     return vec_spmm(col, indptr_c, eid_c, indices_c, row, indptr_r, eid_r, indices_r, a, v,
                     n_rows=None if q.size(0) == v.size(0) else q.size(0))
+
+
+def _no_transforms(name):
+    if not _native_takes():
+        raise RuntimeError(f"{name} cannot be traced and has no rules for torch.func's transforms")
+
+
+def add_layer_norm(x, residual=None, weight=None, bias=None, eps=1e-5):
+    """Layer norm of x + residual over the last axis, (z - mean(z)) / sqrt(var(z) + eps) * weight + bias with z = x + residual: what a block
+    does behind attention and feed-forward (modules/attention.py:79, :81), in one pass over memory and with its gradients in another.
+    float32, float64 or bfloat16, contiguous, all of one type; residual like x or None, weight and bias (x.size(-1),) or None.  z, mean and
+    variance are held in 32 bits (64 for float64) and the result is rounded once.  Deterministic."""
+    _no_transforms("add_layer_norm")
+    return _native.add_layer_norm(x, residual, weight, bias, float(eps))
+
+
+def relu_linear8(a, weight, bias=None, dropout_p=0.0, seed=None):
+    """linear(dropout(relu(a)), weight, bias), the second half of a feed-forward (modules/attention.py:18-19), that keeps one byte an
+    activation for its backward instead of relu's result, dropout's and its mask (graphop.relu8_forward): the outputs and the gradients of a
+    and bias are those of the exact activations, the gradient of weight is formed with the activations in 8 bits.  float32 or bfloat16.
+    dropout_p > 0 hashes (seed, index); seed=None draws one from torch's CPU generator, as bpt_attention does."""
+    _no_transforms("relu_linear8")
+    if dropout_p > 0 and seed is None:
+        seed = int(torch.randint(0, 2 ** 62, (1,)).item())
+    return _native.relu_linear8(a, weight, bias, float(dropout_p), int(seed or 0) & (2 ** 64 - 1))

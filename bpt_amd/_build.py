@@ -62,6 +62,11 @@ def build_plan(verbose=True):
     return PLAN_SO
 
 
+def build_score(verbose=True):
+    _run([HIPCC] + HIP_FLAGS + [os.path.join(CSRC, "bptscore.hip"), "-o", SCORE_SO], verbose)
+    return SCORE_SO
+
+
 def build_block(verbose=True):
     _run([HIPCC] + HIP_FLAGS + [os.path.join(CSRC, "bptblock.hip"), "-o", BLOCK_SO], verbose)
     return BLOCK_SO
@@ -78,7 +83,7 @@ def build_op(verbose=True):
     _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-DTORCH_EXTENSION_NAME=bptop",
           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM"]
          + [f"-I{p}" for p in include] + [os.path.join(CSRC, "bptop.cpp"), os.path.join(CSRC, "bptblockop.cpp"), "-o", OP_SO, f"-L{libs}", f"-L{CSRC}",
-                                          "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python", "-ltorch", "-l:libbptattn.so", "-l:libbptplan.so", "-l:libbptblock.so", "-Wl,-rpath,$ORIGIN"], verbose)
+                                          "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python", "-ltorch", "-l:libbptattn.so", "-l:libbptplan.so", "-l:libbptscore.so", "-l:libbptblock.so", "-Wl,-rpath,$ORIGIN"], verbose)
     return OP_SO
 
 
@@ -86,7 +91,7 @@ def build_all(verbose=True):
     """The HIP compilations take most of the time and run side by side."""
     from concurrent.futures import ThreadPoolExecutor
     with ThreadPoolExecutor(2) as pool:
-        others = pool.map(lambda build: build(verbose), (build_plan, build_block))
+        others = pool.map(lambda build: build(verbose), (build_plan, build_score, build_block))
         graph, attn = build_graph(verbose), build_attn(verbose)
         return (graph, attn, *others, build_op(verbose))
 

@@ -6,7 +6,7 @@ There is no Python or CPU fallback for the device ops: if libbptattn.so is missi
 import ctypes
 import os
 
-from ._build import ATTN_SO, GRAPH_SO, PLAN_SO
+from ._build import ATTN_SO, GRAPH_SO, PLAN_SO, SCORE_SO
 
 c_i64 = ctypes.c_int64
 c_vp = ctypes.c_void_p
@@ -20,6 +20,11 @@ class PlanStruct(ctypes.Structure):
                 ("grp_chunks", c_vp), ("n_groups", c_i64), ("grp_R", c_i64), ("grp_max_chunk", c_i64),
                 ("n_grp_entries", c_i64), ("grp_eids", c_vp), ("bias_by_pair", c_i64),
                 ("n_index_nodes", c_i64), ("max_degree", c_i64)]
+
+
+class ScoreStruct(ctypes.Structure):
+    """Mirror of `bpt_score` (include/bptscore.h)."""
+    _fields_ = [("cap", ctypes.c_float), ("slopes", c_vp), ("pos_q", c_vp), ("pos_k", c_vp)]
 
 
 class PlanInfo(ctypes.Structure):
@@ -112,9 +117,20 @@ BUILD_API = {
     "bpt_build_pair_numbers": (ctypes.c_int, [c_vp, c_vp, c_i64, c_i64, c_vp, c_vp, c_vp]),
 }
 
+_PS = ctypes.POINTER(ScoreStruct)
+_score_tail = [ctypes.c_float, ctypes.c_float, ctypes.c_uint64, ctypes.c_int, ctypes.c_int, c_vp]      # scale, dropout_p, seed, h, dtype, stream
+# libbptscore (include/bptscore.h): attention with capped scores and distance
+SCORE_API = {
+    "bpt_score_forward_workspace_bytes": (c_i64, [_PP, ctypes.c_int]),
+    "bpt_score_backward_workspace_bytes": (c_i64, [_PP, _PP, ctypes.c_int, ctypes.c_int, ctypes.c_int]),
+    "bpt_score_forward": (ctypes.c_int, [_PP, _PS, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64] + _score_tail),
+    "bpt_score_backward": (ctypes.c_int, [_PP, _PP, _PS] + [c_vp] * 13 + [c_i64] + _score_tail),
+}
+
 _graph = None
 _attn = None
 _plan = None
+_score = None
 
 
 def _load(path, api, what):
@@ -151,6 +167,13 @@ def plan_lib():
     if _plan is None:
         _plan = _load(PLAN_SO, {**PLAN_API, **BUILD_API}, "libbptplan (plans built on the GPU)")
     return _plan
+
+
+def score_lib():
+    global _score
+    if _score is None:
+        _score = _load(SCORE_SO, SCORE_API, "libbptscore (attention with capped scores and distance)")
+    return _score
 
 
 def check_graph(status):

@@ -3956,7 +3956,7 @@ int run_attn_fwd(const bpt_plan *P, const void *q, const void *k, const void *v,
 #define LAUNCH_FWD_TILE_PARTS(DR, BI, SP)                                                                                            \
     hipLaunchKernelGGL((k_attn_fwd_tile<T, H, D, HW, DR, BI, false, SP>), dim3(group_grid(P) * (H * SP / HW)), dim3(HW * WAVE), 0, s, *P, \
                        (const T *)q, (const T *)k, (const T *)v, (T *)o, lse, ws_acc, ws_ml, scale * LOG2E, drop.thr, drop.seed, drop.inv, bias, \
-                       Narrow{}, Keep{})
+                       Narrow{}, Keep{}, NoMod{})
 #define LAUNCH_FWD_TILE(DR, BI)                                                                                                      \
     do {                                                                                                                             \
         if (parts == 4) LAUNCH_FWD_TILE_PARTS(DR, BI, 4);                                                                            \
@@ -3983,7 +3983,7 @@ int run_attn_fwd(const bpt_plan *P, const void *q, const void *k, const void *v,
 #define LAUNCH_FWD_TILE_PARTS(DR, BI, SP)                                                                                                \
     hipLaunchKernelGGL((k_attn_fwd_rows_bf16<H, D, HW, TILE_BF16_WPE, DR, BI, SP>), dim3(group_grid(P) * (H * SP / HW)), \
                        dim3(HW * WAVE), 0, s, *P, (const bf16_t *)q, (const bf16_t *)k, (const bf16_t *)v, (bf16_t *)o, lse, ws_acc, ws_ml, \
-                       scale * LOG2E, drop.thr, drop.seed, drop.inv, bias)
+                       scale * LOG2E, drop.thr, drop.seed, drop.inv, bias, NoMod{})
 #define LAUNCH_FWD_TILE(DR, BI)                                                                                                          \
     do {                                                                                                                                 \
         if (parts == 4) LAUNCH_FWD_TILE_PARTS(DR, BI, 4);                                                                                \
@@ -4073,7 +4073,7 @@ int run_attn_bwd(const bpt_plan *Pin, const bpt_plan *Pout, const void *q, const
 #define LAUNCH_DST_TILE_PARTS(DR, BI, SP)                                                                                              \
     hipLaunchKernelGGL((k_attn_bwd_dst_tile<T, H, D, HW, DR, BI, false, SP>), dim3(group_grid(Pin) * (H * SP / HW)), dim3(HW * WAVE), 0, s, \
                        *Pin, (const T *)q, (const T *)k, (const T *)v, (const T *)o, (const T *)d_o, lse, (T *)dq, pds, ws_rows, scale,    \
-                       scale * LOG2E, drop.thr, drop.seed, drop.inv, bias, ds_out, Narrow{})
+                       scale * LOG2E, drop.thr, drop.seed, drop.inv, bias, ds_out, Narrow{}, NoMod{})
 #define LAUNCH_DST_TILE(DR, BI)                                                                                                        \
     do {                                                                                                                               \
         if (parts == 4) LAUNCH_DST_TILE_PARTS(DR, BI, 4);                                                                              \
@@ -4124,7 +4124,7 @@ int run_attn_bwd(const bpt_plan *Pin, const bpt_plan *Pout, const void *q, const
     hipLaunchKernelGGL((k_attn_bwd_dst_rows_bf16<H, D, HW, TILE_BF16_WPE_DST, DR, BI, PD, SP>),                              \
                        dim3(group_grid(Pin) * (H * SP / HW)), dim3(HW * WAVE), 0, s, *Pin, (const bf16_t *)q, (const bf16_t *)k, (const bf16_t *)v, (const bf16_t *)o,             \
                        (const bf16_t *)d_o, lse, (bf16_t *)dq, (uint32_t *)ws, (float2 *)ws, ws_rows, scale, scale * LOG2E, drop.thr,       \
-                       drop.seed, drop.inv, bias, ds_out)
+                       drop.seed, drop.inv, bias, ds_out, NoMod{})
 #define LAUNCH_DST_TILE(DR, BI, PD)                                                                                                      \
     do {                                                                                                                                 \
         if (parts == 4) LAUNCH_DST_TILE_PARTS(DR, BI, PD, 4);                                                                            \
@@ -4151,7 +4151,7 @@ int run_attn_bwd(const bpt_plan *Pin, const bpt_plan *Pout, const void *q, const
 #define LAUNCH_SRC_AGAIN_PARTS(DR, SP)                                                                                                   \
     hipLaunchKernelGGL((k_attn_bwd_src_tile_bf16_again<H, D, HW, TILE_BF16_WPE_AGAIN, DR, SP>), dim3(group_grid(Pout) * (H * SP / HW)),      \
                        dim3(HW * WAVE), 0, s, *Pout, (const bf16_t *)q, (const bf16_t *)k, (const bf16_t *)v, (const bf16_t *)d_o,         \
-                       (const float2 *)ws, (bf16_t *)dk, (bf16_t *)dv, ws_dk, ws_dv, scale, scale * LOG2E, drop.thr, drop.seed, drop.inv)
+                       (const float2 *)ws, (bf16_t *)dk, (bf16_t *)dv, ws_dk, ws_dv, scale, scale * LOG2E, drop.thr, drop.seed, drop.inv, NoMod{})
 #define LAUNCH_SRC_PDS(SP)                                                                                                               \
     hipLaunchKernelGGL((k_attn_bwd_src_tile_bf16<H, D, HW, TILE_BF16_WPE_SRC, false, SP>), dim3(group_grid(Pout) * (H * SP / HW)), \
                        dim3(HW * WAVE), 0, s, *Pout, (const bf16_t *)q, (const bf16_t *)d_o, (const uint32_t *)ws, (bf16_t *)dk, (bf16_t *)dv, \
@@ -4262,7 +4262,7 @@ int run_attn_fwd_narrow(const bpt_plan *P, const void *q, const void *k, const v
     do {                                                                                                                                 \
         if constexpr (sizeof(T) == 4)                                                                                                    \
             hipLaunchKernelGGL((k_attn_fwd_tile<T, 16, 64, HW, DR, 0, true, SP>), grid, block, 0, s, *P, (const T *)q, (const T *)k,         \
-                               (const T *)v, (T *)o, lse, ws_acc, ws_ml, scale * LOG2E, drop.thr, drop.seed, drop.inv, (const float *)nullptr, np, keep); \
+                               (const T *)v, (T *)o, lse, ws_acc, ws_ml, scale * LOG2E, drop.thr, drop.seed, drop.inv, (const float *)nullptr, np, keep, NoMod{}); \
         else                                                                                                                             \
             hipLaunchKernelGGL((k_attn_fwd_tile_bf16<16, 64, HW, TILE_BF16_WPE, DR, SP>), grid, block, 0, s, *P,                             \
                                (const T *)q, (const T *)k, (const T *)v, (T *)o, lse, ws_acc, ws_ml, scale * LOG2E, drop.thr, drop.seed,       \
@@ -4304,7 +4304,7 @@ int run_attn_bwd_narrow(const bpt_plan *Pin, const bpt_plan *Pout, const void *q
         if constexpr (sizeof(T) == 4)                                                                                                    \
             hipLaunchKernelGGL((k_attn_bwd_dst_tile<T, 16, 64, HW, DR, 0, true, SP>), grid, block, 0, s, *Pin, (const T *)q,                 \
                                (const T *)k, (const T *)v, (const T *)o, (const T *)d_o, lse, (T *)dq, pds, ws_dq, scale, scale * LOG2E,       \
-                               drop.thr, drop.seed, drop.inv, (const float *)nullptr, (float *)nullptr, np);                                \
+                               drop.thr, drop.seed, drop.inv, (const float *)nullptr, (float *)nullptr, np, NoMod{});                                \
         else                                                                                                                             \
             hipLaunchKernelGGL((k_attn_bwd_dst_tile_bf16<16, 64, HW, TILE_BF16_WPE_DST, DR, SP>), grid, block, 0, s, *Pin,                   \
                                (const T *)q, (const T *)k, (const T *)v, (const T *)o, (const T *)d_o, lse, (T *)dq, pds, ws_dq, \

@@ -493,7 +493,7 @@ __device__ __forceinline__ int lane_bcast(int x, int src_lane) { return __builti
 // Common start of the tile kernels.  HW heads (= wavefronts) per workgroup: workgroup b handles head slice
 // (b / 8) % (H / HW) of group (b / 8) / (H / HW) of XCD b % 8's range.
 struct TileCtx {
-    int lane, wv, c, g, head, p_begin, p_end, part;
+    int lane, wv, c, g, head, p_begin, p_end, part, grp;
     int2 member;                 // (row, slot) of member c
     uint32_t offa, offv;         // byte offsets of this lane inside a node row: its 16-column slice of the head (operands of the
                                  // products that contract over columns, + 64 t bytes per step), and its columns 4 c .. 4 c + 3
@@ -512,6 +512,7 @@ __device__ __forceinline__ bool tile_begin(const bpt_plan &P, TileCtx &t, const 
     const int x = block & 7, w = (int)(block >> 3) / HS;
     const int grp = __builtin_amdgcn_readfirstlane(P.grp_chunks[x]) + w;
     if (grp >= __builtin_amdgcn_readfirstlane(P.grp_chunks[x + 1])) return false;
+    t.grp = grp;
     t.member = reinterpret_cast<const int2 *>(P.grp_members)[(size_t)grp * TILE_R + t.c];
     t.p_begin = __builtin_amdgcn_readfirstlane(P.grp_ptr[grp]);
     t.p_end = __builtin_amdgcn_readfirstlane(P.grp_ptr[grp + 1]);
@@ -861,11 +862,74 @@ __device__ __forceinline__ void tile_walk_first_ahead(int nblk, IssueFirst &&fir
     issue_loads_first();
 }
 
-template <typename T, int H, int D, int HW, bool DROP, int BIAS, bool NARROW = false, int SP = 1>
+// Scores that are capped and lowered by distance (MOD): with u = scale (q.k + term),
+//   s = cap tanh(u / cap) - slope[head] |pos[dst] - pos[src]|,   ds/du = 1 - tanh^2(u / cap),   dslope[head] = -sum over the pairs of dL/ds |pos - pos|
+// A pair costs a handful of vector instructions more (tile_mod_scores), a block one load of its entries' positions by sixteen lanes, which
+// travels with the block's rows and reaches the lanes through LDS, and nothing of an edge's size is read or written.
+struct ScoreMod {
+    float to_tanh, from_tanh;          // scale / cap, and cap in base-2 units; to_tanh 0: not capped
+    const float *slopes;               // (heads), or null: no distance
+    const float *pos_member, *pos_entry;       // positions of the plan's rows, of the rows its indices name
+    float *part;                       // destination side: [group][head][part] sums of dL/ds |pos - pos|, or null
+};
+struct NoMod {};
+template <bool MOD> struct ModArg { typedef NoMod type; };
+template <> struct ModArg<true> { typedef ScoreMod type; };
+
+// tanh of the block's four u, and 1 - tanh^2.  |u| <= 1/2, where nearly all scores lie (u is a score of a few units over a cap of tens): odd
+// polynomial, u + u w (c0 + c1 w + c2 w^2 + c3 w^3) with w = u^2, fitted by weighted least squares to the relative error, 1.5e-8 (1.25 half steps
+// of float32 as evaluated); a wavefront without a larger |u| evaluates nothing else.  Beyond, (1 - e) / (1 + e) with e = exp(-2 |u|), whose
+// difference keeps its digits there.  (1 - e) / (1 + e) everywhere costs less for large |u| but is off by 2^-24 absolutely, which times a
+// cap of 50 is more than all other roundings of a score.
+__device__ __forceinline__ float tile_tanh_small(float u) {
+    const float w = u * u;
+    const float p = fmaf(fmaf(fmaf(0.01724148355424404f, w, -0.05304549261927605f), w, 0.13325878977775574f), w, -0.333331435918808f);
+    return fmaf(u, w * p, u);
+}
+// s (base-2 units) and ds/du of the pairs whose q.k (+ term) is x; pos_e: positions of the pairs' entries
+__device__ __forceinline__ void tile_mod_scores(const ScoreMod &md, float scale_log2e, float slope_log2e, float pos_m, const float (&pos_e)[4],
+                                                const float (&x)[4], float (&s)[4], float (&du)[4]) {
+    if (md.to_tanh != 0.f) {
+        float u[4], t[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) u[r] = x[r] * md.to_tanh;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) t[r] = tile_tanh_small(u[r]);
+        const float top = fmaxf(fmaxf(fabsf(u[0]), fabsf(u[1])), fmaxf(fabsf(u[2]), fabsf(u[3])));
+        if (__builtin_amdgcn_ballot_w64(top > 0.5f) != 0) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float e = __builtin_amdgcn_exp2f(fabsf(u[r]) * (-2.f * LOG2E));
+                const float far = copysignf((1.f - e) * __builtin_amdgcn_rcpf(1.f + e), u[r]);
+                t[r] = fabsf(u[r]) > 0.5f ? far : t[r];
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            s[r] = t[r] * md.from_tanh;
+            du[r] = fmaf(-t[r], t[r], 1.f);
+        }
+    } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) { s[r] = x[r] * scale_log2e; du[r] = 1.f; }
+    }
+    if (md.slopes) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[r] = fmaf(-slope_log2e, fabsf(pos_m - pos_e[r]), s[r]);
+    }
+}
+// dslope of a wavefront's pairs (part s of SP of a group and head): the sum over its lanes
+template <int SP> __device__ __forceinline__ void tile_put_slope_part(const ScoreMod &md, const TileCtx &t, int heads, float x) {
+    if (!md.part) return;
+    x = groups_sum(head_sum<16>(x));
+    if (t.lane == 0) md.part[((size_t)t.grp * heads + t.head) * SP + t.part] = x;
+}
+
+template <typename T, int H, int D, int HW, bool DROP, int BIAS, bool NARROW = false, int SP = 1, bool MOD = false>
 __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(4))) void k_attn_fwd_tile(
     bpt_plan P, const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v, T *__restrict__ o, float *__restrict__ lse,
     float *__restrict__ ws_acc, float *__restrict__ ws_ml, float scale_log2e, uint32_t drop_thr, uint32_t drop_seed, float drop_inv,
-    const float *__restrict__ bias, Narrow nw, Keep keep) {
+    const float *__restrict__ bias, Narrow nw, Keep keep, typename ModArg<MOD>::type md) {
     const int Hs = NARROW ? nw.h : H;                             // heads as lse, workspace and dropout keys count them
     const uint32_t RB = NARROW ? (uint32_t)(nw.heads * nw.d) * sizeof(T) : (uint32_t)(H * D * sizeof(T));        // bytes of a node row
     int block = (int)blockIdx.x;
@@ -880,6 +944,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(4))) 
     int *fst = BIAS == 2 ? fst_lds[t.wv] : nullptr;
     __shared__ __attribute__((aligned(16))) float kt_lds[HW][TILE_R * TILE_KT_STRIDE];
     float *kt = kt_lds[t.wv];
+    __shared__ float pos_lds[HW][MOD ? TILE_R : 1];              // positions of the block's entries
     TileEntryRegs er;
     if (t.p_end > t.p_begin) tile_ask_entries(P, t.p_begin, min(TILE_CHUNK, t.p_end - t.p_begin), t.lane, er);
     issue_loads_first();
@@ -892,11 +957,18 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(4))) 
     const char *const qrow = reinterpret_cast<const char *>(q) + (size_t)max(t.member.x, 0) * RB + t.offa;
     // (with the score term the sixteen registers are not there; with dropout they just are, and it does not pay: L = 8192 level, 6 x 50
     // with dropout 97.7 -> 100 us)
-    constexpr bool AHEAD = !DROP && BIAS == 0;
+    constexpr bool AHEAD = !DROP && BIAS == 0 && !MOD;
     if constexpr (!AHEAD) {
         float4 qr[4];
         tile_ask_members<NARROW>(t, q, RB, qr);
         tile_rows_to_operand<NARROW>(kt, qr, c, g, qb, nw);
+    }
+    float slope = 0.f, pos_m = 0.f;
+    if constexpr (MOD) {
+        if (md.slopes) {
+            slope = md.slopes[t.head] * LOG2E;
+            pos_m = md.pos_member[max(t.member.x, 0)];
+        }
     }
     floatx4v acc[4];
 #pragma unroll
@@ -909,6 +981,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(4))) 
         int mk[4], nv;                                            // bit c of mk[r]: the pair (entry 4 r + g, member c) exists; nv: entries of the block that exist
         int xe[DROP || BIAS == 1 ? 4 : 1];
         float bz[BIAS ? 4 : 1];
+        float pos;                                                // of entry c, in the first lane group
     };
     for (int p0 = t.p_begin; p0 < t.p_end; p0 += TILE_CHUNK) {
         const int cnt = min(TILE_CHUNK, t.p_end - p0), nblk = (cnt + TILE_R - 1) / TILE_R;
@@ -922,6 +995,9 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(4))) 
         auto issue_rest = [&](Blk &B, int b) {
             if constexpr (DROP || BIAS == 1) tile_pair_eids(P, p0 + TILE_R * b + g, t.p_end, c, B.xe, 4);
             B.nv = min(TILE_R, cnt - TILE_R * b);
+            if constexpr (MOD) {
+                if (md.slopes && g == 0) B.pos = md.pos_entry[ent[TILE_R * b + c].x];
+            }
             int idxv[4];
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
@@ -942,9 +1018,23 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(4))) 
         };
         auto compute = [&](const Blk &B) {
             float kr[16];
+            if constexpr (MOD) {
+                if (md.slopes && g == 0) pos_lds[t.wv][c] = B.pos;
+            }
             tile_rows_to_operand<NARROW>(kt, B.kq, c, g, kr, nw);
             const floatx4v st = tile_dot(kr, qb);
             float sc[4];
+            if constexpr (MOD) {
+                float x[4], pos_e[4], du[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    x[r] = BIAS ? st[r] + B.bz[BIAS ? r : 0] : st[r];
+                    pos_e[r] = md.slopes ? pos_lds[t.wv][4 * r + g] : 0.f;
+                }
+                tile_mod_scores(md, scale_log2e, slope, pos_m, pos_e, x, sc, du);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) sc[r] = where_pair(B.mk[r], c, sc[r]);
+            } else
 #pragma unroll
             for (int r = 0; r < 4; ++r)
                 sc[r] = where_pair(B.mk[r], c, BIAS ? fmaf(st[r], scale_log2e, B.bz[BIAS ? r : 0] * scale_log2e) : st[r] * scale_log2e);
@@ -1010,12 +1100,12 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(4))) 
 // source side's layout instead (scattered 8-byte stores here, contiguous reads there) cost this kernel a third of its
 // time (126 against 85 us at L = 4096, k = 32); letting the source side recompute p and ds (two more products there,
 // delta (n, H) handed over) measured slower than either on every graph tried.
-template <typename T, int H, int D, int HW, bool DROP, int BIAS, bool NARROW = false, int SP = 1>
-__global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP || BIAS ? 3 : 4))) void k_attn_bwd_dst_tile(
+template <typename T, int H, int D, int HW, bool DROP, int BIAS, bool NARROW = false, int SP = 1, bool MOD = false>
+__global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP || BIAS || MOD ? 3 : 4))) void k_attn_bwd_dst_tile(
     bpt_plan P, const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v, const T *__restrict__ o,
     const T *__restrict__ d_o, const float *__restrict__ lse, T *__restrict__ dq, float2 *__restrict__ pds, float *__restrict__ ws_dq,
     float scale, float scale_log2e, uint32_t drop_thr, uint32_t drop_seed, float drop_inv, const float *__restrict__ bias,
-    float *__restrict__ ds_out, Narrow nw) {
+    float *__restrict__ ds_out, Narrow nw, typename ModArg<MOD>::type md) {
     const int Hs = NARROW ? nw.h : H;
     const uint32_t RB = NARROW ? (uint32_t)(nw.heads * nw.d) * sizeof(T) : (uint32_t)(H * D * sizeof(T));
     TileCtx t;
@@ -1026,6 +1116,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP 
     int *fst = fst_lds[t.wv];
     __shared__ __attribute__((aligned(16))) float kt_lds[HW][TILE_R * TILE_KT_STRIDE];
     float *kt = kt_lds[t.wv];
+    __shared__ float pos_lds[HW][MOD ? TILE_R : 1];
     TileEntryRegs er;
     if (t.p_end > t.p_begin) tile_ask_entries(P, t.p_begin, min(TILE_CHUNK, t.p_end - t.p_begin), t.lane, er);
     issue_loads_first();
@@ -1090,6 +1181,13 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP 
 #pragma unroll
         for (int i = 0; i < 4; ++i) dob_h[i][t.lane] = floatx4v{dob[4 * i], dob[4 * i + 1], dob[4 * i + 2], dob[4 * i + 3]};
     }
+    float slope = 0.f, pos_m = 0.f, slope_sum = 0.f;
+    if constexpr (MOD) {
+        if (md.slopes) {
+            slope = md.slopes[t.head] * LOG2E;
+            pos_m = md.pos_member[max(t.member.x, 0)];
+        }
+    }
     floatx4v acc[4];
 #pragma unroll
     for (int nb = 0; nb < 4; ++nb) acc[nb] = floatx4v{0.f, 0.f, 0.f, 0.f};
@@ -1098,6 +1196,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP 
         int b, nv;                                                // which block of the piece; entries of it that exist
         int xe[DROP || BIAS == 1 ? 4 : 1];
         float bz[BIAS ? 4 : 1];
+        float pos;                                                // of entry c, in the first lane group
     };
     for (int p0 = t.p_begin; p0 < t.p_end; p0 += TILE_CHUNK) {
         const int cnt = min(TILE_CHUNK, t.p_end - p0), nblk = (cnt + TILE_R - 1) / TILE_R;
@@ -1106,6 +1205,9 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP 
         auto issue = [&](Blk &B, int b) {
             if constexpr (DROP || BIAS == 1) tile_pair_eids(P, p0 + TILE_R * b + g, t.p_end, c, B.xe, 4);
             B.b = b;
+            if constexpr (MOD) {
+                if (md.slopes && g == 0) B.pos = md.pos_entry[ent[TILE_R * b + c].x];
+            }
             B.nv = min(TILE_R, cnt - TILE_R * b);
             int idxv[4];
 #pragma unroll
@@ -1132,6 +1234,9 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP 
                 mask[r] = ent[at].y;
                 number[r] = tile_pair_number(fst[at], mask[r], c);
             }
+            if constexpr (MOD) {
+                if (md.slopes && g == 0) pos_lds[t.wv][c] = B.pos;
+            }
             floatx4v st;
             {
                 float kr[16];
@@ -1147,14 +1252,29 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP 
                 dob[4 * i] = x[0]; dob[4 * i + 1] = x[1]; dob[4 * i + 2] = x[2]; dob[4 * i + 3] = x[3];
             }
             const floatx4v dp = tile_dot(va, dob);
-            float ds[4];
+            float ds[4], sm[4], du[4], pos_e[4];
+            if constexpr (MOD) {
+                float x[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    x[r] = BIAS ? st[r] + B.bz[BIAS ? r : 0] : st[r];
+                    pos_e[r] = md.slopes ? pos_lds[t.wv][4 * r + g] : 0.f;
+                }
+                tile_mod_scores(md, scale_log2e, slope, pos_m, pos_e, x, sm, du);
+            }
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                float pe = where_pair_or_zero(mask[r], c, __builtin_amdgcn_exp2f((BIAS ? fmaf(st[r], scale_log2e, B.bz[BIAS ? r : 0] * scale_log2e) : st[r] * scale_log2e) - lse_c));
+                float pe = where_pair_or_zero(mask[r], c, __builtin_amdgcn_exp2f((MOD ? sm[r] : BIAS ? fmaf(st[r], scale_log2e, B.bz[BIAS ? r : 0] * scale_log2e) : st[r] * scale_log2e) - lse_c));
                 float mt = 1.f;                                   // dropout multiplier of this pair (as in the forward)
                 if constexpr (DROP)
                     mt = dropout_keep((uint32_t)B.xe[DROP ? r : 0] * (uint32_t)Hs + (uint32_t)t.head, drop_seed, drop_thr, drop_inv);
-                ds[r] = pe * (dp[r] * mt - delta) * scale;
+                if constexpr (MOD) {
+                    ds[r] = where_pair_or_zero(mask[r], c, pe * (dp[r] * mt - delta));
+                    if (md.part) slope_sum = fmaf(ds[r], fabsf(pos_m - pos_e[r]), slope_sum);
+                    ds[r] *= du[r] * scale;
+                } else {
+                    ds[r] = pe * (dp[r] * mt - delta) * scale;
+                }
                 pe *= mt;                                         // what multiplies v (forward) and dO (dV)
                 if ((mask[r] >> c) & 1) {
                     pds_h[(uint32_t)number[r]] = make_float2(pe, ds[r]);
@@ -1166,6 +1286,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP 
         tile_walk<Blk>(nblk, issue, compute);
         wave_lds_fence();
     }
+    if constexpr (MOD) tile_put_slope_part<SP>(md, t, Hs, slope_sum);
     if constexpr (SP > 1) {
         tile_park(kt, acc, t.lane);
         __syncthreads();
@@ -1480,11 +1601,11 @@ __device__ __forceinline__ void tile_store_sums(const TileCtx &t, float *sh, con
     wave_lds_fence();
 }
 
-template <int H, int D, int HW, int WPE, bool DROP, int BIAS, int SP>
-__global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP || BIAS ? WPE - 1 : WPE))) void k_attn_fwd_rows_bf16(
+template <int H, int D, int HW, int WPE, bool DROP, int BIAS, int SP, bool MOD = false>
+__global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP || BIAS || MOD ? WPE - 1 : WPE))) void k_attn_fwd_rows_bf16(
     bpt_plan P, const bf16_t *__restrict__ q, const bf16_t *__restrict__ k, const bf16_t *__restrict__ v, bf16_t *__restrict__ o,
     float *__restrict__ lse, float *__restrict__ ws_acc, float *__restrict__ ws_ml, float scale_log2e, uint32_t drop_thr,
-    uint32_t drop_seed, float drop_inv, const float *__restrict__ bias) {
+    uint32_t drop_seed, float drop_inv, const float *__restrict__ bias, typename ModArg<MOD>::type md) {
     constexpr uint32_t RB = H * D * 2;
     const Narrow nw{};
     TileCtx t;
@@ -1496,6 +1617,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP 
     constexpr int PIECE = 2 * TILE_ROWS_FLOATS_BF16 + 4 * TILE_R;      // (the turned sums' rows are longer)
     static_assert(PIECE >= TILE_PART_FWD_FLOATS && PIECE >= TILE_R * TILE_TURN_STRIDE, "parts and turned sums fit the rows' piece");
     __shared__ __attribute__((aligned(16))) float piece[HW][PIECE];
+    __shared__ __attribute__((aligned(16))) float pos_lds[HW][MOD ? TILE_R : 4];      // positions of the block's entries
     char *const k_lds = reinterpret_cast<char *>(piece[t.wv]), *const v_lds = k_lds + 4 * TILE_ROWS_FLOATS_BF16;
     TileEntryRegs er;
     if (t.p_end > t.p_begin) tile_ask_entries(P, t.p_begin, min(TILE_CHUNK, t.p_end - t.p_begin), t.lane, er);
@@ -1510,6 +1632,13 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP 
     }
     issue_loads_first();
     Bf8 qb[2];
+    float slope = 0.f, pos_m = 0.f;
+    if constexpr (MOD) {
+        if (md.slopes) {
+            slope = md.slopes[t.head] * LOG2E;
+            pos_m = md.pos_member[max(t.member.x, 0)];
+        }
+    }
     floatx4v acc[4];
 #pragma unroll
     for (int nb = 0; nb < 4; ++nb) acc[nb] = floatx4v{0.f, 0.f, 0.f, 0.f};
@@ -1519,6 +1648,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP 
         uintx4v kr[2], vr[2];
         int xe[DROP || BIAS == 1 ? 4 : 1];
         float bz[BIAS ? 4 : 1];
+        float pos;                                                // of entry c, in the first lane group
     };
     for (int p0 = t.p_begin; p0 < t.p_end; p0 += TILE_CHUNK) {
         const int cnt = min(TILE_CHUNK, t.p_end - p0), nblk = (cnt + TILE_R - 1) / TILE_R;
@@ -1526,6 +1656,9 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP 
         tile_put_entries(er, ent, cnt, t.lane, fst);
         auto issue = [&](Blk &B, int b) {
             if constexpr (DROP || BIAS == 1) tile_pair_eids(P, p0 + TILE_R * b + 4 * g, t.p_end, c, B.xe);
+            if constexpr (MOD) {
+                if (md.slopes && g == 0) B.pos = md.pos_entry[ent[TILE_R * b + c].x];
+            }
             uint32_t off[2];
             tile_entry_offsets<RB>(t, ent + TILE_R * b, off);
             tile_ask_rows_bf16(kb, off, B.kr);
@@ -1561,6 +1694,9 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP 
             }
             tile_put_rows_bf16(k_lds, B.kr, t.lane);
             tile_put_rows_bf16(v_lds, B.vr, t.lane);
+            if constexpr (MOD) {
+                if (md.slopes && g == 0) pos_lds[t.wv][c] = B.pos;
+            }
             wave_lds_fence();
             if (b + 1 < nblk) issue(B, b + 1);
             issue_loads_first();
@@ -1568,6 +1704,16 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP 
             tile_operand_bf16(k_lds, c, g, kr);
             const floatx4v st = tile_dot_bf16(kr, qb);
             float sc[4];
+            if constexpr (MOD) {
+                float x[4], du[4];
+                const floatx4v pe = *reinterpret_cast<const floatx4v *>(&pos_lds[t.wv][4 * g]);
+                const float pos_e[4] = {pe[0], pe[1], pe[2], pe[3]};
+#pragma unroll
+                for (int r = 0; r < 4; ++r) x[r] = BIAS ? st[r] + bz[BIAS ? r : 0] : st[r];
+                tile_mod_scores(md, scale_log2e, slope, pos_m, pos_e, x, sc, du);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) sc[r] = where_pair(mk[r], c, sc[r]);
+            } else
 #pragma unroll
             for (int r = 0; r < 4; ++r) sc[r] = where_pair(mk[r], c, (BIAS ? st[r] + bz[BIAS ? r : 0] : st[r]) * scale_log2e);
             const float mb = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3]));
@@ -1624,12 +1770,12 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP 
 // Destination side.  PDS: (p, ds) of the pairs go to the scratch for the source side that reads them back; otherwise that side
 // forms them again (k_attn_bwd_src_tile_bf16_again) and all it is handed is (lse, delta) of the rows, `stat` (n, H): the
 // segments of a split row write the same values.
-template <int H, int D, int HW, int WPE, bool DROP, int BIAS, bool PDS, int SP>
-__global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP || BIAS ? WPE - 1 : WPE))) void k_attn_bwd_dst_rows_bf16(
+template <int H, int D, int HW, int WPE, bool DROP, int BIAS, bool PDS, int SP, bool MOD = false>
+__global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP || BIAS || MOD ? WPE - 1 : WPE))) void k_attn_bwd_dst_rows_bf16(
     bpt_plan P, const bf16_t *__restrict__ q, const bf16_t *__restrict__ k, const bf16_t *__restrict__ v, const bf16_t *__restrict__ o,
     const bf16_t *__restrict__ d_o, const float *__restrict__ lse, bf16_t *__restrict__ dq, uint32_t *__restrict__ pds,
     float2 *__restrict__ stat, float *__restrict__ ws_dq, float scale, float scale_log2e, uint32_t drop_thr, uint32_t drop_seed, float drop_inv,
-    const float *__restrict__ bias, float *__restrict__ ds_out) {
+    const float *__restrict__ bias, float *__restrict__ ds_out, typename ModArg<MOD>::type md) {
     static_assert(PDS || BIAS == 0, "the score term's gradient is stored by the pair's position");
     constexpr uint32_t RB = H * D * 2;
     const Narrow nw{};
@@ -1642,6 +1788,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP 
     constexpr int PIECE = 2 * TILE_ROWS_FLOATS_BF16 + 4 * TILE_R;      // (the turned sums' rows are longer)
     static_assert(PIECE >= TILE_PART_FLOATS && PIECE >= TILE_R * TILE_TURN_STRIDE, "parts and turned sums fit the rows' piece");
     __shared__ __attribute__((aligned(16))) float piece[HW][PIECE];
+    __shared__ __attribute__((aligned(16))) float pos_lds[HW][MOD ? TILE_R : 4];
     char *const k_lds = reinterpret_cast<char *>(piece[t.wv]), *const v_lds = k_lds + 4 * TILE_ROWS_FLOATS_BF16;
     TileEntryRegs er;
     if (t.p_end > t.p_begin) tile_ask_entries(P, t.p_begin, min(TILE_CHUNK, t.p_end - t.p_begin), t.lane, er);
@@ -1684,6 +1831,13 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP 
         }
         lse_c = lane_bcast(lse_c, c);
     }
+    float slope = 0.f, pos_m = 0.f, slope_sum = 0.f;
+    if constexpr (MOD) {
+        if (md.slopes) {
+            slope = md.slopes[t.head] * LOG2E;
+            pos_m = md.pos_member[max(t.member.x, 0)];
+        }
+    }
     floatx4v acc[4];
 #pragma unroll
     for (int nb = 0; nb < 4; ++nb) acc[nb] = floatx4v{0.f, 0.f, 0.f, 0.f};
@@ -1691,6 +1845,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP 
         uintx4v kr[2], vr[2];
         int xe[DROP || BIAS == 1 ? 4 : 1];
         float bz[BIAS ? 4 : 1];
+        float pos;                                                // of entry c, in the first lane group
     };
     for (int p0 = t.p_begin; p0 < t.p_end; p0 += TILE_CHUNK) {
         const int cnt = min(TILE_CHUNK, t.p_end - p0), nblk = (cnt + TILE_R - 1) / TILE_R;
@@ -1703,6 +1858,9 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP 
         };
         auto issue = [&](Blk &B, int b) {
             if constexpr (DROP || BIAS == 1) tile_pair_eids(P, p0 + TILE_R * b + 4 * g, t.p_end, c, B.xe);
+            if constexpr (MOD) {
+                if (md.slopes && g == 0) B.pos = md.pos_entry[ent[TILE_R * b + c].x];
+            }
             uint32_t off[2];
             tile_entry_offsets<RB>(t, ent + TILE_R * b, off);
             tile_ask_rows_bf16(kb, off, B.kr);
@@ -1731,6 +1889,9 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP 
             }
             tile_put_rows_bf16(k_lds, B.kr, t.lane);
             tile_put_rows_bf16(v_lds, B.vr, t.lane);
+            if constexpr (MOD) {
+                if (md.slopes && g == 0) pos_lds[t.wv][c] = B.pos;
+            }
             wave_lds_fence();
             if (b + 1 < nblk) issue(B, b + 1);
             issue_loads_first();
@@ -1739,14 +1900,30 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP 
             const floatx4v st = tile_dot_bf16(row, qb);
             tile_operand_bf16(v_lds, c, g, row);
             const floatx4v dp = tile_dot_bf16(row, dob);
-            float ds[4];
+            float ds[4], sm[4], du[4], pos_e[4];
+            if constexpr (MOD) {
+                float x[4];
+                const floatx4v at_e = *reinterpret_cast<const floatx4v *>(&pos_lds[t.wv][4 * g]);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    x[r] = BIAS ? st[r] + bz[BIAS ? r : 0] : st[r];
+                    pos_e[r] = at_e[r];
+                }
+                tile_mod_scores(md, scale_log2e, slope, pos_m, pos_e, x, sm, du);
+            }
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                float pe = where_pair_or_zero(mk[r], c, __builtin_amdgcn_exp2f((BIAS ? st[r] + bz[BIAS ? r : 0] : st[r]) * scale_log2e - lse_c));
+                float pe = where_pair_or_zero(mk[r], c, __builtin_amdgcn_exp2f(MOD ? sm[r] - lse_c : (BIAS ? st[r] + bz[BIAS ? r : 0] : st[r]) * scale_log2e - lse_c));
                 float mt = 1.f;                                   // dropout multiplier of this pair (as in the forward)
                 if constexpr (DROP)
                     mt = dropout_keep((uint32_t)xe[DROP ? r : 0] * (uint32_t)H + (uint32_t)t.head, drop_seed, drop_thr, drop_inv);
-                ds[r] = pe * (dp[r] * mt - delta) * scale;
+                if constexpr (MOD) {
+                    ds[r] = where_pair_or_zero(mk[r], c, pe * (dp[r] * mt - delta));
+                    if (md.part) slope_sum = fmaf(ds[r], fabsf(pos_m - pos_e[r]), slope_sum);
+                    ds[r] *= du[r] * scale;
+                } else {
+                    ds[r] = pe * (dp[r] * mt - delta) * scale;
+                }
                 pe *= mt;                                         // what multiplies v (forward) and dO (dV)
                 if (PDS && ((mk[r] >> c) & 1)) {
                     pds_h[pos[r]] = pack_bf16(pe, ds[r]);
@@ -1761,6 +1938,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP 
             issue_loads_first();
         }
     }
+    if constexpr (MOD) tile_put_slope_part<SP>(md, t, H, slope_sum);
     if constexpr (SP > 1) {
         tile_sums_by_row(piece[t.wv], acc, c, g);
         tile_park(piece[t.wv], acc, t.lane);
@@ -2093,11 +2271,11 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(WPE))
 // 30.9; L = 32768, k = 2 235 -> 221; 32-graph batch 102.5 -> 99.2; L = 512 and L = 8192 with dropout level.  (6 heads of 50
 // columns with dropout lost 2 %: heads of fewer than 64 columns keep the scratch.)  float32 keeps it too: there the two
 // products are 1024 cycles of the matrix pipeline per block.  122 registers: compiled for four wavefronts per SIMD.
-template <int H, int D, int HW, int WPE, bool DROP, int SP = 1>
+template <int H, int D, int HW, int WPE, bool DROP, int SP = 1, bool MOD = false>
 __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(WPE))) void k_attn_bwd_src_tile_bf16_again(
     bpt_plan P, const bf16_t *__restrict__ q, const bf16_t *__restrict__ k, const bf16_t *__restrict__ v, const bf16_t *__restrict__ d_o,
     const float2 *__restrict__ stat, bf16_t *__restrict__ dk, bf16_t *__restrict__ dv, float *__restrict__ ws_dk, float *__restrict__ ws_dv,
-    float scale, float scale_log2e, uint32_t drop_thr, uint32_t drop_seed, float drop_inv) {
+    float scale, float scale_log2e, uint32_t drop_thr, uint32_t drop_seed, float drop_inv, typename ModArg<MOD>::type md) {
     constexpr uint32_t RB = H * D * 2;
     const Narrow nw{};
     TileCtx t;
@@ -2106,6 +2284,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(WPE))
     constexpr int ENT = TILE_CHUNK * 2, ROWS = 2 * TILE_ROWS_FLOATS_BF16 + 4 * TILE_R, LIVE = ENT + ROWS + 2 * TILE_R, PIECE = SP > 1 ? 2 * TILE_PART_FLOATS : LIVE;
     static_assert(PIECE >= LIVE && ROWS >= TILE_R * TILE_TURN_STRIDE, "the lists and the turned sums fit");
     __shared__ __attribute__((aligned(16))) float piece[HW][PIECE];
+    __shared__ __attribute__((aligned(16))) float pos_lds[HW][MOD ? TILE_R : 4];
     int2 *ent = reinterpret_cast<int2 *>(piece[t.wv]);
     char *const q_lds = reinterpret_cast<char *>(piece[t.wv] + ENT), *const d_lds = q_lds + 4 * TILE_ROWS_FLOATS_BF16;
     float2 *const st_lds = reinterpret_cast<float2 *>(piece[t.wv] + ENT + ROWS);
@@ -2129,6 +2308,13 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(WPE))
         tile_operand_bf16(d_lds, c, g, vb);
         wave_lds_fence();
     }
+    float slope = 0.f, pos_m = 0.f;
+    if constexpr (MOD) {
+        if (md.slopes) {
+            slope = md.slopes[t.head] * LOG2E;
+            pos_m = md.pos_member[max(t.member.x, 0)];
+        }
+    }
     floatx4v ak[4], av[4];
 #pragma unroll
     for (int nb = 0; nb < 4; ++nb) { ak[nb] = floatx4v{0.f, 0.f, 0.f, 0.f}; av[nb] = floatx4v{0.f, 0.f, 0.f, 0.f}; }
@@ -2136,6 +2322,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(WPE))
         uintx4v qr[2], dr[2];
         float2 ld;                                                // (lse, delta) of entry c, in the first lane group
         int xe[DROP ? 4 : 1];
+        float pos;                                                // of entry c, in the first lane group
     };
     for (int p0 = t.p_begin; p0 < t.p_end; p0 += TILE_CHUNK) {
         const int cnt = min(TILE_CHUNK, t.p_end - p0), nblk = (cnt + TILE_R - 1) / TILE_R;
@@ -2143,6 +2330,9 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(WPE))
         tile_put_entries(er, ent, cnt, t.lane);
         auto issue = [&](Blk &B, int b) {
             if constexpr (DROP) tile_pair_eids(P, p0 + TILE_R * b + 4 * g, t.p_end, c, B.xe);
+            if constexpr (MOD) {
+                if (md.slopes && g == 0) B.pos = md.pos_entry[ent[TILE_R * b + c].x];
+            }
             if (g == 0) B.ld = stat_h[(size_t)ent[TILE_R * b + c].x * H];
             uint32_t off[2];
             tile_entry_offsets<RB>(t, ent + TILE_R * b, off);
@@ -2159,6 +2349,9 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(WPE))
             tile_put_rows_bf16(q_lds, B.qr, t.lane);
             tile_put_rows_bf16(d_lds, B.dr, t.lane);
             if (g == 0) st_lds[c] = B.ld;
+            if constexpr (MOD) {
+                if (md.slopes && g == 0) pos_lds[t.wv][c] = B.pos;
+            }
             wave_lds_fence();
             if (b + 1 < nblk) issue(B, b + 1);
             issue_loads_first();
@@ -2169,14 +2362,19 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(WPE))
             const float lse_e[4] = {l01[0], l01[2], l23[0], l23[2]}, delta_e[4] = {l01[1], l01[3], l23[1], l23[3]};
             tile_operand_bf16(d_lds, c, g, row);
             const floatx4v dp = tile_dot_bf16(row, vb);
-            float pe[4], ds[4];
+            float pe[4], ds[4], sm[4], du[4];
+            if constexpr (MOD) {
+                const floatx4v at_e = *reinterpret_cast<const floatx4v *>(&pos_lds[t.wv][4 * g]);
+                const float pos_e[4] = {at_e[0], at_e[1], at_e[2], at_e[3]}, x[4] = {st[0], st[1], st[2], st[3]};
+                tile_mod_scores(md, scale_log2e, slope, pos_m, pos_e, x, sm, du);
+            }
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const float p = where_pair_or_zero(mk[r], c, __builtin_amdgcn_exp2f(st[r] * scale_log2e - lse_e[r]));
+                const float p = where_pair_or_zero(mk[r], c, __builtin_amdgcn_exp2f((MOD ? sm[r] : st[r] * scale_log2e) - lse_e[r]));
                 float mt = 1.f;                                   // dropout multiplier of this pair (as in the forward)
                 if constexpr (DROP)
                     mt = dropout_keep((uint32_t)xe[DROP ? r : 0] * (uint32_t)H + (uint32_t)t.head, drop_seed, drop_thr, drop_inv);
-                ds[r] = where_pair_or_zero(mk[r], c, p * (dp[r] * mt - delta_e[r]) * scale);
+                ds[r] = where_pair_or_zero(mk[r], c, MOD ? p * (dp[r] * mt - delta_e[r]) * (du[r] * scale) : p * (dp[r] * mt - delta_e[r]) * scale);
                 pe[r] = p * mt;
             }
             Bf4 pa, da;

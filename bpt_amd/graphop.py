@@ -19,7 +19,7 @@ import threading
 
 import torch
 
-from ._lib import BPT_ERR_UNSUPPORTED, BptStatusError, PlanStruct, attn_lib, check_attn
+from ._lib import BPT_ERR_UNSUPPORTED, BptStatusError, PlanStruct, ScoreStruct, attn_lib, check_attn, score_lib
 from ._native import native as _native
 from . import plan as _plan
 from .plan import GROUP_ORDER_SRC, TILE_GROUP_R, PlanCache, plan_cache
@@ -28,6 +28,7 @@ __all__ = ["maskedmm_csr_forward", "maskedmm_csr_backward", "node_mul_edge_forwa
            "sparse_softmax_forward", "sparse_softmax_backward", "vector_spmm_forward", "vector_spmm_backward"]
 
 _LIB = attn_lib()          # fail at import time if the HIP library is missing
+_SCORE_LIB = score_lib()
 if _native.plan_bytes() != ctypes.sizeof(PlanStruct):
     raise ImportError("bptop was built for another bpt_plan: rebuild with `python -m bpt_amd._build`")
 PlanCache.native = _native
@@ -1236,6 +1237,162 @@ _FORCE_GENERIC = False
 def force_generic_enabled():
     """What set_force_generic last set."""
     return _FORCE_GENERIC
+
+
+
+# ---- fused attention with capped scores and distance (no counterpart in the reference) --------------------------------------------
+class Score(collections.namedtuple("Score", "cap slopes pos_q pos_k")):
+    """The score options of a call: cap (0.0: none), slopes (h,) float32 or None, positions of the query and of the key rows, float32."""
+    __slots__ = ()
+
+
+def score_options(score_cap, slopes, pos, q, k):
+    """Score of bpt_attention's arguments, checked, or None where none is given."""
+    if score_cap is None and slopes is None and pos is None:
+        return None
+    cap = 0.0
+    if score_cap is not None:
+        cap = float(score_cap)
+        if not (0.0 < cap <= 3.0e38):
+            raise ValueError("score_cap must be a finite positive number")
+    if (slopes is None) != (pos is None):
+        raise ValueError("slopes and pos go together")
+    if slopes is None:
+        return Score(cap, None, None, None)
+    pos_q, pos_k = pos if isinstance(pos, (tuple, list)) else (pos, pos)
+    for t, n, name in ((slopes, _hd(q)[0], "slopes"), (pos_q, q.size(0), "pos (of the query rows)"), (pos_k, k.size(0), "pos (of the key rows)")):
+        _check_input(t, name)
+        if t.dtype != torch.float32:
+            raise RuntimeError(f"{name} must be float32")
+        if t.device != q.device:
+            raise ValueError("all tensors of a call must be on one device")
+        _expect_shape(t, (n,), name)
+    if pos_q.requires_grad or pos_k.requires_grad:
+        raise ValueError("pos has no gradient: pass it detached")
+    return Score(cap, slopes, pos_q, pos_k)
+
+
+def score_padded_shape(q):
+    """(h', 64): the heads that the fused kernels with score options run q's (h, d, dtype) as (equal to (h, d): as it is), else None."""
+    if q.dim() != 3 or q.dtype not in (torch.float32, torch.bfloat16) or q.size(2) > 64:
+        return None
+    heads = [n for n in ((4, 8, 16) if q.dtype == torch.float32 else (8, 16)) if n >= q.size(1)]
+    return (heads[0], 64) if heads and q.size(1) > 0 and q.size(2) > 0 else None
+
+
+def score_supported(eid_c, q, k):
+    """Whether the fused kernels with score options may run a call on q's padded shape: they are tile kernels."""
+    cfg, shape = _SETTINGS, score_padded_shape(q)
+    return (shape is not None and not _FORCE_GENERIC and cfg.use_groups and _tiles(q, *shape, None, 0.0, None, cfg) and TILE_BACKWARD is not False
+            and eid_c.numel() > 0 and q.size(0) > 0 and k.size(0) > 0
+            and max(q.size(0), k.size(0)) * shape[0] * 64 * q.element_size() < 2 ** 32)
+
+
+def _score_plan_in(graph, q, k, built=None):
+    col, indptr_c, eid_c, indices_c = graph[4:]
+    return plan_cache.get(col, indptr_c, eid_c, indices_c, q.size(0), k.size(0), seg_len=_tile_seg_of(eid_c.size(0), q.size(0), k.size(0)),
+                          prefer_device=True, groups=(TILE_ROWS, None), built=built)
+
+
+def _score_plan_out(graph, q, k, built=None):
+    row, indptr_r, eid_r, indices_r = graph[:4]
+    return plan_cache.get(row, indptr_r, eid_r, indices_r, k.size(0), q.size(0), seg_len=_tile_seg_of(eid_r.size(0), q.size(0), k.size(0)),
+                          prefer_device=True, groups=(TILE_ROWS, _plan.tile_order_src(k.size(0), eid_r.size(0))), built=built)
+
+
+def _score_linked(pi, po, k):
+    return po.linked_to(pi, TILE_ROWS, order=_plan.tile_order_src(k.size(0), po.n_edges), partner_order=None, pair_numbers=True)
+
+
+def score_covers(graph, q, k, train):
+    """Whether the plans of a call whose shape score_supported() takes cover every edge (they are built here where they are new, both
+    sides' together for a call with a backward), as the tile kernels need."""
+    plans = (None, None)
+    if train:
+        seg = _tile_seg_of(graph[6].size(0), q.size(0), k.size(0))
+        sides = [(*graph[4:], q.size(0), k.size(0), seg, None), (*graph[:4], k.size(0), q.size(0), seg, _plan.tile_order_src(k.size(0), graph[2].size(0)))]
+        if all(t.dim() == 1 and t.dtype == torch.int64 and t.is_contiguous() and t.device == q.device for t in graph):
+            plans = plan_cache.put_tile_plans(sides) or plans
+    pi = _score_plan_in(graph, q, k, plans[0])
+    return pi.covers_all_edges and (not train or _score_plan_out(graph, q, k, plans[1]).covers_all_edges)
+
+
+def _score_struct(score):
+    return ctypes.byref(ScoreStruct(score.cap, *(None if t is None else t.data_ptr() for t in score[1:])))
+
+
+def _check_score_call(graph, q, k, v, score, bias):
+    _check_all(col=graph[4], indptr_c=graph[5], eid_c=graph[6], indices_c=graph[7], q=q, k=k, v=v)
+    _same_dtype(q, k, v)
+    h, d = _hd(q)
+    if score_padded_shape(q) != (h, d):
+        raise RuntimeError("attention with score options has no fused kernel for this shape and type")
+    _expect_index(graph[6], graph[7])
+    _expect_shape(k, (k.size(0),) + tuple(q.shape[1:]), "k")
+    _expect_shape(v, k.shape, "v")
+    _check_bias(bias, graph[6].size(0), h, q.device, _SETTINGS)
+    if score.slopes is not None:
+        for t, n, name in ((score.slopes, h, "slopes"), (score.pos_q, q.size(0), "pos_q"), (score.pos_k, k.size(0), "pos_k")):
+            _check_input(t, name)
+            if t.dtype != torch.float32 or t.device != q.device:
+                raise ValueError(f"{name} must be float32 on {q.device}")
+            _expect_shape(t, (n,), name)
+    return h
+
+
+def score_attention_forward(col, indptr_c, eid_c, indices_c, q, k, v, score, scale=None, dropout_p=0.0, seed=0, bias=None):
+    """(o, lse) as attention_forward's, of scores u = (q[dst].k[src] + bias[e]) scale that become score.cap tanh(u / score.cap) -
+    score.slopes[head] |pos_q[dst] - pos_k[src]| (a Score).  Shapes that score_padded_shape() leaves as they are; bias by edge id."""
+    graph = (None,) * 4 + (col, indptr_c, eid_c, indices_c)
+    h = _check_score_call(graph, q, k, v, score, bias)
+    scale = 1.0 / math.sqrt(q.size(2)) if scale is None else float(scale)
+    plan = _score_plan_in(graph, q, k)
+    if not plan.covers_all_edges:
+        raise RuntimeError("attention with score options needs units that cover every edge")
+    ref = ctypes.byref(plan.ensure_groups(TILE_ROWS)["struct"])
+    o = torch.empty_like(q)
+    lse = torch.empty((q.size(0), h), dtype=torch.float32, device=q.device)
+    nws = _SCORE_LIB.bpt_score_forward_workspace_bytes(ref, h)
+    ws = torch.empty(nws, dtype=torch.uint8, device=q.device) if nws else None
+    with _on_device_of(q):
+        check_attn(_SCORE_LIB.bpt_score_forward(ref, _score_struct(score), _ptr(q), _ptr(k), _ptr(v), _ptr(bias), _ptr(o), _ptr(lse), _ptr(ws), nws, scale,
+                                                float(dropout_p), int(seed) & (2 ** 64 - 1), h, _dtype(q), _stream()), "score_attention_forward")
+    return o, lse
+
+
+def score_attention_backward(row, indptr_r, eid_r, indices_r, col, indptr_c, eid_c, indices_c, q, k, v, o, lse, do, score, scale=None, dropout_p=0.0,
+                             seed=0, bias=None, need_slopes=True):
+    """(dq, dk, dv, dslopes, ds) of score_attention_forward: dslopes (h,) float32, None without slopes or need_slopes; ds as
+    attention_backward's with bias, the gradient of q.k + bias per edge and head by edge id, None without."""
+    graph = (row, indptr_r, eid_r, indices_r, col, indptr_c, eid_c, indices_c)
+    h = _check_score_call(graph, q, k, v, score, bias)
+    do = do.contiguous()
+    if do.data_ptr() % 16:
+        do = do.clone()
+    _check_all(row=row, indptr_r=indptr_r, eid_r=eid_r, indices_r=indices_r, o=o, lse=lse, do=do)
+    _same_dtype(q, o, do)
+    _expect_index(eid_r, indices_r)
+    _expect_shape(eid_r, eid_c.shape, "eid_r")
+    _expect_shape(o, q.shape, "o")
+    _expect_shape(do, q.shape, "do")
+    if lse.dtype != torch.float32 or lse.device != q.device:
+        raise ValueError("lse must be the float32 tensor that score_attention_forward returned")
+    _expect_shape(lse, (q.size(0), h), "lse")
+    scale = 1.0 / math.sqrt(q.size(2)) if scale is None else float(scale)
+    pi, po = _score_plan_in(graph, q, k), _score_plan_out(graph, q, k)
+    if not (pi.covers_all_edges and po.covers_all_edges):
+        raise RuntimeError("attention with score options needs units that cover every edge")
+    in_ref, out_ref = ctypes.byref(pi.ensure_groups(TILE_ROWS)["struct"]), ctypes.byref(_score_linked(pi, po, k))
+    dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+    ds = torch.empty((eid_c.size(0) + 1, h), dtype=torch.float32, device=q.device) if bias is not None else None
+    dslopes = torch.empty_like(score.slopes) if score.slopes is not None and need_slopes else None
+    nws = _SCORE_LIB.bpt_score_backward_workspace_bytes(in_ref, out_ref, h, _dtype(q), int(bias is not None))
+    ws = torch.empty(nws, dtype=torch.uint8, device=q.device)
+    with _on_device_of(q):
+        check_attn(_SCORE_LIB.bpt_score_backward(in_ref, out_ref, _score_struct(score), _ptr(q), _ptr(k), _ptr(v), _ptr(bias), _ptr(o), _ptr(do), _ptr(lse),
+                                                 _ptr(dq), _ptr(dk), _ptr(dv), _ptr(ds), _ptr(dslopes), _ptr(ws), nws, scale, float(dropout_p),
+                                                 int(seed) & (2 ** 64 - 1), h, _dtype(q), _stream()), "score_attention_backward")
+    return dq, dk, dv, dslopes, None if ds is None else ds[:-1]
 
 
 # ---- relu kept in 8 bits (bpt_amd/csrc/bptblock.hip; no counterpart in the reference) ---------------------------------------------

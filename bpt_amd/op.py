@@ -12,7 +12,7 @@ from ._native import native as _native
 from .graphop import (maskedmm_csr_backward, maskedmm_csr_forward, node_mul_edge_backward, node_mul_edge_forward,
                       sparse_softmax_backward, sparse_softmax_forward, vector_spmm_backward, vector_spmm_forward)
 
-__all__ = ["SparseSoftmax", "MaskedMMCSR", "NodeMulEdge", "VectorSPMM", "BPTAttention", "EdgeTypeEmbedding",
+__all__ = ["SparseSoftmax", "MaskedMMCSR", "NodeMulEdge", "VectorSPMM", "BPTAttention", "BPTScoreAttention", "EdgeTypeEmbedding",
            "sparse_softmax", "masked_mm", "node_mul_edge", "vec_spmm", "bpt_attention", "edge_type_embedding",
            "add_layer_norm", "relu_linear8"]
 
@@ -106,8 +106,9 @@ class BPTRelAttention(Function):
 
     @staticmethod
     def forward(ctx, row, indptr_r, eid_r, indices_r, col, indptr_c, eid_c, indices_c, q, k, v, scale, dropout_p, seed,
-                table, etype, on_tiles=None, train=False):
-        """on_tiles: None or, outside of stream capture, a list, which receives the term's index tensors (_rel_aux, and those in the order of the
+                table, etype, on_tiles=None, train=False, score=None, slopes=None):
+        """score: None or the score options (graphop.Score; slopes: its slopes once more, for their gradient): the term then goes by edge id.
+        on_tiles: None or, outside of stream capture, a list, which receives the term's index tensors (_rel_aux, and those in the order of the
         tiles) and, for a call that is going to have a backward (train), both passes' plans, where the term is formed over the tiles."""
         aux = _rel_aux(etype, col, indptr_c, eid_c, table.size(0))
         table = table.contiguous()
@@ -117,7 +118,7 @@ class BPTRelAttention(Function):
         # where forward and backward both run on the tile kernels, the term and its gradient are stored head-major in the
         # order in which the tiles meet the edges (rows_slot: the place of every in-CSR slot) instead of by edge id
         graph = (row, indptr_r, eid_r, indices_r, col, indptr_c, eid_c, indices_c, q, k)
-        order = _g.attention_pair_order(*graph, dropout_p) if ctx.on_chip else None
+        order = _g.attention_pair_order(*graph, dropout_p) if ctx.on_chip and score is None else None
         ctx.rows_slot = None
         if order is not None:
             pair = order[1]["pair_of_eid"]
@@ -149,22 +150,32 @@ class BPTRelAttention(Function):
             bias = _g.rel_bias_forward(col, indptr_c, eid_c, aux["number_slot"], q, table, used_types=aux["used_types"])
         else:
             bias = _g.rel_bias_forward(col, indptr_c, eid_c, aux["etype_slot"], q, table)
-        o, lse = _g.attention_forward(col, indptr_c, eid_c, indices_c, q, k, v, scale, dropout_p, seed, bias=bias,
-                                      bias_by_pair=ctx.rows_slot is not None)
-        ctx.save_for_backward(row, indptr_r, eid_r, indices_r, col, indptr_c, eid_c, indices_c, q, k, v, o, lse, bias, table)
+        if score is not None:
+            o, lse = _g.score_attention_forward(col, indptr_c, eid_c, indices_c, q, k, v, score, scale, dropout_p, seed, bias)
+        else:
+            o, lse = _g.attention_forward(col, indptr_c, eid_c, indices_c, q, k, v, scale, dropout_p, seed, bias=bias,
+                                          bias_by_pair=ctx.rows_slot is not None)
+        ctx.save_for_backward(row, indptr_r, eid_r, indices_r, col, indptr_c, eid_c, indices_c, q, k, v, o, lse, bias, table,
+                              *(() if score is None else score[1:]))
+        ctx.cap = None if score is None else score.cap
         ctx.scale, ctx.dropout_p, ctx.seed, ctx.aux, ctx.etype = scale, dropout_p, seed, aux, etype
         return o
 
     @staticmethod
     def backward(ctx, do):
-        row, indptr_r, eid_r, indices_r, col, indptr_c, eid_c, indices_c, q, k, v, o, lse, bias, table = ctx.saved_tensors
-        aux = ctx.aux
+        row, indptr_r, eid_r, indices_r, col, indptr_c, eid_c, indices_c, q, k, v, o, lse, bias, table = ctx.saved_tensors[:15]
+        aux, dslopes = ctx.aux, None
         if ctx.rows_slot is not None:
             dq, dk, dv, dtable = _rel_backward(*ctx.saved_tensors, do, ctx.scale, ctx.dropout_p, ctx.seed, ctx.rows_slot, aux["number_slot"],
                                                aux["used"], aux["used_types"])
-            return None, None, None, None, None, None, None, None, dq, dk, dv, None, None, None, dtable, None, None, None
-        dq, dk, dv, ds = _g.attention_backward(row, indptr_r, eid_r, indices_r, col, indptr_c, eid_c, indices_c,
-                                               q, k, v, o, lse, do, ctx.scale, ctx.dropout_p, ctx.seed, bias=bias)
+            return None, None, None, None, None, None, None, None, dq, dk, dv, None, None, None, dtable, None, None, None, None, None
+        if ctx.cap is not None:
+            dq, dk, dv, dslopes, ds = _g.score_attention_backward(row, indptr_r, eid_r, indices_r, col, indptr_c, eid_c, indices_c, q, k, v, o, lse, do,
+                                                                  _g.Score(ctx.cap, *ctx.saved_tensors[15:]), ctx.scale, ctx.dropout_p, ctx.seed, bias,
+                                                                  ctx.needs_input_grad[19])
+        else:
+            dq, dk, dv, ds = _g.attention_backward(row, indptr_r, eid_r, indices_r, col, indptr_c, eid_c, indices_c,
+                                                   q, k, v, o, lse, do, ctx.scale, ctx.dropout_p, ctx.seed, bias=bias)
         if ctx.on_chip:
             dtable = _g.rel_bias_backward(col, indptr_c, eid_c, aux["number_slot"], aux["used"], aux["used_types"], ds, q, table, dq)
         else:
@@ -175,7 +186,27 @@ class BPTRelAttention(Function):
             dq = vector_spmm_forward(col, indptr_c, eid_c, aux["etype_slot"], ds, table_h, n_rows=q.size(0), out=dq)
             dtable = vector_spmm_forward(t_row, t_indptr, t_order, t_dst, ds, q, n_rows=table.size(0))
             dtable = dtable.float().sum(1).to(table.dtype)
-        return None, None, None, None, None, None, None, None, dq, dk, dv, None, None, None, dtable, None, None, None
+        return None, None, None, None, None, None, None, None, dq, dk, dv, None, None, None, dtable, None, None, None, None, dslopes
+
+
+class BPTScoreAttention(Function):
+    """BPTAttention with score options (graphop.Score): u = q.k scale becomes cap tanh(u / cap) - slopes[head] |pos[dst] - pos[src]|.  Saves what
+    BPTAttention does; slopes (the options' own, once more) get their gradient."""
+
+    @staticmethod
+    def forward(ctx, row, indptr_r, eid_r, indices_r, col, indptr_c, eid_c, indices_c, q, k, v, slopes, score, scale, dropout_p, seed):
+        o, lse = _g.score_attention_forward(col, indptr_c, eid_c, indices_c, q, k, v, score, scale, dropout_p, seed)
+        ctx.save_for_backward(row, indptr_r, eid_r, indices_r, col, indptr_c, eid_c, indices_c, q, k, v, o, lse, *score[1:])
+        ctx.cap, ctx.scale, ctx.dropout_p, ctx.seed = score.cap, scale, dropout_p, seed
+        return o
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, do):
+        tensors = ctx.saved_tensors
+        dq, dk, dv, dslopes, _ = _g.score_attention_backward(*tensors[:13], do, _g.Score(ctx.cap, *tensors[13:]), ctx.scale, ctx.dropout_p, ctx.seed,
+                                                             need_slopes=ctx.needs_input_grad[11])
+        return None, None, None, None, None, None, None, None, dq, dk, dv, dslopes, None, None, None, None
 
 
 def _rel_backward(row, indptr_r, eid_r, indices_r, col, indptr_c, eid_c, indices_c, q, k, v, o, lse, bias, table, do, scale, dropout_p, seed, rows_slot,
@@ -362,8 +393,68 @@ def _served_natively(graph):
     return graph[0] is not None and graph[1] is not None and graph[2] is not None and graph[3] is not None and not torch.jit.is_tracing()
 
 
+def _edge_distance(score, col, indptr_c, eid_c, indices_c):
+    """|pos_q[dst] - pos_k[src]| by edge id (0 for edges that no unit covers)."""
+    dst = torch.repeat_interleave(col, indptr_c[1:] - indptr_c[:-1])
+    slots = torch.arange(dst.numel(), device=dst.device) + indptr_c[0]
+    far = (score.pos_q.index_select(0, dst) - score.pos_k.index_select(0, indices_c.index_select(0, slots))).abs()
+    return torch.zeros(eid_c.numel(), dtype=far.dtype, device=far.device).index_copy(0, eid_c.index_select(0, slots), far)
+
+
+def _score_chain(graph, q, k, v, scale, dropout_p, rel_table, etype, score):
+    """Attention with score options as the chain of separate operators, for shapes and types without a fused kernel: the (E, h) scores are
+    capped and lowered in 32 bits (64 for float64)."""
+    row, indptr_r, eid_r, indices_r, col, indptr_c, eid_c, indices_c = graph
+    e = masked_mm(*graph, k, q)
+    if rel_table is not None:
+        e = e + node_mul_edge(col, indptr_c, eid_c, q, edge_type_embedding(rel_table, etype))
+    e = (e if e.dtype == torch.float64 else e.float()) * scale
+    if score.cap:
+        e = score.cap * torch.tanh(e / score.cap)
+    if score.slopes is not None:
+        far = _edge_distance(score, col, indptr_c, eid_c, indices_c).to(e.dtype)
+        e = e - (score.slopes.to(e.dtype) * far[:, None] if e.dim() == 2 else score.slopes.to(e.dtype) * far)
+    a = torch.nn.functional.dropout(sparse_softmax(col, indptr_c, eid_c, e.contiguous()), p=float(dropout_p), training=dropout_p > 0)
+    return vec_spmm(col, indptr_c, eid_c, indices_c, row, indptr_r, eid_r, indices_r, a.to(v.dtype), v, n_rows=None if q.size(0) == v.size(0) else q.size(0))
+
+
+def _score_attention(graph, q, k, v, scale, fused, dropout_p, seed, rel_table, etype, score):
+    """bpt_attention with score options."""
+    train = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, rel_table, score.slopes))
+    runs = fused is not False and _native_takes() and _g.score_supported(graph[6], q, k) and (not train or all(t is not None for t in graph[:4]))
+    if not runs:
+        if fused:
+            raise RuntimeError("attention with score options has no fused kernel for this call")
+        return _score_chain(graph, q, k, v, scale, dropout_p, rel_table, etype, score)
+    if dropout_p > 0 and seed is None:
+        seed = int(torch.randint(0, 2 ** 62, (1,)).item())
+    seed = int(seed or 0)
+    h, d = q.size(1), q.size(2)
+    hp, dp = _g.score_padded_shape(q)
+    on16 = lambda x: x.clone() if x.data_ptr() % 16 else x          # (the tile kernels read 16 bytes a lane)
+    if (hp, dp) != (h, d):
+        # as the narrow heads of the plain layer with relative positions: zero columns and heads add nothing
+        q, k, v = (torch.nn.functional.pad(x, (0, dp - d, 0, hp - h)) for x in (q, k, v))
+        rel_table = None if rel_table is None else torch.nn.functional.pad(rel_table, (0, dp - d))
+        if score.slopes is not None:
+            score = score._replace(slopes=torch.nn.functional.pad(score.slopes, (0, hp - h)))
+    else:
+        q, k, v = on16(q), on16(k), on16(v)
+    if not _g.score_covers(graph, q, k, train):
+        if fused:
+            raise RuntimeError("attention with score options needs units that cover every edge")
+        return _score_chain(graph, q[:, :h, :d].contiguous(), k[:, :h, :d].contiguous(), v[:, :h, :d].contiguous(), scale, dropout_p,
+                            None if rel_table is None else rel_table[:, :d].contiguous(), etype,
+                            score if score.slopes is None else score._replace(slopes=score.slopes[:h].contiguous()))
+    if rel_table is not None:
+        o = BPTRelAttention.apply(*graph, q, k, v, scale, float(dropout_p), seed, rel_table, etype, None, False, score, score.slopes)
+    else:
+        o = BPTScoreAttention.apply(*graph, q, k, v, score.slopes, score, scale, float(dropout_p), seed)
+    return o if (hp, dp) == (h, d) else o[:, :h, :d].contiguous()
+
+
 def bpt_attention(row, indptr_r, eid_r, indices_r, col, indptr_c, eid_c, indices_c, q, k, v, scale=None, fused=None,
-                  dropout_p=0.0, seed=None, rel_table=None, etype=None):
+                  dropout_p=0.0, seed=None, rel_table=None, etype=None, score_cap=None, slopes=None, pos=None):
     """Attention over the graph: (ROW, INDPTR_R, out_eid, out_idx) is the out-CSR side (rows =
     sources), (COL, INDPTR_C, in_eid, in_idx) the in-CSR side (rows = destinations), exactly the
     eight graph arguments modules/attention.py:66-67 passes to masked_mm.
@@ -376,10 +467,21 @@ def bpt_attention(row, indptr_r, eid_r, indices_r, col, indptr_c, eid_c, indices
     unfused path uses torch's dropout, so the two paths drop different elements.
 
     rel_table (n_types, d) and etype (E,) int64 add the rel_pos term q[dst] . rel_table[etype[e]] to the score of
-    edge e (attention.py:69-71); the gradient of rel_table is returned like any other."""
+    edge e (attention.py:69-71); the gradient of rel_table is returned like any other.
+
+    Score options (not in the reference): with u the scaled score, term included,
+    score_cap c > 0 makes it c tanh(u / c), which bounds it by c;
+    slopes (h,) float32 and pos, float32 positions of the rows (one tensor, or a pair (of the query rows, of the key rows)), lower it by
+    slopes[head] * |pos[dst] - pos[src]| behind the cap.  slopes get a gradient, pos does not.  Heads of up to 64 columns, 16 of them,
+    in float32 and bfloat16 run fused (narrow ones on padded copies), other shapes and float64 through the chain.  Edges are the
+    graph's: documents that must not see each other are its separate components."""
     scale = 1.0 / math.sqrt(q.size(-1)) if scale is None else float(scale)
     if (rel_table is None) != (etype is None):
         raise ValueError("rel_table and etype go together")
+    score = _g.score_options(score_cap, slopes, pos, q, k)
+    if score is not None:
+        return _score_attention((row, indptr_r, eid_r, indices_r, col, indptr_c, eid_c, indices_c), q, k, v, scale, fused, dropout_p, seed, rel_table, etype,
+                                score)
     padded = None
     if fused is None:
         fused = _g.attention_supported(q)

@@ -118,7 +118,7 @@ BUILD_API = {
 }
 
 _PS = ctypes.POINTER(ScoreStruct)
-_score_tail = [ctypes.c_float, ctypes.c_float, ctypes.c_uint64, ctypes.c_int, ctypes.c_int, c_vp]      # scale, dropout_p, seed, h, dtype, stream
+_score_tail = [ctypes.c_float, ctypes.c_float, ctypes.c_uint64] + [ctypes.c_int] * 4 + [c_vp]      # scale, dropout_p, seed, heads, d, h, dtype, stream
 # libbptscore (include/bptscore.h): attention with capped scores and distance
 SCORE_API = {
     "bpt_score_forward_workspace_bytes": (c_i64, [_PP, ctypes.c_int]),

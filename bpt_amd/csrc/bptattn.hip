@@ -3725,12 +3725,6 @@ inline bool has_groups(const bpt_plan *P, int h, int d, size_t elem) {
            fits32((P->n_grp_entries + GRP_PAD_ENTRIES) * P->grp_R, (int64_t)h * 8);
 }
 
-// a tile in parts: one head a workgroup, so that no wavefront of it lies past the last head
-inline Narrow narrow_parts(Narrow nw, int parts) {
-    if (parts > 1) nw.slices = nw.heads;
-    return nw;
-}
-
 // The separate operators on tiles: float32, groups of 16 rows with their edge ids.  Heads of 64 columns, 4, 8 or 16 of them, whose rows
 // lie on 16 bytes, take the kernels of those shapes, all others of 4 to 64 columns the narrow ones (rows on 4 bytes).
 bool product_tiles_ok(const bpt_plan *P, int h, int d, int dtype) {

@@ -29,13 +29,14 @@
 #include "../../include/bptattn.h"
 #include "../../include/bptbuild.h"
 #include "../../include/bptplan.h"
+#include "../../include/bptscore.h"
 
 namespace py = pybind11;
 using at::Tensor;
 
 namespace {
 
-enum Kind { ATTN_FWD = 0, ATTN_BWD = 1, ATTN_FWD_NARROW = 2, ATTN_BWD_NARROW = 3, MM_FWD = 4, MM_BWD = 5, SPMM_FWD = 6, SPMM_BWD = 7, SOFTMAX = 8, REL_FWD = 9, REL_TRAIN = 10 };
+enum Kind { ATTN_FWD = 0, ATTN_BWD = 1, ATTN_FWD_NARROW = 2, ATTN_BWD_NARROW = 3, MM_FWD = 4, MM_BWD = 5, SPMM_FWD = 6, SPMM_BWD = 7, SOFTMAX = 8, REL_FWD = 9, REL_TRAIN = 10, SCORE_FWD = 11, SCORE_TRAIN = 12 };
 
 constexpr size_t MAX_TENSORS = 9, MAX_EXTRA = 7, MAX_ENTRIES = 512;
 
@@ -521,6 +522,133 @@ std::optional<Tensor> rel_attention(const Tensor &row, const Tensor &indptr_r, c
     if (!r) return std::nullopt;
     if (!train) return std::get<0>(*r);
     return RelAttention::apply(row, indptr_r, eid_r, indices_r, col, indptr_c, eid_c, indices_c, q, k, v, table, e, *r, scale, p, (int64_t)seed);
+}
+
+// ---- fused attention with capped scores and distance (op.BPTScoreAttention), h: the heads it is computed as ----------------------
+using MaybeTensor = std::optional<Tensor>;
+
+struct ScoreOptions {
+    double cap;
+    Tensor slopes, pos_q, pos_k;      // undefined: no distance
+    bpt_score pack() const {
+        auto at = [](const Tensor &t) { return t.defined() ? t.data_ptr<float>() : nullptr; };
+        return bpt_score{(float)cap, at(slopes), at(pos_q), at(pos_k)};
+    }
+};
+
+bool score_options(const ScoreOptions &o, const Tensor &q, const Tensor &k) {
+    if (!(o.cap >= 0.0)) return false;
+    if (!o.slopes.defined()) return !o.pos_q.defined() && !o.pos_k.defined();
+    auto ok = [&](const Tensor &t, int64_t n) {
+        return t.defined() && t.scalar_type() == at::kFloat && t.device() == q.device() && t.is_contiguous() && t.dim() == 1 && t.size(0) == n;
+    };
+    return ok(o.slopes, q.size(1)) && ok(o.pos_q, q.size(0)) && ok(o.pos_k, k.size(0));
+}
+
+EntryPtr score_entry(Kind kind, const std::vector<const Tensor *> &graph, const Tensor &q, const Tensor &k, const Tensor &v, double p, int64_t h) {
+    Shape s;
+    for (const Tensor *t : graph)
+        if (!t->defined()) return nullptr;
+    if (!attention_shape(q, k, v, p, s)) return nullptr;
+    for (size_t i = 2; i < graph.size(); i += 4)
+        if (graph[i]->sizes() != graph[i + 1]->sizes() || graph[i]->sizes() != graph[2]->sizes()) return nullptr;
+    Key key;
+    if (!make_key(key, kind, graph, q.device(), {s.nq, s.nk, h, s.d, s.dt, p > 0.0, s.h})) return nullptr;
+    return find(key);
+}
+
+std::optional<std::tuple<Tensor, Tensor>> score_forward_known(const EntryPtr &e, const Tensor &q, const Tensor &k, const Tensor &v, const ScoreOptions &opt,
+                                                              double scale, double p, uint64_t seed, int h) {
+    c10::DeviceGuard guard(q.device());
+    Tensor o = at::empty_like(q), lse = at::empty({q.size(0), h}, q.options().dtype(at::kFloat)), ws;
+    const int64_t bytes = bpt_score_forward_workspace_bytes(&e->a, h);
+    if (bytes > 0) ws = at::empty({bytes}, q.options().dtype(at::kByte));
+    const bpt_score score = opt.pack();
+    if (bpt_score_forward(&e->a, &score, q.data_ptr(), k.data_ptr(), v.data_ptr(), nullptr, o.data_ptr(), lse.data_ptr<float>(), bytes > 0 ? ws.data_ptr() : nullptr,
+                          bytes, (float)scale, (float)p, seed, (int)q.size(1), (int)q.size(2), h, dtype_code(q.scalar_type()), stream_of(q.device())) != BPT_OK)
+        return std::nullopt;
+    return std::make_tuple(o, lse);
+}
+
+std::optional<std::array<Tensor, 4>> score_backward_known(const EntryPtr &e, const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &o, const Tensor &lse,
+                                                          const Tensor &d_o, const ScoreOptions &opt, double scale, double p, uint64_t seed, int h, bool need_slopes) {
+    // (the entry was found for the forward's tensors; a hook on saved tensors may give back others)
+    Shape s;
+    if (!attention_shape(q, k, v, p, s) || !like(o, q) || !like(d_o, q) || o.sizes() != q.sizes() || d_o.sizes() != q.sizes()) return std::nullopt;
+    if (s.nq != e->a.n_rows || s.nk != e->b.n_rows || !float_matrix(lse, q.device(), s.nq, h) || !score_options(opt, q, k)) return std::nullopt;
+    c10::DeviceGuard guard(q.device());
+    Tensor dq = at::empty_like(q), dk = at::empty_like(k), dv = at::empty_like(v), dslopes;
+    if (opt.slopes.defined() && need_slopes) dslopes = at::empty_like(opt.slopes);
+    const int64_t bytes = bpt_score_backward_workspace_bytes(&e->a, &e->b, h, s.dt, 0);
+    const Tensor ws = at::empty({std::max<int64_t>(bytes, 16)}, q.options().dtype(at::kByte));
+    const bpt_score score = opt.pack();
+    if (bpt_score_backward(&e->a, &e->b, &score, q.data_ptr(), k.data_ptr(), v.data_ptr(), nullptr, o.data_ptr(), d_o.data_ptr(), lse.data_ptr<float>(),
+                           dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), nullptr, dslopes.defined() ? dslopes.data_ptr<float>() : nullptr, ws.data_ptr(), bytes,
+                           (float)scale, (float)p, seed, s.h, s.d, h, s.dt, stream_of(q.device())) != BPT_OK)
+        return std::nullopt;
+    return std::array<Tensor, 4>{dq, dk, dv, dslopes};
+}
+
+// (o, lse: what the forward has computed already: a call that the library refuses never becomes a node)
+struct ScoreAttention : torch::autograd::Function<ScoreAttention> {
+    static Tensor forward(torch::autograd::AutogradContext *ctx, const Tensor &row, const Tensor &indptr_r, const Tensor &eid_r, const Tensor &indices_r,
+                          const Tensor &col, const Tensor &indptr_c, const Tensor &eid_c, const Tensor &indices_c, const Tensor &q, const Tensor &k,
+                          const Tensor &v, const MaybeTensor &slopes, const ScoreOptions &opt, const EntryPtr &e, const std::tuple<Tensor, Tensor> &r,
+                          double scale, double p, int64_t seed, int64_t h) {
+        const auto &[o, lse] = r;
+        ctx->save_for_backward({row, indptr_r, eid_r, indices_r, col, indptr_c, eid_c, indices_c, q, k, v, o, lse, opt.slopes, opt.pos_q, opt.pos_k});
+        ctx->saved_data["entry"] = c10::IValue::make_capsule(c10::make_intrusive<RelHold>(e));
+        ctx->saved_data["cap"] = opt.cap;
+        ctx->saved_data["scale"] = scale;
+        ctx->saved_data["p"] = p;
+        ctx->saved_data["seed"] = seed;
+        ctx->saved_data["h"] = h;
+        return o;
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
+        TORCH_CHECK(!at::GradMode::is_enabled(), "attention with score options is not differentiable twice");
+        const auto t = ctx->get_saved_variables();
+        const double scale = ctx->saved_data["scale"].toDouble(), p = ctx->saved_data["p"].toDouble();
+        const uint64_t seed = (uint64_t)ctx->saved_data["seed"].toInt();
+        const int h = (int)ctx->saved_data["h"].toInt();
+        const EntryPtr e = c10::static_intrusive_pointer_cast<RelHold>(ctx->saved_data["entry"].toCapsule())->e;
+        const ScoreOptions opt{ctx->saved_data["cap"].toDouble(), t[13], t[14], t[15]};
+        const bool need_slopes = opt.slopes.defined() && ctx->needs_input_grad(11);
+        Tensor d_o = grads[0].contiguous();
+        if (reinterpret_cast<uintptr_t>(d_o.data_ptr()) & 15) d_o = d_o.clone();
+        auto r = score_backward_known(e, t[8], t[9], t[10], t[11], t[12], d_o, opt, scale, p, seed, h, need_slopes);
+        if (!r)
+            r = with_python([&] {
+                auto maybe = [](const Tensor &x) { return x.defined() ? py::cast(x) : py::none().cast<py::object>(); };
+                const py::object score = python("Score")(opt.cap, maybe(opt.slopes), maybe(opt.pos_q), maybe(opt.pos_k));
+                const py::tuple five = python("score_attention_backward")(t[0], t[1], t[2], t[3], t[4], t[5], t[6], t[7], t[8], t[9], t[10], t[11], t[12], d_o, score,
+                                                                          scale, p, seed, py::none(), need_slopes);
+                std::array<Tensor, 4> out;
+                for (size_t i = 0; i < 4; ++i)
+                    if (!five[i].is_none()) out[i] = five[i].cast<Tensor>();
+                return out;
+            });
+        torch::autograd::variable_list out(19);
+        for (int i = 0; i < 4; ++i) out[8 + i] = (*r)[i];
+        return out;
+    }
+};
+
+// op.BPTScoreAttention of a call whose plans are known, or None
+MaybeTensor score_attention(const MaybeTensor &row, const MaybeTensor &indptr_r, const MaybeTensor &eid_r, const MaybeTensor &indices_r, const Tensor &col,
+                            const Tensor &indptr_c, const Tensor &eid_c, const Tensor &indices_c, const Tensor &q, const Tensor &k, const Tensor &v,
+                            const MaybeTensor &slopes, const MaybeTensor &pos_q, const MaybeTensor &pos_k, double cap, double scale, double p, uint64_t seed,
+                            int64_t h) {
+    const ScoreOptions opt{cap, slopes.value_or(Tensor()), pos_q.value_or(Tensor()), pos_k.value_or(Tensor())};
+    const Tensor none, &r0 = row ? *row : none, &r1 = indptr_r ? *indptr_r : none, &r2 = eid_r ? *eid_r : none, &r3 = indices_r ? *indices_r : none;
+    const bool train = differentiated({&q, &k, &v}) || (opt.slopes.defined() && differentiated({&opt.slopes}));
+    const EntryPtr e = train ? score_entry(SCORE_TRAIN, {&col, &indptr_c, &eid_c, &indices_c, &r0, &r1, &r2, &r3}, q, k, v, p, h)
+                             : score_entry(SCORE_FWD, {&col, &indptr_c, &eid_c, &indices_c}, q, k, v, p, h);
+    if (!e || !score_options(opt, q, k)) return std::nullopt;
+    const auto r = score_forward_known(e, q, k, v, opt, scale, p, seed, (int)h);
+    if (!r) return std::nullopt;
+    if (!train) return std::get<0>(*r);
+    return ScoreAttention::apply(r0, r1, r2, r3, col, indptr_c, eid_c, indices_c, q, k, v, slopes, opt, e, *r, scale, p, (int64_t)seed, h);
 }
 
 // ---- the separate operators (modules/op.py:10-58 of the reference) -----------------------------------------------------------
@@ -1018,6 +1146,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.attr("SOFTMAX") = (int)SOFTMAX;
     m.attr("REL_FWD") = (int)REL_FWD;
     m.attr("REL_TRAIN") = (int)REL_TRAIN;
+    m.attr("SCORE_FWD") = (int)SCORE_FWD;
+    m.attr("SCORE_TRAIN") = (int)SCORE_TRAIN;
     m.def("masked_mm", &masked_mm);
     m.def("sparse_softmax", &sparse_softmax);
     m.def("vec_spmm", &vec_spmm);
@@ -1031,6 +1161,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("build_tile_plans", &build_tile_plans);
     m.def("count_rows", &count_rows);
     m.def("rel_attention", &rel_attention);
+    m.def("score_attention", &score_attention);
     m.def("remember", &remember);
     m.def("remember_rel", &remember_rel);
     m.def("forget", &forget);

@@ -6,9 +6,40 @@
 
 namespace {
 
-// dslopes[head] = -(sum of the tiles' parts), a workgroup a head, in a fixed order; how many tiles there are stands in the plan
+// Split rows, a workgroup each, from the sums of their segments (bfloat16, comment at k_attn_bwd_dst_rows_bf16): delta of the row to the source side,
+// and what the slopes' gradient gains by it, fix[split row][head].
+__global__ __launch_bounds__(BLOCK) void k_score_split(const int32_t *__restrict__ heavy, const float2 *__restrict__ split, float2 *__restrict__ stat,
+                                                       float *__restrict__ fix, int heads) {
+    __shared__ float2 meet[BLOCK];
+    const int row = heavy[3 * blockIdx.x], s0 = heavy[3 * blockIdx.x + 1], ns = heavy[3 * blockIdx.x + 2];
+    const int head = threadIdx.x % heads, lane = threadIdx.x / heads, lanes = BLOCK / heads;      // (8 or 16 heads)
+    float2 x = make_float2(0.f, 0.f);
+    for (int i = lane; i < ns; i += lanes) {
+        const float2 y = split[(size_t)(s0 + i) * heads + head];
+        x.x += y.x;
+        x.y += y.y;
+    }
+    meet[threadIdx.x] = x;
+    for (int o = lanes / 2; o > 0; o >>= 1) {
+        __syncthreads();
+        if (lane < o) {
+            const float2 y = meet[threadIdx.x + o * heads];
+            x.x += y.x;
+            x.y += y.y;
+            meet[threadIdx.x] = x;
+        }
+    }
+    if (lane == 0) {
+        float2 *const at = stat + (size_t)row * heads + head;
+        fix[(size_t)blockIdx.x * heads + head] = (at->y - x.x) * x.y;
+        at->y = x.x;
+    }
+}
+
+// dslopes[head] = -(sum of the tiles' parts and of what split rows gained), a workgroup a head, in a fixed order; how many tiles there are stands in the
+// plan
 __global__ __launch_bounds__(BLOCK) void k_slope_finish(const float *__restrict__ part, const int32_t *__restrict__ n_groups, int heads, int parts,
-                                                        float *__restrict__ dslopes) {
+                                                        const float *__restrict__ fix, int n_fix, float *__restrict__ dslopes) {
     __shared__ double meet[BLOCK];
     const int head = blockIdx.x, n = __builtin_amdgcn_readfirstlane(*n_groups) * parts;
     auto at = [&](int i) { return part[((size_t)(i / parts) * heads + head) * parts + i % parts]; };
@@ -22,6 +53,7 @@ __global__ __launch_bounds__(BLOCK) void k_slope_finish(const float *__restrict_
         for (int u = 0; u < 8; ++u) x += v[u];
     }
     for (; i < n; i += BLOCK) x += at(i);
+    for (i = threadIdx.x; i < n_fix; i += BLOCK) x += fix[(size_t)i * heads + head];
     meet[threadIdx.x] = x;
     for (int o = BLOCK / 2; o > 0; o >>= 1) {
         __syncthreads();
@@ -37,6 +69,7 @@ inline int64_t scratch_bytes(const bpt_plan *Pin, const bpt_plan *Pout, int h, i
 }
 constexpr int MOST_PARTS = 4;
 inline int64_t slope_bytes(const bpt_plan *Pin, int h) { return round16(Pin->n_groups * h * MOST_PARTS * 4); }
+inline int64_t split_bytes(const bpt_plan *Pin, int h) { return round16(Pin->n_slots * h * 8) + round16(Pin->n_heavy * h * 4); }
 
 inline ScoreMod make_mod(const bpt_score *sc, float scale, bool entries_are_keys, float *part) {
     ScoreMod m{};
@@ -101,9 +134,13 @@ int run_backward(const bpt_plan *Pin, const bpt_plan *Pout, const bpt_score *sc,
     at += scratch_bytes(Pin, Pout, H, dtype, biased);
     float *part = dslopes ? (float *)at : nullptr;
     at += slope_bytes(Pin, H);
+    float2 *split = (float2 *)at;
+    float *fix = (float *)(at + round16(Pin->n_slots * H * 8));
+    if (again) at += split_bytes(Pin, H);
     float *ws_dq = (float *)at, *ws_dk = ws_dq + (size_t)Pin->n_slots * H * D, *ws_dv = ws_dk + (size_t)Pout->n_slots * H * D;
     const int parts_in = tile_parts(Pin, H, sizeof(T)), parts_out = tile_parts(Pout, H, sizeof(T));
-    const ScoreMod md = make_mod(sc, scale, true, part);
+    ScoreMod md = make_mod(sc, scale, true, part);
+    md.split = split;
     pick(drop.thr != 0, biased, parts_in, [&](auto dr, auto bi, auto sp) {
         const dim3 grid((unsigned)(group_grid(Pin) * (H * sp() / HW))), block(HW * WAVE);
         if constexpr (sizeof(T) == 4)
@@ -117,6 +154,9 @@ int run_backward(const bpt_plan *Pin, const bpt_plan *Pout, const bpt_score *sc,
     });
     int st = launch_status();
     if (st != BPT_OK) return st;
+    const bool fixed = again && Pin->n_heavy > 0;
+    if (fixed)
+        hipLaunchKernelGGL(k_score_split, dim3((unsigned)Pin->n_heavy), dim3(BLOCK), 0, s, Pin->heavy, (const float2 *)split, (float2 *)scratch, fix, H);
     pick(drop.thr != 0, biased, parts_out, [&](auto dr, auto bi, auto sp) {
         const dim3 grid((unsigned)(group_grid(Pout) * (H * sp() / HW))), block(HW * WAVE);
         if constexpr (sizeof(T) == 4)
@@ -136,21 +176,82 @@ int run_backward(const bpt_plan *Pin, const bpt_plan *Pout, const bpt_score *sc,
         hipLaunchKernelGGL((k_combine_sum3<T>), dim3((unsigned)(Pin->n_heavy + Pout->n_heavy), H * D / (4 * WAVE), 2), dim3(BLOCK), 0, s, Pin->heavy,
                            (int)Pin->n_heavy, (const float *)ws_dq, (T *)dq, Pout->heavy, (const float *)ws_dk, (T *)dk, (T *)dv, H * D,
                            (size_t)Pout->n_slots * H * D, Narrow{});
-    if (dslopes) hipLaunchKernelGGL(k_slope_finish, dim3(H), dim3(BLOCK), 0, s, (const float *)part, Pin->grp_chunks + 8, H, parts_in, dslopes);
+    if (dslopes) hipLaunchKernelGGL(k_slope_finish, dim3(H), dim3(BLOCK), 0, s, (const float *)part, Pin->grp_chunks + 8, H, parts_in,
+                                    (const float *)fix, fixed ? (int)Pin->n_heavy : 0, dslopes);
     return launch_status();
 }
 
-inline int check_score(const bpt_plan *P, const bpt_score *sc, int h, int dtype, float dropout_p, const float *bias) {
+// Heads of fewer than 64 columns in float32, read as they are.  (bfloat16 ones run on padded copies: their kernels hand (p, ds) over in 16 bits each,
+// with delta from O as stored.)
+int run_forward_narrow(const bpt_plan *P, const bpt_score *sc, const float *q, const float *k, const float *v, float *o, float *lse, void *ws, float scale,
+                       Dropout drop, const Narrow &nw, hipStream_t s) {
+    float *ws_acc = (float *)ws, *ws_ml = ws_acc ? ws_acc + (size_t)P->n_slots * nw.h * 64 : nullptr;
+    const ScoreMod md = make_mod(sc, scale, true, nullptr);
+    const int parts = tile_parts(P, nw.heads, 4);
+    const Narrow np = narrow_parts(nw, parts);
+    pick(drop.thr != 0, false, parts, [&](auto dr, auto, auto sp) {
+        constexpr int HW = sp() == 1 ? NARROW_HW : sp();
+        hipLaunchKernelGGL((k_attn_fwd_tile<float, 16, 64, HW, dr(), 0, true, sp(), true>), dim3((unsigned)(group_grid(P) * np.slices)), dim3(HW * WAVE), 0, s, *P,
+                           q, k, v, o, lse, ws_acc, ws_ml, scale * LOG2E, drop.thr, drop.seed, drop.inv, (const float *)nullptr, np, Keep{}, md);
+    });
+    const int st = launch_status();
+    if (st != BPT_OK || P->n_heavy == 0) return st;
+    hipLaunchKernelGGL((k_attn_fwd_combine<float, 16, 64, true>), dim3((unsigned)P->n_heavy, nw.heads), dim3(BLOCK), 0, s, P->heavy, (const float *)ws_acc,
+                       (const float *)ws_ml, o, lse, nw, (float *)nullptr);
+    return launch_status();
+}
+
+int run_backward_narrow(const bpt_plan *Pin, const bpt_plan *Pout, const bpt_score *sc, const float *q, const float *k, const float *v, const float *o,
+                        const float *d_o, const float *lse, float *dq, float *dk, float *dv, float *dslopes, void *ws, float scale, Dropout drop, const Narrow &nw,
+                        hipStream_t s) {
+    char *at = (char *)ws;
+    float2 *scratch = (float2 *)at;
+    at += scratch_bytes(Pin, Pout, nw.h, BPT_F32, false);
+    float *part = dslopes ? (float *)at : nullptr;
+    at += slope_bytes(Pin, nw.h);
+    const int C = nw.h * 64;
+    float *ws_dq = (float *)at, *ws_dk = ws_dq + (size_t)Pin->n_slots * C, *ws_dv = ws_dk + (size_t)Pout->n_slots * C;
+    const int parts = tile_parts(Pin, nw.heads, 4), parts_src = tile_parts(Pout, nw.heads, 4);
+    const Narrow np = narrow_parts(nw, parts), np_src = narrow_parts(nw, parts_src);
+    const ScoreMod md = make_mod(sc, scale, true, part);
+    pick(drop.thr != 0, false, parts, [&](auto dr, auto, auto sp) {
+        constexpr int HW = sp() == 1 ? NARROW_HW : sp();
+        hipLaunchKernelGGL((k_attn_bwd_dst_tile<float, 16, 64, HW, dr(), 0, true, sp(), true>), dim3((unsigned)(group_grid(Pin) * np.slices)), dim3(HW * WAVE), 0, s,
+                           *Pin, q, k, v, o, d_o, lse, dq, scratch, ws_dq, scale, scale * LOG2E, drop.thr, drop.seed, drop.inv, (const float *)nullptr,
+                           (float *)nullptr, np, md);
+    });
+    int st = launch_status();
+    if (st != BPT_OK) return st;
+    pick(false, false, parts_src, [&](auto, auto, auto sp) {
+        constexpr int HW = sp() == 1 ? NARROW_HW : sp();
+        hipLaunchKernelGGL((k_attn_bwd_src_tile<float, 16, 64, HW, true, sp()>), dim3((unsigned)(group_grid(Pout) * np_src.slices)), dim3(HW * WAVE), 0, s, *Pout, q,
+                           d_o, (const float2 *)scratch, dk, dv, ws_dk, ws_dv, np_src);
+    });
+    st = launch_status();
+    if (st != BPT_OK) return st;
+    if (Pin->n_heavy + Pout->n_heavy > 0)
+        hipLaunchKernelGGL((k_combine_sum3<float, true>), dim3((unsigned)(Pin->n_heavy + Pout->n_heavy), C / (4 * WAVE), 2), dim3(BLOCK), 0, s, Pin->heavy,
+                           (int)Pin->n_heavy, (const float *)ws_dq, dq, Pout->heavy, (const float *)ws_dk, dk, dv, C, (size_t)Pout->n_slots * C, nw);
+    if (dslopes) hipLaunchKernelGGL(k_slope_finish, dim3(nw.heads), dim3(BLOCK), 0, s, (const float *)part, Pin->grp_chunks + 8, nw.h, parts,
+                                    (const float *)nullptr, 0, dslopes);
+    return launch_status();
+}
+
+inline int check_score(const bpt_plan *P, const bpt_score *sc, int heads, int d, int h, int dtype, float dropout_p, const float *bias, Narrow &nw) {
     const int st = check_plan(P, true);
     if (st != BPT_OK) return st;
     if (!sc) return BPT_ERR_NULL;
     if (dtype != BPT_F32 && dtype != BPT_BF16) return dtype == BPT_F64 ? BPT_ERR_UNSUPPORTED : BPT_ERR_DTYPE;
     if (h != 8 && h != 16 && !(h == 4 && dtype == BPT_F32)) return BPT_ERR_UNSUPPORTED;
+    if (heads < 1 || d < 1) return BPT_ERR_SHAPE;
+    const bool narrow = heads != h || d != 64;
+    if (narrow && (dtype != BPT_F32 || bias || heads > h || d < 4 || d > 64)) return BPT_ERR_UNSUPPORTED;
+    nw = narrow ? Narrow{d, heads, h, (heads + NARROW_HW - 1) / NARROW_HW} : Narrow{};
     if (!(sc->cap >= 0.f && sc->cap <= 3.0e38f) || !(dropout_p >= 0.f && dropout_p < 1.f)) return BPT_ERR_SIZE;
     if (sc->slopes && (!sc->pos_q || !sc->pos_k)) return BPT_ERR_NULL;
     if (P->n_rows == 0 || P->n_groups == 0) return P->n_edges == 0 ? BPT_OK : BPT_ERR_UNSUPPORTED;
     if (!has_tiles(P, h, 64, dtype == BPT_BF16 ? 2 : 4)) return BPT_ERR_UNSUPPORTED;
-    if ((bias || dropout_p > 0.f) && !P->grp_eids) return BPT_ERR_PLAN;
+    if ((bias || dropout_p > 0.f || narrow) && !P->grp_eids) return BPT_ERR_PLAN;
     if (bias && P->bias_by_pair) return BPT_ERR_PLAN;
     return BPT_OK;
 }
@@ -182,28 +283,35 @@ int64_t bpt_score_forward_workspace_bytes(const bpt_plan *plan_in, int h) {
 
 int64_t bpt_score_backward_workspace_bytes(const bpt_plan *plan_in, const bpt_plan *plan_out, int h, int dtype, int has_bias) {
     if (!plan_in || !plan_out || h < 1 || (dtype != BPT_F32 && dtype != BPT_BF16)) return -1;
-    return scratch_bytes(plan_in, plan_out, h, dtype, has_bias != 0) + slope_bytes(plan_in, h) +
+    return scratch_bytes(plan_in, plan_out, h, dtype, has_bias != 0) + slope_bytes(plan_in, h) + (dtype == BPT_BF16 && !has_bias ? split_bytes(plan_in, h) : 0) +
            round16((plan_in->n_slots + 2 * plan_out->n_slots) * (int64_t)h * 64 * 4);
 }
 
 int bpt_score_forward(const bpt_plan *plan_in, const bpt_score *score, const void *q, const void *k, const void *v, const float *bias, void *o, float *lse,
-                      void *workspace, int64_t workspace_bytes, float scale, float dropout_p, uint64_t dropout_seed, int h, int dtype, void *stream) {
-    const int st = check_score(plan_in, score, h, dtype, dropout_p, bias);
+                      void *workspace, int64_t workspace_bytes, float scale, float dropout_p, uint64_t dropout_seed, int heads, int d, int h, int dtype,
+                      void *stream) {
+    Narrow nw;
+    const int st = check_score(plan_in, score, heads, d, h, dtype, dropout_p, bias, nw);
     if (st != BPT_OK) return st;
     if (plan_in->n_rows == 0) return BPT_OK;
     if (plan_in->n_groups == 0) return BPT_ERR_UNSUPPORTED;
     if (!q || !k || !v || !o || !lse) return BPT_ERR_NULL;
-    if (!on16({q, k, v, o, workspace})) return BPT_ERR_UNSUPPORTED;
+    if (!aligned16(workspace) || (nw.heads == 0 && !on16({q, k, v, o}))) return BPT_ERR_UNSUPPORTED;
     const int64_t need = bpt_score_forward_workspace_bytes(plan_in, h);
     if (need > 0 && (!workspace || workspace_bytes < need)) return BPT_ERR_WORKSPACE;
     const Dropout drop = make_dropout(dropout_p, dropout_seed);
+    if (nw.heads > 0)
+        return run_forward_narrow(plan_in, score, (const float *)q, (const float *)k, (const float *)v, (float *)o, lse, workspace, scale, drop, nw,
+                                  (hipStream_t)stream);
     DISPATCH((run_forward<T, H>(plan_in, score, q, k, v, bias, o, lse, workspace, scale, drop, (hipStream_t)stream)))
 }
 
 int bpt_score_backward(const bpt_plan *plan_in, const bpt_plan *plan_out, const bpt_score *score, const void *q, const void *k, const void *v,
                        const float *bias, const void *o, const void *d_o, const float *lse, void *dq, void *dk, void *dv, float *ds_out, float *dslopes,
-                       void *workspace, int64_t workspace_bytes, float scale, float dropout_p, uint64_t dropout_seed, int h, int dtype, void *stream) {
-    int st = check_score(plan_in, score, h, dtype, dropout_p, bias);
+                       void *workspace, int64_t workspace_bytes, float scale, float dropout_p, uint64_t dropout_seed, int heads, int d, int h, int dtype,
+                      void *stream) {
+    Narrow nw;
+    int st = check_score(plan_in, score, heads, d, h, dtype, dropout_p, bias, nw);
     if (st != BPT_OK) return st;
     st = check_plan(plan_out, true);
     if (st != BPT_OK) return st;
@@ -212,9 +320,12 @@ int bpt_score_backward(const bpt_plan *plan_in, const bpt_plan *plan_out, const 
     if ((bias != nullptr) != (ds_out != nullptr) || (dslopes && !score->slopes)) return BPT_ERR_NULL;
     if (dropout_p > 0.f && dtype == BPT_BF16 && !bias && !plan_out->grp_eids) return BPT_ERR_PLAN;
     if (!q || !k || !v || !o || !d_o || !lse || !dq || !dk || !dv) return BPT_ERR_NULL;
-    if (!on16({q, k, v, o, d_o, dq, dk, dv, workspace})) return BPT_ERR_UNSUPPORTED;
+    if (!aligned16(workspace) || (nw.heads == 0 && !on16({q, k, v, o, d_o, dq, dk, dv}))) return BPT_ERR_UNSUPPORTED;
     if (!workspace || workspace_bytes < bpt_score_backward_workspace_bytes(plan_in, plan_out, h, dtype, bias != nullptr)) return BPT_ERR_WORKSPACE;
     const Dropout drop = make_dropout(dropout_p, dropout_seed);
+    if (nw.heads > 0)
+        return run_backward_narrow(plan_in, plan_out, score, (const float *)q, (const float *)k, (const float *)v, (const float *)o, (const float *)d_o, lse,
+                                   (float *)dq, (float *)dk, (float *)dv, dslopes, workspace, scale, drop, nw, (hipStream_t)stream);
     DISPATCH((run_backward<T, H>(plan_in, plan_out, score, q, k, v, bias, o, d_o, lse, dq, dk, dv, ds_out, dslopes, workspace, scale, drop, (hipStream_t)stream)))
 }
 

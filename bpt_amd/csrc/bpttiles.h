@@ -871,6 +871,7 @@ struct ScoreMod {
     const float *slopes;               // (heads), or null: no distance
     const float *pos_member, *pos_entry;       // positions of the plan's rows, of the rows its indices name
     float *part;                       // destination side: [group][head][part] sums of dL/ds |pos - pos|, or null
+    float2 *split;                     // bfloat16 destination side: [slot][head] sums of p dP and of p |pos - pos| over a split row's segment
 };
 struct NoMod {};
 template <bool MOD> struct ModArg { typedef NoMod type; };
@@ -1770,14 +1771,21 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP 
 // Destination side.  PDS: (p, ds) of the pairs go to the scratch for the source side that reads them back; otherwise that side
 // forms them again (k_attn_bwd_src_tile_bf16_again) and all it is handed is (lse, delta) of the rows, `stat` (n, H): the
 // segments of a split row write the same values.
+// MOD without a score term: delta = dO . O with O as stored is off by O's rounding and by that of the p that O was summed with, both 2^-9 of each
+// term, which all pairs of a row share: at L = 32768, k = 8 dq and dk come out 0.0041 off (0.0017 is one rounding of the result) and the slopes'
+// gradient, a sum over all pairs that nothing rounds, as far.  The pairs of a whole row give delta in 32 bits, sum p dP, once they have all been seen:
+//   ds = p (dP - delta') du  corrected by  (delta' - delta) sum p du K  in dq and by  (delta' - delta) sum p |pos - pos|  in the slopes' gradient,
+// the source side is handed delta.  One more product a block over the K rows at hand.  dq of a split row keeps delta' (it has many pairs, each with a
+// small p); its segments leave their sums, from which k_score_split forms the other two before the source side runs.
 template <int H, int D, int HW, int WPE, bool DROP, int BIAS, bool PDS, int SP, bool MOD = false>
-__global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP || BIAS || MOD ? WPE - 1 : WPE))) void k_attn_bwd_dst_rows_bf16(
+__global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(MOD && (DROP || BIAS) ? WPE - 2 : DROP || BIAS || MOD ? WPE - 1 : WPE))) void k_attn_bwd_dst_rows_bf16(
     bpt_plan P, const bf16_t *__restrict__ q, const bf16_t *__restrict__ k, const bf16_t *__restrict__ v, const bf16_t *__restrict__ o,
     const bf16_t *__restrict__ d_o, const float *__restrict__ lse, bf16_t *__restrict__ dq, uint32_t *__restrict__ pds,
     float2 *__restrict__ stat, float *__restrict__ ws_dq, float scale, float scale_log2e, uint32_t drop_thr, uint32_t drop_seed, float drop_inv,
     const float *__restrict__ bias, float *__restrict__ ds_out, typename ModArg<MOD>::type md) {
     static_assert(PDS || BIAS == 0, "the score term's gradient is stored by the pair's position");
     constexpr uint32_t RB = H * D * 2;
+    constexpr bool FIX = MOD && !PDS;                             // delta from the pairs (comment above)
     const Narrow nw{};
     TileCtx t;
     if (!tile_begin<bf16_t, H, D, HW, false, SP>(P, t, nw)) return;
@@ -1826,7 +1834,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP 
         wave_lds_fence();
         const float d0 = lane_bcast(part[0], 8 * (c & 7)), d1 = lane_bcast(part[1], 8 * (c & 7));
         delta = c < 8 ? d0 : d1;
-        if constexpr (!PDS) {
+        if constexpr (!PDS && !FIX) {
             if (g == 0 && t.part == 0 && t.member.x >= 0) stat[at] = make_float2(lse_c, delta);
         }
         lse_c = lane_bcast(lse_c, c);
@@ -1841,6 +1849,10 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP 
     floatx4v acc[4];
 #pragma unroll
     for (int nb = 0; nb < 4; ++nb) acc[nb] = floatx4v{0.f, 0.f, 0.f, 0.f};
+    float dp_sum = 0.f, far_sum = 0.f;
+    floatx4v pk[FIX ? 4 : 1];                                     // sum of p du K, laid out as acc
+#pragma unroll
+    for (int nb = 0; nb < (FIX ? 4 : 0); ++nb) pk[nb] = floatx4v{0.f, 0.f, 0.f, 0.f};
     struct Blk {
         uintx4v kr[2], vr[2];
         int xe[DROP || BIAS == 1 ? 4 : 1];
@@ -1900,7 +1912,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP 
             const floatx4v st = tile_dot_bf16(row, qb);
             tile_operand_bf16(v_lds, c, g, row);
             const floatx4v dp = tile_dot_bf16(row, dob);
-            float ds[4], sm[4], du[4], pos_e[4];
+            float ds[4], sm[4], du[4], pos_e[4], pdu[4];
             if constexpr (MOD) {
                 float x[4];
                 const floatx4v at_e = *reinterpret_cast<const floatx4v *>(&pos_lds[t.wv][4 * g]);
@@ -1918,9 +1930,15 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP 
                 if constexpr (DROP)
                     mt = dropout_keep((uint32_t)xe[DROP ? r : 0] * (uint32_t)H + (uint32_t)t.head, drop_seed, drop_thr, drop_inv);
                 if constexpr (MOD) {
-                    ds[r] = where_pair_or_zero(mk[r], c, pe * (dp[r] * mt - delta));
+                    const float x = where_pair_or_zero(mk[r], c, pe * (dp[r] * mt));
+                    ds[r] = fmaf(-pe, delta, x);
                     if (md.part) slope_sum = fmaf(ds[r], fabsf(pos_m - pos_e[r]), slope_sum);
                     ds[r] *= du[r] * scale;
+                    if constexpr (FIX) {
+                        dp_sum += x;
+                        if (md.part) far_sum = fmaf(pe, fabsf(pos_m - pos_e[r]), far_sum);
+                        pdu[r] = pe * (du[r] * scale);
+                    }
                 } else {
                     ds[r] = pe * (dp[r] * mt - delta) * scale;
                 }
@@ -1934,8 +1952,37 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP 
             da.u[0] = pack_bf16(ds[0], ds[1]);
             da.u[1] = pack_bf16(ds[2], ds[3]);
             tile_axpy_rows_bf16(da, k_lds, c, g, acc);
+            if constexpr (FIX) {
+                da.u[0] = pack_bf16(pdu[0], pdu[1]);
+                da.u[1] = pack_bf16(pdu[2], pdu[3]);
+                tile_axpy_rows_bf16(da, k_lds, c, g, pk);
+            }
             wave_lds_fence();                                     // (read before the next block's are written)
             issue_loads_first();
+        }
+    }
+    if constexpr (FIX) {
+        float whole = groups_sum(dp_sum), far = groups_sum(far_sum);      // of member c, of this part
+        if constexpr (SP > 1) {
+            __shared__ float2 meet[HW][TILE_R];
+            if (g == 0) meet[t.wv][c] = make_float2(whole, far);
+            __syncthreads();
+            whole = far = 0.f;
+#pragma unroll
+            for (int i = 0; i < SP; ++i) {
+                const float2 x = meet[i * (HW / SP) + t.wv % (HW / SP)][c];
+                whole += x.x;
+                far += x.y;
+            }
+        }
+        const bool segment = t.member.y >= 0;
+        const float better = segment ? delta : whole, less = delta - better;
+        slope_sum = fmaf(less, far_sum, slope_sum);
+#pragma unroll
+        for (int nb = 0; nb < 4; ++nb) acc[nb] += less * pk[nb];
+        if (g == 0 && t.part == 0 && t.member.x >= 0) {
+            stat[(size_t)t.member.x * H + t.head] = make_float2(lse_c, better);
+            if (segment) md.split[(size_t)t.member.y * H + t.head] = make_float2(whole, far);
         }
     }
     if constexpr (MOD) tile_put_slope_part<SP>(md, t, H, slope_sum);
@@ -2272,7 +2319,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(WPE))
 // columns with dropout lost 2 %: heads of fewer than 64 columns keep the scratch.)  float32 keeps it too: there the two
 // products are 1024 cycles of the matrix pipeline per block.  122 registers: compiled for four wavefronts per SIMD.
 template <int H, int D, int HW, int WPE, bool DROP, int SP = 1, bool MOD = false>
-__global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(WPE))) void k_attn_bwd_src_tile_bf16_again(
+__global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(MOD && DROP ? WPE - 1 : WPE))) void k_attn_bwd_src_tile_bf16_again(
     bpt_plan P, const bf16_t *__restrict__ q, const bf16_t *__restrict__ k, const bf16_t *__restrict__ v, const bf16_t *__restrict__ d_o,
     const float2 *__restrict__ stat, bf16_t *__restrict__ dk, bf16_t *__restrict__ dv, float *__restrict__ ws_dk, float *__restrict__ ws_dv,
     float scale, float scale_log2e, uint32_t drop_thr, uint32_t drop_seed, float drop_inv, typename ModArg<MOD>::type md) {
@@ -2501,6 +2548,12 @@ inline int tile_parts(const bpt_plan *P, int heads, size_t elem, bool plain_forw
         return w <= 3072 || (w <= 6144 && each >= 2) || (parts == 2 && w <= most && each >= 4);
     };
     return pays(4) ? 4 : pays(2) ? 2 : 1;
+}
+
+// a tile in parts: one head a workgroup, so that no wavefront of it lies past the last head
+inline Narrow narrow_parts(Narrow nw, int parts) {
+    if (parts > 1) nw.slices = nw.heads;
+    return nw;
 }
 
 }  // namespace

@@ -1273,11 +1273,20 @@ def score_options(score_cap, slopes, pos, q, k):
 
 
 def score_padded_shape(q):
-    """(h', 64): the heads that the fused kernels with score options run q's (h, d, dtype) as (equal to (h, d): as it is), else None."""
+    """(h', 64): what the fused kernels with score options compute q's (h, d, dtype) as (equal to (h, d): rows of 64 columns, as they are), else
+    None."""
     if q.dim() != 3 or q.dtype not in (torch.float32, torch.bfloat16) or q.size(2) > 64:
         return None
     heads = [n for n in ((4, 8, 16) if q.dtype == torch.float32 else (8, 16)) if n >= q.size(1)]
     return (heads[0], 64) if heads and q.size(1) > 0 and q.size(2) > 0 else None
+
+
+def score_reads(q, rel=False):
+    """Whether the kernels read rows like q as they are: the shapes that score_padded_shape() leaves alone, and without a relative-position term
+    (rel) narrow heads of 4 columns or more in float32.  Others run on padded copies: bfloat16 because its kernels for narrow heads would hand the
+    source side pairs whose delta is off (comment at k_attn_bwd_dst_rows_bf16)."""
+    shape = score_padded_shape(q)
+    return shape is not None and (shape == _hd(q) or (not rel and q.dtype == torch.float32 and q.size(2) >= 4))
 
 
 def score_supported(eid_c, q, k):
@@ -1304,17 +1313,37 @@ def _score_linked(pi, po, k):
     return po.linked_to(pi, TILE_ROWS, order=_plan.tile_order_src(k.size(0), po.n_edges), partner_order=None, pair_numbers=True)
 
 
-def score_covers(graph, q, k, train):
-    """Whether the plans of a call whose shape score_supported() takes cover every edge (they are built here where they are new, both
-    sides' together for a call with a backward), as the tile kernels need."""
-    plans = (None, None)
+def prepare_score(graph, q, k, dropout_p, train):
+    """Builds the plans of a call that score_supported() and score_reads() take, where they are new (both sides' together for a call with a
+    backward), and leaves them with the native host path.  False where one does not cover every edge, as the tile kernels need."""
+    generation, plans = _native.generation(), (None, None)
+    index = graph if train else graph[4:]
+    for t in index:
+        _check_input(t, "every index tensor")
+        if t.dim() != 1 or t.dtype != torch.int64 or t.device != q.device:
+            raise ValueError(f"index tensors must be 1-D int64 on {q.device}")
+    _expect_index(graph[6], graph[7])
     if train:
+        _expect_index(graph[2], graph[3])
+        _expect_shape(graph[2], graph[6].shape, "eid_r")
         seg = _tile_seg_of(graph[6].size(0), q.size(0), k.size(0))
         sides = [(*graph[4:], q.size(0), k.size(0), seg, None), (*graph[:4], k.size(0), q.size(0), seg, _plan.tile_order_src(k.size(0), graph[2].size(0)))]
-        if all(t.dim() == 1 and t.dtype == torch.int64 and t.is_contiguous() and t.device == q.device for t in graph):
+        if plan_cache.may_hold(sides):
             plans = plan_cache.put_tile_plans(sides) or plans
     pi = _score_plan_in(graph, q, k, plans[0])
-    return pi.covers_all_edges and (not train or _score_plan_out(graph, q, k, plans[1]).covers_all_edges)
+    if not pi.covers_all_edges:
+        return False
+    numbers = [q.size(0), k.size(0), score_padded_shape(q)[0], q.size(2), _dtype(q), int(dropout_p > 0.0), q.size(1)]
+    in_struct = pi.ensure_groups(TILE_ROWS)["struct"]
+    plan_cache.remember((pi,), generation, _native.SCORE_FWD, list(graph[4:]), numbers, ctypes.addressof(in_struct), 0)
+    if train:
+        po = _score_plan_out(graph, q, k, plans[1])
+        if not po.covers_all_edges:
+            return False
+        out_struct = _score_linked(pi, po, k)
+        plan_cache.remember((pi, po), generation, _native.SCORE_TRAIN, list(graph[4:]) + list(graph[:4]), numbers, ctypes.addressof(in_struct),
+                            ctypes.addressof(out_struct))
+    return True
 
 
 def _score_struct(score):
@@ -1324,15 +1353,16 @@ def _score_struct(score):
 def _check_score_call(graph, q, k, v, score, bias):
     _check_all(col=graph[4], indptr_c=graph[5], eid_c=graph[6], indices_c=graph[7], q=q, k=k, v=v)
     _same_dtype(q, k, v)
-    h, d = _hd(q)
-    if score_padded_shape(q) != (h, d):
+    heads, d = _hd(q)
+    if not score_reads(q, bias is not None):
         raise RuntimeError("attention with score options has no fused kernel for this shape and type")
+    h = score_padded_shape(q)[0]
     _expect_index(graph[6], graph[7])
     _expect_shape(k, (k.size(0),) + tuple(q.shape[1:]), "k")
     _expect_shape(v, k.shape, "v")
     _check_bias(bias, graph[6].size(0), h, q.device, _SETTINGS)
     if score.slopes is not None:
-        for t, n, name in ((score.slopes, h, "slopes"), (score.pos_q, q.size(0), "pos_q"), (score.pos_k, k.size(0), "pos_k")):
+        for t, n, name in ((score.slopes, heads, "slopes"), (score.pos_q, q.size(0), "pos_q"), (score.pos_k, k.size(0), "pos_k")):
             _check_input(t, name)
             if t.dtype != torch.float32 or t.device != q.device:
                 raise ValueError(f"{name} must be float32 on {q.device}")
@@ -1342,7 +1372,8 @@ def _check_score_call(graph, q, k, v, score, bias):
 
 def score_attention_forward(col, indptr_c, eid_c, indices_c, q, k, v, score, scale=None, dropout_p=0.0, seed=0, bias=None):
     """(o, lse) as attention_forward's, of scores u = (q[dst].k[src] + bias[e]) scale that become score.cap tanh(u / score.cap) -
-    score.slopes[head] |pos_q[dst] - pos_k[src]| (a Score).  Shapes that score_padded_shape() leaves as they are; bias by edge id."""
+    score.slopes[head] |pos_q[dst] - pos_k[src]| (a Score).  Shapes that score_reads() takes; lse has the heads of score_padded_shape(); bias by
+    edge id."""
     graph = (None,) * 4 + (col, indptr_c, eid_c, indices_c)
     h = _check_score_call(graph, q, k, v, score, bias)
     scale = 1.0 / math.sqrt(q.size(2)) if scale is None else float(scale)
@@ -1356,7 +1387,8 @@ def score_attention_forward(col, indptr_c, eid_c, indices_c, q, k, v, score, sca
     ws = torch.empty(nws, dtype=torch.uint8, device=q.device) if nws else None
     with _on_device_of(q):
         check_attn(_SCORE_LIB.bpt_score_forward(ref, _score_struct(score), _ptr(q), _ptr(k), _ptr(v), _ptr(bias), _ptr(o), _ptr(lse), _ptr(ws), nws, scale,
-                                                float(dropout_p), int(seed) & (2 ** 64 - 1), h, _dtype(q), _stream()), "score_attention_forward")
+                                                float(dropout_p), int(seed) & (2 ** 64 - 1), q.size(1), q.size(2), h, _dtype(q), _stream()),
+                   "score_attention_forward")
     return o, lse
 
 
@@ -1391,7 +1423,8 @@ def score_attention_backward(row, indptr_r, eid_r, indices_r, col, indptr_c, eid
     with _on_device_of(q):
         check_attn(_SCORE_LIB.bpt_score_backward(in_ref, out_ref, _score_struct(score), _ptr(q), _ptr(k), _ptr(v), _ptr(bias), _ptr(o), _ptr(do), _ptr(lse),
                                                  _ptr(dq), _ptr(dk), _ptr(dv), _ptr(ds), _ptr(dslopes), _ptr(ws), nws, scale, float(dropout_p),
-                                                 int(seed) & (2 ** 64 - 1), h, _dtype(q), _stream()), "score_attention_backward")
+                                                 int(seed) & (2 ** 64 - 1), q.size(1), q.size(2), h, _dtype(q), _stream()),
+                   "score_attention_backward")
     return dq, dk, dv, dslopes, None if ds is None else ds[:-1]
 
 

@@ -428,29 +428,34 @@ def _score_attention(graph, q, k, v, scale, fused, dropout_p, seed, rel_table, e
         return _score_chain(graph, q, k, v, scale, dropout_p, rel_table, etype, score)
     if dropout_p > 0 and seed is None:
         seed = int(torch.randint(0, 2 ** 62, (1,)).item())
-    seed = int(seed or 0)
-    h, d = q.size(1), q.size(2)
-    hp, dp = _g.score_padded_shape(q)
-    on16 = lambda x: x.clone() if x.data_ptr() % 16 else x          # (the tile kernels read 16 bytes a lane)
-    if (hp, dp) != (h, d):
+    seed, dropout_p = int(seed or 0), float(dropout_p)
+    (h, d), (hp, dp) = q.shape[1:], _g.score_padded_shape(q)
+    rel, as_it_is = rel_table is not None, _g.score_reads(q, rel_table is not None)
+    given = q, k, v, rel_table, score
+    if not as_it_is:
         # as the narrow heads of the plain layer with relative positions: zero columns and heads add nothing
         q, k, v = (torch.nn.functional.pad(x, (0, dp - d, 0, hp - h)) for x in (q, k, v))
-        rel_table = None if rel_table is None else torch.nn.functional.pad(rel_table, (0, dp - d))
+        rel_table = torch.nn.functional.pad(rel_table, (0, dp - d)) if rel else None
         if score.slopes is not None:
             score = score._replace(slopes=torch.nn.functional.pad(score.slopes, (0, hp - h)))
-    else:
-        q, k, v = on16(q), on16(k), on16(v)
-    if not _g.score_covers(graph, q, k, train):
-        if fused:
-            raise RuntimeError("attention with score options needs units that cover every edge")
-        return _score_chain(graph, q[:, :h, :d].contiguous(), k[:, :h, :d].contiguous(), v[:, :h, :d].contiguous(), scale, dropout_p,
-                            None if rel_table is None else rel_table[:, :d].contiguous(), etype,
-                            score if score.slopes is None else score._replace(slopes=score.slopes[:h].contiguous()))
-    if rel_table is not None:
-        o = BPTRelAttention.apply(*graph, q, k, v, scale, float(dropout_p), seed, rel_table, etype, None, False, score, score.slopes)
-    else:
-        o = BPTScoreAttention.apply(*graph, q, k, v, score.slopes, score, scale, float(dropout_p), seed)
-    return o if (hp, dp) == (h, d) else o[:, :h, :d].contiguous()
+    elif d == 64:
+        q, k, v = (x.clone() if x.data_ptr() % 16 else x for x in (q, k, v))          # (the kernels read 16 bytes a lane)
+    o = None
+    if not rel:
+        native = lambda: _native.score_attention(*graph, q, k, v, *score[1:], score.cap, scale, dropout_p, seed & (2 ** 64 - 1), hp)
+        o = native()
+    if o is None:
+        if not _g.prepare_score(graph, q, k, dropout_p, train):
+            if fused:
+                raise RuntimeError("attention with score options needs units that cover every edge")
+            return _score_chain(graph, *given[:3], scale, dropout_p, given[3], etype, given[4])
+        if rel:
+            o = BPTRelAttention.apply(*graph, q, k, v, scale, dropout_p, seed, rel_table, etype, None, False, score, score.slopes)
+        else:
+            o = native()
+            if o is None:                                         # (a cache too small for the plans leaves nothing with the native host path)
+                o = BPTScoreAttention.apply(*graph, q, k, v, score.slopes, score, scale, dropout_p, seed)
+    return o if as_it_is else o[:, :h, :d].contiguous()
 
 
 def bpt_attention(row, indptr_r, eid_r, indices_r, col, indptr_c, eid_c, indices_c, q, k, v, scale=None, fused=None,
@@ -473,7 +478,7 @@ def bpt_attention(row, indptr_r, eid_r, indices_r, col, indptr_c, eid_c, indices
     score_cap c > 0 makes it c tanh(u / c), which bounds it by c;
     slopes (h,) float32 and pos, float32 positions of the rows (one tensor, or a pair (of the query rows, of the key rows)), lower it by
     slopes[head] * |pos[dst] - pos[src]| behind the cap.  slopes get a gradient, pos does not.  Heads of up to 64 columns, 16 of them,
-    in float32 and bfloat16 run fused (narrow ones on padded copies), other shapes and float64 through the chain.  Edges are the
+    in float32 and bfloat16 run fused (bfloat16 narrow ones on padded copies), other shapes and float64 through the chain.  Edges are the
     graph's: documents that must not see each other are its separate components."""
     scale = 1.0 / math.sqrt(q.size(-1)) if scale is None else float(scale)
     if (rel_table is None) != (etype is None):

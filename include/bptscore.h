@@ -2,8 +2,9 @@
  *
  * The fused pass of bptattn.h (bpt_attention_forward / _backward) with, for an edge and head and u = (q[dst].k[src] + bias) scale,
  *   s = cap tanh(u / cap)   (s = u where cap is 0)   - slopes[head] |pos_q[dst] - pos_k[src]|   (where slopes is given)
- * in place of u.  Heads of 64 columns; float32 with 4, 8 or 16 of them, bfloat16 with 8 or 16.  Plans carry groups of 16 rows (tiles), the
- * source side's the pair numbers of the destination side's; grp_eids where there is dropout or a bias.  Conventions, status codes,
+ * in place of u.  Heads of 64 columns; float32 with 4, 8 or 16 of them, bfloat16 with 8 or 16; float32 without a bias also heads of 4 to 64 columns as
+ * they are, `heads` of them, computed as h = 4, 8 or 16 (h is what lse (n, h), the workspace and dropout's hash count).  Plans carry groups of 16 rows
+ * (tiles), the source side's the pair numbers of the destination side's; grp_eids where there is dropout or a bias.  Conventions, status codes,
  * plans, bias, ds_out, dropout and lse are those of bptattn.h (bias by edge id: bias_by_pair is refused).  Deterministic; nothing is allocated.
  */
 #ifndef BPTSCORE_H
@@ -19,7 +20,7 @@ extern "C" {
 
 typedef struct {
     float cap;                        /* 0: not capped; finite and positive otherwise */
-    const float *slopes;              /* (h) float32, or NULL: no distance */
+    const float *slopes;              /* (heads) float32, or NULL: no distance */
     const float *pos_q, *pos_k;       /* float32 positions of the query rows and of the key rows, with slopes */
 } bpt_score;
 
@@ -27,12 +28,14 @@ int64_t bpt_score_forward_workspace_bytes(const bpt_plan *plan_in, int h);
 int64_t bpt_score_backward_workspace_bytes(const bpt_plan *plan_in, const bpt_plan *plan_out, int h, int dtype, int has_bias);
 
 int bpt_score_forward(const bpt_plan *plan_in, const bpt_score *score, const void *q, const void *k, const void *v, const float *bias, void *o, float *lse,
-                      void *workspace, int64_t workspace_bytes, float scale, float dropout_p, uint64_t dropout_seed, int h, int dtype, void *stream);
+                      void *workspace, int64_t workspace_bytes, float scale, float dropout_p, uint64_t dropout_seed, int heads, int d, int h, int dtype,
+                      void *stream);
 
-/* ds_out goes with bias; dslopes (h) float32 or NULL: dL/dslopes = -sum over the edges of dL/ds |pos_q[dst] - pos_k[src]|. */
+/* ds_out goes with bias; dslopes (heads) float32 or NULL: dL/dslopes = -sum over the edges of dL/ds |pos_q[dst] - pos_k[src]|. */
 int bpt_score_backward(const bpt_plan *plan_in, const bpt_plan *plan_out, const bpt_score *score, const void *q, const void *k, const void *v,
                        const float *bias, const void *o, const void *d_o, const float *lse, void *dq, void *dk, void *dv, float *ds_out, float *dslopes,
-                       void *workspace, int64_t workspace_bytes, float scale, float dropout_p, uint64_t dropout_seed, int h, int dtype, void *stream);
+                       void *workspace, int64_t workspace_bytes, float scale, float dropout_p, uint64_t dropout_seed, int heads, int d, int h, int dtype,
+                      void *stream);
 
 #ifdef __cplusplus
 }

@@ -839,58 +839,6 @@ __global__ __launch_bounds__(BLOCK) void k_softmax_split_quads(bpt_plan P, const
 // ------------------------------------------------------------------------------------------
 // fast family: compile-time (H, D), f32 / bf16
 // ------------------------------------------------------------------------------------------
-template <typename T, int H_, int D_> struct Lay {
-    static constexpr int H = H_, D = D_, C = H_ * D_;
-    static constexpr int LPH = 64 / H_;                 // lanes per head
-    static constexpr int EPL = C / 64;                  // elements per lane (all of one head)
-    static constexpr int VE = 16 / (int)sizeof(T);      // elements per 16-byte vector
-    static constexpr int NV = EPL / VE;                 // 16-byte vectors per lane
-    static_assert(64 % H_ == 0 && C % 64 == 0 && EPL % VE == 0 && NV >= 1, "unsupported fast shape");
-    static_assert(LPH >= 4, "the row-group kernels broadcast per-member values inside quads of one head");
-    static_assert(D_ == NV * LPH * VE, "layout does not tile the head");
-    // element offset inside a node row of vector i of `lane`: LPH consecutive lanes cover
-    // LPH*16 contiguous bytes of their head
-    static __device__ __forceinline__ int off(int lane, int i) { return (lane / LPH) * D + (i * LPH + lane % LPH) * VE; }
-};
-
-template <typename T, int H, int D>
-__device__ __forceinline__ void load_row(const T *__restrict__ row, int lane, float (&out)[Lay<T, H, D>::EPL]) {
-    using L = Lay<T, H, D>;
-#pragma unroll
-    for (int i = 0; i < L::NV; ++i) {
-        if constexpr (sizeof(T) == 4) {
-            const float4 v = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(row) + L::off(lane, i));
-            out[4 * i] = v.x; out[4 * i + 1] = v.y; out[4 * i + 2] = v.z; out[4 * i + 3] = v.w;
-        } else {
-            const uint4 v = *reinterpret_cast<const uint4 *>(reinterpret_cast<const uint16_t *>(row) + L::off(lane, i));
-            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                out[8 * i + 2 * c] = __uint_as_float(w[c] << 16);
-                out[8 * i + 2 * c + 1] = __uint_as_float(w[c] & 0xffff0000u);
-            }
-        }
-    }
-}
-
-template <typename T, int H, int D>
-__device__ __forceinline__ void store_row(T *__restrict__ row, int lane, const float (&in)[Lay<T, H, D>::EPL]) {
-    using L = Lay<T, H, D>;
-#pragma unroll
-    for (int i = 0; i < L::NV; ++i) {
-        if constexpr (sizeof(T) == 4) {
-            *reinterpret_cast<float4 *>(reinterpret_cast<float *>(row) + L::off(lane, i)) =
-                make_float4(in[4 * i], in[4 * i + 1], in[4 * i + 2], in[4 * i + 3]);
-        } else {
-            uint32_t w[4];
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-                w[c] = (uint32_t)f32_to_bf16(in[8 * i + 2 * c]) | ((uint32_t)f32_to_bf16(in[8 * i + 2 * c + 1]) << 16);
-            *reinterpret_cast<uint4 *>(reinterpret_cast<uint16_t *>(row) + L::off(lane, i)) = make_uint4(w[0], w[1], w[2], w[3]);
-        }
-    }
-}
-
 // The D elements of an (E, D) edge-feature row that go with this lane's slice of a head (every head's lanes read
 // the same D elements).
 template <typename T, int H, int D>
@@ -914,49 +862,8 @@ __device__ __forceinline__ void load_head_row(const T *__restrict__ row, int lan
     }
 }
 
-// f32 partial rows in the workspace are stored in natural column order (the combine kernels
-// index them by column), whatever the element type of the node tensors
-template <typename T, int H, int D>
-__device__ __forceinline__ void store_row_ws(float *__restrict__ row, int lane, const float (&in)[Lay<T, H, D>::EPL]) {
-    using L = Lay<T, H, D>;
-#pragma unroll
-    for (int i = 0; i < L::NV; ++i)
-#pragma unroll
-        for (int c = 0; c < L::VE / 4; ++c)
-            *reinterpret_cast<float4 *>(row + L::off(lane, i) + 4 * c) =
-                make_float4(in[L::VE * i + 4 * c], in[L::VE * i + 4 * c + 1], in[L::VE * i + 4 * c + 2], in[L::VE * i + 4 * c + 3]);
-}
-
-template <int N> __device__ __forceinline__ float dot_n(const float (&a)[N], const float (&b)[N]) {
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < N; ++i) s = fmaf(a[i], b[i], s);
-    return s;
-}
-
 // weight loads for the fast SpMM: the unfused API passes T-typed edge data, the fused backward f32
 template <typename WT> __device__ __forceinline__ float ld_w(const WT *p) { return Elem<WT>::ld(p); }
-
-// NW wavefronts (a workgroup) share an item: each takes whole batches of its edges, as many as the others, and the sums meet in
-// LDS.  False: no such item (the whole workgroup).  parts: how many wavefronts have edges (one at least).
-template <int NW, int BATCH> __device__ __forceinline__ bool fetch_item_part(const bpt_plan &P, Item &it, int &part, int &parts) {
-    part = 0;
-    parts = 1;
-    if constexpr (NW == 1) return fetch_item(P, it);
-    const int w = xcd_contiguous_block();
-    if (w >= (int)P.n_items) return false;
-    const int4 v = reinterpret_cast<const int4 *>(P.items)[w];
-    it.row = __builtin_amdgcn_readfirstlane(v.x);
-    it.begin = __builtin_amdgcn_readfirstlane(v.y);
-    it.end = __builtin_amdgcn_readfirstlane(v.z);
-    it.slot = __builtin_amdgcn_readfirstlane(v.w);
-    const int deg = it.end - it.begin, per = (deg + NW * BATCH - 1) / (NW * BATCH) * BATCH;
-    part = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    parts = max(1, (deg + max(per, 1) - 1) / max(per, 1));
-    it.begin = min(it.begin + part * per, it.end);
-    it.end = min(it.begin + per, it.end);
-    return true;
-}
 
 // the wavefronts' sums of one item in the first wavefront, in their order; the others are done.  By the whole workgroup.
 template <int NW, int N> __device__ __forceinline__ bool parts_meet(float (&acc)[N], int part, int parts, int lane) {
@@ -3192,7 +3099,6 @@ inline bool fast_shape(int h, int d, int dtype) {
     return false;
 }
 
-constexpr int FAST_BATCH = 4;
 
 // ---- generic launchers (dtype dispatch) ----
 template <typename T, int MODE>
@@ -3370,28 +3276,6 @@ int spmm_edge_generic(const bpt_plan *P, const void *W, const void *X, void *Y, 
 }
 
 // ---- fast launchers ----
-// Wavefronts a work item for the kernels that walk single rows.  The fused kernels walk them on graphs of fewer than 1536 items (with
-// row groups switched off: on any), the separate operators' SpMM where it is handed a plan without groups.  There a launch lasts
-// as long as its longest item: 16 batches of four edges one after the other, each a round trip to memory.  Forward / destination
-// side / source side, one -> four -> eight wavefronts an item, 8 x 64 float32 unless said otherwise, us:
-//   127 items (L = 64)                  9.4 / 13.7 / 7.2  -> 4.7 / 6.4 / 4.2   -> 4.8 / 5.6 / 4.2;   SpMM 7.5 -> 4.0 -> 3.8
-//   539 (L = 256, k = 16)              11.1 / 16.6 / 14.4 -> 9.2 / 11.7 / 11.6 -> 8.2 / 9.4 / 10.8;  bfloat16 12.2 / 16.9 / 15.5 -> 6.0 / 7.3 / 7.4 -> 5.6 / 6.6 / 7.4
-//   816 (L = 400)                      11.4 / 16.6 / 13.8 -> 7.9 / 10.0 / 11.0 -> 9.0 / 10.4 / 10.5; SpMM 10.8 -> 6.7 -> 6.7
-//   1434 (L = 700, k = 1)              15.7 / 21.2 / 15.0 -> 10.1 / 12.0 / 12.2 -> 11.3 / 12.8 / 12.6; SpMM 11.6 -> 7.9 -> 7.1
-//   2050 (L = 1000, k = 1, no groups)  16.8 / 22.2 / 17.9 -> 11.0 / 14.0 / 13.6 -> 14.1 / 17.0 / 15.4; SpMM 11.6 -> 8.4 -> 8.2
-// Larger launches fill the GPU with a wavefront an item.  Rows of 1024 columns take twice the registers and the LDS: eight
-// wavefronts an item of them are one round of the chip up to 256 items, beyond it four are faster.  16 x 64:
-//   268 (L = 130, k = 4)               16.3 / 22.7 / 16.7 -> 7.9 / 10.4 / 9.3   -> 8.2 / 10.2 / 9.4;   bfloat16 16.4 / 21.3 / 19.6 -> 7.6 / 9.6 / 8.7 -> 8.3 / 8.7 / 11.4
-//   324 (L = 160, k = 4)               15.7 / 22.1 / 18.1 -> 8.5 / 10.2 / 13.1  -> 10.2 / 12.0 / 12.6; bfloat16 16.0 / 20.7 / 19.8 -> 7.6 / 9.6 / 11.5 -> 10.5 / 10.8 / 12.2
-//   585 (L = 256, k = 16, both ways)   18.7 / 26.8 / 23.4 -> 18.6 / 21.2 / 19.4 -> 22.3 / 24.3 / 21.2
-// A float32 forward of 512 columns or more that already has a wavefront for each of the 1024 SIMDs and 25 edges or more an
-// item waits for the rate of its loads, not for one item: one -> four, 8 x 64 and 16 x 64, 983 items of 25 790 edges 11.7 -> 12.4 and 19.1 ->
-// 21.0; 957 of 32 613 12.0 -> 12.2 and 19.7 -> 20.4; (1018 of 23 540 11.3 -> 11.2 and 18.2 -> 18.7; 756 items 11.2 -> 10.4 and 18.6 -> 17.1).
-inline int row_parts(const bpt_plan *P, int columns, bool forward_f32 = false) {
-    if (P->n_items <= (columns > 512 ? 288 : 640)) return 8;
-    if (forward_f32 && columns >= 512 && P->n_items > 800 && P->n_items <= 1024 && P->n_edges >= 25000) return 1;
-    return P->n_items <= 2048 ? 4 : 1;
-}
 template <typename T, int H, int D>
 int run_sddmm_fast(const bpt_plan *P, const void *A, const void *B, void *y, hipStream_t s) {
     if (P->n_items == 0) return BPT_OK;

@@ -62,6 +62,95 @@ __global__ __launch_bounds__(BLOCK) void k_slope_finish(const float *__restrict_
     if (threadIdx.x == 0) dslopes[head] = (float)-meet[0];
 }
 
+// Forward of few query rows (a decoder that takes one token at a time): a tile would walk a row's neighbours in one chain with fifteen of its sixteen
+// rows empty.  Here a workgroup of NW wavefronts has a row or a segment of one, a wavefront whole rows of K and V, lane l columns of head l / (64 / H), four
+// edges in flight, and the segments are merged as those of the tiles' split rows.  Without dropout and score term.
+template <typename T, int H, int D, int BATCH, int NW>
+__global__ __launch_bounds__(NW == 1 ? BLOCK : NW * WAVE) void k_score_fwd_rows(bpt_plan P, const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v,
+                                                                                T *__restrict__ o, float *__restrict__ lse, float *__restrict__ ws_acc,
+                                                                                float *__restrict__ ws_ml, float scale_log2e, ScoreMod md) {
+    using L = Lay<T, H, D>;
+    Item it;
+    int part, parts;
+    if (!fetch_item_part<NW, BATCH>(P, it, part, parts)) return;
+    const int lane = threadIdx.x & 63, head = lane / L::LPH;
+    float qv[L::EPL], acc[L::EPL];
+    load_row<T, H, D>(q + (size_t)it.row * L::C, lane, qv);
+#pragma unroll
+    for (int i = 0; i < L::EPL; ++i) acc[i] = 0.f;
+    const float slope = md.slopes ? md.slopes[head] * LOG2E : 0.f, pos_m = md.slopes ? md.pos_member[it.row] : 0.f;
+    float m = M_INIT_LOG2, l = 0.f;
+    for (int p0 = it.begin; p0 < it.end; p0 += WAVE) {
+        const int cnt = min(WAVE, it.end - p0);
+        const int my_idx = lane < cnt ? P.idx[p0 + lane] : 0;
+        const float my_pos = md.slopes && lane < cnt ? md.pos_entry[my_idx] : 0.f;
+        for (int b = 0; b < cnt; b += BATCH) {
+            float kv[BATCH][L::EPL], vv[BATCH][L::EPL], x[BATCH], pos_e[BATCH], s[BATCH], du[BATCH];
+#pragma unroll
+            for (int e = 0; e < BATCH; ++e) {
+                const int j = (b + e < cnt) ? b + e : b, src = __builtin_amdgcn_readlane(my_idx, j);
+                pos_e[e] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(my_pos), j));
+                load_row<T, H, D>(k + (size_t)src * L::C, lane, kv[e]);
+                load_row<T, H, D>(v + (size_t)src * L::C, lane, vv[e]);
+            }
+            issue_loads_first();
+#pragma unroll
+            for (int e = 0; e < BATCH; ++e) x[e] = head_sum<L::LPH>(dot_n<L::EPL>(qv, kv[e]));
+            tile_mod_scores(md, scale_log2e, slope, pos_m, pos_e, x, s, du);
+            float mx = m;
+#pragma unroll
+            for (int e = 0; e < BATCH; ++e) {
+                s[e] = (b + e < cnt) ? s[e] : -INFINITY;
+                mx = fmaxf(mx, s[e]);
+            }
+            const float alpha = __builtin_amdgcn_exp2f(m - mx);
+            l *= alpha;
+#pragma unroll
+            for (int i = 0; i < L::EPL; ++i) acc[i] *= alpha;
+#pragma unroll
+            for (int e = 0; e < BATCH; ++e) {
+                const float pe = __builtin_amdgcn_exp2f(s[e] - mx);
+                l += pe;
+#pragma unroll
+                for (int i = 0; i < L::EPL; ++i) acc[i] = fmaf(pe, vv[e][i], acc[i]);
+            }
+            m = mx;
+        }
+    }
+    if constexpr (NW > 1) {
+        __shared__ float held[NW - 1][L::EPL + 2][WAVE];
+        if (part > 0 && part < parts) {
+#pragma unroll
+            for (int i = 0; i < L::EPL; ++i) held[part - 1][i][lane] = acc[i];
+            held[part - 1][L::EPL][lane] = m;
+            held[part - 1][L::EPL + 1][lane] = l;
+        }
+        __syncthreads();
+        if (part > 0) return;
+        for (int w = 0; w < parts - 1; ++w) {
+            const float mw = held[w][L::EPL][lane], mx = fmaxf(m, mw);
+            const float a = __builtin_amdgcn_exp2f(m - mx), b = __builtin_amdgcn_exp2f(mw - mx);
+            l = fmaf(b, held[w][L::EPL + 1][lane], a * l);
+#pragma unroll
+            for (int i = 0; i < L::EPL; ++i) acc[i] = fmaf(b, held[w][i][lane], a * acc[i]);
+            m = mx;
+        }
+    }
+    if (it.slot < 0) {
+        const float inv = l > 0.f ? 1.f / l : 0.f;
+#pragma unroll
+        for (int i = 0; i < L::EPL; ++i) acc[i] *= inv;
+        store_row<T, H, D>(o + (size_t)it.row * L::C, lane, acc);
+        if (lane % L::LPH == 0) lse[(size_t)it.row * H + head] = l > 0.f ? m + log2f(l) : 0.f;
+    } else {
+        store_row_ws<T, H, D>(ws_acc + (size_t)it.slot * L::C, lane, acc);
+        if (lane % L::LPH == 0) {
+            ws_ml[((size_t)it.slot * H + head) * 2] = m;
+            ws_ml[((size_t)it.slot * H + head) * 2 + 1] = l;
+        }
+    }
+}
+
 // The scratch of the two backward kernels: (p, ds) of the edges, or in bfloat16 without a bias (lse, delta) of the rows
 inline int64_t scratch_bytes(const bpt_plan *Pin, const bpt_plan *Pout, int h, int dtype, bool biased) {
     if (dtype == BPT_BF16 && !biased) return round16(std::max(Pin->n_rows, Pout->n_index_nodes) * h * 8);
@@ -74,8 +163,14 @@ inline int64_t split_bytes(const bpt_plan *Pin, int h) { return round16(Pin->n_s
 inline ScoreMod make_mod(const bpt_score *sc, float scale, bool entries_are_keys, float *part) {
     ScoreMod m{};
     if (sc->cap > 0.f) {
-        m.to_tanh = scale / sc->cap;
+        const double to = (double)scale / sc->cap, w = to * to;
+        m.to_tanh = (float)to;
         m.from_tanh = sc->cap * LOG2E;
+        m.c[0] = (float)(-0.333331435918808 * w);
+        m.c[1] = (float)(0.13325878977775574 * w * w);
+        m.c[2] = (float)(-0.05304549261927605 * w * w * w);
+        m.c[3] = (float)(0.01724148355424404 * w * w * w * w);
+        m.far = (float)(0.25 / w);
     }
     m.slopes = sc->slopes;
     m.pos_member = entries_are_keys ? sc->pos_q : sc->pos_k;
@@ -106,6 +201,17 @@ int run_forward(const bpt_plan *P, const bpt_score *sc, const void *q, const voi
     constexpr int D = 64, HW = 4;
     float *ws_acc = (float *)ws, *ws_ml = ws_acc ? ws_acc + (size_t)P->n_slots * H * D : nullptr;
     const ScoreMod md = make_mod(sc, scale, true, nullptr);
+    if (P->n_groups == 0) {
+        auto rows = [&](auto nw) {
+            hipLaunchKernelGGL((k_score_fwd_rows<T, H, D, FAST_BATCH, nw()>), dim3(nw() == 1 ? grid_for(P) : (int)P->n_items), dim3(nw() == 1 ? BLOCK : nw() * WAVE), 0,
+                               s, *P, (const T *)q, (const T *)k, (const T *)v, (T *)o, lse, ws_acc, ws_ml, scale * LOG2E, md);
+        };
+        switch (row_parts(P, H * D)) {
+        case 8: rows(std::integral_constant<int, 8>{}); break;
+        case 4: rows(std::integral_constant<int, 4>{}); break;
+        default: rows(std::integral_constant<int, 1>{}); break;
+        }
+    } else
     pick(drop.thr != 0, bias != nullptr, tile_parts(P, H, sizeof(T)), [&](auto dr, auto bi, auto sp) {
         const dim3 grid((unsigned)(group_grid(P) * (H * sp() / HW))), block(HW * WAVE);
         if constexpr (sizeof(T) == 4)
@@ -237,7 +343,8 @@ int run_backward_narrow(const bpt_plan *Pin, const bpt_plan *Pout, const bpt_sco
     return launch_status();
 }
 
-inline int check_score(const bpt_plan *P, const bpt_score *sc, int heads, int d, int h, int dtype, float dropout_p, const float *bias, Narrow &nw) {
+inline int check_score(const bpt_plan *P, const bpt_score *sc, int heads, int d, int h, int dtype, float scale, float dropout_p, const float *bias,
+                       Narrow &nw, bool rows_too) {
     const int st = check_plan(P, true);
     if (st != BPT_OK) return st;
     if (!sc) return BPT_ERR_NULL;
@@ -247,9 +354,10 @@ inline int check_score(const bpt_plan *P, const bpt_score *sc, int heads, int d,
     const bool narrow = heads != h || d != 64;
     if (narrow && (dtype != BPT_F32 || bias || heads > h || d < 4 || d > 64)) return BPT_ERR_UNSUPPORTED;
     nw = narrow ? Narrow{d, heads, h, (heads + NARROW_HW - 1) / NARROW_HW} : Narrow{};
-    if (!(sc->cap >= 0.f && sc->cap <= 3.0e38f) || !(dropout_p >= 0.f && dropout_p < 1.f)) return BPT_ERR_SIZE;
+    if (!(sc->cap >= 0.f && sc->cap <= 3.0e38f) || (sc->cap > 0.f && !(fabsf(scale) <= 1.0e4f * sc->cap)) || !(dropout_p >= 0.f && dropout_p < 1.f)) return BPT_ERR_SIZE;
     if (sc->slopes && (!sc->pos_q || !sc->pos_k)) return BPT_ERR_NULL;
-    if (P->n_rows == 0 || P->n_groups == 0) return P->n_edges == 0 ? BPT_OK : BPT_ERR_UNSUPPORTED;
+    if (P->n_rows == 0) return P->n_edges == 0 ? BPT_OK : BPT_ERR_UNSUPPORTED;
+    if (rows_too && P->n_groups == 0 && !narrow && !bias && !(dropout_p > 0.f)) return BPT_OK;
     if (!has_tiles(P, h, 64, dtype == BPT_BF16 ? 2 : 4)) return BPT_ERR_UNSUPPORTED;
     if ((bias || dropout_p > 0.f || narrow) && !P->grp_eids) return BPT_ERR_PLAN;
     if (bias && P->bias_by_pair) return BPT_ERR_PLAN;
@@ -291,10 +399,9 @@ int bpt_score_forward(const bpt_plan *plan_in, const bpt_score *score, const voi
                       void *workspace, int64_t workspace_bytes, float scale, float dropout_p, uint64_t dropout_seed, int heads, int d, int h, int dtype,
                       void *stream) {
     Narrow nw;
-    const int st = check_score(plan_in, score, heads, d, h, dtype, dropout_p, bias, nw);
+    const int st = check_score(plan_in, score, heads, d, h, dtype, scale, dropout_p, bias, nw, true);
     if (st != BPT_OK) return st;
     if (plan_in->n_rows == 0) return BPT_OK;
-    if (plan_in->n_groups == 0) return BPT_ERR_UNSUPPORTED;
     if (!q || !k || !v || !o || !lse) return BPT_ERR_NULL;
     if (!aligned16(workspace) || (nw.heads == 0 && !on16({q, k, v, o}))) return BPT_ERR_UNSUPPORTED;
     const int64_t need = bpt_score_forward_workspace_bytes(plan_in, h);
@@ -311,7 +418,7 @@ int bpt_score_backward(const bpt_plan *plan_in, const bpt_plan *plan_out, const 
                        void *workspace, int64_t workspace_bytes, float scale, float dropout_p, uint64_t dropout_seed, int heads, int d, int h, int dtype,
                       void *stream) {
     Narrow nw;
-    int st = check_score(plan_in, score, heads, d, h, dtype, dropout_p, bias, nw);
+    int st = check_score(plan_in, score, heads, d, h, dtype, scale, dropout_p, bias, nw, false);
     if (st != BPT_OK) return st;
     st = check_plan(plan_out, true);
     if (st != BPT_OK) return st;

@@ -314,6 +314,100 @@ template <int LPH> __device__ __forceinline__ float head_sum(float x) {
 // save registers and waits for every load separately.
 __device__ __forceinline__ void issue_loads_first() { __builtin_amdgcn_sched_barrier(0); }
 
+// ---- a node row over the lanes of a wavefront (the kernels that walk single rows) ----
+template <typename T, int H_, int D_> struct Lay {
+    static constexpr int H = H_, D = D_, C = H_ * D_;
+    static constexpr int LPH = 64 / H_;                 // lanes per head
+    static constexpr int EPL = C / 64;                  // elements per lane (all of one head)
+    static constexpr int VE = 16 / (int)sizeof(T);      // elements per 16-byte vector
+    static constexpr int NV = EPL / VE;                 // 16-byte vectors per lane
+    static_assert(64 % H_ == 0 && C % 64 == 0 && EPL % VE == 0 && NV >= 1, "unsupported fast shape");
+    static_assert(LPH >= 4, "the row-group kernels broadcast per-member values inside quads of one head");
+    static_assert(D_ == NV * LPH * VE, "layout does not tile the head");
+    // element offset inside a node row of vector i of `lane`: LPH consecutive lanes cover
+    // LPH*16 contiguous bytes of their head
+    static __device__ __forceinline__ int off(int lane, int i) { return (lane / LPH) * D + (i * LPH + lane % LPH) * VE; }
+};
+
+template <typename T, int H, int D>
+__device__ __forceinline__ void load_row(const T *__restrict__ row, int lane, float (&out)[Lay<T, H, D>::EPL]) {
+    using L = Lay<T, H, D>;
+#pragma unroll
+    for (int i = 0; i < L::NV; ++i) {
+        if constexpr (sizeof(T) == 4) {
+            const float4 v = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(row) + L::off(lane, i));
+            out[4 * i] = v.x; out[4 * i + 1] = v.y; out[4 * i + 2] = v.z; out[4 * i + 3] = v.w;
+        } else {
+            const uint4 v = *reinterpret_cast<const uint4 *>(reinterpret_cast<const uint16_t *>(row) + L::off(lane, i));
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                out[8 * i + 2 * c] = __uint_as_float(w[c] << 16);
+                out[8 * i + 2 * c + 1] = __uint_as_float(w[c] & 0xffff0000u);
+            }
+        }
+    }
+}
+
+template <typename T, int H, int D>
+__device__ __forceinline__ void store_row(T *__restrict__ row, int lane, const float (&in)[Lay<T, H, D>::EPL]) {
+    using L = Lay<T, H, D>;
+#pragma unroll
+    for (int i = 0; i < L::NV; ++i) {
+        if constexpr (sizeof(T) == 4) {
+            *reinterpret_cast<float4 *>(reinterpret_cast<float *>(row) + L::off(lane, i)) =
+                make_float4(in[4 * i], in[4 * i + 1], in[4 * i + 2], in[4 * i + 3]);
+        } else {
+            uint32_t w[4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                w[c] = (uint32_t)f32_to_bf16(in[8 * i + 2 * c]) | ((uint32_t)f32_to_bf16(in[8 * i + 2 * c + 1]) << 16);
+            *reinterpret_cast<uint4 *>(reinterpret_cast<uint16_t *>(row) + L::off(lane, i)) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    }
+}
+
+// f32 partial rows in the workspace are stored in natural column order (the combine kernels
+// index them by column), whatever the element type of the node tensors
+template <typename T, int H, int D>
+__device__ __forceinline__ void store_row_ws(float *__restrict__ row, int lane, const float (&in)[Lay<T, H, D>::EPL]) {
+    using L = Lay<T, H, D>;
+#pragma unroll
+    for (int i = 0; i < L::NV; ++i)
+#pragma unroll
+        for (int c = 0; c < L::VE / 4; ++c)
+            *reinterpret_cast<float4 *>(row + L::off(lane, i) + 4 * c) =
+                make_float4(in[L::VE * i + 4 * c], in[L::VE * i + 4 * c + 1], in[L::VE * i + 4 * c + 2], in[L::VE * i + 4 * c + 3]);
+}
+
+template <int N> __device__ __forceinline__ float dot_n(const float (&a)[N], const float (&b)[N]) {
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) s = fmaf(a[i], b[i], s);
+    return s;
+}
+
+// NW wavefronts (a workgroup) share an item: each takes whole batches of its edges, as many as the others, and the sums meet in
+// LDS.  False: no such item (the whole workgroup).  parts: how many wavefronts have edges (one at least).
+template <int NW, int BATCH> __device__ __forceinline__ bool fetch_item_part(const bpt_plan &P, Item &it, int &part, int &parts) {
+    part = 0;
+    parts = 1;
+    if constexpr (NW == 1) return fetch_item(P, it);
+    const int w = xcd_contiguous_block();
+    if (w >= (int)P.n_items) return false;
+    const int4 v = reinterpret_cast<const int4 *>(P.items)[w];
+    it.row = __builtin_amdgcn_readfirstlane(v.x);
+    it.begin = __builtin_amdgcn_readfirstlane(v.y);
+    it.end = __builtin_amdgcn_readfirstlane(v.z);
+    it.slot = __builtin_amdgcn_readfirstlane(v.w);
+    const int deg = it.end - it.begin, per = (deg + NW * BATCH - 1) / (NW * BATCH) * BATCH;
+    part = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    parts = max(1, (deg + max(per, 1) - 1) / max(per, 1));
+    it.begin = min(it.begin + part * per, it.end);
+    it.end = min(it.begin + per, it.end);
+    return true;
+}
+
 // Combine the (m, l, acc) partials of each split row.  Grid (n_heavy, C / 64): one block per split row
 // and 64-column strip; wave w folds slots w, w+4, ... with a running maximum (one pass, eight
 // independent loads per step), then the four wave results are merged in wave order.
@@ -868,6 +962,7 @@ __device__ __forceinline__ void tile_walk_first_ahead(int nblk, IssueFirst &&fir
 // travels with the block's rows and reaches the lanes through LDS, and nothing of an edge's size is read or written.
 struct ScoreMod {
     float to_tanh, from_tanh;          // scale / cap, and cap in base-2 units; to_tanh 0: not capped
+    float c[4], far;                   // tile_mod_scores: the polynomial's coefficients and bound for x^2
     const float *slopes;               // (heads), or null: no distance
     const float *pos_member, *pos_entry;       // positions of the plan's rows, of the rows its indices name
     float *part;                       // destination side: [group][head][part] sums of dL/ds |pos - pos|, or null
@@ -877,38 +972,34 @@ struct NoMod {};
 template <bool MOD> struct ModArg { typedef NoMod type; };
 template <> struct ModArg<true> { typedef ScoreMod type; };
 
-// tanh of the block's four u, and 1 - tanh^2.  |u| <= 1/2, where nearly all scores lie (u is a score of a few units over a cap of tens): odd
-// polynomial, u + u w (c0 + c1 w + c2 w^2 + c3 w^3) with w = u^2, fitted by weighted least squares to the relative error, 1.5e-8 (1.25 half steps
-// of float32 as evaluated); a wavefront without a larger |u| evaluates nothing else.  Beyond, (1 - e) / (1 + e) with e = exp(-2 |u|), whose
-// difference keeps its digits there.  (1 - e) / (1 + e) everywhere costs less for large |u| but is off by 2^-24 absolutely, which times a
-// cap of 50 is more than all other roundings of a score.
-__device__ __forceinline__ float tile_tanh_small(float u) {
-    const float w = u * u;
-    const float p = fmaf(fmaf(fmaf(0.01724148355424404f, w, -0.05304549261927605f), w, 0.13325878977775574f), w, -0.333331435918808f);
-    return fmaf(u, w * p, u);
-}
-// s (base-2 units) and ds/du of the pairs whose q.k (+ term) is x; pos_e: positions of the pairs' entries
+// s (base-2 units) and ds/du of four pairs whose q.k (+ term) is x; pos_e: positions of the pairs' entries.
+// |u / cap| <= 1/2, where nearly all scores lie (a score is a few units, a cap tens): tanh z = z + z w (c0 + c1 w + c2 w^2 + c3 w^3) with w = z^2,
+// fitted by weighted least squares to the relative error, 1.5e-8 (1.25 half steps of float32 as evaluated); the factor scale / cap sits in the
+// coefficients, cap in the scaled score, and a wavefront without a larger score evaluates nothing else.  Beyond, (1 - e) / (1 + e) with
+// e = exp(-2 |z|), whose difference keeps its digits there; for small z it is off by 2^-24 absolutely, which times a cap of 50 is more than all other
+// roundings of a score.
 __device__ __forceinline__ void tile_mod_scores(const ScoreMod &md, float scale_log2e, float slope_log2e, float pos_m, const float (&pos_e)[4],
                                                 const float (&x)[4], float (&s)[4], float (&du)[4]) {
     if (md.to_tanh != 0.f) {
-        float u[4], t[4];
+        float w[4];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) u[r] = x[r] * md.to_tanh;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) t[r] = tile_tanh_small(u[r]);
-        const float top = fmaxf(fmaxf(fabsf(u[0]), fabsf(u[1])), fmaxf(fabsf(u[2]), fabsf(u[3])));
-        if (__builtin_amdgcn_ballot_w64(top > 0.5f) != 0) {
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const float e = __builtin_amdgcn_exp2f(fabsf(u[r]) * (-2.f * LOG2E));
-                const float far = copysignf((1.f - e) * __builtin_amdgcn_rcpf(1.f + e), u[r]);
-                t[r] = fabsf(u[r]) > 0.5f ? far : t[r];
-            }
-        }
+        for (int r = 0; r < 4; ++r) w[r] = x[r] * x[r];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            s[r] = t[r] * md.from_tanh;
-            du[r] = fmaf(-t[r], t[r], 1.f);
+            const float wp = w[r] * fmaf(fmaf(fmaf(md.c[3], w[r], md.c[2]), w[r], md.c[1]), w[r], md.c[0]);
+            const float xs = x[r] * scale_log2e, t = x[r] * md.to_tanh;
+            s[r] = fmaf(xs, wp, xs);
+            const float th = fmaf(t, wp, t);
+            du[r] = fmaf(-th, th, 1.f);
+        }
+        if (__builtin_amdgcn_ballot_w64(fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3])) > md.far) != 0) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float e = __builtin_amdgcn_exp2f(fabsf(x[r] * md.to_tanh) * (-2.f * LOG2E));
+                const float th = copysignf((1.f - e) * __builtin_amdgcn_rcpf(1.f + e), x[r] * md.to_tanh);
+                s[r] = w[r] > md.far ? th * md.from_tanh : s[r];
+                du[r] = w[r] > md.far ? fmaf(-th, th, 1.f) : du[r];
+            }
         }
     } else {
 #pragma unroll
@@ -1778,7 +1869,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP 
 // the source side is handed delta.  One more product a block over the K rows at hand.  dq of a split row keeps delta' (it has many pairs, each with a
 // small p); its segments leave their sums, from which k_score_split forms the other two before the source side runs.
 template <int H, int D, int HW, int WPE, bool DROP, int BIAS, bool PDS, int SP, bool MOD = false>
-__global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(MOD && (DROP || BIAS) ? WPE - 2 : DROP || BIAS || MOD ? WPE - 1 : WPE))) void k_attn_bwd_dst_rows_bf16(
+__global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(MOD ? WPE - 2 : DROP || BIAS ? WPE - 1 : WPE))) void k_attn_bwd_dst_rows_bf16(
     bpt_plan P, const bf16_t *__restrict__ q, const bf16_t *__restrict__ k, const bf16_t *__restrict__ v, const bf16_t *__restrict__ o,
     const bf16_t *__restrict__ d_o, const float *__restrict__ lse, bf16_t *__restrict__ dq, uint32_t *__restrict__ pds,
     float2 *__restrict__ stat, float *__restrict__ ws_dq, float scale, float scale_log2e, uint32_t drop_thr, uint32_t drop_seed, float drop_inv,
@@ -2319,7 +2410,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(WPE))
 // columns with dropout lost 2 %: heads of fewer than 64 columns keep the scratch.)  float32 keeps it too: there the two
 // products are 1024 cycles of the matrix pipeline per block.  122 registers: compiled for four wavefronts per SIMD.
 template <int H, int D, int HW, int WPE, bool DROP, int SP = 1, bool MOD = false>
-__global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(MOD && DROP ? WPE - 1 : WPE))) void k_attn_bwd_src_tile_bf16_again(
+__global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(MOD ? WPE - 1 : WPE))) void k_attn_bwd_src_tile_bf16_again(
     bpt_plan P, const bf16_t *__restrict__ q, const bf16_t *__restrict__ k, const bf16_t *__restrict__ v, const bf16_t *__restrict__ d_o,
     const float2 *__restrict__ stat, bf16_t *__restrict__ dk, bf16_t *__restrict__ dv, float *__restrict__ ws_dk, float *__restrict__ ws_dv,
     float scale, float scale_log2e, uint32_t drop_thr, uint32_t drop_seed, float drop_inv, typename ModArg<MOD>::type md) {
@@ -2554,6 +2645,30 @@ inline int tile_parts(const bpt_plan *P, int heads, size_t elem, bool plain_forw
 inline Narrow narrow_parts(Narrow nw, int parts) {
     if (parts > 1) nw.slices = nw.heads;
     return nw;
+}
+
+constexpr int FAST_BATCH = 4;
+// Wavefronts a work item for the kernels that walk single rows.  The fused kernels walk them on graphs of fewer than 1536 items (with
+// row groups switched off: on any), the separate operators' SpMM where it is handed a plan without groups.  There a launch lasts
+// as long as its longest item: 16 batches of four edges one after the other, each a round trip to memory.  Forward / destination
+// side / source side, one -> four -> eight wavefronts an item, 8 x 64 float32 unless said otherwise, us:
+//   127 items (L = 64)                  9.4 / 13.7 / 7.2  -> 4.7 / 6.4 / 4.2   -> 4.8 / 5.6 / 4.2;   SpMM 7.5 -> 4.0 -> 3.8
+//   539 (L = 256, k = 16)              11.1 / 16.6 / 14.4 -> 9.2 / 11.7 / 11.6 -> 8.2 / 9.4 / 10.8;  bfloat16 12.2 / 16.9 / 15.5 -> 6.0 / 7.3 / 7.4 -> 5.6 / 6.6 / 7.4
+//   816 (L = 400)                      11.4 / 16.6 / 13.8 -> 7.9 / 10.0 / 11.0 -> 9.0 / 10.4 / 10.5; SpMM 10.8 -> 6.7 -> 6.7
+//   1434 (L = 700, k = 1)              15.7 / 21.2 / 15.0 -> 10.1 / 12.0 / 12.2 -> 11.3 / 12.8 / 12.6; SpMM 11.6 -> 7.9 -> 7.1
+//   2050 (L = 1000, k = 1, no groups)  16.8 / 22.2 / 17.9 -> 11.0 / 14.0 / 13.6 -> 14.1 / 17.0 / 15.4; SpMM 11.6 -> 8.4 -> 8.2
+// Larger launches fill the GPU with a wavefront an item.  Rows of 1024 columns take twice the registers and the LDS: eight
+// wavefronts an item of them are one round of the chip up to 256 items, beyond it four are faster.  16 x 64:
+//   268 (L = 130, k = 4)               16.3 / 22.7 / 16.7 -> 7.9 / 10.4 / 9.3   -> 8.2 / 10.2 / 9.4;   bfloat16 16.4 / 21.3 / 19.6 -> 7.6 / 9.6 / 8.7 -> 8.3 / 8.7 / 11.4
+//   324 (L = 160, k = 4)               15.7 / 22.1 / 18.1 -> 8.5 / 10.2 / 13.1  -> 10.2 / 12.0 / 12.6; bfloat16 16.0 / 20.7 / 19.8 -> 7.6 / 9.6 / 11.5 -> 10.5 / 10.8 / 12.2
+//   585 (L = 256, k = 16, both ways)   18.7 / 26.8 / 23.4 -> 18.6 / 21.2 / 19.4 -> 22.3 / 24.3 / 21.2
+// A float32 forward of 512 columns or more that already has a wavefront for each of the 1024 SIMDs and 25 edges or more an
+// item waits for the rate of its loads, not for one item: one -> four, 8 x 64 and 16 x 64, 983 items of 25 790 edges 11.7 -> 12.4 and 19.1 ->
+// 21.0; 957 of 32 613 12.0 -> 12.2 and 19.7 -> 20.4; (1018 of 23 540 11.3 -> 11.2 and 18.2 -> 18.7; 756 items 11.2 -> 10.4 and 18.6 -> 17.1).
+inline int row_parts(const bpt_plan *P, int columns, bool forward_f32 = false) {
+    if (P->n_items <= (columns > 512 ? 288 : 640)) return 8;
+    if (forward_f32 && columns >= 512 && P->n_items > 800 && P->n_items <= 1024 && P->n_edges >= 25000) return 1;
+    return P->n_items <= 2048 ? 4 : 1;
 }
 
 }  // namespace

@@ -1246,7 +1246,7 @@ class Score(collections.namedtuple("Score", "cap slopes pos_q pos_k")):
     __slots__ = ()
 
 
-def score_options(score_cap, slopes, pos, q, k):
+def score_options(score_cap, slopes, pos, q, k, scale):
     """Score of bpt_attention's arguments, checked, or None where none is given."""
     if score_cap is None and slopes is None and pos is None:
         return None
@@ -1255,6 +1255,8 @@ def score_options(score_cap, slopes, pos, q, k):
         cap = float(score_cap)
         if not (0.0 < cap <= 3.0e38):
             raise ValueError("score_cap must be a finite positive number")
+        if not abs(scale) <= 1.0e4 * cap:
+            raise ValueError("score_cap must be at least |scale| / 10^4")
     if (slopes is None) != (pos is None):
         raise ValueError("slopes and pos go together")
     if slopes is None:
@@ -1297,6 +1299,23 @@ def score_supported(eid_c, q, k):
             and max(q.size(0), k.size(0)) * shape[0] * 64 * q.element_size() < 2 ** 32)
 
 
+SCORE_ROWS = None            # testing / measurement hook: True / False force the forward of few rows on / off the kernel that walks single rows
+
+
+def _score_rows(eid_c, q, dropout_p, bias, train):
+    """Whether a forward without a backward walks single rows (a decoder's tokens) instead of tiles, whose wavefronts walk a row's neighbours in one chain.
+    Rows of n edges each, tiles / single rows, us, 8 heads float32 and 16 heads bfloat16:
+      n = 256    1 row 7.5 / 7.4 and 5.4 / 9.1;   8 rows 7.6 / 7.5 and 5.4 / 9.0
+      n = 2048   1 row 49 / 7.7 and 25 / 9.2;     4 rows 27 / 7.7 and 16 / 9.3;    8 rows 15 / 8.2 and 9.9 / 9.6;   16 rows 10.2 / 10.9 and 7.8 / 12.8
+      n = 8192   1 row 91 / 11 and 44 / 12;       4 rows 28 / 14 and 16 / 15;      8 rows 18 / 18 and 11 / 22;      16 rows 13 / 27 and 11 / 33"""
+    if train or dropout_p > 0.0 or bias is not None or score_padded_shape(q) != _hd(q):
+        return False
+    if SCORE_ROWS is not None:
+        return SCORE_ROWS
+    rows, edges = q.size(0), eid_c.size(0)
+    return edges >= 384 * rows and (rows <= 4 or (rows <= 8 and edges <= 4096 * rows))
+
+
 def _score_plan_in(graph, q, k, built=None):
     col, indptr_c, eid_c, indices_c = graph[4:]
     return plan_cache.get(col, indptr_c, eid_c, indices_c, q.size(0), k.size(0), seg_len=_tile_seg_of(eid_c.size(0), q.size(0), k.size(0)),
@@ -1330,11 +1349,12 @@ def prepare_score(graph, q, k, dropout_p, train):
         sides = [(*graph[4:], q.size(0), k.size(0), seg, None), (*graph[:4], k.size(0), q.size(0), seg, _plan.tile_order_src(k.size(0), graph[2].size(0)))]
         if plan_cache.may_hold(sides):
             plans = plan_cache.put_tile_plans(sides) or plans
-    pi = _score_plan_in(graph, q, k, plans[0])
+    few = _score_rows(graph[6], q, dropout_p, None, train)
+    pi = plan_cache.get(*graph[4:], q.size(0), k.size(0), prefer_device=True) if few else _score_plan_in(graph, q, k, plans[0])
     if not pi.covers_all_edges:
         return False
     numbers = [q.size(0), k.size(0), score_padded_shape(q)[0], q.size(2), _dtype(q), int(dropout_p > 0.0), q.size(1)]
-    in_struct = pi.ensure_groups(TILE_ROWS)["struct"]
+    in_struct = pi.struct if few else pi.ensure_groups(TILE_ROWS)["struct"]
     plan_cache.remember((pi,), generation, _native.SCORE_FWD, list(graph[4:]), numbers, ctypes.addressof(in_struct), 0)
     if train:
         po = _score_plan_out(graph, q, k, plans[1])
@@ -1370,17 +1390,18 @@ def _check_score_call(graph, q, k, v, score, bias):
     return h
 
 
-def score_attention_forward(col, indptr_c, eid_c, indices_c, q, k, v, score, scale=None, dropout_p=0.0, seed=0, bias=None):
+def score_attention_forward(col, indptr_c, eid_c, indices_c, q, k, v, score, scale=None, dropout_p=0.0, seed=0, bias=None, train=True):
     """(o, lse) as attention_forward's, of scores u = (q[dst].k[src] + bias[e]) scale that become score.cap tanh(u / score.cap) -
     score.slopes[head] |pos_q[dst] - pos_k[src]| (a Score).  Shapes that score_reads() takes; lse has the heads of score_padded_shape(); bias by
-    edge id."""
+    edge id.  train=False: there is no backward to come, few rows are walked one by one."""
     graph = (None,) * 4 + (col, indptr_c, eid_c, indices_c)
     h = _check_score_call(graph, q, k, v, score, bias)
     scale = 1.0 / math.sqrt(q.size(2)) if scale is None else float(scale)
-    plan = _score_plan_in(graph, q, k)
+    few = _score_rows(graph[6], q, dropout_p, bias, train)
+    plan = plan_cache.get(*graph[4:], q.size(0), k.size(0), prefer_device=True) if few else _score_plan_in(graph, q, k)
     if not plan.covers_all_edges:
         raise RuntimeError("attention with score options needs units that cover every edge")
-    ref = ctypes.byref(plan.ensure_groups(TILE_ROWS)["struct"])
+    ref = ctypes.byref(plan.struct if few else plan.ensure_groups(TILE_ROWS)["struct"])
     o = torch.empty_like(q)
     lse = torch.empty((q.size(0), h), dtype=torch.float32, device=q.device)
     nws = _SCORE_LIB.bpt_score_forward_workspace_bytes(ref, h)

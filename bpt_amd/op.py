@@ -195,7 +195,7 @@ class BPTScoreAttention(Function):
 
     @staticmethod
     def forward(ctx, row, indptr_r, eid_r, indices_r, col, indptr_c, eid_c, indices_c, q, k, v, slopes, score, scale, dropout_p, seed):
-        o, lse = _g.score_attention_forward(col, indptr_c, eid_c, indices_c, q, k, v, score, scale, dropout_p, seed)
+        o, lse = _g.score_attention_forward(col, indptr_c, eid_c, indices_c, q, k, v, score, scale, dropout_p, seed, train=any(ctx.needs_input_grad))
         ctx.save_for_backward(row, indptr_r, eid_r, indices_r, col, indptr_c, eid_c, indices_c, q, k, v, o, lse, *score[1:])
         ctx.cap, ctx.scale, ctx.dropout_p, ctx.seed = score.cap, scale, dropout_p, seed
         return o
@@ -483,7 +483,7 @@ def bpt_attention(row, indptr_r, eid_r, indices_r, col, indptr_c, eid_c, indices
     scale = 1.0 / math.sqrt(q.size(-1)) if scale is None else float(scale)
     if (rel_table is None) != (etype is None):
         raise ValueError("rel_table and etype go together")
-    score = _g.score_options(score_cap, slopes, pos, q, k)
+    score = _g.score_options(score_cap, slopes, pos, q, k, scale)
     if score is not None:
         return _score_attention((row, indptr_r, eid_r, indices_r, col, indptr_c, eid_c, indices_c), q, k, v, scale, fused, dropout_p, seed, rel_table, etype,
                                 score)

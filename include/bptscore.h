@@ -4,7 +4,8 @@
  *   s = cap tanh(u / cap)   (s = u where cap is 0)   - slopes[head] |pos_q[dst] - pos_k[src]|   (where slopes is given)
  * in place of u.  Heads of 64 columns; float32 with 4, 8 or 16 of them, bfloat16 with 8 or 16; float32 without a bias also heads of 4 to 64 columns as
  * they are, `heads` of them, computed as h = 4, 8 or 16 (h is what lse (n, h), the workspace and dropout's hash count).  Plans carry groups of 16 rows
- * (tiles), the source side's the pair numbers of the destination side's; grp_eids where there is dropout or a bias.  Conventions, status codes,
+ * (tiles), the source side's the pair numbers of the destination side's; grp_eids where there is dropout or a bias.  A forward on a plan without
+ * groups walks single rows (heads of 64 columns, no dropout, no bias): few rows of many edges.  Conventions, status codes,
  * plans, bias, ds_out, dropout and lse are those of bptattn.h (bias by edge id: bias_by_pair is refused).  Deterministic; nothing is allocated.
  */
 #ifndef BPTSCORE_H
@@ -19,7 +20,7 @@ extern "C" {
 #endif
 
 typedef struct {
-    float cap;                        /* 0: not capped; finite and positive otherwise */
+    float cap;                        /* 0: not capped; otherwise finite and at least |scale| / 10^4 */
     const float *slopes;              /* (heads) float32, or NULL: no distance */
     const float *pos_q, *pos_k;       /* float32 positions of the query rows and of the key rows, with slopes */
 } bpt_score;

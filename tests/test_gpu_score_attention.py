@@ -360,6 +360,8 @@ def test_refusals():
     for cap in (0.0, -1.0, float("inf"), float("nan")):
         with pytest.raises(ValueError, match="score_cap"):
             go(score_cap=cap)
+    with pytest.raises(ValueError, match="at least"):
+        go(score_cap=1e-6)
     with pytest.raises(ValueError, match="go together"):
         go(slopes=dev["slopes"])
     with pytest.raises(ValueError, match="go together"):

@@ -415,6 +415,7 @@ template <typename T> inline int norm_parts(int64_t rows, int64_t cols) {
     if (cols > norm_longest<T>()) return (int)std::min<int64_t>(NORM_PARTS_LONG, std::max<int64_t>(rows, 1));
     const NormShape s = norm_shape(cols, cols < norm_ve<T>() ? 1 : norm_ve<T>());
     const int64_t slots = NORM_BLOCK / s.tpr;
+    if (rows <= 2 * slots) return 1;                             // (no partial sums, one launch less)
     return (int)std::min<int64_t>(NORM_PARTS, std::max<int64_t>((rows + slots - 1) / slots, 1));
 }
 

@@ -172,7 +172,7 @@ std::tuple<Tensor, Tensor> relu8_backward(const Tensor &dy, const Tensor &codes,
 
 void check_relu_linear(const Tensor &a, const Tensor &w, const Tensor &b, double p) {
     check_relu8(a, p, "a");
-    TORCH_CHECK_VALUE(a.dim() >= 1, "a must have an axis");
+    TORCH_CHECK_VALUE(a.dim() >= 1 && a.size(-1) >= 1, "a must have a last axis of one element at least");
     check_like(w, a, "weight");
     TORCH_CHECK_VALUE(w.dim() == 2 && w.size(1) == a.size(-1), "weight must be (outputs, ", a.size(-1), "), got ", w.sizes());
     if (b.defined()) {
@@ -181,8 +181,12 @@ void check_relu_linear(const Tensor &a, const Tensor &w, const Tensor &b, double
     }
 }
 
+// the products are of the tensors as they are, also inside autocast (whose results the backward would meet in another type)
+using NoAutocast = c10::impl::ExcludeDispatchKeyGuard;
+
 struct ReluLinear8 : torch::autograd::Function<ReluLinear8> {
     static Tensor forward(AutogradContext *ctx, const Tensor &a, const Tensor &w, const Optional &b, double p, int64_t seed) {
+        const NoAutocast as_it_is(c10::DispatchKey::AutocastCUDA);
         const auto [y, codes, exps] = relu8_forward(a, p, (uint64_t)seed);
         ctx->save_for_backward({codes, exps, w});
         ctx->saved_data["p"] = p;
@@ -192,6 +196,7 @@ struct ReluLinear8 : torch::autograd::Function<ReluLinear8> {
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
         TORCH_CHECK(!at::GradMode::is_enabled(), "relu_linear8 is not differentiable twice");
         if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+        const NoAutocast as_it_is(c10::DispatchKey::AutocastCUDA);
         const auto t = ctx->get_saved_variables();
         const Tensor &codes = t[0], &exps = t[1], &w = t[2];
         const double p = ctx->saved_data["p"].toDouble();
@@ -222,6 +227,7 @@ Tensor relu_linear8(const Tensor &a, const Tensor &weight, const Optional &bias,
     const Tensor b = bias.value_or(Tensor());
     check_relu_linear(a, weight, b, p);
     if (differentiated({&a, &weight, &b})) return ReluLinear8::apply(a, weight, bias, p, (int64_t)seed);
+    const NoAutocast as_it_is(c10::DispatchKey::AutocastCUDA);
     if (p == 0.0) return at::linear(at::relu(a), weight, bias);     // (nothing to keep)
     return at::linear(std::get<0>(relu8_forward(a, p, seed)), weight, bias);
 }

@@ -19,6 +19,7 @@
 #include <algorithm>
 #include <array>
 #include <atomic>
+#include <cmath>
 #include <cstring>
 #include <memory>
 #include <mutex>
@@ -637,9 +638,12 @@ struct ScoreAttention : torch::autograd::Function<ScoreAttention> {
 // op.BPTScoreAttention of a call whose plans are known, or None
 MaybeTensor score_attention(const MaybeTensor &row, const MaybeTensor &indptr_r, const MaybeTensor &eid_r, const MaybeTensor &indices_r, const Tensor &col,
                             const Tensor &indptr_c, const Tensor &eid_c, const Tensor &indices_c, const Tensor &q, const Tensor &k, const Tensor &v,
-                            const MaybeTensor &slopes, const MaybeTensor &pos_q, const MaybeTensor &pos_k, double cap, double scale, double p, uint64_t seed,
-                            int64_t h) {
-    const ScoreOptions opt{cap, slopes.value_or(Tensor()), pos_q.value_or(Tensor()), pos_k.value_or(Tensor())};
+                            const MaybeTensor &slopes, const MaybeTensor &pos_q, const MaybeTensor &pos_k, std::optional<double> score_cap, double scale, double p,
+                            uint64_t seed, int64_t h) {
+    // (what graphop.score_options refuses is left to it)
+    if (score_cap && !(*score_cap > 0.0 && *score_cap <= 3.0e38 && std::abs(scale) <= 1.0e4 * *score_cap)) return std::nullopt;
+    if ((pos_q && pos_q->requires_grad()) || (pos_k && pos_k->requires_grad())) return std::nullopt;
+    const ScoreOptions opt{score_cap.value_or(0.0), slopes.value_or(Tensor()), pos_q.value_or(Tensor()), pos_k.value_or(Tensor())};
     const Tensor none, &r0 = row ? *row : none, &r1 = indptr_r ? *indptr_r : none, &r2 = eid_r ? *eid_r : none, &r3 = indices_r ? *indices_r : none;
     const bool train = differentiated({&q, &k, &v}) || (opt.slopes.defined() && differentiated({&opt.slopes}));
     const EntryPtr e = train ? score_entry(SCORE_TRAIN, {&col, &indptr_c, &eid_c, &indices_c, &r0, &r1, &r2, &r3}, q, k, v, p, h)

@@ -1247,9 +1247,7 @@ class Score(collections.namedtuple("Score", "cap slopes pos_q pos_k")):
 
 
 def score_options(score_cap, slopes, pos, q, k, scale):
-    """Score of bpt_attention's arguments, checked, or None where none is given."""
-    if score_cap is None and slopes is None and pos is None:
-        return None
+    """Score of bpt_attention's arguments, checked."""
     cap = 0.0
     if score_cap is not None:
         cap = float(score_cap)
@@ -1261,6 +1259,8 @@ def score_options(score_cap, slopes, pos, q, k, scale):
         raise ValueError("slopes and pos go together")
     if slopes is None:
         return Score(cap, None, None, None)
+    if isinstance(pos, (tuple, list)) and len(pos) != 2:
+        raise ValueError("pos must be a tensor or a pair of them: of the query rows and of the key rows")
     pos_q, pos_k = pos if isinstance(pos, (tuple, list)) else (pos, pos)
     for t, n, name in ((slopes, _hd(q)[0], "slopes"), (pos_q, q.size(0), "pos (of the query rows)"), (pos_k, k.size(0), "pos (of the key rows)")):
         _check_input(t, name)

@@ -418,8 +418,26 @@ def _score_chain(graph, q, k, v, scale, dropout_p, rel_table, etype, score):
     return vec_spmm(col, indptr_c, eid_c, indices_c, row, indptr_r, eid_r, indices_r, a.to(v.dtype), v, n_rows=None if q.size(0) == v.size(0) else q.size(0))
 
 
-def _score_attention(graph, q, k, v, scale, fused, dropout_p, seed, rel_table, etype, score):
+def _score_known(graph, q, k, v, scale, dropout_p, seed, score_cap, slopes, pos):
+    """A call with score options whose plans the native host path knows, which checks it there, or None."""
+    if not _native_takes() or _g.force_generic_enabled():
+        return None
+    shape = _g.score_padded_shape(q)
+    pos = tuple(pos) if isinstance(pos, (tuple, list)) else (pos, pos)
+    if shape is None or len(pos) != 2:
+        return None
+    return _native.score_attention(*graph, q, k, v, slopes, *pos, score_cap, scale, dropout_p, seed & (2 ** 64 - 1), shape[0])
+
+
+def _score_attention(graph, q, k, v, scale, fused, dropout_p, seed, rel_table, etype, score_cap, slopes, pos):
     """bpt_attention with score options."""
+    if fused is not False and rel_table is None:
+        if dropout_p > 0 and seed is None:
+            seed = int(torch.randint(0, 2 ** 62, (1,)).item())
+        o = _score_known(graph, q, k, v, scale, float(dropout_p), int(seed or 0), score_cap, slopes, pos)
+        if o is not None:
+            return o
+    score = _g.score_options(score_cap, slopes, pos, q, k, scale)
     train = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, rel_table, score.slopes))
     runs = fused is not False and _native_takes() and _g.score_supported(graph[6], q, k) and (not train or all(t is not None for t in graph[:4]))
     if not runs:
@@ -440,21 +458,19 @@ def _score_attention(graph, q, k, v, scale, fused, dropout_p, seed, rel_table, e
             score = score._replace(slopes=torch.nn.functional.pad(score.slopes, (0, hp - h)))
     elif d == 64:
         q, k, v = (x.clone() if x.data_ptr() % 16 else x for x in (q, k, v))          # (the kernels read 16 bytes a lane)
-    o = None
-    if not rel:
-        native = lambda: _native.score_attention(*graph, q, k, v, *score[1:], score.cap, scale, dropout_p, seed & (2 ** 64 - 1), hp)
-        o = native()
+    known = lambda: None if rel else _score_known(graph, q, k, v, scale, dropout_p, seed, score.cap or None, score.slopes,
+                                                  None if score.slopes is None else score[2:])
+    o = known()
     if o is None:
         if not _g.prepare_score(graph, q, k, dropout_p, train):
             if fused:
                 raise RuntimeError("attention with score options needs units that cover every edge")
             return _score_chain(graph, *given[:3], scale, dropout_p, given[3], etype, given[4])
-        if rel:
-            o = BPTRelAttention.apply(*graph, q, k, v, scale, dropout_p, seed, rel_table, etype, None, False, score, score.slopes)
-        else:
-            o = native()
-            if o is None:                                         # (a cache too small for the plans leaves nothing with the native host path)
-                o = BPTScoreAttention.apply(*graph, q, k, v, score.slopes, score, scale, dropout_p, seed)
+        o = known()
+    if o is None and rel:
+        o = BPTRelAttention.apply(*graph, q, k, v, scale, dropout_p, seed, rel_table, etype, None, False, score, score.slopes)
+    elif o is None:                                               # (a cache too small for the plans leaves nothing with the native host path)
+        o = BPTScoreAttention.apply(*graph, q, k, v, score.slopes, score, scale, dropout_p, seed)
     return o if as_it_is else o[:, :h, :d].contiguous()
 
 
@@ -483,10 +499,9 @@ def bpt_attention(row, indptr_r, eid_r, indices_r, col, indptr_c, eid_c, indices
     scale = 1.0 / math.sqrt(q.size(-1)) if scale is None else float(scale)
     if (rel_table is None) != (etype is None):
         raise ValueError("rel_table and etype go together")
-    score = _g.score_options(score_cap, slopes, pos, q, k, scale)
-    if score is not None:
+    if score_cap is not None or slopes is not None or pos is not None:
         return _score_attention((row, indptr_r, eid_r, indices_r, col, indptr_c, eid_c, indices_c), q, k, v, scale, fused, dropout_p, seed, rel_table, etype,
-                                score)
+                                score_cap, slopes, pos)
     padded = None
     if fused is None:
         fused = _g.attention_supported(q)

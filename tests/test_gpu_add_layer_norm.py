@@ -168,6 +168,23 @@ def test_gradient_against_differences():
     assert torch.autograd.gradgradcheck(lambda *a: op.add_layer_norm(*a), args)
 
 
+def test_gradients_of_some_inputs_only():
+    from bpt_amd import op
+    t = {n: v.to(DEV) for n, v in make((300, 96), torch.float32).items()}
+    names = ("x", "residual", "weight", "bias")
+    full = [t[n].clone().requires_grad_(True) for n in names]
+    want = torch.autograd.grad(op.add_layer_norm(*full), full, t["dy"])
+    for i in range(4):
+        args = [t[n] for n in names]
+        args[i] = args[i].clone().requires_grad_(True)
+        (got,) = torch.autograd.grad(op.add_layer_norm(*args), args[i], t["dy"])
+        assert torch.equal(got, want[i])
+    x = t["x"].clone().requires_grad_(True)                       # (no residual, no weight: the places move up)
+    b = t["bias"].clone().requires_grad_(True)
+    dx, db = torch.autograd.grad(op.add_layer_norm(x, None, None, b), (x, b), t["dy"])
+    assert torch.equal(db, want[3]) and torch.isfinite(dx).all()
+
+
 def test_one_tensor_twice():
     """x is residual too: its gradient is both."""
     from bpt_amd import op

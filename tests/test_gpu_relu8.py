@@ -192,6 +192,19 @@ def test_relu_linear_needs_no_gradient_of_some():
         assert torch.equal(got, want[i])
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_relu_linear_inside_autocast(dtype):
+    """The products are of the tensors as they are."""
+    from bpt_amd import op
+    a, w = (torch.randn(s, device=DEV).to(TYPES[dtype]).requires_grad_(True) for s in ((20, 64), (8, 64)))
+    do = torch.randn(20, 8, device=DEV).to(TYPES[dtype])
+    want = torch.autograd.grad(op.relu_linear8(a, w), (a, w), do)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        out = op.relu_linear8(a, w)
+        got = torch.autograd.grad(out, (a, w), do)
+    assert out.dtype == TYPES[dtype] and all(torch.equal(x, y) for x, y in zip(got, want))
+
+
 def test_replays_of_a_captured_pair_match_the_eager_one():
     from bpt_amd import graphop
     a, dy = make(50000, "f32"), make(50000, "f32", 1)
@@ -230,6 +243,8 @@ def test_refusals():
         graphop.relu8_backward(a, codes, exps[:2].contiguous())
     with pytest.raises(ValueError, match="uint8"):
         graphop.relu8_backward(a, exps, exps)
+    with pytest.raises(ValueError, match="last axis"):
+        op.relu_linear8(a[:, :0].contiguous(), torch.randn(8, 0, device=DEV))
     with pytest.raises(ValueError, match="weight must be"):
         op.relu_linear8(a, torch.randn(8, 32, device=DEV))
     w = torch.randn(8, 64, device=DEV, requires_grad=True)

@@ -196,6 +196,47 @@ def test_a_graph_that_fills_the_chip(dtype):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_tiles_in_two_parts_and_long_rows(dtype):
+    """About 2056 wavefronts of five blocks: two wavefronts a tile; the last row has 4096 edges, in many segments."""
+    check(make(("window", 4096, 64), 8, 64, dtype, 30.0, True), fused=True)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_plans_built_on_the_host(dtype):
+    from bpt_amd import plan
+    old = plan.set_device_build(False)
+    try:
+        check(make(("bpt", 400, 4), 8, 64, dtype, 30.0, True), fused=True)
+    finally:
+        plan.set_device_build(old)
+
+
+def test_a_cache_too_small_for_the_plans():
+    """Nothing is left with the native host path: the Python function runs, again and again."""
+    from bpt_amd.plan import plan_cache
+    old = plan_cache._cap, plan_cache._max_bytes
+    plan_cache.set_limits(1, 1)
+    try:
+        check(make(("bpt", 300, 4), 8, 64, "f32", 30.0, True), fused=True)
+        check(make(("bpt", 300, 4), 6, 50, "f32", 30.0, True), fused=True)
+    finally:
+        plan_cache.set_limits(*old)
+
+
+def test_generic_kernels_forced():
+    from bpt_amd import graphop
+    c = make(("bpt", 100, 4), 8, 64, "f32", 30.0, True)
+    args, _ = check(c)
+    graphop.set_force_generic(True)
+    try:
+        check(c)
+        with pytest.raises(RuntimeError, match="no fused kernel"):
+            run(c, args, fused=True)
+    finally:
+        graphop.set_force_generic(False)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("cap", [0.5, 4.0])
 def test_saturated_scores(cap, dtype):
     """Scores of tens over a cap of few: tanh is +-1 and its derivative 0 to the last digit."""
@@ -357,9 +398,13 @@ def test_refusals():
     args = graph_args(c["src"].numpy(), c["dst"].numpy(), c["q"].size(0), c["k"].size(0))
     dev = on_device(c, False)
     go = lambda **kw: op.bpt_attention(*args, dev["q"], dev["k"], dev["v"], **kw)
+    for opts in (dict(score_cap=3.0), dict(slopes=dev["slopes"], pos=dev["pos_q"])):      # (what follows is refused of a graph that is known, too)
+        go(**opts), go(**opts)
     for cap in (0.0, -1.0, float("inf"), float("nan")):
         with pytest.raises(ValueError, match="score_cap"):
             go(score_cap=cap)
+    with pytest.raises(ValueError, match="pair"):
+        go(slopes=dev["slopes"], pos=(dev["pos_q"],))
     with pytest.raises(ValueError, match="at least"):
         go(score_cap=1e-6)
     with pytest.raises(ValueError, match="go together"):

@@ -36,13 +36,19 @@ __global__ __launch_bounds__(BLOCK) void k_score_split(const int32_t *__restrict
     }
 }
 
-// dslopes[head] = -(sum of the tiles' parts and of what split rows gained), a workgroup a head, in a fixed order; how many tiles there are stands in the
-// plan
-__global__ __launch_bounds__(BLOCK) void k_slope_finish(const float *__restrict__ part, const int32_t *__restrict__ n_groups, int heads, int parts,
-                                                        const float *__restrict__ fix, int n_fix, float *__restrict__ dslopes) {
+// dslopes[head] = -(sum of the tiles' parts and of what split rows gained), by a workgroup, in a fixed order; how many tiles there are stands in the plan
+struct SlopeSum {
+    const float *part;                 // [group][head][part]
+    const int32_t *n_groups;
+    int heads, parts;                  // as part counts them
+    const float *fix;                  // [split row][head]
+    int n_fix, wanted;                 // heads to sum up, or 0
+    float *dslopes;
+};
+__device__ __forceinline__ void slope_sum_block(const SlopeSum &m, int head) {
     __shared__ double meet[BLOCK];
-    const int head = blockIdx.x, n = __builtin_amdgcn_readfirstlane(*n_groups) * parts;
-    auto at = [&](int i) { return part[((size_t)(i / parts) * heads + head) * parts + i % parts]; };
+    const int n = __builtin_amdgcn_readfirstlane(*m.n_groups) * m.parts;
+    auto at = [&](int i) { return m.part[((size_t)(i / m.parts) * m.heads + head) * m.parts + i % m.parts]; };
     double x = 0.0;
     int i = threadIdx.x;
     for (; i + 7 * BLOCK < n; i += 8 * BLOCK) {
@@ -53,13 +59,38 @@ __global__ __launch_bounds__(BLOCK) void k_slope_finish(const float *__restrict_
         for (int u = 0; u < 8; ++u) x += v[u];
     }
     for (; i < n; i += BLOCK) x += at(i);
-    for (i = threadIdx.x; i < n_fix; i += BLOCK) x += fix[(size_t)i * heads + head];
+    for (i = threadIdx.x; i < m.n_fix; i += BLOCK) x += m.fix[(size_t)i * m.heads + head];
     meet[threadIdx.x] = x;
     for (int o = BLOCK / 2; o > 0; o >>= 1) {
         __syncthreads();
         if ((int)threadIdx.x < o) meet[threadIdx.x] += meet[threadIdx.x + o];
     }
-    if (threadIdx.x == 0) dslopes[head] = (float)-meet[0];
+    if (threadIdx.x == 0) m.dslopes[head] = (float)-meet[0];
+}
+
+// The backward's last launch: k_combine_sum3's sums of split rows (dq; dk and dv) and, in workgroups of their own in front of them, the slopes' gradient, which
+// as a launch by itself cost 4 us (8 at L = 32768, k = 8).  Grid (m.wanted + n_a + n_b, C / 256, 2).
+template <typename T, bool NARROW>
+__global__ __launch_bounds__(BLOCK) void k_score_merge(SlopeSum m, const int32_t *__restrict__ heavy_a, int n_a, const float *__restrict__ ws_a, T *__restrict__ YA,
+                                                       const int32_t *__restrict__ heavy_b, const float *__restrict__ ws_b, T *__restrict__ YB0, T *__restrict__ YB1,
+                                                       int C, size_t ws_stride_b, Narrow nw) {
+    const int x = (int)blockIdx.x - m.wanted;
+    if (x < 0) {
+        if (blockIdx.y == 0 && blockIdx.z == 0) slope_sum_block(m, (int)blockIdx.x);
+    } else if (x < n_a) {
+        if (blockIdx.z == 0) combine_sum_block4<T, NARROW>(heavy_a + 3 * x, ws_a, YA, C, false, -1, nw);
+    } else {
+        combine_sum_block4<T, NARROW>(heavy_b + 3 * (x - n_a), ws_b + (size_t)blockIdx.z * ws_stride_b, blockIdx.z == 0 ? YB0 : YB1, C, false, -1, nw);
+    }
+}
+template <typename T, bool NARROW>
+int run_merge(const SlopeSum &m, const bpt_plan *Pin, const bpt_plan *Pout, const float *ws_dq, T *dq, const float *ws_dk, T *dk, T *dv, int C, const Narrow &nw,
+              hipStream_t s) {
+    const unsigned blocks = (unsigned)(m.wanted + Pin->n_heavy + Pout->n_heavy);
+    if (blocks == 0) return BPT_OK;
+    hipLaunchKernelGGL((k_score_merge<T, NARROW>), dim3(blocks, Pin->n_heavy + Pout->n_heavy > 0 ? C / (4 * WAVE) : 1, Pin->n_heavy + Pout->n_heavy > 0 ? 2 : 1), dim3(BLOCK), 0,
+                       s, m, Pin->heavy, (int)Pin->n_heavy, ws_dq, dq, Pout->heavy, ws_dk, dk, dv, C, (size_t)Pout->n_slots * C, nw);
+    return launch_status();
 }
 
 // Forward of few query rows (a decoder that takes one token at a time): a tile would walk a row's neighbours in one chain with fifteen of its sixteen
@@ -278,13 +309,8 @@ int run_backward(const bpt_plan *Pin, const bpt_plan *Pout, const bpt_score *sc,
     });
     st = launch_status();
     if (st != BPT_OK) return st;
-    if (Pin->n_heavy + Pout->n_heavy > 0)
-        hipLaunchKernelGGL((k_combine_sum3<T>), dim3((unsigned)(Pin->n_heavy + Pout->n_heavy), H * D / (4 * WAVE), 2), dim3(BLOCK), 0, s, Pin->heavy,
-                           (int)Pin->n_heavy, (const float *)ws_dq, (T *)dq, Pout->heavy, (const float *)ws_dk, (T *)dk, (T *)dv, H * D,
-                           (size_t)Pout->n_slots * H * D, Narrow{});
-    if (dslopes) hipLaunchKernelGGL(k_slope_finish, dim3(H), dim3(BLOCK), 0, s, (const float *)part, Pin->grp_chunks + 8, H, parts_in,
-                                    (const float *)fix, fixed ? (int)Pin->n_heavy : 0, dslopes);
-    return launch_status();
+    const SlopeSum sum{part, Pin->grp_chunks + 8, H, parts_in, fix, fixed ? (int)Pin->n_heavy : 0, dslopes ? H : 0, dslopes};
+    return run_merge<T, false>(sum, Pin, Pout, ws_dq, (T *)dq, ws_dk, (T *)dk, (T *)dv, H * D, Narrow{}, s);
 }
 
 // Heads of fewer than 64 columns in float32, read as they are.  (bfloat16 ones run on padded copies: their kernels hand (p, ds) over in 16 bits each,
@@ -335,12 +361,8 @@ int run_backward_narrow(const bpt_plan *Pin, const bpt_plan *Pout, const bpt_sco
     });
     st = launch_status();
     if (st != BPT_OK) return st;
-    if (Pin->n_heavy + Pout->n_heavy > 0)
-        hipLaunchKernelGGL((k_combine_sum3<float, true>), dim3((unsigned)(Pin->n_heavy + Pout->n_heavy), C / (4 * WAVE), 2), dim3(BLOCK), 0, s, Pin->heavy,
-                           (int)Pin->n_heavy, (const float *)ws_dq, dq, Pout->heavy, (const float *)ws_dk, dk, dv, C, (size_t)Pout->n_slots * C, nw);
-    if (dslopes) hipLaunchKernelGGL(k_slope_finish, dim3(nw.heads), dim3(BLOCK), 0, s, (const float *)part, Pin->grp_chunks + 8, nw.h, parts,
-                                    (const float *)nullptr, 0, dslopes);
-    return launch_status();
+    const SlopeSum sum{part, Pin->grp_chunks + 8, nw.h, parts, nullptr, 0, dslopes ? nw.heads : 0, dslopes};
+    return run_merge<float, true>(sum, Pin, Pout, ws_dq, dq, ws_dk, dk, dv, C, nw, s);
 }
 
 inline int check_score(const bpt_plan *P, const bpt_score *sc, int heads, int d, int h, int dtype, float scale, float dropout_p, const float *bias,

@@ -4144,7 +4144,7 @@ int run_attn_fwd_narrow(const bpt_plan *P, const void *q, const void *k, const v
         else                                                                                                                             \
             hipLaunchKernelGGL((k_attn_fwd_tile_bf16<16, 64, HW, TILE_BF16_WPE, DR, SP>), grid, block, 0, s, *P,                             \
                                (const T *)q, (const T *)k, (const T *)v, (T *)o, lse, ws_acc, ws_ml, scale * LOG2E, drop.thr, drop.seed,       \
-                               drop.inv, np, keep);                                                                                        \
+                               drop.inv, np, keep, NoMod{});                                                                                        \
     } while (0)
 #define LAUNCH_FWD(DR)                                                                                                                   \
     do {                                                                                                                                 \

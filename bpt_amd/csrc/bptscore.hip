@@ -313,23 +313,29 @@ int run_backward(const bpt_plan *Pin, const bpt_plan *Pout, const bpt_score *sc,
     return run_merge<T, false>(sum, Pin, Pout, ws_dq, (T *)dq, ws_dk, (T *)dk, (T *)dv, H * D, Narrow{}, s);
 }
 
-// Heads of fewer than 64 columns in float32, read as they are.  (bfloat16 ones run on padded copies: their kernels hand (p, ds) over in 16 bits each,
-// with delta from O as stored.)
-int run_forward_narrow(const bpt_plan *P, const bpt_score *sc, const float *q, const float *k, const float *v, float *o, float *lse, void *ws, float scale,
+// Heads of fewer than 64 columns, read as they are; the backward in float32 alone (bfloat16's for such heads would hand (p, ds) over in 16 bits each, with
+// delta from O as stored: graphop pads copies for it).
+template <typename T>
+int run_forward_narrow(const bpt_plan *P, const bpt_score *sc, const void *q, const void *k, const void *v, void *o, float *lse, void *ws, float scale,
                        Dropout drop, const Narrow &nw, hipStream_t s) {
     float *ws_acc = (float *)ws, *ws_ml = ws_acc ? ws_acc + (size_t)P->n_slots * nw.h * 64 : nullptr;
     const ScoreMod md = make_mod(sc, scale, true, nullptr);
-    const int parts = tile_parts(P, nw.heads, 4);
+    const int parts = tile_parts(P, nw.heads, sizeof(T));
     const Narrow np = narrow_parts(nw, parts);
     pick(drop.thr != 0, false, parts, [&](auto dr, auto, auto sp) {
         constexpr int HW = sp() == 1 ? NARROW_HW : sp();
-        hipLaunchKernelGGL((k_attn_fwd_tile<float, 16, 64, HW, dr(), 0, true, sp(), true>), dim3((unsigned)(group_grid(P) * np.slices)), dim3(HW * WAVE), 0, s, *P,
-                           q, k, v, o, lse, ws_acc, ws_ml, scale * LOG2E, drop.thr, drop.seed, drop.inv, (const float *)nullptr, np, Keep{}, md);
+        const dim3 grid((unsigned)(group_grid(P) * np.slices)), block(HW * WAVE);
+        if constexpr (sizeof(T) == 4)
+            hipLaunchKernelGGL((k_attn_fwd_tile<T, 16, 64, HW, dr(), 0, true, sp(), true>), grid, block, 0, s, *P, (const T *)q, (const T *)k, (const T *)v, (T *)o,
+                               lse, ws_acc, ws_ml, scale * LOG2E, drop.thr, drop.seed, drop.inv, (const float *)nullptr, np, Keep{}, md);
+        else
+            hipLaunchKernelGGL((k_attn_fwd_tile_bf16<16, 64, HW, TILE_BF16_WPE, dr(), sp(), true>), grid, block, 0, s, *P, (const T *)q, (const T *)k, (const T *)v,
+                               (T *)o, lse, ws_acc, ws_ml, scale * LOG2E, drop.thr, drop.seed, drop.inv, np, Keep{}, md);
     });
     const int st = launch_status();
     if (st != BPT_OK || P->n_heavy == 0) return st;
-    hipLaunchKernelGGL((k_attn_fwd_combine<float, 16, 64, true>), dim3((unsigned)P->n_heavy, nw.heads), dim3(BLOCK), 0, s, P->heavy, (const float *)ws_acc,
-                       (const float *)ws_ml, o, lse, nw, (float *)nullptr);
+    hipLaunchKernelGGL((k_attn_fwd_combine<T, 16, 64, true>), dim3((unsigned)P->n_heavy, nw.heads), dim3(BLOCK), 0, s, P->heavy, (const float *)ws_acc,
+                       (const float *)ws_ml, (T *)o, lse, nw, (T *)nullptr);
     return launch_status();
 }
 
@@ -366,7 +372,7 @@ int run_backward_narrow(const bpt_plan *Pin, const bpt_plan *Pout, const bpt_sco
 }
 
 inline int check_score(const bpt_plan *P, const bpt_score *sc, int heads, int d, int h, int dtype, float scale, float dropout_p, const float *bias,
-                       Narrow &nw, bool rows_too) {
+                       Narrow &nw, bool forward) {
     const int st = check_plan(P, true);
     if (st != BPT_OK) return st;
     if (!sc) return BPT_ERR_NULL;
@@ -374,12 +380,12 @@ inline int check_score(const bpt_plan *P, const bpt_score *sc, int heads, int d,
     if (h != 8 && h != 16 && !(h == 4 && dtype == BPT_F32)) return BPT_ERR_UNSUPPORTED;
     if (heads < 1 || d < 1) return BPT_ERR_SHAPE;
     const bool narrow = heads != h || d != 64;
-    if (narrow && (dtype != BPT_F32 || bias || heads > h || d < 4 || d > 64)) return BPT_ERR_UNSUPPORTED;
+    if (narrow && ((dtype != BPT_F32 && (!forward || d % 2 != 0)) || bias || heads > h || d < 4 || d > 64)) return BPT_ERR_UNSUPPORTED;
     nw = narrow ? Narrow{d, heads, h, (heads + NARROW_HW - 1) / NARROW_HW} : Narrow{};
     if (!(sc->cap >= 0.f && sc->cap <= 3.0e38f) || (sc->cap > 0.f && !(fabsf(scale) <= 1.0e4f * sc->cap)) || !(dropout_p >= 0.f && dropout_p < 1.f)) return BPT_ERR_SIZE;
     if (sc->slopes && (!sc->pos_q || !sc->pos_k)) return BPT_ERR_NULL;
     if (P->n_rows == 0) return P->n_edges == 0 ? BPT_OK : BPT_ERR_UNSUPPORTED;
-    if (rows_too && P->n_groups == 0 && !narrow && !bias && !(dropout_p > 0.f)) return BPT_OK;
+    if (forward && P->n_groups == 0 && !narrow && !bias && !(dropout_p > 0.f)) return BPT_OK;
     if (!has_tiles(P, h, 64, dtype == BPT_BF16 ? 2 : 4)) return BPT_ERR_UNSUPPORTED;
     if ((bias || dropout_p > 0.f || narrow) && !P->grp_eids) return BPT_ERR_PLAN;
     if (bias && P->bias_by_pair) return BPT_ERR_PLAN;
@@ -388,6 +394,11 @@ inline int check_score(const bpt_plan *P, const bpt_score *sc, int heads, int d,
 inline bool on16(std::initializer_list<const void *> ps) {
     for (const void *p : ps)
         if (!aligned16(p)) return false;
+    return true;
+}
+inline bool on4(std::initializer_list<const void *> ps) {
+    for (const void *p : ps)
+        if (reinterpret_cast<uintptr_t>(p) & 3) return false;
     return true;
 }
 
@@ -425,13 +436,13 @@ int bpt_score_forward(const bpt_plan *plan_in, const bpt_score *score, const voi
     if (st != BPT_OK) return st;
     if (plan_in->n_rows == 0) return BPT_OK;
     if (!q || !k || !v || !o || !lse) return BPT_ERR_NULL;
-    if (!aligned16(workspace) || (nw.heads == 0 && !on16({q, k, v, o}))) return BPT_ERR_UNSUPPORTED;
+    if (!aligned16(workspace) || (nw.heads == 0 ? !on16({q, k, v, o}) : !on4({q, k, v, o}))) return BPT_ERR_UNSUPPORTED;
     const int64_t need = bpt_score_forward_workspace_bytes(plan_in, h);
     if (need > 0 && (!workspace || workspace_bytes < need)) return BPT_ERR_WORKSPACE;
     const Dropout drop = make_dropout(dropout_p, dropout_seed);
     if (nw.heads > 0)
-        return run_forward_narrow(plan_in, score, (const float *)q, (const float *)k, (const float *)v, (float *)o, lse, workspace, scale, drop, nw,
-                                  (hipStream_t)stream);
+        return dtype == BPT_F32 ? run_forward_narrow<float>(plan_in, score, q, k, v, o, lse, workspace, scale, drop, nw, (hipStream_t)stream)
+                                : run_forward_narrow<bf16_t>(plan_in, score, q, k, v, o, lse, workspace, scale, drop, nw, (hipStream_t)stream);
     DISPATCH((run_forward<T, H>(plan_in, score, q, k, v, bias, o, lse, workspace, scale, drop, (hipStream_t)stream)))
 }
 

@@ -2088,11 +2088,11 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(MOD ?
 }
 
 // Heads of fewer than 64 columns (their rows on 4 bytes): rows of 8 bytes a lane, kept in registers.
-template <int H, int D, int HW, int WPE, bool DROP, int SP>
-__global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(WPE))) void k_attn_fwd_tile_bf16(
+template <int H, int D, int HW, int WPE, bool DROP, int SP, bool MOD = false>
+__global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(MOD ? WPE - 1 : WPE))) void k_attn_fwd_tile_bf16(
     bpt_plan P, const bf16_t *__restrict__ q, const bf16_t *__restrict__ k, const bf16_t *__restrict__ v, bf16_t *__restrict__ o,
     float *__restrict__ lse, float *__restrict__ ws_acc, float *__restrict__ ws_ml, float scale_log2e, uint32_t drop_thr,
-    uint32_t drop_seed, float drop_inv, Narrow nw, Keep keep) {
+    uint32_t drop_seed, float drop_inv, Narrow nw, Keep keep, typename ModArg<MOD>::type md) {
     const int Hs = nw.h;                                          // heads as lse, workspace and dropout keys count them
     const uint32_t RB = (uint32_t)(nw.heads * nw.d) * 2;          // bytes of a node row
     const int block = keep_or_tile<HW * WAVE>(keep);
@@ -2105,6 +2105,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(WPE))
     constexpr int PIECE = SP > 1 ? TILE_PART_FWD_FLOATS : TILE_KT_FLOATS_BF16;
     static_assert(PIECE >= TILE_KT_FLOATS_BF16, "the rows fit");
     __shared__ __attribute__((aligned(16))) float piece[HW][PIECE];
+    __shared__ __attribute__((aligned(16))) float pos_lds[HW][MOD ? TILE_R : 4];      // positions of the block's entries
     char *kt = reinterpret_cast<char *>(piece[t.wv]);
     TileEntryRegs er;
     if (t.p_end > t.p_begin) tile_ask_entries(P, t.p_begin, min(TILE_CHUNK, t.p_end - t.p_begin), t.lane, er);
@@ -2114,6 +2115,13 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(WPE))
     const char *kb = reinterpret_cast<const char *>(k), *vb = reinterpret_cast<const char *>(v);
     Bf8 qb[2];
     tile_load_row_bf16(reinterpret_cast<const char *>(q) + (size_t)max(t.member.x, 0) * RB + offr, qb, g, nw);
+    float slope = 0.f, pos_m = 0.f;
+    if constexpr (MOD) {
+        if (md.slopes) {
+            slope = md.slopes[t.head] * LOG2E;
+            pos_m = md.pos_member[max(t.member.x, 0)];
+        }
+    }
     floatx4v acc[4];
 #pragma unroll
     for (int nb = 0; nb < 4; ++nb) acc[nb] = floatx4v{0.f, 0.f, 0.f, 0.f};
@@ -2124,6 +2132,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(WPE))
         uint2 vr[4];
         int mk[4];                                                // bit c of mk[r]: the pair (entry 4 g + r, member c) exists
         int xe[DROP ? 4 : 1];
+        float pos;                                                // of entry c, in the first lane group
     };
     for (int p0 = t.p_begin; p0 < t.p_end; p0 += TILE_CHUNK) {
         const int cnt = min(TILE_CHUNK, t.p_end - p0), nblk = (cnt + TILE_R - 1) / TILE_R;
@@ -2137,6 +2146,9 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(WPE))
             for (int r = 0; r < 4; ++r) B.kq[r] = tile_row4_bf16<true>(kb + ((uint32_t)idxv[r] * RB + offc));
         };
         auto issue_rest = [&](Blk &B, int b) {
+            if constexpr (MOD) {
+                if (md.slopes && g == 0) B.pos = md.pos_entry[ent[TILE_R * b + c].x];
+            }
             if constexpr (DROP) tile_pair_eids(P, p0 + TILE_R * b + 4 * g, t.p_end, c, B.xe);
             const int4 e01 = *reinterpret_cast<const int4 *>(&ent[TILE_R * b + 4 * g]);
             const int4 e23 = *reinterpret_cast<const int4 *>(&ent[TILE_R * b + 4 * g + 2]);
@@ -2147,9 +2159,20 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(WPE))
         };
         auto compute = [&](const Blk &B) {
             Bf8 kr[2];
+            if constexpr (MOD) {
+                if (md.slopes && g == 0) pos_lds[t.wv][c] = B.pos;
+            }
             tile_rows_to_operand_bf16(kt, B.kq, c, g, kr, nw);
             const floatx4v st = tile_dot_bf16(kr, qb);
             float sc[4];
+            if constexpr (MOD) {
+                const floatx4v at_e = *reinterpret_cast<const floatx4v *>(&pos_lds[t.wv][4 * g]);
+                const float pos_e[4] = {at_e[0], at_e[1], at_e[2], at_e[3]}, x[4] = {st[0], st[1], st[2], st[3]};
+                float du[4];
+                tile_mod_scores(md, scale_log2e, slope, pos_m, pos_e, x, sc, du);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) sc[r] = where_pair(B.mk[r], c, sc[r]);
+            } else
 #pragma unroll
             for (int r = 0; r < 4; ++r) sc[r] = where_pair(B.mk[r], c, st[r] * scale_log2e);
             const float mb = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3]));

@@ -1284,11 +1284,16 @@ def score_padded_shape(q):
 
 
 def score_reads(q, rel=False):
-    """Whether the kernels read rows like q as they are: the shapes that score_padded_shape() leaves alone, and without a relative-position term
-    (rel) narrow heads of 4 columns or more in float32.  Others run on padded copies: bfloat16 because its kernels for narrow heads would hand the
-    source side pairs whose delta is off (comment at k_attn_bwd_dst_rows_bf16)."""
+    """Whether the forward reads rows like q as they are: the shapes that score_padded_shape() leaves alone, and without a relative-position term
+    (rel) narrow heads of 4 columns or more, an even number of them in bfloat16.  Others run on padded copies."""
     shape = score_padded_shape(q)
-    return shape is not None and (shape == _hd(q) or (not rel and q.dtype == torch.float32 and q.size(2) >= 4))
+    return shape is not None and (shape == _hd(q) or (not rel and q.size(2) >= 4 and (q.dtype == torch.float32 or q.size(2) % 2 == 0)))
+
+
+def _score_reads_backward(q):
+    """... and the backward, which runs bfloat16's narrow heads on padded copies: their kernels would hand the source side pairs whose delta is
+    off (comment at k_attn_bwd_dst_rows_bf16)."""
+    return q.dtype == torch.float32 or score_padded_shape(q) == _hd(q)
 
 
 def score_supported(eid_c, q, k):
@@ -1419,6 +1424,14 @@ def score_attention_backward(row, indptr_r, eid_r, indices_r, col, indptr_c, eid
     attention_backward's with bias, the gradient of q.k + bias per edge and head by edge id, None without."""
     graph = (row, indptr_r, eid_r, indices_r, col, indptr_c, eid_c, indices_c)
     h = _check_score_call(graph, q, k, v, score, bias)
+    if not _score_reads_backward(q):
+        _expect_shape(o, q.shape, "o")
+        _expect_shape(do, q.shape, "do")
+        heads, d = _hd(q)
+        wide = score if score.slopes is None else score._replace(slopes=torch.nn.functional.pad(score.slopes, (0, h - heads)))
+        grads = score_attention_backward(*graph, *(_pad_heads(x, h) for x in (q, k, v, o)), lse, _pad_heads(do, h), wide,
+                                         1.0 / math.sqrt(d) if scale is None else scale, dropout_p, seed, None, need_slopes)
+        return tuple(x[:, :heads, :d].contiguous() for x in grads[:3]) + (None if grads[3] is None else grads[3][:heads].contiguous(), None)
     do = do.contiguous()
     if do.data_ptr() % 16:
         do = do.clone()

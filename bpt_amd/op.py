@@ -456,8 +456,8 @@ def _score_attention(graph, q, k, v, scale, fused, dropout_p, seed, rel_table, e
         rel_table = torch.nn.functional.pad(rel_table, (0, dp - d)) if rel else None
         if score.slopes is not None:
             score = score._replace(slopes=torch.nn.functional.pad(score.slopes, (0, hp - h)))
-    elif d == 64:
-        q, k, v = (x.clone() if x.data_ptr() % 16 else x for x in (q, k, v))          # (the kernels read 16 bytes a lane)
+    else:
+        q, k, v = (x.clone() if x.data_ptr() % 16 else x for x in (q, k, v))          # (the kernels read 16 bytes a lane, of narrow rows 4)
     known = lambda: None if rel else _score_known(graph, q, k, v, scale, dropout_p, seed, score.cap or None, score.slopes,
                                                   None if score.slopes is None else score[2:])
     o = known()
@@ -494,7 +494,7 @@ def bpt_attention(row, indptr_r, eid_r, indices_r, col, indptr_c, eid_c, indices
     score_cap c > 0 makes it c tanh(u / c), which bounds it by c;
     slopes (h,) float32 and pos, float32 positions of the rows (one tensor, or a pair (of the query rows, of the key rows)), lower it by
     slopes[head] * |pos[dst] - pos[src]| behind the cap.  slopes get a gradient, pos does not.  Heads of up to 64 columns, 16 of them,
-    in float32 and bfloat16 run fused (bfloat16 narrow ones on padded copies), other shapes and float64 through the chain.  Edges are the
+    in float32 and bfloat16 run fused (bfloat16 narrow ones on padded copies in the backward), other shapes and float64 through the chain.  Edges are the
     graph's: documents that must not see each other are its separate components."""
     scale = 1.0 / math.sqrt(q.size(-1)) if scale is None else float(scale)
     if (rel_table is None) != (etype is None):

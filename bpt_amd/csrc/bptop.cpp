@@ -578,16 +578,6 @@ std::optional<std::array<Tensor, 4>> score_backward_known(const EntryPtr &e, con
     if (!attention_shape(q, k, v, p, s) || !like(o, q) || !like(d_o, q) || o.sizes() != q.sizes() || d_o.sizes() != q.sizes()) return std::nullopt;
     if (s.nq != e->a.n_rows || s.nk != e->b.n_rows || !float_matrix(lse, q.device(), s.nq, h) || !score_options(opt, q, k)) return std::nullopt;
     c10::DeviceGuard guard(q.device());
-    if (s.dt == BPT_BF16 && (s.h != h || s.d != 64)) {        // (graphop._score_reads_backward)
-        auto wide = [&](const Tensor &x) { return at::constant_pad_nd(x, {0, 64 - s.d, 0, h - s.h}); };
-        auto as_given = [&](const Tensor &x) { return x.narrow(1, 0, s.h).narrow(2, 0, s.d).contiguous(); };
-        const ScoreOptions padded{opt.cap, opt.slopes.defined() ? at::constant_pad_nd(opt.slopes, {0, h - s.h}) : Tensor(), opt.pos_q, opt.pos_k};
-        auto r = score_backward_known(e, wide(q), wide(k), wide(v), wide(o), lse, wide(d_o), padded, scale, p, seed, h, need_slopes);
-        if (!r) return std::nullopt;
-        for (size_t i = 0; i < 3; ++i) (*r)[i] = as_given((*r)[i]);
-        if ((*r)[3].defined()) (*r)[3] = (*r)[3].narrow(0, 0, s.h).contiguous();
-        return r;
-    }
     Tensor dq = at::empty_like(q), dk = at::empty_like(k), dv = at::empty_like(v), dslopes;
     if (opt.slopes.defined() && need_slopes) dslopes = at::empty_like(opt.slopes);
     const int64_t bytes = bpt_score_backward_workspace_bytes(&e->a, &e->b, h, s.dt, 0);
@@ -627,7 +617,6 @@ struct ScoreAttention : torch::autograd::Function<ScoreAttention> {
         const bool need_slopes = opt.slopes.defined() && ctx->needs_input_grad(11);
         Tensor d_o = grads[0].contiguous();
         if (reinterpret_cast<uintptr_t>(d_o.data_ptr()) & 15) d_o = d_o.clone();
-        at::NoGradGuard plain;
         auto r = score_backward_known(e, t[8], t[9], t[10], t[11], t[12], d_o, opt, scale, p, seed, h, need_slopes);
         if (!r)
             r = with_python([&] {

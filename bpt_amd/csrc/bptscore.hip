@@ -182,6 +182,272 @@ __global__ __launch_bounds__(NW == 1 ? BLOCK : NW * WAVE) void k_score_fwd_rows(
     }
 }
 
+// bfloat16 heads of fewer than 64 columns, read as they are (Narrow in bpttiles.h): the two sides of the backward, k_attn_bwd_dst_rows_bf16 and
+// k_attn_bwd_src_tile_bf16_again with rows of 8 bytes a lane, kept in registers for the products over the entries and turned in LDS for those over the
+// columns.  delta comes from the pairs in 32 bits, as there, so p and ds are formed twice rather than handed over in 16 bits each.
+// Bound by the loads' latency (a block's rows are asked for when it begins, three or four wavefronts a SIMD cover for one another; compiled for three or four,
+// either side is level, four spills the source side).  8192 tokens, k = 4, 6 x 50 bfloat16: 22.6 + 25.7 us, the training pass 102.7 us of which 81 are kernels;
+// on copies padded to 8 x 64 the pass took 208.  12 x 64: 49 + 50 us, the pass 157, on copies 298.
+constexpr int NARROW_WPE_DST = 4, NARROW_WPE_SRC = 3;
+template <int HW, bool DROP, int SP>
+__global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(NARROW_WPE_DST))) void k_score_bwd_dst_narrow_bf16(
+    bpt_plan P, const bf16_t *__restrict__ q, const bf16_t *__restrict__ k, const bf16_t *__restrict__ v, const bf16_t *__restrict__ o,
+    const bf16_t *__restrict__ d_o, const float *__restrict__ lse, bf16_t *__restrict__ dq, float2 *__restrict__ stat, float *__restrict__ ws_dq, float scale,
+    float scale_log2e, uint32_t drop_thr, uint32_t drop_seed, float drop_inv, Narrow nw, ScoreMod md) {
+    constexpr int H = 16, D = 64;
+    const int Hs = nw.h;
+    const uint32_t RB = (uint32_t)(nw.heads * nw.d) * 2;
+    TileCtx t;
+    if (!tile_begin<bf16_t, H, D, HW, true, SP>(P, t, nw)) return;
+    __shared__ int2 ent_lds[HW][TILE_CHUNK];
+    int2 *const ent = ent_lds[t.wv];
+    constexpr int PIECE = SP > 1 ? TILE_PART_FLOATS : TILE_KT_FLOATS_BF16;
+    static_assert(PIECE >= TILE_KT_FLOATS_BF16, "the rows fit");
+    __shared__ __attribute__((aligned(16))) float piece[HW][PIECE];
+    __shared__ __attribute__((aligned(16))) float pos_lds[HW][TILE_R];
+    char *const kt = reinterpret_cast<char *>(piece[t.wv]);
+    TileEntryRegs er;
+    if (t.p_end > t.p_begin) tile_ask_entries(P, t.p_begin, min(TILE_CHUNK, t.p_end - t.p_begin), t.lane, er);
+    issue_loads_first();
+    const int c = t.c, g = t.g;
+    const uint32_t offc = t.offv;
+    const char *kb = reinterpret_cast<const char *>(k), *vb = reinterpret_cast<const char *>(v);
+    const size_t mrow = (size_t)max(t.member.x, 0) * RB + t.offa, at = (size_t)max(t.member.x, 0) * Hs + t.head;
+    Bf8 qb[2], dob[2];
+    float delta = 0.f;
+    {
+        Bf8 ob[2];
+        tile_load_row_bf16(reinterpret_cast<const char *>(q) + mrow, qb, g, nw);
+        tile_load_row_bf16(reinterpret_cast<const char *>(d_o) + mrow, dob, g, nw);
+        tile_load_row_bf16(reinterpret_cast<const char *>(o) + mrow, ob, g, nw);
+#pragma unroll
+        for (int h2 = 0; h2 < 2; ++h2) {
+            const uint32_t a[4] = {dob[h2].q.x, dob[h2].q.y, dob[h2].q.z, dob[h2].q.w}, b[4] = {ob[h2].q.x, ob[h2].q.y, ob[h2].q.z, ob[h2].q.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                delta = fmaf(__uint_as_float(a[i] << 16), __uint_as_float(b[i] << 16), delta);
+                delta = fmaf(__uint_as_float(a[i] & 0xffff0000u), __uint_as_float(b[i] & 0xffff0000u), delta);
+            }
+        }
+        delta = groups_sum(delta);                                // dO . O of member c, this head
+    }
+    const float lse_c = lse[at];
+    float slope = 0.f, pos_m = 0.f, slope_sum = 0.f, dp_sum = 0.f, far_sum = 0.f;
+    if (md.slopes) {
+        slope = md.slopes[t.head] * LOG2E;
+        pos_m = md.pos_member[max(t.member.x, 0)];
+    }
+    floatx4v acc[4], pk[4];                                       // pk: sum of p du K
+#pragma unroll
+    for (int nb = 0; nb < 4; ++nb) { acc[nb] = floatx4v{0.f, 0.f, 0.f, 0.f}; pk[nb] = floatx4v{0.f, 0.f, 0.f, 0.f}; }
+    struct Blk {
+        uint2 kc[4], vc[4];                                       // columns 4 c .. 4 c + 3 of the K / V rows of entries 4 g + r
+        int mk[4];                                                // bit c of mk[r]: the pair (entry 4 g + r, member c) exists
+        int xe[DROP ? 4 : 1];
+        float pos;                                                // of entry c, in the first lane group
+    };
+    for (int p0 = t.p_begin; p0 < t.p_end; p0 += TILE_CHUNK) {
+        const int cnt = min(TILE_CHUNK, t.p_end - p0), nblk = (cnt + TILE_R - 1) / TILE_R;
+        if (p0 != t.p_begin) tile_ask_entries(P, p0, cnt, t.lane, er);
+        tile_put_entries(er, ent, cnt, t.lane);
+        auto issue = [&](Blk &B, int b) {
+            if constexpr (DROP) tile_pair_eids(P, p0 + TILE_R * b + 4 * g, t.p_end, c, B.xe);
+            if (md.slopes && g == 0) B.pos = md.pos_entry[ent[TILE_R * b + c].x];
+            const int4 e01 = *reinterpret_cast<const int4 *>(&ent[TILE_R * b + 4 * g]);
+            const int4 e23 = *reinterpret_cast<const int4 *>(&ent[TILE_R * b + 4 * g + 2]);
+            const int idxv[4] = {e01.x, e01.z, e23.x, e23.z};
+            B.mk[0] = e01.y; B.mk[1] = e01.w; B.mk[2] = e23.y; B.mk[3] = e23.w;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) B.kc[r] = tile_row4_bf16<true>(kb + ((uint32_t)idxv[r] * RB + offc));
+#pragma unroll
+            for (int r = 0; r < 4; ++r) B.vc[r] = tile_row4_bf16<true>(vb + ((uint32_t)idxv[r] * RB + offc));
+        };
+        auto compute = [&](const Blk &B) {
+            if (md.slopes && g == 0) pos_lds[t.wv][c] = B.pos;
+            Bf8 row[2];
+            tile_rows_to_operand_bf16(kt, B.kc, c, g, row, nw);
+            const floatx4v st = tile_dot_bf16(row, qb);
+            tile_rows_to_operand_bf16(kt, B.vc, c, g, row, nw);
+            const floatx4v dp = tile_dot_bf16(row, dob);
+            const floatx4v at_e = *reinterpret_cast<const floatx4v *>(&pos_lds[t.wv][4 * g]);
+            const float pos_e[4] = {at_e[0], at_e[1], at_e[2], at_e[3]}, x[4] = {st[0], st[1], st[2], st[3]};
+            float sm[4], du[4], ds[4], pdu[4];
+            tile_mod_scores(md, scale_log2e, slope, pos_m, pos_e, x, sm, du);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float pe = where_pair_or_zero(B.mk[r], c, __builtin_amdgcn_exp2f(sm[r] - lse_c));
+                float mt = 1.f;                                   // dropout multiplier of this pair (as in the forward)
+                if constexpr (DROP) mt = dropout_keep((uint32_t)B.xe[DROP ? r : 0] * (uint32_t)Hs + (uint32_t)t.head, drop_seed, drop_thr, drop_inv);
+                const float y = where_pair_or_zero(B.mk[r], c, pe * (dp[r] * mt));
+                ds[r] = fmaf(-pe, delta, y);
+                dp_sum += y;
+                if (md.part) {
+                    const float far = fabsf(pos_m - pos_e[r]);
+                    slope_sum = fmaf(ds[r], far, slope_sum);
+                    far_sum = fmaf(pe, far, far_sum);
+                }
+                ds[r] *= du[r] * scale;
+                pdu[r] = pe * (du[r] * scale);
+            }
+            Bf4 da;
+            da.u[0] = pack_bf16(ds[0], ds[1]);
+            da.u[1] = pack_bf16(ds[2], ds[3]);
+            tile_axpy_bf16(da, B.kc, acc);
+            da.u[0] = pack_bf16(pdu[0], pdu[1]);
+            da.u[1] = pack_bf16(pdu[2], pdu[3]);
+            tile_axpy_bf16(da, B.kc, pk);
+        };
+        tile_walk<Blk>(nblk, issue, compute);
+        wave_lds_fence();
+    }
+    float whole = groups_sum(dp_sum), far = groups_sum(far_sum);  // of member c, of this part
+    if constexpr (SP > 1) {
+        __shared__ float2 meet[HW][TILE_R];
+        if (g == 0) meet[t.wv][c] = make_float2(whole, far);
+        __syncthreads();
+        whole = far = 0.f;
+#pragma unroll
+        for (int i = 0; i < SP; ++i) {
+            const float2 x = meet[i * (HW / SP) + t.wv % (HW / SP)][c];
+            whole += x.x;
+            far += x.y;
+        }
+    }
+    const bool segment = t.member.y >= 0;
+    const float better = segment ? delta : whole, less = delta - better;
+    slope_sum = fmaf(less, far_sum, slope_sum);
+    // (lane (c, g) of the sums holds members 4 g + r, less is member c's)
+    float less_m[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) less_m[r] = lane_bcast(less, 4 * g + r);
+#pragma unroll
+    for (int nb = 0; nb < 4; ++nb)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[nb][r] = fmaf(less_m[r], pk[nb][r], acc[nb][r]);
+    if (g == 0 && t.part == 0 && t.member.x >= 0) {
+        stat[at] = make_float2(lse_c, better);
+        if (segment) md.split[(size_t)t.member.y * Hs + t.head] = make_float2(whole, far);
+    }
+    tile_put_slope_part<SP>(md, t, Hs, slope_sum);
+    if constexpr (SP > 1) {
+        tile_park(piece[t.wv], acc, t.lane);
+        __syncthreads();
+        tile_meet_and_store<SP, H, D, true>(piece[t.wv % (HW / SP)], (HW / SP) * PIECE, t, dq, ws_dq, nw);
+    } else {
+        tile_store_rows<H, D, false, true>(t, acc, 1.f, dq, ws_dq, nw);
+    }
+}
+
+template <int HW, bool DROP, int SP>
+__global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(NARROW_WPE_SRC))) void k_score_bwd_src_narrow_bf16(
+    bpt_plan P, const bf16_t *__restrict__ q, const bf16_t *__restrict__ k, const bf16_t *__restrict__ v, const bf16_t *__restrict__ d_o,
+    const float2 *__restrict__ stat, bf16_t *__restrict__ dk, bf16_t *__restrict__ dv, float *__restrict__ ws_dk, float *__restrict__ ws_dv, float scale,
+    float scale_log2e, uint32_t drop_thr, uint32_t drop_seed, float drop_inv, Narrow nw, ScoreMod md) {
+    constexpr int H = 16, D = 64;
+    const int Hs = nw.h;
+    const uint32_t RB = (uint32_t)(nw.heads * nw.d) * 2;
+    TileCtx t;
+    if (!tile_begin<bf16_t, H, D, HW, true, SP>(P, t, nw)) return;
+    // a wavefront's piece: its entry list, the rows being turned, the entries' (lse, delta) and positions; afterwards (SP > 1) what it has summed up
+    constexpr int ENT = TILE_CHUNK * 2, STAT = ENT + TILE_KT_FLOATS_BF16, LIVE = STAT + 3 * TILE_R, PIECE = SP > 1 && 2 * TILE_PART_FLOATS > LIVE ? 2 * TILE_PART_FLOATS : LIVE;
+    __shared__ __attribute__((aligned(16))) float piece[HW][PIECE];
+    int2 *const ent = reinterpret_cast<int2 *>(piece[t.wv]);
+    char *const kt = reinterpret_cast<char *>(piece[t.wv] + ENT);
+    float2 *const st_lds = reinterpret_cast<float2 *>(piece[t.wv] + STAT);
+    float *const pos_lds = piece[t.wv] + STAT + 2 * TILE_R;
+    TileEntryRegs er;
+    if (t.p_end > t.p_begin) tile_ask_entries(P, t.p_begin, min(TILE_CHUNK, t.p_end - t.p_begin), t.lane, er);
+    issue_loads_first();
+    const int c = t.c, g = t.g;
+    const uint32_t offc = t.offv;
+    const char *qb = reinterpret_cast<const char *>(q), *db = reinterpret_cast<const char *>(d_o);
+    const float2 *const stat_h = stat + t.head;
+    const size_t mrow = (size_t)max(t.member.x, 0) * RB + t.offa;
+    Bf8 kr[2], vr[2];
+    tile_load_row_bf16(reinterpret_cast<const char *>(k) + mrow, kr, g, nw);
+    tile_load_row_bf16(reinterpret_cast<const char *>(v) + mrow, vr, g, nw);
+    float slope = 0.f, pos_m = 0.f;
+    if (md.slopes) {
+        slope = md.slopes[t.head] * LOG2E;
+        pos_m = md.pos_member[max(t.member.x, 0)];
+    }
+    floatx4v ak[4], av[4];
+#pragma unroll
+    for (int nb = 0; nb < 4; ++nb) { ak[nb] = floatx4v{0.f, 0.f, 0.f, 0.f}; av[nb] = floatx4v{0.f, 0.f, 0.f, 0.f}; }
+    struct Blk {
+        uint2 qr[4], dr[4];
+        float2 ld;                                                // (lse, delta) of entry c, in the first lane group
+        int mk[4];                                                // bit c of mk[r]: the pair (entry 4 g + r, member c) exists
+        int xe[DROP ? 4 : 1];
+        float pos;                                                // of entry c, in the first lane group
+    };
+    for (int p0 = t.p_begin; p0 < t.p_end; p0 += TILE_CHUNK) {
+        const int cnt = min(TILE_CHUNK, t.p_end - p0), nblk = (cnt + TILE_R - 1) / TILE_R;
+        if (p0 != t.p_begin) tile_ask_entries(P, p0, cnt, t.lane, er);
+        tile_put_entries(er, ent, cnt, t.lane);
+        auto issue = [&](Blk &B, int b) {
+            if constexpr (DROP) tile_pair_eids(P, p0 + TILE_R * b + 4 * g, t.p_end, c, B.xe);
+            if (g == 0) {
+                const int at = ent[TILE_R * b + c].x;
+                B.ld = stat_h[(size_t)at * Hs];
+                if (md.slopes) B.pos = md.pos_entry[at];
+            }
+            const int4 e01 = *reinterpret_cast<const int4 *>(&ent[TILE_R * b + 4 * g]);
+            const int4 e23 = *reinterpret_cast<const int4 *>(&ent[TILE_R * b + 4 * g + 2]);
+            const int idxv[4] = {e01.x, e01.z, e23.x, e23.z};
+            B.mk[0] = e01.y; B.mk[1] = e01.w; B.mk[2] = e23.y; B.mk[3] = e23.w;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) B.qr[r] = tile_row4_bf16<true>(qb + ((uint32_t)idxv[r] * RB + offc));
+#pragma unroll
+            for (int r = 0; r < 4; ++r) B.dr[r] = tile_row4_bf16<true>(db + ((uint32_t)idxv[r] * RB + offc));
+        };
+        auto compute = [&](const Blk &B) {
+            if (g == 0) {
+                st_lds[c] = B.ld;
+                if (md.slopes) pos_lds[c] = B.pos;
+            }
+            Bf8 row[2];
+            tile_rows_to_operand_bf16(kt, B.qr, c, g, row, nw);
+            const floatx4v st = tile_dot_bf16(row, kr);
+            tile_rows_to_operand_bf16(kt, B.dr, c, g, row, nw);
+            const floatx4v dp = tile_dot_bf16(row, vr);
+            const floatx4v l01 = *reinterpret_cast<const floatx4v *>(&st_lds[4 * g]), l23 = *reinterpret_cast<const floatx4v *>(&st_lds[4 * g + 2]);
+            const float lse_e[4] = {l01[0], l01[2], l23[0], l23[2]}, delta_e[4] = {l01[1], l01[3], l23[1], l23[3]};
+            const floatx4v at_e = *reinterpret_cast<const floatx4v *>(&pos_lds[4 * g]);
+            const float pos_e[4] = {at_e[0], at_e[1], at_e[2], at_e[3]}, x[4] = {st[0], st[1], st[2], st[3]};
+            float sm[4], du[4], pe[4], ds[4];
+            tile_mod_scores(md, scale_log2e, slope, pos_m, pos_e, x, sm, du);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float p = where_pair_or_zero(B.mk[r], c, __builtin_amdgcn_exp2f(sm[r] - lse_e[r]));
+                float mt = 1.f;                                   // dropout multiplier of this pair (as in the forward)
+                if constexpr (DROP) mt = dropout_keep((uint32_t)B.xe[DROP ? r : 0] * (uint32_t)Hs + (uint32_t)t.head, drop_seed, drop_thr, drop_inv);
+                ds[r] = where_pair_or_zero(B.mk[r], c, p * (dp[r] * mt - delta_e[r]) * (du[r] * scale));
+                pe[r] = p * mt;
+            }
+            Bf4 pa, da;
+            da.u[0] = pack_bf16(ds[0], ds[1]); da.u[1] = pack_bf16(ds[2], ds[3]);
+            pa.u[0] = pack_bf16(pe[0], pe[1]); pa.u[1] = pack_bf16(pe[2], pe[3]);
+            tile_axpy_bf16(da, B.qr, ak);
+            tile_axpy_bf16(pa, B.dr, av);
+        };
+        tile_walk<Blk>(nblk, issue, compute);
+        wave_lds_fence();
+    }
+    if constexpr (SP > 1) {
+        constexpr int NEXT = (HW / SP) * PIECE;
+        tile_park(piece[t.wv], ak, t.lane);
+        tile_park(piece[t.wv] + TILE_PART_FLOATS, av, t.lane);
+        __syncthreads();
+        const float *const part0 = piece[t.wv % (HW / SP)];
+        tile_meet_and_store<SP, H, D, true>(part0, NEXT, t, dk, ws_dk, nw);
+        tile_meet_and_store<SP, H, D, true>(part0 + TILE_PART_FLOATS, NEXT, t, dv, ws_dv, nw);
+    } else {
+        tile_store_rows<H, D, false, true>(t, ak, 1.f, dk, ws_dk, nw);
+        tile_store_rows<H, D, false, true>(t, av, 1.f, dv, ws_dv, nw);
+    }
+}
+
 // The scratch of the two backward kernels: (p, ds) of the edges, or in bfloat16 without a bias (lse, delta) of the rows
 inline int64_t scratch_bytes(const bpt_plan *Pin, const bpt_plan *Pout, int h, int dtype, bool biased) {
     if (dtype == BPT_BF16 && !biased) return round16(std::max(Pin->n_rows, Pout->n_index_nodes) * h * 8);
@@ -313,8 +579,7 @@ int run_backward(const bpt_plan *Pin, const bpt_plan *Pout, const bpt_score *sc,
     return run_merge<T, false>(sum, Pin, Pout, ws_dq, (T *)dq, ws_dk, (T *)dk, (T *)dv, H * D, Narrow{}, s);
 }
 
-// Heads of fewer than 64 columns, read as they are; the backward in float32 alone (bfloat16's for such heads would hand (p, ds) over in 16 bits each, with
-// delta from O as stored: graphop pads copies for it).
+// Heads of fewer than 64 columns, read as they are.
 template <typename T>
 int run_forward_narrow(const bpt_plan *P, const bpt_score *sc, const void *q, const void *k, const void *v, void *o, float *lse, void *ws, float scale,
                        Dropout drop, const Narrow &nw, hipStream_t s) {
@@ -339,36 +604,56 @@ int run_forward_narrow(const bpt_plan *P, const bpt_score *sc, const void *q, co
     return launch_status();
 }
 
-int run_backward_narrow(const bpt_plan *Pin, const bpt_plan *Pout, const bpt_score *sc, const float *q, const float *k, const float *v, const float *o,
-                        const float *d_o, const float *lse, float *dq, float *dk, float *dv, float *dslopes, void *ws, float scale, Dropout drop, const Narrow &nw,
+template <typename T>
+int run_backward_narrow(const bpt_plan *Pin, const bpt_plan *Pout, const bpt_score *sc, const void *q_, const void *k_, const void *v_, const void *o_,
+                        const void *d_o_, const float *lse, void *dq_, void *dk_, void *dv_, float *dslopes, void *ws, float scale, Dropout drop, const Narrow &nw,
                         hipStream_t s) {
+    constexpr bool F32 = sizeof(T) == 4;
+    const T *q = (const T *)q_, *k = (const T *)k_, *v = (const T *)v_, *o = (const T *)o_, *d_o = (const T *)d_o_;
+    T *dq = (T *)dq_, *dk = (T *)dk_, *dv = (T *)dv_;
     char *at = (char *)ws;
     float2 *scratch = (float2 *)at;
-    at += scratch_bytes(Pin, Pout, nw.h, BPT_F32, false);
+    at += scratch_bytes(Pin, Pout, nw.h, F32 ? BPT_F32 : BPT_BF16, false);
     float *part = dslopes ? (float *)at : nullptr;
     at += slope_bytes(Pin, nw.h);
+    float2 *split = (float2 *)at;
+    float *fix = (float *)(at + round16(Pin->n_slots * nw.h * 8));
+    if (!F32) at += split_bytes(Pin, nw.h);
     const int C = nw.h * 64;
     float *ws_dq = (float *)at, *ws_dk = ws_dq + (size_t)Pin->n_slots * C, *ws_dv = ws_dk + (size_t)Pout->n_slots * C;
-    const int parts = tile_parts(Pin, nw.heads, 4), parts_src = tile_parts(Pout, nw.heads, 4);
+    const int parts = tile_parts(Pin, nw.heads, sizeof(T)), parts_src = tile_parts(Pout, nw.heads, sizeof(T));
     const Narrow np = narrow_parts(nw, parts), np_src = narrow_parts(nw, parts_src);
-    const ScoreMod md = make_mod(sc, scale, true, part);
+    ScoreMod md = make_mod(sc, scale, true, part);
+    md.split = split;
     pick(drop.thr != 0, false, parts, [&](auto dr, auto, auto sp) {
         constexpr int HW = sp() == 1 ? NARROW_HW : sp();
-        hipLaunchKernelGGL((k_attn_bwd_dst_tile<float, 16, 64, HW, dr(), 0, true, sp(), true>), dim3((unsigned)(group_grid(Pin) * np.slices)), dim3(HW * WAVE), 0, s,
-                           *Pin, q, k, v, o, d_o, lse, dq, scratch, ws_dq, scale, scale * LOG2E, drop.thr, drop.seed, drop.inv, (const float *)nullptr,
-                           (float *)nullptr, np, md);
+        const dim3 grid((unsigned)(group_grid(Pin) * np.slices)), block(HW * WAVE);
+        if constexpr (F32)
+            hipLaunchKernelGGL((k_attn_bwd_dst_tile<float, 16, 64, HW, dr(), 0, true, sp(), true>), grid, block, 0, s, *Pin, q, k, v, o, d_o, lse, dq, scratch, ws_dq,
+                               scale, scale * LOG2E, drop.thr, drop.seed, drop.inv, (const float *)nullptr, (float *)nullptr, np, md);
+        else
+            hipLaunchKernelGGL((k_score_bwd_dst_narrow_bf16<HW, dr(), sp()>), grid, block, 0, s, *Pin, q, k, v, o, d_o, lse, dq, scratch, ws_dq, scale, scale * LOG2E,
+                               drop.thr, drop.seed, drop.inv, np, md);
     });
     int st = launch_status();
     if (st != BPT_OK) return st;
-    pick(false, false, parts_src, [&](auto, auto, auto sp) {
+    const bool fixed = !F32 && Pin->n_heavy > 0;
+    if (fixed)          // (the padding heads' sums are not used)
+        hipLaunchKernelGGL(k_score_split, dim3((unsigned)Pin->n_heavy), dim3(BLOCK), 0, s, Pin->heavy, (const float2 *)split, scratch, fix, nw.h);
+    pick(!F32 && drop.thr != 0, false, parts_src, [&](auto dr, auto, auto sp) {
         constexpr int HW = sp() == 1 ? NARROW_HW : sp();
-        hipLaunchKernelGGL((k_attn_bwd_src_tile<float, 16, 64, HW, true, sp()>), dim3((unsigned)(group_grid(Pout) * np_src.slices)), dim3(HW * WAVE), 0, s, *Pout, q,
-                           d_o, (const float2 *)scratch, dk, dv, ws_dk, ws_dv, np_src);
+        const dim3 grid((unsigned)(group_grid(Pout) * np_src.slices)), block(HW * WAVE);
+        if constexpr (F32)
+            hipLaunchKernelGGL((k_attn_bwd_src_tile<float, 16, 64, HW, true, sp()>), grid, block, 0, s, *Pout, q, d_o, (const float2 *)scratch, dk, dv, ws_dk, ws_dv,
+                               np_src);
+        else
+            hipLaunchKernelGGL((k_score_bwd_src_narrow_bf16<HW, dr(), sp()>), grid, block, 0, s, *Pout, q, k, v, d_o, (const float2 *)scratch, dk, dv, ws_dk, ws_dv,
+                               scale, scale * LOG2E, drop.thr, drop.seed, drop.inv, np_src, make_mod(sc, scale, false, nullptr));
     });
     st = launch_status();
     if (st != BPT_OK) return st;
-    const SlopeSum sum{part, Pin->grp_chunks + 8, nw.h, parts, nullptr, 0, dslopes ? nw.heads : 0, dslopes};
-    return run_merge<float, true>(sum, Pin, Pout, ws_dq, dq, ws_dk, dk, dv, C, nw, s);
+    const SlopeSum sum{part, Pin->grp_chunks + 8, nw.h, parts, fix, fixed ? (int)Pin->n_heavy : 0, dslopes ? nw.heads : 0, dslopes};
+    return run_merge<T, true>(sum, Pin, Pout, ws_dq, dq, ws_dk, dk, dv, C, nw, s);
 }
 
 inline int check_score(const bpt_plan *P, const bpt_score *sc, int heads, int d, int h, int dtype, float scale, float dropout_p, const float *bias,
@@ -380,7 +665,7 @@ inline int check_score(const bpt_plan *P, const bpt_score *sc, int heads, int d,
     if (h != 8 && h != 16 && !(h == 4 && dtype == BPT_F32)) return BPT_ERR_UNSUPPORTED;
     if (heads < 1 || d < 1) return BPT_ERR_SHAPE;
     const bool narrow = heads != h || d != 64;
-    if (narrow && ((dtype != BPT_F32 && (!forward || d % 2 != 0)) || bias || heads > h || d < 4 || d > 64)) return BPT_ERR_UNSUPPORTED;
+    if (narrow && ((dtype != BPT_F32 && d % 2 != 0) || bias || heads > h || d < 4 || d > 64)) return BPT_ERR_UNSUPPORTED;
     nw = narrow ? Narrow{d, heads, h, (heads + NARROW_HW - 1) / NARROW_HW} : Narrow{};
     if (!(sc->cap >= 0.f && sc->cap <= 3.0e38f) || (sc->cap > 0.f && !(fabsf(scale) <= 1.0e4f * sc->cap)) || !(dropout_p >= 0.f && dropout_p < 1.f)) return BPT_ERR_SIZE;
     if (sc->slopes && (!sc->pos_q || !sc->pos_k)) return BPT_ERR_NULL;
@@ -460,12 +745,12 @@ int bpt_score_backward(const bpt_plan *plan_in, const bpt_plan *plan_out, const 
     if ((bias != nullptr) != (ds_out != nullptr) || (dslopes && !score->slopes)) return BPT_ERR_NULL;
     if (dropout_p > 0.f && dtype == BPT_BF16 && !bias && !plan_out->grp_eids) return BPT_ERR_PLAN;
     if (!q || !k || !v || !o || !d_o || !lse || !dq || !dk || !dv) return BPT_ERR_NULL;
-    if (!aligned16(workspace) || (nw.heads == 0 && !on16({q, k, v, o, d_o, dq, dk, dv}))) return BPT_ERR_UNSUPPORTED;
+    if (!aligned16(workspace) || (nw.heads == 0 ? !on16({q, k, v, o, d_o, dq, dk, dv}) : !on4({q, k, v, o, d_o, dq, dk, dv}))) return BPT_ERR_UNSUPPORTED;
     if (!workspace || workspace_bytes < bpt_score_backward_workspace_bytes(plan_in, plan_out, h, dtype, bias != nullptr)) return BPT_ERR_WORKSPACE;
     const Dropout drop = make_dropout(dropout_p, dropout_seed);
     if (nw.heads > 0)
-        return run_backward_narrow(plan_in, plan_out, score, (const float *)q, (const float *)k, (const float *)v, (const float *)o, (const float *)d_o, lse,
-                                   (float *)dq, (float *)dk, (float *)dv, dslopes, workspace, scale, drop, nw, (hipStream_t)stream);
+        return dtype == BPT_F32 ? run_backward_narrow<float>(plan_in, plan_out, score, q, k, v, o, d_o, lse, dq, dk, dv, dslopes, workspace, scale, drop, nw, (hipStream_t)stream)
+                                : run_backward_narrow<bf16_t>(plan_in, plan_out, score, q, k, v, o, d_o, lse, dq, dk, dv, dslopes, workspace, scale, drop, nw, (hipStream_t)stream);
     DISPATCH((run_backward<T, H>(plan_in, plan_out, score, q, k, v, bias, o, d_o, lse, dq, dk, dv, ds_out, dslopes, workspace, scale, drop, (hipStream_t)stream)))
 }
 

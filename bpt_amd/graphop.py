@@ -1290,12 +1290,6 @@ def score_reads(q, rel=False):
     return shape is not None and (shape == _hd(q) or (not rel and q.size(2) >= 4 and (q.dtype == torch.float32 or q.size(2) % 2 == 0)))
 
 
-def _score_reads_backward(q):
-    """... and the backward, which runs bfloat16's narrow heads on padded copies: their kernels would hand the source side pairs whose delta is
-    off (comment at k_attn_bwd_dst_rows_bf16)."""
-    return q.dtype == torch.float32 or score_padded_shape(q) == _hd(q)
-
-
 def score_supported(eid_c, q, k):
     """Whether the fused kernels with score options may run a call on q's padded shape: they are tile kernels."""
     cfg, shape = _SETTINGS, score_padded_shape(q)
@@ -1424,14 +1418,6 @@ def score_attention_backward(row, indptr_r, eid_r, indices_r, col, indptr_c, eid
     attention_backward's with bias, the gradient of q.k + bias per edge and head by edge id, None without."""
     graph = (row, indptr_r, eid_r, indices_r, col, indptr_c, eid_c, indices_c)
     h = _check_score_call(graph, q, k, v, score, bias)
-    if not _score_reads_backward(q):
-        _expect_shape(o, q.shape, "o")
-        _expect_shape(do, q.shape, "do")
-        heads, d = _hd(q)
-        wide = score if score.slopes is None else score._replace(slopes=torch.nn.functional.pad(score.slopes, (0, h - heads)))
-        grads = score_attention_backward(*graph, *(_pad_heads(x, h) for x in (q, k, v, o)), lse, _pad_heads(do, h), wide,
-                                         1.0 / math.sqrt(d) if scale is None else scale, dropout_p, seed, None, need_slopes)
-        return tuple(x[:, :heads, :d].contiguous() for x in grads[:3]) + (None if grads[3] is None else grads[3][:heads].contiguous(), None)
     do = do.contiguous()
     if do.data_ptr() % 16:
         do = do.clone()

@@ -494,7 +494,7 @@ def bpt_attention(row, indptr_r, eid_r, indices_r, col, indptr_c, eid_c, indices
     score_cap c > 0 makes it c tanh(u / c), which bounds it by c;
     slopes (h,) float32 and pos, float32 positions of the rows (one tensor, or a pair (of the query rows, of the key rows)), lower it by
     slopes[head] * |pos[dst] - pos[src]| behind the cap.  slopes get a gradient, pos does not.  Heads of up to 64 columns, 16 of them,
-    in float32 and bfloat16 run fused (bfloat16 narrow ones on padded copies in the backward), other shapes and float64 through the chain.  Edges are the
+    in float32 and bfloat16 run fused, other shapes and float64 through the chain.  Edges are the
     graph's: documents that must not see each other are its separate components."""
     scale = 1.0 / math.sqrt(q.size(-1)) if scale is None else float(scale)
     if (rel_table is None) != (etype is None):

@@ -196,9 +196,10 @@ def test_a_graph_that_fills_the_chip(dtype):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
-def test_tiles_in_two_parts_and_long_rows(dtype):
-    """About 2056 wavefronts of five blocks: two wavefronts a tile; the last row has 4096 edges, in many segments."""
-    check(make(("window", 4096, 64), 8, 64, dtype, 30.0, True), fused=True)
+@pytest.mark.parametrize("heads,d", [(8, 64), (6, 50)])
+def test_tiles_in_two_parts_and_long_rows(heads, d, dtype):
+    """About 2056 wavefronts (1542 of six heads) of five blocks: two wavefronts a tile; the last row has 4096 edges, in many segments."""
+    check(make(("window", 4096, 64), heads, d, dtype, 30.0, True), fused=True)
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])

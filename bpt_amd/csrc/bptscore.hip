@@ -168,11 +168,11 @@ __global__ __launch_bounds__(NW == 1 ? BLOCK : NW * WAVE) void k_score_fwd_rows(
         }
     }
     if (it.slot < 0) {
-        const float inv = l > 0.f ? 1.f / l : 0.f;
+        const float inv = has_sum<true>(l) ? 1.f / l : 0.f;
 #pragma unroll
         for (int i = 0; i < L::EPL; ++i) acc[i] *= inv;
         store_row<T, H, D>(o + (size_t)it.row * L::C, lane, acc);
-        if (lane % L::LPH == 0) lse[(size_t)it.row * H + head] = l > 0.f ? m + log2f(l) : 0.f;
+        if (lane % L::LPH == 0) lse[(size_t)it.row * H + head] = has_sum<true>(l) ? m + log2f(l) : 0.f;
     } else {
         store_row_ws<T, H, D>(ws_acc + (size_t)it.slot * L::C, lane, acc);
         if (lane % L::LPH == 0) {
@@ -188,7 +188,7 @@ __global__ __launch_bounds__(NW == 1 ? BLOCK : NW * WAVE) void k_score_fwd_rows(
 // Bound by the loads' latency (a block's rows are asked for when it begins, three or four wavefronts a SIMD cover for one another; compiled for three or four,
 // either side is level, four spills the source side).  8192 tokens, k = 4, 6 x 50 bfloat16: 22.6 + 25.7 us, the training pass 102.7 us of which 81 are kernels;
 // on copies padded to 8 x 64 the pass took 208.  12 x 64: 49 + 50 us, the pass 157, on copies 298.
-constexpr int NARROW_WPE_DST = 4, NARROW_WPE_SRC = 3;
+constexpr int NARROW_WPE_DST = 3, NARROW_WPE_SRC = 3;
 template <int HW, bool DROP, int SP>
 __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(NARROW_WPE_DST))) void k_score_bwd_dst_narrow_bf16(
     bpt_plan P, const bf16_t *__restrict__ q, const bf16_t *__restrict__ k, const bf16_t *__restrict__ v, const bf16_t *__restrict__ o,
@@ -246,6 +246,9 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(NARRO
         int xe[DROP ? 4 : 1];
         float pos;                                                // of entry c, in the first lane group
     };
+    auto walk = [&](auto again) __attribute__((always_inline)) {
+    constexpr bool CAREFUL = decltype(again)::value;
+    if constexpr (CAREFUL) tile_ask_entries(P, t.p_begin, min(TILE_CHUNK, t.p_end - t.p_begin), t.lane, er);
     for (int p0 = t.p_begin; p0 < t.p_end; p0 += TILE_CHUNK) {
         const int cnt = min(TILE_CHUNK, t.p_end - p0), nblk = (cnt + TILE_R - 1) / TILE_R;
         if (p0 != t.p_begin) tile_ask_entries(P, p0, cnt, t.lane, er);
@@ -283,22 +286,35 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(NARRO
                 dp_sum += y;
                 if (md.part) {
                     const float far = fabsf(pos_m - pos_e[r]);
-                    slope_sum = fmaf(ds[r], far, slope_sum);
-                    far_sum = fmaf(pe, far, far_sum);
+                    slope_sum += pair_if<CAREFUL>(B.mk[r], c, ds[r] * far);
+                    far_sum += pair_if<CAREFUL>(B.mk[r], c, pe * far);
                 }
-                ds[r] *= du[r] * scale;
-                pdu[r] = pe * (du[r] * scale);
+                ds[r] = pair_if<CAREFUL>(B.mk[r], c, ds[r] * (du[r] * scale));
+                pdu[r] = pair_if<CAREFUL>(B.mk[r], c, pe * (du[r] * scale));
             }
-            Bf4 da;
-            da.u[0] = pack_bf16(ds[0], ds[1]);
-            da.u[1] = pack_bf16(ds[2], ds[3]);
-            tile_axpy_bf16(da, B.kc, acc);
-            da.u[0] = pack_bf16(pdu[0], pdu[1]);
-            da.u[1] = pack_bf16(pdu[2], pdu[3]);
-            tile_axpy_bf16(da, B.kc, pk);
+            if constexpr (CAREFUL) {
+                tile_axpy_pairs(ds, B.mk, B.kc, c, g, acc);
+                tile_axpy_pairs(pdu, B.mk, B.kc, c, g, pk);
+            } else {
+                Bf4 da;
+                da.u[0] = pack_bf16(ds[0], ds[1]);
+                da.u[1] = pack_bf16(ds[2], ds[3]);
+                tile_axpy_bf16(da, B.kc, acc);
+                da.u[0] = pack_bf16(pdu[0], pdu[1]);
+                da.u[1] = pack_bf16(pdu[2], pdu[3]);
+                tile_axpy_bf16(da, B.kc, pk);
+            }
         };
         tile_walk<Blk>(nblk, issue, compute);
         wave_lds_fence();
+    }
+    };
+    walk(std::false_type{});
+    if (tile_any_odd(tile_odd(acc) + tile_odd(pk) + (slope_sum + far_sum) * 0.f)) {      // (what does not exist must not reach the sums: tile_odd)
+#pragma unroll
+            for (int nb = 0; nb < 4; ++nb) { acc[nb] = floatx4v{0.f, 0.f, 0.f, 0.f}; pk[nb] = floatx4v{0.f, 0.f, 0.f, 0.f}; }
+            slope_sum = far_sum = dp_sum = 0.f;
+            walk(std::true_type{});
     }
     float whole = groups_sum(dp_sum), far = groups_sum(far_sum);  // of member c, of this part
     if constexpr (SP > 1) {
@@ -314,7 +330,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(NARRO
         }
     }
     const bool segment = t.member.y >= 0;
-    const float better = segment ? delta : whole, less = delta - better;
+    const float better = segment ? delta : whole, less = delta == delta ? delta - better : 0.f;      // (as in k_attn_bwd_dst_rows_bf16)
     slope_sum = fmaf(less, far_sum, slope_sum);
     // (lane (c, g) of the sums holds members 4 g + r, less is member c's)
     float less_m[4];
@@ -381,6 +397,9 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(NARRO
         int xe[DROP ? 4 : 1];
         float pos;                                                // of entry c, in the first lane group
     };
+    auto walk = [&](auto again) __attribute__((always_inline)) {
+    constexpr bool CAREFUL = decltype(again)::value;
+    if constexpr (CAREFUL) tile_ask_entries(P, t.p_begin, min(TILE_CHUNK, t.p_end - t.p_begin), t.lane, er);
     for (int p0 = t.p_begin; p0 < t.p_end; p0 += TILE_CHUNK) {
         const int cnt = min(TILE_CHUNK, t.p_end - p0), nblk = (cnt + TILE_R - 1) / TILE_R;
         if (p0 != t.p_begin) tile_ask_entries(P, p0, cnt, t.lane, er);
@@ -425,14 +444,26 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(NARRO
                 ds[r] = where_pair_or_zero(B.mk[r], c, p * (dp[r] * mt - delta_e[r]) * (du[r] * scale));
                 pe[r] = p * mt;
             }
-            Bf4 pa, da;
-            da.u[0] = pack_bf16(ds[0], ds[1]); da.u[1] = pack_bf16(ds[2], ds[3]);
-            pa.u[0] = pack_bf16(pe[0], pe[1]); pa.u[1] = pack_bf16(pe[2], pe[3]);
-            tile_axpy_bf16(da, B.qr, ak);
-            tile_axpy_bf16(pa, B.dr, av);
+            if constexpr (CAREFUL) {
+                tile_axpy_pairs(ds, B.mk, B.qr, c, g, ak);
+                tile_axpy_pairs(pe, B.mk, B.dr, c, g, av);
+            } else {
+                Bf4 pa, da;
+                da.u[0] = pack_bf16(ds[0], ds[1]); da.u[1] = pack_bf16(ds[2], ds[3]);
+                pa.u[0] = pack_bf16(pe[0], pe[1]); pa.u[1] = pack_bf16(pe[2], pe[3]);
+                tile_axpy_bf16(da, B.qr, ak);
+                tile_axpy_bf16(pa, B.dr, av);
+            }
         };
         tile_walk<Blk>(nblk, issue, compute);
         wave_lds_fence();
+    }
+    };
+    walk(std::false_type{});
+    if (tile_any_odd(tile_odd(ak) + tile_odd(av))) {      // (what does not exist must not reach the sums: tile_odd)
+#pragma unroll
+            for (int nb = 0; nb < 4; ++nb) { ak[nb] = floatx4v{0.f, 0.f, 0.f, 0.f}; av[nb] = floatx4v{0.f, 0.f, 0.f, 0.f}; }
+            walk(std::true_type{});
     }
     if constexpr (SP > 1) {
         constexpr int NEXT = (HW / SP) * PIECE;
@@ -520,7 +551,7 @@ int run_forward(const bpt_plan *P, const bpt_score *sc, const void *q, const voi
     });
     const int st = launch_status();
     if (st != BPT_OK || P->n_heavy == 0) return st;
-    hipLaunchKernelGGL((k_attn_fwd_combine<T, H, D>), dim3((unsigned)P->n_heavy, H * D / WAVE), dim3(BLOCK), 0, s, P->heavy, (const float *)ws_acc,
+    hipLaunchKernelGGL((k_attn_fwd_combine<T, H, D, false, true>), dim3((unsigned)P->n_heavy, H * D / WAVE), dim3(BLOCK), 0, s, P->heavy, (const float *)ws_acc,
                        (const float *)ws_ml, (T *)o, lse, Narrow{}, (T *)nullptr);
     return launch_status();
 }
@@ -563,10 +594,10 @@ int run_backward(const bpt_plan *Pin, const bpt_plan *Pout, const bpt_score *sc,
     pick(drop.thr != 0, biased, parts_out, [&](auto dr, auto bi, auto sp) {
         const dim3 grid((unsigned)(group_grid(Pout) * (H * sp() / HW))), block(HW * WAVE);
         if constexpr (sizeof(T) == 4)
-            hipLaunchKernelGGL((k_attn_bwd_src_tile<T, H, D, HW, false, sp()>), grid, block, 0, s, *Pout, (const T *)q, (const T *)d_o, (const float2 *)scratch,
+            hipLaunchKernelGGL((k_attn_bwd_src_tile<T, H, D, HW, false, sp(), true>), grid, block, 0, s, *Pout, (const T *)q, (const T *)d_o, (const float2 *)scratch,
                                (T *)dk, (T *)dv, ws_dk, ws_dv, Narrow{});
         else if constexpr (bi() != 0)
-            hipLaunchKernelGGL((k_attn_bwd_src_tile_bf16<H, D, HW, TILE_BF16_WPE_SRC, false, sp()>), grid, block, 0, s, *Pout, (const T *)q, (const T *)d_o,
+            hipLaunchKernelGGL((k_attn_bwd_src_tile_bf16<H, D, HW, TILE_BF16_WPE_SRC, false, sp(), true>), grid, block, 0, s, *Pout, (const T *)q, (const T *)d_o,
                                (const uint32_t *)scratch, (T *)dk, (T *)dv, ws_dk, ws_dv, Narrow{});
         else
             hipLaunchKernelGGL((k_attn_bwd_src_tile_bf16_again<H, D, HW, TILE_BF16_WPE_AGAIN, dr(), sp(), true>), grid, block, 0, s, *Pout, (const T *)q,
@@ -599,7 +630,7 @@ int run_forward_narrow(const bpt_plan *P, const bpt_score *sc, const void *q, co
     });
     const int st = launch_status();
     if (st != BPT_OK || P->n_heavy == 0) return st;
-    hipLaunchKernelGGL((k_attn_fwd_combine<T, 16, 64, true>), dim3((unsigned)P->n_heavy, nw.heads), dim3(BLOCK), 0, s, P->heavy, (const float *)ws_acc,
+    hipLaunchKernelGGL((k_attn_fwd_combine<T, 16, 64, true, true>), dim3((unsigned)P->n_heavy, nw.heads), dim3(BLOCK), 0, s, P->heavy, (const float *)ws_acc,
                        (const float *)ws_ml, (T *)o, lse, nw, (T *)nullptr);
     return launch_status();
 }
@@ -644,7 +675,7 @@ int run_backward_narrow(const bpt_plan *Pin, const bpt_plan *Pout, const bpt_sco
         constexpr int HW = sp() == 1 ? NARROW_HW : sp();
         const dim3 grid((unsigned)(group_grid(Pout) * np_src.slices)), block(HW * WAVE);
         if constexpr (F32)
-            hipLaunchKernelGGL((k_attn_bwd_src_tile<float, 16, 64, HW, true, sp()>), grid, block, 0, s, *Pout, q, d_o, (const float2 *)scratch, dk, dv, ws_dk, ws_dv,
+            hipLaunchKernelGGL((k_attn_bwd_src_tile<float, 16, 64, HW, true, sp(), true>), grid, block, 0, s, *Pout, q, d_o, (const float2 *)scratch, dk, dv, ws_dk, ws_dv,
                                np_src);
         else
             hipLaunchKernelGGL((k_score_bwd_src_narrow_bf16<HW, dr(), sp()>), grid, block, 0, s, *Pout, q, k, v, d_o, (const float2 *)scratch, dk, dv, ws_dk, ws_dv,

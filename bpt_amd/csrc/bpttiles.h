@@ -408,10 +408,13 @@ template <int NW, int BATCH> __device__ __forceinline__ bool fetch_item_part(con
     return true;
 }
 
+// Whether a row's softmax has a denominator.  MOD (ScoreMod, below): NaN is one, the row is NaN then.
+template <bool MOD> __device__ __forceinline__ bool has_sum(float l) { return MOD ? l != 0.f : l > 0.f; }
+
 // Combine the (m, l, acc) partials of each split row.  Grid (n_heavy, C / 64): one block per split row
 // and 64-column strip; wave w folds slots w, w+4, ... with a running maximum (one pass, eight
 // independent loads per step), then the four wave results are merged in wave order.
-template <typename T, int HC, int D, bool NARROW = false>
+template <typename T, int HC, int D, bool NARROW = false, bool MOD = false>
 __global__ __launch_bounds__(BLOCK) void k_attn_fwd_combine(const int32_t *__restrict__ heavy, const float *__restrict__ ws_acc,
                                                             const float *__restrict__ ws_ml, T *__restrict__ o, float *__restrict__ lse,
                                                             Narrow nw, T *__restrict__ o_keep = nullptr) {
@@ -478,12 +481,12 @@ __global__ __launch_bounds__(BLOCK) void k_attn_fwd_combine(const int32_t *__res
             L = fmaf(pl[i][lane], wgt, L);
             A = fmaf(pa[i][lane], wgt, A);
         }
-        if (!NARROW) Elem<T>::st(o + (size_t)row * C + j, L > 0.f ? A / L : 0.f);
+        if (!NARROW) Elem<T>::st(o + (size_t)row * C + j, has_sum<MOD>(L) ? A / L : 0.f);
         else if (lane < nw.d) {
-            Elem<T>::st(o + (size_t)row * (nw.heads * nw.d) + head * nw.d + lane, L > 0.f ? A / L : 0.f);
-            if (o_keep) Elem<T>::st(o_keep + (size_t)row * (nw.heads * nw.d) + head * nw.d + lane, L > 0.f ? A / L : 0.f);
+            Elem<T>::st(o + (size_t)row * (nw.heads * nw.d) + head * nw.d + lane, has_sum<MOD>(L) ? A / L : 0.f);
+            if (o_keep) Elem<T>::st(o_keep + (size_t)row * (nw.heads * nw.d) + head * nw.d + lane, has_sum<MOD>(L) ? A / L : 0.f);
         }
-        if (j % D == 0) lse[(size_t)row * H + head] = L > 0.f ? Mx + log2f(L) : 0.f;
+        if (j % D == 0) lse[(size_t)row * H + head] = has_sum<MOD>(L) ? Mx + log2f(L) : 0.f;
     }
 }
 
@@ -812,7 +815,7 @@ __device__ __forceinline__ void tile_meet_and_store(const float *part0, int stri
 }
 // ... and for the forward: with the parts' exponent references and denominators (left behind the accumulators by member)
 constexpr int TILE_PART_FWD_FLOATS = TILE_PART_FLOATS + 2 * TILE_R;
-template <int SP, int H, int D, bool NARROW, typename T>
+template <int SP, int H, int D, bool NARROW, bool MOD, typename T>
 __device__ __forceinline__ void tile_meet_forward(float *mine, const float *part0, int stride, const TileCtx &t, const floatx4v (&acc)[4], float &mref,
                                                   float &lt, T *__restrict__ out, float *__restrict__ ws, const Narrow &nw,
                                                   T *__restrict__ also) {
@@ -836,7 +839,7 @@ __device__ __forceinline__ void tile_meet_forward(float *mine, const float *part
     }
     mref = M;
     lt = l;
-    const float inv = l > 0.f ? 1.f / l : 0.f;
+    const float inv = has_sum<MOD>(l) ? 1.f / l : 0.f;
 #pragma unroll
     for (int i = 0; i < RS; ++i) {
         const int r = t.part * RS + i;
@@ -972,6 +975,46 @@ struct NoMod {};
 template <bool MOD> struct ModArg { typedef NoMod type; };
 template <> struct ModArg<true> { typedef ScoreMod type; };
 
+// What stands in rows that are not a member's neighbours must not reach its sums, and a product over a block's entries lets it: 0 x NaN.  So a wavefront whose
+// sums (of any member) are not finite walks its tile once more (CAREFUL), with products that add the existing pairs alone and with every
+// value of a pair that does not exist set to zero.  Rows that are finite, as nearly all are, cost this one look at the sums.
+template <int N> __device__ __forceinline__ float tile_odd(const floatx4v (&acc)[N]) {         // 0, or NaN where something is infinite or NaN
+    float x = 0.f;
+#pragma unroll
+    for (int nb = 0; nb < N; ++nb)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x = fmaf(acc[nb][r], 0.f, x);
+    return x;
+}
+__device__ __forceinline__ bool tile_any_odd(float x) { return __builtin_amdgcn_ballot_w64(x != 0.f) != 0; }
+template <bool ON> __device__ __forceinline__ float pair_if(int mask, int bit, float x) {        // x; with ON, 0 of a pair that does not exist
+    if constexpr (ON) return where_pair_or_zero(mask, bit, x);
+    else return x;
+}
+__device__ __forceinline__ float4 tile_four(const float4 &x) { return x; }
+__device__ __forceinline__ float4 tile_four(const uint2 &x) {
+    return make_float4(__uint_as_float(x.x << 16), __uint_as_float(x.x & 0xffff0000u), __uint_as_float(x.y << 16), __uint_as_float(x.y & 0xffff0000u));
+}
+// acc[nb][i] (member 4 g + i, column 4 c + nb) += w x rows over the pairs that exist; lane (c, g), register r: weight of member c with the entry whose
+// columns 4 c .. 4 c + 3 it has and whose mask is mk[r]
+template <typename Row> __device__ __forceinline__ void tile_axpy_pairs(const float (&w)[4], const int (&mk)[4], const Row (&rows)[4], int c, int g, floatx4v (&acc)[4]) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const float4 mine = tile_four(rows[r]);
+#pragma unroll 1
+        for (int from = 0; from < 4; ++from) {
+            const int at = 16 * from + c, mask = lane_bcast(mk[r], 16 * from);
+            const float row[4] = {lane_bcast(mine.x, at), lane_bcast(mine.y, at), lane_bcast(mine.z, at), lane_bcast(mine.w, at)};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float x = lane_bcast(w[r], 16 * from + 4 * g + i);
+#pragma unroll
+                for (int nb = 0; nb < 4; ++nb) acc[nb][i] = (mask >> (4 * g + i)) & 1 ? fmaf(x, row[nb], acc[nb][i]) : acc[nb][i];
+            }
+        }
+    }
+}
+
 // s (base-2 units) and ds/du of four pairs whose q.k (+ term) is x; pos_e: positions of the pairs' entries.
 // |u / cap| <= 1/2, where nearly all scores lie (a score is a few units, a cap tens): tanh z = z + z w (c0 + c1 w + c2 w^2 + c3 w^3) with w = z^2,
 // fitted by weighted least squares to the relative error, 1.5e-8 (1.25 half steps of float32 as evaluated); the factor scale / cap sits in the
@@ -1075,6 +1118,9 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(4))) 
         float bz[BIAS ? 4 : 1];
         float pos;                                                // of entry c, in the first lane group
     };
+    auto walk = [&](auto again) __attribute__((always_inline)) {
+    constexpr bool CAREFUL = decltype(again)::value;
+    if constexpr (CAREFUL) tile_ask_entries(P, t.p_begin, min(TILE_CHUNK, t.p_end - t.p_begin), t.lane, er);
     for (int p0 = t.p_begin; p0 < t.p_end; p0 += TILE_CHUNK) {
         const int cnt = min(TILE_CHUNK, t.p_end - p0), nblk = (cnt + TILE_R - 1) / TILE_R;
         if (p0 != t.p_begin) tile_ask_entries(P, p0, cnt, t.lane, er);
@@ -1155,24 +1201,37 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(4))) 
                 if constexpr (DROP)
                     pr[r] *= dropout_keep((uint32_t)B.xe[DROP ? r : 0] * (uint32_t)Hs + (uint32_t)t.head, drop_seed, drop_thr, drop_inv);
             }
-            tile_axpy_upto(pr, B.vr, acc, B.nv);
+            if constexpr (CAREFUL) tile_axpy_pairs(pr, B.mk, B.vr, c, g, acc);
+            else tile_axpy_upto(pr, B.vr, acc, B.nv);
         };
         auto issue = [&](Blk &B, int b) { issue_k(B, b); issue_rest(B, b); };
         if constexpr (!AHEAD) tile_walk<Blk>(nblk, issue, compute);
         else tile_walk_first_ahead<Blk>(nblk, issue_k, issue_rest, compute, [&]() { if (p0 == t.p_begin) tile_load16<NARROW>(qrow, qb, g, nw); });
         wave_lds_fence();                                         // the piece is read to the end before the next one is staged
     }
+    };
+    walk(std::false_type{});
+    if constexpr (MOD) {
+        if (tile_any_odd(tile_odd(acc))) {      // (what does not exist must not reach the sums: tile_odd)
+#pragma unroll
+            for (int nb = 0; nb < 4; ++nb) acc[nb] = floatx4v{0.f, 0.f, 0.f, 0.f};
+            mref = M_INIT_LOG2;
+            lrun = 0.f;
+            fresh = true;
+            walk(std::true_type{});
+        }
+    }
     float lt = groups_sum(lrun);                                 // denominator of member c, in its four lanes
     if constexpr (SP > 1) {
         static_assert(TILE_PART_FWD_FLOATS <= TILE_R * TILE_KT_STRIDE, "a part fits its wavefront's piece");
-        tile_meet_forward<SP, H, D, NARROW>(kt, kt_lds[t.wv % (HW / SP)], (HW / SP) * TILE_R * TILE_KT_STRIDE, t, acc, mref, lt, o, ws_acc, nw, o_keep);
+        tile_meet_forward<SP, H, D, NARROW, MOD>(kt, kt_lds[t.wv % (HW / SP)], (HW / SP) * TILE_R * TILE_KT_STRIDE, t, acc, mref, lt, o, ws_acc, nw, o_keep);
         if (t.part != 0) return;
     } else {
-        tile_store_rows<H, D, true, NARROW>(t, acc, lt > 0.f ? 1.f / lt : 0.f, o, ws_acc, nw, o_keep);
+        tile_store_rows<H, D, true, NARROW>(t, acc, has_sum<MOD>(lt) ? 1.f / lt : 0.f, o, ws_acc, nw, o_keep);
     }
     if (g == 0 && t.member.x >= 0) {                              // lanes 0 .. 15: one member each
         if (t.member.y < 0) {
-            lse[(size_t)t.member.x * Hs + t.head] = lt > 0.f ? mref + log2f(lt) : 0.f;
+            lse[(size_t)t.member.x * Hs + t.head] = has_sum<MOD>(lt) ? mref + log2f(lt) : 0.f;
         } else {
             ws_ml[((size_t)t.member.y * Hs + t.head) * 2] = mref;
             ws_ml[((size_t)t.member.y * Hs + t.head) * 2 + 1] = lt;
@@ -1290,6 +1349,9 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP 
         float bz[BIAS ? 4 : 1];
         float pos;                                                // of entry c, in the first lane group
     };
+    auto walk = [&](auto again) __attribute__((always_inline)) {
+    constexpr bool CAREFUL = decltype(again)::value;
+    if constexpr (CAREFUL) tile_ask_entries(P, t.p_begin, min(TILE_CHUNK, t.p_end - t.p_begin), t.lane, er);
     for (int p0 = t.p_begin; p0 < t.p_end; p0 += TILE_CHUNK) {
         const int cnt = min(TILE_CHUNK, t.p_end - p0), nblk = (cnt + TILE_R - 1) / TILE_R;
         if (p0 != t.p_begin) tile_ask_entries(P, p0, cnt, t.lane, er);
@@ -1362,8 +1424,8 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP 
                     mt = dropout_keep((uint32_t)B.xe[DROP ? r : 0] * (uint32_t)Hs + (uint32_t)t.head, drop_seed, drop_thr, drop_inv);
                 if constexpr (MOD) {
                     ds[r] = where_pair_or_zero(mask[r], c, pe * (dp[r] * mt - delta));
-                    if (md.part) slope_sum = fmaf(ds[r], fabsf(pos_m - pos_e[r]), slope_sum);
-                    ds[r] *= du[r] * scale;
+                    if (md.part) slope_sum += pair_if<CAREFUL>(mask[r], c, ds[r] * fabsf(pos_m - pos_e[r]));
+                    ds[r] = pair_if<CAREFUL>(mask[r], c, ds[r] * (du[r] * scale));
                 } else {
                     ds[r] = pe * (dp[r] * mt - delta) * scale;
                 }
@@ -1373,10 +1435,21 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP 
                     if constexpr (BIAS) ds_out[tile_bias_at<H, BIAS>(P, t.head, B.xe[BIAS == 1 ? r : 0], number[r])] = ds[r];   // dL/d(score before scaling)
                 }
             }
-            tile_axpy_upto(ds, B.kc, acc, B.nv);
+            if constexpr (CAREFUL) tile_axpy_pairs(ds, mask, B.kc, c, g, acc);
+            else tile_axpy_upto(ds, B.kc, acc, B.nv);
         };
         tile_walk<Blk>(nblk, issue, compute);
         wave_lds_fence();
+    }
+    };
+    walk(std::false_type{});
+    if constexpr (MOD) {
+        if (tile_any_odd(tile_odd(acc) + slope_sum * 0.f)) {      // (what does not exist must not reach the sums: tile_odd)
+#pragma unroll
+            for (int nb = 0; nb < 4; ++nb) acc[nb] = floatx4v{0.f, 0.f, 0.f, 0.f};
+            slope_sum = 0.f;
+            walk(std::true_type{});
+        }
     }
     if constexpr (MOD) tile_put_slope_part<SP>(md, t, Hs, slope_sum);
     if constexpr (SP > 1) {
@@ -1407,7 +1480,7 @@ __device__ __forceinline__ void tile_pair_positions(const bpt_plan &P, int entry
     const intx4u x = *reinterpret_cast<const intx4u *>(P.grp_pairs + (size_t)entry * TILE_R + 4 * g);
     pos[0] = x[0]; pos[1] = x[1]; pos[2] = x[2]; pos[3] = x[3];
 }
-template <typename T, int H, int D, int HW, bool NARROW = false, int SP = 1>
+template <typename T, int H, int D, int HW, bool NARROW = false, int SP = 1, bool MOD = false>
 __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(4))) void k_attn_bwd_src_tile(
     bpt_plan P, const T *__restrict__ q, const T *__restrict__ d_o, const float2 *__restrict__ pds, T *__restrict__ dk, T *__restrict__ dv,
     float *__restrict__ ws_dk, float *__restrict__ ws_dv, Narrow nw) {
@@ -1439,6 +1512,12 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(4))) 
     auto positions = [&](int first_entry) { tile_pair_positions(P, min(first_entry + c, t.p_end - 1), g, pos); };
     if (t.p_end > t.p_begin) positions(t.p_begin);
     issue_loads_first();
+    auto walk = [&](auto again) __attribute__((always_inline)) {
+    constexpr bool CAREFUL = decltype(again)::value;
+    if constexpr (CAREFUL) {
+        tile_ask_entries(P, t.p_begin, min(TILE_CHUNK, t.p_end - t.p_begin), t.lane, er);
+        positions(t.p_begin);
+    }
     for (int p0 = t.p_begin; p0 < t.p_end; p0 += TILE_CHUNK) {
         const int cnt = min(TILE_CHUNK, t.p_end - p0), nblk = (cnt + TILE_R - 1) / TILE_R;
         if (p0 != t.p_begin) tile_ask_entries(P, p0, cnt, t.lane, er);
@@ -1474,8 +1553,13 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(4))) 
                 ds[r] = where_pair_or_zero(B.mk[r], c, w.y);
             }
             wave_lds_fence();                                     // (read before the next block's are written)
-            tile_axpy_upto(ds, B.qr, ak, B.nv);
-            tile_axpy_upto(pe, B.dr, av, B.nv);
+            if constexpr (CAREFUL) {
+                tile_axpy_pairs(ds, B.mk, B.qr, c, g, ak);
+                tile_axpy_pairs(pe, B.mk, B.dr, c, g, av);
+            } else {
+                tile_axpy_upto(ds, B.qr, ak, B.nv);
+                tile_axpy_upto(pe, B.dr, av, B.nv);
+            }
         };
         for (int b = 0; b < nblk; ++b) {
             Blk B;
@@ -1492,6 +1576,15 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(4))) 
             issue_loads_first();
         }
         wave_lds_fence();
+    }
+    };
+    walk(std::false_type{});
+    if constexpr (MOD) {
+        if (tile_any_odd(tile_odd(ak) + tile_odd(av))) {      // (what does not exist must not reach the sums: tile_odd)
+#pragma unroll
+            for (int nb = 0; nb < 4; ++nb) { ak[nb] = floatx4v{0.f, 0.f, 0.f, 0.f}; av[nb] = floatx4v{0.f, 0.f, 0.f, 0.f}; }
+            walk(std::true_type{});
+        }
     }
     if constexpr (SP > 1) {
         constexpr int NEXT = (HW / SP) * PIECE;
@@ -1653,6 +1746,23 @@ __device__ __forceinline__ void tile_axpy_rows_bf16(const Bf4 &w, const char *kt
         acc[nb] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(cols, w.v, acc[nb], 0, 0, 0);
     }
 }
+// ... over the pairs that exist (tile_odd), lane (c, g), register r of w and mk: entry 4 g + r
+__device__ __forceinline__ void tile_axpy_pairs_bf16(const float (&w)[4], const int (&mk)[4], const char *kt, int c, int g, floatx4v (&acc)[4]) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll 1
+        for (int from = 0; from < 4; ++from) {
+            const int e = 4 * from + r, at = e * 128 + 16 * ((g >> 1) ^ piece_turn(e)) + 8 * (g & 1), mask = lane_bcast(mk[r], 16 * from);
+            const float x = lane_bcast(w[r], 16 * from + c);
+#pragma unroll
+            for (int nb = 0; nb < 4; ++nb) {
+                const float4 row = tile_four(*reinterpret_cast<const uint2 *>(kt + (at ^ (32 * nb))));
+                const float cols[4] = {row.x, row.y, row.z, row.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[nb][i] = (mask >> c) & 1 ? fmaf(x, cols[i], acc[nb][i]) : acc[nb][i];
+            }
+        }
+}
 // Such sums through LDS (TILE_R * TILE_TURN_STRIDE floats): into the tile kernels' other order (lane (c, g), register r: columns 4 c .. 4 c + 3
 // of member 4 g + r), or to where the members' rows go.
 constexpr int TILE_TURN_STRIDE = 68;
@@ -1742,6 +1852,9 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP 
         float bz[BIAS ? 4 : 1];
         float pos;                                                // of entry c, in the first lane group
     };
+    auto walk = [&](auto again) __attribute__((always_inline)) {
+    constexpr bool CAREFUL = decltype(again)::value;
+    if constexpr (CAREFUL) tile_ask_entries(P, t.p_begin, min(TILE_CHUNK, t.p_end - t.p_begin), t.lane, er);
     for (int p0 = t.p_begin; p0 < t.p_end; p0 += TILE_CHUNK) {
         const int cnt = min(TILE_CHUNK, t.p_end - p0), nblk = (cnt + TILE_R - 1) / TILE_R;
         if (p0 != t.p_begin) tile_ask_entries(P, p0, cnt, t.lane, er);
@@ -1769,7 +1882,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP 
         Blk B;
         issue(B, 0);
         issue_loads_first();
-        if (p0 == t.p_begin) {
+        if (!CAREFUL && p0 == t.p_begin) {
             tile_put_rows_bf16(k_lds, qr, t.lane);
             wave_lds_fence();
             tile_operand_bf16(k_lds, c, g, qb);
@@ -1828,22 +1941,38 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP 
                 if constexpr (DROP)
                     pr[r] *= dropout_keep((uint32_t)xe[DROP ? r : 0] * (uint32_t)H + (uint32_t)t.head, drop_seed, drop_thr, drop_inv);
             }
-            Bf4 pa;
-            pa.u[0] = pack_bf16(pr[0], pr[1]);
-            pa.u[1] = pack_bf16(pr[2], pr[3]);
-            tile_axpy_rows_bf16(pa, v_lds, c, g, acc);
+            if constexpr (CAREFUL) {
+                tile_axpy_pairs_bf16(pr, mk, v_lds, c, g, acc);
+            } else {
+                Bf4 pa;
+                pa.u[0] = pack_bf16(pr[0], pr[1]);
+                pa.u[1] = pack_bf16(pr[2], pr[3]);
+                tile_axpy_rows_bf16(pa, v_lds, c, g, acc);
+            }
             wave_lds_fence();                                     // (read before the next block's are written)
             issue_loads_first();
+        }
+    }
+    };
+    walk(std::false_type{});
+    if constexpr (MOD) {
+        if (tile_any_odd(tile_odd(acc))) {      // (what does not exist must not reach the sums: tile_odd)
+#pragma unroll
+            for (int nb = 0; nb < 4; ++nb) acc[nb] = floatx4v{0.f, 0.f, 0.f, 0.f};
+            mref = M_INIT_LOG2;
+            lrun = 0.f;
+            fresh = true;
+            walk(std::true_type{});
         }
     }
     float lt = groups_sum(lrun);
     if constexpr (SP > 1) {
         tile_sums_by_row(piece[t.wv], acc, c, g);
-        tile_meet_forward<SP, H, D, false>(piece[t.wv], piece[t.wv % (HW / SP)], (HW / SP) * PIECE, t, acc, mref, lt, o, ws_acc, nw, static_cast<bf16_t *>(nullptr));
+        tile_meet_forward<SP, H, D, false, MOD>(piece[t.wv], piece[t.wv % (HW / SP)], (HW / SP) * PIECE, t, acc, mref, lt, o, ws_acc, nw, static_cast<bf16_t *>(nullptr));
         if (t.part != 0) return;
     } else {
         if (t.member.y < 0) {                                     // (segments of a split row are stored as summed up)
-            const float inv = lt > 0.f ? 1.f / lt : 0.f;
+            const float inv = has_sum<MOD>(lt) ? 1.f / lt : 0.f;
 #pragma unroll
             for (int nb = 0; nb < 4; ++nb) acc[nb] *= inv;
         }
@@ -1851,7 +1980,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP 
     }
     if (g == 0 && t.member.x >= 0) {
         if (t.member.y < 0) {
-            lse[(size_t)t.member.x * H + t.head] = lt > 0.f ? mref + log2f(lt) : 0.f;
+            lse[(size_t)t.member.x * H + t.head] = has_sum<MOD>(lt) ? mref + log2f(lt) : 0.f;
         } else {
             ws_ml[((size_t)t.member.y * H + t.head) * 2] = mref;
             ws_ml[((size_t)t.member.y * H + t.head) * 2 + 1] = lt;
@@ -1943,13 +2072,16 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(MOD ?
     float dp_sum = 0.f, far_sum = 0.f;
     floatx4v pk[FIX ? 4 : 1];                                     // sum of p du K, laid out as acc
 #pragma unroll
-    for (int nb = 0; nb < (FIX ? 4 : 0); ++nb) pk[nb] = floatx4v{0.f, 0.f, 0.f, 0.f};
+    for (int nb = 0; nb < (FIX ? 4 : 1); ++nb) pk[nb] = floatx4v{0.f, 0.f, 0.f, 0.f};
     struct Blk {
         uintx4v kr[2], vr[2];
         int xe[DROP || BIAS == 1 ? 4 : 1];
         float bz[BIAS ? 4 : 1];
         float pos;                                                // of entry c, in the first lane group
     };
+    auto walk = [&](auto again) __attribute__((always_inline)) {
+    constexpr bool CAREFUL = decltype(again)::value;
+    if constexpr (CAREFUL) tile_ask_entries(P, t.p_begin, min(TILE_CHUNK, t.p_end - t.p_begin), t.lane, er);
     for (int p0 = t.p_begin; p0 < t.p_end; p0 += TILE_CHUNK) {
         const int cnt = min(TILE_CHUNK, t.p_end - p0), nblk = (cnt + TILE_R - 1) / TILE_R;
         if (p0 != t.p_begin) tile_ask_entries(P, p0, cnt, t.lane, er);
@@ -2023,12 +2155,12 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(MOD ?
                 if constexpr (MOD) {
                     const float x = where_pair_or_zero(mk[r], c, pe * (dp[r] * mt));
                     ds[r] = fmaf(-pe, delta, x);
-                    if (md.part) slope_sum = fmaf(ds[r], fabsf(pos_m - pos_e[r]), slope_sum);
-                    ds[r] *= du[r] * scale;
+                    if (md.part) slope_sum += pair_if<CAREFUL>(mk[r], c, ds[r] * fabsf(pos_m - pos_e[r]));
+                    ds[r] = pair_if<CAREFUL>(mk[r], c, ds[r] * (du[r] * scale));
                     if constexpr (FIX) {
                         dp_sum += x;
-                        if (md.part) far_sum = fmaf(pe, fabsf(pos_m - pos_e[r]), far_sum);
-                        pdu[r] = pe * (du[r] * scale);
+                        if (md.part) far_sum += pair_if<CAREFUL>(mk[r], c, pe * fabsf(pos_m - pos_e[r]));
+                        pdu[r] = pair_if<CAREFUL>(mk[r], c, pe * (du[r] * scale));
                     }
                 } else {
                     ds[r] = pe * (dp[r] * mt - delta) * scale;
@@ -2039,17 +2171,34 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(MOD ?
                     if constexpr (BIAS) ds_out[tile_bias_at<H, BIAS>(P, t.head, xe[BIAS == 1 ? r : 0], pos[r])] = ds[r];   // dL/d(score before scaling)
                 }
             }
-            Bf4 da;
-            da.u[0] = pack_bf16(ds[0], ds[1]);
-            da.u[1] = pack_bf16(ds[2], ds[3]);
-            tile_axpy_rows_bf16(da, k_lds, c, g, acc);
-            if constexpr (FIX) {
-                da.u[0] = pack_bf16(pdu[0], pdu[1]);
-                da.u[1] = pack_bf16(pdu[2], pdu[3]);
-                tile_axpy_rows_bf16(da, k_lds, c, g, pk);
+            if constexpr (CAREFUL) {
+                tile_axpy_pairs_bf16(ds, mk, k_lds, c, g, acc);
+                if constexpr (FIX) tile_axpy_pairs_bf16(pdu, mk, k_lds, c, g, pk);
+            } else {
+                Bf4 da;
+                da.u[0] = pack_bf16(ds[0], ds[1]);
+                da.u[1] = pack_bf16(ds[2], ds[3]);
+                tile_axpy_rows_bf16(da, k_lds, c, g, acc);
+                if constexpr (FIX) {
+                    da.u[0] = pack_bf16(pdu[0], pdu[1]);
+                    da.u[1] = pack_bf16(pdu[2], pdu[3]);
+                    tile_axpy_rows_bf16(da, k_lds, c, g, pk);
+                }
             }
             wave_lds_fence();                                     // (read before the next block's are written)
             issue_loads_first();
+        }
+    }
+    };
+    walk(std::false_type{});
+    if constexpr (MOD) {
+        if (tile_any_odd(tile_odd(acc) + tile_odd(pk) + (slope_sum + far_sum) * 0.f)) {      // (what does not exist must not reach the sums: tile_odd)
+#pragma unroll
+            for (int nb = 0; nb < 4; ++nb) acc[nb] = floatx4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int nb = 0; nb < (FIX ? 4 : 1); ++nb) pk[nb] = floatx4v{0.f, 0.f, 0.f, 0.f};
+            slope_sum = far_sum = dp_sum = 0.f;
+            walk(std::true_type{});
         }
     }
     if constexpr (FIX) {
@@ -2067,7 +2216,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(MOD ?
             }
         }
         const bool segment = t.member.y >= 0;
-        const float better = segment ? delta : whole, less = delta - better;
+        const float better = segment ? delta : whole, less = delta == delta ? delta - better : 0.f;      // (NaN: the pairs, if there are any, are NaN as they are)
         slope_sum = fmaf(less, far_sum, slope_sum);
 #pragma unroll
         for (int nb = 0; nb < 4; ++nb) acc[nb] += less * pk[nb];
@@ -2134,6 +2283,9 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(MOD ?
         int xe[DROP ? 4 : 1];
         float pos;                                                // of entry c, in the first lane group
     };
+    auto walk = [&](auto again) __attribute__((always_inline)) {
+    constexpr bool CAREFUL = decltype(again)::value;
+    if constexpr (CAREFUL) tile_ask_entries(P, t.p_begin, min(TILE_CHUNK, t.p_end - t.p_begin), t.lane, er);
     for (int p0 = t.p_begin; p0 < t.p_end; p0 += TILE_CHUNK) {
         const int cnt = min(TILE_CHUNK, t.p_end - p0), nblk = (cnt + TILE_R - 1) / TILE_R;
         if (p0 != t.p_begin) tile_ask_entries(P, p0, cnt, t.lane, er);
@@ -2199,26 +2351,42 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(MOD ?
                 if constexpr (DROP)
                     pr[r] *= dropout_keep((uint32_t)B.xe[DROP ? r : 0] * (uint32_t)Hs + (uint32_t)t.head, drop_seed, drop_thr, drop_inv);
             }
-            Bf4 pa;
-            pa.u[0] = pack_bf16(pr[0], pr[1]);
-            pa.u[1] = pack_bf16(pr[2], pr[3]);
-            tile_axpy_bf16(pa, B.vr, acc);
+            if constexpr (CAREFUL) {
+                tile_axpy_pairs(pr, B.mk, B.vr, c, g, acc);
+            } else {
+                Bf4 pa;
+                pa.u[0] = pack_bf16(pr[0], pr[1]);
+                pa.u[1] = pack_bf16(pr[2], pr[3]);
+                tile_axpy_bf16(pa, B.vr, acc);
+            }
         };
         auto issue = [&](Blk &B, int b) { issue_k(B, b); issue_rest(B, b); };
         if constexpr (DROP) tile_walk<Blk>(nblk, issue, compute);      // (the K rows ahead: eight registers more)
         else tile_walk_first_ahead<Blk>(nblk, issue_k, issue_rest, compute, []() {});
         wave_lds_fence();
     }
+    };
+    walk(std::false_type{});
+    if constexpr (MOD) {
+        if (tile_any_odd(tile_odd(acc))) {      // (what does not exist must not reach the sums: tile_odd)
+#pragma unroll
+            for (int nb = 0; nb < 4; ++nb) acc[nb] = floatx4v{0.f, 0.f, 0.f, 0.f};
+            mref = M_INIT_LOG2;
+            lrun = 0.f;
+            fresh = true;
+            walk(std::true_type{});
+        }
+    }
     float lt = groups_sum(lrun);
     if constexpr (SP > 1) {
-        tile_meet_forward<SP, H, D, true>(piece[t.wv], piece[t.wv % (HW / SP)], (HW / SP) * PIECE, t, acc, mref, lt, o, ws_acc, nw, o_keep);
+        tile_meet_forward<SP, H, D, true, MOD>(piece[t.wv], piece[t.wv % (HW / SP)], (HW / SP) * PIECE, t, acc, mref, lt, o, ws_acc, nw, o_keep);
         if (t.part != 0) return;
     } else {
-        tile_store_rows<H, D, true, true>(t, acc, lt > 0.f ? 1.f / lt : 0.f, o, ws_acc, nw, o_keep);
+        tile_store_rows<H, D, true, true>(t, acc, has_sum<MOD>(lt) ? 1.f / lt : 0.f, o, ws_acc, nw, o_keep);
     }
     if (g == 0 && t.member.x >= 0) {
         if (t.member.y < 0) {
-            lse[(size_t)t.member.x * Hs + t.head] = lt > 0.f ? mref + log2f(lt) : 0.f;
+            lse[(size_t)t.member.x * Hs + t.head] = has_sum<MOD>(lt) ? mref + log2f(lt) : 0.f;
         } else {
             ws_ml[((size_t)t.member.y * Hs + t.head) * 2] = mref;
             ws_ml[((size_t)t.member.y * Hs + t.head) * 2 + 1] = lt;
@@ -2334,7 +2502,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP 
 }
 
 constexpr int TILE_WT_STRIDE_BF16 = 20;
-template <int H, int D, int HW, int WPE, bool NARROW = false, int SP = 1>
+template <int H, int D, int HW, int WPE, bool NARROW = false, int SP = 1, bool MOD = false>
 __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(WPE))) void k_attn_bwd_src_tile_bf16(
     bpt_plan P, const bf16_t *__restrict__ q, const bf16_t *__restrict__ d_o, const uint32_t *__restrict__ pds, bf16_t *__restrict__ dk,
     bf16_t *__restrict__ dv, float *__restrict__ ws_dk, float *__restrict__ ws_dv, Narrow nw) {
@@ -2358,6 +2526,8 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(WPE))
         uint32_t w[4];                                            // (p, ds) of the pairs (entry c, member 4 g + r)
         int mk[4];                                                // bit c of mk[r]: the pair (entry 4 g + r, member c) exists
     };
+    auto walk = [&](auto again) __attribute__((always_inline)) {
+    constexpr bool CAREFUL = decltype(again)::value;
     for (int p0 = t.p_begin; p0 < t.p_end; p0 += TILE_CHUNK) {
         const int cnt = min(TILE_CHUNK, t.p_end - p0), nblk = (cnt + TILE_R - 1) / TILE_R;
         tile_stage_entries(P, ent, p0, cnt, t.lane);
@@ -2398,14 +2568,31 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(WPE))
             wave_lds_fence();                                     // (read before the next block's are written)
 #pragma unroll
             for (int r = 0; r < 4; ++r) w[r] &= (uint32_t)__builtin_amdgcn_sbfe(B.mk[r], c, 1);       // the scratch of pairs that do not exist is not initialised
-            Bf4 pa, da;
-            pa.u[0] = pack_lo16(w[0], w[1]); pa.u[1] = pack_lo16(w[2], w[3]);
-            da.u[0] = pack_hi16(w[0], w[1]); da.u[1] = pack_hi16(w[2], w[3]);
-            tile_axpy_bf16(da, B.qr, ak);
-            tile_axpy_bf16(pa, B.dr, av);
+            if constexpr (CAREFUL) {
+                float pe[4], ds[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) { pe[r] = __uint_as_float(w[r] << 16); ds[r] = __uint_as_float(w[r] & 0xffff0000u); }
+                tile_axpy_pairs(ds, B.mk, B.qr, c, g, ak);
+                tile_axpy_pairs(pe, B.mk, B.dr, c, g, av);
+            } else {
+                Bf4 pa, da;
+                pa.u[0] = pack_lo16(w[0], w[1]); pa.u[1] = pack_lo16(w[2], w[3]);
+                da.u[0] = pack_hi16(w[0], w[1]); da.u[1] = pack_hi16(w[2], w[3]);
+                tile_axpy_bf16(da, B.qr, ak);
+                tile_axpy_bf16(pa, B.dr, av);
+            }
         };
         tile_walk<Blk>(nblk, issue, compute);
         wave_lds_fence();
+    }
+    };
+    walk(std::false_type{});
+    if constexpr (MOD) {
+        if (tile_any_odd(tile_odd(ak) + tile_odd(av))) {      // (what does not exist must not reach the sums: tile_odd)
+#pragma unroll
+            for (int nb = 0; nb < 4; ++nb) { ak[nb] = floatx4v{0.f, 0.f, 0.f, 0.f}; av[nb] = floatx4v{0.f, 0.f, 0.f, 0.f}; }
+            walk(std::true_type{});
+        }
     }
     if constexpr (SP > 1) {
         constexpr int NEXT = (HW / SP) * PIECE;
@@ -2485,6 +2672,9 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(MOD ?
         int xe[DROP ? 4 : 1];
         float pos;                                                // of entry c, in the first lane group
     };
+    auto walk = [&](auto again) __attribute__((always_inline)) {
+    constexpr bool CAREFUL = decltype(again)::value;
+    if constexpr (CAREFUL) tile_ask_entries(P, t.p_begin, min(TILE_CHUNK, t.p_end - t.p_begin), t.lane, er);
     for (int p0 = t.p_begin; p0 < t.p_end; p0 += TILE_CHUNK) {
         const int cnt = min(TILE_CHUNK, t.p_end - p0), nblk = (cnt + TILE_R - 1) / TILE_R;
         if (p0 != t.p_begin) tile_ask_entries(P, p0, cnt, t.lane, er);
@@ -2538,13 +2728,27 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(MOD ?
                 ds[r] = where_pair_or_zero(mk[r], c, MOD ? p * (dp[r] * mt - delta_e[r]) * (du[r] * scale) : p * (dp[r] * mt - delta_e[r]) * scale);
                 pe[r] = p * mt;
             }
-            Bf4 pa, da;
-            da.u[0] = pack_bf16(ds[0], ds[1]); da.u[1] = pack_bf16(ds[2], ds[3]);
-            pa.u[0] = pack_bf16(pe[0], pe[1]); pa.u[1] = pack_bf16(pe[2], pe[3]);
-            tile_axpy_rows_bf16(da, q_lds, c, g, ak);
-            tile_axpy_rows_bf16(pa, d_lds, c, g, av);
+            if constexpr (CAREFUL) {
+                tile_axpy_pairs_bf16(ds, mk, q_lds, c, g, ak);
+                tile_axpy_pairs_bf16(pe, mk, d_lds, c, g, av);
+            } else {
+                Bf4 pa, da;
+                da.u[0] = pack_bf16(ds[0], ds[1]); da.u[1] = pack_bf16(ds[2], ds[3]);
+                pa.u[0] = pack_bf16(pe[0], pe[1]); pa.u[1] = pack_bf16(pe[2], pe[3]);
+                tile_axpy_rows_bf16(da, q_lds, c, g, ak);
+                tile_axpy_rows_bf16(pa, d_lds, c, g, av);
+            }
             wave_lds_fence();                                     // (read before the next block's are written)
             issue_loads_first();
+        }
+    }
+    };
+    walk(std::false_type{});
+    if constexpr (MOD) {
+        if (tile_any_odd(tile_odd(ak) + tile_odd(av))) {      // (what does not exist must not reach the sums: tile_odd)
+#pragma unroll
+            for (int nb = 0; nb < 4; ++nb) { ak[nb] = floatx4v{0.f, 0.f, 0.f, 0.f}; av[nb] = floatx4v{0.f, 0.f, 0.f, 0.f}; }
+            walk(std::true_type{});
         }
     }
     float *const turn = reinterpret_cast<float *>(q_lds);

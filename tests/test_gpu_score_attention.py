@@ -121,7 +121,9 @@ def reference(c, drop=None):
     if "table" in c:
         per = (du[..., None] * qe).sum(1), (du_b[..., None] * qe.abs()).sum(1) + (n_e * h / 30 + 64) * E * (du.abs()[..., None] * qe.abs()).sum(1)
         out["dtable"] = tuple(seg(y, c["etype"], 30) for y in per)
-        out["dq"] = (out["dq"][0], out["dq"][1] + F * out["dq"][0].abs() + F * seg(du.abs()[..., None] * ke.abs(), dst, n_q))      # dq is stored, read and added to
+        # dq is formed in two steps, sum ds k stored in the result's type, then read and sum ds table added: ds is rounded on its way into the first alone, and the
+        # sum is once more where it is stored, F of sum |ds| |k| each (also where k and table cancel in sum ds (k + table), which the terms above go by), of ds as computed
+        out["dq"] = (out["dq"][0], out["dq"][1] + F * out["dq"][0].abs() + 2 * F * seg((du.abs() + du_b)[..., None] * ke.abs(), dst, n_q))
     return out
 
 
@@ -295,6 +297,43 @@ def test_gradients_against_differences():
         want = ((value[0] - value[1]) / (2 * step)).item()
         have = (got["d" + n].cpu().double() * way.double()).sum().item()
         assert abs(have - want) <= 0.02 * max(abs(want), got["d" + n].norm().item() / way.numel() ** 0.5), (n, have, want)
+
+
+def close_where_finite(got, want, name, dtype):
+    """As close(), of results that are infinite or NaN where the formula's are, and only there."""
+    value, bound = want
+    got = got.detach().cpu().double()
+    fine = value.isfinite()
+    assert torch.equal(got.isfinite(), fine), f"{name}: {int((~got.isfinite() & fine).sum())} of {int(fine.sum())} finite results are not, {int((got.isfinite() & ~fine).sum())} are that must not be"
+    if fine.any():
+        close(got[fine], (value[fine], bound[fine]), name, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("heads,d,rel", [(8, 64, False), (6, 50, False), (8, 64, True)])
+@pytest.mark.parametrize("kind", [("bpt", 300, 4), ("random", 1000, 300), ("memory", 40, 300), ("bpt", 5000, 4)], ids=str)
+@pytest.mark.parametrize("where", ["v", "k", "q", "do", "pos"])
+def test_what_stands_in_rows_that_are_not_neighbours(where, kind, heads, d, rel, dtype):
+    """One row (the last of the second third; of positions, one without edges) is infinite in its first column and NaN in its second."""
+    c = make(kind, heads, d, dtype, 30.0, True, rel=rel)
+    c = {n: t.clone() if torch.is_tensor(t) and n not in ("pos_q", "pos_k") else t for n, t in c.items()}
+    if where == "pos":
+        lone = np.setdiff1d(np.arange(c["q"].size(0)), np.concatenate([c["dst"].numpy(), c["src"].numpy()] if c["q"].size(0) == c["k"].size(0) else [c["dst"].numpy()]))
+        if not len(lone):
+            pytest.skip("every row has edges")
+        same = c["pos_q"] is c["pos_k"]
+        c["pos_q"] = c["pos_q"].clone()
+        c["pos_q"][torch.from_numpy(lone)] = torch.tensor([float("inf"), float("nan")]).repeat(len(lone))[:len(lone)]
+        if same:
+            c["pos_k"] = c["pos_q"]
+    else:
+        row = c[where].size(0) * 2 // 3 - 1
+        c[where][row, :, 0], c[where][row, :, 1] = float("inf"), float("nan")
+    args = graph_args(c["src"].numpy(), c["dst"].numpy(), c["q"].size(0), c["k"].size(0))
+    ref = reference(c)
+    got = run(c, args, True)
+    for n, want in ref.items():
+        close_where_finite(got[n], want, n, torch.float32 if n == "dslopes" else c["q"].dtype)
 
 
 def test_without_options_is_the_plain_layer():

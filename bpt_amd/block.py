@@ -30,17 +30,17 @@ from .op import (add_layer_norm, bpt_attention, edge_type_embedding, masked_mm, 
 __all__ = ["PositionwiseFeedForward", "BPTBlock", "BPTMemBlock"]
 
 
-def _as_it_is(norm):
-    """Whether a call of norm is LayerNorm's own forward and nothing else."""
-    return (type(norm) is nn.LayerNorm and "forward" not in norm.__dict__ and len(norm.normalized_shape) == 1
-            and not (norm._forward_hooks or norm._forward_pre_hooks or norm._backward_hooks or norm._backward_pre_hooks)
+def _as_it_is(module, kind):
+    """Whether a call of module is the forward of kind, a class of torch.nn, and nothing else."""
+    return (type(module) is kind and "forward" not in module.__dict__
+            and not (module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks)
             and not nn.modules.module._has_any_global_hook())
 
 
 def _add_norm(norm, x, residual, fused):
     """norm(x + residual) (attention.py:79, :81), by add_layer_norm where that computes the same: a LayerNorm over the last axis as it is, GPU tensors
     of one type, nothing that casts, traces or transforms."""
-    if (fused and _as_it_is(norm) and x.is_cuda and x.is_contiguous() and x.dtype in (torch.float32, torch.float64, torch.bfloat16) and x.dim() > 0
+    if (fused and _as_it_is(norm, nn.LayerNorm) and len(norm.normalized_shape) == 1 and x.is_cuda and x.is_contiguous() and x.dtype in (torch.float32, torch.float64, torch.bfloat16) and x.dim() > 0
             and x.size(-1) == norm.normalized_shape[0] and x.shape == residual.shape and not torch.is_autocast_enabled() and plain_call(x, residual)
             and all(t is None or (t.dtype == x.dtype and t.device == x.device and t.is_contiguous()) for t in (residual, norm.weight, norm.bias))):
         return add_layer_norm(x, residual, norm.weight, norm.bias, norm.eps)
@@ -76,10 +76,11 @@ class PositionwiseFeedForward(nn.Module):
         self.dropout = nn.Dropout(dropout)
 
     def forward(self, x):
-        if self.keep8:
+        # (modules that someone has replaced, hooked or told to drop everything are called)
+        if self.keep8 and x.is_cuda and _as_it_is(self.w_2, nn.Linear) and _as_it_is(self.dropout, nn.Dropout) and not self.dropout.p >= 1.0:
             a, w, b = self.w_1(x).contiguous(), self.w_2.weight, self.w_2.bias
             if torch.is_autocast_enabled():
-                w, b = w.to(a.dtype), b.to(a.dtype)
+                w, b = w.to(a.dtype), None if b is None else b.to(a.dtype)
             return relu_linear8(a, w, b, self.dropout.p if self.training else 0.0)
         return self.w_2(self.dropout(torch.relu(self.w_1(x))))
 

@@ -213,6 +213,7 @@ struct ReluLinear8 : torch::autograd::Function<ReluLinear8> {
         if (need_b) {                                             // (the column sums of the layer norm's backward)
             c10::DeviceGuard guard(d_o.device());
             db = at::empty({outer}, d_o.options());
+            if (outer == 0) return {da, dw, db, Tensor(), Tensor()};
             const int64_t bytes = bpt_add_norm_workspace_bytes(rows, outer, dtype_code(d_o));
             const Tensor ws = at::empty({bytes}, d_o.options().dtype(at::kByte));
             check_status(bpt_add_norm_backward(ptr(d_o), nullptr, nullptr, nullptr, ptr(d_o), nullptr, nullptr, ptr(db), ptr(ws), bytes, rows, outer,

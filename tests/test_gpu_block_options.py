@@ -150,6 +150,35 @@ def test_keep8_keeps_less():
     assert held[1] <= 4096 * 2048 * (1 + 1 / 64) + 2 ** 20 and held[0] >= 8 * 4096 * 2048
 
 
+def test_keep8_calls_modules_that_are_not_as_they_were():
+    """A hook on the second layer, a layer of another class and a dropout of everything: torch's modules run, with their results."""
+    from bpt_amd.block import PositionwiseFeedForward
+    x = torch.randn(50, 64, device=DEV)
+
+    class Doubled(torch.nn.Linear):
+        def forward(self, x):
+            return 2 * super().forward(x)
+
+    def pair(p=0.0):
+        torch.manual_seed(3)
+        plain = PositionwiseFeedForward(64, 256, p).to(DEV)
+        kept = copy.deepcopy(plain)
+        kept.keep8 = True
+        return plain, kept
+    plain, kept = pair()
+    for f in (plain, kept):
+        f.w_2.register_forward_hook(lambda m, i, o: 3 * o)
+    assert torch.equal(plain(x), kept(x))
+    plain, kept = pair()
+    for f in (plain, kept):
+        f.w_2.__class__ = Doubled
+    assert torch.equal(plain(x), kept(x))
+    plain, kept = pair(1.0)
+    assert torch.equal(plain(x), kept(x)) and torch.equal(kept(x), kept.w_2.bias.expand(50, 64))
+    plain, kept = pair()
+    assert torch.equal(plain.cpu()(x.cpu()), kept.cpu()(x.cpu()))
+
+
 def test_the_norms_of_a_block_are_layer_norms():
     """The kernel and the module agree to rounding; a hook on the module, a module of the caller's and autocast are honoured."""
     from bpt_amd.block import BPTBlock

@@ -192,6 +192,15 @@ def test_relu_linear_needs_no_gradient_of_some():
         assert torch.equal(got, want[i])
 
 
+def test_relu_linear_of_no_rows_and_to_no_outputs():
+    from bpt_amd import op
+    for rows, outer in ((0, 16), (5, 0), (0, 0)):
+        a, w, b = (torch.randn(*s, device=DEV, requires_grad=True) for s in ((rows, 64), (outer, 64), (outer,)))
+        y = op.relu_linear8(a, w, b)
+        grads = torch.autograd.grad(y, (a, w, b), torch.ones_like(y))
+        assert y.shape == (rows, outer) and [g.shape for g in grads] == [a.shape, w.shape, b.shape] and not any(g.any() for g in grads)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_relu_linear_inside_autocast(dtype):
     """The products are of the tensors as they are."""

@@ -1,4 +1,5 @@
-"""ctypes bindings of the two native libraries (C ABIs in include/bptgraph.h and include/bptattn.h).
+"""ctypes bindings of the native libraries (C ABIs in include/bptgraph.h, bptattn.h, bptplan.h and bptscore.h; include/bptblock.h is called by
+bptop.so alone).
 
 There is no Python or CPU fallback for the device ops: if libbptattn.so is missing, importing
 `bpt_amd.graphop` raises.  Build with `python -m bpt_amd._build`.

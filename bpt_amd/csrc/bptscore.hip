@@ -7,32 +7,35 @@
 namespace {
 
 // Split rows, a workgroup each, from the sums of their segments (bfloat16, comment at k_attn_bwd_dst_rows_bf16): delta of the row to the source side,
-// and what the slopes' gradient gains by it, fix[split row][head].
-__global__ __launch_bounds__(BLOCK) void k_score_split(const int32_t *__restrict__ heavy, const float2 *__restrict__ split, float2 *__restrict__ stat,
-                                                       float *__restrict__ fix, int heads) {
-    __shared__ float2 meet[BLOCK];
+// and, fix[split row][head], (delta' - delta) and what the slopes' gradient gains by it.
+__global__ __launch_bounds__(BLOCK) void k_score_split(const int32_t *__restrict__ heavy, const float4 *__restrict__ split, float2 *__restrict__ stat,
+                                                       float2 *__restrict__ fix, int heads) {
+    __shared__ float4 meet[BLOCK];
     const int row = heavy[3 * blockIdx.x], s0 = heavy[3 * blockIdx.x + 1], ns = heavy[3 * blockIdx.x + 2];
     const int head = threadIdx.x % heads, lane = threadIdx.x / heads, lanes = BLOCK / heads;      // (8 or 16 heads)
-    float2 x = make_float2(0.f, 0.f);
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int i = lane; i < ns; i += lanes) {
-        const float2 y = split[(size_t)(s0 + i) * heads + head];
+        const float4 y = split[(size_t)(s0 + i) * heads + head];
         x.x += y.x;
         x.y += y.y;
+        x.z += y.z;
     }
     meet[threadIdx.x] = x;
     for (int o = lanes / 2; o > 0; o >>= 1) {
         __syncthreads();
         if (lane < o) {
-            const float2 y = meet[threadIdx.x + o * heads];
+            const float4 y = meet[threadIdx.x + o * heads];
             x.x += y.x;
             x.y += y.y;
+            x.z += y.z;
             meet[threadIdx.x] = x;
         }
     }
     if (lane == 0) {
         float2 *const at = stat + (size_t)row * heads + head;
-        fix[(size_t)blockIdx.x * heads + head] = (at->y - x.x) * x.y;
-        at->y = x.x;
+        const float delta = at->y, better = x.z == 0.f ? delta : x.x / x.z, less = delta == delta ? delta - better : 0.f;
+        fix[(size_t)blockIdx.x * heads + head] = make_float2(less, less * x.y);
+        at->y = better;
     }
 }
 
@@ -41,7 +44,7 @@ struct SlopeSum {
     const float *part;                 // [group][head][part]
     const int32_t *n_groups;
     int heads, parts;                  // as part counts them
-    const float *fix;                  // [split row][head]
+    const float2 *fix;                 // [split row][head], the second of the two
     int n_fix, wanted;                 // heads to sum up, or 0
     float *dslopes;
 };
@@ -59,7 +62,7 @@ __device__ __forceinline__ void slope_sum_block(const SlopeSum &m, int head) {
         for (int u = 0; u < 8; ++u) x += v[u];
     }
     for (; i < n; i += BLOCK) x += at(i);
-    for (i = threadIdx.x; i < m.n_fix; i += BLOCK) x += m.fix[(size_t)i * m.heads + head];
+    for (i = threadIdx.x; i < m.n_fix; i += BLOCK) x += m.fix[(size_t)i * m.heads + head].y;
     meet[threadIdx.x] = x;
     for (int o = BLOCK / 2; o > 0; o >>= 1) {
         __syncthreads();
@@ -68,28 +71,89 @@ __device__ __forceinline__ void slope_sum_block(const SlopeSum &m, int head) {
     if (threadIdx.x == 0) m.dslopes[head] = (float)-meet[0];
 }
 
+// dq of a split row, 128 columns (blockIdx.y, blockIdx.z): the sum of its segments' and (delta' - delta) times that of what they left of p du K; half wavefront i
+// takes segments i, i + 8, ..., up to eight in flight
+template <bool NARROW>
+__device__ __forceinline__ void merge_dq_block(const int32_t *__restrict__ hv, const float *__restrict__ ws, const bf16_t *__restrict__ low,
+                                               const float2 *__restrict__ fix, bf16_t *__restrict__ dq, int C, const Narrow &nw) {
+    constexpr int HALVES = 2 * WAVES_PER_BLOCK;
+    __shared__ float4 part[2][HALVES][WAVE / 2];
+    const int row = hv[0], s0 = hv[1], ns = hv[2];
+    const int lane = threadIdx.x & 31, half = threadIdx.x >> 5, j = (((int)blockIdx.y * 2 + (int)blockIdx.z) * 32 + lane) * 4;
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f), b = s;
+    const size_t first = (size_t)s0 * C + j;
+    int k = half;
+    auto take = [&](auto n) {
+        float4 t[n()];
+        uint2 u[n()];
+#pragma unroll
+        for (int i = 0; i < n(); ++i) {
+            const size_t at = first + (size_t)(k + i * HALVES) * C;
+            t[i] = *reinterpret_cast<const float4 *>(ws + at);
+            u[i] = *reinterpret_cast<const uint2 *>(low + at);
+        }
+        issue_loads_first();
+#pragma unroll
+        for (int i = 0; i < n(); ++i) {
+            const float4 y = tile_four(u[i]);
+            s.x += t[i].x; s.y += t[i].y; s.z += t[i].z; s.w += t[i].w;
+            b.x += y.x; b.y += y.y; b.z += y.z; b.w += y.w;
+        }
+        k += n() * HALVES;
+    };
+    while (k + 7 * HALVES < ns) take(std::integral_constant<int, 8>{});
+    if (k + 3 * HALVES < ns) take(std::integral_constant<int, 4>{});
+    if (k + HALVES < ns) take(std::integral_constant<int, 2>{});
+    if (k < ns) take(std::integral_constant<int, 1>{});
+    part[0][half][lane] = s;
+    part[1][half][lane] = b;
+    __syncthreads();
+    if (half != 0) return;
+    s = part[0][0][lane];
+    b = part[1][0][lane];
+#pragma unroll
+    for (int i = 1; i < HALVES; ++i) {
+        const float4 x = part[0][i][lane], y = part[1][i][lane];
+        s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
+        b.x += y.x; b.y += y.y; b.z += y.z; b.w += y.w;
+    }
+    const int head = j >> 6, col = j & 63;
+    const float less = fix[head].x;
+    const float x[4] = {fmaf(less, b.x, s.x), fmaf(less, b.y, s.y), fmaf(less, b.z, s.z), fmaf(less, b.w, s.w)};
+    if constexpr (NARROW) {                                       // 64 columns of the partials per head, d of the result
+        bf16_t *const at = dq + (size_t)row * (nw.heads * nw.d) + head * nw.d + col;
+        for (int e = 0; e < 4; ++e)
+            if (head < nw.heads && col + e < nw.d) Elem<bf16_t>::st(at + e, x[e]);
+    } else {
+        store4<bf16_t>(dq + (size_t)row * C + j, make_float4(x[0], x[1], x[2], x[3]));
+    }
+}
+
 // The backward's last launch: k_combine_sum3's sums of split rows (dq; dk and dv) and, in workgroups of their own in front of them, the slopes' gradient, which
 // as a launch by itself cost 4 us (8 at L = 32768, k = 8).  Grid (m.wanted + n_a + n_b, C / 256, 2).
 template <typename T, bool NARROW>
-__global__ __launch_bounds__(BLOCK) void k_score_merge(SlopeSum m, const int32_t *__restrict__ heavy_a, int n_a, const float *__restrict__ ws_a, T *__restrict__ YA,
-                                                       const int32_t *__restrict__ heavy_b, const float *__restrict__ ws_b, T *__restrict__ YB0, T *__restrict__ YB1,
+__global__ __launch_bounds__(BLOCK) void k_score_merge(SlopeSum m, const int32_t *__restrict__ heavy_a, int n_a, const float *__restrict__ ws_a,
+                                                       const bf16_t *__restrict__ low, T *__restrict__ YA, const int32_t *__restrict__ heavy_b, const float *__restrict__ ws_b, T *__restrict__ YB0, T *__restrict__ YB1,
                                                        int C, size_t ws_stride_b, Narrow nw) {
     const int x = (int)blockIdx.x - m.wanted;
     if (x < 0) {
         if (blockIdx.y == 0 && blockIdx.z == 0) slope_sum_block(m, (int)blockIdx.x);
     } else if (x < n_a) {
+        if constexpr (sizeof(T) == 2) {
+            if (low) return merge_dq_block<NARROW>(heavy_a + 3 * x, ws_a, low, m.fix + (size_t)x * m.heads, YA, C, nw);
+        }
         if (blockIdx.z == 0) combine_sum_block4<T, NARROW>(heavy_a + 3 * x, ws_a, YA, C, false, -1, nw);
     } else {
         combine_sum_block4<T, NARROW>(heavy_b + 3 * (x - n_a), ws_b + (size_t)blockIdx.z * ws_stride_b, blockIdx.z == 0 ? YB0 : YB1, C, false, -1, nw);
     }
 }
 template <typename T, bool NARROW>
-int run_merge(const SlopeSum &m, const bpt_plan *Pin, const bpt_plan *Pout, const float *ws_dq, T *dq, const float *ws_dk, T *dk, T *dv, int C, const Narrow &nw,
+int run_merge(const SlopeSum &m, const bpt_plan *Pin, const bpt_plan *Pout, const float *ws_dq, const bf16_t *low, T *dq, const float *ws_dk, T *dk, T *dv, int C, const Narrow &nw,
               hipStream_t s) {
     const unsigned blocks = (unsigned)(m.wanted + Pin->n_heavy + Pout->n_heavy);
     if (blocks == 0) return BPT_OK;
     hipLaunchKernelGGL((k_score_merge<T, NARROW>), dim3(blocks, Pin->n_heavy + Pout->n_heavy > 0 ? C / (4 * WAVE) : 1, Pin->n_heavy + Pout->n_heavy > 0 ? 2 : 1), dim3(BLOCK), 0,
-                       s, m, Pin->heavy, (int)Pin->n_heavy, ws_dq, dq, Pout->heavy, ws_dk, dk, dv, C, (size_t)Pout->n_slots * C, nw);
+                       s, m, Pin->heavy, (int)Pin->n_heavy, ws_dq, low, dq, Pout->heavy, ws_dk, dk, dv, C, (size_t)Pout->n_slots * C, nw);
     return launch_status();
 }
 
@@ -232,7 +296,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(NARRO
         delta = groups_sum(delta);                                // dO . O of member c, this head
     }
     const float lse_c = lse[at];
-    float slope = 0.f, pos_m = 0.f, slope_sum = 0.f, dp_sum = 0.f, far_sum = 0.f;
+    float slope = 0.f, pos_m = 0.f, slope_sum = 0.f, dp_sum = 0.f, far_sum = 0.f, p_sum = 0.f;
     if (md.slopes) {
         slope = md.slopes[t.head] * LOG2E;
         pos_m = md.pos_member[max(t.member.x, 0)];
@@ -284,6 +348,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(NARRO
                 const float y = where_pair_or_zero(B.mk[r], c, pe * (dp[r] * mt));
                 ds[r] = fmaf(-pe, delta, y);
                 dp_sum += y;
+                p_sum += pe;
                 if (md.part) {
                     const float far = fabsf(pos_m - pos_e[r]);
                     slope_sum += pair_if<CAREFUL>(B.mk[r], c, ds[r] * far);
@@ -313,24 +378,16 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(NARRO
     if (tile_any_odd(tile_odd(acc) + tile_odd(pk) + (slope_sum + far_sum) * 0.f)) {      // (what does not exist must not reach the sums: tile_odd)
 #pragma unroll
             for (int nb = 0; nb < 4; ++nb) { acc[nb] = floatx4v{0.f, 0.f, 0.f, 0.f}; pk[nb] = floatx4v{0.f, 0.f, 0.f, 0.f}; }
-            slope_sum = far_sum = dp_sum = 0.f;
+            slope_sum = far_sum = dp_sum = p_sum = 0.f;
             walk(std::true_type{});
     }
-    float whole = groups_sum(dp_sum), far = groups_sum(far_sum);  // of member c, of this part
+    float4 sums = make_float4(groups_sum(dp_sum), groups_sum(far_sum), groups_sum(p_sum), 0.f);      // of member c, of this part
     if constexpr (SP > 1) {
-        __shared__ float2 meet[HW][TILE_R];
-        if (g == 0) meet[t.wv][c] = make_float2(whole, far);
-        __syncthreads();
-        whole = far = 0.f;
-#pragma unroll
-        for (int i = 0; i < SP; ++i) {
-            const float2 x = meet[i * (HW / SP) + t.wv % (HW / SP)][c];
-            whole += x.x;
-            far += x.y;
-        }
+        __shared__ float4 meet[HW][TILE_R];
+        tile_parts_sum<SP, HW>(meet, t, sums);
     }
     const bool segment = t.member.y >= 0;
-    const float better = segment ? delta : whole, less = delta == delta ? delta - better : 0.f;      // (as in k_attn_bwd_dst_rows_bf16)
+    const float better = segment || sums.z == 0.f ? delta : sums.x / sums.z, less = delta == delta ? delta - better : 0.f;      // (as in k_attn_bwd_dst_rows_bf16)
     slope_sum = fmaf(less, far_sum, slope_sum);
     // (lane (c, g) of the sums holds members 4 g + r, less is member c's)
     float less_m[4];
@@ -342,8 +399,9 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(NARRO
         for (int r = 0; r < 4; ++r) acc[nb][r] = fmaf(less_m[r], pk[nb][r], acc[nb][r]);
     if (g == 0 && t.part == 0 && t.member.x >= 0) {
         stat[at] = make_float2(lse_c, better);
-        if (segment) md.split[(size_t)t.member.y * Hs + t.head] = make_float2(whole, far);
+        if (segment) md.split[(size_t)t.member.y * Hs + t.head] = sums;
     }
+    if (__builtin_amdgcn_ballot_w64(segment) != 0) tile_put_low<SP, H, D, true>(md, t, piece[t.wv], piece[t.wv % (HW / SP)], (HW / SP) * PIECE, pk, nw);
     tile_put_slope_part<SP>(md, t, Hs, slope_sum);
     if constexpr (SP > 1) {
         tile_park(piece[t.wv], acc, t.lane);
@@ -486,7 +544,16 @@ inline int64_t scratch_bytes(const bpt_plan *Pin, const bpt_plan *Pout, int h, i
 }
 constexpr int MOST_PARTS = 4;
 inline int64_t slope_bytes(const bpt_plan *Pin, int h) { return round16(Pin->n_groups * h * MOST_PARTS * 4); }
-inline int64_t split_bytes(const bpt_plan *Pin, int h) { return round16(Pin->n_slots * h * 8) + round16(Pin->n_heavy * h * 4); }
+// bfloat16's segments: [slot][head] sums, [slot][column] of p du K, [split row][head] of k_score_split
+struct SplitSums {
+    float4 *sums;
+    bf16_t *low;
+    float2 *fix;
+};
+inline SplitSums split_sums(char *at, const bpt_plan *Pin, int h) {
+    return SplitSums{(float4 *)at, (bf16_t *)(at + Pin->n_slots * h * 16), (float2 *)(at + Pin->n_slots * h * (16 + 64 * 2))};
+}
+inline int64_t split_bytes(const bpt_plan *Pin, int h) { return Pin->n_slots * h * (16 + 64 * 2) + round16(Pin->n_heavy * h * 8); }
 
 inline ScoreMod make_mod(const bpt_score *sc, float scale, bool entries_are_keys, float *part) {
     ScoreMod m{};
@@ -568,13 +635,13 @@ int run_backward(const bpt_plan *Pin, const bpt_plan *Pout, const bpt_score *sc,
     at += scratch_bytes(Pin, Pout, H, dtype, biased);
     float *part = dslopes ? (float *)at : nullptr;
     at += slope_bytes(Pin, H);
-    float2 *split = (float2 *)at;
-    float *fix = (float *)(at + round16(Pin->n_slots * H * 8));
+    const SplitSums split = split_sums(at, Pin, H);
     if (again) at += split_bytes(Pin, H);
     float *ws_dq = (float *)at, *ws_dk = ws_dq + (size_t)Pin->n_slots * H * D, *ws_dv = ws_dk + (size_t)Pout->n_slots * H * D;
     const int parts_in = tile_parts(Pin, H, sizeof(T)), parts_out = tile_parts(Pout, H, sizeof(T));
     ScoreMod md = make_mod(sc, scale, true, part);
-    md.split = split;
+    md.split = split.sums;
+    md.low = split.low;
     pick(drop.thr != 0, biased, parts_in, [&](auto dr, auto bi, auto sp) {
         const dim3 grid((unsigned)(group_grid(Pin) * (H * sp() / HW))), block(HW * WAVE);
         if constexpr (sizeof(T) == 4)
@@ -590,7 +657,7 @@ int run_backward(const bpt_plan *Pin, const bpt_plan *Pout, const bpt_score *sc,
     if (st != BPT_OK) return st;
     const bool fixed = again && Pin->n_heavy > 0;
     if (fixed)
-        hipLaunchKernelGGL(k_score_split, dim3((unsigned)Pin->n_heavy), dim3(BLOCK), 0, s, Pin->heavy, (const float2 *)split, (float2 *)scratch, fix, H);
+        hipLaunchKernelGGL(k_score_split, dim3((unsigned)Pin->n_heavy), dim3(BLOCK), 0, s, Pin->heavy, (const float4 *)split.sums, (float2 *)scratch, split.fix, H);
     pick(drop.thr != 0, biased, parts_out, [&](auto dr, auto bi, auto sp) {
         const dim3 grid((unsigned)(group_grid(Pout) * (H * sp() / HW))), block(HW * WAVE);
         if constexpr (sizeof(T) == 4)
@@ -606,8 +673,8 @@ int run_backward(const bpt_plan *Pin, const bpt_plan *Pout, const bpt_score *sc,
     });
     st = launch_status();
     if (st != BPT_OK) return st;
-    const SlopeSum sum{part, Pin->grp_chunks + 8, H, parts_in, fix, fixed ? (int)Pin->n_heavy : 0, dslopes ? H : 0, dslopes};
-    return run_merge<T, false>(sum, Pin, Pout, ws_dq, (T *)dq, ws_dk, (T *)dk, (T *)dv, H * D, Narrow{}, s);
+    const SlopeSum sum{part, Pin->grp_chunks + 8, H, parts_in, split.fix, fixed ? (int)Pin->n_heavy : 0, dslopes ? H : 0, dslopes};
+    return run_merge<T, false>(sum, Pin, Pout, ws_dq, fixed ? split.low : nullptr, (T *)dq, ws_dk, (T *)dk, (T *)dv, H * D, Narrow{}, s);
 }
 
 // Heads of fewer than 64 columns, read as they are.
@@ -647,15 +714,15 @@ int run_backward_narrow(const bpt_plan *Pin, const bpt_plan *Pout, const bpt_sco
     at += scratch_bytes(Pin, Pout, nw.h, F32 ? BPT_F32 : BPT_BF16, false);
     float *part = dslopes ? (float *)at : nullptr;
     at += slope_bytes(Pin, nw.h);
-    float2 *split = (float2 *)at;
-    float *fix = (float *)(at + round16(Pin->n_slots * nw.h * 8));
+    const SplitSums split = split_sums(at, Pin, nw.h);
     if (!F32) at += split_bytes(Pin, nw.h);
     const int C = nw.h * 64;
     float *ws_dq = (float *)at, *ws_dk = ws_dq + (size_t)Pin->n_slots * C, *ws_dv = ws_dk + (size_t)Pout->n_slots * C;
     const int parts = tile_parts(Pin, nw.heads, sizeof(T)), parts_src = tile_parts(Pout, nw.heads, sizeof(T));
     const Narrow np = narrow_parts(nw, parts), np_src = narrow_parts(nw, parts_src);
     ScoreMod md = make_mod(sc, scale, true, part);
-    md.split = split;
+    md.split = split.sums;
+    md.low = split.low;
     pick(drop.thr != 0, false, parts, [&](auto dr, auto, auto sp) {
         constexpr int HW = sp() == 1 ? NARROW_HW : sp();
         const dim3 grid((unsigned)(group_grid(Pin) * np.slices)), block(HW * WAVE);
@@ -670,7 +737,7 @@ int run_backward_narrow(const bpt_plan *Pin, const bpt_plan *Pout, const bpt_sco
     if (st != BPT_OK) return st;
     const bool fixed = !F32 && Pin->n_heavy > 0;
     if (fixed)          // (the padding heads' sums are not used)
-        hipLaunchKernelGGL(k_score_split, dim3((unsigned)Pin->n_heavy), dim3(BLOCK), 0, s, Pin->heavy, (const float2 *)split, scratch, fix, nw.h);
+        hipLaunchKernelGGL(k_score_split, dim3((unsigned)Pin->n_heavy), dim3(BLOCK), 0, s, Pin->heavy, (const float4 *)split.sums, scratch, split.fix, nw.h);
     pick(!F32 && drop.thr != 0, false, parts_src, [&](auto dr, auto, auto sp) {
         constexpr int HW = sp() == 1 ? NARROW_HW : sp();
         const dim3 grid((unsigned)(group_grid(Pout) * np_src.slices)), block(HW * WAVE);
@@ -683,8 +750,8 @@ int run_backward_narrow(const bpt_plan *Pin, const bpt_plan *Pout, const bpt_sco
     });
     st = launch_status();
     if (st != BPT_OK) return st;
-    const SlopeSum sum{part, Pin->grp_chunks + 8, nw.h, parts, fix, fixed ? (int)Pin->n_heavy : 0, dslopes ? nw.heads : 0, dslopes};
-    return run_merge<T, true>(sum, Pin, Pout, ws_dq, dq, ws_dk, dk, dv, C, nw, s);
+    const SlopeSum sum{part, Pin->grp_chunks + 8, nw.h, parts, split.fix, fixed ? (int)Pin->n_heavy : 0, dslopes ? nw.heads : 0, dslopes};
+    return run_merge<T, true>(sum, Pin, Pout, ws_dq, fixed ? split.low : nullptr, dq, ws_dk, dk, dv, C, nw, s);
 }
 
 inline int check_score(const bpt_plan *P, const bpt_score *sc, int heads, int d, int h, int dtype, float scale, float dropout_p, const float *bias,

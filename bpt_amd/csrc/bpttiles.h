@@ -969,7 +969,8 @@ struct ScoreMod {
     const float *slopes;               // (heads), or null: no distance
     const float *pos_member, *pos_entry;       // positions of the plan's rows, of the rows its indices name
     float *part;                       // destination side: [group][head][part] sums of dL/ds |pos - pos|, or null
-    float2 *split;                     // bfloat16 destination side: [slot][head] sums of p dP and of p |pos - pos| over a split row's segment
+    float4 *split;                     // bfloat16 destination side: [slot][head] sums of p dP, of p |pos - pos| and of p over a split row's segment
+    bf16_t *low;                       // ... and [slot][column] of p du K
 };
 struct NoMod {};
 template <bool MOD> struct ModArg { typedef NoMod type; };
@@ -1051,6 +1052,39 @@ __device__ __forceinline__ void tile_mod_scores(const ScoreMod &md, float scale_
     if (md.slopes) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) s[r] = fmaf(-slope_log2e, fabsf(pos_m - pos_e[r]), s[r]);
+    }
+}
+// What the segments among the tile's members have summed up (lane (c, g), register r: columns 4 c .. 4 c + 3 of member 4 g + r), rounded, to md.low
+template <int H, int D, bool NARROW> __device__ __forceinline__ void tile_store_low(const ScoreMod &md, const TileCtx &t, int r, const float4 &x, const Narrow &nw) {
+    const int at = lane_bcast(tile_where(t.member), 4 * t.g + r);
+    if (at >= -1 || (NARROW && 4 * t.c >= nw.d)) return;
+    bf16_t *const to = md.low + (size_t)(-2 - at) * (NARROW ? nw.h * D : H * D) + t.head * D + (NARROW ? narrow_col(nw, t.c) : 4 * t.c);
+    *reinterpret_cast<uintx2u *>(to) = uintx2u{pack_bf16(x.x, x.y), pack_bf16(x.z, x.w)};
+}
+template <int SP, int H, int D, bool NARROW>
+__device__ __forceinline__ void tile_put_low(const ScoreMod &md, const TileCtx &t, float *mine, const float *part0, int stride, const floatx4v (&acc)[4], const Narrow &nw) {
+    if constexpr (SP > 1) {
+        constexpr int RS = 4 / SP;
+        const float none[SP] = {};
+        tile_park(mine, acc, t.lane);
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < RS; ++i) tile_store_low<H, D, NARROW>(md, t, t.part * RS + i, tile_meet<SP, false>(part0, stride, t.part * RS + i, t, none), nw);
+        __syncthreads();
+    } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) tile_store_low<H, D, NARROW>(md, t, r, make_float4(acc[0][r], acc[1][r], acc[2][r], acc[3][r]), nw);
+    }
+}
+// sums of member c over the SP parts of a tile, in their order
+template <int SP, int HW> __device__ __forceinline__ void tile_parts_sum(float4 (&meet)[HW][TILE_R], const TileCtx &t, float4 &sums) {
+    if (t.g == 0) meet[t.wv][t.c] = sums;
+    __syncthreads();
+    sums = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < SP; ++i) {
+        const float4 x = meet[i * (HW / SP) + t.wv % (HW / SP)][t.c];
+        sums.x += x.x; sums.y += x.y; sums.z += x.z; sums.w += x.w;
     }
 }
 // dslope of a wavefront's pairs (part s of SP of a group and head): the sum over its lanes
@@ -1993,10 +2027,11 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP 
 // segments of a split row write the same values.
 // MOD without a score term: delta = dO . O with O as stored is off by O's rounding and by that of the p that O was summed with, both 2^-9 of each
 // term, which all pairs of a row share: at L = 32768, k = 8 dq and dk come out 0.0041 off (0.0017 is one rounding of the result) and the slopes'
-// gradient, a sum over all pairs that nothing rounds, as far.  The pairs of a whole row give delta in 32 bits, sum p dP, once they have all been seen:
+// gradient, a sum over all pairs that nothing rounds, as far.  The pairs of a whole row give delta in 32 bits, sum p dP / sum p, once they have all been seen:
 //   ds = p (dP - delta') du  corrected by  (delta' - delta) sum p du K  in dq and by  (delta' - delta) sum p |pos - pos|  in the slopes' gradient,
-// the source side is handed delta.  One more product a block over the K rows at hand.  dq of a split row keeps delta' (it has many pairs, each with a
-// small p); its segments leave their sums, from which k_score_split forms the other two before the source side runs.
+// the source side is handed delta.  (The sum of p, 1 but for the rounding of lse, keeps the sum of ds over a row at zero, by which distances in the hundreds multiply.)
+// One more product a block over the K rows at hand.  The segments of a split row leave their sums, that of p du K rounded to bfloat16 (2^-9 of a
+// correction that is 2^-8 of dq): k_score_split forms delta and the slopes' correction before the source side runs, k_score_merge dq's.
 template <int H, int D, int HW, int WPE, bool DROP, int BIAS, bool PDS, int SP, bool MOD = false>
 __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(MOD ? WPE - 2 : DROP || BIAS ? WPE - 1 : WPE))) void k_attn_bwd_dst_rows_bf16(
     bpt_plan P, const bf16_t *__restrict__ q, const bf16_t *__restrict__ k, const bf16_t *__restrict__ v, const bf16_t *__restrict__ o,
@@ -2069,7 +2104,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(MOD ?
     floatx4v acc[4];
 #pragma unroll
     for (int nb = 0; nb < 4; ++nb) acc[nb] = floatx4v{0.f, 0.f, 0.f, 0.f};
-    float dp_sum = 0.f, far_sum = 0.f;
+    float dp_sum = 0.f, far_sum = 0.f, p_sum = 0.f;
     floatx4v pk[FIX ? 4 : 1];                                     // sum of p du K, laid out as acc
 #pragma unroll
     for (int nb = 0; nb < (FIX ? 4 : 1); ++nb) pk[nb] = floatx4v{0.f, 0.f, 0.f, 0.f};
@@ -2159,6 +2194,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(MOD ?
                     ds[r] = pair_if<CAREFUL>(mk[r], c, ds[r] * (du[r] * scale));
                     if constexpr (FIX) {
                         dp_sum += x;
+                        p_sum += pe;
                         if (md.part) far_sum += pair_if<CAREFUL>(mk[r], c, pe * fabsf(pos_m - pos_e[r]));
                         pdu[r] = pair_if<CAREFUL>(mk[r], c, pe * (du[r] * scale));
                     }
@@ -2197,32 +2233,28 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(MOD ?
             for (int nb = 0; nb < 4; ++nb) acc[nb] = floatx4v{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int nb = 0; nb < (FIX ? 4 : 1); ++nb) pk[nb] = floatx4v{0.f, 0.f, 0.f, 0.f};
-            slope_sum = far_sum = dp_sum = 0.f;
+            slope_sum = far_sum = dp_sum = p_sum = 0.f;
             walk(std::true_type{});
         }
     }
     if constexpr (FIX) {
-        float whole = groups_sum(dp_sum), far = groups_sum(far_sum);      // of member c, of this part
+        float4 sums = make_float4(groups_sum(dp_sum), groups_sum(far_sum), groups_sum(p_sum), 0.f);      // of member c, of this part
         if constexpr (SP > 1) {
-            __shared__ float2 meet[HW][TILE_R];
-            if (g == 0) meet[t.wv][c] = make_float2(whole, far);
-            __syncthreads();
-            whole = far = 0.f;
-#pragma unroll
-            for (int i = 0; i < SP; ++i) {
-                const float2 x = meet[i * (HW / SP) + t.wv % (HW / SP)][c];
-                whole += x.x;
-                far += x.y;
-            }
+            __shared__ float4 meet[HW][TILE_R];
+            tile_parts_sum<SP, HW>(meet, t, sums);
         }
         const bool segment = t.member.y >= 0;
-        const float better = segment ? delta : whole, less = delta == delta ? delta - better : 0.f;      // (NaN: the pairs, if there are any, are NaN as they are)
+        const float better = segment || sums.z == 0.f ? delta : sums.x / sums.z, less = delta == delta ? delta - better : 0.f;      // (NaN: the pairs, if there are any, are NaN as they are)
         slope_sum = fmaf(less, far_sum, slope_sum);
 #pragma unroll
         for (int nb = 0; nb < 4; ++nb) acc[nb] += less * pk[nb];
         if (g == 0 && t.part == 0 && t.member.x >= 0) {
             stat[(size_t)t.member.x * H + t.head] = make_float2(lse_c, better);
-            if (segment) md.split[(size_t)t.member.y * H + t.head] = make_float2(whole, far);
+            if (segment) md.split[(size_t)t.member.y * H + t.head] = sums;
+        }
+        if (__builtin_amdgcn_ballot_w64(segment) != 0) {          // (the parts of a tile have the same members)
+            tile_sums_by_row(piece[t.wv], pk, c, g);
+            tile_put_low<SP, H, D, false>(md, t, piece[t.wv], piece[t.wv % (HW / SP)], (HW / SP) * PIECE, pk, nw);
         }
     }
     if constexpr (MOD) tile_put_slope_part<SP>(md, t, H, slope_sum);

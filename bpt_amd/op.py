@@ -170,6 +170,8 @@ class BPTRelAttention(Function):
                                                aux["used"], aux["used_types"])
             return None, None, None, None, None, None, None, None, dq, dk, dv, None, None, None, dtable, None, None, None, None, None
         if ctx.cap is not None:
+            if torch.is_grad_enabled():
+                raise RuntimeError("attention with score options is not differentiable twice")
             dq, dk, dv, dslopes, ds = _g.score_attention_backward(row, indptr_r, eid_r, indices_r, col, indptr_c, eid_c, indices_c, q, k, v, o, lse, do,
                                                                   _g.Score(ctx.cap, *ctx.saved_tensors[15:]), ctx.scale, ctx.dropout_p, ctx.seed, bias,
                                                                   ctx.needs_input_grad[19])

@@ -247,10 +247,11 @@ def test_saturated_scores(cap, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
-@pytest.mark.parametrize("heads,d", [(8, 64), (6, 50)])
-def test_dropout(heads, d, dtype):
+@pytest.mark.parametrize("heads,d,kind,rel", [(8, 64, ("bpt", 300, 4), False), (6, 50, ("bpt", 300, 4), False), (6, 50, ("memory", 40, 300), False),
+                                              (12, 64, ("window", 2000, 40), False), (8, 64, ("bpt", 300, 4), True), (6, 50, ("random", 90, 1500), True)], ids=str)
+def test_dropout(heads, d, kind, rel, dtype):
     from bpt_amd import graphop
-    c = make(("bpt", 300, 4), heads, d, dtype, 30.0, True)
+    c = make(kind, heads, d, dtype, 30.0, True, rel=rel)
     hp = graphop.score_padded_shape(c["q"])[0]
     mask = graphop.attention_dropout_mask(None, None, c["src"], None, torch.empty(1, hp, 64), None, 0.2, 77)[:, :heads]
     check(c, fused=True, drop=mask.double(), dropout_p=0.2, seed=77)
@@ -430,6 +431,25 @@ def test_replays_of_a_captured_pass_match_the_eager_one():
         torch.cuda.synchronize()
         for got, want in zip(captured, step()):
             assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("heads,d", [(8, 64), (16, 64), (6, 50)])
+@pytest.mark.parametrize("kind", [("bpt", 700, 4), ("memory", 71, 774), ("window", 1500, 40)], ids=str)
+def test_slopes_of_bfloat16_rows_are_summed_in_32_bits(kind, heads, d):
+    """Nothing that the slopes' gradient is summed from is rounded to bfloat16 (delta comes from the pairs): float32's bound, of the same values."""
+    c = make(kind, heads, d, "bf16", 15.0, True)
+    wide = {n: t.float() if torch.is_tensor(t) and t.dtype == torch.bfloat16 else t for n, t in c.items()}
+    got = run(c, graph_args(c["src"].numpy(), c["dst"].numpy(), c["q"].size(0), c["k"].size(0)), True)
+    close(got["dslopes"], reference(wide)["dslopes"], "dslopes", torch.float32)
+
+
+@pytest.mark.parametrize("rel", [False, True])
+def test_a_second_derivative_is_refused(rel):
+    c = make(("bpt", 30, 2), 8, 64, "f32", 30.0, True, rel=rel)
+    args = graph_args(c["src"].numpy(), c["dst"].numpy(), c["q"].size(0), c["k"].size(0))
+    dev = on_device(c)
+    with pytest.raises(RuntimeError, match="differentiable twice"):
+        torch.autograd.grad(call(c, dev, args), dev["q"], dev["do"], create_graph=True)
 
 
 def test_refusals():

@@ -7,7 +7,7 @@
 namespace {
 
 // Split rows, a workgroup each, from the sums of their segments (bfloat16, comment at k_attn_bwd_dst_rows_bf16): delta of the row to the source side,
-// and, fix[split row][head], (delta' - delta) and what the slopes' gradient gains by it.
+// and, fix[split row][head], (delta' - delta) and what the slopes' gradient gains by it.  float32 (no stat): the latter alone, of the sum of ds that should be zero.
 __global__ __launch_bounds__(BLOCK) void k_score_split(const int32_t *__restrict__ heavy, const float4 *__restrict__ split, float2 *__restrict__ stat,
                                                        float2 *__restrict__ fix, int heads) {
     __shared__ float4 meet[BLOCK];
@@ -31,7 +31,8 @@ __global__ __launch_bounds__(BLOCK) void k_score_split(const int32_t *__restrict
             meet[threadIdx.x] = x;
         }
     }
-    if (lane == 0) {
+    if (lane == 0 && !stat) fix[(size_t)blockIdx.x * heads + head] = make_float2(0.f, x.z == 0.f ? 0.f : -x.x / x.z * x.y);
+    if (lane == 0 && stat) {
         float2 *const at = stat + (size_t)row * heads + head;
         const float delta = at->y, better = x.z == 0.f ? delta : x.x / x.z, less = delta == delta ? delta - better : 0.f;
         fix[(size_t)blockIdx.x * heads + head] = make_float2(less, less * x.y);
@@ -550,10 +551,14 @@ struct SplitSums {
     bf16_t *low;
     float2 *fix;
 };
-inline SplitSums split_sums(char *at, const bpt_plan *Pin, int h) {
-    return SplitSums{(float4 *)at, (bf16_t *)(at + Pin->n_slots * h * 16), (float2 *)(at + Pin->n_slots * h * (16 + 64 * 2))};
+inline int64_t split_slot_bytes(int h, bool low) { return h * (16 + (low ? 64 * 2 : 0)); }
+inline SplitSums split_sums(char *at, const bpt_plan *Pin, int h, bool low) {
+    return SplitSums{(float4 *)at, low ? (bf16_t *)(at + Pin->n_slots * h * 16) : nullptr, (float2 *)(at + Pin->n_slots * split_slot_bytes(h, low))};
 }
-inline int64_t split_bytes(const bpt_plan *Pin, int h) { return Pin->n_slots * h * (16 + 64 * 2) + round16(Pin->n_heavy * h * 8); }
+inline int64_t split_bytes(const bpt_plan *Pin, int h, bool low) { return Pin->n_slots * split_slot_bytes(h, low) + round16(Pin->n_heavy * h * 8); }
+// Whether split rows' sums are looked at: bfloat16's always (delta); float32's, a launch of 5 us for the slopes' gradient alone, where they are half of the rows or more (few
+// queries of a long memory: 101 rows of 185 keys 1.1e-6 -> 6e-7 off).  Of a graph with few of them they carry little: L = 8192, 127 split rows, 2.7e-7 without.
+inline bool split_counts(const bpt_plan *Pin, bool f32, bool slopes) { return Pin->n_heavy > 0 && (!f32 || (slopes && 2 * Pin->n_heavy >= Pin->n_rows)); }
 
 inline ScoreMod make_mod(const bpt_score *sc, float scale, bool entries_are_keys, float *part) {
     ScoreMod m{};
@@ -635,12 +640,12 @@ int run_backward(const bpt_plan *Pin, const bpt_plan *Pout, const bpt_score *sc,
     at += scratch_bytes(Pin, Pout, H, dtype, biased);
     float *part = dslopes ? (float *)at : nullptr;
     at += slope_bytes(Pin, H);
-    const SplitSums split = split_sums(at, Pin, H);
-    if (again) at += split_bytes(Pin, H);
+    const SplitSums split = split_sums(at, Pin, H, again);
+    if (again || sizeof(T) == 4) at += split_bytes(Pin, H, again);
     float *ws_dq = (float *)at, *ws_dk = ws_dq + (size_t)Pin->n_slots * H * D, *ws_dv = ws_dk + (size_t)Pout->n_slots * H * D;
     const int parts_in = tile_parts(Pin, H, sizeof(T)), parts_out = tile_parts(Pout, H, sizeof(T));
     ScoreMod md = make_mod(sc, scale, true, part);
-    md.split = split.sums;
+    md.split = again || split_counts(Pin, sizeof(T) == 4, dslopes != nullptr) ? split.sums : nullptr;
     md.low = split.low;
     pick(drop.thr != 0, biased, parts_in, [&](auto dr, auto bi, auto sp) {
         const dim3 grid((unsigned)(group_grid(Pin) * (H * sp() / HW))), block(HW * WAVE);
@@ -655,9 +660,9 @@ int run_backward(const bpt_plan *Pin, const bpt_plan *Pout, const bpt_score *sc,
     });
     int st = launch_status();
     if (st != BPT_OK) return st;
-    const bool fixed = again && Pin->n_heavy > 0;
+    const bool fixed = (again || sizeof(T) == 4) && split_counts(Pin, sizeof(T) == 4, dslopes != nullptr);
     if (fixed)
-        hipLaunchKernelGGL(k_score_split, dim3((unsigned)Pin->n_heavy), dim3(BLOCK), 0, s, Pin->heavy, (const float4 *)split.sums, (float2 *)scratch, split.fix, H);
+        hipLaunchKernelGGL(k_score_split, dim3((unsigned)Pin->n_heavy), dim3(BLOCK), 0, s, Pin->heavy, (const float4 *)split.sums, sizeof(T) == 4 ? (float2 *)nullptr : (float2 *)scratch, split.fix, H);
     pick(drop.thr != 0, biased, parts_out, [&](auto dr, auto bi, auto sp) {
         const dim3 grid((unsigned)(group_grid(Pout) * (H * sp() / HW))), block(HW * WAVE);
         if constexpr (sizeof(T) == 4)
@@ -714,14 +719,14 @@ int run_backward_narrow(const bpt_plan *Pin, const bpt_plan *Pout, const bpt_sco
     at += scratch_bytes(Pin, Pout, nw.h, F32 ? BPT_F32 : BPT_BF16, false);
     float *part = dslopes ? (float *)at : nullptr;
     at += slope_bytes(Pin, nw.h);
-    const SplitSums split = split_sums(at, Pin, nw.h);
-    if (!F32) at += split_bytes(Pin, nw.h);
+    const SplitSums split = split_sums(at, Pin, nw.h, !F32);
+    at += split_bytes(Pin, nw.h, !F32);
     const int C = nw.h * 64;
     float *ws_dq = (float *)at, *ws_dk = ws_dq + (size_t)Pin->n_slots * C, *ws_dv = ws_dk + (size_t)Pout->n_slots * C;
     const int parts = tile_parts(Pin, nw.heads, sizeof(T)), parts_src = tile_parts(Pout, nw.heads, sizeof(T));
     const Narrow np = narrow_parts(nw, parts), np_src = narrow_parts(nw, parts_src);
     ScoreMod md = make_mod(sc, scale, true, part);
-    md.split = split.sums;
+    md.split = !F32 || split_counts(Pin, F32, dslopes != nullptr) ? split.sums : nullptr;
     md.low = split.low;
     pick(drop.thr != 0, false, parts, [&](auto dr, auto, auto sp) {
         constexpr int HW = sp() == 1 ? NARROW_HW : sp();
@@ -735,9 +740,9 @@ int run_backward_narrow(const bpt_plan *Pin, const bpt_plan *Pout, const bpt_sco
     });
     int st = launch_status();
     if (st != BPT_OK) return st;
-    const bool fixed = !F32 && Pin->n_heavy > 0;
+    const bool fixed = split_counts(Pin, F32, dslopes != nullptr);
     if (fixed)          // (the padding heads' sums are not used)
-        hipLaunchKernelGGL(k_score_split, dim3((unsigned)Pin->n_heavy), dim3(BLOCK), 0, s, Pin->heavy, (const float4 *)split.sums, scratch, split.fix, nw.h);
+        hipLaunchKernelGGL(k_score_split, dim3((unsigned)Pin->n_heavy), dim3(BLOCK), 0, s, Pin->heavy, (const float4 *)split.sums, F32 ? nullptr : scratch, split.fix, nw.h);
     pick(!F32 && drop.thr != 0, false, parts_src, [&](auto dr, auto, auto sp) {
         constexpr int HW = sp() == 1 ? NARROW_HW : sp();
         const dim3 grid((unsigned)(group_grid(Pout) * np_src.slices)), block(HW * WAVE);
@@ -807,7 +812,7 @@ int64_t bpt_score_forward_workspace_bytes(const bpt_plan *plan_in, int h) {
 
 int64_t bpt_score_backward_workspace_bytes(const bpt_plan *plan_in, const bpt_plan *plan_out, int h, int dtype, int has_bias) {
     if (!plan_in || !plan_out || h < 1 || (dtype != BPT_F32 && dtype != BPT_BF16)) return -1;
-    return scratch_bytes(plan_in, plan_out, h, dtype, has_bias != 0) + slope_bytes(plan_in, h) + (dtype == BPT_BF16 && !has_bias ? split_bytes(plan_in, h) : 0) +
+    return scratch_bytes(plan_in, plan_out, h, dtype, has_bias != 0) + slope_bytes(plan_in, h) + (dtype == BPT_F32 || !has_bias ? split_bytes(plan_in, h, dtype == BPT_BF16) : 0) +
            round16((plan_in->n_slots + 2 * plan_out->n_slots) * (int64_t)h * 64 * 4);
 }
 

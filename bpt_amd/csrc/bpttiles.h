@@ -969,8 +969,8 @@ struct ScoreMod {
     const float *slopes;               // (heads), or null: no distance
     const float *pos_member, *pos_entry;       // positions of the plan's rows, of the rows its indices name
     float *part;                       // destination side: [group][head][part] sums of dL/ds |pos - pos|, or null
-    float4 *split;                     // bfloat16 destination side: [slot][head] sums of p dP, of p |pos - pos| and of p over a split row's segment
-    bf16_t *low;                       // ... and [slot][column] of p du K
+    float4 *split;                     // destination side: [slot][head] sums of p dP (float32: of ds before du), of p |pos - pos| and of p over a split row's segment, or null
+    bf16_t *low;                       // bfloat16 destination side: [slot][column] sums of p du K
 };
 struct NoMod {};
 template <bool MOD> struct ModArg { typedef NoMod type; };
@@ -1366,7 +1366,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP 
 #pragma unroll
         for (int i = 0; i < 4; ++i) dob_h[i][t.lane] = floatx4v{dob[4 * i], dob[4 * i + 1], dob[4 * i + 2], dob[4 * i + 3]};
     }
-    float slope = 0.f, pos_m = 0.f, slope_sum = 0.f;
+    float slope = 0.f, pos_m = 0.f, slope_sum = 0.f, far_sum = 0.f, ds_sum = 0.f, p_sum = 0.f;
     if constexpr (MOD) {
         if (md.slopes) {
             slope = md.slopes[t.head] * LOG2E;
@@ -1458,7 +1458,13 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP 
                     mt = dropout_keep((uint32_t)B.xe[DROP ? r : 0] * (uint32_t)Hs + (uint32_t)t.head, drop_seed, drop_thr, drop_inv);
                 if constexpr (MOD) {
                     ds[r] = where_pair_or_zero(mask[r], c, pe * (dp[r] * mt - delta));
-                    if (md.part) slope_sum += pair_if<CAREFUL>(mask[r], c, ds[r] * fabsf(pos_m - pos_e[r]));
+                    if (md.part) {
+                        const float far = fabsf(pos_m - pos_e[r]);
+                        slope_sum += pair_if<CAREFUL>(mask[r], c, ds[r] * far);
+                        far_sum += pair_if<CAREFUL>(mask[r], c, pe * far);
+                        ds_sum += pair_if<CAREFUL>(mask[r], c, ds[r]);
+                        p_sum += pe;
+                    }
                     ds[r] = pair_if<CAREFUL>(mask[r], c, ds[r] * (du[r] * scale));
                 } else {
                     ds[r] = pe * (dp[r] * mt - delta) * scale;
@@ -1478,14 +1484,27 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP 
     };
     walk(std::false_type{});
     if constexpr (MOD) {
-        if (tile_any_odd(tile_odd(acc) + slope_sum * 0.f)) {      // (what does not exist must not reach the sums: tile_odd)
+        if (tile_any_odd(tile_odd(acc) + (slope_sum + far_sum) * 0.f)) {      // (what does not exist must not reach the sums: tile_odd)
 #pragma unroll
             for (int nb = 0; nb < 4; ++nb) acc[nb] = floatx4v{0.f, 0.f, 0.f, 0.f};
-            slope_sum = 0.f;
+            slope_sum = far_sum = ds_sum = p_sum = 0.f;
             walk(std::true_type{});
         }
     }
-    if constexpr (MOD) tile_put_slope_part<SP>(md, t, Hs, slope_sum);
+    if constexpr (MOD) {
+        if (md.part) {
+            // The sum of a row's ds is zero, but for delta's rounding and the pairs', by which the row's mean distance multiplies: taken off
+            float4 sums = make_float4(groups_sum(ds_sum), groups_sum(far_sum), groups_sum(p_sum), 0.f);      // of member c, of this part
+            if constexpr (SP > 1) {
+                __shared__ float4 meet[HW][TILE_R];
+                tile_parts_sum<SP, HW>(meet, t, sums);
+            }
+            const bool segment = t.member.y >= 0;
+            if (!segment && sums.z != 0.f) slope_sum = fmaf(-sums.x / sums.z, far_sum, slope_sum);
+            if (segment && md.split && g == 0 && t.part == 0) md.split[(size_t)t.member.y * Hs + t.head] = sums;
+        }
+        tile_put_slope_part<SP>(md, t, Hs, slope_sum);
+    }
     if constexpr (SP > 1) {
         tile_park(kt, acc, t.lane);
         __syncthreads();

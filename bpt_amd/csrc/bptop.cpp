@@ -641,7 +641,7 @@ MaybeTensor score_attention(const MaybeTensor &row, const MaybeTensor &indptr_r,
                             const MaybeTensor &slopes, const MaybeTensor &pos_q, const MaybeTensor &pos_k, std::optional<double> score_cap, double scale, double p,
                             uint64_t seed, int64_t h) {
     // (what graphop.score_options refuses is left to it)
-    if (score_cap && !(*score_cap > 0.0 && *score_cap <= 3.0e38 && std::abs(scale) <= 1.0e4 * *score_cap)) return std::nullopt;
+    if (score_cap && !(*score_cap >= 1.0e-10 && *score_cap <= 1.0e10 && std::abs(scale) <= std::min(1.0e4 * *score_cap, 1.0e6))) return std::nullopt;
     if ((pos_q && pos_q->requires_grad()) || (pos_k && pos_k->requires_grad())) return std::nullopt;
     const ScoreOptions opt{score_cap.value_or(0.0), slopes.value_or(Tensor()), pos_q.value_or(Tensor()), pos_k.value_or(Tensor())};
     const Tensor none, &r0 = row ? *row : none, &r1 = indptr_r ? *indptr_r : none, &r2 = eid_r ? *eid_r : none, &r3 = indices_r ? *indices_r : none;

@@ -355,8 +355,8 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(NARRO
                     slope_sum += pair_if<CAREFUL>(B.mk[r], c, ds[r] * far);
                     far_sum += pair_if<CAREFUL>(B.mk[r], c, pe * far);
                 }
-                ds[r] = pair_if<CAREFUL>(B.mk[r], c, ds[r] * (du[r] * scale));
-                pdu[r] = pair_if<CAREFUL>(B.mk[r], c, pe * (du[r] * scale));
+                ds[r] = pair_if<CAREFUL>(B.mk[r], c, ds[r] * du[r]);
+                pdu[r] = pair_if<CAREFUL>(B.mk[r], c, pe * du[r]);
             }
             if constexpr (CAREFUL) {
                 tile_axpy_pairs(ds, B.mk, B.kc, c, g, acc);
@@ -500,7 +500,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(NARRO
                 const float p = where_pair_or_zero(B.mk[r], c, __builtin_amdgcn_exp2f(sm[r] - lse_e[r]));
                 float mt = 1.f;                                   // dropout multiplier of this pair (as in the forward)
                 if constexpr (DROP) mt = dropout_keep((uint32_t)B.xe[DROP ? r : 0] * (uint32_t)Hs + (uint32_t)t.head, drop_seed, drop_thr, drop_inv);
-                ds[r] = where_pair_or_zero(B.mk[r], c, p * (dp[r] * mt - delta_e[r]) * (du[r] * scale));
+                ds[r] = where_pair_or_zero(B.mk[r], c, p * (dp[r] * mt - delta_e[r]) * du[r]);
                 pe[r] = p * mt;
             }
             if constexpr (CAREFUL) {
@@ -562,14 +562,16 @@ inline bool split_counts(const bpt_plan *Pin, bool f32, bool slopes) { return Pi
 
 inline ScoreMod make_mod(const bpt_score *sc, float scale, bool entries_are_keys, float *part) {
     ScoreMod m{};
+    m.scale = scale;
     if (sc->cap > 0.f) {
-        const double to = (double)scale / sc->cap, w = to * to;
+        const double to = (double)scale / sc->cap, w = to * to, base2 = (double)scale * 1.4426950408889634;
         m.to_tanh = (float)to;
         m.from_tanh = sc->cap * LOG2E;
-        m.c[0] = (float)(-0.333331435918808 * w);
-        m.c[1] = (float)(0.13325878977775574 * w * w);
-        m.c[2] = (float)(-0.05304549261927605 * w * w * w);
-        m.c[3] = (float)(0.01724148355424404 * w * w * w * w);
+        m.slope_of = (float)(-(double)scale / ((double)m.from_tanh * m.from_tanh));
+        m.c[0] = (float)(-0.333331435918808 * w * base2);
+        m.c[1] = (float)(0.13325878977775574 * w * w * base2);
+        m.c[2] = (float)(-0.05304549261927605 * w * w * w * base2);
+        m.c[3] = (float)(0.01724148355424404 * w * w * w * w * base2);
         m.far = (float)(0.25 / w);
     }
     m.slopes = sc->slopes;
@@ -770,7 +772,9 @@ inline int check_score(const bpt_plan *P, const bpt_score *sc, int heads, int d,
     const bool narrow = heads != h || d != 64;
     if (narrow && ((dtype != BPT_F32 && d % 2 != 0) || bias || heads > h || d < 4 || d > 64)) return BPT_ERR_UNSUPPORTED;
     nw = narrow ? Narrow{d, heads, h, (heads + NARROW_HW - 1) / NARROW_HW} : Narrow{};
-    if (!(sc->cap >= 0.f && sc->cap <= 3.0e38f) || (sc->cap > 0.f && !(fabsf(scale) <= 1.0e4f * sc->cap)) || !(dropout_p >= 0.f && dropout_p < 1.f)) return BPT_ERR_SIZE;
+    // (within these bounds the polynomial's coefficients and squares of scores are ordinary numbers: make_mod, tile_mod_scores)
+    const bool capped = sc->cap != 0.f;
+    if ((capped && !(sc->cap >= 0.9e-10f && sc->cap <= 1.1e10f && fabsf(scale) <= 1.01e4f * sc->cap && fabsf(scale) <= 1.01e6f)) || !(dropout_p >= 0.f && dropout_p < 1.f)) return BPT_ERR_SIZE;
     if (sc->slopes && (!sc->pos_q || !sc->pos_k)) return BPT_ERR_NULL;
     if (P->n_rows == 0) return P->n_edges == 0 ? BPT_OK : BPT_ERR_UNSUPPORTED;
     if (forward && P->n_groups == 0 && !narrow && !bias && !(dropout_p > 0.f)) return BPT_OK;

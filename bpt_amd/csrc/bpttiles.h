@@ -966,6 +966,7 @@ __device__ __forceinline__ void tile_walk_first_ahead(int nblk, IssueFirst &&fir
 struct ScoreMod {
     float to_tanh, from_tanh;          // scale / cap, and cap in base-2 units; to_tanh 0: not capped
     float c[4], far;                   // tile_mod_scores: the polynomial's coefficients and bound for x^2
+    float scale, slope_of;             // ... scale, and -scale / from_tanh^2
     const float *slopes;               // (heads), or null: no distance
     const float *pos_member, *pos_entry;       // positions of the plan's rows, of the rows its indices name
     float *part;                       // destination side: [group][head][part] sums of dL/ds |pos - pos|, or null
@@ -1016,10 +1017,10 @@ template <typename Row> __device__ __forceinline__ void tile_axpy_pairs(const fl
     }
 }
 
-// s (base-2 units) and ds/du of four pairs whose q.k (+ term) is x; pos_e: positions of the pairs' entries.
+// s (base-2 units) and scale ds/du of four pairs whose q.k (+ term) is x; pos_e: positions of the pairs' entries.
 // |u / cap| <= 1/2, where nearly all scores lie (a score is a few units, a cap tens): tanh z = z + z w (c0 + c1 w + c2 w^2 + c3 w^3) with w = z^2,
-// fitted by weighted least squares to the relative error, 1.5e-8 (1.25 half steps of float32 as evaluated); the factor scale / cap sits in the
-// coefficients, cap in the scaled score, and a wavefront without a larger score evaluates nothing else.  Beyond, (1 - e) / (1 + e) with
+// fitted by weighted least squares to the relative error, 1.5e-8; scale, cap and the change to base 2 sit in the coefficients, s = x (c + w' (...)) with w' = x^2,
+// scale ds/du = scale - scale (s / cap)^2, and a wavefront without a larger score evaluates nothing else.  Beyond, (1 - e) / (1 + e) with
 // e = exp(-2 |z|), whose difference keeps its digits there; for small z it is off by 2^-24 absolutely, which times a cap of 50 is more than all other
 // roundings of a score.
 __device__ __forceinline__ void tile_mod_scores(const ScoreMod &md, float scale_log2e, float slope_log2e, float pos_m, const float (&pos_e)[4],
@@ -1030,11 +1031,8 @@ __device__ __forceinline__ void tile_mod_scores(const ScoreMod &md, float scale_
         for (int r = 0; r < 4; ++r) w[r] = x[r] * x[r];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const float wp = w[r] * fmaf(fmaf(fmaf(md.c[3], w[r], md.c[2]), w[r], md.c[1]), w[r], md.c[0]);
-            const float xs = x[r] * scale_log2e, t = x[r] * md.to_tanh;
-            s[r] = fmaf(xs, wp, xs);
-            const float th = fmaf(t, wp, t);
-            du[r] = fmaf(-th, th, 1.f);
+            s[r] = x[r] * fmaf(fmaf(fmaf(fmaf(md.c[3], w[r], md.c[2]), w[r], md.c[1]), w[r], md.c[0]), w[r], scale_log2e);
+            du[r] = fmaf(s[r] * s[r], md.slope_of, md.scale);
         }
         if (__builtin_amdgcn_ballot_w64(fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3])) > md.far) != 0) {
 #pragma unroll
@@ -1042,12 +1040,12 @@ __device__ __forceinline__ void tile_mod_scores(const ScoreMod &md, float scale_
                 const float e = __builtin_amdgcn_exp2f(fabsf(x[r] * md.to_tanh) * (-2.f * LOG2E));
                 const float th = copysignf((1.f - e) * __builtin_amdgcn_rcpf(1.f + e), x[r] * md.to_tanh);
                 s[r] = w[r] > md.far ? th * md.from_tanh : s[r];
-                du[r] = w[r] > md.far ? fmaf(-th, th, 1.f) : du[r];
+                du[r] = w[r] > md.far ? fmaf(-th, th, 1.f) * md.scale : du[r];
             }
         }
     } else {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) { s[r] = x[r] * scale_log2e; du[r] = 1.f; }
+        for (int r = 0; r < 4; ++r) { s[r] = x[r] * scale_log2e; du[r] = md.scale; }
     }
     if (md.slopes) {
 #pragma unroll
@@ -1465,7 +1463,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP 
                         ds_sum += pair_if<CAREFUL>(mask[r], c, ds[r]);
                         p_sum += pe;
                     }
-                    ds[r] = pair_if<CAREFUL>(mask[r], c, ds[r] * (du[r] * scale));
+                    ds[r] = pair_if<CAREFUL>(mask[r], c, ds[r] * du[r]);
                 } else {
                     ds[r] = pe * (dp[r] * mt - delta) * scale;
                 }
@@ -2210,12 +2208,12 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(MOD ?
                     const float x = where_pair_or_zero(mk[r], c, pe * (dp[r] * mt));
                     ds[r] = fmaf(-pe, delta, x);
                     if (md.part) slope_sum += pair_if<CAREFUL>(mk[r], c, ds[r] * fabsf(pos_m - pos_e[r]));
-                    ds[r] = pair_if<CAREFUL>(mk[r], c, ds[r] * (du[r] * scale));
+                    ds[r] = pair_if<CAREFUL>(mk[r], c, ds[r] * du[r]);
                     if constexpr (FIX) {
                         dp_sum += x;
                         p_sum += pe;
                         if (md.part) far_sum += pair_if<CAREFUL>(mk[r], c, pe * fabsf(pos_m - pos_e[r]));
-                        pdu[r] = pair_if<CAREFUL>(mk[r], c, pe * (du[r] * scale));
+                        pdu[r] = pair_if<CAREFUL>(mk[r], c, pe * du[r]);
                     }
                 } else {
                     ds[r] = pe * (dp[r] * mt - delta) * scale;
@@ -2776,7 +2774,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(MOD ?
                 float mt = 1.f;                                   // dropout multiplier of this pair (as in the forward)
                 if constexpr (DROP)
                     mt = dropout_keep((uint32_t)xe[DROP ? r : 0] * (uint32_t)H + (uint32_t)t.head, drop_seed, drop_thr, drop_inv);
-                ds[r] = where_pair_or_zero(mk[r], c, MOD ? p * (dp[r] * mt - delta_e[r]) * (du[r] * scale) : p * (dp[r] * mt - delta_e[r]) * scale);
+                ds[r] = where_pair_or_zero(mk[r], c, MOD ? p * (dp[r] * mt - delta_e[r]) * du[r] : p * (dp[r] * mt - delta_e[r]) * scale);
                 pe[r] = p * mt;
             }
             if constexpr (CAREFUL) {

@@ -1251,10 +1251,10 @@ def score_options(score_cap, slopes, pos, q, k, scale):
     cap = 0.0
     if score_cap is not None:
         cap = float(score_cap)
-        if not (0.0 < cap <= 3.0e38):
-            raise ValueError("score_cap must be a finite positive number")
-        if not abs(scale) <= 1.0e4 * cap:
-            raise ValueError("score_cap must be at least |scale| / 10^4")
+        if not 1.0e-10 <= cap <= 1.0e10:
+            raise ValueError("score_cap must lie between 10^-10 and 10^10")
+        if not abs(scale) <= min(1.0e4 * cap, 1.0e6):
+            raise ValueError("score_cap must be at least |scale| / 10^4, and |scale| at most 10^6")
     if (slopes is None) != (pos is None):
         raise ValueError("slopes and pos go together")
     if slopes is None:

@@ -493,7 +493,7 @@ def bpt_attention(row, indptr_r, eid_r, indices_r, col, indptr_c, eid_c, indices
     edge e (attention.py:69-71); the gradient of rel_table is returned like any other.
 
     Score options (not in the reference): with u the scaled score, term included,
-    score_cap c > 0 makes it c tanh(u / c), which bounds it by c;
+    score_cap c > 0 (10^-10 to 10^10, and at least |scale| / 10^4) makes it c tanh(u / c), which bounds it by c;
     slopes (h,) float32 and pos, float32 positions of the rows (one tensor, or a pair (of the query rows, of the key rows)), lower it by
     slopes[head] * |pos[dst] - pos[src]| behind the cap.  slopes get a gradient, pos does not.  Heads of up to 64 columns, 16 of them,
     in float32 and bfloat16 run fused, other shapes and float64 through the chain.  Edges are the

@@ -20,7 +20,7 @@ extern "C" {
 #endif
 
 typedef struct {
-    float cap;                        /* 0: not capped; otherwise finite and at least |scale| / 10^4 */
+    float cap;                        /* 0: not capped; otherwise between 10^-10 and 10^10 and at least |scale| / 10^4, with |scale| <= 10^6 */
     const float *slopes;              /* (heads) float32, or NULL: no distance */
     const float *pos_q, *pos_k;       /* float32 positions of the query rows and of the key rows, with slopes */
 } bpt_score;

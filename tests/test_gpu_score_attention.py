@@ -258,6 +258,24 @@ def test_dropout(heads, d, kind, rel, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("cap,scale", [(1e-10, 1e-10), (1e10, 0.125), (1e10, 1e6), (0.0125, 125.0), (1e-10, 1e-6)])
+def test_the_largest_and_smallest_caps(cap, scale, dtype):
+    """Every value is an ordinary number there.  (q is scaled so that the scores are a few units or caps, whichever is less.)"""
+    c = make(("bpt", 60, 2), 8, 64, dtype, 0.0, True, q_scale=min(0.125, cap) / scale)
+    args = graph_args(c["src"].numpy(), c["dst"].numpy(), c["q"].size(0), c["k"].size(0))
+    dev = on_device(c)
+    from bpt_amd import op
+    o = op.bpt_attention(*args, dev["q"], dev["k"], dev["v"], scale=scale, score_cap=cap, slopes=dev["slopes"], pos=dev["pos_q"], fused=True)
+    grads = torch.autograd.grad(o, [dev["q"], dev["k"], dev["v"], dev["slopes"]], dev["do"])
+    chain = op.bpt_attention(*args, *(dev[n].double() for n in ("q", "k", "v")), scale=scale, score_cap=cap, slopes=dev["slopes"], pos=dev["pos_q"])
+    want = torch.autograd.grad(chain, [dev["q"], dev["k"], dev["v"], dev["slopes"]], dev["do"].double())
+    # F: o, and ds and p on their way into a product and the result, half a step each of the norm; float32's roundings are far below 2e-5 of the norm here
+    F = 4 * 2.0 ** -8 if dtype == "bf16" else 2e-5
+    for name, got, ref in zip(("o", "dq", "dk", "dv", "dslopes"), (o, *grads), (chain, *want)):
+        assert got.isfinite().all() and (got.double() - ref.double()).norm() <= F * ref.double().norm(), (name, (got.double() - ref.double()).norm() / ref.double().norm())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("heads,d", [(8, 64), (16, 64), (6, 50)])
 @pytest.mark.parametrize("cap,distance", [(30.0, False), (15.0, True)])
 def test_with_relative_positions(heads, d, cap, distance, dtype):

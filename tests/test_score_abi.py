@@ -62,9 +62,9 @@ def test_a_forward_that_does_not_fit_is_refused():
     assert forward(heads=0) == C["BPT_ERR_SHAPE"] and forward(d=0) == C["BPT_ERR_SHAPE"]
     for bad in (dict(heads=9), dict(d=3), dict(d=65), dict(heads=6, bias=p), dict(heads=6, d=49, dtype=2)):
         assert forward(**bad) == C["BPT_ERR_UNSUPPORTED"], bad
-    for cap in (-1.0, float("inf"), float("nan"), 1e-6):
+    for cap in (-1.0, float("inf"), float("nan"), 1e-6, 1e-11, 1e11):
         assert forward(score=(cap, None, None, None)) == C["BPT_ERR_SIZE"], cap
-    assert forward(scale=float("nan")) == C["BPT_ERR_SIZE"]
+    assert forward(scale=float("nan")) == C["BPT_ERR_SIZE"] and forward(score=(1e9, None, None, None), scale=1e7) == C["BPT_ERR_SIZE"]
     for rate in (-0.1, 1.0, float("nan")):
         assert forward(p=rate) == C["BPT_ERR_SIZE"], rate
     assert forward(score=(0.0, p, None, p)) == C["BPT_ERR_NULL"] and forward(score=(0.0, p, p, None)) == C["BPT_ERR_NULL"]
@@ -108,7 +108,7 @@ def test_what_the_operator_refuses():
     graph = (e, ptr, e, e, e, ptr, e, e)
     q = torch.randn(3, 8, 64)
     go = lambda **kw: op.bpt_attention(*graph, q, q, q, **kw)
-    for cap in (0.0, -2.0, float("inf"), float("nan"), 1e-9):
+    for cap in (0.0, -2.0, float("inf"), float("nan"), 1e-9, 1e-11, 1e11):
         with pytest.raises(ValueError, match="score_cap"):
             go(score_cap=cap)
     with pytest.raises(ValueError, match="go together"):

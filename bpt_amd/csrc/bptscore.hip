@@ -7,7 +7,7 @@
 namespace {
 
 // Split rows, a workgroup each, from the sums of their segments (bfloat16, comment at k_attn_bwd_dst_rows_bf16): delta of the row to the source side,
-// and, fix[split row][head], (delta' - delta) and what the slopes' gradient gains by it.  float32 (no stat): the latter alone, of the sum of ds that should be zero.
+// and, fix[split row][head], (delta' - delta) and what the slopes' gradient gains by it.  float32 and with a score term (no stat): the latter alone, of the sum of ds that should be zero.
 __global__ __launch_bounds__(BLOCK) void k_score_split(const int32_t *__restrict__ heavy, const float4 *__restrict__ split, float2 *__restrict__ stat,
                                                        float2 *__restrict__ fix, int heads) {
     __shared__ float4 meet[BLOCK];
@@ -556,9 +556,9 @@ inline SplitSums split_sums(char *at, const bpt_plan *Pin, int h, bool low) {
     return SplitSums{(float4 *)at, low ? (bf16_t *)(at + Pin->n_slots * h * 16) : nullptr, (float2 *)(at + Pin->n_slots * split_slot_bytes(h, low))};
 }
 inline int64_t split_bytes(const bpt_plan *Pin, int h, bool low) { return Pin->n_slots * split_slot_bytes(h, low) + round16(Pin->n_heavy * h * 8); }
-// Whether split rows' sums are looked at: bfloat16's always (delta); float32's, a launch of 5 us for the slopes' gradient alone, where they are half of the rows or more (few
+// Whether split rows' sums are looked at: bfloat16's always (delta); float32's and those with a score term, a launch of 5 us for the slopes' gradient alone, where they are half of the rows or more (few
 // queries of a long memory: 101 rows of 185 keys 1.1e-6 -> 6e-7 off).  Of a graph with few of them they carry little: L = 8192, 127 split rows, 2.7e-7 without.
-inline bool split_counts(const bpt_plan *Pin, bool f32, bool slopes) { return Pin->n_heavy > 0 && (!f32 || (slopes && 2 * Pin->n_heavy >= Pin->n_rows)); }
+inline bool split_counts(const bpt_plan *Pin, bool again, bool slopes) { return Pin->n_heavy > 0 && (again || (slopes && 2 * Pin->n_heavy >= Pin->n_rows)); }
 
 inline ScoreMod make_mod(const bpt_score *sc, float scale, bool entries_are_keys, float *part) {
     ScoreMod m{};
@@ -643,11 +643,12 @@ int run_backward(const bpt_plan *Pin, const bpt_plan *Pout, const bpt_score *sc,
     float *part = dslopes ? (float *)at : nullptr;
     at += slope_bytes(Pin, H);
     const SplitSums split = split_sums(at, Pin, H, again);
-    if (again || sizeof(T) == 4) at += split_bytes(Pin, H, again);
+    at += split_bytes(Pin, H, again);
     float *ws_dq = (float *)at, *ws_dk = ws_dq + (size_t)Pin->n_slots * H * D, *ws_dv = ws_dk + (size_t)Pout->n_slots * H * D;
     const int parts_in = tile_parts(Pin, H, sizeof(T)), parts_out = tile_parts(Pout, H, sizeof(T));
     ScoreMod md = make_mod(sc, scale, true, part);
-    md.split = again || split_counts(Pin, sizeof(T) == 4, dslopes != nullptr) ? split.sums : nullptr;
+    const bool fixed = split_counts(Pin, again, dslopes != nullptr);
+    md.split = fixed ? split.sums : nullptr;
     md.low = split.low;
     pick(drop.thr != 0, biased, parts_in, [&](auto dr, auto bi, auto sp) {
         const dim3 grid((unsigned)(group_grid(Pin) * (H * sp() / HW))), block(HW * WAVE);
@@ -662,9 +663,8 @@ int run_backward(const bpt_plan *Pin, const bpt_plan *Pout, const bpt_score *sc,
     });
     int st = launch_status();
     if (st != BPT_OK) return st;
-    const bool fixed = (again || sizeof(T) == 4) && split_counts(Pin, sizeof(T) == 4, dslopes != nullptr);
     if (fixed)
-        hipLaunchKernelGGL(k_score_split, dim3((unsigned)Pin->n_heavy), dim3(BLOCK), 0, s, Pin->heavy, (const float4 *)split.sums, sizeof(T) == 4 ? (float2 *)nullptr : (float2 *)scratch, split.fix, H);
+        hipLaunchKernelGGL(k_score_split, dim3((unsigned)Pin->n_heavy), dim3(BLOCK), 0, s, Pin->heavy, (const float4 *)split.sums, again ? (float2 *)scratch : (float2 *)nullptr, split.fix, H);
     pick(drop.thr != 0, biased, parts_out, [&](auto dr, auto bi, auto sp) {
         const dim3 grid((unsigned)(group_grid(Pout) * (H * sp() / HW))), block(HW * WAVE);
         if constexpr (sizeof(T) == 4)
@@ -681,7 +681,7 @@ int run_backward(const bpt_plan *Pin, const bpt_plan *Pout, const bpt_score *sc,
     st = launch_status();
     if (st != BPT_OK) return st;
     const SlopeSum sum{part, Pin->grp_chunks + 8, H, parts_in, split.fix, fixed ? (int)Pin->n_heavy : 0, dslopes ? H : 0, dslopes};
-    return run_merge<T, false>(sum, Pin, Pout, ws_dq, fixed ? split.low : nullptr, (T *)dq, ws_dk, (T *)dk, (T *)dv, H * D, Narrow{}, s);
+    return run_merge<T, false>(sum, Pin, Pout, ws_dq, again && fixed ? split.low : nullptr, (T *)dq, ws_dk, (T *)dk, (T *)dv, H * D, Narrow{}, s);
 }
 
 // Heads of fewer than 64 columns, read as they are.
@@ -728,7 +728,8 @@ int run_backward_narrow(const bpt_plan *Pin, const bpt_plan *Pout, const bpt_sco
     const int parts = tile_parts(Pin, nw.heads, sizeof(T)), parts_src = tile_parts(Pout, nw.heads, sizeof(T));
     const Narrow np = narrow_parts(nw, parts), np_src = narrow_parts(nw, parts_src);
     ScoreMod md = make_mod(sc, scale, true, part);
-    md.split = !F32 || split_counts(Pin, F32, dslopes != nullptr) ? split.sums : nullptr;
+    const bool fixed = split_counts(Pin, !F32, dslopes != nullptr);
+    md.split = fixed ? split.sums : nullptr;
     md.low = split.low;
     pick(drop.thr != 0, false, parts, [&](auto dr, auto, auto sp) {
         constexpr int HW = sp() == 1 ? NARROW_HW : sp();
@@ -742,7 +743,6 @@ int run_backward_narrow(const bpt_plan *Pin, const bpt_plan *Pout, const bpt_sco
     });
     int st = launch_status();
     if (st != BPT_OK) return st;
-    const bool fixed = split_counts(Pin, F32, dslopes != nullptr);
     if (fixed)          // (the padding heads' sums are not used)
         hipLaunchKernelGGL(k_score_split, dim3((unsigned)Pin->n_heavy), dim3(BLOCK), 0, s, Pin->heavy, (const float4 *)split.sums, F32 ? nullptr : scratch, split.fix, nw.h);
     pick(!F32 && drop.thr != 0, false, parts_src, [&](auto dr, auto, auto sp) {
@@ -758,7 +758,7 @@ int run_backward_narrow(const bpt_plan *Pin, const bpt_plan *Pout, const bpt_sco
     st = launch_status();
     if (st != BPT_OK) return st;
     const SlopeSum sum{part, Pin->grp_chunks + 8, nw.h, parts, split.fix, fixed ? (int)Pin->n_heavy : 0, dslopes ? nw.heads : 0, dslopes};
-    return run_merge<T, true>(sum, Pin, Pout, ws_dq, fixed ? split.low : nullptr, dq, ws_dk, dk, dv, C, nw, s);
+    return run_merge<T, true>(sum, Pin, Pout, ws_dq, !F32 && fixed ? split.low : nullptr, dq, ws_dk, dk, dv, C, nw, s);
 }
 
 inline int check_score(const bpt_plan *P, const bpt_score *sc, int heads, int d, int h, int dtype, float scale, float dropout_p, const float *bias,
@@ -816,7 +816,7 @@ int64_t bpt_score_forward_workspace_bytes(const bpt_plan *plan_in, int h) {
 
 int64_t bpt_score_backward_workspace_bytes(const bpt_plan *plan_in, const bpt_plan *plan_out, int h, int dtype, int has_bias) {
     if (!plan_in || !plan_out || h < 1 || (dtype != BPT_F32 && dtype != BPT_BF16)) return -1;
-    return scratch_bytes(plan_in, plan_out, h, dtype, has_bias != 0) + slope_bytes(plan_in, h) + (dtype == BPT_F32 || !has_bias ? split_bytes(plan_in, h, dtype == BPT_BF16) : 0) +
+    return scratch_bytes(plan_in, plan_out, h, dtype, has_bias != 0) + slope_bytes(plan_in, h) + split_bytes(plan_in, h, dtype == BPT_BF16 && !has_bias) +
            round16((plan_in->n_slots + 2 * plan_out->n_slots) * (int64_t)h * 64 * 4);
 }
 

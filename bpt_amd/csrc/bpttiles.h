@@ -970,7 +970,7 @@ struct ScoreMod {
     const float *slopes;               // (heads), or null: no distance
     const float *pos_member, *pos_entry;       // positions of the plan's rows, of the rows its indices name
     float *part;                       // destination side: [group][head][part] sums of dL/ds |pos - pos|, or null
-    float4 *split;                     // destination side: [slot][head] sums of p dP (float32: of ds before du), of p |pos - pos| and of p over a split row's segment, or null
+    float4 *split;                     // destination side: [slot][head] sums of p dP (float32 and with a score term: of ds before du), of p |pos - pos| and of p over a split row's segment, or null
     bf16_t *low;                       // bfloat16 destination side: [slot][column] sums of p du K
 };
 struct NoMod {};
@@ -1084,6 +1084,19 @@ template <int SP, int HW> __device__ __forceinline__ void tile_parts_sum(float4 
         const float4 x = meet[i * (HW / SP) + t.wv % (HW / SP)][t.c];
         sums.x += x.x; sums.y += x.y; sums.z += x.z; sums.w += x.w;
     }
+}
+// The sum of a row's ds is zero, but for delta's rounding and the pairs', by which the row's mean distance multiplies: taken off slope_sum.  The rows of
+// segments are left to k_score_split, where it runs.
+template <int SP, int HW>
+__device__ __forceinline__ void tile_slope_fix(const ScoreMod &md, const TileCtx &t, int heads, float ds_sum, float far_sum, float p_sum, float &slope_sum) {
+    float4 sums = make_float4(groups_sum(ds_sum), groups_sum(far_sum), groups_sum(p_sum), 0.f);      // of member c, of this part
+    if constexpr (SP > 1) {
+        __shared__ float4 meet[HW][TILE_R];
+        tile_parts_sum<SP, HW>(meet, t, sums);
+    }
+    const bool segment = t.member.y >= 0;
+    if (!segment && sums.z != 0.f) slope_sum = fmaf(-sums.x / sums.z, far_sum, slope_sum);
+    if (segment && md.split && t.g == 0 && t.part == 0) md.split[(size_t)t.member.y * heads + t.head] = sums;
 }
 // dslope of a wavefront's pairs (part s of SP of a group and head): the sum over its lanes
 template <int SP> __device__ __forceinline__ void tile_put_slope_part(const ScoreMod &md, const TileCtx &t, int heads, float x) {
@@ -1490,17 +1503,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP 
         }
     }
     if constexpr (MOD) {
-        if (md.part) {
-            // The sum of a row's ds is zero, but for delta's rounding and the pairs', by which the row's mean distance multiplies: taken off
-            float4 sums = make_float4(groups_sum(ds_sum), groups_sum(far_sum), groups_sum(p_sum), 0.f);      // of member c, of this part
-            if constexpr (SP > 1) {
-                __shared__ float4 meet[HW][TILE_R];
-                tile_parts_sum<SP, HW>(meet, t, sums);
-            }
-            const bool segment = t.member.y >= 0;
-            if (!segment && sums.z != 0.f) slope_sum = fmaf(-sums.x / sums.z, far_sum, slope_sum);
-            if (segment && md.split && g == 0 && t.part == 0) md.split[(size_t)t.member.y * Hs + t.head] = sums;
-        }
+        if (md.part) tile_slope_fix<SP, HW>(md, t, Hs, ds_sum, far_sum, p_sum, slope_sum);
         tile_put_slope_part<SP>(md, t, Hs, slope_sum);
     }
     if constexpr (SP > 1) {
@@ -2047,6 +2050,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP 
 // gradient, a sum over all pairs that nothing rounds, as far.  The pairs of a whole row give delta in 32 bits, sum p dP / sum p, once they have all been seen:
 //   ds = p (dP - delta') du  corrected by  (delta' - delta) sum p du K  in dq and by  (delta' - delta) sum p |pos - pos|  in the slopes' gradient,
 // the source side is handed delta.  (The sum of p, 1 but for the rounding of lse, keeps the sum of ds over a row at zero, by which distances in the hundreds multiply.)
+// With a score term the pairs leave for the source side as they are formed, so dq, dk and dv keep delta', the slopes' gradient does not (tile_slope_fix).
 // One more product a block over the K rows at hand.  The segments of a split row leave their sums, that of p du K rounded to bfloat16 (2^-9 of a
 // correction that is 2^-8 of dq): k_score_split forms delta and the slopes' correction before the source side runs, k_score_merge dq's.
 template <int H, int D, int HW, int WPE, bool DROP, int BIAS, bool PDS, int SP, bool MOD = false>
@@ -2207,12 +2211,19 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(MOD ?
                 if constexpr (MOD) {
                     const float x = where_pair_or_zero(mk[r], c, pe * (dp[r] * mt));
                     ds[r] = fmaf(-pe, delta, x);
-                    if (md.part) slope_sum += pair_if<CAREFUL>(mk[r], c, ds[r] * fabsf(pos_m - pos_e[r]));
+                    if (md.part) {
+                        const float far = fabsf(pos_m - pos_e[r]);
+                        slope_sum += pair_if<CAREFUL>(mk[r], c, ds[r] * far);
+                        far_sum += pair_if<CAREFUL>(mk[r], c, pe * far);
+                        if constexpr (!FIX) {
+                            dp_sum += pair_if<CAREFUL>(mk[r], c, ds[r]);
+                            p_sum += pe;
+                        }
+                    }
                     ds[r] = pair_if<CAREFUL>(mk[r], c, ds[r] * du[r]);
                     if constexpr (FIX) {
                         dp_sum += x;
                         p_sum += pe;
-                        if (md.part) far_sum += pair_if<CAREFUL>(mk[r], c, pe * fabsf(pos_m - pos_e[r]));
                         pdu[r] = pair_if<CAREFUL>(mk[r], c, pe * du[r]);
                     }
                 } else {
@@ -2274,7 +2285,12 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(MOD ?
             tile_put_low<SP, H, D, false>(md, t, piece[t.wv], piece[t.wv % (HW / SP)], (HW / SP) * PIECE, pk, nw);
         }
     }
-    if constexpr (MOD) tile_put_slope_part<SP>(md, t, H, slope_sum);
+    if constexpr (MOD) {
+        if constexpr (!FIX) {
+            if (md.part) tile_slope_fix<SP, HW>(md, t, H, dp_sum, far_sum, p_sum, slope_sum);
+        }
+        tile_put_slope_part<SP>(md, t, H, slope_sum);
+    }
     if constexpr (SP > 1) {
         tile_sums_by_row(piece[t.wv], acc, c, g);
         tile_park(piece[t.wv], acc, t.lane);

@@ -451,11 +451,12 @@ def test_replays_of_a_captured_pass_match_the_eager_one():
             assert torch.equal(got, want)
 
 
-@pytest.mark.parametrize("heads,d", [(8, 64), (16, 64), (6, 50)])
-@pytest.mark.parametrize("kind", [("bpt", 700, 4), ("memory", 71, 774), ("window", 1500, 40)], ids=str)
-def test_slopes_of_bfloat16_rows_are_summed_in_32_bits(kind, heads, d):
-    """Nothing that the slopes' gradient is summed from is rounded to bfloat16 (delta comes from the pairs): float32's bound, of the same values."""
-    c = make(kind, heads, d, "bf16", 15.0, True)
+@pytest.mark.parametrize("heads,d,kind,rel", [(h, d, kind, False) for h, d in ((8, 64), (16, 64), (6, 50)) for kind in (("bpt", 700, 4), ("memory", 71, 774), ("window", 1500, 40))]
+                         + [(h, d, kind, True) for h, d in ((8, 64), (6, 50)) for kind in (("random", 900, 15000), ("memory", 71, 774))], ids=str)
+def test_slopes_of_bfloat16_rows_are_summed_in_32_bits(heads, d, kind, rel):
+    """Nothing that the slopes' gradient is summed from is rounded to bfloat16 (delta comes from the pairs): float32's bound, of the same values.  With a score term this
+    holds where no row is split or half of them are."""
+    c = make(kind, heads, d, "bf16", 15.0, True, rel=rel)
     wide = {n: t.float() if torch.is_tensor(t) and t.dtype == torch.bfloat16 else t for n, t in c.items()}
     got = run(c, graph_args(c["src"].numpy(), c["dst"].numpy(), c["q"].size(0), c["k"].size(0)), True)
     close(got["dslopes"], reference(wide)["dslopes"], "dslopes", torch.float32)

@@ -1315,15 +1315,25 @@ def _score_rows(eid_c, q, dropout_p, bias, train):
     return edges >= 384 * rows and (rows <= 4 or (rows <= 8 and edges <= 4096 * rows))
 
 
+def _score_seg(n_edges, q, k):
+    """_tile_seg_of, but shorter items where few long rows of one node set attend to another (a memory) and 256 edges an item leave fewer than 3000 items times
+    heads: a tile is sixteen items, which share nothing there, walked in one chain.  Kernels of a training pass, us, items of 32 | 64 | 128 | 256 edges:
+      float32 8 heads   2 rows of 8192  51 | 58 | 80 | 129;   1 of 2048  46 | 73 | 123 | 123;   8 of 8192  51 | 45 | 46 | 57;   71 of 774  43 | 39 | 38 | 48;   32 of 4096  46 | 42 | 39 | 42
+      bfloat16          2 of 8192  40 | 39 | 46 | 68;   16 heads, 8 of 2505  34 | 31 | 31 | 34;   16 heads, 16 of 8192  67 | 55 | 48 | 45;   128 of 4096  97 | 73 | 59 | 51"""
+    if TILE_SEG_LEN is None and q.size(0) != k.size(0) and n_edges >= 256 * q.size(0):
+        return next((seg for seg in (256, 128, 64) if n_edges * q.size(1) >= 3000 * seg), 32)
+    return _tile_seg_of(n_edges, q.size(0), k.size(0))
+
+
 def _score_plan_in(graph, q, k, built=None):
     col, indptr_c, eid_c, indices_c = graph[4:]
-    return plan_cache.get(col, indptr_c, eid_c, indices_c, q.size(0), k.size(0), seg_len=_tile_seg_of(eid_c.size(0), q.size(0), k.size(0)),
+    return plan_cache.get(col, indptr_c, eid_c, indices_c, q.size(0), k.size(0), seg_len=_score_seg(eid_c.size(0), q, k),
                           prefer_device=True, groups=(TILE_ROWS, None), built=built)
 
 
 def _score_plan_out(graph, q, k, built=None):
     row, indptr_r, eid_r, indices_r = graph[:4]
-    return plan_cache.get(row, indptr_r, eid_r, indices_r, k.size(0), q.size(0), seg_len=_tile_seg_of(eid_r.size(0), q.size(0), k.size(0)),
+    return plan_cache.get(row, indptr_r, eid_r, indices_r, k.size(0), q.size(0), seg_len=_score_seg(eid_r.size(0), q, k),
                           prefer_device=True, groups=(TILE_ROWS, _plan.tile_order_src(k.size(0), eid_r.size(0))), built=built)
 
 
@@ -1344,7 +1354,7 @@ def prepare_score(graph, q, k, dropout_p, train):
     if train:
         _expect_index(graph[2], graph[3])
         _expect_shape(graph[2], graph[6].shape, "eid_r")
-        seg = _tile_seg_of(graph[6].size(0), q.size(0), k.size(0))
+        seg = _score_seg(graph[6].size(0), q, k)
         sides = [(*graph[4:], q.size(0), k.size(0), seg, None), (*graph[:4], k.size(0), q.size(0), seg, _plan.tile_order_src(k.size(0), graph[2].size(0)))]
         if plan_cache.may_hold(sides):
             plans = plan_cache.put_tile_plans(sides) or plans

@@ -3,10 +3,11 @@
  * The fused pass of bptattn.h (bpt_attention_forward / _backward) with, for an edge and head and u = (q[dst].k[src] + bias) scale,
  *   s = cap tanh(u / cap)   (s = u where cap is 0)   - slopes[head] |pos_q[dst] - pos_k[src]|   (where slopes is given)
  * in place of u.  Heads of 64 columns; float32 with 4, 8 or 16 of them, bfloat16 with 8 or 16; without a bias also heads of 4 to 64 columns as
- * they are (bfloat16: of an even number of columns; rows start on 4 bytes), `heads` of them, computed as h = 4, 8 or 16 (h is what lse (n, h), the workspace and dropout's hash count).  Plans carry groups of 16 rows
- * (tiles), the source side's the pair numbers of the destination side's; grp_eids where there is dropout or a bias.  A forward on a plan without
- * groups walks single rows (heads of 64 columns, no dropout, no bias): few rows of many edges.  Conventions, status codes,
- * plans, bias, ds_out, dropout and lse are those of bptattn.h (bias by edge id: bias_by_pair is refused).  Deterministic; nothing is allocated.
+ * they are (bfloat16: of an even number of columns; rows start on 4 bytes), `heads` of them, computed as h = 4, 8 or 16, which is what lse (n, h),
+ * the workspace and dropout's hash count.  Plans carry groups of 16 rows (tiles), the source side's the pair numbers of the destination side's;
+ * grp_eids where there is dropout or a bias.  A forward on a plan without groups walks single rows (heads of 64 columns, no dropout, no bias): few
+ * rows of many edges.  Conventions, status codes, plans, bias, ds_out, dropout and lse are those of bptattn.h (bias by edge id: bias_by_pair is
+ * refused; a row with a NaN score is NaN, and so is its lse).  Deterministic; nothing is allocated.
  */
 #ifndef BPTSCORE_H
 #define BPTSCORE_H

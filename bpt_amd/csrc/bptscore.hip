@@ -556,9 +556,13 @@ inline SplitSums split_sums(char *at, const bpt_plan *Pin, int h, bool low) {
     return SplitSums{(float4 *)at, low ? (bf16_t *)(at + Pin->n_slots * h * 16) : nullptr, (float2 *)(at + Pin->n_slots * split_slot_bytes(h, low))};
 }
 inline int64_t split_bytes(const bpt_plan *Pin, int h, bool low) { return Pin->n_slots * split_slot_bytes(h, low) + round16(Pin->n_heavy * h * 8); }
-// Whether split rows' sums are looked at: bfloat16's always (delta); float32's and those with a score term, a launch of 5 us for the slopes' gradient alone, where they are half of the rows or more (few
-// queries of a long memory: 101 rows of 185 keys 1.1e-6 -> 6e-7 off).  Of a graph with few of them they carry little: L = 8192, 127 split rows, 2.7e-7 without.
-inline bool split_counts(const bpt_plan *Pin, bool again, bool slopes) { return Pin->n_heavy > 0 && (again || (slopes && 2 * Pin->n_heavy >= Pin->n_rows)); }
+// Whether split rows' sums are looked at: bfloat16's always, for delta (again) or, with a score term, for the slopes' gradient, which a delta from o as stored puts off
+// by more than itself where the long rows' parts cancel (L = 8192, 127 split rows, 1.1e-5 of the sum of its terms' absolute values, 1.1e-9 with them; the launch: a training pass 173.6 -> 176.5 us).
+// float32's, a launch of 5 us for the slopes' gradient alone, where they are half of the rows or more (few queries of a long memory: 101 rows of 185 keys
+// 1.1e-6 -> 6e-7 off).  Of a graph with few of them they carry little there: L = 8192, 127 split rows, 2.7e-7 without.
+inline bool split_counts(const bpt_plan *Pin, bool again, bool slopes, bool rounded) {
+    return Pin->n_heavy > 0 && (again || (slopes && (rounded || 2 * Pin->n_heavy >= Pin->n_rows)));
+}
 
 inline ScoreMod make_mod(const bpt_score *sc, float scale, bool entries_are_keys, float *part) {
     ScoreMod m{};
@@ -647,7 +651,7 @@ int run_backward(const bpt_plan *Pin, const bpt_plan *Pout, const bpt_score *sc,
     float *ws_dq = (float *)at, *ws_dk = ws_dq + (size_t)Pin->n_slots * H * D, *ws_dv = ws_dk + (size_t)Pout->n_slots * H * D;
     const int parts_in = tile_parts(Pin, H, sizeof(T)), parts_out = tile_parts(Pout, H, sizeof(T));
     ScoreMod md = make_mod(sc, scale, true, part);
-    const bool fixed = split_counts(Pin, again, dslopes != nullptr);
+    const bool fixed = split_counts(Pin, again, dslopes != nullptr, sizeof(T) == 2);
     md.split = fixed ? split.sums : nullptr;
     md.low = split.low;
     pick(drop.thr != 0, biased, parts_in, [&](auto dr, auto bi, auto sp) {
@@ -728,7 +732,7 @@ int run_backward_narrow(const bpt_plan *Pin, const bpt_plan *Pout, const bpt_sco
     const int parts = tile_parts(Pin, nw.heads, sizeof(T)), parts_src = tile_parts(Pout, nw.heads, sizeof(T));
     const Narrow np = narrow_parts(nw, parts), np_src = narrow_parts(nw, parts_src);
     ScoreMod md = make_mod(sc, scale, true, part);
-    const bool fixed = split_counts(Pin, !F32, dslopes != nullptr);
+    const bool fixed = split_counts(Pin, !F32, dslopes != nullptr, !F32);
     md.split = fixed ? split.sums : nullptr;
     md.low = split.low;
     pick(drop.thr != 0, false, parts, [&](auto dr, auto, auto sp) {

@@ -1022,7 +1022,8 @@ template <typename Row> __device__ __forceinline__ void tile_axpy_pairs(const fl
 // fitted by weighted least squares to the relative error, 1.5e-8; scale, cap and the change to base 2 sit in the coefficients, s = x (c + w' (...)) with w' = x^2,
 // scale ds/du = scale - scale (s / cap)^2, and a wavefront without a larger score evaluates nothing else.  Beyond, (1 - e) / (1 + e) with
 // e = exp(-2 |z|), whose difference keeps its digits there; for small z it is off by 2^-24 absolutely, which times a cap of 50 is more than all other
-// roundings of a score.
+// roundings of a score.  The derivative is 4 e / (1 + e)^2 there: 1 - tanh^2 has lost half its digits at |z| = 4 and all of them at 9.  Below 2^-53 (|z| = 18.7)
+// it counts as 0, as 1 - tanh^2 does in 64 bits.
 __device__ __forceinline__ void tile_mod_scores(const ScoreMod &md, float scale_log2e, float slope_log2e, float pos_m, const float (&pos_e)[4],
                                                 const float (&x)[4], float (&s)[4], float (&du)[4]) {
     if (md.to_tanh != 0.f) {
@@ -1037,10 +1038,9 @@ __device__ __forceinline__ void tile_mod_scores(const ScoreMod &md, float scale_
         if (__builtin_amdgcn_ballot_w64(fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3])) > md.far) != 0) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const float e = __builtin_amdgcn_exp2f(fabsf(x[r] * md.to_tanh) * (-2.f * LOG2E));
-                const float th = copysignf((1.f - e) * __builtin_amdgcn_rcpf(1.f + e), x[r] * md.to_tanh);
-                s[r] = w[r] > md.far ? th * md.from_tanh : s[r];
-                du[r] = w[r] > md.far ? fmaf(-th, th, 1.f) * md.scale : du[r];
+                const float e = __builtin_amdgcn_exp2f(fabsf(x[r] * md.to_tanh) * (-2.f * LOG2E)), inv = __builtin_amdgcn_rcpf(1.f + e);
+                s[r] = w[r] > md.far ? copysignf((1.f - e) * inv, x[r] * md.to_tanh) * md.from_tanh : s[r];
+                du[r] = w[r] > md.far ? (e < 0x1p-55f ? 0.f : 4.f * e * inv * inv * md.scale) : du[r];
             }
         }
     } else {

@@ -403,6 +403,21 @@ def _edge_distance(score, col, indptr_c, eid_c, indices_c):
     return torch.zeros(eid_c.numel(), dtype=far.dtype, device=far.device).index_copy(0, eid_c.index_select(0, slots), far)
 
 
+class _Capped(Function):
+    """cap tanh(u / cap), whose derivative is formed as 1 / cosh^2(u / cap): 1 - tanh^2, which torch's tanh hands back, keeps no digits in 32 bits beyond 9 caps."""
+
+    @staticmethod
+    def forward(ctx, u, cap):
+        ctx.save_for_backward(u)
+        ctx.cap = cap
+        return cap * torch.tanh(u / cap)
+
+    @staticmethod
+    def backward(ctx, grad):
+        (u,) = ctx.saved_tensors
+        return grad / torch.cosh(u / ctx.cap).square(), None
+
+
 def _score_chain(graph, q, k, v, scale, dropout_p, rel_table, etype, score):
     """Attention with score options as the chain of separate operators, for shapes and types without a fused kernel: the (E, h) scores are
     capped and lowered in 32 bits (64 for float64)."""
@@ -412,7 +427,7 @@ def _score_chain(graph, q, k, v, scale, dropout_p, rel_table, etype, score):
         e = e + node_mul_edge(col, indptr_c, eid_c, q, edge_type_embedding(rel_table, etype))
     e = (e if e.dtype == torch.float64 else e.float()) * scale
     if score.cap:
-        e = score.cap * torch.tanh(e / score.cap)
+        e = _Capped.apply(e, score.cap)
     if score.slopes is not None:
         far = _edge_distance(score, col, indptr_c, eid_c, indices_c).to(e.dtype)
         e = e - (score.slopes.to(e.dtype) * far[:, None] if e.dim() == 2 else score.slopes.to(e.dtype) * far)

@@ -175,7 +175,7 @@ __global__ __launch_bounds__(NW == 1 ? BLOCK : NW * WAVE) void k_score_fwd_rows(
 #pragma unroll
     for (int i = 0; i < L::EPL; ++i) acc[i] = 0.f;
     const float slope = md.slopes ? md.slopes[head] * LOG2E : 0.f, pos_m = md.slopes ? md.pos_member[it.row] : 0.f;
-    float m = M_INIT_LOG2, l = 0.f;
+    float m = m_init<true>(), l = 0.f;
     for (int p0 = it.begin; p0 < it.end; p0 += WAVE) {
         const int cnt = min(WAVE, it.end - p0);
         const int my_idx = lane < cnt ? P.idx[p0 + lane] : 0;

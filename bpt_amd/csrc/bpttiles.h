@@ -19,6 +19,9 @@ constexpr int WAVES_PER_BLOCK = 4;
 constexpr int BLOCK = WAVE * WAVES_PER_BLOCK;
 constexpr float M_INIT_LOG2 = -1.4426950408889634e9f;   // -1e9 (graphop_kernel.cu:428) in base-2 units
 constexpr float LOG2E = 1.4426950408889634f;
+// Where a running maximum starts.  MOD (score options): a slope times a distance has no bound that scores of products have, and a row whose scores all lie below the
+// start would count as empty.
+template <bool MOD> constexpr float m_init() { return MOD ? -3.0e38f : M_INIT_LOG2; }
 
 // ------------------------------------------------------------------------------------------
 // element types
@@ -426,7 +429,7 @@ __global__ __launch_bounds__(BLOCK) void k_attn_fwd_combine(const int32_t *__res
     const int j = blockIdx.y * WAVE + lane, head = j / D;
     const float *ml = ws_ml + ((size_t)s0 * H + head) * 2;      // slot stride 2*H
     const float *col = ws_acc + (size_t)s0 * C + j;              // slot stride C
-    float M = M_INIT_LOG2, lsum = 0.f, a = 0.f;
+    float M = m_init<MOD>(), lsum = 0.f, a = 0.f;
     int kk = w;
     float tm[16], tl[16], ta[16];
     auto ask = [&](int u, int nth) {
@@ -826,7 +829,7 @@ __device__ __forceinline__ void tile_meet_forward(float *mine, const float *part
         mine[TILE_PART_FLOATS + 2 * t.c + 1] = lt;
     }
     __syncthreads();
-    float wgt[SP], l = 0.f, M = M_INIT_LOG2;
+    float wgt[SP], l = 0.f, M = m_init<MOD>();
 #pragma unroll
     for (int s = 0; s < SP; ++s) {
         wgt[s] = part0[s * stride + TILE_PART_FLOATS + 2 * t.c];
@@ -1153,7 +1156,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(4))) 
     floatx4v acc[4];
 #pragma unroll
     for (int nb = 0; nb < 4; ++nb) acc[nb] = floatx4v{0.f, 0.f, 0.f, 0.f};
-    float mref = M_INIT_LOG2, lrun = 0.f;
+    float mref = m_init<MOD>(), lrun = 0.f;
     bool fresh = true;                                            // nothing has been summed up yet
     struct Blk {
         float4 kq[4];                                             // columns 4 c .. 4 c + 3 of the K rows of entries 4 r + g
@@ -1260,7 +1263,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(4))) 
         if (tile_any_odd(tile_odd(acc))) {      // (what does not exist must not reach the sums: tile_odd)
 #pragma unroll
             for (int nb = 0; nb < 4; ++nb) acc[nb] = floatx4v{0.f, 0.f, 0.f, 0.f};
-            mref = M_INIT_LOG2;
+            mref = m_init<MOD>();
             lrun = 0.f;
             fresh = true;
             walk(std::true_type{});
@@ -1898,7 +1901,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP 
     floatx4v acc[4];
 #pragma unroll
     for (int nb = 0; nb < 4; ++nb) acc[nb] = floatx4v{0.f, 0.f, 0.f, 0.f};
-    float mref = M_INIT_LOG2, lrun = 0.f;
+    float mref = m_init<MOD>(), lrun = 0.f;
     bool fresh = true;                                            // nothing has been summed up yet
     struct Blk {
         uintx4v kr[2], vr[2];
@@ -2013,7 +2016,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP 
         if (tile_any_odd(tile_odd(acc))) {      // (what does not exist must not reach the sums: tile_odd)
 #pragma unroll
             for (int nb = 0; nb < 4; ++nb) acc[nb] = floatx4v{0.f, 0.f, 0.f, 0.f};
-            mref = M_INIT_LOG2;
+            mref = m_init<MOD>();
             lrun = 0.f;
             fresh = true;
             walk(std::true_type{});
@@ -2339,7 +2342,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(MOD ?
     floatx4v acc[4];
 #pragma unroll
     for (int nb = 0; nb < 4; ++nb) acc[nb] = floatx4v{0.f, 0.f, 0.f, 0.f};
-    float mref = M_INIT_LOG2, lrun = 0.f;
+    float mref = m_init<MOD>(), lrun = 0.f;
     bool fresh = true;                                            // nothing has been summed up yet
     struct Blk {
         uint2 kq[4];                                              // columns 4 c .. 4 c + 3 of the K rows of entries 4 g + r
@@ -2436,7 +2439,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(MOD ?
         if (tile_any_odd(tile_odd(acc))) {      // (what does not exist must not reach the sums: tile_odd)
 #pragma unroll
             for (int nb = 0; nb < 4; ++nb) acc[nb] = floatx4v{0.f, 0.f, 0.f, 0.f};
-            mref = M_INIT_LOG2;
+            mref = m_init<MOD>();
             lrun = 0.f;
             fresh = true;
             walk(std::true_type{});

@@ -395,12 +395,15 @@ def _served_natively(graph):
     return graph[0] is not None and graph[1] is not None and graph[2] is not None and graph[3] is not None and not torch.jit.is_tracing()
 
 
-def _edge_distance(score, col, indptr_c, eid_c, indices_c):
-    """|pos_q[dst] - pos_k[src]| by edge id (0 for edges that no unit covers)."""
+def _edge_distance(score, col, indptr_c, eid_c, indices_c, dtype):
+    """|pos_q[dst] - pos_k[src]| less that of dst's nearest in-edge, by edge id (0 for edges that no unit covers).  Softmax does not change when a row's scores
+    move together, and what is left of a slope times a distance lies near the scores that it is added to, whatever the positions are."""
     dst = torch.repeat_interleave(col, indptr_c[1:] - indptr_c[:-1])
     slots = torch.arange(dst.numel(), device=dst.device) + indptr_c[0]
-    far = (score.pos_q.index_select(0, dst) - score.pos_k.index_select(0, indices_c.index_select(0, slots))).abs()
-    return torch.zeros(eid_c.numel(), dtype=far.dtype, device=far.device).index_copy(0, eid_c.index_select(0, slots), far)
+    far = (score.pos_q.index_select(0, dst) - score.pos_k.index_select(0, indices_c.index_select(0, slots))).abs().to(dtype)
+    near = torch.full((score.pos_q.size(0),), float("inf"), dtype=dtype, device=far.device).scatter_reduce(0, dst, far, "amin")
+    far = far - torch.where(near.isfinite(), near, torch.zeros_like(near)).index_select(0, dst)
+    return torch.zeros(eid_c.numel(), dtype=dtype, device=far.device).index_copy(0, eid_c.index_select(0, slots), far)
 
 
 class _Capped(Function):
@@ -429,7 +432,7 @@ def _score_chain(graph, q, k, v, scale, dropout_p, rel_table, etype, score):
     if score.cap:
         e = _Capped.apply(e, score.cap)
     if score.slopes is not None:
-        far = _edge_distance(score, col, indptr_c, eid_c, indices_c).to(e.dtype)
+        far = _edge_distance(score, col, indptr_c, eid_c, indices_c, e.dtype)
         e = e - (score.slopes.to(e.dtype) * far[:, None] if e.dim() == 2 else score.slopes.to(e.dtype) * far)
     a = torch.nn.functional.dropout(sparse_softmax(col, indptr_c, eid_c, e.contiguous()), p=float(dropout_p), training=dropout_p > 0)
     return vec_spmm(col, indptr_c, eid_c, indices_c, row, indptr_r, eid_r, indices_r, a.to(v.dtype), v, n_rows=None if q.size(0) == v.size(0) else q.size(0))
@@ -511,7 +514,8 @@ def bpt_attention(row, indptr_r, eid_r, indices_r, col, indptr_c, eid_c, indices
     score_cap c > 0 (10^-10 to 10^10, and at least |scale| / 10^4) makes it c tanh(u / c), which bounds it by c;
     slopes (h,) float32 and pos, float32 positions of the rows (one tensor, or a pair (of the query rows, of the key rows)), lower it by
     slopes[head] * |pos[dst] - pos[src]| behind the cap.  slopes get a gradient, pos does not.  Heads of up to 64 columns, 16 of them,
-    in float32 and bfloat16 run fused, other shapes and float64 through the chain.  Edges are the
+    in float32 and bfloat16 run fused, other shapes and float64 through the chain.  The fused kernels hold scores in 32 bits: where even a row's nearest
+    key lies at slope * distance = m, its probabilities are off by a few 2^-24 m, relative (positions that count from the same place keep m small).  Edges are the
     graph's: documents that must not see each other are its separate components."""
     scale = 1.0 / math.sqrt(q.size(-1)) if scale is None else float(scale)
     if (rel_table is None) != (etype is None):

@@ -1364,7 +1364,8 @@ def prepare_score(graph, q, k, dropout_p, train):
         return False
     numbers = [q.size(0), k.size(0), score_padded_shape(q)[0], q.size(2), _dtype(q), int(dropout_p > 0.0), q.size(1)]
     in_struct = pi.struct if few else pi.ensure_groups(TILE_ROWS)["struct"]
-    plan_cache.remember((pi,), generation, _native.SCORE_FWD, list(graph[4:]), numbers, ctypes.addressof(in_struct), 0)
+    if not (train and _score_rows(graph[6], q, dropout_p, None, False)):      # (a forward without gradients is answered by the plan of its own rule, whatever was called before)
+        plan_cache.remember((pi,), generation, _native.SCORE_FWD, list(graph[4:]), numbers, ctypes.addressof(in_struct), 0)
     if train:
         po = _score_plan_out(graph, q, k, plans[1])
         if not po.covers_all_edges:

@@ -40,9 +40,11 @@ def _as_it_is(module, kind):
 def _add_norm(norm, x, residual, fused):
     """norm(x + residual) (attention.py:79, :81), by add_layer_norm where that computes the same: a LayerNorm over the last axis as it is, GPU tensors
     of one type, nothing that casts, traces or transforms."""
-    if (fused and _as_it_is(norm, nn.LayerNorm) and len(norm.normalized_shape) == 1 and x.is_cuda and x.is_contiguous() and x.dtype in (torch.float32, torch.float64, torch.bfloat16) and x.dim() > 0
-            and x.size(-1) == norm.normalized_shape[0] and x.shape == residual.shape and not torch.is_autocast_enabled() and plain_call(x, residual)
-            and all(t is None or (t.dtype == x.dtype and t.device == x.device and t.is_contiguous()) for t in (residual, norm.weight, norm.bias))):
+    if (fused and _as_it_is(norm, nn.LayerNorm) and len(norm.normalized_shape) == 1 and x.is_cuda and x.is_contiguous()
+            and x.dtype in (torch.float32, torch.float64, torch.bfloat16) and x.dim() > 0 and x.size(-1) == norm.normalized_shape[0]
+            and x.shape == residual.shape and not torch.is_autocast_enabled()
+            and all(t is None or (t.dtype == x.dtype and t.device == x.device and t.is_contiguous()) for t in (residual, norm.weight, norm.bias))
+            and plain_call(x, residual, norm.weight, norm.bias)):
         return add_layer_norm(x, residual, norm.weight, norm.bias, norm.eps)
     return norm(x + residual)
 

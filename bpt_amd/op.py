@@ -571,8 +571,9 @@ def bpt_attention(row, indptr_r, eid_r, indices_r, col, indptr_c, eid_c, indices
 
 
 def plain_call(*tensors):
-    """Whether nothing looks into a call on these tensors: no trace, no transform of torch.func, no tangent of forward-mode differentiation, no
-    subclass of Tensor with rules of its own."""
+    """Whether nothing looks into a call on these tensors (None: an argument left out): no trace, no transform of torch.func, no tangent of forward-mode
+    differentiation, no subclass of Tensor with rules of its own."""
+    tensors = [t for t in tensors if t is not None]
     return (_native_takes() and not torch.compiler.is_compiling() and all(type(t) in (torch.Tensor, torch.nn.Parameter) for t in tensors)
             and (torch.autograd.forward_ad._current_level < 0 or all(torch.autograd.forward_ad.unpack_dual(t).tangent is None for t in tensors)))
 

@@ -66,7 +66,8 @@ def _score_options(block, pos):
 
 
 class PositionwiseFeedForward(nn.Module):
-    """FFN(x) = max(0, x W_1 + b_1) W_2 + b_2   (modules/attention.py:8-19).  keep8: the activations are kept in 8 bits for the backward."""
+    """FFN(x) = max(0, x W_1 + b_1) W_2 + b_2   (modules/attention.py:8-19).  keep8: the activations are kept in 8 bits for the backward, where they are
+    float32 or bfloat16 GPU tensors and nothing traces or transforms the call."""
 
     keep8 = False           # (also of a module that was pickled without the option)
 
@@ -78,13 +79,16 @@ class PositionwiseFeedForward(nn.Module):
         self.dropout = nn.Dropout(dropout)
 
     def forward(self, x):
+        a = self.w_1(x)
         # (modules that someone has replaced, hooked or told to drop everything are called)
-        if self.keep8 and x.is_cuda and _as_it_is(self.w_2, nn.Linear) and _as_it_is(self.dropout, nn.Dropout) and not self.dropout.p >= 1.0:
-            a, w, b = self.w_1(x).contiguous(), self.w_2.weight, self.w_2.bias
-            if torch.is_autocast_enabled():
+        if self.keep8 and a.is_cuda and _as_it_is(self.w_2, nn.Linear) and _as_it_is(self.dropout, nn.Dropout) and not self.dropout.p >= 1.0:
+            w, b, cast = self.w_2.weight, self.w_2.bias, torch.is_autocast_enabled()
+            if cast:
                 w, b = w.to(a.dtype), None if b is None else b.to(a.dtype)
-            return relu_linear8(a, w, b, self.dropout.p if self.training else 0.0)
-        return self.w_2(self.dropout(torch.relu(self.w_1(x))))
+            if (a.dtype in (torch.float32, torch.bfloat16) and not (cast and a.dtype != torch.get_autocast_dtype("cuda")) and a.dim() > 0 and a.size(-1) > 0
+                    and all(t is None or (t.dtype == a.dtype and t.device == a.device and t.is_contiguous()) for t in (w, b)) and plain_call(a, w, b)):
+                return relu_linear8(a.contiguous(), w, b, self.dropout.p if self.training else 0.0)
+        return self.w_2(self.dropout(torch.relu(a)))
 
 
 class BPTBlock(nn.Module):

@@ -150,21 +150,33 @@ Three relu8_forward(const Tensor &a, double p, uint64_t seed) {
     return {y, codes, exps};
 }
 
-// da: null, or the tensor that receives da (dy itself, where nobody else has it)
-std::tuple<Tensor, Tensor> relu8_backward_into(const Tensor &dy, const Tensor &codes, const Tensor &exps, double p, const Tensor &into) {
-    check_relu8(dy, p, "dy");
+// the codes and exponents of a gradient like dy
+void check_codes(const Tensor &codes, const Tensor &exps, const Tensor &dy) {
     check_input(codes, "codes");
     check_input(exps, "exps");
     TORCH_CHECK_VALUE(codes.scalar_type() == at::kByte && exps.scalar_type() == at::kChar, "codes must be uint8 and exps int8, as relu8_forward returns them");
     TORCH_CHECK_VALUE(codes.device() == dy.device() && exps.device() == dy.device(), "all tensors of a call must be on one device");
     check_shape(codes, dy.sizes(), "codes");
     check_shape(exps, {(dy.numel() + BPT_RELU8_BLOCK - 1) / BPT_RELU8_BLOCK}, "exps");
+}
+
+// into: null, or the tensor that receives da (dy itself, where nobody else has it)
+std::tuple<Tensor, Tensor> relu8_backward_into(const Tensor &dy, const Tensor &codes, const Tensor &exps, double p, const Tensor &into) {
+    check_relu8(dy, p, "dy");
+    check_codes(codes, exps, dy);
     c10::DeviceGuard guard(dy.device());
     Tensor da = into.defined() ? into : at::empty_like(dy), y8 = at::empty_like(dy);
     check_status(bpt_relu8_backward(ptr(dy), (const uint8_t *)ptr(codes), (const int8_t *)ptr(exps), ptr(da), ptr(y8), dy.numel(), (float)p, dtype_code(dy),
                                     stream_of(dy)),
                  "relu8_backward");
     return {da, y8};
+}
+// what the codes stand for, in y8
+void relu8_values(const Tensor &codes, const Tensor &exps, Tensor &y8) {
+    check_codes(codes, exps, y8);
+    c10::DeviceGuard guard(y8.device());
+    check_status(bpt_relu8_backward(nullptr, (const uint8_t *)ptr(codes), (const int8_t *)ptr(exps), nullptr, ptr(y8), y8.numel(), 0.f, dtype_code(y8), stream_of(y8)),
+                 "relu8_backward");
 }
 std::tuple<Tensor, Tensor> relu8_backward(const Tensor &dy, const Tensor &codes, const Tensor &exps, double p) {
     return relu8_backward_into(dy, codes, exps, p, Tensor());
@@ -204,11 +216,15 @@ struct ReluLinear8 : torch::autograd::Function<ReluLinear8> {
         const int64_t inner = w.size(1), outer = w.size(0), rows = inner ? codes.numel() / inner : 0;
         const Tensor d_o = grads[0].contiguous().view({rows, outer});
         Tensor da, dw, db;
-        if (need_a || need_w) {
-            const Tensor dy = need_a ? at::mm(d_o, w) : at::empty({rows, inner}, d_o.options());
+        if (need_a) {
+            const Tensor dy = at::mm(d_o, w);
             const auto [d, y8] = relu8_backward_into(dy, codes.view({rows, inner}), exps, p, dy);
-            if (need_a) da = d.view(codes.sizes());
+            da = d.view(codes.sizes());
             if (need_w) dw = at::mm(d_o.t(), y8);
+        } else if (need_w) {                                      // (nobody reads dy, so nobody forms it)
+            Tensor y8 = at::empty({rows, inner}, d_o.options());
+            relu8_values(codes.view({rows, inner}), exps, y8);
+            dw = at::mm(d_o.t(), y8);
         }
         if (need_b) {                                             // (the column sums of the layer norm's backward)
             c10::DeviceGuard guard(d_o.device());

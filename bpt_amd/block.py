@@ -9,8 +9,8 @@ DGL graph object (`g.ndata['h']`, `g.edata['etype']`) and writes the result back
 
 Attention core: the fused kernels (`op.bpt_attention`: rel_pos term and attention dropout included), or with
 `fused=False` the four operators composed exactly as attention.py:66-77 does.
-Residual and LayerNorm: one kernel each way (`op.add_layer_norm`) on GPU tensors of one type, the torch module otherwise and with
-`fused=False`.  Projections and the feed-forward are torch modules (rocBLAS GEMMs).
+Residual and LayerNorm: one kernel each way (`op.add_layer_norm`) on GPU tensors of one type and rows of up to 16 KiB, the torch module
+otherwise and with `fused=False`.  Projections and the feed-forward are torch modules (rocBLAS GEMMs).
 
 Options the reference does not have, off by default (then nothing of them is a parameter, and the results are the reference's):
   score_cap   attention scores become cap tanh(score / cap)
@@ -38,11 +38,13 @@ def _as_it_is(module, kind):
 
 
 def _add_norm(norm, x, residual, fused):
-    """norm(x + residual) (attention.py:79, :81), by add_layer_norm where that computes the same: a LayerNorm over the last axis as it is, GPU tensors
-    of one type, nothing that casts, traces or transforms."""
+    """norm(x + residual) (attention.py:79, :81), by add_layer_norm where that computes the same and is the faster way: a LayerNorm over the last axis as it is,
+    GPU tensors of one type, nothing that casts, traces or transforms, rows that a workgroup's registers hold (16 KiB).  Longer rows are walked three times:
+    forward | training, us, add_layer_norm / torch, 16383 rows of 4096 columns float32 145 / 263 | 352 / 736, of 4104 301 / 275 | 767 / 782; of 8192 columns
+    bfloat16 152 / 305 | 378 / 898, of 8200 757 / 317 | 1952 / 955; in float64, where torch's is slower, of 2048 columns 146 / 381 | 370 / 843, of 4104 515 / 730 | 1345 / 1556."""
     if (fused and _as_it_is(norm, nn.LayerNorm) and len(norm.normalized_shape) == 1 and x.is_cuda and x.is_contiguous()
             and x.dtype in (torch.float32, torch.float64, torch.bfloat16) and x.dim() > 0 and x.size(-1) == norm.normalized_shape[0]
-            and x.shape == residual.shape and not torch.is_autocast_enabled()
+            and (x.dtype == torch.float64 or x.size(-1) * x.element_size() <= 16384) and x.shape == residual.shape and not torch.is_autocast_enabled()
             and all(t is None or (t.dtype == x.dtype and t.device == x.device and t.is_contiguous()) for t in (residual, norm.weight, norm.bias))
             and plain_call(x, residual, norm.weight, norm.bias)):
         return add_layer_norm(x, residual, norm.weight, norm.bias, norm.eps)

@@ -587,7 +587,8 @@ def add_layer_norm(x, residual=None, weight=None, bias=None, eps=1e-5):
     """Layer norm of x + residual over the last axis, (z - mean(z)) / sqrt(var(z) + eps) * weight + bias with z = x + residual: what a block
     does behind attention and feed-forward (modules/attention.py:79, :81), in one pass over memory and with its gradients in another.
     float32, float64 or bfloat16, contiguous, all of one type; residual like x or None, weight and bias (x.size(-1),) or None.  z, mean and
-    variance are held in 32 bits (64 for float64) and the result is rounded once.  Deterministic."""
+    variance are held in 32 bits (64 for float64) and the result is rounded once.  Rows of up to 16 KiB are read once, longer ones three times.
+    Deterministic."""
     _no_transforms("add_layer_norm")
     return _native.add_layer_norm(x, residual, weight, bias, float(eps))
 

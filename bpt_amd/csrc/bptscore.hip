@@ -134,8 +134,8 @@ __device__ __forceinline__ void merge_dq_block(const int32_t *__restrict__ hv, c
 // as a launch by itself cost 4 us (8 at L = 32768, k = 8).  Grid (m.wanted + n_a + n_b, C / 256, 2).
 template <typename T, bool NARROW>
 __global__ __launch_bounds__(BLOCK) void k_score_merge(SlopeSum m, const int32_t *__restrict__ heavy_a, int n_a, const float *__restrict__ ws_a,
-                                                       const bf16_t *__restrict__ low, T *__restrict__ YA, const int32_t *__restrict__ heavy_b, const float *__restrict__ ws_b, T *__restrict__ YB0, T *__restrict__ YB1,
-                                                       int C, size_t ws_stride_b, Narrow nw) {
+                                                       const bf16_t *__restrict__ low, T *__restrict__ YA, const int32_t *__restrict__ heavy_b,
+                                                       const float *__restrict__ ws_b, T *__restrict__ YB0, T *__restrict__ YB1, int C, size_t ws_stride_b, Narrow nw) {
     const int x = (int)blockIdx.x - m.wanted;
     if (x < 0) {
         if (blockIdx.y == 0 && blockIdx.z == 0) slope_sum_block(m, (int)blockIdx.x);
@@ -557,7 +557,8 @@ inline SplitSums split_sums(char *at, const bpt_plan *Pin, int h, bool low) {
 }
 inline int64_t split_bytes(const bpt_plan *Pin, int h, bool low) { return Pin->n_slots * split_slot_bytes(h, low) + round16(Pin->n_heavy * h * 8); }
 // Whether split rows' sums are looked at: bfloat16's always, for delta (again) or, with a score term, for the slopes' gradient, which a delta from o as stored puts off
-// by more than itself where the long rows' parts cancel (L = 8192, 127 split rows, 1.1e-5 of the sum of its terms' absolute values, 1.1e-9 with them; the launch: a training pass 173.6 -> 176.5 us).
+// by more than itself where the long rows' parts cancel (L = 8192, 127 split rows, 1.1e-5 of the sum of its terms' absolute values, 1.1e-9 with them; the launch: a
+// training pass 173.6 -> 176.5 us).
 // float32's, a launch of 5 us for the slopes' gradient alone, where they are half of the rows or more (few queries of a long memory: 101 rows of 185 keys
 // 1.1e-6 -> 6e-7 off).  Of a graph with few of them they carry little there: L = 8192, 127 split rows, 2.7e-7 without.
 inline bool split_counts(const bpt_plan *Pin, bool again, bool slopes, bool rounded) {
@@ -668,7 +669,8 @@ int run_backward(const bpt_plan *Pin, const bpt_plan *Pout, const bpt_score *sc,
     int st = launch_status();
     if (st != BPT_OK) return st;
     if (fixed)
-        hipLaunchKernelGGL(k_score_split, dim3((unsigned)Pin->n_heavy), dim3(BLOCK), 0, s, Pin->heavy, (const float4 *)split.sums, again ? (float2 *)scratch : (float2 *)nullptr, split.fix, H);
+        hipLaunchKernelGGL(k_score_split, dim3((unsigned)Pin->n_heavy), dim3(BLOCK), 0, s, Pin->heavy, (const float4 *)split.sums,
+                           again ? (float2 *)scratch : (float2 *)nullptr, split.fix, H);
     pick(drop.thr != 0, biased, parts_out, [&](auto dr, auto bi, auto sp) {
         const dim3 grid((unsigned)(group_grid(Pout) * (H * sp() / HW))), block(HW * WAVE);
         if constexpr (sizeof(T) == 4)
@@ -778,7 +780,8 @@ inline int check_score(const bpt_plan *P, const bpt_score *sc, int heads, int d,
     nw = narrow ? Narrow{d, heads, h, (heads + NARROW_HW - 1) / NARROW_HW} : Narrow{};
     // (within these bounds the polynomial's coefficients and squares of scores are ordinary numbers: make_mod, tile_mod_scores)
     const bool capped = sc->cap != 0.f;
-    if ((capped && !(sc->cap >= 0.9e-10f && sc->cap <= 1.1e10f && fabsf(scale) <= 1.01e4f * sc->cap && fabsf(scale) <= 1.01e6f)) || !(dropout_p >= 0.f && dropout_p < 1.f)) return BPT_ERR_SIZE;
+    if (capped && !(sc->cap >= 0.9e-10f && sc->cap <= 1.1e10f && fabsf(scale) <= 1.01e4f * sc->cap && fabsf(scale) <= 1.01e6f)) return BPT_ERR_SIZE;
+    if (!(dropout_p >= 0.f && dropout_p < 1.f)) return BPT_ERR_SIZE;
     if (sc->slopes && (!sc->pos_q || !sc->pos_k)) return BPT_ERR_NULL;
     if (P->n_rows == 0) return P->n_edges == 0 ? BPT_OK : BPT_ERR_UNSUPPORTED;
     if (forward && P->n_groups == 0 && !narrow && !bias && !(dropout_p > 0.f)) return BPT_OK;

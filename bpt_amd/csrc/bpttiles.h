@@ -973,7 +973,8 @@ struct ScoreMod {
     const float *slopes;               // (heads), or null: no distance
     const float *pos_member, *pos_entry;       // positions of the plan's rows, of the rows its indices name
     float *part;                       // destination side: [group][head][part] sums of dL/ds |pos - pos|, or null
-    float4 *split;                     // destination side: [slot][head] sums of p dP (float32 and with a score term: of ds before du), of p |pos - pos| and of p over a split row's segment, or null
+    float4 *split;                     // destination side: [slot][head] sums of p dP (float32 and with a score term: of ds before du), of p |pos - pos| and of
+                                       // p over a split row's segment, or null
     bf16_t *low;                       // bfloat16 destination side: [slot][column] sums of p du K
 };
 struct NoMod {};

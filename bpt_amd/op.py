@@ -515,7 +515,8 @@ def bpt_attention(row, indptr_r, eid_r, indices_r, col, indptr_c, eid_c, indices
     slopes (h,) float32 and pos, float32 positions of the rows (one tensor, or a pair (of the query rows, of the key rows)), lower it by
     slopes[head] * |pos[dst] - pos[src]| behind the cap.  slopes get a gradient, pos does not.  Heads of up to 64 columns, 16 of them,
     in float32 and bfloat16 run fused, other shapes and float64 through the chain.  The fused kernels hold scores in 32 bits: where even a row's nearest
-    key lies at slope * distance = m, its probabilities are off by a few 2^-24 m, relative (positions that count from the same place keep m small).  Edges are the
+    key lies at slope * distance = m, its scores and the log of their sum are off by a few 2^-24 m, which is a factor of its probabilities: positions of
+    queries and keys that count from the same place keep m small, and m beyond 10^6 leaves gradients few digits.  Edges are the
     graph's: documents that must not see each other are its separate components."""
     scale = 1.0 / math.sqrt(q.size(-1)) if scale is None else float(scale)
     if (rel_table is None) != (etype is None):

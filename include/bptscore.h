@@ -7,8 +7,8 @@
  * the workspace and dropout's hash count.  Plans carry groups of 16 rows (tiles), the source side's the pair numbers of the destination side's;
  * grp_eids where there is dropout or a bias.  A forward on a plan without groups walks single rows (heads of 64 columns, no dropout, no bias): few
  * rows of many edges.  Conventions, status codes, plans, bias, ds_out, dropout and lse are those of bptattn.h (bias by edge id: bias_by_pair is
- * refused; a row with a NaN score is NaN, and so is its lse; scores may lie as low as -2 * 10^38, held in 32 bits: with m the largest of a row's, its
- * probabilities are off by a few 2^-24 |m|, relative).  Deterministic; nothing is allocated.
+ * refused; a row with a NaN score is NaN, and so is its lse; scores may lie as low as -2 * 10^38, held in 32 bits: with m the largest of a row's, they and
+ * its lse are off by a few 2^-24 |m|, an exponent's error in its probabilities).  Deterministic; nothing is allocated.
  */
 #ifndef BPTSCORE_H
 #define BPTSCORE_H

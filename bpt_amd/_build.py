@@ -4,8 +4,9 @@
   bpt_amd/csrc/libbptattn.so   gfx950 HIP (hipcc)        <- bptattn.hip, bpttiles.h
   bpt_amd/csrc/libbptscore.so  gfx950 HIP (hipcc)        <- bptscore.hip, bpttiles.h  (attention with capped scores and distance)
   bpt_amd/csrc/libbptblock.so  gfx950 HIP (hipcc)        <- bptblock.hip, bpttiles.h  (layer norm of a sum, relu kept in 8 bits)
+  bpt_amd/csrc/libbptlinear.so gfx950 HIP (hipcc)       <- bptlinear.hip, bpttiles.h  (matrix products with an epilogue, dropout)
   bpt_amd/csrc/libbptplan.so   gfx950 HIP (hipcc)        <- bptplan.hip  (plans built on the GPU; rocPRIM headers)
-  bpt_amd/csrc/bptop.so        host C++ (g++, torch)     <- bptop.cpp, bptblockop.cpp  (host side of the ops and their autograd; links them)
+  bpt_amd/csrc/bptop.so        host C++ (g++, torch)     <- bptop.cpp, bptblockop.cpp, bptlinearop.cpp, bpthost.h  (host side of the ops and their autograd; links them)
 
 hipcc cross-compiles for gfx950 without a GPU.  Run `python -m bpt_amd._build`.
 """
@@ -19,6 +20,7 @@ ATTN_SO = os.path.join(CSRC, "libbptattn.so")
 PLAN_SO = os.path.join(CSRC, "libbptplan.so")
 SCORE_SO = os.path.join(CSRC, "libbptscore.so")
 BLOCK_SO = os.path.join(CSRC, "libbptblock.so")
+LINEAR_SO = os.path.join(CSRC, "libbptlinear.so")
 OP_SO = os.path.join(CSRC, "bptop.so")
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
@@ -72,6 +74,11 @@ def build_block(verbose=True):
     return BLOCK_SO
 
 
+def build_linear(verbose=True):
+    _run([HIPCC] + HIP_FLAGS + [os.path.join(CSRC, "bptlinear.hip"), "-o", LINEAR_SO], verbose)
+    return LINEAR_SO
+
+
 def build_op(verbose=True):
     """After the HIP libraries, which it links (found beside it at run time)."""
     import sysconfig
@@ -82,8 +89,8 @@ def build_op(verbose=True):
     libs = os.path.join(os.path.dirname(torch.__file__), "lib")
     _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-DTORCH_EXTENSION_NAME=bptop",
           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM"]
-         + [f"-I{p}" for p in include] + [os.path.join(CSRC, "bptop.cpp"), os.path.join(CSRC, "bptblockop.cpp"), "-o", OP_SO, f"-L{libs}", f"-L{CSRC}",
-                                          "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python", "-ltorch", "-l:libbptattn.so", "-l:libbptplan.so", "-l:libbptscore.so", "-l:libbptblock.so", "-Wl,-rpath,$ORIGIN"], verbose)
+         + [f"-I{p}" for p in include] + [os.path.join(CSRC, "bptop.cpp"), os.path.join(CSRC, "bptblockop.cpp"), os.path.join(CSRC, "bptlinearop.cpp"), "-o", OP_SO, f"-L{libs}", f"-L{CSRC}",
+                                          "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python", "-ltorch", "-l:libbptattn.so", "-l:libbptplan.so", "-l:libbptscore.so", "-l:libbptblock.so", "-l:libbptlinear.so", "-Wl,-rpath,$ORIGIN"], verbose)
     return OP_SO
 
 
@@ -91,7 +98,7 @@ def build_all(verbose=True):
     """The HIP compilations take most of the time and run side by side."""
     from concurrent.futures import ThreadPoolExecutor
     with ThreadPoolExecutor(2) as pool:
-        others = pool.map(lambda build: build(verbose), (build_plan, build_score, build_block))
+        others = pool.map(lambda build: build(verbose), (build_plan, build_score, build_block, build_linear))
         graph, attn = build_graph(verbose), build_attn(verbose)
         return (graph, attn, *others, build_op(verbose))
 

@@ -1,54 +1,10 @@
 // The host side of the operators of a transformer block around its attention (include/bptblock.h), part of bptop.so: checks,
 // allocation, launches and autograd without the interpreter.  They have no plans: a call is checked and launched, nothing is kept.
-#include <torch/extension.h>
+#include "bpthost.h"
 
-#include <c10/core/DeviceGuard.h>
-#include <c10/hip/HIPStream.h>
-
-#include <optional>
-#include <tuple>
-
-#include "../../include/bptattn.h"
 #include "../../include/bptblock.h"
 
-namespace py = pybind11;
-using at::Tensor;
-using torch::autograd::AutogradContext;
-using torch::autograd::variable_list;
-
 namespace {
-
-using Optional = std::optional<Tensor>;
-
-void *stream_of(const Tensor &t) { return (void *)c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
-
-void check_status(int st, const char *what) { TORCH_CHECK(st == BPT_OK, what, ": ", bpt_strerror(st), " (status ", st, ")"); }
-
-void check_input(const Tensor &t, const char *name) {
-    TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
-    TORCH_CHECK(t.layout() == at::kStrided && t.is_contiguous(), name, " must be contiguous");
-}
-void check_like(const Tensor &t, const Tensor &x, const char *name) {
-    check_input(t, name);
-    TORCH_CHECK(t.scalar_type() == x.scalar_type(), "all floating point arguments must share one dtype");
-    TORCH_CHECK_VALUE(t.device() == x.device(), "all tensors of a call must be on one device");
-}
-void check_shape(const Tensor &t, at::IntArrayRef shape, const char *name) {
-    TORCH_CHECK_VALUE(t.sizes() == shape, name, " must have shape ", shape, ", got ", t.sizes());
-}
-
-int dtype_code(const Tensor &t) {
-    const auto s = t.scalar_type();
-    return s == at::kFloat ? BPT_F32 : s == at::kBFloat16 ? BPT_BF16 : s == at::kDouble ? BPT_F64 : -1;
-}
-
-bool differentiated(std::initializer_list<const Tensor *> tensors) {
-    for (const Tensor *t : tensors)
-        if (t->defined() && ((at::GradMode::is_enabled() && t->requires_grad()) || t->_fw_grad(/*level=*/0).defined())) return true;
-    return false;
-}
-
-void *ptr(const Tensor &t) { return t.defined() && t.numel() ? t.data_ptr() : nullptr; }
 
 // ---- layer norm of a sum ------------------------------------------------------------------------------------------------------
 void check_norm(const Tensor &x, const Tensor &r, const Tensor &w, const Tensor &b, double eps) {

@@ -1,0 +1,769 @@
+// libbptlinear: gfx950 kernels of matrix products with an epilogue and of dropout from a counter-based generator (C ABI in include/bptlinear.h).
+#include "bpttiles.h"
+
+#include "../../include/bptlinear.h"
+
+namespace {
+
+// ---- elements ------------------------------------------------------------------------------------------------------------------
+typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
+typedef uint32_t uintx4_on4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t uintx4_on2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t uintx2v __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short shortx4 __attribute__((ext_vector_type(4)));
+template <typename T> struct Raw { typedef uint32_t type; typedef uintx4_on4 vec; };
+template <> struct Raw<bf16_t> { typedef uint16_t type; typedef uintx4_on2 vec; };
+
+template <typename T> constexpr int ve() { return 16 / (int)sizeof(T); }       // elements of 16 bytes
+
+// four neighbouring elements, on a multiple of their size
+__device__ __forceinline__ floatx4 load4(const float *p) { return *reinterpret_cast<const floatx4 *>(p); }
+__device__ __forceinline__ floatx4 load4(const bf16_t *p) {
+    const uintx2v w = *reinterpret_cast<const uintx2v *>(p);
+    return floatx4{__uint_as_float(w[0] << 16), __uint_as_float(w[0] & 0xffff0000u), __uint_as_float(w[1] << 16), __uint_as_float(w[1] & 0xffff0000u)};
+}
+__device__ __forceinline__ void store4(float *p, floatx4 v) { *reinterpret_cast<floatx4 *>(p) = v; }
+__device__ __forceinline__ void store4(bf16_t *p, floatx4 v) { *reinterpret_cast<uintx2v *>(p) = uintx2v{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])}; }
+
+// ---- Philox-4x32-10 --------------------------------------------------------------------------------------------------------------
+// A word an element, four elements a counter.  Ten rounds are twenty 64-bit products a counter, a quarter of the vector units' rate each.
+struct Drop {
+    uint32_t thr, k0, k1;        // thr 0: nothing is dropped
+    float inv;
+};
+inline Drop make_drop(double p, uint64_t seed) {
+    if (!(p > 0.0)) return Drop{0u, 0u, 0u, 1.f};
+    const double t = p * 4294967296.0;
+    return Drop{(uint32_t)(t >= 4294967295.0 ? 4294967295.0 : t < 1.0 ? 1.0 : t), (uint32_t)seed, (uint32_t)(seed >> 32), (float)(1.0 / (1.0 - p))};
+}
+__device__ __forceinline__ uintx4 philox(uint64_t counter, uint32_t k0, uint32_t k1) {
+    uint32_t c0 = (uint32_t)counter, c1 = (uint32_t)(counter >> 32), c2 = 0u, c3 = 0u;
+#pragma unroll
+    for (int r = 0; r < 10; ++r) {
+        const uint64_t p = (uint64_t)c0 * 0xD2511F53u, q = (uint64_t)c2 * 0xCD9E8D57u;
+        c0 = (uint32_t)(q >> 32) ^ c1 ^ k0;
+        c1 = (uint32_t)q;
+        c2 = (uint32_t)(p >> 32) ^ c3 ^ k1;
+        c3 = (uint32_t)p;
+        k0 += 0x9E3779B9u;
+        k1 += 0xBB67AE85u;
+    }
+    return uintx4{c0, c1, c2, c3};
+}
+// the words of elements at .. at + 3: those of one counter, or of two where at is no multiple of 4
+__device__ __forceinline__ uintx4 drop_words(uint64_t at, const Drop &d) {
+    const uintx4 a = philox(at >> 2, d.k0, d.k1);
+    const int s = (int)at & 3;
+    if (s == 0) return a;
+    const uintx4 b = philox((at >> 2) + 1, d.k0, d.k1);
+    return s == 1 ? uintx4{a[1], a[2], a[3], b[0]} : s == 2 ? uintx4{a[2], a[3], b[0], b[1]} : uintx4{a[3], b[0], b[1], b[2]};
+}
+// (a choice, not a product: a dropped infinity is 0)
+__device__ __forceinline__ floatx4 dropped(floatx4 v, uintx4 words, const Drop &d) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = words[e] >= d.thr ? v[e] * d.inv : 0.f;
+    return v;
+}
+
+// ---- activations -------------------------------------------------------------------------------------------------------------------
+// (erfc keeps its digits where a is far below zero, 1 + erf does not)
+__device__ __forceinline__ float normal_cdf(float a) { return 0.5f * erfcf(a * -0.70710678118654752f); }
+__device__ __forceinline__ float activated(float a, int act) {
+    if (act == BPT_ACT_RELU) return a <= 0.f ? 0.f : a;           // (NaN stays)
+    if (act == BPT_ACT_GELU) return a * normal_cdf(a);
+    return a;
+}
+// g act'(a)
+__device__ __forceinline__ float activated_back(float g, float a, int act) {
+    if (act == BPT_ACT_RELU) return a <= 0.f ? 0.f : g;
+    if (act == BPT_ACT_GELU) return g * (normal_cdf(a) + a * expf(-0.5f * a * a) * 0.39894228040143268f);
+    return g;
+}
+
+// What follows a product: four neighbouring columns of a row at a time.
+template <typename T> struct Epilogue {
+    const T *bias, *residual;
+    T *y, *kept;
+    int64_t cols;
+    int act;
+    Drop drop;
+    bool quads;                  // rows, and with them quads, start on four elements everywhere
+    __device__ __forceinline__ void operator()(floatx4 v, int64_t row, int64_t col) const {
+        const int64_t at = row * cols + col;
+        if (quads) {
+            if (bias) v += load4(bias + col);
+            if (kept) store4(kept + at, v);
+            if (act != BPT_ACT_NONE) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = activated(v[e], act);
+            }
+            if (drop.thr) v = dropped(v, philox((uint64_t)at >> 2, drop.k0, drop.k1), drop);
+            if (residual) v += load4(residual + at);
+            store4(y + at, v);
+            return;
+        }
+        uintx4 words{0u, 0u, 0u, 0u};
+        if (drop.thr) words = drop_words((uint64_t)at, drop);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (col + e >= cols) break;
+            float x = v[e];
+            if (bias) x += Elem<T>::ld(bias + col + e);
+            if (kept) Elem<T>::st(kept + at + e, x);
+            x = activated(x, act);
+            if (drop.thr) x = words[e] >= drop.thr ? x * drop.inv : 0.f;
+            if (residual) x += Elem<T>::ld(residual + at + e);
+            Elem<T>::st(y + at + e, x);
+        }
+    }
+};
+
+// ---- products on tiles ----------------------------------------------------------------------------------------------------------
+// out[q][p] = sum over r of B(q, r) A(p, r), P columns next to each other in memory.  The three products of a layer:
+//   forward  A = weight (p, r) by rows,       B = x (q, r) by rows
+//   dx       A = weight, (r, p) in memory,    B = g by rows
+//   dweight  A = x, (r, p) in memory,         B = g, (r, q) in memory
+// A workgroup of four wavefronts owns a tile of TB x TB; the reduction goes through LDS 128 bytes a row at a time (32 float32, 64 bfloat16), two
+// buffers, the next one's 16-byte loads straight into LDS while this one is multiplied.  Fragments are 16 rows x 16 bytes a lane: one
+// 16x16x32 product in bfloat16, four 16x16x4 in float32, whose reduction indices (4 g + j for lane group g and product j) only have to agree
+// between the operands.  A is the matrix instructions' first operand, so a lane ends with four neighbouring columns of a row.
+// An operand by rows lies in LDS as rows of eight 16-byte chunks, chunk c at c ^ (row & 7): the sixteen rows that a fragment reads at one chunk
+// spread over the banks.  One that has the reduction outside lies as rows of TB elements; float32 fragments are read word by word, bfloat16
+// ones by transposing loads (lane i of sixteen gives the address of 4 columns of row i / 4 and gets column i of four rows), and chunks are
+// shifted by row so that the four lane groups meet different banks.
+// What does not start on 16 bytes, and the last piece of a ragged reduction, goes through registers, where what lies outside is made zero.
+template <typename T> constexpr int step() { return 128 / (int)sizeof(T); }     // the reduction's share of one buffer
+
+template <typename T, int TB> __device__ __forceinline__ int cols_shift(int r) {
+    constexpr int CHUNKS = TB * (int)sizeof(T) / 16;
+    if constexpr (sizeof(T) == 4) return ((r >> 2 & 3) << 2) & (CHUNKS - 1);
+    return (((r & 3) | (r >> 3 & 1) << 2) << 1) & (CHUNKS - 1);
+}
+
+// VE elements of a line from p on, of which `n` exist (the others: zero)
+template <typename T> __device__ __forceinline__ uintx4 load_upto(const T *p, int64_t n) {
+    typedef typename Raw<T>::type raw;
+    if (n >= ve<T>()) return *reinterpret_cast<const typename Raw<T>::vec *>(p);
+    uint64_t half[2] = {0, 0};
+#pragma unroll 1
+    for (int e = 0; e < (int)n; ++e) {
+        const int bit = e * 8 * (int)sizeof(T);
+        const uint64_t x = (uint64_t) reinterpret_cast<const raw *>(p)[e] << (bit & 63);
+        half[0] |= bit < 64 ? x : 0;
+        half[1] |= bit < 64 ? 0 : x;
+    }
+    return uintx4{(uint32_t)half[0], (uint32_t)(half[0] >> 32), (uint32_t)half[1], (uint32_t)(half[1] >> 32)};
+}
+
+// one operand's way from memory to LDS
+template <typename T, int TB, bool COLS> struct Stage {
+    static constexpr int N = TB * 8 / BLOCK, VE = ve<T>(), CHUNKS = COLS ? TB * (int)sizeof(T) / 16 : 8;
+    const T *base;               // of this tile's first row (column) and the first step
+    int64_t ld, stride;          // elements of a row in memory; from step to step
+    int left, reduce;            // rows (columns) from base on; the reduction's length from base on
+    uint32_t off[N];             // bytes from base, of a lane's vectors where they are whole
+
+    static __device__ __forceinline__ int slot(int i) { return (i * WAVES_PER_BLOCK + (int)(threadIdx.x >> 6)) * WAVE + (int)(threadIdx.x & 63); }
+    static __device__ __forceinline__ int line(int i) { return slot(i) / CHUNKS; }
+    static __device__ __forceinline__ int first(int i) {           // first element of the vector within its line
+        const int l = line(i);
+        return ((slot(i) % CHUNKS) ^ (COLS ? cols_shift<T, TB>(l) : l & 7)) * VE;
+    }
+    // (a stage starts at step s of the reduction and tile row / column t)
+    __device__ __forceinline__ Stage(const T *p, int64_t ld_, int64_t n, int64_t reduce_, int64_t t, int64_t s) : ld(ld_) {
+        const int64_t r0 = s * step<T>();
+        base = COLS ? p + r0 * ld + t : p + t * ld + r0;
+        stride = COLS ? ld * step<T>() : step<T>();
+        left = (int)(n - t < TB ? n - t : TB);
+        reduce = (int)(reduce_ - r0);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            // (past the end: the last row, the last vector of a row; nothing of them is stored)
+            const int l = COLS ? line(i) : min(line(i), left - 1), f = COLS ? min(first(i), left - VE) : first(i);
+            off[i] = (uint32_t)((l * ld + f) * (int64_t)sizeof(T));
+        }
+    }
+    __device__ __forceinline__ void direct(int s, char *lds) const {
+        const char *const at = reinterpret_cast<const char *>(base + s * stride);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(at + off[i]),
+                                             (__attribute__((address_space(3))) void *)(lds + (i * WAVES_PER_BLOCK + (int)(threadIdx.x >> 6)) * WAVE * 16), 16, 0, 0);
+    }
+    __device__ __forceinline__ void load(int s, uintx4 (&v)[N]) const {
+        const T *const at = base + s * stride;
+        const int rest = reduce - s * step<T>();
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int l = line(i), f = first(i), lines = COLS ? rest : left, cols = COLS ? left : rest;
+            v[i] = l < lines ? load_upto(at + l * ld + f, cols - f) : uintx4{0u, 0u, 0u, 0u};
+        }
+    }
+    __device__ __forceinline__ void store(const uintx4 (&v)[N], char *lds) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) *reinterpret_cast<uintx4 *>(lds + slot(i) * 16) = v[i];
+    }
+};
+
+// the 16 bytes that a lane has of fragment rows from .. from + 15 at half `half` of a buffer
+template <typename T, int TB, bool COLS> __device__ __forceinline__ uintx4 fragment(const char *lds, int from, int half) {
+    const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+    if constexpr (!COLS) {
+        return *reinterpret_cast<const uintx4 *>(lds + (from + c) * 128 + ((half * 4 + g) ^ (c & 7)) * 16);
+    } else if constexpr (sizeof(T) == 4) {
+        uintx4 v;
+        const int r = half * 16 + 4 * g, col = from + c;
+        const char *const p = lds + r * (TB * 4) + (((col >> 2) ^ cols_shift<T, TB>(r)) << 4) + (col & 3) * 4;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const uint32_t *>(p + j * (TB * 4));
+        return v;
+    } else {
+        uintx4 v;
+        const int col = from + (c & 3) * 4;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const int r = half * 32 + 8 * g + 4 * t + (c >> 2);
+            const char *const p = lds + r * (TB * 2) + (((col >> 3) ^ cols_shift<T, TB>(r)) << 4) + (col & 7) * 2;
+            const shortx4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) shortx4 *)const_cast<char *>(p));
+            const uintx2v w = __builtin_bit_cast(uintx2v, x);
+            v[2 * t] = w[0];
+            v[2 * t + 1] = w[1];
+        }
+        return v;
+    }
+}
+template <typename T> __device__ __forceinline__ floatx4 multiply(uintx4 a, uintx4 b, floatx4 c) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[j]), __uint_as_float(b[j]), c, 0, 0, 0);
+        return c;
+    } else {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
+}
+
+struct Product {
+    int64_t P, Q, R;             // columns, rows, reduction
+    int64_t lda, ldb;
+    int tiles_p, tiles, splits;  // tiles of a row of them, of the result; shares of the reduction
+    int steps, per_split;        // steps of the reduction, of a share
+};
+
+// The sums leave through LDS, so that a row of the tile is written (and bias, residual read) as one run of memory.
+// part: null, or (splits, Q, P) sums of the shares, which k_linear_finish adds up
+template <typename T, int TB, bool ACOLS, bool BCOLS, bool DIRECT>
+__global__ __launch_bounds__(BLOCK, TB == 128 ? 2 : 4) void k_linear_tiles(const T *__restrict__ a, const T *__restrict__ b, Product m, Epilogue<T> out,
+                                                                           float *__restrict__ part) {
+    constexpr int WT = TB / 2, F = WT / 16;                        // a wavefront's part of the tile, in fragments
+    __shared__ __attribute__((aligned(16))) char lds[4 * TB * 128];
+    const int id = xcd_contiguous_block(), split = id / m.tiles, tile = id - split * m.tiles;
+    const int64_t q0 = (int64_t)(tile / m.tiles_p) * TB, p0 = (int64_t)(tile % m.tiles_p) * TB;
+    const int s0 = split * m.per_split, n = min(m.per_split, m.steps - s0);
+    const Stage<T, TB, ACOLS> sa(a, m.lda, m.P, m.R, p0, s0);
+    const Stage<T, TB, BCOLS> sb(b, m.ldb, m.Q, m.R, q0, s0);
+    const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, wp = (w & 1) * WT, wq = (w >> 1) * WT;
+    floatx4 acc[F][F];
+#pragma unroll
+    for (int i = 0; i < F; ++i)
+#pragma unroll
+        for (int j = 0; j < F; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+    auto buffer = [&](int s, int operand) { return lds + ((s & 1) * 2 + operand) * (TB * 128); };
+    auto compute = [&](int s) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            uintx4 fa[F], fb[F];
+#pragma unroll
+            for (int i = 0; i < F; ++i) fa[i] = fragment<T, TB, ACOLS>(buffer(s, 0), wp + 16 * i, half);
+#pragma unroll
+            for (int j = 0; j < F; ++j) fb[j] = fragment<T, TB, BCOLS>(buffer(s, 1), wq + 16 * j, half);
+#pragma unroll
+            for (int i = 0; i < F; ++i)
+#pragma unroll
+                for (int j = 0; j < F; ++j) acc[i][j] = multiply<T>(fa[i], fb[j], acc[i][j]);
+        }
+    };
+    int s = 0;
+    if constexpr (DIRECT) {
+        const int whole = min(n, sa.reduce / step<T>());
+        auto ask = [&](int t) {
+            sa.direct(t, buffer(t, 0));
+            sb.direct(t, buffer(t, 1));
+        };
+        if (whole > 0) ask(0);
+        for (; s < whole; ++s) {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");       // (this wavefront's part of step s is in LDS)
+            __syncthreads();                                       // (everyone's is, and what the other buffer held has been read)
+            if (s + 1 < whole) ask(s + 1);
+            compute(s);
+        }
+    }
+    for (; s < n; ++s) {                                           // (the ragged end, or everything)
+        uintx4 va[Stage<T, TB, ACOLS>::N], vb[Stage<T, TB, BCOLS>::N];
+        sa.load(s, va);
+        sb.load(s, vb);
+        sa.store(va, buffer(s, 0));                                // (what it held was read before the last barrier)
+        sb.store(vb, buffer(s, 1));
+        __syncthreads();
+        compute(s);
+    }
+    __syncthreads();
+    // the tile as rows of TB floats, quad i of row q at i ^ q: sixteen rows' quads of a fragment spread over the banks
+    constexpr int QUADS = TB / 4;
+    floatx4 *const sums = reinterpret_cast<floatx4 *>(lds);
+#pragma unroll
+    for (int j = 0; j < F; ++j)
+#pragma unroll
+        for (int i = 0; i < F; ++i) {
+            const int q = wq + 16 * j + (lane & 15), quad = (wp + 16 * i) / 4 + (lane >> 4);
+            sums[q * QUADS + (quad ^ (q & (QUADS - 1)))] = acc[i][j];
+        }
+    __syncthreads();
+    const int64_t left_q = m.Q - q0;
+#pragma unroll 2
+    for (int i = threadIdx.x; i < TB * QUADS; i += BLOCK) {
+        const int q = i / QUADS, quad = i % QUADS;
+        const int64_t p = p0 + quad * 4;
+        if (q >= left_q || p >= m.P) continue;
+        const floatx4 v = sums[q * QUADS + (quad ^ (q & (QUADS - 1)))];
+        if (!part) {
+            out(v, q0 + q, p);
+            continue;
+        }
+        float *const to = part + ((int64_t)split * m.Q + q0 + q) * m.P + p;
+        if ((m.P & 3) == 0) {
+            store4(to, v);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (p + e < m.P) to[e] = v[e];
+        }
+    }
+}
+
+// the shares' sums in their order, and what follows the product
+template <typename T>
+__global__ __launch_bounds__(BLOCK) void k_linear_finish(const float *__restrict__ part, int splits, int64_t rows, int64_t cols, Epilogue<T> out) {
+    const int64_t quads = (cols + 3) / 4, i = (int64_t)blockIdx.x * BLOCK + threadIdx.x;
+    if (i >= rows * quads) return;
+    const int64_t row = i / quads, col = (i - row * quads) * 4, n = rows * cols;
+    const float *const p = part + row * cols + col;
+    floatx4 v{0.f, 0.f, 0.f, 0.f};
+    if ((cols & 3) == 0) {
+        int s = 0;
+        for (; s + 4 <= splits; s += 4) {
+            floatx4 t[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) t[u] = load4(p + (s + u) * n);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) v += t[u];
+        }
+        for (; s < splits; ++s) v += load4(p + s * n);
+    } else {
+        for (int s = 0; s < splits; ++s) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (col + e < cols) v[e] += p[s * n + e];
+        }
+    }
+    out(v, row, col);
+}
+
+// ---- few rows ----------------------------------------------------------------------------------------------------------------------
+// Forward of up to 16 NQ rows: bound by the latency of reading the weight once.  A workgroup has 16 columns and all rows, its wavefronts share the
+// reduction and meet in LDS; fragments come straight from memory, sixteen lanes' rows of 64 bytes each.
+constexpr int FEW_WAVES = 8;
+template <typename T, bool WHOLE> __device__ __forceinline__ uintx4 few_load(const T *row, int64_t k, int64_t R) {
+    if constexpr (WHOLE) {
+        if (k < R) return *reinterpret_cast<const uintx4 *>(row + k);
+        return uintx4{0u, 0u, 0u, 0u};
+    }
+    return k < R ? load_upto(row + k, R - k) : uintx4{0u, 0u, 0u, 0u};
+}
+template <typename T, int NQ, bool WHOLE>
+__global__ __launch_bounds__(FEW_WAVES *WAVE) void k_linear_few(const T *__restrict__ w, const T *__restrict__ x, int64_t P, int64_t Q, int64_t R, Epilogue<T> out) {
+    constexpr int K = 4 * ve<T>();                                 // the reduction's share of a fragment
+    __shared__ floatx4 meet[FEW_WAVES][NQ][WAVE];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+    const int64_t p0 = (int64_t)blockIdx.x * 16, p = p0 + c;
+    const T *const wr = w + (p < P ? p : P - 1) * R;
+    const T *xr[NQ];
+#pragma unroll
+    for (int j = 0; j < NQ; ++j) xr[j] = x + (16 * j + c < Q ? 16 * j + c : Q - 1) * R;
+    floatx4 acc[NQ];
+#pragma unroll
+    for (int j = 0; j < NQ; ++j) acc[j] = floatx4{0.f, 0.f, 0.f, 0.f};
+    constexpr int U = NQ == 1 ? 4 : NQ == 2 ? 4 : 2;
+    for (int64_t k0 = (int64_t)wave * K; k0 < R; k0 += (int64_t)FEW_WAVES * K * U) {
+        uintx4 a[U], b[U][NQ];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t k = k0 + (int64_t)u * FEW_WAVES * K + g * ve<T>();
+            a[u] = few_load<T, WHOLE>(wr, k, R);
+#pragma unroll
+            for (int j = 0; j < NQ; ++j) b[u][j] = few_load<T, WHOLE>(xr[j], k, R);
+        }
+        issue_loads_first();
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int j = 0; j < NQ; ++j) acc[j] = multiply<T>(a[u], b[u][j], acc[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < NQ; ++j) meet[wave][j][lane] = acc[j];
+    __syncthreads();
+    for (int j = wave; j < NQ; j += FEW_WAVES) {
+        floatx4 v = meet[0][j][lane];
+#pragma unroll
+        for (int i = 1; i < FEW_WAVES; ++i) v += meet[i][j][lane];
+        const int64_t q = 16 * j + c, col = p0 + 4 * g;
+        if (q < Q && col < P) out(v, q, col);
+    }
+}
+
+// ---- the gradient before the products ------------------------------------------------------------------------------------------
+// g = dy dropout' act'(a), and the sums of its columns: bound by memory, dy and a read and g written once.  A workgroup has 64 lanes' columns (four each) and
+// every parts-th four rows; its wavefronts meet in LDS, the workgroups in k_linear_sums, in a fixed order.
+template <typename T>
+__global__ __launch_bounds__(BLOCK) void k_linear_grad(const T *dy, const T *__restrict__ kept, int kept_is_result, T *g, float *__restrict__ part, int64_t rows,
+                                                       int64_t cols, int act, Drop drop, bool quads) {
+    __shared__ floatx4 meet[WAVES_PER_BLOCK][WAVE];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int64_t col = ((int64_t)blockIdx.x * WAVE + lane) * 4;
+    constexpr int U = 4;
+    floatx4 sum{0.f, 0.f, 0.f, 0.f};
+    const int64_t stride = (int64_t)gridDim.y * WAVES_PER_BLOCK;
+    for (int64_t row = (int64_t)blockIdx.y * WAVES_PER_BLOCK + wave; row < rows; row += stride * U) {
+        floatx4 v[U], a[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t r = row + u * stride, at = r * cols + col;
+            v[u] = a[u] = floatx4{0.f, 0.f, 0.f, 0.f};
+            if (r >= rows || col >= cols) continue;
+            if (quads) {
+                v[u] = load4(dy + at);
+                if (act != BPT_ACT_NONE) a[u] = load4(kept + at);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (col + e < cols) {
+                        v[u][e] = Elem<T>::ld(dy + at + e);
+                        if (act != BPT_ACT_NONE) a[u][e] = Elem<T>::ld(kept + at + e);
+                    }
+            }
+        }
+        issue_loads_first();
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t r = row + u * stride, at = r * cols + col;
+            if (r >= rows || col >= cols) continue;
+            if (drop.thr) {
+                if (kept_is_result) v[u] *= drop.inv;              // (what was dropped is 0 in the result)
+                else v[u] = dropped(v[u], drop_words((uint64_t)at, drop), drop);
+            }
+            if (act != BPT_ACT_NONE) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[u][e] = activated_back(v[u][e], a[u][e], act);
+            }
+            if (quads) {
+                if (g) store4(g + at, v[u]);
+                sum += v[u];
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (col + e < cols) {
+                        if (g) Elem<T>::st(g + at + e, v[u][e]);
+                        sum[e] += v[u][e];
+                    }
+            }
+        }
+    }
+    if (!part) return;
+    meet[wave][lane] = sum;
+    __syncthreads();
+    if (wave != 0) return;
+#pragma unroll
+    for (int i = 1; i < WAVES_PER_BLOCK; ++i) sum += meet[i][lane];
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (col + e < cols) part[(int64_t)blockIdx.y * cols + col + e] = sum[e];
+}
+// 16 columns a workgroup, sixteen lanes a column take parts p, p + 16, ...; the sixteen are added in their order
+template <typename T> __global__ __launch_bounds__(BLOCK) void k_linear_sums(const float *__restrict__ part, int parts, T *__restrict__ out, int64_t cols) {
+    __shared__ float meet[16][17];
+    const int c = threadIdx.x & 15, k = threadIdx.x >> 4;
+    const int64_t at = (int64_t)blockIdx.x * 16 + c;
+    float v = 0.f;
+    if (at < cols)
+        for (int p = k; p < parts; p += 16) v += part[(int64_t)p * cols + at];
+    meet[k][c] = v;
+    __syncthreads();
+    if (k != 0 || at >= cols) return;
+    v = meet[0][c];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) v += meet[i][c];
+    Elem<T>::st(out + at, v);
+}
+
+// ---- dropout -----------------------------------------------------------------------------------------------------------------------
+// y = residual + dropout(x): bound by memory, the words are formed while the loads are on their way.  A lane has 16 bytes a turn.
+template <typename T, bool AL>
+__global__ __launch_bounds__(BLOCK) void k_dropout(const T *x, const T *residual, T *y, int64_t n, Drop drop) {
+    constexpr int VE = ve<T>(), U = 4;
+    typedef typename Raw<T>::vec loose;
+    const int64_t first = ((int64_t)blockIdx.x * U * BLOCK + threadIdx.x) * VE;
+    auto fetch = [](const T *p) -> uintx4 {
+        if constexpr (AL) return *reinterpret_cast<const uintx4 *>(p);
+        return *reinterpret_cast<const loose *>(p);
+    };
+    auto wide = [](uintx4 v, int h) {
+        if constexpr (sizeof(T) == 4) return __builtin_bit_cast(floatx4, v);
+        return floatx4{__uint_as_float(v[2 * h] << 16), __uint_as_float(v[2 * h] & 0xffff0000u), __uint_as_float(v[2 * h + 1] << 16),
+                       __uint_as_float(v[2 * h + 1] & 0xffff0000u)};
+    };
+    uintx4 vx[U], vr[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int64_t at = first + (int64_t)u * BLOCK * VE;
+        if (at + VE > n) continue;
+        vx[u] = fetch(x + at);
+        if (residual) vr[u] = fetch(residual + at);
+    }
+    issue_loads_first();
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int64_t at = first + (int64_t)u * BLOCK * VE;
+        if (at + VE <= n) {
+            uintx4 o;
+#pragma unroll
+            for (int h = 0; h < VE / 4; ++h) {
+                floatx4 v = dropped(wide(vx[u], h), philox((uint64_t)(at >> 2) + h, drop.k0, drop.k1), drop);
+                if (residual) v += wide(vr[u], h);
+                if constexpr (sizeof(T) == 4) {
+                    o = __builtin_bit_cast(uintx4, v);
+                } else {
+                    o[2 * h] = pack_bf16(v[0], v[1]);
+                    o[2 * h + 1] = pack_bf16(v[2], v[3]);
+                }
+            }
+            if constexpr (AL) *reinterpret_cast<uintx4 *>(y + at) = o;
+            else *reinterpret_cast<loose *>(y + at) = o;
+        } else if (at < n) {
+#pragma unroll
+            for (int h = 0; h < VE / 4; ++h) {
+                const uintx4 words = philox((uint64_t)(at >> 2) + h, drop.k0, drop.k1);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int64_t i = at + 4 * h + e;
+                    if (i >= n) continue;
+                    float v = words[e] >= drop.thr ? Elem<T>::ld(x + i) * drop.inv : 0.f;
+                    if (residual) v += Elem<T>::ld(residual + i);
+                    Elem<T>::st(y + i, v);
+                }
+            }
+        }
+    }
+}
+
+// ---- launchers -------------------------------------------------------------------------------------------------------------------
+inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+inline bool on(std::initializer_list<const void *> ps, uintptr_t bytes) {
+    for (const void *p : ps)
+        if ((uintptr_t)p % bytes) return false;
+    return true;
+}
+
+// Which tiles, and into how many shares the reduction goes.
+struct Choice { int tb, splits; };
+inline Choice choose(int64_t P, int64_t Q, int64_t R, int step) {
+    const int64_t steps = ceil_div(R, step), big = ceil_div(P, 128) * ceil_div(Q, 128), small = ceil_div(P, 64) * ceil_div(Q, 64);
+    if (big >= 256) return Choice{128, 1};
+    if (steps >= 64) return Choice{128, (int)std::min<int64_t>(steps / 16, ceil_div(512, big))};
+    if (small >= 256 || steps < 8) return Choice{64, 1};
+    return Choice{64, (int)std::min<int64_t>(steps / 4, ceil_div(512, small))};
+}
+template <typename T> inline Product product(int64_t P, int64_t Q, int64_t R, int64_t lda, int64_t ldb, Choice &ch) {
+    ch = choose(P, Q, R, step<T>());
+    Product m{P, Q, R, lda, ldb, 0, 0, 0, 0, 0};
+    m.tiles_p = (int)ceil_div(P, ch.tb);
+    m.tiles = (int)(m.tiles_p * ceil_div(Q, ch.tb));
+    m.steps = (int)ceil_div(R, step<T>());
+    m.per_split = (int)ceil_div(m.steps, ch.splits);
+    m.splits = (int)ceil_div(m.steps, m.per_split);
+    return m;
+}
+template <typename T> inline int64_t product_workspace(int64_t P, int64_t Q, int64_t R) {
+    Choice ch;
+    const Product m = product<T>(P, Q, R, 0, 0, ch);
+    return m.splits > 1 ? (int64_t)m.splits * P * Q * 4 : 0;
+}
+
+template <typename T, int TB, bool AC, bool BC> int launch_tiles(const T *a, const T *b, const Product &m, const Epilogue<T> &out, float *part, hipStream_t s) {
+    // (a lane's offsets into a step count 32 bits: 128 rows of 2^22 elements)
+    const bool direct = on({a, b}, 16) && m.lda % ve<T>() == 0 && m.ldb % ve<T>() == 0 && std::max(m.lda, m.ldb) <= (int64_t)1 << 22;
+    const dim3 grid((unsigned)(m.tiles * (int64_t)m.splits));
+    if (direct) hipLaunchKernelGGL((k_linear_tiles<T, TB, AC, BC, true>), grid, dim3(BLOCK), 0, s, a, b, m, out, part);
+    else hipLaunchKernelGGL((k_linear_tiles<T, TB, AC, BC, false>), grid, dim3(BLOCK), 0, s, a, b, m, out, part);
+    return launch_status();
+}
+// out's rows and columns are the product's
+template <typename T, bool AC, bool BC>
+int run_product(const T *a, const T *b, int64_t P, int64_t Q, int64_t R, int64_t lda, int64_t ldb, const Epilogue<T> &out, void *ws, hipStream_t s) {
+    Choice ch;
+    const Product m = product<T>(P, Q, R, lda, ldb, ch);
+    float *const part = m.splits > 1 ? (float *)ws : nullptr;
+    const int st = ch.tb == 128 ? launch_tiles<T, 128, AC, BC>(a, b, m, out, part, s) : launch_tiles<T, 64, AC, BC>(a, b, m, out, part, s);
+    if (st != BPT_OK || !part) return st;
+    hipLaunchKernelGGL((k_linear_finish<T>), dim3((unsigned)ceil_div(Q * ceil_div(P, 4), BLOCK)), dim3(BLOCK), 0, s, part, m.splits, Q, P, out);
+    return launch_status();
+}
+template <typename T> inline Epilogue<T> plain_epilogue(T *y, int64_t cols) {
+    return Epilogue<T>{nullptr, nullptr, y, nullptr, cols, BPT_ACT_NONE, make_drop(0.0, 0), cols % 4 == 0 && on({y}, 4 * sizeof(T))};
+}
+
+constexpr int64_t FEW_ROWS = 64;
+template <typename T>
+int run_forward(const void *x_, const void *w_, const void *b_, const void *r_, void *y_, void *kept_, void *ws, int64_t rows, int64_t inner, int64_t outer, int act,
+                Drop drop, hipStream_t s) {
+    const T *x = (const T *)x_, *w = (const T *)w_;
+    const Epilogue<T> out{(const T *)b_, (const T *)r_, (T *)y_, (T *)kept_, outer, act, drop, outer % 4 == 0 && on({b_, r_, y_, kept_}, 4 * sizeof(T))};
+    if (rows <= FEW_ROWS) {
+        const bool whole = inner % ve<T>() == 0 && on({x, w}, 16);
+        const dim3 grid((unsigned)ceil_div(outer, 16)), block(FEW_WAVES * WAVE);
+#define LAUNCH(NQ) \
+    if (whole) hipLaunchKernelGGL((k_linear_few<T, NQ, true>), grid, block, 0, s, w, x, outer, rows, inner, out); \
+    else hipLaunchKernelGGL((k_linear_few<T, NQ, false>), grid, block, 0, s, w, x, outer, rows, inner, out)
+        if (rows <= 16) { LAUNCH(1); }
+        else if (rows <= 32) { LAUNCH(2); }
+        else { LAUNCH(4); }
+#undef LAUNCH
+        return launch_status();
+    }
+    return run_product<T, false, false>(w, x, outer, rows, inner, inner, inner, out, ws, s);
+}
+
+// workgroups that share the rows of one strip of 256 columns
+inline int grad_parts(int64_t rows, int64_t cols) {
+    const int64_t strips = ceil_div(cols, 4 * WAVE);
+    return (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(rows, 4 * WAVES_PER_BLOCK), ceil_div(2048, strips)));
+}
+template <typename T>
+int run_grad(const void *dy_, const void *kept_, int result, void *g_, void *db_, void *ws, int64_t rows, int64_t cols, int act, Drop drop, hipStream_t s) {
+    const int parts = grad_parts(rows, cols);
+    const bool quads = cols % 4 == 0 && on({dy_, act != BPT_ACT_NONE ? kept_ : nullptr, g_}, 4 * sizeof(T));
+    float *const part = db_ ? (float *)ws : nullptr;
+    if (rows > 0)
+        hipLaunchKernelGGL((k_linear_grad<T>), dim3((unsigned)ceil_div(cols, 4 * WAVE), parts), dim3(BLOCK), 0, s, (const T *)dy_, (const T *)kept_, result, (T *)g_, part,
+                           rows, cols, act, drop, quads);
+    const int st = launch_status();
+    if (st != BPT_OK || !db_) return st;
+    hipLaunchKernelGGL((k_linear_sums<T>), dim3((unsigned)ceil_div(cols, 16)), dim3(BLOCK), 0, s, part, rows > 0 ? parts : 0, (T *)db_, cols);
+    return launch_status();
+}
+
+template <typename T> int run_dropout(const void *x, const void *r, void *y, int64_t n, Drop drop, hipStream_t s) {
+    const dim3 grid((unsigned)ceil_div(n, (int64_t)BLOCK * 4 * ve<T>()));
+    if (on({x, r, y}, 16)) hipLaunchKernelGGL((k_dropout<T, true>), grid, dim3(BLOCK), 0, s, (const T *)x, (const T *)r, (T *)y, n, drop);
+    else hipLaunchKernelGGL((k_dropout<T, false>), grid, dim3(BLOCK), 0, s, (const T *)x, (const T *)r, (T *)y, n, drop);
+    return launch_status();
+}
+
+inline bool is_type(int dtype) { return dtype == BPT_F32 || dtype == BPT_BF16; }
+inline bool is_share(double p) { return p >= 0.0 && p < 1.0; }
+// (grids count tiles, quads and rows in 31 bits)
+inline bool is_size(int64_t rows, int64_t inner, int64_t outer) {
+    const int64_t most = (int64_t)1 << 28;
+    if (rows < 0 || inner < 1 || outer < 0 || rows > most || inner > most || outer > most) return false;
+    const double cells = 1.0 * ((int64_t)1 << 38);
+    return (double)rows * outer <= cells && (double)rows * inner <= cells && (double)inner * outer <= cells;
+}
+
+}  // namespace
+
+extern "C" {
+
+#define FOR_TYPE(call) (dtype == BPT_F32 ? call<float> : call<bf16_t>)
+
+int64_t bpt_linear_forward_workspace_bytes(int64_t rows, int64_t inner, int64_t outer, int dtype) {
+    if (!is_type(dtype) || !is_size(rows, inner, outer)) return -1;
+    if (rows <= FEW_ROWS || outer == 0) return 0;
+    return FOR_TYPE(product_workspace)(outer, rows, inner);
+}
+
+int bpt_linear_forward(const void *x, const void *weight, const void *bias, const void *residual, void *y, void *kept, void *workspace, int64_t workspace_bytes,
+                       int64_t rows, int64_t inner, int64_t outer, int act, double dropout_p, uint64_t seed, int dtype, void *stream) {
+    if (!is_type(dtype)) return BPT_ERR_DTYPE;
+    if (!is_size(rows, inner, outer) || !is_share(dropout_p)) return BPT_ERR_SIZE;
+    if (act < BPT_ACT_NONE || act > BPT_ACT_GELU) return BPT_ERR_UNSUPPORTED;
+    if (rows == 0 || outer == 0) return BPT_OK;
+    if (!x || !weight || !y) return BPT_ERR_NULL;
+    const int64_t need = bpt_linear_forward_workspace_bytes(rows, inner, outer, dtype);
+    if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace))) return BPT_ERR_WORKSPACE;
+    return FOR_TYPE(run_forward)(x, weight, bias, residual, y, kept, workspace, rows, inner, outer, act, make_drop(dropout_p, seed), (hipStream_t)stream);
+}
+
+int64_t bpt_linear_grad_workspace_bytes(int64_t rows, int64_t outer, int dtype) {
+    if (!is_type(dtype) || !is_size(rows, 1, outer)) return -1;
+    return outer == 0 ? 0 : (int64_t)grad_parts(rows, outer) * outer * 4;
+}
+
+int bpt_linear_grad(const void *dy, const void *kept, int kept_is_result, void *g, void *dbias, void *workspace, int64_t workspace_bytes, int64_t rows, int64_t outer,
+                    int act, double dropout_p, uint64_t seed, int dtype, void *stream) {
+    if (!is_type(dtype)) return BPT_ERR_DTYPE;
+    if (!is_size(rows, 1, outer) || !is_share(dropout_p)) return BPT_ERR_SIZE;
+    if (act < BPT_ACT_NONE || act > BPT_ACT_GELU || (kept_is_result && act != BPT_ACT_RELU)) return BPT_ERR_UNSUPPORTED;
+    if (outer == 0 || (!g && !dbias) || (rows == 0 && !dbias)) return BPT_OK;
+    if (rows > 0 && (!dy || (act != BPT_ACT_NONE && !kept))) return BPT_ERR_NULL;
+    if (dbias && (!workspace || workspace_bytes < bpt_linear_grad_workspace_bytes(rows, outer, dtype) || !aligned16(workspace))) return BPT_ERR_WORKSPACE;
+    return FOR_TYPE(run_grad)(dy, kept, kept_is_result, g, dbias, workspace, rows, outer, act, make_drop(dropout_p, seed), (hipStream_t)stream);
+}
+
+int64_t bpt_linear_input_grad_workspace_bytes(int64_t rows, int64_t inner, int64_t outer, int dtype) {
+    if (!is_type(dtype) || !is_size(rows, inner, outer) || outer < 1) return -1;
+    return rows == 0 ? 0 : FOR_TYPE(product_workspace)(inner, rows, outer);
+}
+
+int bpt_linear_input_grad(const void *g, const void *weight, void *dx, void *workspace, int64_t workspace_bytes, int64_t rows, int64_t inner, int64_t outer, int dtype,
+                          void *stream) {
+    if (!is_type(dtype)) return BPT_ERR_DTYPE;
+    if (!is_size(rows, inner, outer) || outer < 1) return BPT_ERR_SIZE;
+    if (rows == 0) return BPT_OK;
+    if (!g || !weight || !dx) return BPT_ERR_NULL;
+    const int64_t need = bpt_linear_input_grad_workspace_bytes(rows, inner, outer, dtype);
+    if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace))) return BPT_ERR_WORKSPACE;
+    hipStream_t s = (hipStream_t)stream;
+    if (dtype == BPT_F32)
+        return run_product<float, true, false>((const float *)weight, (const float *)g, inner, rows, outer, inner, outer, plain_epilogue((float *)dx, inner), workspace, s);
+    return run_product<bf16_t, true, false>((const bf16_t *)weight, (const bf16_t *)g, inner, rows, outer, inner, outer, plain_epilogue((bf16_t *)dx, inner), workspace, s);
+}
+
+int64_t bpt_linear_weight_grad_workspace_bytes(int64_t rows, int64_t inner, int64_t outer, int dtype) {
+    if (!is_type(dtype) || !is_size(rows, inner, outer) || rows < 1) return -1;
+    return outer == 0 ? 0 : FOR_TYPE(product_workspace)(inner, outer, rows);
+}
+
+int bpt_linear_weight_grad(const void *g, const void *x, void *dweight, void *workspace, int64_t workspace_bytes, int64_t rows, int64_t inner, int64_t outer, int dtype,
+                           void *stream) {
+    if (!is_type(dtype)) return BPT_ERR_DTYPE;
+    if (!is_size(rows, inner, outer) || rows < 1) return BPT_ERR_SIZE;
+    if (outer == 0) return BPT_OK;
+    if (!g || !x || !dweight) return BPT_ERR_NULL;
+    const int64_t need = bpt_linear_weight_grad_workspace_bytes(rows, inner, outer, dtype);
+    if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace))) return BPT_ERR_WORKSPACE;
+    hipStream_t s = (hipStream_t)stream;
+    if (dtype == BPT_F32)
+        return run_product<float, true, true>((const float *)x, (const float *)g, inner, outer, rows, inner, outer, plain_epilogue((float *)dweight, inner), workspace, s);
+    return run_product<bf16_t, true, true>((const bf16_t *)x, (const bf16_t *)g, inner, outer, rows, inner, outer, plain_epilogue((bf16_t *)dweight, inner), workspace, s);
+}
+
+int bpt_dropout(const void *x, const void *residual, void *y, int64_t n, double dropout_p, uint64_t seed, int dtype, void *stream) {
+    if (!is_type(dtype)) return BPT_ERR_DTYPE;
+    if (n < 0 || n > (int64_t)1 << 40 || !is_share(dropout_p)) return BPT_ERR_SIZE;
+    if (n == 0) return BPT_OK;
+    if (!x || !y) return BPT_ERR_NULL;
+    return FOR_TYPE(run_dropout)(x, residual, y, n, make_drop(dropout_p, seed), (hipStream_t)stream);
+}
+
+#undef FOR_TYPE
+
+}  // extern "C"

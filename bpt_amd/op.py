@@ -14,7 +14,7 @@ from .graphop import (maskedmm_csr_backward, maskedmm_csr_forward, node_mul_edge
 
 __all__ = ["SparseSoftmax", "MaskedMMCSR", "NodeMulEdge", "VectorSPMM", "BPTAttention", "BPTScoreAttention", "EdgeTypeEmbedding",
            "sparse_softmax", "masked_mm", "node_mul_edge", "vec_spmm", "bpt_attention", "edge_type_embedding",
-           "add_layer_norm", "relu_linear8"]
+           "add_layer_norm", "relu_linear8", "linear_act", "dropout"]
 
 
 class SparseSoftmax(Function):
@@ -603,3 +603,33 @@ def relu_linear8(a, weight, bias=None, dropout_p=0.0, seed=None):
     if dropout_p > 0 and seed is None:
         seed = int(torch.randint(0, 2 ** 62, (1,)).item())
     return _native.relu_linear8(a, weight, bias, float(dropout_p), int(seed or 0) & (2 ** 64 - 1))
+
+
+_ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2}
+
+
+def linear_act(x, weight, bias=None, activation=None, residual=None, dropout_p=0.0, seed=None):
+    """residual + dropout(act(x weight^T + bias)) in one pass: a projection or one half of a feed-forward with what a block does behind it
+    (modules/attention.py:18-19, :79, :81).  x (..., inner), weight (outer, inner), bias (outer,) or None, residual (..., outer) or None, contiguous,
+    float32 or bfloat16, all of one type; activation None, "relu" or "gelu" (a (1 + erf(a / sqrt 2)) / 2).  Sums, bias, activation, dropout and
+    the residual sum are held in 32 bits and the result is rounded once.  dropout_p > 0 drops by (seed, index) as `dropout` does, the mask is
+    formed again in the backward; seed=None draws one from torch's CPU generator, as bpt_attention does (a captured call drops the same elements
+    at every replay).  For the backward it keeps x, weight and, with an activation, one tensor like the result: relu's own, where no
+    residual is added to it.  Deterministic; not differentiable twice."""
+    _no_transforms("linear_act")
+    if activation not in _ACTIVATIONS:
+        raise ValueError('activation must be None, "relu" or "gelu"')
+    if dropout_p > 0 and seed is None:
+        seed = int(torch.randint(0, 2 ** 62, (1,)).item())
+    return _native.linear_act(x, weight, bias, residual, _ACTIVATIONS[activation], float(dropout_p), int(seed or 0) & (2 ** 64 - 1))
+
+
+def dropout(x, dropout_p, seed=None, residual=None):
+    """residual + x with a share dropout_p of its elements 0 and the others divided by 1 - dropout_p; residual like x or None.  Element i (its place in
+    memory) is dropped where word i % 4 of Philox-4x32-10 (Salmon et al. 2011) of the counter (i // 4, 0) under the key seed lies below
+    dropout_p 2^32: nothing is stored, the backward forms the words again.  seed=None draws one from torch's CPU generator.  float32 or bfloat16,
+    contiguous; the sum is held in 32 bits.  In evaluation pass dropout_p=0."""
+    _no_transforms("dropout")
+    if dropout_p > 0 and seed is None:
+        seed = int(torch.randint(0, 2 ** 62, (1,)).item())
+    return _native.dropout(x, residual, float(dropout_p), int(seed or 0) & (2 ** 64 - 1))

@@ -5,6 +5,7 @@
   bpt_amd/csrc/libbptscore.so  gfx950 HIP (hipcc)        <- bptscore.hip, bpttiles.h  (attention with capped scores and distance)
   bpt_amd/csrc/libbptblock.so  gfx950 HIP (hipcc)        <- bptblock.hip, bpttiles.h  (layer norm of a sum, relu kept in 8 bits)
   bpt_amd/csrc/libbptlinear.so gfx950 HIP (hipcc)       <- bptlinear.hip, bpttiles.h  (matrix products with an epilogue, dropout)
+  bpt_amd/csrc/libbptbias.so   gfx950 HIP (hipcc)        <- bptbias.hip, bpttiles.h  (bias of scores by buckets)
   bpt_amd/csrc/libbptplan.so   gfx950 HIP (hipcc)        <- bptplan.hip  (plans built on the GPU; rocPRIM headers)
   bpt_amd/csrc/bptop.so        host C++ (g++, torch)     <- bptop.cpp, bptblockop.cpp, bptlinearop.cpp, bpthost.h  (host side of the ops and their autograd; links them)
 
@@ -21,6 +22,7 @@ PLAN_SO = os.path.join(CSRC, "libbptplan.so")
 SCORE_SO = os.path.join(CSRC, "libbptscore.so")
 BLOCK_SO = os.path.join(CSRC, "libbptblock.so")
 LINEAR_SO = os.path.join(CSRC, "libbptlinear.so")
+BIAS_SO = os.path.join(CSRC, "libbptbias.so")
 OP_SO = os.path.join(CSRC, "bptop.so")
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
@@ -79,6 +81,11 @@ def build_linear(verbose=True):
     return LINEAR_SO
 
 
+def build_bias(verbose=True):
+    _run([HIPCC] + HIP_FLAGS + [os.path.join(CSRC, "bptbias.hip"), "-o", BIAS_SO], verbose)
+    return BIAS_SO
+
+
 def build_op(verbose=True):
     """After the HIP libraries, which it links (found beside it at run time)."""
     import sysconfig
@@ -98,7 +105,7 @@ def build_all(verbose=True):
     """The HIP compilations take most of the time and run side by side."""
     from concurrent.futures import ThreadPoolExecutor
     with ThreadPoolExecutor(2) as pool:
-        others = pool.map(lambda build: build(verbose), (build_plan, build_score, build_block, build_linear))
+        others = pool.map(lambda build: build(verbose), (build_plan, build_score, build_block, build_linear, build_bias))
         graph, attn = build_graph(verbose), build_attn(verbose)
         return (graph, attn, *others, build_op(verbose))
 

@@ -1,5 +1,5 @@
-"""ctypes bindings of the native libraries (C ABIs in include/bptgraph.h, bptattn.h, bptplan.h and bptscore.h; include/bptblock.h is called by
-bptop.so alone).
+"""ctypes bindings of the native libraries (C ABIs in include/bptgraph.h, bptattn.h, bptplan.h, bptscore.h and bptbias.h; include/bptblock.h and
+bptlinear.h are called by bptop.so alone).
 
 There is no Python or CPU fallback for the device ops: if libbptattn.so is missing, importing
 `bpt_amd.graphop` raises.  Build with `python -m bpt_amd._build`.
@@ -7,7 +7,7 @@ There is no Python or CPU fallback for the device ops: if libbptattn.so is missi
 import ctypes
 import os
 
-from ._build import ATTN_SO, GRAPH_SO, PLAN_SO, SCORE_SO
+from ._build import ATTN_SO, BIAS_SO, GRAPH_SO, PLAN_SO, SCORE_SO
 
 c_i64 = ctypes.c_int64
 c_vp = ctypes.c_void_p
@@ -128,10 +128,21 @@ SCORE_API = {
     "bpt_score_backward": (ctypes.c_int, [_PP, _PP, _PS] + [c_vp] * 13 + [c_i64] + _score_tail),
 }
 
+_bias_tail = [c_i64, c_i64, ctypes.c_int, ctypes.c_double]      # n_edges, n_buckets, h, factor
+# libbptbias (include/bptbias.h): bias of scores by buckets
+BIAS_API = {
+    "bpt_bucket_bias_forward": (ctypes.c_int, [c_vp] * 3 + _bias_tail + [ctypes.c_int] * 3 + [c_vp]),
+    "bpt_bucket_bias_backward_workspace_bytes": (c_i64, [c_i64, c_i64, ctypes.c_int, ctypes.c_int]),
+    "bpt_bucket_bias_backward": (ctypes.c_int, [c_vp] * 4 + [c_i64] + _bias_tail + [ctypes.c_int] * 2 + [c_vp]),
+    "bpt_bucket_pairs_forward": (ctypes.c_int, [c_vp] * 5 + _bias_tail + [ctypes.c_int, c_vp]),
+    "bpt_bucket_pairs_backward": (ctypes.c_int, [c_vp] * 4 + [c_i64] + _bias_tail + [ctypes.c_int, c_vp]),
+}
+
 _graph = None
 _attn = None
 _plan = None
 _score = None
+_bias = None
 
 
 def _load(path, api, what):
@@ -175,6 +186,13 @@ def score_lib():
     if _score is None:
         _score = _load(SCORE_SO, SCORE_API, "libbptscore (attention with capped scores and distance)")
     return _score
+
+
+def bias_lib():
+    global _bias
+    if _bias is None:
+        _bias = _load(BIAS_SO, BIAS_API, "libbptbias (bias of scores by buckets)")
+    return _bias
 
 
 def check_graph(status):

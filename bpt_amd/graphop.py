@@ -19,7 +19,7 @@ import threading
 
 import torch
 
-from ._lib import BPT_ERR_UNSUPPORTED, BptStatusError, PlanStruct, ScoreStruct, attn_lib, check_attn, score_lib
+from ._lib import BPT_ERR_UNSUPPORTED, BptStatusError, PlanStruct, ScoreStruct, attn_lib, check_attn, bias_lib, score_lib
 from ._native import native as _native
 from . import plan as _plan
 from .plan import GROUP_ORDER_SRC, TILE_GROUP_R, PlanCache, plan_cache
@@ -29,6 +29,7 @@ __all__ = ["maskedmm_csr_forward", "maskedmm_csr_backward", "node_mul_edge_forwa
 
 _LIB = attn_lib()          # fail at import time if the HIP library is missing
 _SCORE_LIB = score_lib()
+_BIAS_LIB = bias_lib()
 if _native.plan_bytes() != ctypes.sizeof(PlanStruct):
     raise ImportError("bptop was built for another bpt_plan: rebuild with `python -m bpt_amd._build`")
 PlanCache.native = _native
@@ -1474,3 +1475,84 @@ def relu8_backward(dy, codes, exps, dropout_p=0.0):
     """(da, y8): the gradient of relu8_forward's a, dy / (1 - dropout_p) where the code is not 0 and 0 elsewhere, and what the codes stand
     for (exact in either type), in dy's type."""
     return _native.relu8_backward(dy, codes, exps, float(dropout_p))
+
+
+# ---- bias of scores by buckets (bpt_amd/csrc/bptbias.hip; no counterpart in the reference) ----------------------------------------
+def _check_buckets(buckets, device):
+    _check_input(buckets, "buckets")
+    if buckets.dim() != 1 or buckets.dtype != torch.int64:
+        raise ValueError("buckets must be a 1-D int64 tensor")
+    if buckets.device != device:
+        raise ValueError("all tensors of a call must be on one device")
+
+
+def bucket_plan(graph, q, k, dropout_p):
+    """The in-side's tile plan of a forward with a bias by buckets (q of a padded shape), or None where it does not run on tiles that cover every edge."""
+    col, indptr_c, eid_c, indices_c = graph[4:]
+    seg = _tile_seg_without_plan(col, eid_c.size(0), q, k, q.size(1), q.size(2), dropout_p, q, _SETTINGS)
+    if seg is None:
+        return None
+    plan = plan_cache.get(col, indptr_c, eid_c, indices_c, q.size(0), k.size(0), seg_len=seg, prefer_device=True, groups=(TILE_ROWS, None))
+    return plan if plan.covers_all_edges else None
+
+
+def bucket_bias_forward(table, buckets, factor=1.0, term=False):
+    """bias[e, head] = factor * table[buckets[e], head] of table (n, h), float32, float64 or bfloat16, and buckets (E,) int64: (E, h) of table's type, or with
+    term the float32 (E + 1, h) that attention_forward takes as bias.  A bucket outside of table adds 0."""
+    _check_input(table, "table")
+    if table.dim() != 2 or table.size(0) < 1 or table.size(1) < 1:
+        raise ValueError("table must be (n_buckets, heads)")
+    _check_buckets(buckets, table.device)
+    (n, h), E = table.shape, buckets.size(0)
+    bias = torch.empty((E + int(term), h), dtype=torch.float32 if term else table.dtype, device=table.device)
+    with _on_device_of(table):
+        check_attn(_BIAS_LIB.bpt_bucket_bias_forward(_ptr(table), _ptr(buckets), _ptr(bias), E, n, h, float(factor), int(term), _dtype(table), _dtype(bias), _stream()),
+                   "bucket_bias_forward")
+    return bias
+
+
+def bucket_bias_backward(ds, buckets, table, factor=1.0):
+    """The gradient of bucket_bias_forward's table: dtable[b, head] = factor * the sum of ds[e, head] over the edges of bucket b; ds (E, h) of table's
+    type or float32.  Sums of 32 bits (64 for float64) in a fixed order."""
+    _check_input(ds, "ds")
+    _check_buckets(buckets, table.device)
+    (n, h), E = table.shape, buckets.size(0)
+    _expect_shape(ds, (E, h), "ds")
+    if ds.device != table.device:
+        raise ValueError("all tensors of a call must be on one device")
+    dtable = torch.empty((n, h), dtype=table.dtype, device=table.device)
+    with _on_device_of(table):
+        nws = _BIAS_LIB.bpt_bucket_bias_backward_workspace_bytes(E, n, h, _dtype(table))
+        if nws < 0:
+            raise ValueError("bias_table has too many buckets or heads")
+        ws = torch.empty(nws, dtype=torch.uint8, device=table.device)
+        check_attn(_BIAS_LIB.bpt_bucket_bias_backward(_ptr(ds), _ptr(buckets), _ptr(dtable), _ptr(ws), nws, E, n, h, float(factor), _dtype(table), _dtype(ds), _stream()),
+                   "bucket_bias_backward")
+    return dtable
+
+
+def bucket_pairs_forward(table, buckets, order, factor=1.0):
+    """(codes, bias): bucket_bias_forward's term in the order of a tile plan's pairs (order: attention_pair_order's), bias float32 (h, E) as attention_forward
+    takes it with bias_by_pair, codes what bucket_pairs_backward takes."""
+    (n, h), E = table.shape, buckets.size(0)
+    codes, bias = torch.empty(E, dtype=torch.int16, device=table.device), torch.empty((h, E), dtype=torch.float32, device=table.device)
+    eids = order[1]["eid_of_pair"]
+    _expect_shape(eids, (E,), "buckets")
+    with _on_device_of(table):
+        check_attn(_BIAS_LIB.bpt_bucket_pairs_forward(_ptr(table), _ptr(buckets), _ptr(eids), _ptr(codes), _ptr(bias), E, n, h, float(factor), _dtype(table), _stream()),
+                   "bucket_pairs_forward")
+    return codes, bias
+
+
+def bucket_pairs_backward(ds, codes, table, factor=1.0):
+    """bucket_bias_backward of ds (h, E), in the order of codes."""
+    (n, h), E = table.shape, codes.size(0)
+    _check_all(ds=ds, codes=codes)
+    _expect_shape(ds, (h, E), "ds")
+    dtable = torch.empty((n, h), dtype=table.dtype, device=table.device)
+    with _on_device_of(table):
+        nws = _BIAS_LIB.bpt_bucket_bias_backward_workspace_bytes(E, n, h, _dtype(table))
+        ws = torch.empty(nws, dtype=torch.uint8, device=table.device)
+        check_attn(_BIAS_LIB.bpt_bucket_pairs_backward(_ptr(ds), _ptr(codes), _ptr(dtable), _ptr(ws), nws, E, n, h, float(factor), _dtype(table), _stream()),
+                   "bucket_pairs_backward")
+    return dtable

@@ -14,7 +14,7 @@ from .graphop import (maskedmm_csr_backward, maskedmm_csr_forward, node_mul_edge
 
 __all__ = ["SparseSoftmax", "MaskedMMCSR", "NodeMulEdge", "VectorSPMM", "BPTAttention", "BPTScoreAttention", "EdgeTypeEmbedding",
            "sparse_softmax", "masked_mm", "node_mul_edge", "vec_spmm", "bpt_attention", "edge_type_embedding",
-           "add_layer_norm", "relu_linear8", "linear_act", "dropout"]
+           "add_layer_norm", "relu_linear8", "linear_act", "dropout", "bucket_bias", "BucketBias", "BPTBucketAttention"]
 
 
 class SparseSoftmax(Function):
@@ -209,6 +209,60 @@ class BPTScoreAttention(Function):
         dq, dk, dv, dslopes, _ = _g.score_attention_backward(*tensors[:13], do, _g.Score(ctx.cap, *tensors[13:]), ctx.scale, ctx.dropout_p, ctx.seed,
                                                              need_slopes=ctx.needs_input_grad[11])
         return None, None, None, None, None, None, None, None, dq, dk, dv, dslopes, None, None, None, None
+
+
+class BucketBias(Function):
+    """(E, h) rows of a (n, h) table by buckets (E,), with the sums of their gradients by buckets."""
+
+    @staticmethod
+    def forward(ctx, table, buckets):
+        ctx.save_for_backward(table, buckets)
+        return _g.bucket_bias_forward(table, buckets)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        table, buckets = ctx.saved_tensors
+        return _g.bucket_bias_backward(grad.contiguous(), buckets, table), None
+
+
+class BPTBucketAttention(Function):
+    """BPTAttention with scores scale q.k + table[buckets[e], head], with or without score options (score, slopes: as BPTRelAttention's), whose
+    cap then bounds the sum.  The fused kernels add a term before the scale: it is formed as table / scale, and the gradient of the table is the sum of
+    the term's by buckets, divided by the scale.  order: None, the term goes by edge id, or attention_pair_order's, it goes in the order of the tiles."""
+
+    @staticmethod
+    def forward(ctx, row, indptr_r, eid_r, indices_r, col, indptr_c, eid_c, indices_c, q, k, v, scale, dropout_p, seed, table, buckets, order=None, score=None,
+                slopes=None):
+        codes = None
+        if order is not None:
+            codes, bias = _g.bucket_pairs_forward(table, buckets, order, 1.0 / scale)
+        else:
+            bias = _g.bucket_bias_forward(table, buckets, 1.0 / scale, term=True)
+        if score is not None:
+            o, lse = _g.score_attention_forward(col, indptr_c, eid_c, indices_c, q, k, v, score, scale, dropout_p, seed, bias)
+        else:
+            o, lse = _g.attention_forward(col, indptr_c, eid_c, indices_c, q, k, v, scale, dropout_p, seed, bias=bias, bias_by_pair=order is not None)
+        ctx.save_for_backward(row, indptr_r, eid_r, indices_r, col, indptr_c, eid_c, indices_c, q, k, v, o, lse, bias, table, buckets if codes is None else codes,
+                              *(() if score is None else score[1:]))
+        ctx.cap, ctx.by_pair = None if score is None else score.cap, order is not None
+        ctx.scale, ctx.dropout_p, ctx.seed = scale, dropout_p, seed
+        return o
+
+    @staticmethod
+    def backward(ctx, do):
+        if torch.is_grad_enabled():
+            raise RuntimeError("attention with a bias by buckets is not differentiable twice")
+        tensors = ctx.saved_tensors
+        graph, (q, k, v, o, lse, bias, table, buckets), dslopes, dtable = tensors[:8], tensors[8:16], None, None
+        if ctx.cap is not None:
+            dq, dk, dv, dslopes, ds = _g.score_attention_backward(*graph, q, k, v, o, lse, do, _g.Score(ctx.cap, *tensors[16:]), ctx.scale, ctx.dropout_p, ctx.seed, bias,
+                                                                  ctx.needs_input_grad[18])
+        else:
+            dq, dk, dv, ds = _g.attention_backward(*graph, q, k, v, o, lse, do, ctx.scale, ctx.dropout_p, ctx.seed, bias=bias, bias_by_pair=ctx.by_pair)
+        if ctx.needs_input_grad[14]:
+            dtable = (_g.bucket_pairs_backward if ctx.by_pair else _g.bucket_bias_backward)(ds, buckets, table, 1.0 / ctx.scale)
+        return None, None, None, None, None, None, None, None, dq, dk, dv, None, None, None, dtable, None, None, None, dslopes
 
 
 def _rel_backward(row, indptr_r, eid_r, indices_r, col, indptr_c, eid_c, indices_c, q, k, v, o, lse, bias, table, do, scale, dropout_p, seed, rows_slot,
@@ -421,20 +475,30 @@ class _Capped(Function):
         return grad / torch.cosh(u / ctx.cap).square(), None
 
 
-def _score_chain(graph, q, k, v, scale, dropout_p, rel_table, etype, score):
-    """Attention with score options as the chain of separate operators, for shapes and types without a fused kernel: the (E, h) scores are
+def _score_chain(graph, q, k, v, scale, dropout_p, rel_table, etype, score, bias_table=None, buckets=None):
+    """Attention with score options or a bias by buckets as the chain of separate operators, for shapes and types without a fused kernel: the (E, h) scores are
     capped and lowered in 32 bits (64 for float64)."""
     row, indptr_r, eid_r, indices_r, col, indptr_c, eid_c, indices_c = graph
     e = masked_mm(*graph, k, q)
     if rel_table is not None:
         e = e + node_mul_edge(col, indptr_c, eid_c, q, edge_type_embedding(rel_table, etype))
     e = (e if e.dtype == torch.float64 else e.float()) * scale
+    hidden = None
+    if bias_table is not None:
+        bias = bucket_bias(bias_table, buckets).to(e.dtype).view(e.shape)
+        e = e + bias
+        if not score.cap:                     # (sparse_softmax takes no -infinity: a row of nothing else would be NaN)
+            hidden = bias.detach() == -math.inf
+            e = e.masked_fill(hidden, -1.0e8)
     if score.cap:
         e = _Capped.apply(e, score.cap)
     if score.slopes is not None:
         far = _edge_distance(score, col, indptr_c, eid_c, indices_c, e.dtype)
         e = e - (score.slopes.to(e.dtype) * far[:, None] if e.dim() == 2 else score.slopes.to(e.dtype) * far)
-    a = torch.nn.functional.dropout(sparse_softmax(col, indptr_c, eid_c, e.contiguous()), p=float(dropout_p), training=dropout_p > 0)
+    a = sparse_softmax(col, indptr_c, eid_c, e.contiguous())
+    if hidden is not None:
+        a = a.masked_fill(hidden, 0.0)
+    a = torch.nn.functional.dropout(a, p=float(dropout_p), training=dropout_p > 0)
     return vec_spmm(col, indptr_c, eid_c, indices_c, row, indptr_r, eid_r, indices_r, a.to(v.dtype), v, n_rows=None if q.size(0) == v.size(0) else q.size(0))
 
 
@@ -494,8 +558,53 @@ def _score_attention(graph, q, k, v, scale, fused, dropout_p, seed, rel_table, e
     return o if as_it_is else o[:, :h, :d].contiguous()
 
 
+def _bucket_attention(graph, q, k, v, scale, fused, dropout_p, seed, bias_table, buckets, score_cap, slopes, pos):
+    """bpt_attention with a bias by buckets, and score options or not."""
+    h = q.size(1) if q.dim() == 3 else 1
+    if bias_table.dim() != 2 or bias_table.size(0) < 1 or bias_table.size(1) != h:
+        raise ValueError(f"bias_table must be (n_buckets, {h}), got {tuple(bias_table.shape)}")
+    if buckets.dim() != 1 or buckets.dtype != torch.int64 or buckets.size(0) != graph[6].size(0):
+        raise ValueError("buckets must be a 1-D int64 tensor with one element for every edge")
+    if bias_table.dtype != q.dtype:
+        raise RuntimeError("all floating point arguments must share one dtype")
+    if bias_table.device != q.device or buckets.device != q.device:
+        raise ValueError("all tensors of a call must be on one device")
+    bias_table = bias_table.contiguous()
+    score = None if score_cap is None and slopes is None and pos is None else _g.score_options(score_cap, slopes, pos, q, k, scale)
+    train = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, bias_table, slopes))
+    runs = fused is not False and _native_takes() and 1e-6 <= abs(scale) <= 1e6 and _g.score_supported(graph[6], q, k)
+    given, given_table, order = (q, k, v), bias_table, None
+    if runs:
+        (heads, d), (hp, dp) = q.shape[1:], _g.score_padded_shape(q)
+        slopes, padded = None if score is None else score.slopes, (heads, d) != (hp, dp)
+        if padded:
+            # as with relative positions: zero columns and heads add nothing
+            q, k, v = (torch.nn.functional.pad(x, (0, dp - d, 0, hp - heads)) for x in (q, k, v))
+            bias_table = torch.nn.functional.pad(bias_table, (0, hp - heads))
+            if slopes is not None:
+                slopes = torch.nn.functional.pad(slopes, (0, hp - heads))
+                score = score._replace(slopes=slopes)
+        else:
+            q, k, v = (x.clone() if x.data_ptr() % 16 else x for x in (q, k, v))          # (the kernels read 16 bytes a lane)
+        if train and score is None:
+            order = _g.attention_pair_order(*graph, q, k, dropout_p) if all(t is not None for t in graph[:4]) and bias_table.size(0) < 65535 else None
+            runs = order is not None
+        elif score is None:
+            runs = _g.bucket_plan(graph, q, k, dropout_p) is not None
+        else:
+            runs = (not train or all(t is not None for t in graph[:4])) and _g.prepare_score(graph, q, k, dropout_p, train)
+    if not runs:
+        if fused:
+            raise RuntimeError("attention with a bias by buckets has no fused kernel for this call")
+        return _score_chain(graph, *given, scale, dropout_p, None, None, score or _g.Score(0.0, None, None, None), given_table, buckets)
+    if dropout_p > 0 and seed is None:
+        seed = int(torch.randint(0, 2 ** 62, (1,)).item())
+    o = BPTBucketAttention.apply(*graph, q, k, v, scale, float(dropout_p), int(seed or 0), bias_table, buckets, order, score, slopes)
+    return o[:, :heads, :d].contiguous() if padded else o
+
+
 def bpt_attention(row, indptr_r, eid_r, indices_r, col, indptr_c, eid_c, indices_c, q, k, v, scale=None, fused=None,
-                  dropout_p=0.0, seed=None, rel_table=None, etype=None, score_cap=None, slopes=None, pos=None):
+                  dropout_p=0.0, seed=None, rel_table=None, etype=None, score_cap=None, slopes=None, pos=None, bias_table=None, buckets=None):
     """Attention over the graph: (ROW, INDPTR_R, out_eid, out_idx) is the out-CSR side (rows =
     sources), (COL, INDPTR_C, in_eid, in_idx) the in-CSR side (rows = destinations), exactly the
     eight graph arguments modules/attention.py:66-67 passes to masked_mm.
@@ -510,6 +619,11 @@ def bpt_attention(row, indptr_r, eid_r, indices_r, col, indptr_c, eid_c, indices
     rel_table (n_types, d) and etype (E,) int64 add the rel_pos term q[dst] . rel_table[etype[e]] to the score of
     edge e (attention.py:69-71); the gradient of rel_table is returned like any other.
 
+    bias_table (n, h) of q's type and buckets (E,) int64 (not in the reference) add the scalar bias_table[buckets[e], head] to the scaled score of edge e: a
+    learned bias by distance, edge type or whatever else the caller numbers edges by.  bias_table gets a gradient, summed in a fixed order; an edge
+    whose bucket lies outside of it has no bias, and -infinity hides an edge (a row with nothing left is 0; not with score_cap, which bounds
+    it).  Not together with rel_table.
+
     Score options (not in the reference): with u the scaled score, term included,
     score_cap c > 0 (10^-10 to 10^10, and at least |scale| / 10^4) makes it c tanh(u / c), which bounds it by c;
     slopes (h,) float32 and pos, float32 positions of the rows (one tensor, or a pair (of the query rows, of the key rows)), lower it by
@@ -521,6 +635,13 @@ def bpt_attention(row, indptr_r, eid_r, indices_r, col, indptr_c, eid_c, indices
     scale = 1.0 / math.sqrt(q.size(-1)) if scale is None else float(scale)
     if (rel_table is None) != (etype is None):
         raise ValueError("rel_table and etype go together")
+    if (bias_table is None) != (buckets is None):
+        raise ValueError("bias_table and buckets go together")
+    if bias_table is not None:
+        if rel_table is not None:
+            raise ValueError("bias_table and rel_table do not go together")
+        return _bucket_attention((row, indptr_r, eid_r, indices_r, col, indptr_c, eid_c, indices_c), q, k, v, scale, fused, dropout_p, seed, bias_table, buckets,
+                                 score_cap, slopes, pos)
     if score_cap is not None or slopes is not None or pos is not None:
         return _score_attention((row, indptr_r, eid_r, indices_r, col, indptr_c, eid_c, indices_c), q, k, v, scale, fused, dropout_p, seed, rel_table, etype,
                                 score_cap, slopes, pos)
@@ -633,3 +754,10 @@ def dropout(x, dropout_p, seed=None, residual=None):
     if dropout_p > 0 and seed is None:
         seed = int(torch.randint(0, 2 ** 62, (1,)).item())
     return _native.dropout(x, residual, float(dropout_p), int(seed or 0) & (2 ** 64 - 1))
+
+
+def bucket_bias(table, buckets):
+    """table[buckets] as (E, h) scores: one of the separate operators, to be added to what masked_mm gives.  table (n, h) float32, float64 or bfloat16, buckets (E,)
+    int64; a bucket outside of the table gives 0.  The gradient of table is summed in a fixed order (torch's scatters with atomics)."""
+    _no_transforms("bucket_bias")
+    return BucketBias.apply(table.contiguous(), buckets)

@@ -10,7 +10,7 @@ DGL graph object (`g.ndata['h']`, `g.edata['etype']`) and writes the result back
 Attention core: the fused kernels (`op.bpt_attention`: rel_pos term and attention dropout included), or with
 `fused=False` the four operators composed exactly as attention.py:66-77 does.
 Residual and LayerNorm: one kernel each way (`op.add_layer_norm`) on GPU tensors of one type and rows of up to 16 KiB, the torch module
-otherwise and with `fused=False`.  Projections and the feed-forward are torch modules (rocBLAS GEMMs).
+otherwise and with `fused=False`.  Projections and the feed-forward are torch modules (rocBLAS GEMMs) unless `epilogue` says otherwise.
 
 Options the reference does not have, off by default (then nothing of them is a parameter, and the results are the reference's):
   score_cap   attention scores become cap tanh(score / cap)
@@ -18,14 +18,20 @@ Options the reference does not have, off by default (then nothing of them is a p
               (heads,) is a parameter that starts at 2^(-8 i / heads), i = 1 .. heads
   keep8       the feed-forward keeps its activations in 8 bits for the backward (`op.relu_linear8`): one byte each in place of relu's
               result, dropout's and its mask
+  epilogue    the output projection and the feed-forward run as products with bias, relu, dropout and the residual sum in their epilogue
+              (`op.linear_act`; with keep8 the feed-forward as keep8 has it, then `op.dropout` with the residual): no mask is stored, dropout's
+              decisions come from a counter-based generator seeded from torch's CPU generator.  In bfloat16 the residual sum is rounded before it is
+              normalised
+  bucket_bias scores get a learned scalar of the edge's type and the head: bias_table (bucket_bias, heads), a parameter that starts at 0; the edge types
+              are forward's etype, those outside of the table have no bias.  Not together with rel_pos
 """
 import math
 
 import torch
 import torch.nn as nn
 
-from .op import (add_layer_norm, bpt_attention, edge_type_embedding, masked_mm, node_mul_edge, plain_call, relu_linear8, sparse_softmax,
-                 vec_spmm)
+from .op import (add_layer_norm, bpt_attention, dropout, edge_type_embedding, linear_act, masked_mm, node_mul_edge, plain_call, relu_linear8,
+                 sparse_softmax, vec_spmm)
 
 __all__ = ["PositionwiseFeedForward", "BPTBlock", "BPTMemBlock"]
 
@@ -38,25 +44,65 @@ def _as_it_is(module, kind):
 
 
 def _add_norm(norm, x, residual, fused):
-    """norm(x + residual) (attention.py:79, :81), by add_layer_norm where that computes the same and is the faster way: a LayerNorm over the last axis as it is,
+    """norm(x + residual) (attention.py:79, :81; residual None: norm(x)), by add_layer_norm where that computes the same and is the faster way: a LayerNorm over the last axis as it is,
     GPU tensors of one type, nothing that casts, traces or transforms, rows that a workgroup's registers hold (16 KiB).  Longer rows are walked three times:
     forward | training, us, add_layer_norm / torch, 16383 rows of 4096 columns float32 145 / 263 | 352 / 736, of 4104 301 / 275 | 767 / 782; of 8192 columns
     bfloat16 152 / 305 | 378 / 898, of 8200 757 / 317 | 1952 / 955; in float64, where torch's is slower, of 2048 columns 146 / 381 | 370 / 843, of 4104 515 / 730 | 1345 / 1556."""
     if (fused and _as_it_is(norm, nn.LayerNorm) and len(norm.normalized_shape) == 1 and x.is_cuda and x.is_contiguous()
             and x.dtype in (torch.float32, torch.float64, torch.bfloat16) and x.dim() > 0 and x.size(-1) == norm.normalized_shape[0]
-            and (x.dtype == torch.float64 or x.size(-1) * x.element_size() <= 16384) and x.shape == residual.shape and not torch.is_autocast_enabled()
+            and (x.dtype == torch.float64 or x.size(-1) * x.element_size() <= 16384) and (residual is None or x.shape == residual.shape) and not torch.is_autocast_enabled()
             and all(t is None or (t.dtype == x.dtype and t.device == x.device and t.is_contiguous()) for t in (residual, norm.weight, norm.bias))
             and plain_call(x, residual, norm.weight, norm.bias)):
         return add_layer_norm(x, residual, norm.weight, norm.bias, norm.eps)
-    return norm(x + residual)
+    return norm(x if residual is None else x + residual)
+
+
+def _epilogue_takes(x, residual, drop, *linears):
+    """Whether the products with an epilogue may stand for calls of the linears on x, of drop and of the residual sum: torch's modules as they are, GPU tensors of one
+    type, nothing that casts, traces or transforms."""
+    tensors = [x, residual] + [t for lin in linears for t in (lin.weight, lin.bias)]
+    return (x.is_cuda and x.dtype in (torch.float32, torch.bfloat16) and x.dim() > 0 and x.size(-1) > 0 and not torch.is_autocast_enabled()
+            and all(_as_it_is(lin, nn.Linear) for lin in linears) and _as_it_is(drop, nn.Dropout) and 0.0 <= drop.p < 1.0
+            and all(t is None or (t.dtype == x.dtype and t.device == x.device and t.is_contiguous()) for t in tensors) and plain_call(*tensors))
+
+
+def _share(drop):
+    return drop.p if drop.training else 0.0
+
+
+def _project_add_norm(block, norm, lin, drop, x, residual):
+    """norm(residual + drop(lin(x))) (attention.py:79)."""
+    if block.epilogue and x.size(0) == residual.size(0) and _epilogue_takes(x, residual, drop, lin):
+        return _add_norm(norm, linear_act(x, lin.weight, lin.bias, residual=residual, dropout_p=_share(drop)), None, block.fused)
+    return _add_norm(norm, residual, drop(lin(x)), block.fused)
+
+
+def _feed_forward_add_norm(block, norm, h):
+    """norm(h + drop(ffn(h))) (attention.py:81): block.ffn is a feed-forward and a dropout."""
+    if not (block.epilogue and _as_it_is(block.ffn, nn.Sequential) and len(block.ffn) == 2 and _as_it_is(block.ffn[0], PositionwiseFeedForward)):
+        return _add_norm(norm, h, block.ffn(h), block.fused)
+    ffn, drop = block.ffn
+    if not (_epilogue_takes(h, None, drop, ffn.w_1, ffn.w_2) and _as_it_is(ffn.dropout, nn.Dropout) and 0.0 <= ffn.dropout.p < 1.0):
+        return _add_norm(norm, h, block.ffn(h), block.fused)
+    if ffn.keep8:
+        z = dropout(ffn(h), _share(drop), residual=h)
+    else:
+        a = linear_act(h, ffn.w_1.weight, ffn.w_1.bias, activation="relu", dropout_p=_share(ffn.dropout))
+        z = linear_act(a, ffn.w_2.weight, ffn.w_2.bias, residual=h, dropout_p=_share(drop))
+    return _add_norm(norm, z, None, block.fused)
+
+
+def _check_bucket_bias(rel_pos, bucket_bias):
+    if bucket_bias and rel_pos:
+        raise ValueError("bucket_bias and rel_pos do not go together")
 
 
 def _distance_slopes(h):
     return nn.Parameter(2.0 ** (-8.0 * torch.arange(1, h + 1, dtype=torch.float32) / h))
 
 
-def _score_options(block, pos):
-    """bpt_attention's score options of a block."""
+def _score_options(block, pos, etype):
+    """bpt_attention's score options and bias of a block."""
     opts = {}
     if block.score_cap is not None:
         opts["score_cap"] = block.score_cap
@@ -64,6 +110,10 @@ def _score_options(block, pos):
         if pos is None:
             raise ValueError("distance=True needs the positions of the nodes (pos)")
         opts.update(slopes=block.slopes.float(), pos=pos)
+    if block.bucket_bias:
+        if etype is None:
+            raise ValueError("bucket_bias needs the edge types (etype)")
+        opts.update(bias_table=block.bias_table, buckets=etype)
     return opts
 
 
@@ -95,10 +145,13 @@ class PositionwiseFeedForward(nn.Module):
 
 class BPTBlock(nn.Module):
     MAX_ETYPE = 1000        # modules/attention.py:23
-    score_cap, distance = None, False
+    score_cap, distance, epilogue, bucket_bias = None, False, False, 0
 
-    def __init__(self, dim_model, h, dim_ff, rel_pos=False, drop_h=0.1, drop_a=0.1, fused=True, score_cap=None, distance=False, keep8=False):
+    def __init__(self, dim_model, h, dim_ff, rel_pos=False, drop_h=0.1, drop_a=0.1, fused=True, score_cap=None, distance=False, keep8=False, epilogue=False,
+                 bucket_bias=0):
         super().__init__()
+        _check_bucket_bias(rel_pos, bucket_bias)
+        self.epilogue, self.bucket_bias = epilogue, bucket_bias
         self.fused = fused          # False: the four operators composed exactly as attention.py:66-77 does
         self.score_cap, self.distance = score_cap, distance
         self.dim_model, self.h, self.dim_ff = dim_model, h, dim_ff
@@ -116,6 +169,8 @@ class BPTBlock(nn.Module):
             self.embed_ak = nn.Embedding(self.MAX_ETYPE, self.d_k)
         if distance:
             self.slopes = _distance_slopes(h)
+        if bucket_bias:
+            self.bias_table = nn.Parameter(torch.zeros(bucket_bias, h))
         self.ffn = nn.Sequential(PositionwiseFeedForward(dim_model, dim_ff, dropout=drop_h, keep8=keep8), nn.Dropout(drop_h))
 
     def reset_parameters(self):
@@ -131,7 +186,7 @@ class BPTBlock(nn.Module):
         att_dropout = self.drop_att.p if self.training else 0.0
         if self.rel_pos and etype is None:
             raise ValueError("rel_pos=True needs the edge types (etype)")
-        opts = _score_options(self, pos)
+        opts = _score_options(self, pos, etype)
         if self.fused or opts:
             rel = dict(rel_table=self.embed_ak.weight, etype=etype) if self.rel_pos else {}
             return bpt_attention(*graph, q, k, v, fused=None if self.fused else False, dropout_p=att_dropout, **rel, **opts).view(-1, self.d_k * self.h)
@@ -149,8 +204,8 @@ class BPTBlock(nn.Module):
         k = self.proj_k(h).view(-1, self.h, self.d_k)
         v = self.proj_v(h).view(-1, self.h, self.d_k)
         a = self.attention(q, k, v, csr, etype, pos) if pos is not None else self.attention(q, k, v, csr, etype)
-        h = _add_norm(self.norm_in, h, self.drop_h(self.proj_o(a)), self.fused)
-        return _add_norm(self.norm_inter, h, self.ffn(h), self.fused)
+        h = _project_add_norm(self, self.norm_in, self.proj_o, self.drop_h, a, h)
+        return _feed_forward_add_norm(self, self.norm_inter, h)
 
 
 def _graph_args(csr):
@@ -174,12 +229,15 @@ class BPTMemBlock(nn.Module):
 
     Both attention cores run the fused kernels (`op.bpt_attention`) where they cover the shape; `fused=False` composes
     the four operators exactly as the reference does.  score_cap caps the scores of both, distance (with forward's pos, the positions of this
-    block's nodes) lowers those of the self-attention; keep8 as in BPTBlock."""
+    block's nodes) lowers those of the self-attention, bucket_bias (with etype) adds to these; keep8 and epilogue as in BPTBlock."""
     MAX_ETYPE = 1000        # modules/attention.py:85
-    score_cap, distance = None, False
+    score_cap, distance, epilogue, bucket_bias = None, False, False, 0
 
-    def __init__(self, dim_model, h, dim_ff, rel_pos=False, drop_h=0.1, drop_a=0.1, fused=True, score_cap=None, distance=False, keep8=False):
+    def __init__(self, dim_model, h, dim_ff, rel_pos=False, drop_h=0.1, drop_a=0.1, fused=True, score_cap=None, distance=False, keep8=False, epilogue=False,
+                 bucket_bias=0):
         super().__init__()
+        _check_bucket_bias(rel_pos, bucket_bias)
+        self.epilogue, self.bucket_bias = epilogue, bucket_bias
         self.fused = fused
         self.score_cap, self.distance = score_cap, distance
         self.dim_model, self.h, self.dim_ff = dim_model, h, dim_ff
@@ -196,6 +254,8 @@ class BPTMemBlock(nn.Module):
             self.embed_ak = nn.Embedding(self.MAX_ETYPE, self.d_k)
         if distance:
             self.slopes = _distance_slopes(h)
+        if bucket_bias:
+            self.bias_table = nn.Parameter(torch.zeros(bucket_bias, h))
         self.ffn = nn.Sequential(PositionwiseFeedForward(dim_model, dim_ff, dropout=drop_h, keep8=keep8), nn.Dropout(drop_h))
 
     def reset_parameters(self):
@@ -212,7 +272,7 @@ class BPTMemBlock(nn.Module):
         rel = self.rel_pos and which == 0
         if rel and etype is None:
             raise ValueError("rel_pos=True needs the edge types (etype)")
-        opts = _score_options(self, pos) if which == 0 else {} if self.score_cap is None else dict(score_cap=self.score_cap)
+        opts = _score_options(self, pos, etype) if which == 0 else {} if self.score_cap is None else dict(score_cap=self.score_cap)
         if self.fused or opts:
             extra = dict(rel_table=self.embed_ak.weight, etype=etype) if rel else {}
             return bpt_attention(*graph, q, k, v, fused=None if self.fused else False, dropout_p=p, **extra, **opts).view(-1, self.d_k * self.h)
@@ -228,7 +288,7 @@ class BPTMemBlock(nn.Module):
         heads = lambda proj, x: proj(x).view(-1, self.h, self.d_k)
         # Part I: self-attention (attention.py:118-142)
         a = self._attend(0, heads(self.proj_q[0], h), heads(self.proj_k[0], h), heads(self.proj_v[0], h), csr, etype, pos)
-        h = _add_norm(self.norm_in[0], h, self.drop_h[0](self.proj_o[0](a)), self.fused)
+        h = _project_add_norm(self, self.norm_in[0], self.proj_o[0], self.drop_h[0], a, h)
         # Part II: attention to memory (attention.py:144-168)
         n = h.size(0)
         n_q = csr_inter[1][0].numel() - 1                  # rows of the inter graph's in-CSR
@@ -236,6 +296,6 @@ class BPTMemBlock(nn.Module):
             raise ValueError("the inter graph has fewer destination nodes than the block has states")
         hq = h if n_q == n else torch.cat([h, h.new_zeros(n_q - n, h.size(1))], 0)        # attention.py:148-149
         a = self._attend(1, heads(self.proj_q[1], hq), heads(self.proj_k[1], mem), heads(self.proj_v[1], mem), csr_inter)[:n]
-        h = _add_norm(self.norm_in[1], h, self.drop_h[1](self.proj_o[1](a)), self.fused)
+        h = _project_add_norm(self, self.norm_in[1], self.proj_o[1], self.drop_h[1], a, h)
         # FFN (attention.py:170-171)
-        return _add_norm(self.norm_inter, h, self.ffn(h), self.fused)
+        return _feed_forward_add_norm(self, self.norm_inter, h)

@@ -37,14 +37,15 @@ inline Drop make_drop(double p, uint64_t seed) {
     const double t = p * 4294967296.0;
     return Drop{(uint32_t)(t >= 4294967295.0 ? 4294967295.0 : t < 1.0 ? 1.0 : t), (uint32_t)seed, (uint32_t)(seed >> 32), (float)(1.0 / (1.0 - p))};
 }
+__device__ __forceinline__ uint32_t xor3(uint32_t a, uint32_t b, uint32_t c) { return __builtin_amdgcn_bitop3_b32(a, b, c, 0x96); }
 __device__ __forceinline__ uintx4 philox(uint64_t counter, uint32_t k0, uint32_t k1) {
     uint32_t c0 = (uint32_t)counter, c1 = (uint32_t)(counter >> 32), c2 = 0u, c3 = 0u;
 #pragma unroll
     for (int r = 0; r < 10; ++r) {
         const uint64_t p = (uint64_t)c0 * 0xD2511F53u, q = (uint64_t)c2 * 0xCD9E8D57u;
-        c0 = (uint32_t)(q >> 32) ^ c1 ^ k0;
+        c0 = xor3((uint32_t)(q >> 32), c1, k0);
         c1 = (uint32_t)q;
-        c2 = (uint32_t)(p >> 32) ^ c3 ^ k1;
+        c2 = xor3((uint32_t)(p >> 32), c3, k1);
         c3 = (uint32_t)p;
         k0 += 0x9E3779B9u;
         k1 += 0xBB67AE85u;
@@ -67,17 +68,31 @@ __device__ __forceinline__ floatx4 dropped(floatx4 v, uintx4 words, const Drop &
 }
 
 // ---- activations -------------------------------------------------------------------------------------------------------------------
-// (erfc keeps its digits where a is far below zero, 1 + erf does not)
-__device__ __forceinline__ float normal_cdf(float a) { return 0.5f * erfcf(a * -0.70710678118654752f); }
+// Phi(a) = erfc(-a / sqrt 2) / 2 from e = exp(-a^2 / 2): erfc(z) exp(z^2) = t P(t), t = 1 / (1 + 0.45 z) for z >= 0, P of degree 9 fitted to 1.6e-8 of it (least squares
+// on 4000 points, weights raised where the error is largest); 1.5e-7 with the roundings of float32, also far below zero, where 1 + erf keeps no digits.
+__device__ __forceinline__ float gaussian(float a) { return __builtin_amdgcn_exp2f(a * a * -0.72134752044448170f); }
+__device__ __forceinline__ float normal_cdf(float a, float e) {
+    const float t = __builtin_amdgcn_rcpf(fmaf(fabsf(a), 0.45f * 0.70710678118654752f, 1.f));
+    constexpr float P[10] = {0.253877291f,  0.254068526f,  0.226492773f,  0.184594003f, 0.0902296561f,
+                             0.0373546171f, 0.0662443061f, -0.240835511f, 0.164408172f, -0.0364338496f};
+    float p = P[9];
+#pragma unroll
+    for (int i = 8; i >= 0; --i) p = fmaf(p, t, P[i]);
+    p *= 0.5f * t * e;
+    return a < 0.f ? p : 1.f - p;                                 // (NaN: 1 - NaN)
+}
 __device__ __forceinline__ float activated(float a, int act) {
     if (act == BPT_ACT_RELU) return a <= 0.f ? 0.f : a;           // (NaN stays)
-    if (act == BPT_ACT_GELU) return a * normal_cdf(a);
+    if (act == BPT_ACT_GELU) return a * normal_cdf(a, gaussian(a));
     return a;
 }
 // g act'(a)
 __device__ __forceinline__ float activated_back(float g, float a, int act) {
     if (act == BPT_ACT_RELU) return a <= 0.f ? 0.f : g;
-    if (act == BPT_ACT_GELU) return g * (normal_cdf(a) + a * expf(-0.5f * a * a) * 0.39894228040143268f);
+    if (act == BPT_ACT_GELU) {
+        const float e = gaussian(a);
+        return g * fmaf(a * e, 0.39894228040143268f, normal_cdf(a, e));
+    }
     return g;
 }
 
@@ -86,11 +101,17 @@ template <typename T> struct Epilogue {
     const T *bias, *residual;
     T *y, *kept;
     int64_t cols;
+    float scale;                 // of the product
     int act;
     Drop drop;
     bool quads;                  // rows, and with them quads, start on four elements everywhere
-    __device__ __forceinline__ void operator()(floatx4 v, int64_t row, int64_t col) const {
+    // what the result is added to, where it is read ahead
+    __device__ __forceinline__ floatx4 ask(int64_t row, int64_t col) const {
+        return quads && residual ? load4(residual + row * cols + col) : floatx4{0.f, 0.f, 0.f, 0.f};
+    }
+    __device__ __forceinline__ void operator()(floatx4 v, int64_t row, int64_t col, floatx4 ahead) const {
         const int64_t at = row * cols + col;
+        v *= scale;
         if (quads) {
             if (bias) v += load4(bias + col);
             if (kept) store4(kept + at, v);
@@ -99,7 +120,7 @@ template <typename T> struct Epilogue {
                 for (int e = 0; e < 4; ++e) v[e] = activated(v[e], act);
             }
             if (drop.thr) v = dropped(v, philox((uint64_t)at >> 2, drop.k0, drop.k1), drop);
-            if (residual) v += load4(residual + at);
+            if (residual) v += ahead;
             store4(y + at, v);
             return;
         }
@@ -124,17 +145,20 @@ template <typename T> struct Epilogue {
 //   forward  A = weight (p, r) by rows,       B = x (q, r) by rows
 //   dx       A = weight, (r, p) in memory,    B = g by rows
 //   dweight  A = x, (r, p) in memory,         B = g, (r, q) in memory
-// A workgroup of four wavefronts owns a tile of TB x TB; the reduction goes through LDS 128 bytes a row at a time (32 float32, 64 bfloat16), two
-// buffers, the next one's 16-byte loads straight into LDS while this one is multiplied.  Fragments are 16 rows x 16 bytes a lane: one
+// A workgroup owns a tile of BP x BQ; the reduction goes through LDS RB bytes a row at a time, two buffers: while one is multiplied, the other's
+// 16-byte loads are on their way straight into LDS.  Bound by matrix instructions where the reduction is long (bfloat16 65535 x 4096 -> 1024: 450 to 650 us
+// a product, 850 to 1200 TFLOP/s), by the epilogue's memory and vector instructions where it is short.  Fragments are 16 rows x 16 bytes a lane: one
 // 16x16x32 product in bfloat16, four 16x16x4 in float32, whose reduction indices (4 g + j for lane group g and product j) only have to agree
 // between the operands.  A is the matrix instructions' first operand, so a lane ends with four neighbouring columns of a row.
-// An operand by rows lies in LDS as rows of eight 16-byte chunks, chunk c at c ^ (row & 7): the sixteen rows that a fragment reads at one chunk
-// spread over the banks.  One that has the reduction outside lies as rows of TB elements; float32 fragments are read word by word, bfloat16
+// An operand by rows lies in LDS as rows of RB / 16 chunks, shifted by row (rows_shift): the sixteen rows that a fragment reads at one chunk
+// spread over the banks.  One that has the reduction outside lies as rows of the tile's elements; float32 fragments are read word by word, bfloat16
 // ones by transposing loads (lane i of sixteen gives the address of 4 columns of row i / 4 and gets column i of four rows), and chunks are
 // shifted by row so that the four lane groups meet different banks.
-// What does not start on 16 bytes, and the last piece of a ragged reduction, goes through registers, where what lies outside is made zero.
-template <typename T> constexpr int step() { return 128 / (int)sizeof(T); }     // the reduction's share of one buffer
+// Rows that do not start on 4 bytes, and the last piece of a ragged reduction, go through registers, where what lies outside is made zero.
+template <typename T, int RB> constexpr int step() { return RB / (int)sizeof(T); }     // the reduction's share of one buffer
 
+// (sixteen-byte reads go to LDS sixteen lanes at a time, of lanes 0 .. 31 those of rows 0 - 3 and 12 - 15 of one chunk with rows 4 - 11 of the next)
+template <int RB> __device__ __forceinline__ int rows_shift(int row) { return RB == 128 ? row & 7 : ((row >> 2 ^ row >> 3) & 1) << 1 | (row >> 3 & 1); }
 template <typename T, int TB> __device__ __forceinline__ int cols_shift(int r) {
     constexpr int CHUNKS = TB * (int)sizeof(T) / 16;
     if constexpr (sizeof(T) == 4) return ((r >> 2 & 3) << 2) & (CHUNKS - 1);
@@ -156,44 +180,58 @@ template <typename T> __device__ __forceinline__ uintx4 load_upto(const T *p, in
     return uintx4{(uint32_t)half[0], (uint32_t)(half[0] >> 32), (uint32_t)half[1], (uint32_t)(half[1] >> 32)};
 }
 
+// Sixteen bytes a lane from memory straight to LDS, lane l's to byte 16 l from `to` on (of the wavefront): a buffer descriptor of the whole address range from a
+// uniform start and an offset a lane, so nothing is added per lane and load.  In assembly, because the compiler takes every transposing read of LDS for one that may
+// read what is still on its way and waits for it; the waits are written where they belong (wait_and_meet), and no register is written.
+__device__ __forceinline__ uint32_t lds_place(const char *p) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char *)p; }
+__device__ __forceinline__ uintx4 whole_memory(const void *p) {
+    const uint64_t at = (uint64_t)p;
+    uintx4 d{(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)at), (uint32_t)__builtin_amdgcn_readfirstlane((int)((uint32_t)(at >> 32) & 0xffffu)), 0xffffffffu,
+             0x00027000u};
+    asm volatile("s_nop 4" : "+s"(d));                             // (a scalar register that a vector instruction wrote may be read by a load five states later)
+    return d;
+}
+__device__ __forceinline__ void load_to_lds(uintx4 from, uint32_t offset, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(offset), "s"(from) : "memory", "m0");
+}
+
 // one operand's way from memory to LDS
-template <typename T, int TB, bool COLS> struct Stage {
-    static constexpr int N = TB * 8 / BLOCK, VE = ve<T>(), CHUNKS = COLS ? TB * (int)sizeof(T) / 16 : 8;
+template <typename T, int TB, int RB, int WAVES, bool COLS> struct Stage {
+    static constexpr int N = TB * RB / 16 / (WAVES * WAVE), VE = ve<T>(), CHUNKS = COLS ? TB * (int)sizeof(T) / 16 : RB / 16;
     const T *base;               // of this tile's first row (column) and the first step
     int64_t ld, stride;          // elements of a row in memory; from step to step
     int left, reduce;            // rows (columns) from base on; the reduction's length from base on
     uint32_t off[N];             // bytes from base, of a lane's vectors where they are whole
 
-    static __device__ __forceinline__ int slot(int i) { return (i * WAVES_PER_BLOCK + (int)(threadIdx.x >> 6)) * WAVE + (int)(threadIdx.x & 63); }
+    static __device__ __forceinline__ int slot(int i) { return (i * WAVES + (int)(threadIdx.x >> 6)) * WAVE + (int)(threadIdx.x & 63); }
     static __device__ __forceinline__ int line(int i) { return slot(i) / CHUNKS; }
     static __device__ __forceinline__ int first(int i) {           // first element of the vector within its line
         const int l = line(i);
-        return ((slot(i) % CHUNKS) ^ (COLS ? cols_shift<T, TB>(l) : l & 7)) * VE;
+        return ((slot(i) % CHUNKS) ^ (COLS ? cols_shift<T, TB>(l) : rows_shift<RB>(l))) * VE;
     }
     // (a stage starts at step s of the reduction and tile row / column t)
     __device__ __forceinline__ Stage(const T *p, int64_t ld_, int64_t n, int64_t reduce_, int64_t t, int64_t s) : ld(ld_) {
-        const int64_t r0 = s * step<T>();
+        const int64_t r0 = s * step<T, RB>();
         base = COLS ? p + r0 * ld + t : p + t * ld + r0;
-        stride = COLS ? ld * step<T>() : step<T>();
+        stride = COLS ? ld * step<T, RB>() : step<T, RB>();
         left = (int)(n - t < TB ? n - t : TB);
         reduce = (int)(reduce_ - r0);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            // (past the end: the last row, the last vector of a row; nothing of them is stored)
-            const int l = COLS ? line(i) : min(line(i), left - 1), f = COLS ? min(first(i), left - VE) : first(i);
+            // (past the end: the last row, the vector with a row's last element; nothing of them is stored)
+            const int l = COLS ? line(i) : min(line(i), left - 1), f = COLS ? min(first(i), (left - 1) / VE * VE) : first(i);
             off[i] = (uint32_t)((l * ld + f) * (int64_t)sizeof(T));
         }
     }
-    __device__ __forceinline__ void direct(int s, char *lds) const {
-        const char *const at = reinterpret_cast<const char *>(base + s * stride);
+    __device__ __forceinline__ void direct(int s, const char *lds) const {
+        const uint32_t to = __builtin_amdgcn_readfirstlane(lds_place(lds) + (threadIdx.x >> 6) * (WAVE * 16));
+        const uintx4 from = whole_memory(base + s * stride);
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(at + off[i]),
-                                             (__attribute__((address_space(3))) void *)(lds + (i * WAVES_PER_BLOCK + (int)(threadIdx.x >> 6)) * WAVE * 16), 16, 0, 0);
+        for (int i = 0; i < N; ++i) load_to_lds(from, off[i], to + i * (WAVES * WAVE * 16));
     }
     __device__ __forceinline__ void load(int s, uintx4 (&v)[N]) const {
         const T *const at = base + s * stride;
-        const int rest = reduce - s * step<T>();
+        const int rest = reduce - s * step<T, RB>();
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int l = line(i), f = first(i), lines = COLS ? rest : left, cols = COLS ? left : rest;
@@ -206,14 +244,14 @@ template <typename T, int TB, bool COLS> struct Stage {
     }
 };
 
-// the 16 bytes that a lane has of fragment rows from .. from + 15 at half `half` of a buffer
-template <typename T, int TB, bool COLS> __device__ __forceinline__ uintx4 fragment(const char *lds, int from, int half) {
+// the 16 bytes that a lane has of fragment rows from .. from + 15 at bytes 64 part .. of a buffer's rows
+template <typename T, int TB, int RB, bool COLS> __device__ __forceinline__ uintx4 fragment(const char *lds, int from, int part) {
     const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
     if constexpr (!COLS) {
-        return *reinterpret_cast<const uintx4 *>(lds + (from + c) * 128 + ((half * 4 + g) ^ (c & 7)) * 16);
+        return *reinterpret_cast<const uintx4 *>(lds + (from + c) * RB + ((part * 4 + g) ^ rows_shift<RB>(c)) * 16);
     } else if constexpr (sizeof(T) == 4) {
         uintx4 v;
-        const int r = half * 16 + 4 * g, col = from + c;
+        const int r = part * 16 + 4 * g, col = from + c;
         const char *const p = lds + r * (TB * 4) + (((col >> 2) ^ cols_shift<T, TB>(r)) << 4) + (col & 3) * 4;
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const uint32_t *>(p + j * (TB * 4));
@@ -223,7 +261,7 @@ template <typename T, int TB, bool COLS> __device__ __forceinline__ uintx4 fragm
         const int col = from + (c & 3) * 4;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            const int r = half * 32 + 8 * g + 4 * t + (c >> 2);
+            const int r = part * 32 + 8 * g + 4 * t + (c >> 2);
             const char *const p = lds + r * (TB * 2) + (((col >> 3) ^ cols_shift<T, TB>(r)) << 4) + (col & 7) * 2;
             const shortx4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) shortx4 *)const_cast<char *>(p));
             const uintx2v w = __builtin_bit_cast(uintx2v, x);
@@ -243,6 +281,44 @@ template <typename T> __device__ __forceinline__ floatx4 multiply(uintx4 a, uint
     }
 }
 
+__device__ __forceinline__ void wait_for_lds() { __builtin_amdgcn_s_waitcnt(15 | 7 << 4 | 3 << 14); }
+// Eight float32 as three bfloat16 each, exactly: the upper 16 bits, those of what is left, and what is left then (8 + 8 + 8 digits).
+__device__ __forceinline__ void thirds(uintx4 a, uintx4 b, uintx4 (&out)[3]) {
+    uint32_t x[8], y[8], z[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        x[e] = e < 4 ? a[e & 3] : b[e & 3];
+        y[e] = __float_as_uint(__uint_as_float(x[e]) - __uint_as_float(x[e] & 0xffff0000u));
+        z[e] = __float_as_uint(__uint_as_float(y[e]) - __uint_as_float(y[e] & 0xffff0000u));
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        out[0][e] = __builtin_amdgcn_perm(x[2 * e + 1], x[2 * e], 0x07060302u);
+        out[1][e] = __builtin_amdgcn_perm(y[2 * e + 1], y[2 * e], 0x07060302u);
+        out[2][e] = __builtin_amdgcn_perm(z[2 * e + 1], z[2 * e], 0x07060302u);
+    }
+}
+
+// Waits until at most N of this wavefront's loads are on their way and all that it has asked of LDS is there, then for the workgroup.
+template <int N> __device__ __forceinline__ void wait_and_meet() {
+    issue_loads_first();
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+    wait_for_lds();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    issue_loads_first();
+}
+// The order of what has been written since the last fence: reads of LDS spread evenly between matrix products.
+template <int READS, int PRODUCTS> __device__ __forceinline__ void in_turn() {
+    constexpr int EACH = PRODUCTS / READS > 0 ? PRODUCTS / READS : 1;
+#pragma unroll
+    for (int i = 0; i < READS; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, EACH, 0);
+    }
+}
+
 struct Product {
     int64_t P, Q, R;             // columns, rows, reduction
     int64_t lda, ldb;
@@ -250,93 +326,211 @@ struct Product {
     int steps, per_split;        // steps of the reduction, of a share
 };
 
+// The tiles' shapes: columns, rows, wavefronts over either, bytes of a row and step, buffers, workgroups a compute unit.
+template <int BP_, int BQ_, int GP_, int GQ_, int PER_CU_> struct Shape {
+    static constexpr int BP = BP_, BQ = BQ_, GP = GP_, GQ = GQ_, RB = 128, STAGES = 2, WAVES = GP * GQ, THREADS = WAVES * WAVE;
+    static constexpr int PER_SIMD = (PER_CU_ * WAVES + 3) / 4;     // wavefronts that share a vector unit's registers
+};
+
 // The sums leave through LDS, so that a row of the tile is written (and bias, residual read) as one run of memory.
 // part: null, or (splits, Q, P) sums of the shares, which k_linear_finish adds up
-template <typename T, int TB, bool ACOLS, bool BCOLS, bool DIRECT>
-__global__ __launch_bounds__(BLOCK, TB == 128 ? 2 : 4) void k_linear_tiles(const T *__restrict__ a, const T *__restrict__ b, Product m, Epilogue<T> out,
-                                                                           float *__restrict__ part) {
-    constexpr int WT = TB / 2, F = WT / 16;                        // a wavefront's part of the tile, in fragments
-    __shared__ __attribute__((aligned(16))) char lds[4 * TB * 128];
+template <typename T, typename S, bool ACOLS, bool BCOLS, bool DIRECT, bool THIRDS>
+__global__ __launch_bounds__(S::THREADS, S::PER_SIMD) void k_linear_tiles(const T *__restrict__ a, const T *__restrict__ b, Product m, Epilogue<T> out, float *__restrict__ part) {
+    constexpr int BP = S::BP, BQ = S::BQ, RB = S::RB, STAGES = S::STAGES;
+    constexpr int WP = BP / S::GP, WQ = BQ / S::GQ, FP = WP / 16, FQ = WQ / 16;        // a wavefront's part of the tile, in fragments
+    constexpr int BUFFER = (BP + BQ) * RB;
+    constexpr int PASSES = BP * BQ * 4 <= STAGES * BUFFER ? 1 : 2, JS = FQ / PASSES, ROWS = S::GQ * 16 * JS;      // of sums that LDS takes at a time, fragments and rows
+    static_assert(ROWS * BP * 4 <= STAGES * BUFFER, "");
+    __shared__ __attribute__((aligned(16))) char lds[STAGES * BUFFER];
     const int id = xcd_contiguous_block(), split = id / m.tiles, tile = id - split * m.tiles;
-    const int64_t q0 = (int64_t)(tile / m.tiles_p) * TB, p0 = (int64_t)(tile % m.tiles_p) * TB;
+    const int64_t q0 = (int64_t)(tile / m.tiles_p) * BQ, p0 = (int64_t)(tile % m.tiles_p) * BP;
     const int s0 = split * m.per_split, n = min(m.per_split, m.steps - s0);
-    const Stage<T, TB, ACOLS> sa(a, m.lda, m.P, m.R, p0, s0);
-    const Stage<T, TB, BCOLS> sb(b, m.ldb, m.Q, m.R, q0, s0);
-    const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, wp = (w & 1) * WT, wq = (w >> 1) * WT;
-    floatx4 acc[F][F];
+    typedef Stage<T, BP, RB, S::WAVES, ACOLS> StageA;
+    typedef Stage<T, BQ, RB, S::WAVES, BCOLS> StageB;
+    const StageA sa(a, m.lda, m.P, m.R, p0, s0);
+    const StageB sb(b, m.ldb, m.Q, m.R, q0, s0);
+    const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, wp = w % S::GP * WP, wq = w / S::GP * WQ;
+    floatx4 acc[FP][FQ];
 #pragma unroll
-    for (int i = 0; i < F; ++i)
+    for (int i = 0; i < FP; ++i)
 #pragma unroll
-        for (int j = 0; j < F; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
-    auto buffer = [&](int s, int operand) { return lds + ((s & 1) * 2 + operand) * (TB * 128); };
-    auto compute = [&](int s) {
+        for (int j = 0; j < FQ; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+    uintx4 fa[2][FP], fb[2][FQ];
+    auto read = [&](int into, const char *at, int half) {
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            uintx4 fa[F], fb[F];
+        for (int i = 0; i < FP; ++i) fa[into][i] = fragment<T, BP, RB, ACOLS>(at, wp + 16 * i, half);
 #pragma unroll
-            for (int i = 0; i < F; ++i) fa[i] = fragment<T, TB, ACOLS>(buffer(s, 0), wp + 16 * i, half);
+        for (int j = 0; j < FQ; ++j) fb[into][j] = fragment<T, BQ, RB, BCOLS>(at + BP * RB, wq + 16 * j, half);
+    };
+    auto products = [&](int of) {
 #pragma unroll
-            for (int j = 0; j < F; ++j) fb[j] = fragment<T, TB, BCOLS>(buffer(s, 1), wq + 16 * j, half);
+        for (int j = 0; j < FQ; ++j)
 #pragma unroll
-            for (int i = 0; i < F; ++i)
+            for (int i = 0; i < FP; ++i) acc[i][j] = multiply<T>(fa[of][i], fb[of][j], acc[i][j]);
+    };
+    // float32 by the bfloat16 units: six of the nine products of thirds, those that are left out are below 2^-23 of |a| |b|
+    auto products_of_thirds = [&](const char *at) {
+        uintx4 ta[FP][3], raw[2][2];
+        auto read_b = [&](int j) {
 #pragma unroll
-                for (int j = 0; j < F; ++j) acc[i][j] = multiply<T>(fa[i], fb[j], acc[i][j]);
+            for (int half = 0; half < 2; ++half) raw[j & 1][half] = fragment<T, BQ, RB, BCOLS>(at + BP * RB, wq + 16 * j, half);
+        };
+#pragma unroll
+        for (int i = 0; i < FP; ++i) thirds(fragment<T, BP, RB, ACOLS>(at, wp + 16 * i, 0), fragment<T, BP, RB, ACOLS>(at, wp + 16 * i, 1), ta[i]);
+        read_b(0);
+#pragma unroll
+        for (int j = 0; j < FQ; ++j) {
+            issue_loads_first();                                   // (a fragment ahead, not all of them: they would not fit)
+            if (j + 1 < FQ) read_b(j + 1);
+            uintx4 tb[3];
+            thirds(raw[j & 1][0], raw[j & 1][1], tb);
+            constexpr int OF[6][2] = {{2, 0}, {0, 2}, {1, 1}, {1, 0}, {0, 1}, {0, 0}};
+#pragma unroll
+            for (int t = 0; t < 6; ++t)
+#pragma unroll
+                for (int i = 0; i < FP; ++i) acc[i][j] = multiply<bf16_t>(ta[i][OF[t][0]], tb[OF[t][1]], acc[i][j]);
         }
     };
     int s = 0;
     if constexpr (DIRECT) {
-        const int whole = min(n, sa.reduce / step<T>());
+        constexpr int LOADS = StageA::N + StageB::N;
+        // (the vector with a row's last element may run into the next row: not of the last row of all)
+        const int crosses = (ACOLS && m.P % ve<T>() != 0) || (BCOLS && m.Q % ve<T>() != 0);
+        const int whole = min(n, (sa.reduce - crosses) / step<T, RB>());
         auto ask = [&](int t) {
-            sa.direct(t, buffer(t, 0));
-            sb.direct(t, buffer(t, 1));
+            char *const at = lds + (t & 1) * BUFFER;
+            sa.direct(t, at);
+            sb.direct(t, at + BP * RB);
         };
-        if (whole > 0) ask(0);
-        for (; s < whole; ++s) {
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");       // (this wavefront's part of step s is in LDS)
-            __syncthreads();                                       // (everyone's is, and what the other buffer held has been read)
-            if (s + 1 < whole) ask(s + 1);
-            compute(s);
-        }
-    }
-    for (; s < n; ++s) {                                           // (the ragged end, or everything)
-        uintx4 va[Stage<T, TB, ACOLS>::N], vb[Stage<T, TB, BCOLS>::N];
-        sa.load(s, va);
-        sb.load(s, vb);
-        sa.store(va, buffer(s, 0));                                // (what it held was read before the last barrier)
-        sb.store(vb, buffer(s, 1));
-        __syncthreads();
-        compute(s);
-    }
-    __syncthreads();
-    // the tile as rows of TB floats, quad i of row q at i ^ q: sixteen rows' quads of a fragment spread over the banks
-    constexpr int QUADS = TB / 4;
-    floatx4 *const sums = reinterpret_cast<floatx4 *>(lds);
-#pragma unroll
-    for (int j = 0; j < F; ++j)
-#pragma unroll
-        for (int i = 0; i < F; ++i) {
-            const int q = wq + 16 * j + (lane & 15), quad = (wp + 16 * i) / 4 + (lane >> 4);
-            sums[q * QUADS + (quad ^ (q & (QUADS - 1)))] = acc[i][j];
-        }
-    __syncthreads();
-    const int64_t left_q = m.Q - q0;
-#pragma unroll 2
-    for (int i = threadIdx.x; i < TB * QUADS; i += BLOCK) {
-        const int q = i / QUADS, quad = i % QUADS;
-        const int64_t p = p0 + quad * 4;
-        if (q >= left_q || p >= m.P) continue;
-        const floatx4 v = sums[q * QUADS + (quad ^ (q & (QUADS - 1)))];
-        if (!part) {
-            out(v, q0 + q, p);
-            continue;
-        }
-        float *const to = part + ((int64_t)split * m.Q + q0 + q) * m.P + p;
-        if ((m.P & 3) == 0) {
-            store4(to, v);
+        if constexpr (THIRDS) {
+            if (whole > 0) ask(0);
+            for (; s < whole; ++s) {
+                wait_and_meet<0>();                                // (step s is there, step s - 1 has been read by all)
+                if (s + 1 < whole) ask(s + 1);
+                products_of_thirds(lds + (s & 1) * BUFFER);
+            }
         } else {
+            // Half a step's products run while the other half's fragments, or the next step's first, are read:
+            //   products of (s, 0), reads of (s, 1)  |  step s + 1 is there, step s has been read by all: step s + 2 is asked for  |  products of (s, 1), reads of (s + 1, 0)
+            constexpr int READS = FP * (ACOLS ? (sizeof(T) == 4 ? 4 : 2) : 1) + FQ * (BCOLS ? (sizeof(T) == 4 ? 4 : 2) : 1), PRODUCTS = FP * FQ * (sizeof(T) == 4 ? 4 : 1);
+            if (whole > 0) {
+                ask(0);
+                if (whole > 1) {
+                    ask(1);
+                    wait_and_meet<LOADS>();
+                } else {
+                    wait_and_meet<0>();
+                }
+                read(0, lds, 0);
+            }
+            for (; s < whole; ++s) {
+                wait_for_lds();                                    // (before the next reads, not behind the first of them)
+                issue_loads_first();
+                read(1, lds + (s & 1) * BUFFER, 1);
+                products(0);
+                in_turn<READS, PRODUCTS>();
+                wait_and_meet<0>();
+                if (s + 2 < whole) ask(s + 2);
+                issue_loads_first();
+                read(0, lds + (~s & 1) * BUFFER, 0);               // (behind the last step: what the buffer held, for nobody)
+                products(1);
+                in_turn<READS, PRODUCTS>();
+                issue_loads_first();
+            }
+        }
+    }
+    // Steps first .. n - 1 through registers.
+    auto through_registers = [&](int first, bool in_thirds) {
+        if (first >= n) return;
+        uintx4 va[StageA::N], vb[StageB::N];
+        sa.load(first, va);
+        sb.load(first, vb);
+        __syncthreads();
+        for (int t = first; t < n; ++t) {
+            char *const at = lds + (t & 1) * BUFFER;               // (what it held was read before the last barrier)
+            sa.store(va, at);
+            sb.store(vb, at + BP * RB);
+            __syncthreads();
+            if (t + 1 < n) {
+                sa.load(t + 1, va);
+                sb.load(t + 1, vb);
+            }
+            if (THIRDS && in_thirds) {
+                products_of_thirds(at);
+            } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (p + e < m.P) to[e] = v[e];
+                for (int half = 0; half < 2; ++half) {
+                    read(0, at, half);
+                    products(0);
+                }
+            }
+        }
+    };
+    if constexpr (!THIRDS) {
+        through_registers(s, false);
+    } else {
+        // Thirds of an infinity are infinity and NaN: a tile whose sums are not finite is formed again by the float32 instructions.
+        through_registers(s, true);
+        float odd = 0.f;
+#pragma unroll
+        for (int i = 0; i < FP; ++i)
+#pragma unroll
+            for (int j = 0; j < FQ; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) odd = fmaf(acc[i][j][e], 0.f, odd);
+        if (__syncthreads_or(!(odd == 0.f))) {
+#pragma unroll
+            for (int i = 0; i < FP; ++i)
+#pragma unroll
+                for (int j = 0; j < FQ; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+            through_registers(0, false);
+        }
+    }
+    // the tile, or half of every wavefront's rows at a time, as rows of BP floats, quad i of row r at i ^ r: sixteen rows' quads of a fragment spread over the banks
+    constexpr int QUADS = BP / 4, TURNS = ROWS * QUADS / S::THREADS, U = 4;
+    floatx4 *const sums = reinterpret_cast<floatx4 *>(lds);
+    const int quad = threadIdx.x % QUADS;
+    const int64_t p = p0 + quad * 4, left = m.Q - q0;
+#pragma unroll
+    for (int pass = 0; pass < PASSES; ++pass) {
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < JS; ++j)
+#pragma unroll
+            for (int i = 0; i < FP; ++i) {
+                const int r = w / S::GP * (16 * JS) + 16 * j + (lane & 15), to = (wp + 16 * i) / 4 + (lane >> 4);
+                sums[r * QUADS + (to ^ (r & (QUADS - 1)))] = acc[i][pass * JS + j];
+            }
+        __syncthreads();
+        if (p >= m.P) continue;
+#pragma unroll 1
+        for (int u0 = 0; u0 < TURNS; u0 += U) {
+            floatx4 ahead[U];
+            int r[U], q[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                r[u] = (u0 + u) * (S::THREADS / QUADS) + threadIdx.x / QUADS;
+                q[u] = r[u] / (16 * JS) * WQ + pass * (16 * JS) + r[u] % (16 * JS);
+                if (q[u] < left && !part) ahead[u] = out.ask(q0 + q[u], p);
+            }
+            issue_loads_first();
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (q[u] >= left) continue;
+                const floatx4 v = sums[r[u] * QUADS + (quad ^ (r[u] & (QUADS - 1)))];
+                if (!part) {
+                    out(v, q0 + q[u], p, ahead[u]);
+                    continue;
+                }
+                float *const to = part + ((int64_t)split * m.Q + q0 + q[u]) * m.P + p;
+                if ((m.P & 3) == 0) {
+                    store4(to, v);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (p + e < m.P) to[e] = v[e];
+                }
+            }
         }
     }
 }
@@ -366,7 +560,7 @@ __global__ __launch_bounds__(BLOCK) void k_linear_finish(const float *__restrict
                 if (col + e < cols) v[e] += p[s * n + e];
         }
     }
-    out(v, row, col);
+    out(v, row, col, out.ask(row, col));
 }
 
 // ---- few rows ----------------------------------------------------------------------------------------------------------------------
@@ -417,12 +611,13 @@ __global__ __launch_bounds__(FEW_WAVES *WAVE) void k_linear_few(const T *__restr
 #pragma unroll
         for (int i = 1; i < FEW_WAVES; ++i) v += meet[i][j][lane];
         const int64_t q = 16 * j + c, col = p0 + 4 * g;
-        if (q < Q && col < P) out(v, q, col);
+        if (q < Q && col < P) out(v, q, col, out.ask(q, col));
     }
 }
 
 // ---- the gradient before the products ------------------------------------------------------------------------------------------
-// g = dy dropout' act'(a), and the sums of its columns: bound by memory, dy and a read and g written once.  A workgroup has 64 lanes' columns (four each) and
+// g = dy keep act'(a), keep 0 or 1, and the sums of its columns: bound by memory, dy and a read and g written once.  What dropout divides by is left to the products and
+// the sums, in 32 bits: without an activation, and with relu, g is dy where it is not 0, and nothing is rounded.  A workgroup has 64 lanes' columns (four each) and
 // every parts-th four rows; its wavefronts meet in LDS, the workgroups in k_linear_sums, in a fixed order.
 template <typename T>
 __global__ __launch_bounds__(BLOCK) void k_linear_grad(const T *dy, const T *__restrict__ kept, int kept_is_result, T *g, float *__restrict__ part, int64_t rows,
@@ -457,10 +652,7 @@ __global__ __launch_bounds__(BLOCK) void k_linear_grad(const T *dy, const T *__r
         for (int u = 0; u < U; ++u) {
             const int64_t r = row + u * stride, at = r * cols + col;
             if (r >= rows || col >= cols) continue;
-            if (drop.thr) {
-                if (kept_is_result) v[u] *= drop.inv;              // (what was dropped is 0 in the result)
-                else v[u] = dropped(v[u], drop_words((uint64_t)at, drop), drop);
-            }
+            if (drop.thr && !kept_is_result) v[u] = dropped(v[u], drop_words((uint64_t)at, drop), drop);      // (what was dropped is 0 in the result; drop.inv is 1)
             if (act != BPT_ACT_NONE) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) v[u][e] = activated_back(v[u][e], a[u][e], act);
@@ -489,20 +681,29 @@ __global__ __launch_bounds__(BLOCK) void k_linear_grad(const T *dy, const T *__r
         if (col + e < cols) part[(int64_t)blockIdx.y * cols + col + e] = sum[e];
 }
 // 16 columns a workgroup, sixteen lanes a column take parts p, p + 16, ...; the sixteen are added in their order
-template <typename T> __global__ __launch_bounds__(BLOCK) void k_linear_sums(const float *__restrict__ part, int parts, T *__restrict__ out, int64_t cols) {
+template <typename T> __global__ __launch_bounds__(BLOCK) void k_linear_sums(const float *__restrict__ part, int parts, T *__restrict__ out, int64_t cols, float scale) {
     __shared__ float meet[16][17];
     const int c = threadIdx.x & 15, k = threadIdx.x >> 4;
     const int64_t at = (int64_t)blockIdx.x * 16 + c;
     float v = 0.f;
-    if (at < cols)
-        for (int p = k; p < parts; p += 16) v += part[(int64_t)p * cols + at];
+    if (at < cols) {
+        int p = k;
+        for (; p + 15 * 16 < parts; p += 16 * 16) {
+            float t[16];
+#pragma unroll
+            for (int u = 0; u < 16; ++u) t[u] = part[(int64_t)(p + u * 16) * cols + at];
+#pragma unroll
+            for (int u = 0; u < 16; ++u) v += t[u];
+        }
+        for (; p < parts; p += 16) v += part[(int64_t)p * cols + at];
+    }
     meet[k][c] = v;
     __syncthreads();
     if (k != 0 || at >= cols) return;
     v = meet[0][c];
 #pragma unroll
     for (int i = 1; i < 16; ++i) v += meet[i][c];
-    Elem<T>::st(out + at, v);
+    Elem<T>::st(out + at, v * scale);
 }
 
 // ---- dropout -----------------------------------------------------------------------------------------------------------------------
@@ -573,52 +774,72 @@ inline bool on(std::initializer_list<const void *> ps, uintptr_t bytes) {
     return true;
 }
 
-// Which tiles, and into how many shares the reduction goes.
-struct Choice { int tb, splits; };
-inline Choice choose(int64_t P, int64_t Q, int64_t R, int step) {
-    const int64_t steps = ceil_div(R, step), big = ceil_div(P, 128) * ceil_div(Q, 128), small = ceil_div(P, 64) * ceil_div(Q, 64);
-    if (big >= 256) return Choice{128, 1};
-    if (steps >= 64) return Choice{128, (int)std::min<int64_t>(steps / 16, ceil_div(512, big))};
-    if (small >= 256 || steps < 8) return Choice{64, 1};
-    return Choice{64, (int)std::min<int64_t>(steps / 4, ceil_div(512, small))};
+// Which tiles, and into how many shares the reduction goes.  256 x 256: one workgroup a compute unit, LDS and caches are asked for least, but nothing runs beside its
+// start and end: where a round of the chip is filled (or, by shares, a long reduction fills it) and those are a small part.  128 x 128: two a unit.  64 x 64: where these would
+// leave units idle.  us, by 256 | 128 | 64, bfloat16 (forward of rows x inner -> outer): 65535 x 4096 -> 1024 456 | 597 | 908, 8192 x 4096 -> 4096 221 | 284 | 570, 16383 x 512 -> 2048 53 | 54 | 63,
+// 16383 x 2048 -> 512 73 | 39 | 50, 2000 x 512 -> 2048 24 | 12.6 | 10.6, 1023 x 512 -> 512 24 | 11 | 8.9; dweight (shares) of 65535 x 4096 -> 1024 460 | 571 | 1239, of 16383 x 512 -> 2048
+// 76 | 48 | 68; float32 4096 x 4096 -> 4096 600 | 688 | 911, 16383 x 512 -> 2048 195 | 200 | 242, 1023 x 512 -> 512 78 | 22 | 15.
+typedef Shape<256, 256, 4, 2, 1> Huge;
+typedef Shape<128, 128, 2, 2, 2> Large;
+typedef Shape<64, 64, 2, 2, 4> Small;
+enum Tiles { HUGE, LARGE, SMALL };
+struct Choice {
+    Tiles tiles;
+    int splits;
+};
+template <typename T> inline Choice choose(int64_t P, int64_t Q, int64_t R) {
+    auto count = [&](int64_t b) { return ceil_div(P, b) * ceil_div(Q, b); };
+    const int64_t steps = ceil_div(R, 128 / (int64_t)sizeof(T)), huge = count(256), large = count(128), small = count(64);
+    if (R >= 1024 && huge >= 192 && 4 * huge >= 3 * 256 * ceil_div(huge, 256)) return Choice{HUGE, 1};
+    if (steps >= 512 && huge >= 32 && huge < 192) return Choice{HUGE, (int)(256 / huge)};
+    const int64_t large_splits = std::max<int64_t>(1, std::min<int64_t>(steps / 8, 512 / large)), small_splits = std::max<int64_t>(1, std::min<int64_t>(steps / 4, 512 / small));
+    if (large * large_splits >= 384) return Choice{LARGE, (int)large_splits};
+    return Choice{SMALL, (int)small_splits};
 }
-template <typename T> inline Product product(int64_t P, int64_t Q, int64_t R, int64_t lda, int64_t ldb, Choice &ch) {
-    ch = choose(P, Q, R, step<T>());
-    Product m{P, Q, R, lda, ldb, 0, 0, 0, 0, 0};
-    m.tiles_p = (int)ceil_div(P, ch.tb);
-    m.tiles = (int)(m.tiles_p * ceil_div(Q, ch.tb));
-    m.steps = (int)ceil_div(R, step<T>());
-    m.per_split = (int)ceil_div(m.steps, ch.splits);
-    m.splits = (int)ceil_div(m.steps, m.per_split);
-    return m;
+// f(shape) of a choice
+template <typename T, typename F> inline auto with_shape(Tiles tiles, F &&f) {
+    if (tiles == HUGE) return f(Huge{});
+    return tiles == LARGE ? f(Large{}) : f(Small{});
+}
+template <typename T> inline Product product(int64_t P, int64_t Q, int64_t R, int64_t lda, int64_t ldb, const Choice &ch) {
+    return with_shape<T>(ch.tiles, [&](auto shape) {
+        typedef decltype(shape) S;
+        Product m{P, Q, R, lda, ldb, 0, 0, 0, 0, 0};
+        m.tiles_p = (int)ceil_div(P, S::BP);
+        m.tiles = (int)(m.tiles_p * ceil_div(Q, S::BQ));
+        m.steps = (int)ceil_div(R, step<T, S::RB>());
+        m.per_split = (int)ceil_div(m.steps, ch.splits);
+        m.splits = (int)ceil_div(m.steps, m.per_split);
+        return m;
+    });
 }
 template <typename T> inline int64_t product_workspace(int64_t P, int64_t Q, int64_t R) {
-    Choice ch;
-    const Product m = product<T>(P, Q, R, 0, 0, ch);
+    const Product m = product<T>(P, Q, R, 0, 0, choose<T>(P, Q, R));
     return m.splits > 1 ? (int64_t)m.splits * P * Q * 4 : 0;
 }
 
-template <typename T, int TB, bool AC, bool BC> int launch_tiles(const T *a, const T *b, const Product &m, const Epilogue<T> &out, float *part, hipStream_t s) {
-    // (a lane's offsets into a step count 32 bits: 128 rows of 2^22 elements)
-    const bool direct = on({a, b}, 16) && m.lda % ve<T>() == 0 && m.ldb % ve<T>() == 0 && std::max(m.lda, m.ldb) <= (int64_t)1 << 22;
-    const dim3 grid((unsigned)(m.tiles * (int64_t)m.splits));
-    if (direct) hipLaunchKernelGGL((k_linear_tiles<T, TB, AC, BC, true>), grid, dim3(BLOCK), 0, s, a, b, m, out, part);
-    else hipLaunchKernelGGL((k_linear_tiles<T, TB, AC, BC, false>), grid, dim3(BLOCK), 0, s, a, b, m, out, part);
-    return launch_status();
-}
 // out's rows and columns are the product's
 template <typename T, bool AC, bool BC>
 int run_product(const T *a, const T *b, int64_t P, int64_t Q, int64_t R, int64_t lda, int64_t ldb, const Epilogue<T> &out, void *ws, hipStream_t s) {
-    Choice ch;
+    const Choice ch = choose<T>(P, Q, R);
     const Product m = product<T>(P, Q, R, lda, ldb, ch);
     float *const part = m.splits > 1 ? (float *)ws : nullptr;
-    const int st = ch.tb == 128 ? launch_tiles<T, 128, AC, BC>(a, b, m, out, part, s) : launch_tiles<T, 64, AC, BC>(a, b, m, out, part, s);
+    // Straight to LDS: rows that start on 4 bytes, as loads of several words do (33598 x 300 -> 600 bfloat16, through registers / straight: forward 55 / 53 us, dx 64 / 40, dweight 79 / 31), and hold
+    // a vector at least; a lane's offsets into a step count 32 bits (256 rows of 2^21 elements).
+    const bool direct = on({a, b}, 4) && lda * sizeof(T) % 4 == 0 && ldb * sizeof(T) % 4 == 0 && std::min(lda, ldb) >= ve<T>() && std::max(lda, ldb) <= (int64_t)1 << 21;
+    const dim3 grid((unsigned)(m.tiles * (int64_t)m.splits));
+    const int st = with_shape<T>(ch.tiles, [&](auto shape) {
+        typedef decltype(shape) S;
+        if (direct) hipLaunchKernelGGL((k_linear_tiles<T, S, AC, BC, true, sizeof(T) == 4>), grid, dim3(S::THREADS), 0, s, a, b, m, out, part);
+        else hipLaunchKernelGGL((k_linear_tiles<T, S, AC, BC, false, sizeof(T) == 4>), grid, dim3(S::THREADS), 0, s, a, b, m, out, part);
+        return launch_status();
+    });
     if (st != BPT_OK || !part) return st;
     hipLaunchKernelGGL((k_linear_finish<T>), dim3((unsigned)ceil_div(Q * ceil_div(P, 4), BLOCK)), dim3(BLOCK), 0, s, part, m.splits, Q, P, out);
     return launch_status();
 }
-template <typename T> inline Epilogue<T> plain_epilogue(T *y, int64_t cols) {
-    return Epilogue<T>{nullptr, nullptr, y, nullptr, cols, BPT_ACT_NONE, make_drop(0.0, 0), cols % 4 == 0 && on({y}, 4 * sizeof(T))};
+template <typename T> inline Epilogue<T> plain_epilogue(T *y, int64_t cols, double scale) {
+    return Epilogue<T>{nullptr, nullptr, y, nullptr, cols, (float)scale, BPT_ACT_NONE, make_drop(0.0, 0), cols % 4 == 0 && on({y}, 4 * sizeof(T))};
 }
 
 constexpr int64_t FEW_ROWS = 64;
@@ -626,7 +847,7 @@ template <typename T>
 int run_forward(const void *x_, const void *w_, const void *b_, const void *r_, void *y_, void *kept_, void *ws, int64_t rows, int64_t inner, int64_t outer, int act,
                 Drop drop, hipStream_t s) {
     const T *x = (const T *)x_, *w = (const T *)w_;
-    const Epilogue<T> out{(const T *)b_, (const T *)r_, (T *)y_, (T *)kept_, outer, act, drop, outer % 4 == 0 && on({b_, r_, y_, kept_}, 4 * sizeof(T))};
+    const Epilogue<T> out{(const T *)b_, (const T *)r_, (T *)y_, (T *)kept_, outer, 1.f, act, drop, outer % 4 == 0 && on({b_, r_, y_, kept_}, 4 * sizeof(T))};
     if (rows <= FEW_ROWS) {
         const bool whole = inner % ve<T>() == 0 && on({x, w}, 16);
         const dim3 grid((unsigned)ceil_div(outer, 16)), block(FEW_WAVES * WAVE);
@@ -652,12 +873,14 @@ int run_grad(const void *dy_, const void *kept_, int result, void *g_, void *db_
     const int parts = grad_parts(rows, cols);
     const bool quads = cols % 4 == 0 && on({dy_, act != BPT_ACT_NONE ? kept_ : nullptr, g_}, 4 * sizeof(T));
     float *const part = db_ ? (float *)ws : nullptr;
+    const float inv = drop.inv;
+    drop.inv = 1.f;
     if (rows > 0)
         hipLaunchKernelGGL((k_linear_grad<T>), dim3((unsigned)ceil_div(cols, 4 * WAVE), parts), dim3(BLOCK), 0, s, (const T *)dy_, (const T *)kept_, result, (T *)g_, part,
                            rows, cols, act, drop, quads);
     const int st = launch_status();
     if (st != BPT_OK || !db_) return st;
-    hipLaunchKernelGGL((k_linear_sums<T>), dim3((unsigned)ceil_div(cols, 16)), dim3(BLOCK), 0, s, part, rows > 0 ? parts : 0, (T *)db_, cols);
+    hipLaunchKernelGGL((k_linear_sums<T>), dim3((unsigned)ceil_div(cols, 16)), dim3(BLOCK), 0, s, part, rows > 0 ? parts : 0, (T *)db_, cols, inv);
     return launch_status();
 }
 
@@ -723,8 +946,8 @@ int64_t bpt_linear_input_grad_workspace_bytes(int64_t rows, int64_t inner, int64
     return rows == 0 ? 0 : FOR_TYPE(product_workspace)(inner, rows, outer);
 }
 
-int bpt_linear_input_grad(const void *g, const void *weight, void *dx, void *workspace, int64_t workspace_bytes, int64_t rows, int64_t inner, int64_t outer, int dtype,
-                          void *stream) {
+int bpt_linear_input_grad(const void *g, const void *weight, void *dx, void *workspace, int64_t workspace_bytes, int64_t rows, int64_t inner, int64_t outer,
+                          double scale, int dtype, void *stream) {
     if (!is_type(dtype)) return BPT_ERR_DTYPE;
     if (!is_size(rows, inner, outer) || outer < 1) return BPT_ERR_SIZE;
     if (rows == 0) return BPT_OK;
@@ -733,8 +956,8 @@ int bpt_linear_input_grad(const void *g, const void *weight, void *dx, void *wor
     if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace))) return BPT_ERR_WORKSPACE;
     hipStream_t s = (hipStream_t)stream;
     if (dtype == BPT_F32)
-        return run_product<float, true, false>((const float *)weight, (const float *)g, inner, rows, outer, inner, outer, plain_epilogue((float *)dx, inner), workspace, s);
-    return run_product<bf16_t, true, false>((const bf16_t *)weight, (const bf16_t *)g, inner, rows, outer, inner, outer, plain_epilogue((bf16_t *)dx, inner), workspace, s);
+        return run_product<float, true, false>((const float *)weight, (const float *)g, inner, rows, outer, inner, outer, plain_epilogue((float *)dx, inner, scale), workspace, s);
+    return run_product<bf16_t, true, false>((const bf16_t *)weight, (const bf16_t *)g, inner, rows, outer, inner, outer, plain_epilogue((bf16_t *)dx, inner, scale), workspace, s);
 }
 
 int64_t bpt_linear_weight_grad_workspace_bytes(int64_t rows, int64_t inner, int64_t outer, int dtype) {
@@ -742,8 +965,8 @@ int64_t bpt_linear_weight_grad_workspace_bytes(int64_t rows, int64_t inner, int6
     return outer == 0 ? 0 : FOR_TYPE(product_workspace)(inner, outer, rows);
 }
 
-int bpt_linear_weight_grad(const void *g, const void *x, void *dweight, void *workspace, int64_t workspace_bytes, int64_t rows, int64_t inner, int64_t outer, int dtype,
-                           void *stream) {
+int bpt_linear_weight_grad(const void *g, const void *x, void *dweight, void *workspace, int64_t workspace_bytes, int64_t rows, int64_t inner, int64_t outer,
+                           double scale, int dtype, void *stream) {
     if (!is_type(dtype)) return BPT_ERR_DTYPE;
     if (!is_size(rows, inner, outer) || rows < 1) return BPT_ERR_SIZE;
     if (outer == 0) return BPT_OK;
@@ -752,8 +975,8 @@ int bpt_linear_weight_grad(const void *g, const void *x, void *dweight, void *wo
     if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace))) return BPT_ERR_WORKSPACE;
     hipStream_t s = (hipStream_t)stream;
     if (dtype == BPT_F32)
-        return run_product<float, true, true>((const float *)x, (const float *)g, inner, outer, rows, inner, outer, plain_epilogue((float *)dweight, inner), workspace, s);
-    return run_product<bf16_t, true, true>((const bf16_t *)x, (const bf16_t *)g, inner, outer, rows, inner, outer, plain_epilogue((bf16_t *)dweight, inner), workspace, s);
+        return run_product<float, true, true>((const float *)x, (const float *)g, inner, outer, rows, inner, outer, plain_epilogue((float *)dweight, inner, scale), workspace, s);
+    return run_product<bf16_t, true, true>((const bf16_t *)x, (const bf16_t *)g, inner, outer, rows, inner, outer, plain_epilogue((bf16_t *)dweight, inner, scale), workspace, s);
 }
 
 int bpt_dropout(const void *x, const void *residual, void *y, int64_t n, double dropout_p, uint64_t seed, int dtype, void *stream) {

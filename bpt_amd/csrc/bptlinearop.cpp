@@ -98,6 +98,7 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
         c10::DeviceGuard guard(x.device());
         const int dt = dtype_code(x);
         void *const stream = stream_of(x);
+        const double scale = 1.0 / (1.0 - p);
         Tensor g = dy;
         const bool changes = act != BPT_ACT_NONE || p > 0.0;
         if (changes && (need_x || need_w)) g = at::empty_like(dy);
@@ -114,7 +115,7 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
             if (n.outer > 0) {
                 const int64_t bytes = bpt_linear_input_grad_workspace_bytes(n.rows, n.inner, n.outer, dt);
                 const Tensor ws = workspace(bytes, x);
-                check_status(bpt_linear_input_grad(ptr(g), ptr(w), ptr(out[0]), ptr(ws), bytes, n.rows, n.inner, n.outer, dt, stream), "linear_act's backward");
+                check_status(bpt_linear_input_grad(ptr(g), ptr(w), ptr(out[0]), ptr(ws), bytes, n.rows, n.inner, n.outer, scale, dt, stream), "linear_act's backward");
             }
         }
         if (need_w) {
@@ -122,7 +123,7 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
             if (n.rows > 0) {
                 const int64_t bytes = bpt_linear_weight_grad_workspace_bytes(n.rows, n.inner, n.outer, dt);
                 const Tensor ws = workspace(bytes, x);
-                check_status(bpt_linear_weight_grad(ptr(g), ptr(x), ptr(out[1]), ptr(ws), bytes, n.rows, n.inner, n.outer, dt, stream), "linear_act's backward");
+                check_status(bpt_linear_weight_grad(ptr(g), ptr(x), ptr(out[1]), ptr(ws), bytes, n.rows, n.inner, n.outer, scale, dt, stream), "linear_act's backward");
             }
         }
         return out;

@@ -25,21 +25,22 @@ int bpt_linear_forward(const void *x, const void *weight, const void *bias, cons
                        int64_t workspace_bytes, int64_t rows, int64_t inner, int64_t outer, int act, double dropout_p, uint64_t seed, int dtype,
                        void *stream);
 
-/* g = dy dropout' act'(a), (rows, outer), and where dbias is not NULL its sums over the rows; the workspace is for these.  g may be NULL, and may be dy.
+/* g = dy act'(a) where dropout keeps the element, 0 elsewhere, (rows, outer), and where dbias is not NULL its sums over the rows divided by 1 - dropout_p; the workspace
+ * is for these.  g is not divided: the two products below take 1 / (1 - dropout_p) as scale.  g may be NULL, and may be dy.
  * kept: the forward's kept tensor, or, with BPT_ACT_RELU and kept_is_result, its y (which had no residual); not read without an activation. */
 int64_t bpt_linear_grad_workspace_bytes(int64_t rows, int64_t outer, int dtype);
 int bpt_linear_grad(const void *dy, const void *kept, int kept_is_result, void *g, void *dbias, void *workspace, int64_t workspace_bytes,
                     int64_t rows, int64_t outer, int act, double dropout_p, uint64_t seed, int dtype, void *stream);
 
-/* dx = g weight, (rows, inner). */
+/* dx = scale g weight, (rows, inner). */
 int64_t bpt_linear_input_grad_workspace_bytes(int64_t rows, int64_t inner, int64_t outer, int dtype);
 int bpt_linear_input_grad(const void *g, const void *weight, void *dx, void *workspace, int64_t workspace_bytes, int64_t rows, int64_t inner,
-                          int64_t outer, int dtype, void *stream);
+                          int64_t outer, double scale, int dtype, void *stream);
 
-/* dweight = g^T x, (outer, inner). */
+/* dweight = scale g^T x, (outer, inner). */
 int64_t bpt_linear_weight_grad_workspace_bytes(int64_t rows, int64_t inner, int64_t outer, int dtype);
 int bpt_linear_weight_grad(const void *g, const void *x, void *dweight, void *workspace, int64_t workspace_bytes, int64_t rows, int64_t inner,
-                           int64_t outer, int dtype, void *stream);
+                           int64_t outer, double scale, int dtype, void *stream);
 
 /* y = residual + dropout(x), n elements; residual may be NULL.  y may be x or residual.  The gradient of x is the same call on dy without a residual. */
 int bpt_dropout(const void *x, const void *residual, void *y, int64_t n, double dropout_p, uint64_t seed, int dtype, void *stream);

@@ -2,10 +2,10 @@
 
   bpt_amd/csrc/libbptgraph.so  host C++ (g++)            <- bptgraph.cpp
   bpt_amd/csrc/libbptattn.so   gfx950 HIP (hipcc)        <- bptattn.hip, bpttiles.h
-  bpt_amd/csrc/libbptscore.so  gfx950 HIP (hipcc)        <- bptscore.hip, bpttiles.h  (attention with capped scores and distance)
+  bpt_amd/csrc/libbptscore.so  gfx950 HIP (hipcc)        <- bptscore.hip, bptmod.h, bpttiles.h  (attention with capped scores and distance)
   bpt_amd/csrc/libbptblock.so  gfx950 HIP (hipcc)        <- bptblock.hip, bpttiles.h  (layer norm of a sum, relu kept in 8 bits)
   bpt_amd/csrc/libbptlinear.so gfx950 HIP (hipcc)       <- bptlinear.hip, bpttiles.h  (matrix products with an epilogue, dropout)
-  bpt_amd/csrc/libbptbias.so   gfx950 HIP (hipcc)        <- bptbias.hip, bpttiles.h  (bias of scores by buckets)
+  bpt_amd/csrc/libbptbias.so   gfx950 HIP (hipcc)        <- bptbias.hip, bptmod.h, bpttiles.h  (bias of scores by buckets)
   bpt_amd/csrc/libbptplan.so   gfx950 HIP (hipcc)        <- bptplan.hip  (plans built on the GPU; rocPRIM headers)
   bpt_amd/csrc/bptop.so        host C++ (g++, torch)     <- bptop.cpp, bptblockop.cpp, bptlinearop.cpp, bpthost.h  (host side of the ops and their autograd; links them)
 
@@ -30,7 +30,7 @@ HIP_FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",
     # packed FP32 forms (v_pk_*_f32) are kept out of the generated code on purpose
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
-    "-Wall", "-Wno-unused-variable", "-Wno-unused-but-set-variable",
+    "-Wall", "-Wno-unused-variable", "-Wno-unused-but-set-variable", "-Wno-inline-asm",
 ]
 
 
@@ -97,7 +97,7 @@ def build_op(verbose=True):
     _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-DTORCH_EXTENSION_NAME=bptop",
           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM"]
          + [f"-I{p}" for p in include] + [os.path.join(CSRC, "bptop.cpp"), os.path.join(CSRC, "bptblockop.cpp"), os.path.join(CSRC, "bptlinearop.cpp"), "-o", OP_SO, f"-L{libs}", f"-L{CSRC}",
-                                          "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python", "-ltorch", "-l:libbptattn.so", "-l:libbptplan.so", "-l:libbptscore.so", "-l:libbptblock.so", "-l:libbptlinear.so", "-Wl,-rpath,$ORIGIN"], verbose)
+                                          "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python", "-ltorch", "-l:libbptattn.so", "-l:libbptplan.so", "-l:libbptscore.so", "-l:libbptblock.so", "-l:libbptlinear.so", "-l:libbptbias.so", "-Wl,-rpath,$ORIGIN"], verbose)
     return OP_SO
 
 

@@ -134,8 +134,12 @@ BIAS_API = {
     "bpt_bucket_bias_forward": (ctypes.c_int, [c_vp] * 3 + _bias_tail + [ctypes.c_int] * 3 + [c_vp]),
     "bpt_bucket_bias_backward_workspace_bytes": (c_i64, [c_i64, c_i64, ctypes.c_int, ctypes.c_int]),
     "bpt_bucket_bias_backward": (ctypes.c_int, [c_vp] * 4 + [c_i64] + _bias_tail + [ctypes.c_int] * 2 + [c_vp]),
-    "bpt_bucket_pairs_forward": (ctypes.c_int, [c_vp] * 5 + _bias_tail + [ctypes.c_int, c_vp]),
-    "bpt_bucket_pairs_backward": (ctypes.c_int, [c_vp] * 4 + [c_i64] + _bias_tail + [ctypes.c_int, c_vp]),
+    "bpt_bucket_prepare_bytes": (c_i64, [_PP, _PP, ctypes.c_int]),
+    "bpt_bucket_prepare": (ctypes.c_int, [_PP, _PP, c_vp, c_vp, c_i64, ctypes.c_int, ctypes.c_int, ctypes.c_float, ctypes.c_int, c_vp, c_vp]),
+    "bpt_bucket_attention_forward": (ctypes.c_int, [_PP, _PS] + [c_vp] * 7 + [c_i64, ctypes.c_float, ctypes.c_float, ctypes.c_uint64, ctypes.c_int, ctypes.c_int, c_vp]),
+    "bpt_bucket_attention_backward_workspace_bytes": (c_i64, [_PP, _PP, c_i64] + [ctypes.c_int] * 3),
+    "bpt_bucket_attention_backward": (ctypes.c_int, [_PP, _PP, _PS] + [c_vp] * 13 + [c_i64, c_i64, ctypes.c_int, ctypes.c_float, ctypes.c_float, ctypes.c_uint64,
+                                                                                 ctypes.c_int, ctypes.c_int, c_vp]),
 }
 
 _graph = None

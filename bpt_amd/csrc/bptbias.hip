@@ -1,5 +1,6 @@
-// libbptbias: gfx950 kernels of a learned bias of attention scores by buckets, and its gradient (C ABI in include/bptbias.h).
-#include "bpttiles.h"
+// libbptbias: gfx950 kernels of a learned bias of attention scores by buckets, and its gradient: the separate operator, and the fused attention, whose tile kernels
+// (bpttiles.h) have BUCKETS forms (C ABI in include/bptbias.h).
+#include "bptmod.h"
 
 #include "../../include/bptbias.h"
 
@@ -18,24 +19,6 @@ __global__ __launch_bounds__(BLOCK) void k_bucket_rows(const T *__restrict__ tab
     Elem<O>::st(bias + i, (uint64_t)b < (uint64_t)n_buckets ? (A)Elem<T>::ld(table + b * h + head) * factor : A(0));
 }
 
-// ---- the term in the order of a tile plan's pairs -------------------------------------------------------------------------------
-constexpr uint32_t NO_BUCKET = 65535;
-__global__ __launch_bounds__(BLOCK) void k_bucket_codes(const int64_t *__restrict__ buckets, const int32_t *__restrict__ eid_of_pair, uint16_t *__restrict__ codes,
-                                                        int64_t n_edges, int64_t n_buckets) {
-    const int64_t t = (int64_t)blockIdx.x * BLOCK + threadIdx.x;
-    if (t >= n_edges) return;
-    const int64_t b = buckets[eid_of_pair[t]];
-    codes[t] = (uint16_t)((uint64_t)b < (uint64_t)n_buckets ? (uint32_t)b : NO_BUCKET);
-}
-template <typename T>
-__global__ __launch_bounds__(BLOCK) void k_bucket_terms(const T *__restrict__ table, const uint16_t *__restrict__ codes, float *__restrict__ bias, int64_t n_edges, int h,
-                                                        float factor) {
-    const int64_t t = (int64_t)blockIdx.x * BLOCK + threadIdx.x;
-    if (t >= n_edges) return;
-    const uint32_t b = codes[t];
-    for (int head = 0; head < h; ++head) bias[(int64_t)head * n_edges + t] = b == NO_BUCKET ? 0.f : Elem<T>::ld(table + (int64_t)b * h + head) * factor;
-}
-
 // ---- its gradient --------------------------------------------------------------------------------------------------------------------
 // dtable[b][head] = factor sum over the edges of bucket b of ds[e][head]: bound by memory, ds and the buckets read once.  A lane owns a column of
 // sums in LDS, one a bucket, so nobody shares an address and the order of every sum is fixed: lanes of one head, wavefronts, workgroups
@@ -43,14 +26,12 @@ __global__ __launch_bounds__(BLOCK) void k_bucket_terms(const T *__restrict__ ta
 // Up to SUMS_WIDE buckets a workgroup of four wavefronts has them all (64 KB at 64); of more, one wavefront has 256 and the
 // edges are walked once for each 256.
 constexpr int SUMS_WIDE = 64, SUMS_LONG = 256;
-// In the order of pairs ds is (h, n_edges): a workgroup has one head, a lane a pair.
-template <typename D, typename A, typename B, int WAVES, int ROOM>
-__global__ __launch_bounds__(WAVES *WAVE) void k_bucket_sums(const D *__restrict__ ds, const B *__restrict__ buckets, A *__restrict__ part, int64_t n_edges,
+template <typename D, typename A, int WAVES, int ROOM>
+__global__ __launch_bounds__(WAVES *WAVE) void k_bucket_sums(const D *__restrict__ ds, const int64_t *__restrict__ buckets, A *__restrict__ part, int64_t n_edges,
                                                              int64_t n_buckets, int h) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     A *const sums = reinterpret_cast<A *>(lds) + (size_t)(threadIdx.x >> 6) * ROOM * WAVE;
-    constexpr bool PAIRS = sizeof(B) == 2;
-    const int lane = threadIdx.x & 63, h0 = (int)blockIdx.y * (PAIRS ? 1 : WAVE), heads = PAIRS ? 1 : min(h - h0, WAVE), per = WAVE / heads, mine = lane / heads;
+    const int lane = threadIdx.x & 63, h0 = (int)blockIdx.y * WAVE, heads = min(h - h0, WAVE), per = WAVE / heads, mine = lane / heads;
     const int64_t b0 = (int64_t)blockIdx.z * ROOM;
     const int room = (int)min((int64_t)ROOM, n_buckets - b0);
     for (int b = 0; b < room; ++b) sums[b * WAVE + lane] = A(0);
@@ -63,8 +44,8 @@ __global__ __launch_bounds__(WAVES *WAVE) void k_bucket_sums(const D *__restrict
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const int64_t e = e0 + u * per + mine;
-                b[u] = e < n_edges ? (int64_t)buckets[e] - b0 : -1;
-                x[u] = e < n_edges ? (A)Elem<D>::ld(ds + (PAIRS ? h0 * n_edges + e : e * h + h0 + lane % heads)) : A(0);
+                b[u] = e < n_edges ? buckets[e] - b0 : -1;
+                x[u] = e < n_edges ? (A)Elem<D>::ld(ds + e * h + h0 + lane % heads) : A(0);
             }
             issue_loads_first();
 #pragma unroll
@@ -114,23 +95,147 @@ int run_rows(const void *table, const int64_t *buckets, void *bias, int64_t n_ed
                        (typename Elem<T>::acc_t)factor, spare);
     return launch_status();
 }
-template <typename D, typename T, typename B>
-int run_sums(const void *ds, const B *buckets, void *dtable, void *ws, int64_t n_edges, int64_t n_buckets, int h, double factor, hipStream_t s) {
+template <typename D, typename T>
+int run_sums(const void *ds, const int64_t *buckets, void *dtable, void *ws, int64_t n_edges, int64_t n_buckets, int h, double factor, hipStream_t s) {
     using A = typename Elem<D>::acc_t;
     const int parts = sums_parts(n_edges, h);
-    const unsigned chunks = sizeof(B) == 2 ? (unsigned)h : (unsigned)((h + WAVE - 1) / WAVE);
+    const unsigned chunks = (unsigned)((h + WAVE - 1) / WAVE);
     constexpr int WIDE = SUMS_WIDE * 4 / (int)sizeof(A), LONG = SUMS_LONG * 4 / (int)sizeof(A);
     if (n_buckets <= WIDE)
-        hipLaunchKernelGGL((k_bucket_sums<D, A, B, 4, WIDE>), dim3(parts, chunks, 1), dim3(4 * WAVE), 4 * WIDE * WAVE * sizeof(A), s, (const D *)ds, buckets, (A *)ws, n_edges,
+        hipLaunchKernelGGL((k_bucket_sums<D, A, 4, WIDE>), dim3(parts, chunks, 1), dim3(4 * WAVE), 4 * WIDE * WAVE * sizeof(A), s, (const D *)ds, buckets, (A *)ws, n_edges,
                            n_buckets, h);
     else
-        hipLaunchKernelGGL((k_bucket_sums<D, A, B, 1, LONG>), dim3(parts, chunks, (unsigned)((n_buckets + LONG - 1) / LONG)), dim3(WAVE), LONG * WAVE * sizeof(A), s,
+        hipLaunchKernelGGL((k_bucket_sums<D, A, 1, LONG>), dim3(parts, chunks, (unsigned)((n_buckets + LONG - 1) / LONG)), dim3(WAVE), LONG * WAVE * sizeof(A), s,
                            (const D *)ds, buckets, (A *)ws, n_edges, n_buckets, h);
     const int st = launch_status();
     if (st != BPT_OK) return st;
     hipLaunchKernelGGL((k_bucket_finish<T, A>), dim3((unsigned)((n_buckets * h + 15) / 16)), dim3(BLOCK), 0, s, (const A *)ws, parts, (T *)dtable, n_buckets * h, (A)factor);
     return launch_status();
 }
+
+// ---- the fused attention -----------------------------------------------------------------------------------------------------------
+// One byte a place says which of a head's biases a pair takes, so the passes read 1 / (4 h) of what the term itself would be (float32, h heads, each way), and nothing
+// of an edge's size is written but ds, which is summed up by buckets behind the backward: in float32 from the scratch that the sides hand over anyway, in bfloat16, whose
+// sides hand over none, from the source side's own, rounded to bfloat16 (2^-9 of each of the terms of sums of thousands).
+inline int64_t places(const bpt_plan *p) { return p->n_groups > 0 ? p->n_grp_entries * TILE_R : p->n_edges; }
+inline const int32_t *place_eids(const bpt_plan *p) { return p->n_groups > 0 ? p->grp_eids : p->eid; }
+inline int64_t table_bytes(int h) { return (int64_t)h * 256 * 4; }
+struct Prepared {
+    float *table;
+    uint8_t *codes_in, *codes_out;
+    Prepared(void *at, const bpt_plan *in, int h) : table((float *)at), codes_in((uint8_t *)at + table_bytes(h)), codes_out(codes_in + round16(places(in))) {}
+};
+
+// blockIdx.y: 0 the tables, 1 and 2 the places of either side, four a thread
+template <typename T>
+__global__ __launch_bounds__(BLOCK) void k_bucket_prepare(const T *__restrict__ table, const int64_t *__restrict__ buckets, int n_buckets, int heads, int h, float factor,
+                                                          int64_t n_edges, const int32_t *__restrict__ eids_in, int64_t n_in, const int32_t *__restrict__ eids_out,
+                                                          int64_t n_out, float *__restrict__ tables, uint8_t *__restrict__ codes_in, uint8_t *__restrict__ codes_out) {
+    const int64_t first = ((int64_t)blockIdx.x * BLOCK + threadIdx.x) * 4;
+    if (blockIdx.y == 0) {
+        for (int64_t i = first; i < first + 4 && i < (int64_t)h * 256; ++i) {
+            const int head = (int)(i >> 8), b = (int)i & 255;
+            tables[i] = head < heads && b < n_buckets ? Elem<T>::ld(table + (int64_t)b * heads + head) * factor : 0.f;
+        }
+        return;
+    }
+    const int32_t *const eids = blockIdx.y == 1 ? eids_in : eids_out;
+    uint8_t *const codes = blockIdx.y == 1 ? codes_in : codes_out;
+    const int64_t n = blockIdx.y == 1 ? n_in : n_out;
+    int64_t e[4], b[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) e[u] = first + u < n ? eids[first + u] : -1;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) b[u] = (uint64_t)e[u] < (uint64_t)n_edges ? buckets[e[u]] : -1;
+    uint32_t word = 0;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) word |= ((uint64_t)b[u] < (uint64_t)n_buckets ? (uint32_t)b[u] : (uint32_t)NO_BUCKET) << 8 * u;
+    if (first + 4 <= n) {
+        *reinterpret_cast<uint32_t *>(codes + first) = word;
+    } else {
+        for (int u = 0; u < 4; ++u)
+            if (first + u < n) codes[first + u] = (uint8_t)(word >> 8 * u);
+    }
+}
+
+// dtable's parts from ds at the places of a plan: a workgroup has one head, a lane a place and a column of sums in LDS, as k_bucket_sums.
+// float32: ds is the second of the pairs' (p, ds), [head][pair]; bfloat16: [head][place].
+template <typename T> struct PlaceDs { typedef float2 type; };
+template <> struct PlaceDs<bf16_t> { typedef bf16_t type; };
+template <typename T, int WAVES, int ROOM>
+__global__ __launch_bounds__(WAVES *WAVE) void k_bucket_places(const int4 *__restrict__ entries, const uint8_t *__restrict__ codes, const typename PlaceDs<T>::type *__restrict__ ds,
+                                                               int64_t n, int64_t n_edges, float *__restrict__ part, int n_buckets, int heads) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    float *const sums = reinterpret_cast<float *>(lds) + (threadIdx.x >> 6) * ROOM * WAVE;
+    const int lane = threadIdx.x & 63, head = (int)blockIdx.y, room = min(ROOM, n_buckets);
+    for (int b = 0; b < room; ++b) sums[b * WAVE + lane] = 0.f;
+    constexpr int U = 8;
+    const int64_t wave = (int64_t)blockIdx.x * WAVES + (threadIdx.x >> 6), waves = (int64_t)gridDim.x * WAVES;
+    for (int64_t i0 = wave * WAVE * U; i0 < n; i0 += waves * WAVE * U) {
+        int b[U];
+        float x[U];
+        int4 en[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t i = min(i0 + u * WAVE + lane, n - 1);
+            b[u] = i0 + u * WAVE + lane < n ? codes[i] : NO_BUCKET;
+            if constexpr (sizeof(T) == 4) en[u] = entries[i / TILE_R];
+        }
+        issue_loads_first();
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t i = min(i0 + u * WAVE + lane, n - 1);
+            if constexpr (sizeof(T) == 4) {
+                const int64_t pair = min((int64_t)tile_pair_number(en[u].z, en[u].y, (int)(i % TILE_R)), n_edges - 1);
+                x[u] = b[u] < room ? ds[(int64_t)head * n_edges + pair].y : 0.f;
+            } else {
+                x[u] = b[u] < room ? Elem<bf16_t>::ld(ds + (int64_t)head * n + i) : 0.f;
+            }
+        }
+        issue_loads_first();
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (b[u] < room) sums[b[u] * WAVE + lane] += x[u];
+    }
+    __syncthreads();
+    const float *const all = reinterpret_cast<const float *>(lds);
+    // a bucket a quarter of a wavefront: sixteen lanes add four columns of every wavefront's each, and meet in a fixed order
+    for (int b0 = 0; b0 < room; b0 += WAVES * 4) {
+        const int b = b0 + (int)threadIdx.x / 16, c = threadIdx.x & 15;
+        float v = 0.f;
+        if (b < room) {
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w)
+#pragma unroll
+                for (int u = 0; u < 4; ++u) v += all[((size_t)w * ROOM + b) * WAVE + 16 * u + c];
+        }
+        v = head_sum<16>(v);
+        if (b < room && c == 0) part[((int64_t)blockIdx.x * n_buckets + b) * heads + head] = v;
+    }
+}
+
+constexpr int PLACE_PARTS = 256;
+template <typename T>
+int run_places(const bpt_plan *P, const uint8_t *codes, const typename PlaceDs<T>::type *ds, int64_t n, float *part, T *dtable, int n_buckets, int heads, float factor, hipStream_t s) {
+    const int4 *const entries = (const int4 *)P->grp_entries;
+    // (512 places a turn and wavefront)
+    const int wide = n_buckets <= SUMS_WIDE, parts = (int)std::max<int64_t>(1, std::min<int64_t>(PLACE_PARTS, n / (512 * (wide ? 4 : 1)) + 1));
+    if (wide)
+        hipLaunchKernelGGL((k_bucket_places<T, 4, SUMS_WIDE>), dim3(parts, heads), dim3(4 * WAVE), 4 * SUMS_WIDE * WAVE * 4, s, entries, codes, ds, n, P->n_edges, part, n_buckets,
+                           heads);
+    else
+        hipLaunchKernelGGL((k_bucket_places<T, 1, SUMS_LONG>), dim3(parts, heads), dim3(WAVE), SUMS_LONG * WAVE * 4, s, entries, codes, ds, n, P->n_edges, part, n_buckets, heads);
+    const int st = launch_status();
+    if (st != BPT_OK) return st;
+    hipLaunchKernelGGL((k_bucket_finish<T, float>), dim3((unsigned)(((int64_t)n_buckets * heads + 15) / 16)), dim3(BLOCK), 0, s, part, parts, dtable,
+                       (int64_t)n_buckets * heads, factor);
+    return launch_status();
+}
+
+inline int64_t attention_bytes(const bpt_plan *in, const bpt_plan *out, int h, int dtype) {
+    return scratch_bytes(in, out, h, dtype, false) + slope_bytes(in, h) + split_bytes(in, h, dtype == BPT_BF16) + round16((in->n_slots + 2 * out->n_slots) * (int64_t)h * 64 * 4);
+}
+inline int64_t ds_bytes(const bpt_plan *out, int h, int dtype) { return dtype == BPT_BF16 ? round16(places(out) * h * 2) : 0; }
 
 inline bool is_type(int dtype) { return dtype == BPT_F32 || dtype == BPT_F64 || dtype == BPT_BF16; }
 inline bool is_size(int64_t n_edges, int64_t n_buckets, int h) {
@@ -166,35 +271,96 @@ int bpt_bucket_bias_backward(const void *ds, const int64_t *buckets, void *dtabl
     if (!dtable || (n_edges > 0 && (!ds || !buckets))) return BPT_ERR_NULL;
     if (!workspace || workspace_bytes < bpt_bucket_bias_backward_workspace_bytes(n_edges, n_buckets, h, dtype) || !aligned16(workspace)) return BPT_ERR_WORKSPACE;
     hipStream_t s = (hipStream_t)stream;
-    if (dtype == BPT_F64) return run_sums<double, double, int64_t>(ds, buckets, dtable, workspace, n_edges, n_buckets, h, factor, s);
-    if (dtype == BPT_F32) return run_sums<float, float, int64_t>(ds, buckets, dtable, workspace, n_edges, n_buckets, h, factor, s);
-    if (ds_dtype == BPT_F32) return run_sums<float, bf16_t, int64_t>(ds, buckets, dtable, workspace, n_edges, n_buckets, h, factor, s);
-    return run_sums<bf16_t, bf16_t, int64_t>(ds, buckets, dtable, workspace, n_edges, n_buckets, h, factor, s);
+    if (dtype == BPT_F64) return run_sums<double, double>(ds, buckets, dtable, workspace, n_edges, n_buckets, h, factor, s);
+    if (dtype == BPT_F32) return run_sums<float, float>(ds, buckets, dtable, workspace, n_edges, n_buckets, h, factor, s);
+    if (ds_dtype == BPT_F32) return run_sums<float, bf16_t>(ds, buckets, dtable, workspace, n_edges, n_buckets, h, factor, s);
+    return run_sums<bf16_t, bf16_t>(ds, buckets, dtable, workspace, n_edges, n_buckets, h, factor, s);
 }
 
-int bpt_bucket_pairs_forward(const void *table, const int64_t *buckets, const int32_t *eid_of_pair, uint16_t *codes, float *bias, int64_t n_edges, int64_t n_buckets,
-                             int h, double factor, int dtype, void *stream) {
+int64_t bpt_bucket_prepare_bytes(const bpt_plan *plan_in, const bpt_plan *plan_out, int h) {
+    if (!plan_in || h < 1 || h > 16) return -1;
+    return table_bytes(h) + round16(places(plan_in)) + (plan_out ? round16(places(plan_out)) : 0);
+}
+
+int bpt_bucket_prepare(const bpt_plan *plan_in, const bpt_plan *plan_out, const void *table, const int64_t *buckets, int64_t n_buckets, int heads, int h, float scale,
+                       int dtype, void *prepared, void *stream) {
     if (dtype != BPT_F32 && dtype != BPT_BF16) return BPT_ERR_DTYPE;
-    if (!is_size(n_edges, n_buckets, h) || n_buckets > NO_BUCKET) return BPT_ERR_SIZE;
-    if (n_edges == 0) return BPT_OK;
-    if (!table || !buckets || !eid_of_pair || !codes || !bias) return BPT_ERR_NULL;
+    if (n_buckets < 1 || n_buckets > BPT_MOST_BUCKETS || heads < 1 || heads > h || h > 16 || !(fabsf(scale) > 0.f && fabsf(scale) < INFINITY)) return BPT_ERR_SIZE;
+    for (const bpt_plan *p : {plan_in, plan_out}) {
+        if (p == plan_out && !p) continue;
+        const int st = check_plan(p, true);
+        if (st != BPT_OK) return st;
+        if (p->n_groups > 0 && (!p->grp_eids || p->grp_R != TILE_R)) return BPT_ERR_PLAN;
+    }
+    if (plan_out && plan_out->n_edges != plan_in->n_edges) return BPT_ERR_PLAN;
+    if (!table || !prepared || (plan_in->n_edges > 0 && !buckets)) return BPT_ERR_NULL;
+    if (!aligned16(prepared)) return BPT_ERR_UNSUPPORTED;
+    const Prepared pr(prepared, plan_in, h);
+    const int64_t in = places(plan_in), out = plan_out ? places(plan_out) : 0, most = std::max<int64_t>(std::max(in, out), h * 256);
+    const dim3 grid((unsigned)((most + 4 * BLOCK - 1) / (4 * BLOCK)), plan_out ? 3 : 2);
     hipStream_t s = (hipStream_t)stream;
-    const dim3 grid((unsigned)((n_edges + BLOCK - 1) / BLOCK));
-    hipLaunchKernelGGL(k_bucket_codes, grid, dim3(BLOCK), 0, s, buckets, eid_of_pair, codes, n_edges, n_buckets);
-    if (dtype == BPT_F32) hipLaunchKernelGGL((k_bucket_terms<float>), grid, dim3(BLOCK), 0, s, (const float *)table, codes, bias, n_edges, h, (float)factor);
-    else hipLaunchKernelGGL((k_bucket_terms<bf16_t>), grid, dim3(BLOCK), 0, s, (const bf16_t *)table, codes, bias, n_edges, h, (float)factor);
+    const int32_t *ei = place_eids(plan_in), *eo = plan_out ? place_eids(plan_out) : nullptr;
+    if (dtype == BPT_F32)
+        hipLaunchKernelGGL((k_bucket_prepare<float>), grid, dim3(BLOCK), 0, s, (const float *)table, buckets, (int)n_buckets, heads, h, 1.f / scale, plan_in->n_edges, ei, in,
+                           eo, out, pr.table, pr.codes_in, pr.codes_out);
+    else
+        hipLaunchKernelGGL((k_bucket_prepare<bf16_t>), grid, dim3(BLOCK), 0, s, (const bf16_t *)table, buckets, (int)n_buckets, heads, h, 1.f / scale, plan_in->n_edges, ei,
+                           in, eo, out, pr.table, pr.codes_in, pr.codes_out);
     return launch_status();
 }
 
-int bpt_bucket_pairs_backward(const float *ds, const uint16_t *codes, void *dtable, void *workspace, int64_t workspace_bytes, int64_t n_edges, int64_t n_buckets, int h,
-                              double factor, int dtype, void *stream) {
-    if (dtype != BPT_F32 && dtype != BPT_BF16) return BPT_ERR_DTYPE;
-    if (!is_size(n_edges, n_buckets, h) || n_buckets > NO_BUCKET) return BPT_ERR_SIZE;
-    if (!dtable || (n_edges > 0 && (!ds || !codes))) return BPT_ERR_NULL;
-    if (!workspace || workspace_bytes < bpt_bucket_bias_backward_workspace_bytes(n_edges, n_buckets, h, dtype) || !aligned16(workspace)) return BPT_ERR_WORKSPACE;
+int bpt_bucket_attention_forward(const bpt_plan *plan_in, const bpt_score *score, const void *prepared, const void *q, const void *k, const void *v, void *o, float *lse,
+                                 void *workspace, int64_t workspace_bytes, float scale, float dropout_p, uint64_t dropout_seed, int h, int dtype, void *stream) {
+    Narrow nw;
+    const int st = check_score(plan_in, score, h, 64, h, dtype, scale, dropout_p, nullptr, nw, true);
+    if (st != BPT_OK) return st;
+    if (plan_in->n_rows == 0) return BPT_OK;
+    if (!prepared || !q || !k || !v || !o || !lse) return BPT_ERR_NULL;
+    if (plan_in->n_groups > 0 && !plan_in->grp_eids) return BPT_ERR_PLAN;
+    if (!aligned16(workspace) || !on16({prepared, q, k, v, o})) return BPT_ERR_UNSUPPORTED;
+    const int64_t need = round16(plan_in->n_slots * ((int64_t)h * 64 + 2 * h) * 4);
+    if (need > 0 && (!workspace || workspace_bytes < need)) return BPT_ERR_WORKSPACE;
+    const Prepared pr(const_cast<void *>(prepared), plan_in, h);
+    const BucketArgs b{pr.codes_in, nullptr, pr.table, nullptr, 0};
+    const Dropout drop = make_dropout(dropout_p, dropout_seed);
+    DISPATCH((run_forward<T, H, true>(plan_in, score, q, k, v, nullptr, o, lse, workspace, scale, drop, (hipStream_t)stream, &b)))
+}
+
+int64_t bpt_bucket_attention_backward_workspace_bytes(const bpt_plan *plan_in, const bpt_plan *plan_out, int64_t n_buckets, int heads, int h, int dtype) {
+    if (!plan_in || !plan_out || h < 1 || h > 16 || heads < 1 || heads > h || n_buckets < 1 || n_buckets > BPT_MOST_BUCKETS || (dtype != BPT_F32 && dtype != BPT_BF16)) return -1;
+    return attention_bytes(plan_in, plan_out, h, dtype) + ds_bytes(plan_out, h, dtype) + (int64_t)PLACE_PARTS * n_buckets * heads * 4;
+}
+
+int bpt_bucket_attention_backward(const bpt_plan *plan_in, const bpt_plan *plan_out, const bpt_score *score, const void *prepared, const void *q, const void *k, const void *v,
+                                  const void *o, const void *d_o, const float *lse, void *dq, void *dk, void *dv, void *dtable, float *dslopes, void *workspace,
+                                  int64_t workspace_bytes, int64_t n_buckets, int heads, float scale, float dropout_p, uint64_t dropout_seed, int h, int dtype,
+                                  void *stream) {
+    Narrow nw;
+    int st = check_score(plan_in, score, h, 64, h, dtype, scale, dropout_p, nullptr, nw, false);
+    if (st != BPT_OK) return st;
+    st = check_plan(plan_out, true);
+    if (st != BPT_OK) return st;
+    if (n_buckets < 1 || n_buckets > BPT_MOST_BUCKETS || heads < 1 || heads > h || !(fabsf(scale) > 0.f)) return BPT_ERR_SIZE;
+    if (plan_in->n_edges != plan_out->n_edges) return BPT_ERR_PLAN;
+    if (plan_in->n_groups == 0 || !has_tiles(plan_out, h, 64, dtype == BPT_BF16 ? 2 : 4) || !plan_out->grp_pairs) return BPT_ERR_UNSUPPORTED;
+    if (!plan_in->grp_eids || !plan_out->grp_eids) return BPT_ERR_PLAN;
+    if (!prepared || !q || !k || !v || !o || !d_o || !lse || !dq || !dk || !dv || (dslopes && !score->slopes)) return BPT_ERR_NULL;
+    if (!aligned16(workspace) || !on16({prepared, q, k, v, o, d_o, dq, dk, dv})) return BPT_ERR_UNSUPPORTED;
+    if (!workspace || workspace_bytes < bpt_bucket_attention_backward_workspace_bytes(plan_in, plan_out, n_buckets, heads, h, dtype)) return BPT_ERR_WORKSPACE;
+    const Prepared pr(const_cast<void *>(prepared), plan_in, h);
+    char *const behind = (char *)workspace + attention_bytes(plan_in, plan_out, h, dtype);
+    const BucketArgs b{pr.codes_in, pr.codes_out, pr.table, dtable && dtype == BPT_BF16 ? (bf16_t *)behind : nullptr, places(plan_out)};
+    float *const part = (float *)(behind + ds_bytes(plan_out, h, dtype));
+    const Dropout drop = make_dropout(dropout_p, dropout_seed);
     hipStream_t s = (hipStream_t)stream;
-    if (dtype == BPT_F32) return run_sums<float, float, uint16_t>(ds, codes, dtable, workspace, n_edges, n_buckets, h, factor, s);
-    return run_sums<float, bf16_t, uint16_t>(ds, codes, dtable, workspace, n_edges, n_buckets, h, factor, s);
+    auto attention = [&]() -> int {
+        DISPATCH((run_backward<T, H, true>(plan_in, plan_out, score, q, k, v, nullptr, o, d_o, lse, dq, dk, dv, nullptr, dslopes, workspace, scale, drop, s, &b)))
+    };
+    st = attention();
+    if (st != BPT_OK || !dtable) return st;
+    if (dtype == BPT_F32)
+        return run_places<float>(plan_in, pr.codes_in, (const float2 *)workspace, places(plan_in), part, (float *)dtable, (int)n_buckets, heads, 1.f / scale, s);
+    return run_places<bf16_t>(plan_out, pr.codes_out, (const bf16_t *)behind, places(plan_out), part, (bf16_t *)dtable, (int)n_buckets, heads, 1.f / scale, s);
 }
 
 }  // extern "C"

@@ -30,6 +30,7 @@
 #include "../../include/bptattn.h"
 #include "../../include/bptbuild.h"
 #include "../../include/bptplan.h"
+#include "../../include/bptbias.h"
 #include "../../include/bptscore.h"
 
 namespace py = pybind11;
@@ -655,6 +656,98 @@ MaybeTensor score_attention(const MaybeTensor &row, const MaybeTensor &indptr_r,
     return ScoreAttention::apply(r0, r1, r2, r3, col, indptr_c, eid_c, indices_c, q, k, v, slopes, opt, e, *r, scale, p, (int64_t)seed, h);
 }
 
+// ---- fused attention with a bias by buckets, with score options or not: entries of score_attention ---------------------------------
+// table (n, heads <= h); prepared: what the passes take of it and of the buckets (bpt_bucket_prepare), made for either side where a backward follows
+struct BucketAttention : torch::autograd::Function<BucketAttention> {
+    static Tensor forward(torch::autograd::AutogradContext *ctx, const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &table, const MaybeTensor &slopes,
+                          const Tensor &prepared, const ScoreOptions &opt, const EntryPtr &e, const Tensor &o, const Tensor &lse, double scale, double p,
+                          int64_t seed, int64_t h) {
+        ctx->save_for_backward({q, k, v, o, lse, prepared, opt.slopes, opt.pos_q, opt.pos_k});
+        ctx->saved_data["entry"] = c10::IValue::make_capsule(c10::make_intrusive<RelHold>(e));
+        ctx->saved_data["cap"] = opt.cap;
+        ctx->saved_data["scale"] = scale;
+        ctx->saved_data["p"] = p;
+        ctx->saved_data["seed"] = seed;
+        ctx->saved_data["h"] = h;
+        ctx->saved_data["n_buckets"] = table.size(0);
+        ctx->saved_data["heads"] = table.size(1);
+        return o;
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
+        TORCH_CHECK(!at::GradMode::is_enabled(), "attention with a bias by buckets is not differentiable twice");
+        const auto t = ctx->get_saved_variables();
+        const Tensor &q = t[0], &k = t[1], &v = t[2], &o = t[3], &lse = t[4], &prepared = t[5];
+        const double scale = ctx->saved_data["scale"].toDouble(), p = ctx->saved_data["p"].toDouble();
+        const uint64_t seed = (uint64_t)ctx->saved_data["seed"].toInt();
+        const int64_t h = ctx->saved_data["h"].toInt(), n_buckets = ctx->saved_data["n_buckets"].toInt(), heads = ctx->saved_data["heads"].toInt();
+        const EntryPtr e = c10::static_intrusive_pointer_cast<RelHold>(ctx->saved_data["entry"].toCapsule())->e;
+        const ScoreOptions opt{ctx->saved_data["cap"].toDouble(), t[6], t[7], t[8]};
+        Tensor d_o = grads[0].contiguous();
+        if (reinterpret_cast<uintptr_t>(d_o.data_ptr()) & 15) d_o = d_o.clone();
+        // (a hook on saved tensors may give back others than the forward's; needs_input_grad counts the tensors that were given)
+        Shape s;
+        TORCH_CHECK(attention_shape(q, k, v, p, s) && like(o, q) && like(d_o, q) && o.sizes() == q.sizes() && d_o.sizes() == q.sizes() && s.nq == e->a.n_rows
+                        && s.nk == e->b.n_rows && s.h == h && s.d == 64 && float_matrix(lse, q.device(), s.nq, h) && score_options(opt, q, k)
+                        && prepared.scalar_type() == at::kByte && prepared.device() == q.device() && prepared.is_contiguous()
+                        && prepared.numel() >= bpt_bucket_prepare_bytes(&e->a, &e->b, (int)h),
+                    "attention with a bias by buckets: the saved tensors are not those of the forward");
+        c10::DeviceGuard guard(q.device());
+        Tensor dq = at::empty_like(q), dk = at::empty_like(k), dv = at::empty_like(v), dslopes, dtable;
+        if (opt.slopes.defined() && ctx->needs_input_grad(4)) dslopes = at::empty_like(opt.slopes);
+        if (ctx->needs_input_grad(3)) dtable = at::empty({n_buckets, heads}, q.options());
+        const int64_t bytes = bpt_bucket_attention_backward_workspace_bytes(&e->a, &e->b, n_buckets, (int)heads, (int)h, s.dt);
+        const Tensor ws = at::empty({std::max<int64_t>(bytes, 16)}, q.options().dtype(at::kByte));
+        const bpt_score score = opt.pack();
+        const int st = bpt_bucket_attention_backward(&e->a, &e->b, &score, prepared.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), d_o.data_ptr(),
+                                                     lse.data_ptr<float>(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dtable.defined() ? dtable.data_ptr() : nullptr,
+                                                     dslopes.defined() ? dslopes.data_ptr<float>() : nullptr, ws.data_ptr(), bytes, n_buckets, (int)heads, (float)scale,
+                                                     (float)p, seed, (int)h, s.dt, stream_of(q.device()));
+        TORCH_CHECK(st == BPT_OK, "bucket_attention_backward: error ", st);
+        torch::autograd::variable_list out(14);
+        out[0] = dq;
+        out[1] = dk;
+        out[2] = dv;
+        out[3] = dtable;
+        out[4] = dslopes;
+        return out;
+    }
+};
+
+// op.bpt_attention with bias_table and buckets of a call whose plans are known (rows of h x 64, table of at most h heads), or None
+MaybeTensor bucket_attention(const MaybeTensor &row, const MaybeTensor &indptr_r, const MaybeTensor &eid_r, const MaybeTensor &indices_r, const Tensor &col,
+                             const Tensor &indptr_c, const Tensor &eid_c, const Tensor &indices_c, const Tensor &q, const Tensor &k, const Tensor &v,
+                             const Tensor &bias_table, const Tensor &buckets, const MaybeTensor &slopes, const MaybeTensor &pos_q, const MaybeTensor &pos_k,
+                             std::optional<double> score_cap, double scale, double p, uint64_t seed, int64_t h) {
+    if (score_cap && !(*score_cap >= 1.0e-10 && *score_cap <= 1.0e10 && std::abs(scale) <= std::min(1.0e4 * *score_cap, 1.0e6))) return std::nullopt;
+    if ((pos_q && pos_q->requires_grad()) || (pos_k && pos_k->requires_grad())) return std::nullopt;
+    if (q.dim() != 3 || q.size(1) != h || q.size(2) != 64 || !(std::abs(scale) >= 1.0e-6 && std::abs(scale) <= 1.0e6)) return std::nullopt;
+    if (bias_table.dim() != 2 || !like(bias_table, q) || bias_table.size(0) < 1 || bias_table.size(0) > BPT_MOST_BUCKETS || bias_table.size(1) < 1 || bias_table.size(1) > h)
+        return std::nullopt;
+    if (buckets.scalar_type() != at::kLong || buckets.dim() != 1 || buckets.device() != q.device() || !buckets.is_contiguous() || buckets.numel() != eid_c.numel())
+        return std::nullopt;
+    const ScoreOptions opt{score_cap.value_or(0.0), slopes.value_or(Tensor()), pos_q.value_or(Tensor()), pos_k.value_or(Tensor())};
+    const Tensor none, &r0 = row ? *row : none, &r1 = indptr_r ? *indptr_r : none, &r2 = eid_r ? *eid_r : none, &r3 = indices_r ? *indices_r : none;
+    const bool train = differentiated({&q, &k, &v, &bias_table}) || (opt.slopes.defined() && differentiated({&opt.slopes}));
+    const EntryPtr e = train ? score_entry(SCORE_TRAIN, {&col, &indptr_c, &eid_c, &indices_c, &r0, &r1, &r2, &r3}, q, k, v, p, h)
+                             : score_entry(SCORE_FWD, {&col, &indptr_c, &eid_c, &indices_c}, q, k, v, p, h);
+    if (!e || e->a.n_edges != buckets.numel() || !score_options(opt, q, k)) return std::nullopt;
+    c10::DeviceGuard guard(q.device());
+    const bpt_plan *out = train ? &e->b : nullptr;
+    const int64_t bytes = bpt_score_forward_workspace_bytes(&e->a, (int)h), kept = bpt_bucket_prepare_bytes(&e->a, out, (int)h);
+    if (kept < 0) return std::nullopt;
+    Tensor o = at::empty_like(q), lse = at::empty({q.size(0), h}, q.options().dtype(at::kFloat)), prepared = at::empty({kept}, q.options().dtype(at::kByte)), ws;
+    if (bytes > 0) ws = at::empty({bytes}, q.options().dtype(at::kByte));
+    const bpt_score score = opt.pack();
+    const int dt = dtype_code(q.scalar_type());
+    if (bpt_bucket_prepare(&e->a, out, bias_table.data_ptr(), buckets.data_ptr<int64_t>(), bias_table.size(0), (int)bias_table.size(1), (int)h, (float)scale, dt,
+                           prepared.data_ptr(), stream_of(q.device())) != BPT_OK
+        || bpt_bucket_attention_forward(&e->a, &score, prepared.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr<float>(),
+                                        bytes > 0 ? ws.data_ptr() : nullptr, bytes, (float)scale, (float)p, seed, (int)h, dt, stream_of(q.device())) != BPT_OK)
+        return std::nullopt;
+    if (!train) return o;
+    return BucketAttention::apply(q, k, v, bias_table, slopes, prepared, opt, e, o, lse, scale, p, (int64_t)seed, h);
+}
+
 // ---- the separate operators (modules/op.py:10-58 of the reference) -----------------------------------------------------------
 // masked_mm, sparse_softmax and vec_spmm of (n, h, d) rows and (E, h) edge tensors whose plans are known and cover every edge.  A
 // training pass through the chain cost the host 325 us in Python, at L = 512 as at L = 8192: three calls of its autograd functions,
@@ -1168,6 +1261,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("count_rows", &count_rows);
     m.def("rel_attention", &rel_attention);
     m.def("score_attention", &score_attention);
+    m.def("bucket_attention", &bucket_attention);
     m.def("remember", &remember);
     m.def("remember_rel", &remember_rel);
     m.def("forget", &forget);

@@ -977,9 +977,28 @@ struct ScoreMod {
                                        // p over a split row's segment, or null
     bf16_t *low;                       // bfloat16 destination side: [slot][column] sums of p du K
 };
+// Score options and a learned bias by buckets (BUCKETS): u = scale (q.k) + table[bucket][head].  The buckets of a plan's (entry, member) places are one byte each, read
+// as the edge ids of dropout are and by all heads of a block; a head's 256 biases, divided by scale, lie in LDS.
+struct BucketMod : ScoreMod {
+    const uint8_t *codes;              // [entry][member] of the plan's groups, or of its slots where it has none; NO_BUCKET: none
+    const float *table;                // [head][256], 0 at NO_BUCKET
+    bf16_t *ds;                        // bfloat16 source side: [head][entry][member], dL/d(q.k) of the pairs that exist, or null
+    int64_t places;                    // entries x members
+};
+constexpr int NO_BUCKET = 255;
 struct NoMod {};
-template <bool MOD> struct ModArg { typedef NoMod type; };
-template <> struct ModArg<true> { typedef ScoreMod type; };
+template <bool MOD, bool BUCKETS = false> struct ModArg { typedef NoMod type; };
+template <> struct ModArg<true, false> { typedef ScoreMod type; };
+template <> struct ModArg<true, true> { typedef BucketMod type; };
+// a wavefront's head's biases, into its own part of LDS (behind a fence: wave_lds_fence())
+__device__ __forceinline__ void tile_put_table(const BucketMod &md, int head, int lane, float *to) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) to[i * WAVE + lane] = md.table[(size_t)head * 256 + i * WAVE + lane];
+}
+__device__ __forceinline__ void tile_pair_codes(const BucketMod &md, int first_entry, int p_end, int c, int (&code)[4], int step = 1) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) code[r] = md.codes[(size_t)min(first_entry + step * r, p_end - 1) * TILE_R + c];
+}
 
 // What stands in rows that are not a member's neighbours must not reach its sums, and a product over a block's entries lets it: 0 x NaN.  So a wavefront whose
 // sums (of any member) are not finite walks its tile once more (CAREFUL), with products that add the existing pairs alone and with every
@@ -1109,11 +1128,11 @@ template <int SP> __device__ __forceinline__ void tile_put_slope_part(const Scor
     if (t.lane == 0) md.part[((size_t)t.grp * heads + t.head) * SP + t.part] = x;
 }
 
-template <typename T, int H, int D, int HW, bool DROP, int BIAS, bool NARROW = false, int SP = 1, bool MOD = false>
+template <typename T, int H, int D, int HW, bool DROP, int BIAS, bool NARROW = false, int SP = 1, bool MOD = false, bool BUCKETS = false>
 __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(4))) void k_attn_fwd_tile(
     bpt_plan P, const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v, T *__restrict__ o, float *__restrict__ lse,
     float *__restrict__ ws_acc, float *__restrict__ ws_ml, float scale_log2e, uint32_t drop_thr, uint32_t drop_seed, float drop_inv,
-    const float *__restrict__ bias, Narrow nw, Keep keep, typename ModArg<MOD>::type md) {
+    const float *__restrict__ bias, Narrow nw, Keep keep, typename ModArg<MOD, BUCKETS>::type md) {
     const int Hs = NARROW ? nw.h : H;                             // heads as lse, workspace and dropout keys count them
     const uint32_t RB = NARROW ? (uint32_t)(nw.heads * nw.d) * sizeof(T) : (uint32_t)(H * D * sizeof(T));        // bytes of a node row
     int block = (int)blockIdx.x;
@@ -1129,6 +1148,8 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(4))) 
     __shared__ __attribute__((aligned(16))) float kt_lds[HW][TILE_R * TILE_KT_STRIDE];
     float *kt = kt_lds[t.wv];
     __shared__ float pos_lds[HW][MOD ? TILE_R : 1];              // positions of the block's entries
+    __shared__ float tab_lds[BUCKETS ? HW : 1][BUCKETS ? 256 : 1];
+    if constexpr (BUCKETS) tile_put_table(md, t.head, t.lane, tab_lds[t.wv]);      // (read behind the fences of the first block)
     TileEntryRegs er;
     if (t.p_end > t.p_begin) tile_ask_entries(P, t.p_begin, min(TILE_CHUNK, t.p_end - t.p_begin), t.lane, er);
     issue_loads_first();
@@ -1166,6 +1187,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(4))) 
         int xe[DROP || BIAS == 1 ? 4 : 1];
         float bz[BIAS ? 4 : 1];
         float pos;                                                // of entry c, in the first lane group
+        int code[BUCKETS ? 4 : 1];
     };
     auto walk = [&](auto again) __attribute__((always_inline)) {
     constexpr bool CAREFUL = decltype(again)::value;
@@ -1181,6 +1203,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(4))) 
         };
         auto issue_rest = [&](Blk &B, int b) {
             if constexpr (DROP || BIAS == 1) tile_pair_eids(P, p0 + TILE_R * b + g, t.p_end, c, B.xe, 4);
+            if constexpr (BUCKETS) tile_pair_codes(md, p0 + TILE_R * b + g, t.p_end, c, B.code, 4);
             B.nv = min(TILE_R, cnt - TILE_R * b);
             if constexpr (MOD) {
                 if (md.slopes && g == 0) B.pos = md.pos_entry[ent[TILE_R * b + c].x];
@@ -1216,6 +1239,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(4))) 
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     x[r] = BIAS ? st[r] + B.bz[BIAS ? r : 0] : st[r];
+                    if constexpr (BUCKETS) x[r] += tab_lds[t.wv][B.code[r]];
                     pos_e[r] = md.slopes ? pos_lds[t.wv][4 * r + g] : 0.f;
                 }
                 tile_mod_scores(md, scale_log2e, slope, pos_m, pos_e, x, sc, du);
@@ -1300,12 +1324,12 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(4))) 
 // source side's layout instead (scattered 8-byte stores here, contiguous reads there) cost this kernel a third of its
 // time (126 against 85 us at L = 4096, k = 32); letting the source side recompute p and ds (two more products there,
 // delta (n, H) handed over) measured slower than either on every graph tried.
-template <typename T, int H, int D, int HW, bool DROP, int BIAS, bool NARROW = false, int SP = 1, bool MOD = false>
+template <typename T, int H, int D, int HW, bool DROP, int BIAS, bool NARROW = false, int SP = 1, bool MOD = false, bool BUCKETS = false>
 __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP || BIAS || MOD ? 3 : 4))) void k_attn_bwd_dst_tile(
     bpt_plan P, const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v, const T *__restrict__ o,
     const T *__restrict__ d_o, const float *__restrict__ lse, T *__restrict__ dq, float2 *__restrict__ pds, float *__restrict__ ws_dq,
     float scale, float scale_log2e, uint32_t drop_thr, uint32_t drop_seed, float drop_inv, const float *__restrict__ bias,
-    float *__restrict__ ds_out, Narrow nw, typename ModArg<MOD>::type md) {
+    float *__restrict__ ds_out, Narrow nw, typename ModArg<MOD, BUCKETS>::type md) {
     const int Hs = NARROW ? nw.h : H;
     const uint32_t RB = NARROW ? (uint32_t)(nw.heads * nw.d) * sizeof(T) : (uint32_t)(H * D * sizeof(T));
     TileCtx t;
@@ -1317,6 +1341,8 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP 
     __shared__ __attribute__((aligned(16))) float kt_lds[HW][TILE_R * TILE_KT_STRIDE];
     float *kt = kt_lds[t.wv];
     __shared__ float pos_lds[HW][MOD ? TILE_R : 1];
+    __shared__ float tab_lds[BUCKETS ? HW : 1][BUCKETS ? 256 : 1];
+    if constexpr (BUCKETS) tile_put_table(md, t.head, t.lane, tab_lds[t.wv]);      // (read behind the fences of the first block)
     TileEntryRegs er;
     if (t.p_end > t.p_begin) tile_ask_entries(P, t.p_begin, min(TILE_CHUNK, t.p_end - t.p_begin), t.lane, er);
     issue_loads_first();
@@ -1397,6 +1423,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP 
         int xe[DROP || BIAS == 1 ? 4 : 1];
         float bz[BIAS ? 4 : 1];
         float pos;                                                // of entry c, in the first lane group
+        int code[BUCKETS ? 4 : 1];
     };
     auto walk = [&](auto again) __attribute__((always_inline)) {
     constexpr bool CAREFUL = decltype(again)::value;
@@ -1407,6 +1434,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP 
         tile_put_entries(er, ent, cnt, t.lane, fst);
         auto issue = [&](Blk &B, int b) {
             if constexpr (DROP || BIAS == 1) tile_pair_eids(P, p0 + TILE_R * b + g, t.p_end, c, B.xe, 4);
+            if constexpr (BUCKETS) tile_pair_codes(md, p0 + TILE_R * b + g, t.p_end, c, B.code, 4);
             B.b = b;
             if constexpr (MOD) {
                 if (md.slopes && g == 0) B.pos = md.pos_entry[ent[TILE_R * b + c].x];
@@ -1461,6 +1489,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP 
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     x[r] = BIAS ? st[r] + B.bz[BIAS ? r : 0] : st[r];
+                    if constexpr (BUCKETS) x[r] += tab_lds[t.wv][B.code[r]];
                     pos_e[r] = md.slopes ? pos_lds[t.wv][4 * r + g] : 0.f;
                 }
                 tile_mod_scores(md, scale_log2e, slope, pos_m, pos_e, x, sm, du);
@@ -1861,11 +1890,11 @@ __device__ __forceinline__ void tile_store_sums(const TileCtx &t, float *sh, con
     wave_lds_fence();
 }
 
-template <int H, int D, int HW, int WPE, bool DROP, int BIAS, int SP, bool MOD = false>
+template <int H, int D, int HW, int WPE, bool DROP, int BIAS, int SP, bool MOD = false, bool BUCKETS = false>
 __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP || BIAS || MOD ? WPE - 1 : WPE))) void k_attn_fwd_rows_bf16(
     bpt_plan P, const bf16_t *__restrict__ q, const bf16_t *__restrict__ k, const bf16_t *__restrict__ v, bf16_t *__restrict__ o,
     float *__restrict__ lse, float *__restrict__ ws_acc, float *__restrict__ ws_ml, float scale_log2e, uint32_t drop_thr,
-    uint32_t drop_seed, float drop_inv, const float *__restrict__ bias, typename ModArg<MOD>::type md) {
+    uint32_t drop_seed, float drop_inv, const float *__restrict__ bias, typename ModArg<MOD, BUCKETS>::type md) {
     constexpr uint32_t RB = H * D * 2;
     const Narrow nw{};
     TileCtx t;
@@ -1878,6 +1907,8 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP 
     static_assert(PIECE >= TILE_PART_FWD_FLOATS && PIECE >= TILE_R * TILE_TURN_STRIDE, "parts and turned sums fit the rows' piece");
     __shared__ __attribute__((aligned(16))) float piece[HW][PIECE];
     __shared__ __attribute__((aligned(16))) float pos_lds[HW][MOD ? TILE_R : 4];      // positions of the block's entries
+    __shared__ float tab_lds[BUCKETS ? HW : 1][BUCKETS ? 256 : 1];
+    if constexpr (BUCKETS) tile_put_table(md, t.head, t.lane, tab_lds[t.wv]);      // (read behind the fences of the first block)
     char *const k_lds = reinterpret_cast<char *>(piece[t.wv]), *const v_lds = k_lds + 4 * TILE_ROWS_FLOATS_BF16;
     TileEntryRegs er;
     if (t.p_end > t.p_begin) tile_ask_entries(P, t.p_begin, min(TILE_CHUNK, t.p_end - t.p_begin), t.lane, er);
@@ -1909,6 +1940,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP 
         int xe[DROP || BIAS == 1 ? 4 : 1];
         float bz[BIAS ? 4 : 1];
         float pos;                                                // of entry c, in the first lane group
+        int code[BUCKETS ? 4 : 1];
     };
     auto walk = [&](auto again) __attribute__((always_inline)) {
     constexpr bool CAREFUL = decltype(again)::value;
@@ -1919,6 +1951,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP 
         tile_put_entries(er, ent, cnt, t.lane, fst);
         auto issue = [&](Blk &B, int b) {
             if constexpr (DROP || BIAS == 1) tile_pair_eids(P, p0 + TILE_R * b + 4 * g, t.p_end, c, B.xe);
+            if constexpr (BUCKETS) tile_pair_codes(md, p0 + TILE_R * b + 4 * g, t.p_end, c, B.code);
             if constexpr (MOD) {
                 if (md.slopes && g == 0) B.pos = md.pos_entry[ent[TILE_R * b + c].x];
             }
@@ -1947,12 +1980,13 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP 
             wave_lds_fence();
         }
         for (int b = 0; b < nblk; ++b) {
-            int mk[4], xe[DROP ? 4 : 1];
+            int mk[4], xe[DROP ? 4 : 1], code[BUCKETS ? 4 : 1];
             float bz[BIAS ? 4 : 1];
             tile_masks(ent + TILE_R * b, g, mk);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 if constexpr (DROP) xe[DROP ? r : 0] = B.xe[DROP ? r : 0];
+                if constexpr (BUCKETS) code[r] = B.code[r];
                 if constexpr (BIAS) bz[BIAS ? r : 0] = B.bz[BIAS ? r : 0];
             }
             tile_put_rows_bf16(k_lds, B.kr, t.lane);
@@ -1973,6 +2007,10 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP 
                 const float pos_e[4] = {pe[0], pe[1], pe[2], pe[3]};
 #pragma unroll
                 for (int r = 0; r < 4; ++r) x[r] = BIAS ? st[r] + bz[BIAS ? r : 0] : st[r];
+                if constexpr (BUCKETS) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) x[r] += tab_lds[t.wv][code[r]];
+                }
                 tile_mod_scores(md, scale_log2e, slope, pos_m, pos_e, x, sc, du);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) sc[r] = where_pair(mk[r], c, sc[r]);
@@ -2057,12 +2095,12 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP 
 // With a score term the pairs leave for the source side as they are formed, so dq, dk and dv keep delta', the slopes' gradient does not (tile_slope_fix).
 // One more product a block over the K rows at hand.  The segments of a split row leave their sums, that of p du K rounded to bfloat16 (2^-9 of a
 // correction that is 2^-8 of dq): k_score_split forms delta and the slopes' correction before the source side runs, k_score_merge dq's.
-template <int H, int D, int HW, int WPE, bool DROP, int BIAS, bool PDS, int SP, bool MOD = false>
+template <int H, int D, int HW, int WPE, bool DROP, int BIAS, bool PDS, int SP, bool MOD = false, bool BUCKETS = false>
 __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(MOD ? WPE - 2 : DROP || BIAS ? WPE - 1 : WPE))) void k_attn_bwd_dst_rows_bf16(
     bpt_plan P, const bf16_t *__restrict__ q, const bf16_t *__restrict__ k, const bf16_t *__restrict__ v, const bf16_t *__restrict__ o,
     const bf16_t *__restrict__ d_o, const float *__restrict__ lse, bf16_t *__restrict__ dq, uint32_t *__restrict__ pds,
     float2 *__restrict__ stat, float *__restrict__ ws_dq, float scale, float scale_log2e, uint32_t drop_thr, uint32_t drop_seed, float drop_inv,
-    const float *__restrict__ bias, float *__restrict__ ds_out, typename ModArg<MOD>::type md) {
+    const float *__restrict__ bias, float *__restrict__ ds_out, typename ModArg<MOD, BUCKETS>::type md) {
     static_assert(PDS || BIAS == 0, "the score term's gradient is stored by the pair's position");
     constexpr uint32_t RB = H * D * 2;
     constexpr bool FIX = MOD && !PDS;                             // delta from the pairs (comment above)
@@ -2077,6 +2115,8 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(MOD ?
     static_assert(PIECE >= TILE_PART_FLOATS && PIECE >= TILE_R * TILE_TURN_STRIDE, "parts and turned sums fit the rows' piece");
     __shared__ __attribute__((aligned(16))) float piece[HW][PIECE];
     __shared__ __attribute__((aligned(16))) float pos_lds[HW][MOD ? TILE_R : 4];
+    __shared__ float tab_lds[BUCKETS ? HW : 1][BUCKETS ? 256 : 1];
+    if constexpr (BUCKETS) tile_put_table(md, t.head, t.lane, tab_lds[t.wv]);      // (read behind the fences of the first block)
     char *const k_lds = reinterpret_cast<char *>(piece[t.wv]), *const v_lds = k_lds + 4 * TILE_ROWS_FLOATS_BF16;
     TileEntryRegs er;
     if (t.p_end > t.p_begin) tile_ask_entries(P, t.p_begin, min(TILE_CHUNK, t.p_end - t.p_begin), t.lane, er);
@@ -2138,6 +2178,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(MOD ?
         int xe[DROP || BIAS == 1 ? 4 : 1];
         float bz[BIAS ? 4 : 1];
         float pos;                                                // of entry c, in the first lane group
+        int code[BUCKETS ? 4 : 1];
     };
     auto walk = [&](auto again) __attribute__((always_inline)) {
     constexpr bool CAREFUL = decltype(again)::value;
@@ -2153,6 +2194,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(MOD ?
         };
         auto issue = [&](Blk &B, int b) {
             if constexpr (DROP || BIAS == 1) tile_pair_eids(P, p0 + TILE_R * b + 4 * g, t.p_end, c, B.xe);
+            if constexpr (BUCKETS) tile_pair_codes(md, p0 + TILE_R * b + 4 * g, t.p_end, c, B.code);
             if constexpr (MOD) {
                 if (md.slopes && g == 0) B.pos = md.pos_entry[ent[TILE_R * b + c].x];
             }
@@ -2172,7 +2214,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(MOD ?
         Blk B;
         issue(B, 0);
         for (int b = 0; b < nblk; ++b) {
-            int mk[4], xe[DROP || BIAS == 1 ? 4 : 1];
+            int mk[4], xe[DROP || BIAS == 1 ? 4 : 1], code[BUCKETS ? 4 : 1];
             float bz[BIAS ? 4 : 1];
             uint32_t pos[4];
             tile_masks(ent + TILE_R * b, g, mk);
@@ -2181,6 +2223,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(MOD ?
             for (int r = 0; r < 4; ++r) {
                 if constexpr (DROP || BIAS == 1) xe[DROP || BIAS == 1 ? r : 0] = B.xe[DROP || BIAS == 1 ? r : 0];
                 if constexpr (BIAS) bz[BIAS ? r : 0] = B.bz[BIAS ? r : 0];
+                if constexpr (BUCKETS) code[r] = B.code[r];
             }
             tile_put_rows_bf16(k_lds, B.kr, t.lane);
             tile_put_rows_bf16(v_lds, B.vr, t.lane);
@@ -2202,6 +2245,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(MOD ?
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     x[r] = BIAS ? st[r] + bz[BIAS ? r : 0] : st[r];
+                    if constexpr (BUCKETS) x[r] += tab_lds[t.wv][code[r]];
                     pos_e[r] = at_e[r];
                 }
                 tile_mod_scores(md, scale_log2e, slope, pos_m, pos_e, x, sm, du);
@@ -2688,11 +2732,11 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(WPE))
 // 30.9; L = 32768, k = 2 235 -> 221; 32-graph batch 102.5 -> 99.2; L = 512 and L = 8192 with dropout level.  (6 heads of 50
 // columns with dropout lost 2 %: heads of fewer than 64 columns keep the scratch.)  float32 keeps it too: there the two
 // products are 1024 cycles of the matrix pipeline per block.  122 registers: compiled for four wavefronts per SIMD.
-template <int H, int D, int HW, int WPE, bool DROP, int SP = 1, bool MOD = false>
+template <int H, int D, int HW, int WPE, bool DROP, int SP = 1, bool MOD = false, bool BUCKETS = false>
 __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(MOD ? WPE - 1 : WPE))) void k_attn_bwd_src_tile_bf16_again(
     bpt_plan P, const bf16_t *__restrict__ q, const bf16_t *__restrict__ k, const bf16_t *__restrict__ v, const bf16_t *__restrict__ d_o,
     const float2 *__restrict__ stat, bf16_t *__restrict__ dk, bf16_t *__restrict__ dv, float *__restrict__ ws_dk, float *__restrict__ ws_dv,
-    float scale, float scale_log2e, uint32_t drop_thr, uint32_t drop_seed, float drop_inv, typename ModArg<MOD>::type md) {
+    float scale, float scale_log2e, uint32_t drop_thr, uint32_t drop_seed, float drop_inv, typename ModArg<MOD, BUCKETS>::type md) {
     constexpr uint32_t RB = H * D * 2;
     const Narrow nw{};
     TileCtx t;
@@ -2702,6 +2746,8 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(MOD ?
     static_assert(PIECE >= LIVE && ROWS >= TILE_R * TILE_TURN_STRIDE, "the lists and the turned sums fit");
     __shared__ __attribute__((aligned(16))) float piece[HW][PIECE];
     __shared__ __attribute__((aligned(16))) float pos_lds[HW][MOD ? TILE_R : 4];
+    __shared__ float tab_lds[BUCKETS ? HW : 1][BUCKETS ? 256 : 1];
+    if constexpr (BUCKETS) tile_put_table(md, t.head, t.lane, tab_lds[t.wv]);      // (read behind the fences of the first block)
     int2 *ent = reinterpret_cast<int2 *>(piece[t.wv]);
     char *const q_lds = reinterpret_cast<char *>(piece[t.wv] + ENT), *const d_lds = q_lds + 4 * TILE_ROWS_FLOATS_BF16;
     float2 *const st_lds = reinterpret_cast<float2 *>(piece[t.wv] + ENT + ROWS);
@@ -2740,6 +2786,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(MOD ?
         float2 ld;                                                // (lse, delta) of entry c, in the first lane group
         int xe[DROP ? 4 : 1];
         float pos;                                                // of entry c, in the first lane group
+        int code[BUCKETS ? 4 : 1];
     };
     auto walk = [&](auto again) __attribute__((always_inline)) {
     constexpr bool CAREFUL = decltype(again)::value;
@@ -2750,6 +2797,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(MOD ?
         tile_put_entries(er, ent, cnt, t.lane);
         auto issue = [&](Blk &B, int b) {
             if constexpr (DROP) tile_pair_eids(P, p0 + TILE_R * b + 4 * g, t.p_end, c, B.xe);
+            if constexpr (BUCKETS) tile_pair_codes(md, p0 + TILE_R * b + 4 * g, t.p_end, c, B.code);
             if constexpr (MOD) {
                 if (md.slopes && g == 0) B.pos = md.pos_entry[ent[TILE_R * b + c].x];
             }
@@ -2762,10 +2810,12 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(MOD ?
         Blk B;
         issue(B, 0);
         for (int b = 0; b < nblk; ++b) {
-            int mk[4], xe[DROP ? 4 : 1];
+            int mk[4], xe[DROP ? 4 : 1], code[BUCKETS ? 4 : 1];
             tile_masks(ent + TILE_R * b, g, mk);
 #pragma unroll
             for (int r = 0; r < (DROP ? 4 : 0); ++r) xe[r] = B.xe[r];
+#pragma unroll
+            for (int r = 0; r < (BUCKETS ? 4 : 0); ++r) code[r] = B.code[r];
             tile_put_rows_bf16(q_lds, B.qr, t.lane);
             tile_put_rows_bf16(d_lds, B.dr, t.lane);
             if (g == 0) st_lds[c] = B.ld;
@@ -2785,7 +2835,12 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(MOD ?
             float pe[4], ds[4], sm[4], du[4];
             if constexpr (MOD) {
                 const floatx4v at_e = *reinterpret_cast<const floatx4v *>(&pos_lds[t.wv][4 * g]);
-                const float pos_e[4] = {at_e[0], at_e[1], at_e[2], at_e[3]}, x[4] = {st[0], st[1], st[2], st[3]};
+                const float pos_e[4] = {at_e[0], at_e[1], at_e[2], at_e[3]};
+                float x[4] = {st[0], st[1], st[2], st[3]};
+                if constexpr (BUCKETS) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) x[r] += tab_lds[t.wv][code[r]];
+                }
                 tile_mod_scores(md, scale_log2e, slope, pos_m, pos_e, x, sm, du);
             }
 #pragma unroll
@@ -2796,6 +2851,9 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(MOD ?
                     mt = dropout_keep((uint32_t)xe[DROP ? r : 0] * (uint32_t)H + (uint32_t)t.head, drop_seed, drop_thr, drop_inv);
                 ds[r] = where_pair_or_zero(mk[r], c, MOD ? p * (dp[r] * mt - delta_e[r]) * du[r] : p * (dp[r] * mt - delta_e[r]) * scale);
                 pe[r] = p * mt;
+                if constexpr (BUCKETS) {
+                    if (md.ds && ((mk[r] >> c) & 1)) Elem<bf16_t>::st(md.ds + (size_t)t.head * md.places + (size_t)(p0 + TILE_R * b + 4 * g + r) * TILE_R + c, ds[r]);
+                }
             }
             if constexpr (CAREFUL) {
                 tile_axpy_pairs_bf16(ds, mk, q_lds, c, g, ak);

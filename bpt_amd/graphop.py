@@ -1486,19 +1486,9 @@ def _check_buckets(buckets, device):
         raise ValueError("all tensors of a call must be on one device")
 
 
-def bucket_plan(graph, q, k, dropout_p):
-    """The in-side's tile plan of a forward with a bias by buckets (q of a padded shape), or None where it does not run on tiles that cover every edge."""
-    col, indptr_c, eid_c, indices_c = graph[4:]
-    seg = _tile_seg_without_plan(col, eid_c.size(0), q, k, q.size(1), q.size(2), dropout_p, q, _SETTINGS)
-    if seg is None:
-        return None
-    plan = plan_cache.get(col, indptr_c, eid_c, indices_c, q.size(0), k.size(0), seg_len=seg, prefer_device=True, groups=(TILE_ROWS, None))
-    return plan if plan.covers_all_edges else None
-
-
 def bucket_bias_forward(table, buckets, factor=1.0, term=False):
     """bias[e, head] = factor * table[buckets[e], head] of table (n, h), float32, float64 or bfloat16, and buckets (E,) int64: (E, h) of table's type, or with
-    term the float32 (E + 1, h) that attention_forward takes as bias.  A bucket outside of table adds 0."""
+    term the float32 (E + 1, h) that score_attention_forward takes as bias.  A bucket outside of table adds 0."""
     _check_input(table, "table")
     if table.dim() != 2 or table.size(0) < 1 or table.size(1) < 1:
         raise ValueError("table must be (n_buckets, heads)")
@@ -1528,31 +1518,4 @@ def bucket_bias_backward(ds, buckets, table, factor=1.0):
         ws = torch.empty(nws, dtype=torch.uint8, device=table.device)
         check_attn(_BIAS_LIB.bpt_bucket_bias_backward(_ptr(ds), _ptr(buckets), _ptr(dtable), _ptr(ws), nws, E, n, h, float(factor), _dtype(table), _dtype(ds), _stream()),
                    "bucket_bias_backward")
-    return dtable
-
-
-def bucket_pairs_forward(table, buckets, order, factor=1.0):
-    """(codes, bias): bucket_bias_forward's term in the order of a tile plan's pairs (order: attention_pair_order's), bias float32 (h, E) as attention_forward
-    takes it with bias_by_pair, codes what bucket_pairs_backward takes."""
-    (n, h), E = table.shape, buckets.size(0)
-    codes, bias = torch.empty(E, dtype=torch.int16, device=table.device), torch.empty((h, E), dtype=torch.float32, device=table.device)
-    eids = order[1]["eid_of_pair"]
-    _expect_shape(eids, (E,), "buckets")
-    with _on_device_of(table):
-        check_attn(_BIAS_LIB.bpt_bucket_pairs_forward(_ptr(table), _ptr(buckets), _ptr(eids), _ptr(codes), _ptr(bias), E, n, h, float(factor), _dtype(table), _stream()),
-                   "bucket_pairs_forward")
-    return codes, bias
-
-
-def bucket_pairs_backward(ds, codes, table, factor=1.0):
-    """bucket_bias_backward of ds (h, E), in the order of codes."""
-    (n, h), E = table.shape, codes.size(0)
-    _check_all(ds=ds, codes=codes)
-    _expect_shape(ds, (h, E), "ds")
-    dtable = torch.empty((n, h), dtype=table.dtype, device=table.device)
-    with _on_device_of(table):
-        nws = _BIAS_LIB.bpt_bucket_bias_backward_workspace_bytes(E, n, h, _dtype(table))
-        ws = torch.empty(nws, dtype=torch.uint8, device=table.device)
-        check_attn(_BIAS_LIB.bpt_bucket_pairs_backward(_ptr(ds), _ptr(codes), _ptr(dtable), _ptr(ws), nws, E, n, h, float(factor), _dtype(table), _stream()),
-                   "bucket_pairs_backward")
     return dtable

@@ -227,26 +227,15 @@ class BucketBias(Function):
 
 
 class BPTBucketAttention(Function):
-    """BPTAttention with scores scale q.k + table[buckets[e], head], with or without score options (score, slopes: as BPTRelAttention's), whose
-    cap then bounds the sum.  The fused kernels add a term before the scale: it is formed as table / scale, and the gradient of the table is the sum of
-    the term's by buckets, divided by the scale.  order: None, the term goes by edge id, or attention_pair_order's, it goes in the order of the tiles."""
+    """BPTScoreAttention with scores scale q.k + table[buckets[e], head] for tables of any length, where the native host path has the fused one of short tables.
+    The kernels add a term per edge before the scale: it is formed as table / scale, and the gradient of the table is the sum of the term's by buckets, divided by the scale."""
 
     @staticmethod
-    def forward(ctx, row, indptr_r, eid_r, indices_r, col, indptr_c, eid_c, indices_c, q, k, v, scale, dropout_p, seed, table, buckets, order=None, score=None,
-                slopes=None):
-        codes = None
-        if order is not None:
-            codes, bias = _g.bucket_pairs_forward(table, buckets, order, 1.0 / scale)
-        else:
-            bias = _g.bucket_bias_forward(table, buckets, 1.0 / scale, term=True)
-        if score is not None:
-            o, lse = _g.score_attention_forward(col, indptr_c, eid_c, indices_c, q, k, v, score, scale, dropout_p, seed, bias)
-        else:
-            o, lse = _g.attention_forward(col, indptr_c, eid_c, indices_c, q, k, v, scale, dropout_p, seed, bias=bias, bias_by_pair=order is not None)
-        ctx.save_for_backward(row, indptr_r, eid_r, indices_r, col, indptr_c, eid_c, indices_c, q, k, v, o, lse, bias, table, buckets if codes is None else codes,
-                              *(() if score is None else score[1:]))
-        ctx.cap, ctx.by_pair = None if score is None else score.cap, order is not None
-        ctx.scale, ctx.dropout_p, ctx.seed = scale, dropout_p, seed
+    def forward(ctx, row, indptr_r, eid_r, indices_r, col, indptr_c, eid_c, indices_c, q, k, v, scale, dropout_p, seed, table, buckets, score, slopes):
+        bias = _g.bucket_bias_forward(table, buckets, 1.0 / scale, term=True)
+        o, lse = _g.score_attention_forward(col, indptr_c, eid_c, indices_c, q, k, v, score, scale, dropout_p, seed, bias)
+        ctx.save_for_backward(row, indptr_r, eid_r, indices_r, col, indptr_c, eid_c, indices_c, q, k, v, o, lse, bias, table, buckets, *score[1:])
+        ctx.cap, ctx.scale, ctx.dropout_p, ctx.seed = score.cap, scale, dropout_p, seed
         return o
 
     @staticmethod
@@ -254,15 +243,11 @@ class BPTBucketAttention(Function):
         if torch.is_grad_enabled():
             raise RuntimeError("attention with a bias by buckets is not differentiable twice")
         tensors = ctx.saved_tensors
-        graph, (q, k, v, o, lse, bias, table, buckets), dslopes, dtable = tensors[:8], tensors[8:16], None, None
-        if ctx.cap is not None:
-            dq, dk, dv, dslopes, ds = _g.score_attention_backward(*graph, q, k, v, o, lse, do, _g.Score(ctx.cap, *tensors[16:]), ctx.scale, ctx.dropout_p, ctx.seed, bias,
-                                                                  ctx.needs_input_grad[18])
-        else:
-            dq, dk, dv, ds = _g.attention_backward(*graph, q, k, v, o, lse, do, ctx.scale, ctx.dropout_p, ctx.seed, bias=bias, bias_by_pair=ctx.by_pair)
-        if ctx.needs_input_grad[14]:
-            dtable = (_g.bucket_pairs_backward if ctx.by_pair else _g.bucket_bias_backward)(ds, buckets, table, 1.0 / ctx.scale)
-        return None, None, None, None, None, None, None, None, dq, dk, dv, None, None, None, dtable, None, None, None, dslopes
+        bias, table, buckets = tensors[13:16]
+        dq, dk, dv, dslopes, ds = _g.score_attention_backward(*tensors[:13], do, _g.Score(ctx.cap, *tensors[16:]), ctx.scale, ctx.dropout_p, ctx.seed, bias,
+                                                              ctx.needs_input_grad[17])
+        dtable = _g.bucket_bias_backward(ds, buckets, table, 1.0 / ctx.scale) if ctx.needs_input_grad[14] else None
+        return None, None, None, None, None, None, None, None, dq, dk, dv, None, None, None, dtable, None, None, dslopes
 
 
 def _rel_backward(row, indptr_r, eid_r, indices_r, col, indptr_c, eid_c, indices_c, q, k, v, o, lse, bias, table, do, scale, dropout_p, seed, rows_slot,
@@ -558,6 +543,16 @@ def _score_attention(graph, q, k, v, scale, fused, dropout_p, seed, rel_table, e
     return o if as_it_is else o[:, :h, :d].contiguous()
 
 
+def _bucket_known(graph, q, k, v, scale, dropout_p, seed, bias_table, buckets, score_cap, slopes, pos):
+    """A call with a bias by buckets whose plans the native host path knows, which checks it there, or None."""
+    if not _native_takes() or _g.force_generic_enabled():
+        return None
+    pos = tuple(pos) if isinstance(pos, (tuple, list)) else (pos, pos)
+    if len(pos) != 2 or q.dim() != 3 or _g.score_padded_shape(q) != tuple(q.shape[1:]):
+        return None
+    return _native.bucket_attention(*graph, q, k, v, bias_table, buckets, slopes, *pos, score_cap, scale, dropout_p, seed & (2 ** 64 - 1), q.size(1))
+
+
 def _bucket_attention(graph, q, k, v, scale, fused, dropout_p, seed, bias_table, buckets, score_cap, slopes, pos):
     """bpt_attention with a bias by buckets, and score options or not."""
     h = q.size(1) if q.dim() == 3 else 1
@@ -569,38 +564,43 @@ def _bucket_attention(graph, q, k, v, scale, fused, dropout_p, seed, bias_table,
         raise RuntimeError("all floating point arguments must share one dtype")
     if bias_table.device != q.device or buckets.device != q.device:
         raise ValueError("all tensors of a call must be on one device")
-    bias_table = bias_table.contiguous()
-    score = None if score_cap is None and slopes is None and pos is None else _g.score_options(score_cap, slopes, pos, q, k, scale)
-    train = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, bias_table, slopes))
-    runs = fused is not False and _native_takes() and 1e-6 <= abs(scale) <= 1e6 and _g.score_supported(graph[6], q, k)
-    given, given_table, order = (q, k, v), bias_table, None
+    bias_table, buckets = bias_table.contiguous(), buckets.contiguous()
+    if dropout_p > 0 and seed is None and fused is not False:
+        seed = int(torch.randint(0, 2 ** 62, (1,)).item())
+    seed, dropout_p = int(seed or 0), float(dropout_p)
+    if fused is not False:
+        o = _bucket_known(graph, q, k, v, scale, dropout_p, seed, bias_table, buckets, score_cap, slopes, pos)
+        if o is not None:
+            return o
+    score = _g.Score(0.0, None, None, None) if score_cap is None and slopes is None and pos is None else _g.score_options(score_cap, slopes, pos, q, k, scale)
+    train = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, bias_table, score.slopes))
+    runs = (fused is not False and _native_takes() and 1e-6 <= abs(scale) <= 1e6 and _g.score_supported(graph[6], q, k)
+            and (not train or all(t is not None for t in graph[:4])))
+    given = q, k, v, score
     if runs:
-        (heads, d), (hp, dp) = q.shape[1:], _g.score_padded_shape(q)
-        slopes, padded = None if score is None else score.slopes, (heads, d) != (hp, dp)
+        d, (hp, dp) = q.size(2), _g.score_padded_shape(q)
+        padded = (h, d) != (hp, dp)
         if padded:
             # as with relative positions: zero columns and heads add nothing
-            q, k, v = (torch.nn.functional.pad(x, (0, dp - d, 0, hp - heads)) for x in (q, k, v))
-            bias_table = torch.nn.functional.pad(bias_table, (0, hp - heads))
-            if slopes is not None:
-                slopes = torch.nn.functional.pad(slopes, (0, hp - heads))
-                score = score._replace(slopes=slopes)
+            q, k, v = (torch.nn.functional.pad(x, (0, dp - d, 0, hp - h)) for x in (q, k, v))
+            if score.slopes is not None:
+                score = score._replace(slopes=torch.nn.functional.pad(score.slopes, (0, hp - h)))
         else:
             q, k, v = (x.clone() if x.data_ptr() % 16 else x for x in (q, k, v))          # (the kernels read 16 bytes a lane)
-        if train and score is None:
-            order = _g.attention_pair_order(*graph, q, k, dropout_p) if all(t is not None for t in graph[:4]) and bias_table.size(0) < 65535 else None
-            runs = order is not None
-        elif score is None:
-            runs = _g.bucket_plan(graph, q, k, dropout_p) is not None
-        else:
-            runs = (not train or all(t is not None for t in graph[:4])) and _g.prepare_score(graph, q, k, dropout_p, train)
+        known = lambda: _bucket_known(graph, q, k, v, scale, dropout_p, seed, bias_table, buckets, score.cap or None, score.slopes,
+                                      None if score.slopes is None else score[2:])
+        o = known() if padded else None
+        if o is None:
+            runs = _g.prepare_score(graph, q, k, dropout_p, train)
+            o = known() if runs else None
     if not runs:
         if fused:
             raise RuntimeError("attention with a bias by buckets has no fused kernel for this call")
-        return _score_chain(graph, *given, scale, dropout_p, None, None, score or _g.Score(0.0, None, None, None), given_table, buckets)
-    if dropout_p > 0 and seed is None:
-        seed = int(torch.randint(0, 2 ** 62, (1,)).item())
-    o = BPTBucketAttention.apply(*graph, q, k, v, scale, float(dropout_p), int(seed or 0), bias_table, buckets, order, score, slopes)
-    return o[:, :heads, :d].contiguous() if padded else o
+        return _score_chain(graph, *given[:3], scale, dropout_p, None, None, given[3], bias_table, buckets)
+    if o is None:                                                 # (more buckets than a byte counts, or a cache too small for the plans)
+        o = BPTBucketAttention.apply(*graph, q, k, v, scale, dropout_p, seed, torch.nn.functional.pad(bias_table, (0, hp - h)) if padded else bias_table, buckets,
+                                     score, score.slopes)
+    return o[:, :h, :d].contiguous() if padded else o
 
 
 def bpt_attention(row, indptr_r, eid_r, indices_r, col, indptr_c, eid_c, indices_c, q, k, v, scale=None, fused=None,

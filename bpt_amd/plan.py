@@ -198,7 +198,7 @@ def link_groups_host(grp_dst, grp_src, n_edges):
 def _bias_rows_of(groups_struct, pair_eid, eids, n_edges):
     """For a plan's tile groups: the struct with bias_by_pair set (the per-edge score term is read, and its gradient
     written, head-major at the plan's own pair numbers), the pair number of every edge id, and for every pair number its
-    member index in its tile (the position of its bit in its entry's mask) and its edge id, int32."""
+    member index in its tile (the position of its bit in its entry's mask), int32."""
     pair_of_eid = torch.empty(n_edges, dtype=torch.int64, device=pair_eid.device)
     pair_of_eid[pair_eid[:n_edges].to(torch.int64)] = torch.arange(n_edges, dtype=torch.int64, device=pair_eid.device)
     # eids is (entries, R) with n_edges where an entry has no such member: the pairs in their own order are its other elements
@@ -206,7 +206,7 @@ def _bias_rows_of(groups_struct, pair_eid, eids, n_edges):
     member = (torch.nonzero(eids.reshape(-1) < n_edges).flatten() % R).to(torch.int32)
     st = PlanStruct.from_buffer_copy(groups_struct)
     st.bias_by_pair = 1
-    return {"struct": st, "pair_of_eid": pair_of_eid, "member_of_pair": member, "eid_of_pair": pair_eid[:n_edges].to(torch.int32).contiguous()}
+    return {"struct": st, "pair_of_eid": pair_of_eid, "member_of_pair": member}
 
 
 def pair_numbers_host(grp_mine, grp_theirs, n_edges):

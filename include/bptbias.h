@@ -9,6 +9,8 @@
 
 #include <stdint.h>
 
+#include "bptscore.h"
+
 #ifdef __cplusplus
 extern "C" {
 #endif
@@ -23,14 +25,28 @@ int64_t bpt_bucket_bias_backward_workspace_bytes(int64_t n_edges, int64_t n_buck
 int bpt_bucket_bias_backward(const void *ds, const int64_t *buckets, void *dtable, void *workspace, int64_t workspace_bytes, int64_t n_edges,
                              int64_t n_buckets, int h, double factor, int dtype, int ds_dtype, void *stream);
 
-/* The same in the order of a tile plan's pairs (bias_by_pair of bptattn.h).  eid_of_pair (n_edges) int32: the edge of every pair number; codes (n_edges)
- * uint16: the buckets of the pairs, 65535 where there is none; bias (h, n_edges) float32.  n_buckets <= 65535. */
-int bpt_bucket_pairs_forward(const void *table, const int64_t *buckets, const int32_t *eid_of_pair, uint16_t *codes, float *bias, int64_t n_edges,
-                             int64_t n_buckets, int h, double factor, int dtype, void *stream);
+/* The fused pass of bptscore.h with u = scale (q[dst].k[src]) + table[bucket][head], capped and lowered by distance or not (score as there; all of it 0: neither).
+ * Heads of 64 columns, h = 8 or 16 of them, float32 also 4; up to 255 buckets.  Plans as there, with grp_eids on either side.  scale is not 0.  In bfloat16 delta comes from
+ * the pairs.  A row whose edges are all hidden (-infinity in table, without a cap) is 0. */
+#define BPT_MOST_BUCKETS 255
 
-/* ds (h, n_edges) float32; the workspace is that of bpt_bucket_bias_backward. */
-int bpt_bucket_pairs_backward(const float *ds, const uint16_t *codes, void *dtable, void *workspace, int64_t workspace_bytes, int64_t n_edges,
-                              int64_t n_buckets, int h, double factor, int dtype, void *stream);
+/* What the passes of a call take: the heads' tables and the bucket of every place of the plans, written to `prepared` (on 16 bytes).  plan_out may be NULL where no
+ * backward follows.  table (n_buckets, heads) of dtype, heads <= h (those behind have no bias), buckets (n_edges). */
+int64_t bpt_bucket_prepare_bytes(const bpt_plan *plan_in, const bpt_plan *plan_out, int h);
+int bpt_bucket_prepare(const bpt_plan *plan_in, const bpt_plan *plan_out, const void *table, const int64_t *buckets, int64_t n_buckets, int heads, int h,
+                       float scale, int dtype, void *prepared, void *stream);
+
+/* The workspace is that of bpt_score_forward. */
+int bpt_bucket_attention_forward(const bpt_plan *plan_in, const bpt_score *score, const void *prepared, const void *q, const void *k, const void *v, void *o,
+                                 float *lse, void *workspace, int64_t workspace_bytes, float scale, float dropout_p, uint64_t dropout_seed, int h, int dtype,
+                                 void *stream);
+
+/* dtable (n_buckets, heads) of dtype or NULL; the rest as bpt_score_backward. */
+int64_t bpt_bucket_attention_backward_workspace_bytes(const bpt_plan *plan_in, const bpt_plan *plan_out, int64_t n_buckets, int heads, int h, int dtype);
+int bpt_bucket_attention_backward(const bpt_plan *plan_in, const bpt_plan *plan_out, const bpt_score *score, const void *prepared, const void *q, const void *k,
+                                  const void *v, const void *o, const void *d_o, const float *lse, void *dq, void *dk, void *dv, void *dtable,
+                                  float *dslopes, void *workspace, int64_t workspace_bytes, int64_t n_buckets, int heads, float scale, float dropout_p,
+                                  uint64_t dropout_seed, int h, int dtype, void *stream);
 
 #ifdef __cplusplus
 }

@@ -116,21 +116,24 @@ int run_sums(const void *ds, const int64_t *buckets, void *dtable, void *ws, int
 // ---- the fused attention -----------------------------------------------------------------------------------------------------------
 // One byte a place says which of a head's biases a pair takes, so the passes read 1 / (4 h) of what the term itself would be (float32, h heads, each way), and nothing
 // of an edge's size is written but ds, which is summed up by buckets behind the backward: in float32 from the scratch that the sides hand over anyway, in bfloat16, whose
-// sides hand over none, from the source side's own, rounded to bfloat16 (2^-9 of each of the terms of sums of thousands).
+// sides hand over none, from the source side's own, in 32 bits: L = 32768, k = 8, 16 heads, 211 MB each way.  (In bfloat16 the sums of a table whose terms cancel came out
+// 1.5 times as far off as their own rounding.)
 inline int64_t places(const bpt_plan *p) { return p->n_groups > 0 ? p->n_grp_entries * TILE_R : p->n_edges; }
 inline const int32_t *place_eids(const bpt_plan *p) { return p->n_groups > 0 ? p->grp_eids : p->eid; }
 inline int64_t table_bytes(int h) { return (int64_t)h * 256 * 4; }
 struct Prepared {
     float *table;
-    uint8_t *codes_in, *codes_out;
-    Prepared(void *at, const bpt_plan *in, int h) : table((float *)at), codes_in((uint8_t *)at + table_bytes(h)), codes_out(codes_in + round16(places(in))) {}
+    uint8_t *codes_in, *codes_pairs, *codes_out;      // (the last two for a backward: by pair numbers of the side whose ds is summed up, and by places)
+    Prepared(void *at, const bpt_plan *in, int h)
+        : table((float *)at), codes_in((uint8_t *)at + table_bytes(h)), codes_pairs(codes_in + round16(places(in))), codes_out(codes_pairs + round16(in->n_edges)) {}
 };
 
-// blockIdx.y: 0 the tables, 1 and 2 the places of either side, four a thread
+// blockIdx.y: 0 the tables, 1 and 2 the places of either side, four a thread; by_pair: the side whose pairs' codes are wanted too, or 0
 template <typename T>
 __global__ __launch_bounds__(BLOCK) void k_bucket_prepare(const T *__restrict__ table, const int64_t *__restrict__ buckets, int n_buckets, int heads, int h, float factor,
                                                           int64_t n_edges, const int32_t *__restrict__ eids_in, int64_t n_in, const int32_t *__restrict__ eids_out,
-                                                          int64_t n_out, float *__restrict__ tables, uint8_t *__restrict__ codes_in, uint8_t *__restrict__ codes_out) {
+                                                          int64_t n_out, float *__restrict__ tables, uint8_t *__restrict__ codes_in, uint8_t *__restrict__ codes_out,
+                                                          const int4 *__restrict__ entries, int by_pair, uint8_t *__restrict__ codes_pairs) {
     const int64_t first = ((int64_t)blockIdx.x * BLOCK + threadIdx.x) * 4;
     if (blockIdx.y == 0) {
         for (int64_t i = first; i < first + 4 && i < (int64_t)h * 256; ++i) {
@@ -150,6 +153,15 @@ __global__ __launch_bounds__(BLOCK) void k_bucket_prepare(const T *__restrict__ 
     uint32_t word = 0;
 #pragma unroll
     for (int u = 0; u < 4; ++u) word |= ((uint64_t)b[u] < (uint64_t)n_buckets ? (uint32_t)b[u] : (uint32_t)NO_BUCKET) << 8 * u;
+    if (by_pair == (int)blockIdx.y && first < n) {                // (four places are of one entry)
+        const int4 en = entries[first / TILE_R];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int m = (int)(first % TILE_R) + u;
+            const int64_t pair = tile_pair_number(en.z, en.y, m);
+            if (((en.y >> m) & 1) && (uint64_t)pair < (uint64_t)n_edges) codes_pairs[pair] = (uint8_t)(word >> 8 * u);
+        }
+    }
     if (first + 4 <= n) {
         *reinterpret_cast<uint32_t *>(codes + first) = word;
     } else {
@@ -158,44 +170,53 @@ __global__ __launch_bounds__(BLOCK) void k_bucket_prepare(const T *__restrict__ 
     }
 }
 
-// dtable's parts from ds at the places of a plan: a workgroup has one head, a lane a place and a column of sums in LDS, as k_bucket_sums.
-// float32: ds is the second of the pairs' (p, ds), [head][pair]; bfloat16: [head][place].
-template <typename T> struct PlaceDs { typedef float2 type; };
-template <> struct PlaceDs<bf16_t> { typedef bf16_t type; };
-template <typename T, int WAVES, int ROOM>
-__global__ __launch_bounds__(WAVES *WAVE) void k_bucket_places(const int4 *__restrict__ entries, const uint8_t *__restrict__ codes, const typename PlaceDs<T>::type *__restrict__ ds,
-                                                               int64_t n, int64_t n_edges, float *__restrict__ part, int n_buckets, int heads) {
+// dtable's parts from ds by pairs, [head][pair]: a workgroup has one head, a lane four pairs at a time and a column of sums in LDS, as k_bucket_sums.
+// float32: ds is the second of the pairs' (p, ds); bfloat16: the source side's own.
+template <typename T> struct PairDs { typedef float2 type; };
+template <> struct PairDs<bf16_t> { typedef float type; };
+template <typename T, int WAVES>
+__global__ __launch_bounds__(WAVES *WAVE) void k_bucket_pairs(const uint8_t *__restrict__ codes, const typename PairDs<T>::type *__restrict__ ds, int64_t n, int room,
+                                                              float *__restrict__ part, int heads) {
+    constexpr int U = sizeof(T) == 4 ? 2 : 4;
+    typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    float *const sums = reinterpret_cast<float *>(lds) + (threadIdx.x >> 6) * ROOM * WAVE;
-    const int lane = threadIdx.x & 63, head = (int)blockIdx.y, room = min(ROOM, n_buckets);
+    float *const sums = reinterpret_cast<float *>(lds) + (threadIdx.x >> 6) * room * WAVE;
+    const int lane = threadIdx.x & 63, head = (int)blockIdx.y;
     for (int b = 0; b < room; ++b) sums[b * WAVE + lane] = 0.f;
-    constexpr int U = 8;
-    const int64_t wave = (int64_t)blockIdx.x * WAVES + (threadIdx.x >> 6), waves = (int64_t)gridDim.x * WAVES;
-    for (int64_t i0 = wave * WAVE * U; i0 < n; i0 += waves * WAVE * U) {
-        int b[U];
-        float x[U];
-        int4 en[U];
+    const float *const ds_h = reinterpret_cast<const float *>(ds + (int64_t)head * n);
+    const int64_t wave = (int64_t)blockIdx.x * WAVES + (threadIdx.x >> 6), waves = (int64_t)gridDim.x * WAVES, whole = n & ~3;
+    for (int64_t i0 = wave * WAVE * 4 * U; i0 < whole; i0 += waves * WAVE * 4 * U) {
+        uint32_t word[U];
+        float4u x[U], y[sizeof(T) == 4 ? U : 1];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int64_t i = min(i0 + u * WAVE + lane, n - 1);
-            b[u] = i0 + u * WAVE + lane < n ? codes[i] : NO_BUCKET;
-            if constexpr (sizeof(T) == 4) en[u] = entries[i / TILE_R];
-        }
-        issue_loads_first();
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int64_t i = min(i0 + u * WAVE + lane, n - 1);
+            const int64_t i = i0 + (u * WAVE + lane) * 4, at = min(i, whole - 4);
+            word[u] = *reinterpret_cast<const uint32_t *>(codes + at);
+            if (i >= whole) word[u] = 0xFFFFFFFFu;
             if constexpr (sizeof(T) == 4) {
-                const int64_t pair = min((int64_t)tile_pair_number(en[u].z, en[u].y, (int)(i % TILE_R)), n_edges - 1);
-                x[u] = b[u] < room ? ds[(int64_t)head * n_edges + pair].y : 0.f;
+                x[u] = *reinterpret_cast<const float4u *>(ds_h + 2 * at);
+                y[u] = *reinterpret_cast<const float4u *>(ds_h + 2 * at + 4);
             } else {
-                x[u] = b[u] < room ? Elem<bf16_t>::ld(ds + (int64_t)head * n + i) : 0.f;
+                x[u] = *reinterpret_cast<const float4u *>(ds_h + at);
             }
         }
         issue_loads_first();
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (b[u] < room) sums[b[u] * WAVE + lane] += x[u];
+        for (int u = 0; u < U; ++u) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int b = (int)(word[u] >> 8 * j) & 255;
+                float v;
+                if constexpr (sizeof(T) == 4) v = j < 2 ? x[u][2 * (j & 1) + 1] : y[u][2 * (j & 1) + 1];
+                else v = x[u][j];
+                if (b < room) sums[b * WAVE + lane] += v;
+            }
+        }
+    }
+    if (blockIdx.x == 0 && (int)threadIdx.x < (int)(n - whole)) {      // (up to three behind the last four)
+        const int64_t i = whole + threadIdx.x;
+        const int b = codes[i];
+        if (b < room) sums[b * WAVE + lane] += ds_h[sizeof(T) == 4 ? 2 * i + 1 : i];
     }
     __syncthreads();
     const float *const all = reinterpret_cast<const float *>(lds);
@@ -207,24 +228,23 @@ __global__ __launch_bounds__(WAVES *WAVE) void k_bucket_places(const int4 *__res
 #pragma unroll
             for (int w = 0; w < WAVES; ++w)
 #pragma unroll
-                for (int u = 0; u < 4; ++u) v += all[((size_t)w * ROOM + b) * WAVE + 16 * u + c];
+                for (int u = 0; u < 4; ++u) v += all[((size_t)w * room + b) * WAVE + 16 * u + c];
         }
         v = head_sum<16>(v);
-        if (b < room && c == 0) part[((int64_t)blockIdx.x * n_buckets + b) * heads + head] = v;
+        if (b < room && c == 0) part[((int64_t)blockIdx.x * room + b) * heads + head] = v;
     }
 }
 
-constexpr int PLACE_PARTS = 256;
+// as many workgroups as stay on the chip at a time, of at least a turn's pairs each
+constexpr int PAIR_PARTS = 256;
 template <typename T>
-int run_places(const bpt_plan *P, const uint8_t *codes, const typename PlaceDs<T>::type *ds, int64_t n, float *part, T *dtable, int n_buckets, int heads, float factor, hipStream_t s) {
-    const int4 *const entries = (const int4 *)P->grp_entries;
-    // (512 places a turn and wavefront)
-    const int wide = n_buckets <= SUMS_WIDE, parts = (int)std::max<int64_t>(1, std::min<int64_t>(PLACE_PARTS, n / (512 * (wide ? 4 : 1)) + 1));
-    if (wide)
-        hipLaunchKernelGGL((k_bucket_places<T, 4, SUMS_WIDE>), dim3(parts, heads), dim3(4 * WAVE), 4 * SUMS_WIDE * WAVE * 4, s, entries, codes, ds, n, P->n_edges, part, n_buckets,
-                           heads);
-    else
-        hipLaunchKernelGGL((k_bucket_places<T, 1, SUMS_LONG>), dim3(parts, heads), dim3(WAVE), SUMS_LONG * WAVE * 4, s, entries, codes, ds, n, P->n_edges, part, n_buckets, heads);
+int run_pairs(int64_t n, const uint8_t *codes, const typename PairDs<T>::type *ds, float *part, T *dtable, int n_buckets, int heads, float factor, hipStream_t s) {
+    const int waves = n_buckets <= SUMS_WIDE ? 4 : 1, most = std::min(PAIR_PARTS, (1024 + heads - 1) / heads);
+    const int parts = (int)std::min<int64_t>(most, n / (512 * waves) + 1);
+    const dim3 grid((unsigned)parts, (unsigned)heads);
+    const size_t bytes = (size_t)waves * n_buckets * WAVE * 4;
+    if (waves == 4) hipLaunchKernelGGL((k_bucket_pairs<T, 4>), grid, dim3(4 * WAVE), bytes, s, codes, ds, n, n_buckets, part, heads);
+    else hipLaunchKernelGGL((k_bucket_pairs<T, 1>), grid, dim3(WAVE), bytes, s, codes, ds, n, n_buckets, part, heads);
     const int st = launch_status();
     if (st != BPT_OK) return st;
     hipLaunchKernelGGL((k_bucket_finish<T, float>), dim3((unsigned)(((int64_t)n_buckets * heads + 15) / 16)), dim3(BLOCK), 0, s, part, parts, dtable,
@@ -235,7 +255,7 @@ int run_places(const bpt_plan *P, const uint8_t *codes, const typename PlaceDs<T
 inline int64_t attention_bytes(const bpt_plan *in, const bpt_plan *out, int h, int dtype) {
     return scratch_bytes(in, out, h, dtype, false) + slope_bytes(in, h) + split_bytes(in, h, dtype == BPT_BF16) + round16((in->n_slots + 2 * out->n_slots) * (int64_t)h * 64 * 4);
 }
-inline int64_t ds_bytes(const bpt_plan *out, int h, int dtype) { return dtype == BPT_BF16 ? round16(places(out) * h * 2) : 0; }
+inline int64_t ds_bytes(const bpt_plan *out, int h, int dtype) { return dtype == BPT_BF16 ? round16(out->n_edges * h * 4) : 0; }
 
 inline bool is_type(int dtype) { return dtype == BPT_F32 || dtype == BPT_F64 || dtype == BPT_BF16; }
 inline bool is_size(int64_t n_edges, int64_t n_buckets, int h) {
@@ -279,20 +299,19 @@ int bpt_bucket_bias_backward(const void *ds, const int64_t *buckets, void *dtabl
 
 int64_t bpt_bucket_prepare_bytes(const bpt_plan *plan_in, const bpt_plan *plan_out, int h) {
     if (!plan_in || h < 1 || h > 16) return -1;
-    return table_bytes(h) + round16(places(plan_in)) + (plan_out ? round16(places(plan_out)) : 0);
+    return table_bytes(h) + round16(places(plan_in)) + (plan_out ? round16(plan_in->n_edges) + round16(places(plan_out)) : 0);
 }
 
 int bpt_bucket_prepare(const bpt_plan *plan_in, const bpt_plan *plan_out, const void *table, const int64_t *buckets, int64_t n_buckets, int heads, int h, float scale,
                        int dtype, void *prepared, void *stream) {
     if (dtype != BPT_F32 && dtype != BPT_BF16) return BPT_ERR_DTYPE;
     if (n_buckets < 1 || n_buckets > BPT_MOST_BUCKETS || heads < 1 || heads > h || h > 16 || !(fabsf(scale) > 0.f && fabsf(scale) < INFINITY)) return BPT_ERR_SIZE;
-    for (const bpt_plan *p : {plan_in, plan_out}) {
-        if (p == plan_out && !p) continue;
+    for (const bpt_plan *p : {plan_in, plan_out ? plan_out : plan_in}) {
         const int st = check_plan(p, true);
         if (st != BPT_OK) return st;
         if (p->n_groups > 0 && (!p->grp_eids || p->grp_R != TILE_R)) return BPT_ERR_PLAN;
     }
-    if (plan_out && plan_out->n_edges != plan_in->n_edges) return BPT_ERR_PLAN;
+    if (plan_out && (plan_out->n_edges != plan_in->n_edges || plan_in->n_groups == 0 || plan_out->n_groups == 0)) return BPT_ERR_PLAN;
     if (!table || !prepared || (plan_in->n_edges > 0 && !buckets)) return BPT_ERR_NULL;
     if (!aligned16(prepared)) return BPT_ERR_UNSUPPORTED;
     const Prepared pr(prepared, plan_in, h);
@@ -300,12 +319,15 @@ int bpt_bucket_prepare(const bpt_plan *plan_in, const bpt_plan *plan_out, const 
     const dim3 grid((unsigned)((most + 4 * BLOCK - 1) / (4 * BLOCK)), plan_out ? 3 : 2);
     hipStream_t s = (hipStream_t)stream;
     const int32_t *ei = place_eids(plan_in), *eo = plan_out ? place_eids(plan_out) : nullptr;
+    const bpt_plan *const summed = dtype == BPT_F32 ? plan_in : plan_out;
+    const int by_pair = plan_out ? (dtype == BPT_F32 ? 1 : 2) : 0;
+    const int4 *const entries = plan_out ? (const int4 *)summed->grp_entries : nullptr;
     if (dtype == BPT_F32)
         hipLaunchKernelGGL((k_bucket_prepare<float>), grid, dim3(BLOCK), 0, s, (const float *)table, buckets, (int)n_buckets, heads, h, 1.f / scale, plan_in->n_edges, ei, in,
-                           eo, out, pr.table, pr.codes_in, pr.codes_out);
+                           eo, out, pr.table, pr.codes_in, pr.codes_out, entries, by_pair, pr.codes_pairs);
     else
         hipLaunchKernelGGL((k_bucket_prepare<bf16_t>), grid, dim3(BLOCK), 0, s, (const bf16_t *)table, buckets, (int)n_buckets, heads, h, 1.f / scale, plan_in->n_edges, ei,
-                           in, eo, out, pr.table, pr.codes_in, pr.codes_out);
+                           in, eo, out, pr.table, pr.codes_in, pr.codes_out, entries, by_pair, pr.codes_pairs);
     return launch_status();
 }
 
@@ -321,14 +343,14 @@ int bpt_bucket_attention_forward(const bpt_plan *plan_in, const bpt_score *score
     const int64_t need = round16(plan_in->n_slots * ((int64_t)h * 64 + 2 * h) * 4);
     if (need > 0 && (!workspace || workspace_bytes < need)) return BPT_ERR_WORKSPACE;
     const Prepared pr(const_cast<void *>(prepared), plan_in, h);
-    const BucketArgs b{pr.codes_in, nullptr, pr.table, nullptr, 0};
+    const BucketArgs b{pr.codes_in, nullptr, pr.table, nullptr};
     const Dropout drop = make_dropout(dropout_p, dropout_seed);
     DISPATCH((run_forward<T, H, true>(plan_in, score, q, k, v, nullptr, o, lse, workspace, scale, drop, (hipStream_t)stream, &b)))
 }
 
 int64_t bpt_bucket_attention_backward_workspace_bytes(const bpt_plan *plan_in, const bpt_plan *plan_out, int64_t n_buckets, int heads, int h, int dtype) {
     if (!plan_in || !plan_out || h < 1 || h > 16 || heads < 1 || heads > h || n_buckets < 1 || n_buckets > BPT_MOST_BUCKETS || (dtype != BPT_F32 && dtype != BPT_BF16)) return -1;
-    return attention_bytes(plan_in, plan_out, h, dtype) + ds_bytes(plan_out, h, dtype) + (int64_t)PLACE_PARTS * n_buckets * heads * 4;
+    return attention_bytes(plan_in, plan_out, h, dtype) + ds_bytes(plan_out, h, dtype) + (int64_t)PAIR_PARTS * n_buckets * heads * 4;
 }
 
 int bpt_bucket_attention_backward(const bpt_plan *plan_in, const bpt_plan *plan_out, const bpt_score *score, const void *prepared, const void *q, const void *k, const void *v,
@@ -349,7 +371,7 @@ int bpt_bucket_attention_backward(const bpt_plan *plan_in, const bpt_plan *plan_
     if (!workspace || workspace_bytes < bpt_bucket_attention_backward_workspace_bytes(plan_in, plan_out, n_buckets, heads, h, dtype)) return BPT_ERR_WORKSPACE;
     const Prepared pr(const_cast<void *>(prepared), plan_in, h);
     char *const behind = (char *)workspace + attention_bytes(plan_in, plan_out, h, dtype);
-    const BucketArgs b{pr.codes_in, pr.codes_out, pr.table, dtable && dtype == BPT_BF16 ? (bf16_t *)behind : nullptr, places(plan_out)};
+    const BucketArgs b{pr.codes_in, pr.codes_out, pr.table, dtable && dtype == BPT_BF16 ? (float *)behind : nullptr};
     float *const part = (float *)(behind + ds_bytes(plan_out, h, dtype));
     const Dropout drop = make_dropout(dropout_p, dropout_seed);
     hipStream_t s = (hipStream_t)stream;
@@ -359,8 +381,8 @@ int bpt_bucket_attention_backward(const bpt_plan *plan_in, const bpt_plan *plan_
     st = attention();
     if (st != BPT_OK || !dtable) return st;
     if (dtype == BPT_F32)
-        return run_places<float>(plan_in, pr.codes_in, (const float2 *)workspace, places(plan_in), part, (float *)dtable, (int)n_buckets, heads, 1.f / scale, s);
-    return run_places<bf16_t>(plan_out, pr.codes_out, (const bf16_t *)behind, places(plan_out), part, (bf16_t *)dtable, (int)n_buckets, heads, 1.f / scale, s);
+        return run_pairs<float>(plan_in->n_edges, pr.codes_pairs, (const float2 *)workspace, part, (float *)dtable, n_buckets, heads, 1.f / scale, s);
+    return run_pairs<bf16_t>(plan_in->n_edges, pr.codes_pairs, (const float *)behind, part, (bf16_t *)dtable, n_buckets, heads, 1.f / scale, s);
 }
 
 }  // extern "C"

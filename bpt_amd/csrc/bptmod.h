@@ -597,8 +597,7 @@ inline ScoreMod make_mod(const bpt_score *sc, float scale, bool entries_are_keys
 struct BucketArgs {
     const uint8_t *codes_in, *codes_out;
     const float *table;
-    bf16_t *ds;
-    int64_t places_out;
+    float *ds;
 };
 template <bool BUCKETS> inline typename ModArg<true, BUCKETS>::type with_buckets(const ScoreMod &m, const BucketArgs *b, bool entries_are_keys) {
     if constexpr (BUCKETS) {
@@ -607,7 +606,6 @@ template <bool BUCKETS> inline typename ModArg<true, BUCKETS>::type with_buckets
         r.codes = entries_are_keys ? b->codes_in : b->codes_out;
         r.table = b->table;
         r.ds = b->ds;
-        r.places = b->places_out;
         return r;
     } else {
         return m;

@@ -982,8 +982,7 @@ struct ScoreMod {
 struct BucketMod : ScoreMod {
     const uint8_t *codes;              // [entry][member] of the plan's groups, or of its slots where it has none; NO_BUCKET: none
     const float *table;                // [head][256], 0 at NO_BUCKET
-    bf16_t *ds;                        // bfloat16 source side: [head][entry][member], dL/d(q.k) of the pairs that exist, or null
-    int64_t places;                    // entries x members
+    float *ds;                         // bfloat16 source side: [head][number of the pair], dL/d(q.k), or null
 };
 constexpr int NO_BUCKET = 255;
 struct NoMod {};
@@ -2747,6 +2746,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(MOD ?
     __shared__ __attribute__((aligned(16))) float piece[HW][PIECE];
     __shared__ __attribute__((aligned(16))) float pos_lds[HW][MOD ? TILE_R : 4];
     __shared__ float tab_lds[BUCKETS ? HW : 1][BUCKETS ? 256 : 1];
+    __shared__ int fst_lds[BUCKETS ? HW : 1][BUCKETS ? TILE_CHUNK : 1];            // numbers of the entries' first pairs
     if constexpr (BUCKETS) tile_put_table(md, t.head, t.lane, tab_lds[t.wv]);      // (read behind the fences of the first block)
     int2 *ent = reinterpret_cast<int2 *>(piece[t.wv]);
     char *const q_lds = reinterpret_cast<char *>(piece[t.wv] + ENT), *const d_lds = q_lds + 4 * TILE_ROWS_FLOATS_BF16;
@@ -2794,7 +2794,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(MOD ?
     for (int p0 = t.p_begin; p0 < t.p_end; p0 += TILE_CHUNK) {
         const int cnt = min(TILE_CHUNK, t.p_end - p0), nblk = (cnt + TILE_R - 1) / TILE_R;
         if (p0 != t.p_begin) tile_ask_entries(P, p0, cnt, t.lane, er);
-        tile_put_entries(er, ent, cnt, t.lane);
+        tile_put_entries(er, ent, cnt, t.lane, BUCKETS ? fst_lds[t.wv] : nullptr);
         auto issue = [&](Blk &B, int b) {
             if constexpr (DROP) tile_pair_eids(P, p0 + TILE_R * b + 4 * g, t.p_end, c, B.xe);
             if constexpr (BUCKETS) tile_pair_codes(md, p0 + TILE_R * b + 4 * g, t.p_end, c, B.code);
@@ -2852,7 +2852,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(MOD ?
                 ds[r] = where_pair_or_zero(mk[r], c, MOD ? p * (dp[r] * mt - delta_e[r]) * du[r] : p * (dp[r] * mt - delta_e[r]) * scale);
                 pe[r] = p * mt;
                 if constexpr (BUCKETS) {
-                    if (md.ds && ((mk[r] >> c) & 1)) Elem<bf16_t>::st(md.ds + (size_t)t.head * md.places + (size_t)(p0 + TILE_R * b + 4 * g + r) * TILE_R + c, ds[r]);
+                    if (md.ds && ((mk[r] >> c) & 1)) md.ds[(size_t)t.head * P.n_edges + tile_pair_number(fst_lds[t.wv][TILE_R * b + 4 * g + r], mk[r], c)] = ds[r];
                 }
             }
             if constexpr (CAREFUL) {

@@ -105,6 +105,17 @@ template <typename T> struct Epilogue {
     int act;
     Drop drop;
     bool quads;                  // rows, and with them quads, start on four elements everywhere
+    // four columns, of rows that start on four, of an activation and dropout that the caller has looked up; bias of the columns, residual as read ahead
+    template <int ACT, bool DROP> __device__ __forceinline__ void quad(floatx4 v, int64_t at, floatx4 b, floatx4 ahead) const {
+        v = v * scale + b;
+        if constexpr (ACT != BPT_ACT_NONE) {
+            if (kept) store4(kept + at, v);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = activated(v[e], ACT);
+        }
+        if constexpr (DROP) v = dropped(v, philox((uint64_t)at >> 2, drop.k0, drop.k1), drop);
+        store4(y + at, v + ahead);
+    }
     // what the result is added to, where it is read ahead
     __device__ __forceinline__ floatx4 ask(int64_t row, int64_t col) const {
         return quads && residual ? load4(residual + row * cols + col) : floatx4{0.f, 0.f, 0.f, 0.f};
@@ -154,7 +165,8 @@ template <typename T> struct Epilogue {
 // spread over the banks.  One that has the reduction outside lies as rows of the tile's elements; float32 fragments are read word by word, bfloat16
 // ones by transposing loads (lane i of sixteen gives the address of 4 columns of row i / 4 and gets column i of four rows), and chunks are
 // shifted by row so that the four lane groups meet different banks.
-// Rows that do not start on 4 bytes, and the last piece of a ragged reduction, go through registers, where what lies outside is made zero.
+// The last step of a ragged reduction loads what lies behind it too (up to the matrix' end, where the descriptor ends), and its fragments are made zero there.
+// Rows that do not start on 4 bytes, and float32's last step, go through registers, where what lies outside is made zero.
 template <typename T, int RB> constexpr int step() { return RB / (int)sizeof(T); }     // the reduction's share of one buffer
 
 // (sixteen-byte reads go to LDS sixteen lanes at a time, of lanes 0 .. 31 those of rows 0 - 3 and 12 - 15 of one chunk with rows 4 - 11 of the next)
@@ -180,14 +192,18 @@ template <typename T> __device__ __forceinline__ uintx4 load_upto(const T *p, in
     return uintx4{(uint32_t)half[0], (uint32_t)(half[0] >> 32), (uint32_t)half[1], (uint32_t)(half[1] >> 32)};
 }
 
-// Sixteen bytes a lane from memory straight to LDS, lane l's to byte 16 l from `to` on (of the wavefront): a buffer descriptor of the whole address range from a
-// uniform start and an offset a lane, so nothing is added per lane and load.  In assembly, because the compiler takes every transposing read of LDS for one that may
+// Sixteen bytes a lane from memory straight to LDS, lane l's to byte 16 l from `to` on (of the wavefront): a buffer descriptor of the matrix from a
+// uniform start to its end, behind which nothing is read, and an offset a lane, so nothing is added per lane and load.  In assembly, because the compiler takes every transposing read of LDS for one that may
 // read what is still on its way and waits for it; the waits are written where they belong (wait_and_meet), and no register is written.
 __device__ __forceinline__ uint32_t lds_place(const char *p) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char *)p; }
-__device__ __forceinline__ uintx4 whole_memory(const void *p) {
-    const uint64_t at = (uint64_t)p;
-    uintx4 d{(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)at), (uint32_t)__builtin_amdgcn_readfirstlane((int)((uint32_t)(at >> 32) & 0xffffu)), 0xffffffffu,
-             0x00027000u};
+__device__ __forceinline__ uint64_t uniform(uint64_t x) {
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)x);
+}
+__device__ __forceinline__ uintx4 memory_from(uint64_t at, uint64_t end) {      // (both uniform)
+    const uint64_t bytes = end - at;
+    uint32_t high = (uint32_t)(bytes >> 32);
+    asm volatile("" : "+s"(high));                                 // (a minimum of 64 bits would be a vector comparison)
+    uintx4 d{(uint32_t)at, (uint32_t)(at >> 32) & 0xffffu, high ? 0xffffffffu : (uint32_t)bytes, 0x00027000u};
     asm volatile("s_nop 4" : "+s"(d));                             // (a scalar register that a vector instruction wrote may be read by a load five states later)
     return d;
 }
@@ -199,6 +215,8 @@ __device__ __forceinline__ void load_to_lds(uintx4 from, uint32_t offset, uint32
 template <typename T, int TB, int RB, int WAVES, bool COLS> struct Stage {
     static constexpr int N = TB * RB / 16 / (WAVES * WAVE), VE = ve<T>(), CHUNKS = COLS ? TB * (int)sizeof(T) / 16 : RB / 16;
     const T *base;               // of this tile's first row (column) and the first step
+    uint64_t from, end;          // its address, that behind the matrix, and from step to step
+    int64_t apart;
     int64_t ld, stride;          // elements of a row in memory; from step to step
     int left, reduce;            // rows (columns) from base on; the reduction's length from base on
     uint32_t off[N];             // bytes from base, of a lane's vectors where they are whole
@@ -213,7 +231,10 @@ template <typename T, int TB, int RB, int WAVES, bool COLS> struct Stage {
     __device__ __forceinline__ Stage(const T *p, int64_t ld_, int64_t n, int64_t reduce_, int64_t t, int64_t s) : ld(ld_) {
         const int64_t r0 = s * step<T, RB>();
         base = COLS ? p + r0 * ld + t : p + t * ld + r0;
+        from = uniform((uint64_t)base);
+        end = uniform((uint64_t)(p + ((COLS ? reduce_ : n) - 1) * ld + (COLS ? n : reduce_)));
         stride = COLS ? ld * step<T, RB>() : step<T, RB>();
+        apart = (int64_t)uniform((uint64_t)(stride * (int64_t)sizeof(T)));
         left = (int)(n - t < TB ? n - t : TB);
         reduce = (int)(reduce_ - r0);
 #pragma unroll
@@ -225,9 +246,9 @@ template <typename T, int TB, int RB, int WAVES, bool COLS> struct Stage {
     }
     __device__ __forceinline__ void direct(int s, const char *lds) const {
         const uint32_t to = __builtin_amdgcn_readfirstlane(lds_place(lds) + (threadIdx.x >> 6) * (WAVE * 16));
-        const uintx4 from = whole_memory(base + s * stride);
+        const uintx4 here = memory_from(from + s * apart, end);
 #pragma unroll
-        for (int i = 0; i < N; ++i) load_to_lds(from, off[i], to + i * (WAVES * WAVE * 16));
+        for (int i = 0; i < N; ++i) load_to_lds(here, off[i], to + i * (WAVES * WAVE * 16));
     }
     __device__ __forceinline__ void load(int s, uintx4 (&v)[N]) const {
         const T *const at = base + s * stride;
@@ -394,9 +415,7 @@ __global__ __launch_bounds__(S::THREADS, S::PER_SIMD) void k_linear_tiles(const 
     int s = 0;
     if constexpr (DIRECT) {
         constexpr int LOADS = StageA::N + StageB::N;
-        // (the vector with a row's last element may run into the next row: not of the last row of all)
-        const int crosses = (ACOLS && m.P % ve<T>() != 0) || (BCOLS && m.Q % ve<T>() != 0);
-        const int whole = min(n, (sa.reduce - crosses) / step<T, RB>());
+        const int whole = min(n, sa.reduce / step<T, RB>());       // (of n steps; the one behind them is ragged)
         auto ask = [&](int t) {
             char *const at = lds + (t & 1) * BUFFER;
             sa.direct(t, at);
@@ -413,9 +432,9 @@ __global__ __launch_bounds__(S::THREADS, S::PER_SIMD) void k_linear_tiles(const 
             // Half a step's products run while the other half's fragments, or the next step's first, are read:
             //   products of (s, 0), reads of (s, 1)  |  step s + 1 is there, step s has been read by all: step s + 2 is asked for  |  products of (s, 1), reads of (s + 1, 0)
             constexpr int READS = FP * (ACOLS ? (sizeof(T) == 4 ? 4 : 2) : 1) + FQ * (BCOLS ? (sizeof(T) == 4 ? 4 : 2) : 1), PRODUCTS = FP * FQ * (sizeof(T) == 4 ? 4 : 1);
-            if (whole > 0) {
+            if (n > 0) {
                 ask(0);
-                if (whole > 1) {
+                if (n > 1) {
                     ask(1);
                     wait_and_meet<LOADS>();
                 } else {
@@ -430,12 +449,30 @@ __global__ __launch_bounds__(S::THREADS, S::PER_SIMD) void k_linear_tiles(const 
                 products(0);
                 in_turn<READS, PRODUCTS>();
                 wait_and_meet<0>();
-                if (s + 2 < whole) ask(s + 2);
+                if (s + 2 < n) ask(s + 2);
                 issue_loads_first();
                 read(0, lds + (~s & 1) * BUFFER, 0);               // (behind the last step: what the buffer held, for nobody)
                 products(1);
                 in_turn<READS, PRODUCTS>();
                 issue_loads_first();
+            }
+            if (s < n) {
+                read(1, lds + (s & 1) * BUFFER, 1);
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const int there = sa.reduce - s * step<T, RB>() - (half * 4 + (lane >> 4)) * ve<T>();      // of the lane's elements
+                    static_assert(sizeof(T) == 2, "");
+#pragma unroll
+                    for (int d = 0; d < 4; ++d) {
+                        const uint32_t mask = there >= 2 * d + 2 ? 0xffffffffu : there == 2 * d + 1 ? 0xffffu : 0u;
+#pragma unroll
+                        for (int i = 0; i < FP; ++i) fa[half][i][d] &= mask;
+#pragma unroll
+                        for (int j = 0; j < FQ; ++j) fb[half][j][d] &= mask;
+                    }
+                    products(half);
+                }
+                s = n;
             }
         }
     }
@@ -490,47 +527,86 @@ __global__ __launch_bounds__(S::THREADS, S::PER_SIMD) void k_linear_tiles(const 
     constexpr int QUADS = BP / 4, TURNS = ROWS * QUADS / S::THREADS, U = 4;
     floatx4 *const sums = reinterpret_cast<floatx4 *>(lds);
     const int quad = threadIdx.x % QUADS;
-    const int64_t p = p0 + quad * 4, left = m.Q - q0;
-#pragma unroll
-    for (int pass = 0; pass < PASSES; ++pass) {
-        __syncthreads();
+    const int64_t p = p0 + quad * 4;
+    const int left = (int)(m.Q - q0 < BQ ? m.Q - q0 : BQ);
+    const bool mine = p < m.P;
+    const floatx4 none{0.f, 0.f, 0.f, 0.f}, bias = mine && out.quads && out.bias && !part ? load4(out.bias + p) : none;
+    auto put = [&](auto pass) {
 #pragma unroll
         for (int j = 0; j < JS; ++j)
 #pragma unroll
             for (int i = 0; i < FP; ++i) {
                 const int r = w / S::GP * (16 * JS) + 16 * j + (lane & 15), to = (wp + 16 * i) / 4 + (lane >> 4);
-                sums[r * QUADS + (to ^ (r & (QUADS - 1)))] = acc[i][pass * JS + j];
+                sums[r * QUADS + (to ^ (r & (QUADS - 1)))] = acc[i][pass() * JS + j];
             }
-        __syncthreads();
-        if (p >= m.P) continue;
+    };
 #pragma unroll 1
-        for (int u0 = 0; u0 < TURNS; u0 += U) {
-            floatx4 ahead[U];
-            int r[U], q[U];
+    for (int pass = 0; pass < PASSES; ++pass) {
+        auto line = [&](int u) { return u * (S::THREADS / QUADS) + (int)threadIdx.x / QUADS; };                         // of the sums,
+        auto row = [&](int u) { return line(u) / (16 * JS) * WQ + pass * (16 * JS) + line(u) % (16 * JS); };            // of the tile
+        auto sum = [&](int u) { return sums[line(u) * QUADS + (quad ^ (line(u) & (QUADS - 1)))]; };
+        auto at = [&](int u) { return (q0 + row(u)) * m.P + p; };
+        floatx4 ahead[U];
+        auto ask = [&](int u0) {
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                r[u] = (u0 + u) * (S::THREADS / QUADS) + threadIdx.x / QUADS;
-                q[u] = r[u] / (16 * JS) * WQ + pass * (16 * JS) + r[u] % (16 * JS);
-                if (q[u] < left && !part) ahead[u] = out.ask(q0 + q[u], p);
-            }
-            issue_loads_first();
+            for (int u = 0; u < U; ++u) ahead[u] = row(u0 + u) < left ? load4(out.residual + at(u0 + u)) : none;
+        };
+        const bool added = mine && out.quads && out.residual && !part;
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                if (q[u] >= left) continue;
-                const floatx4 v = sums[r[u] * QUADS + (quad ^ (r[u] & (QUADS - 1)))];
-                if (!part) {
-                    out(v, q0 + q[u], p, ahead[u]);
-                    continue;
-                }
-                float *const to = part + ((int64_t)split * m.Q + q0 + q[u]) * m.P + p;
+        for (int u = 0; u < U; ++u) ahead[u] = none;
+        if (added) ask(0);
+        __syncthreads();
+        if (PASSES == 1 || pass == 0) put(std::integral_constant<int, 0>{});
+        else put(std::integral_constant<int, PASSES - 1>{});
+        __syncthreads();
+        if (!mine) continue;
+        if (part) {
+            float *const to = part + (int64_t)split * m.Q * m.P;
+#pragma unroll U
+            for (int u = 0; u < TURNS; ++u) {
+                if (row(u) >= left) continue;
+                const floatx4 v = sum(u);
                 if ((m.P & 3) == 0) {
-                    store4(to, v);
+                    store4(to + at(u), v);
                 } else {
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        if (p + e < m.P) to[e] = v[e];
+                        if (p + e < m.P) to[at(u) + e] = v[e];
                 }
             }
+            continue;
+        }
+        if (!out.quads) {
+#pragma unroll 1
+            for (int u = 0; u < TURNS; ++u)
+                if (row(u) < left) out(sum(u), q0 + row(u), p, none);
+            continue;
+        }
+        // a loop for each activation, with dropout or without (asked for each four columns, that took 7 us of 50 of a product of 33598 x 300 -> 600 without any)
+        auto leave = [&](auto act, auto drop) {
+#pragma unroll 1
+            for (int u0 = 0; u0 < TURNS; u0 += U) {
+                floatx4 now[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) now[u] = ahead[u];
+                if (added && u0 + U < TURNS) ask(u0 + U);
+                issue_loads_first();
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (row(u0 + u) < left) out.template quad<act(), drop()>(sum(u0 + u), at(u0 + u), bias, now[u]);
+            }
+        };
+        using std::integral_constant;
+        auto with_drop = [&](auto act) {
+            if (out.drop.thr) leave(act, integral_constant<bool, true>{});
+            else leave(act, integral_constant<bool, false>{});
+        };
+        if constexpr (ACOLS || BCOLS) {                            // (the backward's products: nothing follows them)
+            leave(integral_constant<int, BPT_ACT_NONE>{}, integral_constant<bool, false>{});
+        } else {
+            if (out.act == BPT_ACT_RELU) with_drop(integral_constant<int, BPT_ACT_RELU>{});
+            else if (out.act == BPT_ACT_GELU) with_drop(integral_constant<int, BPT_ACT_GELU>{});
+            else with_drop(integral_constant<int, BPT_ACT_NONE>{});
         }
     }
 }

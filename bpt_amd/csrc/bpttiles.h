@@ -994,10 +994,17 @@ __device__ __forceinline__ void tile_put_table(const BucketMod &md, int head, in
 #pragma unroll
     for (int i = 0; i < 4; ++i) to[i * WAVE + lane] = md.table[(size_t)head * 256 + i * WAVE + lane];
 }
-__device__ __forceinline__ void tile_pair_codes(const BucketMod &md, int first_entry, int p_end, int c, int (&code)[4], int step = 1) {
+// float32: the codes of a lane's four places of a block, a byte each
+__device__ __forceinline__ void tile_pair_codes(const BucketMod &md, int first_entry, int p_end, int c, int (&code)[4]) {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) code[r] = md.codes[(size_t)min(first_entry + step * r, p_end - 1) * TILE_R + c];
+    for (int r = 0; r < 4; ++r) code[r] = md.codes[(size_t)min(first_entry + 4 * r, p_end - 1) * TILE_R + c];
 }
+// bfloat16: of a block's 16 x 16 places, four of an entry a lane, one load where those are four: entry lane / 4, members 4 (lane % 4) ..; and of one place, of the block's
+// entry e and this lane's member c (us, L = 32768, k = 8, 16 heads, forward and backward 184 + 262 + 419 -> 167 + 236 + 400; float32, L = 8192: 36 + 57 -> 37 + 59)
+__device__ __forceinline__ int tile_ask_codes(const BucketMod &md, int first_entry, int p_end, int lane) {
+    return reinterpret_cast<const int *>(md.codes)[(size_t)min(first_entry + (lane >> 2), p_end - 1) * 4 + (lane & 3)];
+}
+__device__ __forceinline__ int tile_code(int codes, int e, int c) { return __builtin_amdgcn_ds_bpermute((e * 4 + (c >> 2)) * 4, codes) >> 8 * (c & 3) & 255; }
 
 // What stands in rows that are not a member's neighbours must not reach its sums, and a product over a block's entries lets it: 0 x NaN.  So a wavefront whose
 // sums (of any member) are not finite walks its tile once more (CAREFUL), with products that add the existing pairs alone and with every
@@ -1202,7 +1209,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(4))) 
         };
         auto issue_rest = [&](Blk &B, int b) {
             if constexpr (DROP || BIAS == 1) tile_pair_eids(P, p0 + TILE_R * b + g, t.p_end, c, B.xe, 4);
-            if constexpr (BUCKETS) tile_pair_codes(md, p0 + TILE_R * b + g, t.p_end, c, B.code, 4);
+            if constexpr (BUCKETS) tile_pair_codes(md, p0 + TILE_R * b + g, t.p_end, c, B.code);
             B.nv = min(TILE_R, cnt - TILE_R * b);
             if constexpr (MOD) {
                 if (md.slopes && g == 0) B.pos = md.pos_entry[ent[TILE_R * b + c].x];
@@ -1433,7 +1440,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP 
         tile_put_entries(er, ent, cnt, t.lane, fst);
         auto issue = [&](Blk &B, int b) {
             if constexpr (DROP || BIAS == 1) tile_pair_eids(P, p0 + TILE_R * b + g, t.p_end, c, B.xe, 4);
-            if constexpr (BUCKETS) tile_pair_codes(md, p0 + TILE_R * b + g, t.p_end, c, B.code, 4);
+            if constexpr (BUCKETS) tile_pair_codes(md, p0 + TILE_R * b + g, t.p_end, c, B.code);
             B.b = b;
             if constexpr (MOD) {
                 if (md.slopes && g == 0) B.pos = md.pos_entry[ent[TILE_R * b + c].x];
@@ -1939,7 +1946,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP 
         int xe[DROP || BIAS == 1 ? 4 : 1];
         float bz[BIAS ? 4 : 1];
         float pos;                                                // of entry c, in the first lane group
-        int code[BUCKETS ? 4 : 1];
+        int codes;                                                // BUCKETS: of the block's places (tile_ask_codes)
     };
     auto walk = [&](auto again) __attribute__((always_inline)) {
     constexpr bool CAREFUL = decltype(again)::value;
@@ -1950,7 +1957,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP 
         tile_put_entries(er, ent, cnt, t.lane, fst);
         auto issue = [&](Blk &B, int b) {
             if constexpr (DROP || BIAS == 1) tile_pair_eids(P, p0 + TILE_R * b + 4 * g, t.p_end, c, B.xe);
-            if constexpr (BUCKETS) tile_pair_codes(md, p0 + TILE_R * b + 4 * g, t.p_end, c, B.code);
+            if constexpr (BUCKETS) B.codes = tile_ask_codes(md, p0 + TILE_R * b, t.p_end, t.lane);
             if constexpr (MOD) {
                 if (md.slopes && g == 0) B.pos = md.pos_entry[ent[TILE_R * b + c].x];
             }
@@ -1979,13 +1986,13 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP 
             wave_lds_fence();
         }
         for (int b = 0; b < nblk; ++b) {
-            int mk[4], xe[DROP ? 4 : 1], code[BUCKETS ? 4 : 1];
+            int mk[4], xe[DROP ? 4 : 1], codes = 0;
             float bz[BIAS ? 4 : 1];
             tile_masks(ent + TILE_R * b, g, mk);
+            if constexpr (BUCKETS) codes = B.codes;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 if constexpr (DROP) xe[DROP ? r : 0] = B.xe[DROP ? r : 0];
-                if constexpr (BUCKETS) code[r] = B.code[r];
                 if constexpr (BIAS) bz[BIAS ? r : 0] = B.bz[BIAS ? r : 0];
             }
             tile_put_rows_bf16(k_lds, B.kr, t.lane);
@@ -2008,7 +2015,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(DROP 
                 for (int r = 0; r < 4; ++r) x[r] = BIAS ? st[r] + bz[BIAS ? r : 0] : st[r];
                 if constexpr (BUCKETS) {
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) x[r] += tab_lds[t.wv][code[r]];
+                    for (int r = 0; r < 4; ++r) x[r] += tab_lds[t.wv][tile_code(codes, 4 * g + r, c)];
                 }
                 tile_mod_scores(md, scale_log2e, slope, pos_m, pos_e, x, sc, du);
 #pragma unroll
@@ -2177,7 +2184,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(MOD ?
         int xe[DROP || BIAS == 1 ? 4 : 1];
         float bz[BIAS ? 4 : 1];
         float pos;                                                // of entry c, in the first lane group
-        int code[BUCKETS ? 4 : 1];
+        int codes;                                                // BUCKETS: of the block's places (tile_ask_codes)
     };
     auto walk = [&](auto again) __attribute__((always_inline)) {
     constexpr bool CAREFUL = decltype(again)::value;
@@ -2193,7 +2200,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(MOD ?
         };
         auto issue = [&](Blk &B, int b) {
             if constexpr (DROP || BIAS == 1) tile_pair_eids(P, p0 + TILE_R * b + 4 * g, t.p_end, c, B.xe);
-            if constexpr (BUCKETS) tile_pair_codes(md, p0 + TILE_R * b + 4 * g, t.p_end, c, B.code);
+            if constexpr (BUCKETS) B.codes = tile_ask_codes(md, p0 + TILE_R * b, t.p_end, t.lane);
             if constexpr (MOD) {
                 if (md.slopes && g == 0) B.pos = md.pos_entry[ent[TILE_R * b + c].x];
             }
@@ -2213,16 +2220,16 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(MOD ?
         Blk B;
         issue(B, 0);
         for (int b = 0; b < nblk; ++b) {
-            int mk[4], xe[DROP || BIAS == 1 ? 4 : 1], code[BUCKETS ? 4 : 1];
+            int mk[4], xe[DROP || BIAS == 1 ? 4 : 1], codes = 0;
             float bz[BIAS ? 4 : 1];
             uint32_t pos[4];
             tile_masks(ent + TILE_R * b, g, mk);
+            if constexpr (BUCKETS) codes = B.codes;
             if constexpr (PDS) numbers(b, mk, pos);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 if constexpr (DROP || BIAS == 1) xe[DROP || BIAS == 1 ? r : 0] = B.xe[DROP || BIAS == 1 ? r : 0];
                 if constexpr (BIAS) bz[BIAS ? r : 0] = B.bz[BIAS ? r : 0];
-                if constexpr (BUCKETS) code[r] = B.code[r];
             }
             tile_put_rows_bf16(k_lds, B.kr, t.lane);
             tile_put_rows_bf16(v_lds, B.vr, t.lane);
@@ -2244,7 +2251,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(MOD ?
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     x[r] = BIAS ? st[r] + bz[BIAS ? r : 0] : st[r];
-                    if constexpr (BUCKETS) x[r] += tab_lds[t.wv][code[r]];
+                    if constexpr (BUCKETS) x[r] += tab_lds[t.wv][tile_code(codes, 4 * g + r, c)];
                     pos_e[r] = at_e[r];
                 }
                 tile_mod_scores(md, scale_log2e, slope, pos_m, pos_e, x, sm, du);
@@ -2786,7 +2793,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(MOD ?
         float2 ld;                                                // (lse, delta) of entry c, in the first lane group
         int xe[DROP ? 4 : 1];
         float pos;                                                // of entry c, in the first lane group
-        int code[BUCKETS ? 4 : 1];
+        int codes;                                                // BUCKETS: of the block's places (tile_ask_codes)
     };
     auto walk = [&](auto again) __attribute__((always_inline)) {
     constexpr bool CAREFUL = decltype(again)::value;
@@ -2797,7 +2804,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(MOD ?
         tile_put_entries(er, ent, cnt, t.lane, BUCKETS ? fst_lds[t.wv] : nullptr);
         auto issue = [&](Blk &B, int b) {
             if constexpr (DROP) tile_pair_eids(P, p0 + TILE_R * b + 4 * g, t.p_end, c, B.xe);
-            if constexpr (BUCKETS) tile_pair_codes(md, p0 + TILE_R * b + 4 * g, t.p_end, c, B.code);
+            if constexpr (BUCKETS) B.codes = tile_ask_codes(md, p0 + TILE_R * b, t.p_end, t.lane);
             if constexpr (MOD) {
                 if (md.slopes && g == 0) B.pos = md.pos_entry[ent[TILE_R * b + c].x];
             }
@@ -2810,12 +2817,11 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(MOD ?
         Blk B;
         issue(B, 0);
         for (int b = 0; b < nblk; ++b) {
-            int mk[4], xe[DROP ? 4 : 1], code[BUCKETS ? 4 : 1];
+            int mk[4], xe[DROP ? 4 : 1], codes = 0;
             tile_masks(ent + TILE_R * b, g, mk);
+            if constexpr (BUCKETS) codes = B.codes;
 #pragma unroll
             for (int r = 0; r < (DROP ? 4 : 0); ++r) xe[r] = B.xe[r];
-#pragma unroll
-            for (int r = 0; r < (BUCKETS ? 4 : 0); ++r) code[r] = B.code[r];
             tile_put_rows_bf16(q_lds, B.qr, t.lane);
             tile_put_rows_bf16(d_lds, B.dr, t.lane);
             if (g == 0) st_lds[c] = B.ld;
@@ -2839,7 +2845,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(MOD ?
                 float x[4] = {st[0], st[1], st[2], st[3]};
                 if constexpr (BUCKETS) {
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) x[r] += tab_lds[t.wv][code[r]];
+                    for (int r = 0; r < 4; ++r) x[r] += tab_lds[t.wv][tile_code(codes, 4 * g + r, c)];
                 }
                 tile_mod_scores(md, scale_log2e, slope, pos_m, pos_e, x, sm, du);
             }
@@ -2852,6 +2858,7 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(MOD ?
                 ds[r] = where_pair_or_zero(mk[r], c, MOD ? p * (dp[r] * mt - delta_e[r]) * du[r] : p * (dp[r] * mt - delta_e[r]) * scale);
                 pe[r] = p * mt;
                 if constexpr (BUCKETS) {
+                    // (gathered in LDS and left as one run of memory: 400 -> 417 us at L = 32768, k = 8; past the cache: 437)
                     if (md.ds && ((mk[r] >> c) & 1)) md.ds[(size_t)t.head * P.n_edges + tile_pair_number(fst_lds[t.wv][TILE_R * b + 4 * g + r], mk[r], c)] = ds[r];
                 }
             }

@@ -2841,12 +2841,11 @@ __global__ __launch_bounds__(HW * WAVE) __attribute__((amdgpu_waves_per_eu(MOD ?
             float pe[4], ds[4], sm[4], du[4];
             if constexpr (MOD) {
                 const floatx4v at_e = *reinterpret_cast<const floatx4v *>(&pos_lds[t.wv][4 * g]);
-                const float pos_e[4] = {at_e[0], at_e[1], at_e[2], at_e[3]};
-                float x[4] = {st[0], st[1], st[2], st[3]};
-                if constexpr (BUCKETS) {
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) x[r] += tab_lds[t.wv][tile_code(codes, 4 * g + r, c)];
-                }
+                auto scored = [&](int r) {
+                    if constexpr (BUCKETS) return st[r] + tab_lds[t.wv][tile_code(codes, 4 * g + r, c)];
+                    else return st[r];
+                };
+                const float pos_e[4] = {at_e[0], at_e[1], at_e[2], at_e[3]}, x[4] = {scored(0), scored(1), scored(2), scored(3)};
                 tile_mod_scores(md, scale_log2e, slope, pos_m, pos_e, x, sm, du);
             }
 #pragma unroll

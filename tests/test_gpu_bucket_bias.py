@@ -352,3 +352,81 @@ def test_refusals():
         op.bpt_attention(*args, *(torch.randn(c["q"].size(0), 2, 80, device=DEV) for _ in range(3)), fused=True, bias_table=t[:, :2].contiguous(), buckets=b)
     strided = go(bias_table=t.t().contiguous().t(), buckets=torch.stack([b, b], 1)[:, 0].contiguous())
     assert torch.equal(strided, go(bias_table=t, buckets=b))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n", [255, 256])
+def test_as_many_buckets_as_a_byte_counts(n, dtype):
+    check(make(("bpt", 900, 4), 8, 64, dtype, n=n), fused=True)
+
+
+@pytest.mark.parametrize("scale", [-0.2, 1.5])
+@pytest.mark.parametrize("heads,d,dtype", [(8, 64, "f32"), (6, 50, "bf16")])
+def test_scales(heads, d, dtype, scale):
+    """The bias is added behind the scale, whatever its sign and size."""
+    from bpt_amd import op
+    c = make(("bpt", 300, 4), heads, d, dtype)
+    args = graph_args(c["src"].numpy(), c["dst"].numpy(), c["q"].size(0), c["k"].size(0))
+    dev = on_device(c)
+    o = call(c, dev, args, scale=scale)
+    e = (dev["q"].double()[c["dst"].to(DEV)] * dev["k"].double()[c["src"].to(DEV)]).sum(-1) * scale
+    b = c["buckets"].to(DEV)
+    there = (b >= 0) & (b < 20)
+    e = e + torch.where(there[:, None], dev["bias_table"].double()[torch.where(there, b, 0)], 0.0)
+    dst, src = c["dst"].to(DEV), c["src"].to(DEV)
+    w = torch.exp(e - e.max())
+    total = torch.zeros(c["q"].size(0), heads, dtype=torch.float64, device=DEV).index_add(0, dst, w)
+    want = torch.zeros(o.shape, dtype=torch.float64, device=DEV).index_add(0, dst, (w / total[dst])[:, :, None] * dev["v"].double()[src])
+    half = torch.finfo(c["q"].dtype).eps / 2
+    # 300 terms of a row at most: scores up to 40 with 72 2^-24 of the products' absolute values twice, p and o rounded once each
+    assert ((o.double() - want).abs() <= (2 * half + 2.0 ** -13) * (1 + dev["v"].abs().max().double())).all()
+    got = torch.autograd.grad(o, [dev[n] for n in ("q", "k", "v", "bias_table")], dev["do"])
+    ref = torch.autograd.grad(want, [dev[n] for n in ("q", "k", "v", "bias_table")], dev["do"].double())
+    for x, y in zip(got, ref):
+        assert (x.double() - y.double()).norm() <= (8 * half + 2.0 ** -12) * y.double().norm()
+
+
+def test_some_of_the_gradients():
+    c = make(("bpt", 300, 4), 8, 64, "f32", distance=True)
+    args = graph_args(c["src"].numpy(), c["dst"].numpy(), c["q"].size(0), c["k"].size(0))
+    everything = run(c, args)
+    for names in (["bias_table"], ["slopes"], ["q"], ["v", "bias_table"], ["k", "slopes"]):
+        dev = {n: t.to(DEV).requires_grad_(n in names) for n, t in c.items() if torch.is_tensor(t)}
+        o = call(c, dev, args)
+        for n, g in zip(names, torch.autograd.grad(o, [dev[n] for n in names], dev["do"])):
+            assert torch.equal(g, everything["d" + n]), n
+
+
+def test_views_and_saved_tensors_that_went_elsewhere():
+    c = make(("bpt", 300, 4), 8, 64, "f32", distance=True)
+    args = graph_args(c["src"].numpy(), c["dst"].numpy(), c["q"].size(0), c["k"].size(0))
+    want = run(c, args)
+    dev = on_device(c)
+    leaves = [dev[n] for n in LEAVES if n in dev]
+    names = ["d" + n for n in LEAVES if n in dev]
+    wide = torch.stack((dev["buckets"], dev["buckets"]), 1)
+    views = dict(dev, bias_table=dev["bias_table"].t().contiguous().t(), buckets=wide[:, 1])
+    assert not views["bias_table"].is_contiguous() and not views["buckets"].is_contiguous()
+    o = call(c, views, args)
+    grads = torch.autograd.grad(o, leaves, dev["do"], retain_graph=True)
+    assert torch.equal(o, want["o"]) and all(torch.equal(g, want[n]) for n, g in zip(names, grads))
+    assert all(torch.equal(g, want[n]) for n, g in zip(names, torch.autograd.grad(o, leaves, dev["do"])))
+    with torch.autograd.graph.save_on_cpu():
+        o = call(c, dev, args)
+    grads = torch.autograd.grad(o, leaves, dev["do"].transpose(0, 1).contiguous().transpose(0, 1))
+    assert all(torch.equal(g, want[n]) for n, g in zip(names, grads))
+    with torch.autograd.graph.saved_tensors_hooks(lambda x: x, lambda x: x.double() if x.is_floating_point() else x):
+        o = call(c, dev, args)
+    with pytest.raises(RuntimeError, match="saved tensors"):
+        torch.autograd.grad(o, leaves, dev["do"])
+
+
+def test_two_calls_of_one_graph_before_their_backwards():
+    c, other = make(("bpt", 300, 4), 8, 64, "bf16"), make(("bpt", 300, 4), 8, 64, "bf16", seed=5)
+    args = graph_args(c["src"].numpy(), c["dst"].numpy(), c["q"].size(0), c["k"].size(0))
+    want = run(c, args), run(other, args)
+    devs = on_device(c), on_device(other)
+    outs = [call(x, d, args) for x, d in zip((c, other), devs)]
+    for o, d, w in zip(outs, devs, want):
+        names = [n for n in LEAVES if n in d]
+        assert torch.equal(o, w["o"]) and all(torch.equal(g, w["d" + n]) for n, g in zip(names, torch.autograd.grad(o, [d[n] for n in names], d["do"])))

@@ -130,6 +130,34 @@ def test_what_is_not_finite_stays_in_its_row(rows):
     assert (z == 0).any() and not z.isnan().any()
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("size", [(8190, 1100, 1540), (8190, 1540, 1100), (33001, 1500, 1500), (4099, 300, 302), (5000, 2050, 130)], ids=str)
+def test_large_tiles_and_ragged_reductions(size, dtype):
+    t = inputs(*size, dtype, True, False, seed=9)
+    got, want = run(t, "relu", 0.1, 77), expected(t, "relu", 0.1, 77)
+    for name, w in want.items():
+        check(got[name], w, f"{size} {name}")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("size", [(300, 300, 302), (130, 44, 68), (700, 1030, 258)], ids=str)
+def test_what_stands_behind_a_row_does_not_reach_it(size, dtype):
+    """Rows of NaN next to those that count, and behind the tensors' ends."""
+    rows, inner, outer = size
+    t = inputs(*size, dtype, False, False, seed=3)
+    odd = {n: torch.full((v.size(0) + 100, v.size(1)), float("nan"), dtype=dtype, device=DEV) for n, v in t.items() if n in ("x", "w", "dy")}
+    for n, whole in odd.items():
+        whole[:t[n].size(0)] = t[n]
+    there = dict(t, **{n: whole[:t[n].size(0)] for n, whole in odd.items()})
+    a, b = run(t, None, 0.0, 0), run(there, None, 0.0, 0)
+    assert all(torch.equal(a[n], b[n]) for n in a)
+    t["x"][5], t["w"][7] = float("nan"), float("nan")
+    y = op.linear_act(t["x"], t["w"])
+    assert y[5].isnan().all() and y[:, 7].isnan().all()
+    y[5], y[:, 7] = 0, 0
+    assert y.isfinite().all()
+
+
 def test_leading_axes_nothing_and_one_gradient():
     t = inputs(24, 40, 12, torch.float32, True, True)
     flat = run(t, "gelu", 0.1, 3)

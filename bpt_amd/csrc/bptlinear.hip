@@ -157,8 +157,8 @@ template <typename T> struct Epilogue {
 //   dx       A = weight, (r, p) in memory,    B = g by rows
 //   dweight  A = x, (r, p) in memory,         B = g, (r, q) in memory
 // A workgroup owns a tile of BP x BQ; the reduction goes through LDS RB bytes a row at a time, two buffers: while one is multiplied, the other's
-// 16-byte loads are on their way straight into LDS.  Bound by matrix instructions where the reduction is long (bfloat16 65535 x 4096 -> 1024: 450 to 650 us
-// a product, 850 to 1200 TFLOP/s), by the epilogue's memory and vector instructions where it is short.  Fragments are 16 rows x 16 bytes a lane: one
+// 16-byte loads are on their way straight into LDS.  Bound by matrix instructions where the reduction is long (bfloat16 65535 x 4096 -> 1024: 457 to 600 us
+// a product, 915 to 1200 TFLOP/s), by the epilogue's memory and vector instructions where it is short.  Fragments are 16 rows x 16 bytes a lane: one
 // 16x16x32 product in bfloat16, four 16x16x4 in float32, whose reduction indices (4 g + j for lane group g and product j) only have to agree
 // between the operands.  A is the matrix instructions' first operand, so a lane ends with four neighbouring columns of a row.
 // An operand by rows lies in LDS as rows of RB / 16 chunks, shifted by row (rows_shift): the sixteen rows that a fragment reads at one chunk
@@ -851,10 +851,13 @@ inline bool on(std::initializer_list<const void *> ps, uintptr_t bytes) {
 }
 
 // Which tiles, and into how many shares the reduction goes.  256 x 256: one workgroup a compute unit, LDS and caches are asked for least, but nothing runs beside its
-// start and end: where a round of the chip is filled (or, by shares, a long reduction fills it) and those are a small part.  128 x 128: two a unit.  64 x 64: where these would
-// leave units idle.  us, by 256 | 128 | 64, bfloat16 (forward of rows x inner -> outer): 65535 x 4096 -> 1024 456 | 597 | 908, 8192 x 4096 -> 4096 221 | 284 | 570, 16383 x 512 -> 2048 53 | 54 | 63,
-// 16383 x 2048 -> 512 73 | 39 | 50, 2000 x 512 -> 2048 24 | 12.6 | 10.6, 1023 x 512 -> 512 24 | 11 | 8.9; dweight (shares) of 65535 x 4096 -> 1024 460 | 571 | 1239, of 16383 x 512 -> 2048
-// 76 | 48 | 68; float32 4096 x 4096 -> 4096 600 | 688 | 911, 16383 x 512 -> 2048 195 | 200 | 242, 1023 x 512 -> 512 78 | 22 | 15.
+// start and end: where a round of the chip is filled (or, by shares, a long reduction fills it) and those are a small part.  128 x 128: two a unit, where they fill the chip, by
+// shares too if the reduction is longer than what their sums cost on the way through memory.  64 x 64: where the larger ones would leave units idle.
+// us, by 256 | 128 | 64, bfloat16 (forward of rows x inner -> outer): 65535 x 4096 -> 1024 457 | 582 | 931, 8192 x 4096 -> 4096 223 | 285 | 565, 16383 x 512 -> 2048 45 | 50 | 66,
+// 16383 x 2048 -> 512 55 | 37 | 51, 2000 x 512 -> 2048 20 | 10 | 11, 1023 x 512 -> 512 19 | 9.2 | 8.8; dweight (shares) of 65535 x 4096 -> 1024 475 | 577 | 1226, of 16383 x 512 -> 2048
+// 52 | 45 | 71; float32 4096 x 4096 -> 4096 601 | 709 | 917, 16383 x 512 -> 2048 177 | 181 | 249, 1023 x 512 -> 512 72 | 22 | 15.
+// Two or three shares on 128 x 128 | one on 64 x 64, bfloat16: 4096 x 1024 -> 1024 27 | 17, 2500 x 2048 -> 1024 26 | 22, 2500 x 4096 -> 1024 35 | 41; float32: 3000 x 512 -> 1024 39 | 29,
+// 4096 x 1024 -> 1024 70 | 72, 2048 x 1024 -> 2048 57 | 63.  320 tiles of 128 x 128 | 64 x 64: dx of 2500 x 2048 -> 1024 20 | 24, float32 88 | 80.
 typedef Shape<256, 256, 4, 2, 1> Huge;
 typedef Shape<128, 128, 2, 2, 2> Large;
 typedef Shape<64, 64, 2, 2, 4> Small;
@@ -868,6 +871,9 @@ template <typename T> inline Choice choose(int64_t P, int64_t Q, int64_t R) {
     const int64_t steps = ceil_div(R, 128 / (int64_t)sizeof(T)), huge = count(256), large = count(128), small = count(64);
     if (R >= 1024 && huge >= 192 && 4 * huge >= 3 * 256 * ceil_div(huge, 256)) return Choice{HUGE, 1};
     if (steps >= 512 && huge >= 32 && huge < 192) return Choice{HUGE, (int)(256 / huge)};
+    constexpr bool LOW = sizeof(T) == 2;
+    if (large >= (LOW ? 272 : 384)) return Choice{LARGE, 1};
+    if (small >= 512 && R <= (LOW ? 2048 : 512)) return Choice{SMALL, 1};
     const int64_t large_splits = std::max<int64_t>(1, std::min<int64_t>(steps / 8, 512 / large)), small_splits = std::max<int64_t>(1, std::min<int64_t>(steps / 4, 512 / small));
     if (large * large_splits >= 384) return Choice{LARGE, (int)large_splits};
     return Choice{SMALL, (int)small_splits};
@@ -900,7 +906,7 @@ int run_product(const T *a, const T *b, int64_t P, int64_t Q, int64_t R, int64_t
     const Choice ch = choose<T>(P, Q, R);
     const Product m = product<T>(P, Q, R, lda, ldb, ch);
     float *const part = m.splits > 1 ? (float *)ws : nullptr;
-    // Straight to LDS: rows that start on 4 bytes, as loads of several words do (33598 x 300 -> 600 bfloat16, through registers / straight: forward 55 / 53 us, dx 64 / 40, dweight 79 / 31), and hold
+    // Straight to LDS: rows that start on 4 bytes, as loads of several words do (33598 x 300 -> 600 bfloat16, through registers / straight: dx 64 / 30 us, dweight 79 / 29), and hold
     // a vector at least; a lane's offsets into a step count 32 bits (256 rows of 2^21 elements).
     const bool direct = on({a, b}, 4) && lda * sizeof(T) % 4 == 0 && ldb * sizeof(T) % 4 == 0 && std::min(lda, ldb) >= ve<T>() && std::max(lda, ldb) <= (int64_t)1 << 21;
     const dim3 grid((unsigned)(m.tiles * (int64_t)m.splits));
@@ -918,13 +924,14 @@ template <typename T> inline Epilogue<T> plain_epilogue(T *y, int64_t cols, doub
     return Epilogue<T>{nullptr, nullptr, y, nullptr, cols, (float)scale, BPT_ACT_NONE, make_drop(0.0, 0), cols % 4 == 0 && on({y}, 4 * sizeof(T))};
 }
 
-constexpr int64_t FEW_ROWS = 64;
+// (a launch counts its threads in 32 bits: of more columns the tiles have fewer)
+inline bool few_rows(int64_t rows, int64_t outer) { return rows <= 64 && outer <= (int64_t)1 << 26; }
 template <typename T>
 int run_forward(const void *x_, const void *w_, const void *b_, const void *r_, void *y_, void *kept_, void *ws, int64_t rows, int64_t inner, int64_t outer, int act,
                 Drop drop, hipStream_t s) {
     const T *x = (const T *)x_, *w = (const T *)w_;
     const Epilogue<T> out{(const T *)b_, (const T *)r_, (T *)y_, (T *)kept_, outer, 1.f, act, drop, outer % 4 == 0 && on({b_, r_, y_, kept_}, 4 * sizeof(T))};
-    if (rows <= FEW_ROWS) {
+    if (few_rows(rows, outer)) {
         const bool whole = inner % ve<T>() == 0 && on({x, w}, 16);
         const dim3 grid((unsigned)ceil_div(outer, 16)), block(FEW_WAVES * WAVE);
 #define LAUNCH(NQ) \
@@ -985,7 +992,7 @@ extern "C" {
 
 int64_t bpt_linear_forward_workspace_bytes(int64_t rows, int64_t inner, int64_t outer, int dtype) {
     if (!is_type(dtype) || !is_size(rows, inner, outer)) return -1;
-    if (rows <= FEW_ROWS || outer == 0) return 0;
+    if (few_rows(rows, outer) || outer == 0) return 0;
     return FOR_TYPE(product_workspace)(outer, rows, inner);
 }
 

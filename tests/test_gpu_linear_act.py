@@ -232,6 +232,12 @@ def test_long_rows_of_many_bytes():
     del y
 
 
+def test_more_columns_than_a_launch_of_few_rows_has_threads_for():
+    outer = 2 ** 27 + 5
+    x, w = torch.full((1, 1), 3.0, device=DEV), torch.arange(outer, dtype=torch.float32, device=DEV).view(-1, 1)
+    assert torch.equal(op.linear_act(x, w).view(-1), 3.0 * w.view(-1))
+
+
 def test_seeds_come_from_torch():
     t = inputs(20, 32, 64, torch.float32, False, False)
     torch.manual_seed(5)

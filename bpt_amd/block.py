@@ -18,7 +18,7 @@ Options the reference does not have, off by default (then nothing of them is a p
               (heads,) is a parameter that starts at 2^(-8 i / heads), i = 1 .. heads
   keep8       the feed-forward keeps its activations in 8 bits for the backward (`op.relu_linear8`): one byte each in place of relu's
               result, dropout's and its mask
-  epilogue    the output projection and the feed-forward run as products with bias, relu, dropout and the residual sum in their epilogue
+  epilogue    projections and the feed-forward run as products with bias, relu, dropout and the residual sum in their epilogue
               (`op.linear_act`; with keep8 the feed-forward as keep8 has it, then `op.dropout` with the residual): no mask is stored, dropout's
               decisions come from a counter-based generator seeded from torch's CPU generator.  In bfloat16 the residual sum is rounded before it is
               normalised
@@ -44,8 +44,9 @@ def _as_it_is(module, kind):
 
 
 def _add_norm(norm, x, residual, fused):
-    """norm(x + residual) (attention.py:79, :81; residual None: norm(x)), by add_layer_norm where that computes the same and is the faster way: a LayerNorm over the last axis as it is,
-    GPU tensors of one type, nothing that casts, traces or transforms, rows that a workgroup's registers hold (16 KiB).  Longer rows are walked three times:
+    """norm(x + residual) (attention.py:79, :81; residual None: norm(x)), by add_layer_norm where that computes the same and is the faster way: a LayerNorm
+    over the last axis as it is, GPU tensors of one type, nothing that casts, traces or transforms, rows that a workgroup's registers hold (16 KiB).
+    Longer rows are walked three times:
     forward | training, us, add_layer_norm / torch, 16383 rows of 4096 columns float32 145 / 263 | 352 / 736, of 4104 301 / 275 | 767 / 782; of 8192 columns
     bfloat16 152 / 305 | 378 / 898, of 8200 757 / 317 | 1952 / 955; in float64, where torch's is slower, of 2048 columns 146 / 381 | 370 / 843, of 4104 515 / 730 | 1345 / 1556."""
     if (fused and _as_it_is(norm, nn.LayerNorm) and len(norm.normalized_shape) == 1 and x.is_cuda and x.is_contiguous()
@@ -58,16 +59,23 @@ def _add_norm(norm, x, residual, fused):
 
 
 def _epilogue_takes(x, residual, drop, *linears):
-    """Whether the products with an epilogue may stand for calls of the linears on x, of drop and of the residual sum: torch's modules as they are, GPU tensors of one
+    """Whether the products with an epilogue may stand for calls of the linears on x, of drop (or None) and of the residual sum: torch's modules as they are, GPU tensors of one
     type, nothing that casts, traces or transforms."""
     tensors = [x, residual] + [t for lin in linears for t in (lin.weight, lin.bias)]
     return (x.is_cuda and x.dtype in (torch.float32, torch.bfloat16) and x.dim() > 0 and x.size(-1) > 0 and not torch.is_autocast_enabled()
-            and all(_as_it_is(lin, nn.Linear) for lin in linears) and _as_it_is(drop, nn.Dropout) and 0.0 <= drop.p < 1.0
+            and all(_as_it_is(lin, nn.Linear) for lin in linears) and (drop is None or (_as_it_is(drop, nn.Dropout) and 0.0 <= drop.p < 1.0))
             and all(t is None or (t.dtype == x.dtype and t.device == x.device and t.is_contiguous()) for t in tensors) and plain_call(*tensors))
 
 
 def _share(drop):
     return drop.p if drop.training else 0.0
+
+
+def _project(block, lin, x):
+    """lin(x) (attention.py:62-64)."""
+    if block.epilogue and _epilogue_takes(x, None, None, lin):
+        return linear_act(x, lin.weight, lin.bias)
+    return lin(x)
 
 
 def _project_add_norm(block, norm, lin, drop, x, residual):
@@ -200,9 +208,7 @@ class BPTBlock(nn.Module):
     def forward(self, h, csr, etype=None, pos=None):
         # three GEMMs: one strided-batched GEMM over the stacked weights (its (3, n, h * d_k) result holds q, k, v as the
         # contiguous tensors the kernels need) measured slower, 3.38 against 3.17 ms per layer fwd+bwd at n = 16 383 in float32
-        q = self.proj_q(h).view(-1, self.h, self.d_k)
-        k = self.proj_k(h).view(-1, self.h, self.d_k)
-        v = self.proj_v(h).view(-1, self.h, self.d_k)
+        q, k, v = (_project(self, proj, h).view(-1, self.h, self.d_k) for proj in (self.proj_q, self.proj_k, self.proj_v))
         a = self.attention(q, k, v, csr, etype, pos) if pos is not None else self.attention(q, k, v, csr, etype)
         h = _project_add_norm(self, self.norm_in, self.proj_o, self.drop_h, a, h)
         return _feed_forward_add_norm(self, self.norm_inter, h)
@@ -285,7 +291,7 @@ class BPTMemBlock(nn.Module):
                         n_rows=None if q.size(0) == v.size(0) else q.size(0)).view(-1, self.d_k * self.h)
 
     def forward(self, h, csr, mem, csr_inter, etype=None, pos=None):
-        heads = lambda proj, x: proj(x).view(-1, self.h, self.d_k)
+        heads = lambda proj, x: _project(self, proj, x).view(-1, self.h, self.d_k)
         # Part I: self-attention (attention.py:118-142)
         a = self._attend(0, heads(self.proj_q[0], h), heads(self.proj_k[0], h), heads(self.proj_v[0], h), csr, etype, pos)
         h = _project_add_norm(self, self.norm_in[0], self.proj_o[0], self.drop_h[0], a, h)

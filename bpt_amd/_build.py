@@ -4,7 +4,7 @@
   bpt_amd/csrc/libbptattn.so   gfx950 HIP (hipcc)        <- bptattn.hip, bpttiles.h
   bpt_amd/csrc/libbptscore.so  gfx950 HIP (hipcc)        <- bptscore.hip, bptmod.h, bpttiles.h  (attention with capped scores and distance)
   bpt_amd/csrc/libbptblock.so  gfx950 HIP (hipcc)        <- bptblock.hip, bpttiles.h  (layer norm of a sum, relu kept in 8 bits)
-  bpt_amd/csrc/libbptlinear.so gfx950 HIP (hipcc)       <- bptlinear.hip, bpttiles.h  (matrix products with an epilogue, dropout)
+  bpt_amd/csrc/libbptlinear.so gfx950 HIP (hipcc)        <- bptlinear.hip, bpttiles.h  (matrix products with an epilogue, dropout)
   bpt_amd/csrc/libbptbias.so   gfx950 HIP (hipcc)        <- bptbias.hip, bptmod.h, bpttiles.h  (bias of scores by buckets)
   bpt_amd/csrc/libbptplan.so   gfx950 HIP (hipcc)        <- bptplan.hip  (plans built on the GPU; rocPRIM headers)
   bpt_amd/csrc/bptop.so        host C++ (g++, torch)     <- bptop.cpp, bptblockop.cpp, bptlinearop.cpp, bpthost.h  (host side of the ops and their autograd; links them)
@@ -94,10 +94,12 @@ def build_op(verbose=True):
     rocm = os.path.dirname(os.path.dirname(HIPCC))
     include = cpp_extension.include_paths() + [os.path.join(rocm, "include"), sysconfig.get_paths()["include"]]
     libs = os.path.join(os.path.dirname(torch.__file__), "lib")
+    sources = [os.path.join(CSRC, n) for n in ("bptop.cpp", "bptblockop.cpp", "bptlinearop.cpp")]
+    ours = ["-l:" + os.path.basename(so) for so in (ATTN_SO, PLAN_SO, SCORE_SO, BLOCK_SO, LINEAR_SO, BIAS_SO)]
     _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-DTORCH_EXTENSION_NAME=bptop",
           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM"]
-         + [f"-I{p}" for p in include] + [os.path.join(CSRC, "bptop.cpp"), os.path.join(CSRC, "bptblockop.cpp"), os.path.join(CSRC, "bptlinearop.cpp"), "-o", OP_SO, f"-L{libs}", f"-L{CSRC}",
-                                          "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python", "-ltorch", "-l:libbptattn.so", "-l:libbptplan.so", "-l:libbptscore.so", "-l:libbptblock.so", "-l:libbptlinear.so", "-l:libbptbias.so", "-Wl,-rpath,$ORIGIN"], verbose)
+         + [f"-I{p}" for p in include] + sources + ["-o", OP_SO, f"-L{libs}", f"-L{CSRC}", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python", "-ltorch"] + ours
+         + ["-Wl,-rpath,$ORIGIN"], verbose)
     return OP_SO
 
 

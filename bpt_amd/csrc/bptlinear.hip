@@ -504,7 +504,7 @@ __global__ __launch_bounds__(S::THREADS, S::PER_SIMD) void k_linear_tiles(const 
         }
     };
     if constexpr (!THIRDS) {
-        through_registers(s, false);
+        if constexpr (!DIRECT) through_registers(s, false);
     } else {
         // Thirds of an infinity are infinity and NaN: a tile whose sums are not finite is formed again by the float32 instructions.
         through_registers(s, true);

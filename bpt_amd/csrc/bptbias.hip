@@ -129,6 +129,9 @@ struct Prepared {
         : table((float *)at), codes_in((uint8_t *)at + table_bytes(h)), codes_pairs(codes_in + round16(places(in))), codes_out(codes_pairs + round16(in->n_edges)) {}
 };
 
+// What a table's value of -HIDES and below stands for is -infinity.  A score of that size and a row's lse are off by 3 percent of a factor, of one of 10^9 by any: rows of nothing
+// but such masks would have probabilities that do not add up, and one of the type's lowest values divided by the scale is no number any more.
+constexpr float HIDES = BPT_HIDES;
 // Bound by memory: the edge ids of either side's places, and a bucket of 8 bytes for each that exists, from the caches (L = 8192 6 us; L = 32768, k = 8 36 us).
 // blockIdx.y: 0 the tables, 1 and 2 the places of either side, four a thread; by_pair: the side whose pairs' codes are wanted too, or 0
 template <typename T>
@@ -140,7 +143,8 @@ __global__ __launch_bounds__(BLOCK) void k_bucket_prepare(const T *__restrict__ 
     if (blockIdx.y == 0) {
         for (int64_t i = first; i < first + 4 && i < (int64_t)h * 256; ++i) {
             const int head = (int)(i >> 8), b = (int)i & 255;
-            tables[i] = head < heads && b < n_buckets ? Elem<T>::ld(table + (int64_t)b * heads + head) * factor : 0.f;
+            const float x = head < heads && b < n_buckets ? Elem<T>::ld(table + (int64_t)b * heads + head) : 0.f;
+            tables[i] = (x <= -HIDES ? -INFINITY : x) * factor;
         }
         return;
     }

@@ -1486,6 +1486,9 @@ def _check_buckets(buckets, device):
         raise ValueError("all tensors of a call must be on one device")
 
 
+BUCKET_HIDES = 2.0 ** 19         # values of minus that and below in a bias table hide a bucket's edges (BPT_HIDES in include/bptbias.h)
+
+
 def bucket_bias_forward(table, buckets, factor=1.0, term=False):
     """bias[e, head] = factor * table[buckets[e], head] of table (n, h), float32, float64 or bfloat16, and buckets (E,) int64: (E, h) of table's type, or with
     term the float32 (E + 1, h) that score_attention_forward takes as bias.  A bucket outside of table adds 0."""

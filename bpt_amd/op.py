@@ -232,7 +232,7 @@ class BPTBucketAttention(Function):
 
     @staticmethod
     def forward(ctx, row, indptr_r, eid_r, indices_r, col, indptr_c, eid_c, indices_c, q, k, v, scale, dropout_p, seed, table, buckets, score, slopes):
-        bias = _g.bucket_bias_forward(table, buckets, 1.0 / scale, term=True)
+        bias = _g.bucket_bias_forward(table.masked_fill(table <= -_g.BUCKET_HIDES, -math.inf), buckets, 1.0 / scale, term=True)
         o, lse = _g.score_attention_forward(col, indptr_c, eid_c, indices_c, q, k, v, score, scale, dropout_p, seed, bias)
         ctx.save_for_backward(row, indptr_r, eid_r, indices_r, col, indptr_c, eid_c, indices_c, q, k, v, o, lse, bias, table, buckets, *score[1:])
         ctx.cap, ctx.scale, ctx.dropout_p, ctx.seed = score.cap, scale, dropout_p, seed
@@ -473,7 +473,7 @@ def _score_chain(graph, q, k, v, scale, dropout_p, rel_table, etype, score, bias
         bias = bucket_bias(bias_table, buckets).to(e.dtype).view(e.shape)
         e = e + bias
         if not score.cap:                     # (sparse_softmax takes no -infinity: a row of nothing else would be NaN)
-            hidden = bias.detach() == -math.inf
+            hidden = bias.detach() <= -_g.BUCKET_HIDES
             e = e.masked_fill(hidden, -1.0e8)
     if score.cap:
         e = _Capped.apply(e, score.cap)
@@ -621,7 +621,7 @@ def bpt_attention(row, indptr_r, eid_r, indices_r, col, indptr_c, eid_c, indices
 
     bias_table (n, h) of q's type and buckets (E,) int64 (not in the reference) add the scalar bias_table[buckets[e], head] to the scaled score of edge e: a
     learned bias by distance, edge type or whatever else the caller numbers edges by.  bias_table gets a gradient, summed in a fixed order; an edge
-    whose bucket lies outside of it has no bias, and -infinity hides an edge (a row with nothing left is 0; not with score_cap, which bounds
+    whose bucket lies outside of it has no bias, and -infinity, or any value of -2^19 and below, hides an edge (a row with nothing left is 0; not with score_cap, which bounds
     it).  Not together with rel_table.
 
     Score options (not in the reference): with u the scaled score, term included,

@@ -27,8 +27,9 @@ int bpt_bucket_bias_backward(const void *ds, const int64_t *buckets, void *dtabl
 
 /* The fused pass of bptscore.h with u = scale (q[dst].k[src]) + table[bucket][head], capped and lowered by distance or not (score as there; all of it 0: neither).
  * Heads of 64 columns, h = 8 or 16 of them, float32 also 4; up to 255 buckets.  Plans as there, with grp_eids on either side.  scale is not 0.  In bfloat16 delta comes from
- * the pairs.  A row whose edges are all hidden (-infinity in table, without a cap) is 0. */
+ * the pairs.  Values of -BPT_HIDES and below in table, -infinity among them, hide a bucket's edges (with a cap: their scores are -cap); a row with nothing left is 0. */
 #define BPT_MOST_BUCKETS 255
+#define BPT_HIDES 524288.0f
 
 /* What the passes of a call take: the heads' tables and the bucket of every place of the plans, written to `prepared` (on 16 bytes).  plan_out may be NULL where no
  * backward follows.  table (n_buckets, heads) of dtype, heads <= h (those behind have no bias), buckets (n_edges). */

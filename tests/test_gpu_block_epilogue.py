@@ -152,6 +152,22 @@ def test_modules_that_are_not_as_they_were_are_called():
     assert torch.equal(plain.double()(h.double(), csr), other.double()(h.double(), csr))
 
 
+def test_projections_with_hooks_are_called():
+    from bpt_amd.block import BPTBlock, BPTMemBlock
+    c = case(60)
+    csr, h = to_dev(c["csr"]), c["h"].to(DEV)
+    for kind, args in ((BPTBlock, (h, csr)), (BPTMemBlock, (h, csr, h, csr))):
+        for name in ("proj_q", "proj_k", "proj_v"):
+            torch.manual_seed(3)
+            plain = kind(512, 8, 256, drop_h=0.0, drop_a=0.0).to(DEV)
+            other = copy.deepcopy(plain)
+            other.epilogue = True
+            for b in (plain, other):
+                proj = getattr(b, name)
+                (proj if kind is BPTBlock else proj[0]).register_forward_hook(lambda m, i, o: 2 * o)
+            assert (plain(*args) - other(*args)).abs().max() < 1e-4
+
+
 def test_a_block_made_without_the_options_and_their_parameters():
     from bpt_amd.block import BPTBlock, BPTMemBlock
     for kind in (BPTBlock, BPTMemBlock):

@@ -430,3 +430,30 @@ def test_two_calls_of_one_graph_before_their_backwards():
     for o, d, w in zip(outs, devs, want):
         names = [n for n in LEAVES if n in d]
         assert torch.equal(o, w["o"]) and all(torch.equal(g, w["d" + n]) for n, g in zip(names, torch.autograd.grad(o, [d[n] for n in names], d["do"])))
+
+
+@pytest.mark.parametrize("how", ["fused", "long", "chain"])
+@pytest.mark.parametrize("dtype,mask", [("f32", -2.0 ** 19), ("f32", -1e9), ("f32", torch.finfo(torch.float32).min), ("bf16", -1e6), ("bf16", torch.finfo(torch.bfloat16).min)])
+def test_masks_of_large_numbers_hide(dtype, mask, how):
+    """As -infinity: the same bits.  (long: a table of more buckets than the fastest path takes.)"""
+    c = make(("random", 90, 400), 8, 64, dtype, n=300 if how == "long" else 4)
+    c["buckets"][c["dst"] < 20] = 1
+    c["bias_table"][1] = -math.inf
+    args = graph_args(c["src"].numpy(), c["dst"].numpy(), c["q"].size(0), c["k"].size(0))
+    want = run(c, args, fused=how != "chain")
+    c["bias_table"][1] = mask
+    got = run(c, args, fused=how != "chain")
+    assert not got["o"][:20].any() and all(torch.equal(got[n], want[n]) and got[n].isfinite().all() for n in got)
+
+
+@pytest.mark.parametrize("n", [4, 300])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_a_cap_bounds_masks(dtype, n):
+    c = make(("random", 90, 400), 8, 64, dtype, n=n, cap=15.0)
+    args = graph_args(c["src"].numpy(), c["dst"].numpy(), c["q"].size(0), c["k"].size(0))
+    c["bias_table"][1] = -3000.0                                  # (200 caps: the tangent is -1)
+    want = run(c, args, fused=True)
+    for mask in (-1e9, -math.inf, torch.finfo(c["q"].dtype).min):
+        c["bias_table"][1] = mask
+        got = run(c, args, fused=True)
+        assert all(torch.equal(got[m], want[m]) for m in got), mask

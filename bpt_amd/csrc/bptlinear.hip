@@ -926,14 +926,19 @@ template <typename T> inline Epilogue<T> plain_epilogue(T *y, int64_t cols, doub
     return Epilogue<T>{nullptr, nullptr, y, nullptr, cols, (float)scale, BPT_ACT_NONE, make_drop(0.0, 0), cols % 4 == 0 && on({y}, 4 * sizeof(T))};
 }
 
-// (a launch counts its threads in 32 bits: of more columns the tiles have fewer)
-inline bool few_rows(int64_t rows, int64_t outer) { return rows <= 64 && outer <= (int64_t)1 << 26; }
+// Whether the kernel of few rows takes a forward: every workgroup of it reads all of x, 128 KB at most where it has more than a fragment's rows.  us, few rows | tiles, bfloat16:
+// 16 x 512 -> 512 4.9 | 7.2, 16 x 4096 -> 4096 9.8 | 10.4, 64 x 512 -> 512 4.8 | 6.8, 64 x 1024 -> 4096 7.2 | 8.8, 32 x 2048 -> 512 7.6 | 6.8, 64 x 2048 -> 512 11.5 | 8.3, 64 x 4096 -> 4096
+// 21 | 12.5; float32 16 x 4096 -> 4096 20 | 32, 64 x 512 -> 512 7.3 | 8.5, 32 x 1024 -> 4096 9.1 | 12.3, 64 x 1024 -> 1024 12.7 | 9.6, 32 x 2048 -> 512 14 | 9.7, 64 x 4096 -> 4096 44 | 36.
+// (A launch counts its threads in 32 bits: of more columns the tiles have fewer.)
+inline bool few_rows(int64_t rows, int64_t inner, int64_t outer, int64_t size) {
+    return (rows <= 16 || (rows <= 64 && rows * inner * size <= (int64_t)1 << 17)) && outer <= (int64_t)1 << 26;
+}
 template <typename T>
 int run_forward(const void *x_, const void *w_, const void *b_, const void *r_, void *y_, void *kept_, void *ws, int64_t rows, int64_t inner, int64_t outer, int act,
                 Drop drop, hipStream_t s) {
     const T *x = (const T *)x_, *w = (const T *)w_;
     const Epilogue<T> out{(const T *)b_, (const T *)r_, (T *)y_, (T *)kept_, outer, 1.f, act, drop, outer % 4 == 0 && on({b_, r_, y_, kept_}, 4 * sizeof(T))};
-    if (few_rows(rows, outer)) {
+    if (few_rows(rows, inner, outer, sizeof(T))) {
         const bool whole = inner % ve<T>() == 0 && on({x, w}, 16);
         const dim3 grid((unsigned)ceil_div(outer, 16)), block(FEW_WAVES * WAVE);
 #define LAUNCH(NQ) \
@@ -994,7 +999,7 @@ extern "C" {
 
 int64_t bpt_linear_forward_workspace_bytes(int64_t rows, int64_t inner, int64_t outer, int dtype) {
     if (!is_type(dtype) || !is_size(rows, inner, outer)) return -1;
-    if (few_rows(rows, outer) || outer == 0) return 0;
+    if (few_rows(rows, inner, outer, dtype == BPT_F32 ? 4 : 2) || outer == 0) return 0;
     return FOR_TYPE(product_workspace)(outer, rows, inner);
 }
 

@@ -89,7 +89,7 @@ def run(t, act, p, seed):
 
 
 SIZES = [(1, 1, 1), (1, 512, 2048), (3, 7, 5), (16, 64, 64), (17, 33, 66), (48, 512, 512), (64, 65, 16), (65, 128, 64), (130, 300, 129), (257, 301, 255), (300, 8, 1000),
-         (640, 1040, 136), (2000, 256, 512), (4099, 64, 520), (66, 4096, 72)]
+         (640, 1040, 136), (2000, 256, 512), (4099, 64, 520), (66, 4096, 72), (32, 1024, 200), (33, 2049, 130), (64, 2050, 66), (17, 5000, 40)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])

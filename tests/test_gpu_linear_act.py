@@ -139,6 +139,22 @@ def test_large_tiles_and_ragged_reductions(size, dtype):
         check(got[name], w, f"{size} {name}")
 
 
+@pytest.mark.parametrize("size", [(40, 256, 72), (300, 256, 200), (1300, 1100, 1540)], ids=str)
+@pytest.mark.parametrize("x_by,w_by", [(2.0 ** -120, 2.0 ** 10), (2.0 ** -115, 2.0 ** 15), (2.0 ** -100, 1.0), (2.0 ** 100, 2.0 ** -20), (2.0 ** 124, 2.0 ** -60)])
+def test_low_and_high_numbers(size, x_by, w_by):
+    """Products of numbers near either end of float32's range are as exact as others, where no sum of their terms can leave it, in whatever order they are added: where the terms'
+    absolute values together lie within it.  (Hundreds of terms of dw with x of 2^124 do not: 0.1 2^124 300 is 2^129.)"""
+    t = inputs(*size, torch.float32, False, False, seed=2)
+    t["x"], t["w"] = t["x"].clamp(-2, 2) * x_by, t["w"] * w_by
+    got, want = run(t, None, 0.0, 0), expected(t, None, 0.0, 0)
+    x, w, dy = (t[n].double().abs() for n in ("x", "w", "dy"))
+    for name, terms in (("y", x @ w.T), ("dw", dy.T @ x)):
+        if terms.max() <= torch.finfo(torch.float32).max:
+            check(got[name], want[name], f"{size} {x_by} {name}")
+        else:
+            assert name == "dw" and x_by == 2.0 ** 124
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
 @pytest.mark.parametrize("size", [(300, 300, 302), (130, 44, 68), (700, 1030, 258)], ids=str)
 def test_what_stands_behind_a_row_does_not_reach_it(size, dtype):

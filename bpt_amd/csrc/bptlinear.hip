@@ -864,6 +864,8 @@ inline bool on(std::initializer_list<const void *> ps, uintptr_t bytes) {
 // 52 | 45 | 71; float32 4096 x 4096 -> 4096 601 | 709 | 917, 16383 x 512 -> 2048 177 | 181 | 249, 1023 x 512 -> 512 72 | 22 | 15.
 // Two or three shares on 128 x 128 | one on 64 x 64, bfloat16: 4096 x 1024 -> 1024 27 | 17, 2500 x 2048 -> 1024 26 | 22, 2500 x 4096 -> 1024 35 | 41; float32: 3000 x 512 -> 1024 39 | 29,
 // 4096 x 1024 -> 1024 70 | 72, 2048 x 1024 -> 2048 57 | 63.  320 tiles of 128 x 128 | 64 x 64: dx of 2500 x 2048 -> 1024 20 | 24, float32 88 | 80.
+// Shares of 4 | 8 | 16 steps at least on 64 x 64, bfloat16: 65 x 512 -> 512 9.6 | 5.9 | 5.8, 256 x 1024 -> 1024 8.7 | 8.8 | 7.9, 1023 x 512 -> 512 8.9 | 5.8 | 5.8, 256 x 2048 -> 512 8.6 | 8.8 | 10.1;
+// float32: 65 x 512 -> 512 10.0 | 11.6 | 15.4, 127 x 768 -> 768 10.2 | 12.8 | 20, 256 x 1024 -> 1024 15.1 | 14.1 | 18, dweight of 256 x 512 -> 2048 15.8 | 10.8 | 10.7.
 typedef Shape<256, 256, 4, 2, 1> Huge;
 typedef Shape<128, 128, 2, 2, 2> Large;
 typedef Shape<64, 64, 2, 2, 4> Small;
@@ -880,7 +882,8 @@ template <typename T> inline Choice choose(int64_t P, int64_t Q, int64_t R) {
     constexpr bool LOW = sizeof(T) == 2;
     if (large >= (LOW ? 272 : 384)) return Choice{LARGE, 1};
     if (small >= 512 && R <= (LOW ? 2048 : 512)) return Choice{SMALL, 1};
-    const int64_t large_splits = std::max<int64_t>(1, std::min<int64_t>(steps / 8, 512 / large)), small_splits = std::max<int64_t>(1, std::min<int64_t>(steps / 4, 512 / small));
+    const int64_t large_splits = std::max<int64_t>(1, std::min<int64_t>(steps / 8, 512 / large)), share = small >= 64 ? 8 : 4;
+    const int64_t small_splits = LOW && steps <= 16 ? 1 : std::max<int64_t>(1, std::min<int64_t>(steps / share, 512 / small));
     if (large * large_splits >= 384) return Choice{LARGE, (int)large_splits};
     return Choice{SMALL, (int)small_splits};
 }

@@ -303,12 +303,14 @@ template <typename T> __device__ __forceinline__ floatx4 multiply(uintx4 a, uint
 }
 
 __device__ __forceinline__ void wait_for_lds() { __builtin_amdgcn_s_waitcnt(15 | 7 << 4 | 3 << 14); }
-// Eight float32 as three bfloat16 each, exactly: the upper 16 bits, those of what is left, and what is left then (8 + 8 + 8 digits).
+// Eight float32, times 2^23, as three bfloat16 each, exactly: the upper 16 bits, those of what is left, and what is left then (8 + 8 + 8 digits).  The bfloat16 units take numbers
+// below 2^-126 for 0: 2^23 makes the last digit of float32's lowest number, 2^-149, one of those that count.
+constexpr float THIRDS_BY = 0x1p23f, THIRDS_BACK = 0x1p-46f;       // (of an operand; of a product of two)
 __device__ __forceinline__ void thirds(uintx4 a, uintx4 b, uintx4 (&out)[3]) {
     uint32_t x[8], y[8], z[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-        x[e] = e < 4 ? a[e & 3] : b[e & 3];
+        x[e] = __float_as_uint(__uint_as_float(e < 4 ? a[e & 3] : b[e & 3]) * THIRDS_BY);
         y[e] = __float_as_uint(__uint_as_float(x[e]) - __uint_as_float(x[e] & 0xffff0000u));
         z[e] = __float_as_uint(__uint_as_float(y[e]) - __uint_as_float(y[e] & 0xffff0000u));
     }
@@ -506,26 +508,22 @@ __global__ __launch_bounds__(S::THREADS, S::PER_SIMD) void k_linear_tiles(const 
     if constexpr (!THIRDS) {
         if constexpr (!DIRECT) through_registers(s, false);
     } else {
-        // Thirds of an infinity are infinity and NaN, and those below 2^-126, which the lower ones of a number below 2^-110 are, count as 0: a tile with a sum that is not finite,
-        // or not 0 but as low as sums of such numbers are, is formed again by the float32 instructions.  (x of 1e-37, weights of 1e3: 9e-4 off without, 2e-7 with it.)
+        // Thirds of an infinity are infinity and NaN, and numbers of 2^105 and above, or sums of 2^82, leave float32's range times 2^23 or 2^46: a tile with a sum that is not finite is
+        // formed again by the float32 instructions.
         through_registers(s, true);
-        float odd = 0.f, least = 1.f;
+        float odd = 0.f;
 #pragma unroll
         for (int i = 0; i < FP; ++i)
 #pragma unroll
             for (int j = 0; j < FQ; ++j)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    odd = fmaf(acc[i][j][e], 0.f, odd);
-                    least = fminf(least, acc[i][j][e] == 0.f ? 1.f : fabsf(acc[i][j][e]));
-                }
-        if (__syncthreads_or(!(odd == 0.f) || least < 0x1p-90f)) {
+                for (int e = 0; e < 4; ++e) odd = fmaf(acc[i][j][e], 0.f, odd);
+        const bool again = __syncthreads_or(!(odd == 0.f));
 #pragma unroll
-            for (int i = 0; i < FP; ++i)
+        for (int i = 0; i < FP; ++i)
 #pragma unroll
-                for (int j = 0; j < FQ; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
-            through_registers(0, false);
-        }
+            for (int j = 0; j < FQ; ++j) acc[i][j] = again ? floatx4{0.f, 0.f, 0.f, 0.f} : acc[i][j] * THIRDS_BACK;
+        if (again) through_registers(0, false);
     }
     // the tile, or half of every wavefront's rows at a time, as rows of BP floats, quad i of row r at i ^ r: sixteen rows' quads of a fragment spread over the banks
     constexpr int QUADS = BP / 4, TURNS = ROWS * QUADS / S::THREADS, U = 4;

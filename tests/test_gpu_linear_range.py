@@ -72,3 +72,18 @@ def test_low_numbers_beside_what_is_not_finite(size):
     others = torch.arange(size[0], device=DEV) != 5
     compare("y", y[others], t["x"][others], t["w"].T)
     compare("dx", dx[others], t["dy"][others], t["w"])
+
+
+@pytest.mark.parametrize("size", [(65, 33), (300, 200), (4096, 4096)], ids=str)
+def test_a_product_of_two_numbers(size):
+    """x w of two numbers, by tiles: what the products of bfloat16 leave out is below 2^-21 (1 + 2^-9) = 8.02 u of it and makes it smaller; adding up its parts is off by
+    a step of 2 u at most where the last and largest is added, by 2^-6 of one at each of three before."""
+    rows, outer = size
+    gen = torch.Generator().manual_seed(outer)
+    any_number = lambda n: (torch.randint(0, 2 ** 23, (n,), generator=gen, dtype=torch.int32) + 0x3F800000).view(torch.float32)
+    x, w = torch.zeros(rows, 96, device=DEV), torch.zeros(outer, 96, device=DEV)
+    x[:, 40], w[:, 40] = any_number(rows).to(DEV), any_number(outer).to(DEV)
+    x[3, 40] = w[5, 40] = 1 + 2.0 ** -7 - 2.0 ** -23                # (the lower thirds of either as large as they get)
+    want = x[:, 40, None].double() * w[None, :, 40].double()
+    off = (op.linear_act(x, w).double() - want) / (U * want)
+    assert off.min() >= -(8.02 + 2 + 0.1) and off.max() <= 2 + 0.1

@@ -105,7 +105,7 @@ template <typename T> struct Epilogue {
     int act;
     Drop drop;
     bool quads;                  // rows, and with them quads, start on four elements everywhere
-    // four columns, of rows that start on four, of an activation and dropout that the caller has looked up; bias of the columns, residual as read ahead
+    // four columns, of rows that start on four, of an activation and dropout that the caller has looked up; bias of the columns, residual as read ahead; a is kept of an activation
     template <int ACT, bool DROP> __device__ __forceinline__ void quad(floatx4 v, int64_t at, floatx4 b, floatx4 ahead) const {
         v = v * scale + b;
         if constexpr (ACT != BPT_ACT_NONE) {
@@ -580,10 +580,11 @@ __global__ __launch_bounds__(S::THREADS, S::PER_SIMD) void k_linear_tiles(const 
             }
             continue;
         }
-        if (!out.quads) {
+        constexpr bool FORWARD = !ACOLS && !BCOLS;
+        if (!out.quads || (FORWARD && out.act == BPT_ACT_NONE && out.kept)) {
 #pragma unroll 1
             for (int u = 0; u < TURNS; ++u)
-                if (row(u) < left) out(sum(u), q0 + row(u), p, none);
+                if (row(u) < left) out(sum(u), q0 + row(u), p, FORWARD ? out.ask(q0 + row(u), p) : none);
             continue;
         }
         // a loop for each activation, with dropout or without (asked for each four columns, that took 7 us of 50 of a product of 33598 x 300 -> 600 without any)
@@ -605,7 +606,7 @@ __global__ __launch_bounds__(S::THREADS, S::PER_SIMD) void k_linear_tiles(const 
             if (out.drop.thr) leave(act, integral_constant<bool, true>{});
             else leave(act, integral_constant<bool, false>{});
         };
-        if constexpr (ACOLS || BCOLS) {                            // (the backward's products: nothing follows them)
+        if constexpr (!FORWARD) {                                  // (the backward's products: nothing follows them)
             leave(integral_constant<int, BPT_ACT_NONE>{}, integral_constant<bool, false>{});
         } else {
             if (out.act == BPT_ACT_RELU) with_drop(integral_constant<int, BPT_ACT_RELU>{});

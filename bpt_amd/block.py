@@ -105,6 +105,14 @@ def _check_bucket_bias(rel_pos, bucket_bias):
         raise ValueError("bucket_bias and rel_pos do not go together")
 
 
+def _draw_parameters(block):
+    for name, p in block.named_parameters():
+        if name == "bias_table":
+            nn.init.zeros_(p)
+        elif p.dim() > 1:
+            nn.init.xavier_uniform_(p)
+
+
 def _distance_slopes(h):
     return nn.Parameter(2.0 ** (-8.0 * torch.arange(1, h + 1, dtype=torch.float32) / h))
 
@@ -183,9 +191,7 @@ class BPTBlock(nn.Module):
 
     def reset_parameters(self):
         # modules/attention.py:49-52
-        for p in self.parameters():
-            if p.dim() > 1:
-                nn.init.xavier_uniform_(p)
+        _draw_parameters(self)
 
     def attention(self, q, k, v, csr, etype=None, pos=None):
         """attention.py:66-77: (n, h, d_k) q, k, v -> (n, h * d_k)."""
@@ -266,9 +272,7 @@ class BPTMemBlock(nn.Module):
 
     def reset_parameters(self):
         # modules/attention.py:112-115
-        for p in self.parameters():
-            if p.dim() > 1:
-                nn.init.xavier_uniform_(p)
+        _draw_parameters(self)
 
     def _attend(self, which, q, k, v, csr, etype=None, pos=None):
         """attention.py:130-141 (which = 0, with rel_pos) and :156-163 (which = 1): (n_q, h, d_k) -> (n_q, h * d_k)."""

@@ -117,8 +117,8 @@ def _distance_slopes(h):
     return nn.Parameter(2.0 ** (-8.0 * torch.arange(1, h + 1, dtype=torch.float32) / h))
 
 
-def _score_options(block, pos, etype):
-    """bpt_attention's score options and bias of a block."""
+def _score_options(block, pos, etype, dtype):
+    """bpt_attention's score options and bias of a block whose projections are of dtype (under autocast not its parameters')."""
     opts = {}
     if block.score_cap is not None:
         opts["score_cap"] = block.score_cap
@@ -129,7 +129,7 @@ def _score_options(block, pos, etype):
     if block.bucket_bias:
         if etype is None:
             raise ValueError("bucket_bias needs the edge types (etype)")
-        opts.update(bias_table=block.bias_table, buckets=etype)
+        opts.update(bias_table=block.bias_table.to(dtype), buckets=etype)
     return opts
 
 
@@ -200,7 +200,7 @@ class BPTBlock(nn.Module):
         att_dropout = self.drop_att.p if self.training else 0.0
         if self.rel_pos and etype is None:
             raise ValueError("rel_pos=True needs the edge types (etype)")
-        opts = _score_options(self, pos, etype)
+        opts = _score_options(self, pos, etype, q.dtype)
         if self.fused or opts:
             rel = dict(rel_table=self.embed_ak.weight, etype=etype) if self.rel_pos else {}
             return bpt_attention(*graph, q, k, v, fused=None if self.fused else False, dropout_p=att_dropout, **rel, **opts).view(-1, self.d_k * self.h)
@@ -282,7 +282,7 @@ class BPTMemBlock(nn.Module):
         rel = self.rel_pos and which == 0
         if rel and etype is None:
             raise ValueError("rel_pos=True needs the edge types (etype)")
-        opts = _score_options(self, pos, etype) if which == 0 else {} if self.score_cap is None else dict(score_cap=self.score_cap)
+        opts = _score_options(self, pos, etype, q.dtype) if which == 0 else {} if self.score_cap is None else dict(score_cap=self.score_cap)
         if self.fused or opts:
             extra = dict(rel_table=self.embed_ak.weight, etype=etype) if rel else {}
             return bpt_attention(*graph, q, k, v, fused=None if self.fused else False, dropout_p=p, **extra, **opts).view(-1, self.d_k * self.h)

@@ -766,26 +766,29 @@ __global__ __launch_bounds__(BLOCK) void k_linear_grad(const T *dy, const T *__r
 template <typename T> __global__ __launch_bounds__(BLOCK) void k_linear_sums(const float *__restrict__ part, int parts, T *__restrict__ out, int64_t cols, float scale) {
     __shared__ float meet[16][17];
     const int c = threadIdx.x & 15, k = threadIdx.x >> 4;
-    const int64_t at = (int64_t)blockIdx.x * 16 + c;
-    float v = 0.f;
-    if (at < cols) {
-        int p = k;
-        for (; p + 15 * 16 < parts; p += 16 * 16) {
-            float t[16];
+    for (int64_t first = (int64_t)blockIdx.x * 16; first < cols; first += (int64_t)gridDim.x * 16) {
+        const int64_t at = first + c;
+        float v = 0.f;
+        if (at < cols) {
+            int p = k;
+            for (; p + 15 * 16 < parts; p += 16 * 16) {
+                float t[16];
 #pragma unroll
-            for (int u = 0; u < 16; ++u) t[u] = part[(int64_t)(p + u * 16) * cols + at];
+                for (int u = 0; u < 16; ++u) t[u] = part[(int64_t)(p + u * 16) * cols + at];
 #pragma unroll
-            for (int u = 0; u < 16; ++u) v += t[u];
+                for (int u = 0; u < 16; ++u) v += t[u];
+            }
+            for (; p < parts; p += 16) v += part[(int64_t)p * cols + at];
         }
-        for (; p < parts; p += 16) v += part[(int64_t)p * cols + at];
-    }
-    meet[k][c] = v;
-    __syncthreads();
-    if (k != 0 || at >= cols) return;
-    v = meet[0][c];
+        __syncthreads();                                           // (the turn before has been read)
+        meet[k][c] = v;
+        __syncthreads();
+        if (k != 0 || at >= cols) continue;
+        v = meet[0][c];
 #pragma unroll
-    for (int i = 1; i < 16; ++i) v += meet[i][c];
-    Elem<T>::st(out + at, v * scale);
+        for (int i = 1; i < 16; ++i) v += meet[i][c];
+        Elem<T>::st(out + at, v * scale);
+    }
 }
 
 // ---- dropout -----------------------------------------------------------------------------------------------------------------------
@@ -978,7 +981,8 @@ int run_grad(const void *dy_, const void *kept_, int result, void *g_, void *db_
                            rows, cols, act, drop, quads);
     const int st = launch_status();
     if (st != BPT_OK || !db_) return st;
-    hipLaunchKernelGGL((k_linear_sums<T>), dim3((unsigned)ceil_div(cols, 16)), dim3(BLOCK), 0, s, part, rows > 0 ? parts : 0, (T *)db_, cols, inv);
+    const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div(cols, 16), (int64_t)1 << 20);      // (a launch counts its threads in 32 bits)
+    hipLaunchKernelGGL((k_linear_sums<T>), dim3(blocks), dim3(BLOCK), 0, s, part, rows > 0 ? parts : 0, (T *)db_, cols, inv);
     return launch_status();
 }
 

@@ -326,6 +326,7 @@ int bpt_bucket_prepare(const bpt_plan *plan_in, const bpt_plan *plan_out, const 
     if (!aligned16(prepared)) return BPT_ERR_UNSUPPORTED;
     const Prepared pr(prepared, plan_in, h);
     const int64_t in = places(plan_in), out = plan_out ? places(plan_out) : 0, most = std::max<int64_t>(std::max(in, out), h * 256);
+    if (most > (((int64_t)1 << 32) - BLOCK) * 4) return BPT_ERR_SIZE;      // (a launch counts its threads in 32 bits)
     const dim3 grid((unsigned)((most + 4 * BLOCK - 1) / (4 * BLOCK)), plan_out ? 3 : 2);
     hipStream_t s = (hipStream_t)stream;
     const int32_t *ei = place_eids(plan_in), *eo = plan_out ? place_eids(plan_out) : nullptr;

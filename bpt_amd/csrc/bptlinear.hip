@@ -987,6 +987,7 @@ int run_grad(const void *dy_, const void *kept_, int result, void *g_, void *db_
 }
 
 template <typename T> int run_dropout(const void *x, const void *r, void *y, int64_t n, Drop drop, hipStream_t s) {
+    if (n > (((int64_t)1 << 32) - BLOCK) * 4 * ve<T>()) return BPT_ERR_SIZE;      // (a launch counts its threads in 32 bits)
     const dim3 grid((unsigned)ceil_div(n, (int64_t)BLOCK * 4 * ve<T>()));
     if (on({x, r, y}, 16)) hipLaunchKernelGGL((k_dropout<T, true>), grid, dim3(BLOCK), 0, s, (const T *)x, (const T *)r, (T *)y, n, drop);
     else hipLaunchKernelGGL((k_dropout<T, false>), grid, dim3(BLOCK), 0, s, (const T *)x, (const T *)r, (T *)y, n, drop);

@@ -760,4 +760,4 @@ def bucket_bias(table, buckets):
     """table[buckets] as (E, h) scores: one of the separate operators, to be added to what masked_mm gives.  table (n, h) float32, float64 or bfloat16, buckets (E,)
     int64; a bucket outside of the table gives 0.  The gradient of table is summed in a fixed order (torch's scatters with atomics)."""
     _no_transforms("bucket_bias")
-    return BucketBias.apply(table.contiguous(), buckets)
+    return BucketBias.apply(table.contiguous(), buckets.contiguous())

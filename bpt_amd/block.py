@@ -22,7 +22,7 @@ Options the reference does not have, off by default (then nothing of them is a p
               (`op.linear_act`; with keep8 the feed-forward as keep8 has it, then `op.dropout` with the residual): no mask is stored, dropout's
               decisions come from a counter-based generator seeded from torch's CPU generator.  In bfloat16 the residual sum is rounded before it is
               normalised
-  bucket_bias scores get a learned scalar of the edge's type and the head: bias_table (bucket_bias, heads), a parameter that starts at 0; the edge types
+  bucket_bias scores get a learned scalar of the edge's type and the head: bias_table (bucket_bias, heads), a parameter that starts at 0, taken in q's type; the edge types
               are forward's etype, those outside of the table have no bias.  Not together with rel_pos
 """
 import math

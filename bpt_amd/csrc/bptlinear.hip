@@ -34,7 +34,7 @@ struct Drop {
 };
 inline Drop make_drop(double p, uint64_t seed) {
     if (!(p > 0.0)) return Drop{0u, 0u, 0u, 1.f};
-    const double t = p * 4294967296.0;
+    const double t = p * 4294967296.0;                            // (its whole part counts)
     return Drop{(uint32_t)(t >= 4294967295.0 ? 4294967295.0 : t < 1.0 ? 1.0 : t), (uint32_t)seed, (uint32_t)(seed >> 32), (float)(1.0 / (1.0 - p))};
 }
 __device__ __forceinline__ uint32_t xor3(uint32_t a, uint32_t b, uint32_t c) { return __builtin_amdgcn_bitop3_b32(a, b, c, 0x96); }
@@ -69,7 +69,8 @@ __device__ __forceinline__ floatx4 dropped(floatx4 v, uintx4 words, const Drop &
 
 // ---- activations -------------------------------------------------------------------------------------------------------------------
 // Phi(a) = erfc(-a / sqrt 2) / 2 from e = exp(-a^2 / 2): erfc(z) exp(z^2) = t P(t), t = 1 / (1 + 0.45 z) for z >= 0, P of degree 9 fitted to 1.6e-8 of it (least squares
-// on 4000 points, weights raised where the error is largest); 1.5e-7 with the roundings of float32, also far below zero, where 1 + erf keeps no digits.
+// on 4000 points, weights raised where the error is largest); with the roundings of float32 2e-7 off at most.  Relative to itself, below zero, where 1 + erf keeps no digits: 4e-7 down to
+// -1, 9e-7 to -4, 2e-6 to -6, 8e-6 to -13 (exp2 takes a square that has been rounded); it ends in 0 behind, where it is no normal number any more.
 __device__ __forceinline__ float gaussian(float a) { return __builtin_amdgcn_exp2f(a * a * -0.72134752044448170f); }
 __device__ __forceinline__ float normal_cdf(float a, float e) {
     const float t = __builtin_amdgcn_rcpf(fmaf(fabsf(a), 0.45f * 0.70710678118654752f, 1.f));
@@ -303,9 +304,9 @@ template <typename T> __device__ __forceinline__ floatx4 multiply(uintx4 a, uint
 }
 
 __device__ __forceinline__ void wait_for_lds() { __builtin_amdgcn_s_waitcnt(15 | 7 << 4 | 3 << 14); }
-// Eight float32, times 2^23, as three bfloat16 each, exactly: the upper 16 bits, those of what is left, and what is left then (8 + 8 + 8 digits).  The bfloat16 units take numbers
-// below 2^-126 for 0: 2^23 makes the last digit of float32's lowest number, 2^-149, one of those that count.  (Rounded instead of cut, the thirds would have either sign, and what the
-// products leave out too; but the units round sums of either sign less well: 3 x 16744449 comes out a step off, and it takes 1 to 4 percent longer.)
+// Eight float32, times 2^23, as three bfloat16 each, exactly: the upper 16 bits, those of what is left, and what is left then (8 + 8 + 8 digits).  bfloat16's lowest number is 2^-133, and
+// digits of thirds below it would be lost: 2^23 takes the last digit of float32's lowest, 2^-149, to 2^-126, so that every third is a normal number.  (Rounded instead of cut, the thirds
+// would have either sign, and what the products leave out too; but the units round sums of either sign less well: 3 x 16744449 comes out a step off, and it takes 1 to 4 percent longer.)
 constexpr float THIRDS_BY = 0x1p23f, THIRDS_BACK = 0x1p-46f;       // (of an operand; of a product of two)
 __device__ __forceinline__ void thirds(uintx4 a, uintx4 b, uintx4 (&out)[3]) {
     uint32_t x[8], y[8], z[8];
@@ -865,11 +866,11 @@ inline bool on(std::initializer_list<const void *> ps, uintptr_t bytes) {
 // shares too if the reduction is longer than what their sums cost on the way through memory.  64 x 64: where the larger ones would leave units idle.
 // us, by 256 | 128 | 64, bfloat16 (forward of rows x inner -> outer): 65535 x 4096 -> 1024 457 | 582 | 931, 8192 x 4096 -> 4096 223 | 285 | 565, 16383 x 512 -> 2048 45 | 50 | 66,
 // 16383 x 2048 -> 512 55 | 37 | 51, 2000 x 512 -> 2048 20 | 10 | 11, 1023 x 512 -> 512 19 | 9.2 | 8.8; dweight (shares) of 65535 x 4096 -> 1024 475 | 577 | 1226, of 16383 x 512 -> 2048
-// 52 | 45 | 71; float32 4096 x 4096 -> 4096 601 | 709 | 917, 16383 x 512 -> 2048 177 | 181 | 249, 1023 x 512 -> 512 72 | 22 | 15.
-// Two or three shares on 128 x 128 | one on 64 x 64, bfloat16: 4096 x 1024 -> 1024 27 | 17, 2500 x 2048 -> 1024 26 | 22, 2500 x 4096 -> 1024 35 | 41; float32: 3000 x 512 -> 1024 39 | 29,
-// 4096 x 1024 -> 1024 70 | 72, 2048 x 1024 -> 2048 57 | 63.  320 tiles of 128 x 128 | 64 x 64: dx of 2500 x 2048 -> 1024 20 | 24, float32 88 | 80.
+// 52 | 45 | 71; float32 4096 x 4096 -> 4096 657 | 729 | 986, 16383 x 512 -> 2048 187 | 197 | 272, 1023 x 512 -> 512 77 | 23 | 14.
+// Two or three shares on 128 x 128 | one on 64 x 64, bfloat16: 4096 x 1024 -> 1024 27 | 17, 2500 x 2048 -> 1024 26 | 22, 2500 x 4096 -> 1024 35 | 41; float32: 3000 x 512 -> 1024 38 | 29,
+// 4096 x 1024 -> 1024 59 | 67, 2048 x 1024 -> 2048 61 | 71.  320 tiles of 128 x 128 | 64 x 64: dx of 2500 x 2048 -> 1024 20 | 24, float32 89 | 89.
 // Shares of 4 | 8 | 16 steps at least on 64 x 64, bfloat16: 65 x 512 -> 512 9.6 | 5.9 | 5.8, 256 x 1024 -> 1024 8.7 | 8.8 | 7.9, 1023 x 512 -> 512 8.9 | 5.8 | 5.8, 256 x 2048 -> 512 8.6 | 8.8 | 10.1;
-// float32: 65 x 512 -> 512 10.0 | 11.6 | 15.4, 127 x 768 -> 768 10.2 | 12.8 | 20, 256 x 1024 -> 1024 15.1 | 14.1 | 18, dweight of 256 x 512 -> 2048 15.8 | 10.8 | 10.7.
+// float32: 65 x 512 -> 512 10.6 | 12.1 | 15.8, 127 x 768 -> 768 10.9 | 12.7 | 22, 256 x 1024 -> 1024 14.9 | 13.9 | 19, dweight of 256 x 512 -> 2048 15.4 | 10.4 | 10.4.
 typedef Shape<256, 256, 4, 2, 1> Huge;
 typedef Shape<128, 128, 2, 2, 2> Large;
 typedef Shape<64, 64, 2, 2, 4> Small;
@@ -939,7 +940,7 @@ template <typename T> inline Epilogue<T> plain_epilogue(T *y, int64_t cols, doub
 
 // Whether the kernel of few rows takes a forward: every workgroup of it reads all of x, 128 KB at most where it has more than a fragment's rows.  us, few rows | tiles, bfloat16:
 // 16 x 512 -> 512 4.9 | 7.2, 16 x 4096 -> 4096 9.8 | 10.4, 64 x 512 -> 512 4.8 | 6.8, 64 x 1024 -> 4096 7.2 | 8.8, 32 x 2048 -> 512 7.6 | 6.8, 64 x 2048 -> 512 11.5 | 8.3, 64 x 4096 -> 4096
-// 21 | 12.5; float32 16 x 4096 -> 4096 20 | 32, 64 x 512 -> 512 7.3 | 8.5, 32 x 1024 -> 4096 9.1 | 12.3, 64 x 1024 -> 1024 12.7 | 9.6, 32 x 2048 -> 512 14 | 9.7, 64 x 4096 -> 4096 44 | 36.
+// 21 | 12.5; float32 16 x 4096 -> 4096 19 | 32, 64 x 512 -> 512 8.0 | 10.5, 32 x 1024 -> 4096 9.2 | 12.9, 64 x 1024 -> 1024 12.5 | 10.6, 32 x 2048 -> 512 14 | 10.8, 64 x 4096 -> 4096 43 | 34.
 // (A launch counts its threads in 32 bits: of more columns the tiles have fewer.)
 inline bool few_rows(int64_t rows, int64_t inner, int64_t outer, int64_t size) {
     return (rows <= 16 || (rows <= 64 && rows * inner * size <= (int64_t)1 << 17)) && outer <= (int64_t)1 << 26;

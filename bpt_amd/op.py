@@ -748,7 +748,7 @@ def linear_act(x, weight, bias=None, activation=None, residual=None, dropout_p=0
 def dropout(x, dropout_p, seed=None, residual=None):
     """residual + x with a share dropout_p of its elements 0 and the others divided by 1 - dropout_p; residual like x or None.  Element i (its place in
     memory) is dropped where word i % 4 of Philox-4x32-10 (Salmon et al. 2011) of the counter (i // 4, 0) under the key seed lies below
-    dropout_p 2^32: nothing is stored, the backward forms the words again.  seed=None draws one from torch's CPU generator.  float32 or bfloat16,
+    the whole part of dropout_p 2^32 (1 at least): nothing is stored, the backward forms the words again.  seed=None draws one from torch's CPU generator.  float32 or bfloat16,
     contiguous; the sum is held in 32 bits.  In evaluation pass dropout_p=0."""
     _no_transforms("dropout")
     if dropout_p > 0 and seed is None:

@@ -5,7 +5,8 @@
  * contiguous; any alignment of the element's size is accepted, workspaces start on 16 bytes.  Sums are held in 32 bits.
  *
  * Dropout: element i (its place in memory) takes word i % 4 of Philox-4x32-10 (Salmon et al., "Parallel random numbers: as easy as 1, 2, 3", 2011) of the
- * counter (i / 4, 0) under the key seed.  It becomes 0 where the word is below dropout_p 2^32 and is divided by 1 - dropout_p elsewhere.
+ * counter (i / 4, 0) under the key seed.  It becomes 0 where the word is below the whole part of dropout_p 2^32 (1 where that
+ * is less, 2^32 - 1 at most) and is divided by 1 - dropout_p elsewhere.
  */
 #ifndef BPTLINEAR_H
 #define BPTLINEAR_H

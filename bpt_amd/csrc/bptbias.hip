@@ -13,13 +13,11 @@ template <typename T, typename O>
 __global__ __launch_bounds__(BLOCK) void k_bucket_rows(const T *__restrict__ table, const int64_t *__restrict__ buckets, O *__restrict__ bias, int64_t n_edges,
                                                        int64_t n_buckets, int h, typename Elem<T>::acc_t factor, int spare_row) {
     using A = typename Elem<T>::acc_t;
-    const int64_t n = (n_edges + spare_row) * h;
-    for (int64_t i = (int64_t)blockIdx.x * BLOCK + threadIdx.x; i < n; i += (int64_t)gridDim.x * BLOCK) {
-        const int64_t e = i / h;
-        const int head = (int)(i - e * h);
-        const int64_t b = e < n_edges ? buckets[e] : -1;
-        Elem<O>::st(bias + i, (uint64_t)b < (uint64_t)n_buckets ? (A)Elem<T>::ld(table + b * h + head) * factor : A(0));
-    }
+    const int64_t i = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * BLOCK + threadIdx.x, e = i / h;
+    const int head = (int)(i - e * h);
+    if (e >= n_edges + spare_row) return;
+    const int64_t b = e < n_edges ? buckets[e] : -1;
+    Elem<O>::st(bias + i, (uint64_t)b < (uint64_t)n_buckets ? (A)Elem<T>::ld(table + b * h + head) * factor : A(0));
 }
 
 // ---- its gradient --------------------------------------------------------------------------------------------------------------------
@@ -93,10 +91,10 @@ inline int sums_parts(int64_t n_edges, int h) {
 
 template <typename T, typename O>
 int run_rows(const void *table, const int64_t *buckets, void *bias, int64_t n_edges, int64_t n_buckets, int h, double factor, int spare, hipStream_t s) {
-    const int64_t n = (n_edges + spare) * h;
-    const unsigned blocks = (unsigned)std::min<int64_t>((n + BLOCK - 1) / BLOCK, (int64_t)1 << 23);      // (a launch counts its threads in 32 bits)
-    hipLaunchKernelGGL((k_bucket_rows<T, O>), dim3(blocks), dim3(BLOCK), 0, s, (const T *)table, buckets, (O *)bias, n_edges, n_buckets, h, (typename Elem<T>::acc_t)factor,
-                       spare);
+    // (an axis of a launch counts its threads in 32 bits)
+    const int64_t blocks = ((n_edges + spare) * h + BLOCK - 1) / BLOCK, along = std::min<int64_t>(blocks, (int64_t)1 << 23);
+    hipLaunchKernelGGL((k_bucket_rows<T, O>), dim3((unsigned)along, (unsigned)((blocks + along - 1) / along)), dim3(BLOCK), 0, s, (const T *)table, buckets, (O *)bias, n_edges,
+                       n_buckets, h, (typename Elem<T>::acc_t)factor, spare);
     return launch_status();
 }
 template <typename D, typename T>

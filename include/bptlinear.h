@@ -43,7 +43,7 @@ int64_t bpt_linear_weight_grad_workspace_bytes(int64_t rows, int64_t inner, int6
 int bpt_linear_weight_grad(const void *g, const void *x, void *dweight, void *workspace, int64_t workspace_bytes, int64_t rows, int64_t inner,
                            int64_t outer, double scale, int dtype, void *stream);
 
-/* y = residual + dropout(x), n elements (fewer than 2^36 in float32, 2^37 in bfloat16); residual may be NULL.  y may be x or residual.  The gradient of x is the same call on dy without a residual. */
+/* y = residual + dropout(x), n elements (at most 2^36 - 4096 in float32, 2^37 - 8192 in bfloat16); residual may be NULL.  y may be x or residual.  The gradient of x is the same call on dy without a residual. */
 int bpt_dropout(const void *x, const void *residual, void *y, int64_t n, double dropout_p, uint64_t seed, int dtype, void *stream);
 
 #ifdef __cplusplus
